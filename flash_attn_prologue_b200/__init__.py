@@ -27,6 +27,8 @@ _LAZY = {
     "matmul_bwd_dx": ("gemm_bwd", "matmul_bwd_dx"),
     "matmul_bwd_dw": ("gemm_bwd", "matmul_bwd_dw"),
     "fused_qkv_backward": ("gemm_bwd", "fused_qkv_backward"),
+    "qknorm_rope_scale_gqa": ("gqa", "qknorm_rope_scale_gqa"),
+    "append_paged_kv": ("paged", "append_paged_kv"),
 }
 __all__ = ["qknorm_rope_scale", "qknorm_rope_scale_qkv", "prepare_backend", "RMSNormRoPEScale", "FusedQKV",
            *_LAZY]

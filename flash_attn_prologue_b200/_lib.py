@@ -6,6 +6,7 @@ touches CUDA or the library. There is no fallback: a missing library raises.
 """
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -84,7 +85,18 @@ SIGNATURES = {
     "flash_prologue_ipc_close": ([_vp, _i64], ctypes.c_int),
     "flash_prologue_peer_reduce_emulated": ([_vp, _i64, ctypes.c_int32, ctypes.c_int32, _vp, _vp, _vp,
                                              ctypes.c_uint32, _vp], ctypes.c_int),
+    "flash_prologue_gqa_fwd": ([ctypes.c_char_p, _vp], ctypes.c_int),
+    "flash_prologue_gqa_bwd": ([ctypes.c_char_p, _vp], ctypes.c_int),
+    "flash_prologue_gqa_bwd_workspace_size": ([_i64, _i64, ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
+    "flash_prologue_append_paged": ([ctypes.c_char_p, _vp], ctypes.c_int),
 }
+
+# The argument structs of include/flash_prologue.h whose fields are all 8 bytes
+# wide, packed by struct.pack (a few microseconds less a call than ctypes fields).
+_ROWS, _ROTATION, _CACHE = "Pqqq", "PqqPqqq", "PqqqPqqqqqPqqPPq"
+GQA_ARGS = struct.Struct("@" + 8 * _ROWS + "PP" + _ROTATION + "Pqqq" + "PP" + "Pq" + "Pq" + "6q" + "d")
+APPEND_ARGS = struct.Struct("@" + 4 * _ROWS + "PP" + _ROTATION + _CACHE + "5q" + "d")
+NO_ROWS = (0, 0, 0, 0)
 
 MAX_PEERS = 8
 

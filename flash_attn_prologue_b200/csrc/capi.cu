@@ -260,13 +260,16 @@ extern "C" {
 
 FLASH_PROLOGUE_API int flash_prologue_device_error(int* value, int reset) {
   if (!value) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
-  int a = 0, b = 0, c = 0, d = 0;
-  if (read_device_error(&a, reset != 0) != cudaSuccess ||
-      read_gemm_device_error(&b, reset != 0) != cudaSuccess ||
-      read_gemm_bwd_device_error(&c, reset != 0) != cudaSuccess ||
-      read_peer_device_error(&d, reset != 0) != cudaSuccess)
-    return FLASH_PROLOGUE_ERR_CUDA;
-  *value = a | b | c | d;
+  using Reader = cudaError_t (*)(int*, bool);
+  const Reader readers[] = {read_device_error,      read_gemm_device_error,    read_gemm_bwd_device_error,
+                            read_peer_device_error, read_gqa_fwd_device_error, read_gqa_bwd_device_error};
+  int all = 0;
+  for (Reader read : readers) {
+    int word = 0;
+    if (read(&word, reset != 0) != cudaSuccess) return FLASH_PROLOGUE_ERR_CUDA;
+    all |= word;
+  }
+  *value = all;
   return FLASH_PROLOGUE_OK;
 }
 

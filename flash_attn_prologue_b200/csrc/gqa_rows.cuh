@@ -1,0 +1,136 @@
+// Host-side arguments of the grouped-query prologue kernels (gqa_fwd.cu,
+// gqa_bwd.cu): rows of Q with Hq heads, rows of K (and V) with Hk heads, the
+// rotation picked per token by a position.
+#pragma once
+
+#include "../../include/flash_prologue.h"
+#include "prologue_host.h"
+#include "tma_util.cuh"
+
+namespace flash_prologue {
+
+// Device error word value: an index read from device memory (a position, a
+// page, a length) was out of range; the rows it concerns were not read or written.
+constexpr int kDeviceErrorIndex = 2;
+constexpr int64_t kMaxGqaHeads = 512;
+// Grid bound of the backward, hence its workspace: one partial row a CTA.
+constexpr int kGqaBwdMaxCtasPerSm = 2;
+
+// How the 32 / L row slots of a warp (L = D / 16 lanes a row) map to rows: HS
+// heads of TP consecutive tokens, HS * TP = 32 / L. A warp's token group walks
+// `iters[t]` head blocks of tensor t; `slices` warps share a token group when
+// there are too few groups to fill the GPU.
+struct RowsPlan {
+  int log2_hs;
+  int iters[3];       // head blocks of q, k, v (v: 0 without a cache)
+  int slices;
+  int per_slice;      // head blocks of one slice
+  int64_t groups;     // token groups
+};
+
+struct GqaTables {
+  const float* sin;
+  const float* cos;
+  int64_t sin_n, sin_j, cos_n, cos_j;  // element strides
+  int64_t rows;                        // positions are in [0, rows)
+  const void* positions;               // null: row n of the tables; else int32 / int64 [b, n]
+  int64_t pos_b, pos_n;
+  int pos_is64;
+};
+
+struct PagedTarget {
+  const int32_t* page_table;  // [batch, max_pages]
+  const int32_t* seq_lens;    // [batch], new tokens included
+  const int32_t* cu_seqlens;  // [batch + 1], null: token i is request i's
+  int64_t table_stride;
+  int64_t max_pages, num_pages;
+  int batch;
+  int page_log2;
+};
+
+struct GqaFwdArgs {
+  const void* x[3];    // q, k, v
+  void* y[3];          // q_out, then k_out or the two caches
+  RowStrides sx[3];
+  RowStrides sy[3];    // of a cache: b = page, h = head, n = slot
+  const float* w;      // [2, D] or null (rotation only)
+  const float* scales; // [Hq] or null
+  GqaTables tab;
+  PagedTarget paged;   // page_table null: dense k_out
+  int64_t B, N;
+  int H[3];
+  float eps;
+  RowsPlan p;
+};
+
+struct GqaBwdArgs {
+  const void* x[2];
+  const void* gy[2];
+  void* dx[2];
+  RowStrides sx[2], sgy[2], sdx[2];
+  const float* w;
+  const float* scales;
+  GqaTables tab;
+  float* partials;     // [grid, 2 * D + Hq]
+  int64_t B, N;
+  int H[2];
+  float eps;
+  RowsPlan p;
+};
+
+// A usable peer group for rows of `cols` sums and an epoch of at least 1.
+inline bool valid_peers(const flash_prologue_peers* peers, int64_t epoch, int64_t cols) {
+  return epoch >= 1 && epoch <= UINT32_MAX && peers->world >= 1 && peers->world <= FLASH_PROLOGUE_MAX_PEERS &&
+         peers->rank >= 0 && peers->rank < peers->world && peers->max_cols % 32 == 0 && peers->max_cols >= cols &&
+         peers->wait_ms >= 0 && peers->wait_ms <= 60000;
+}
+
+RowsPlan plan_rows(int64_t tokens, int Hq, int Hk, int Hv, int D, bool heads_inner, int64_t want_warps);
+cudaError_t launch_gqa_fwd(const GqaFwdArgs& a, int dtype, int D, bool vec, cudaStream_t stream);
+int64_t gqa_bwd_grid(const RowsPlan& p, int Hq, int D, int dtype, bool vec);
+cudaError_t launch_gqa_bwd(const GqaBwdArgs& a, float* dw, float* ds, int dtype, int D, bool vec,
+                           const BwdReduce& red, cudaStream_t stream);
+
+// Rotation row of token (b, n); -1 (and the error word) when it is out of range.
+__device__ __forceinline__ int64_t rotation_row(const GqaTables& t, int64_t b, int64_t n) {
+  int64_t pos = n;
+  if (t.positions) {
+    const int64_t i = b * t.pos_b + n * t.pos_n;
+    pos = t.pos_is64 ? static_cast<const int64_t*>(t.positions)[i]
+                     : (int64_t) static_cast<const int32_t*>(t.positions)[i];
+  }
+  if (pos < 0 || pos >= t.rows) {
+    atomicOr(&g_device_error, kDeviceErrorIndex);
+    return -1;
+  }
+  return pos;
+}
+
+template <typename T>
+__device__ __forceinline__ void chunk_zero(Chunk<T>& c) {
+#pragma unroll
+  for (int i = 0; i < Chunk<T>::kWords; ++i) c.w[i] = 0;
+}
+
+// A kernel for each activation type, head dimension and access width.
+#define FLASH_PROLOGUE_GQA_DIMS(T, KERNEL)                                                        \
+  switch (D) {                                                                                    \
+    case 32: return vec ? reinterpret_cast<const void*>(&KERNEL<T, 32, true>)                     \
+                        : reinterpret_cast<const void*>(&KERNEL<T, 32, false>);                   \
+    case 64: return vec ? reinterpret_cast<const void*>(&KERNEL<T, 64, true>)                     \
+                        : reinterpret_cast<const void*>(&KERNEL<T, 64, false>);                   \
+    case 128: return vec ? reinterpret_cast<const void*>(&KERNEL<T, 128, true>)                   \
+                         : reinterpret_cast<const void*>(&KERNEL<T, 128, false>);                 \
+    case 256: return vec ? reinterpret_cast<const void*>(&KERNEL<T, 256, true>)                   \
+                         : reinterpret_cast<const void*>(&KERNEL<T, 256, false>);                 \
+    default: return nullptr;                                                                      \
+  }
+#define FLASH_PROLOGUE_GQA_KERNEL(KERNEL)                                                         \
+  switch (dtype) {                                                                                \
+    case 0: FLASH_PROLOGUE_GQA_DIMS(__nv_bfloat16, KERNEL)                                        \
+    case 1: FLASH_PROLOGUE_GQA_DIMS(__half, KERNEL)                                               \
+    case 2: FLASH_PROLOGUE_GQA_DIMS(float, KERNEL)                                                \
+    default: return nullptr;                                                                      \
+  }
+
+}  // namespace flash_prologue

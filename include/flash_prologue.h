@@ -320,9 +320,9 @@ FLASH_PROLOGUE_API int flash_prologue_bwd_noalloc(const void* q, const int64_t q
 FLASH_PROLOGUE_API int flash_prologue_set_path(int mode);
 
 /*
- * Reads the device error word of the pipelined kernels (0 = none; 1 = a
- * bounded barrier wait gave up, which means the results of that launch are
- * invalid). Synchronous (copies from the device); clears the word if `reset`.
+ * Reads the device error word of the kernels (0 = none; bit 0 = a bounded
+ * barrier wait gave up, which means the results of that launch are invalid;
+ * bit 1 = an index read from device memory was out of range). Synchronous (copies from the device); clears the word if `reset`.
  * No counterpart in the reference (which has no device-side waits).
  */
 FLASH_PROLOGUE_API int flash_prologue_device_error(int* value, int reset);
@@ -436,6 +436,109 @@ FLASH_PROLOGUE_API int flash_prologue_inverse_bwd_dp(const void* q_out, const in
 FLASH_PROLOGUE_API int flash_prologue_peer_reduce_emulated(const float* const* partials, int64_t G,
                        int32_t C, int32_t two_d, float* const* dw, float* const* ds,
                        const flash_prologue_peers* peers, uint32_t epoch, void* stream);
+
+/*
+ * ---------------------------------------------------------------------------
+ * Grouped-query heads and paged caches (no counterpart in the reference, whose
+ * Q and K have equal heads and which ends before attention). The arguments of a
+ * call are one struct of 8-byte fields; fields that a call does not name are
+ * ignored. Rows are [b, h, n, d] views: a pointer and the element strides of b,
+ * h and n; the d stride is 1. A packed [T, H, D] tensor has B = 1, N = T.
+ * An index that the kernels read from device memory (a position, a page, a
+ * length) and find out of range is not followed: the rows it concerns are not
+ * read or written, and bit 1 of the device error word is set
+ * (flash_prologue_device_error() then reports 2, or 3 beside a timeout).
+ */
+typedef struct flash_prologue_rows {
+  void* data;
+  int64_t b, h, n; /* element strides */
+} flash_prologue_rows;
+
+/* FP32 sin/cos of `rows` positions, indexed [position, j], j < D / 2. */
+typedef struct flash_prologue_rotation {
+  const float* sin;
+  int64_t sin_n, sin_j;
+  const float* cos;
+  int64_t cos_n, cos_j;
+  int64_t rows;
+} flash_prologue_rotation;
+
+typedef struct flash_prologue_gqa_args {
+  flash_prologue_rows q, k;                   /* [B, Hq, N, D], [B, Hk, N, D]       */
+  flash_prologue_rows q_out, k_out;           /* forward                            */
+  flash_prologue_rows grad_q_out, grad_k_out; /* backward: upstream gradients       */
+  flash_prologue_rows grad_q, grad_k;         /* backward                           */
+  const float* rmsnorm_weight;                /* [2, 1, D], 16-byte aligned         */
+  const float* scales;                        /* [Hq]                               */
+  flash_prologue_rotation rotation;
+  const void* positions;                      /* NULL: token n uses row n           */
+  int64_t position_b, position_n;             /* element strides                    */
+  int64_t position_bits;                      /* 32 or 64                           */
+  float* grad_rmsnorm_weight;                 /* backward: [2, 1, D]                */
+  float* grad_scales;                         /* backward: [Hq]                     */
+  void* workspace;                            /* backward                           */
+  int64_t workspace_bytes;
+  const flash_prologue_peers* peers;          /* backward: NULL, or sum over ranks  */
+  int64_t epoch;
+  int64_t B, N, Hq, Hk, D, dtype;
+  double eps;
+} flash_prologue_gqa_args;
+
+/*
+ * The prologue with Hq query heads on Hk key heads (Hq a multiple of Hk, at
+ * most 512) and a position per token: rows as in flash_prologue_fwd, turned by
+ * row positions[b, n] of the tables (or row n). D in {32, 64, 128, 256}; BF16,
+ * FP16, FP32. An out-of-range position gives NaN rows and the error word.
+ * The backward overwrites all its outputs; its parameter sums have a fixed
+ * order, so results are identical run to run; upstream gradients may broadcast
+ * (stride 0). With `peers` the parameter gradients come out summed over the
+ * ranks as in flash_prologue_bwd_dp (same epoch sequence).
+ */
+FLASH_PROLOGUE_API int flash_prologue_gqa_fwd(const flash_prologue_gqa_args* args, void* stream);
+FLASH_PROLOGUE_API int flash_prologue_gqa_bwd(const flash_prologue_gqa_args* args, void* stream);
+/* Bytes of workspace flash_prologue_gqa_bwd needs on the current device, whatever the token count. */
+FLASH_PROLOGUE_API int flash_prologue_gqa_bwd_workspace_size(int64_t Hq, int64_t D, size_t* bytes);
+
+/*
+ * A paged cache of K and V and the requests it holds. Request r has
+ * seq_lens[r] tokens, the new ones of the call included; its token at position
+ * p lies in slot p % page_size of page page_table[r, p / page_size]. The new
+ * tokens of all requests are packed: request r's are tokens cu_seqlens[r] ..
+ * cu_seqlens[r + 1] - 1, its last ones; without cu_seqlens every request has
+ * one. Requests may share pages that hold a common beginning. page_size is a
+ * power of two, at least 8.
+ */
+typedef struct flash_prologue_cache {
+  void* k;
+  int64_t k_page, k_slot, k_head; /* element strides; the d stride is 1 */
+  void* v;
+  int64_t v_page, v_slot, v_head;
+  int64_t num_pages, page_size;
+  const int32_t* page_table;      /* [batch, max_pages], rows table_stride apart */
+  int64_t table_stride, max_pages;
+  const int32_t* seq_lens;        /* [batch] */
+  const int32_t* cu_seqlens;      /* [batch + 1] or NULL */
+  int64_t batch;
+} flash_prologue_cache;
+
+typedef struct flash_prologue_append_args {
+  flash_prologue_rows q, k, v;    /* packed rows of the new tokens: stride n per token */
+  flash_prologue_rows q_out;
+  const float* rmsnorm_weight;    /* [2, 1, D], 16-byte aligned; NULL: rotation only   */
+  const float* scales;            /* [Hq]; NULL: Q is not scaled                       */
+  flash_prologue_rotation rotation;
+  flash_prologue_cache cache;
+  int64_t tokens, Hq, Hk, D, dtype;
+  double eps;
+} flash_prologue_append_args;
+
+/*
+ * The prologue on a step's new tokens, each turned by its position in its
+ * request, with K and V written to the cache and Q to q_out. Tokens past the
+ * last request get zero Q rows and no cache write, like tokens whose position,
+ * page or table row is out of range (which also set the error word).
+ */
+FLASH_PROLOGUE_API int flash_prologue_append_paged(const flash_prologue_append_args* args, void* stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */
