@@ -29,6 +29,7 @@ _LAZY = {
     "fused_qkv_backward": ("gemm_bwd", "fused_qkv_backward"),
     "qknorm_rope_scale_gqa": ("gqa", "qknorm_rope_scale_gqa"),
     "append_paged_kv": ("paged", "append_paged_kv"),
+    "paged_attention": ("paged", "paged_attention"),
 }
 __all__ = ["qknorm_rope_scale", "qknorm_rope_scale_qkv", "prepare_backend", "RMSNormRoPEScale", "FusedQKV",
            *_LAZY]

@@ -89,6 +89,9 @@ SIGNATURES = {
     "flash_prologue_gqa_bwd": ([ctypes.c_char_p, _vp], ctypes.c_int),
     "flash_prologue_gqa_bwd_workspace_size": ([_i64, _i64, ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
     "flash_prologue_append_paged": ([ctypes.c_char_p, _vp], ctypes.c_int),
+    "flash_prologue_paged_attention": ([ctypes.c_char_p, _vp], ctypes.c_int),
+    "flash_prologue_paged_attention_workspace_size": ([_i64, _i64, _i64, ctypes.POINTER(ctypes.c_size_t)],
+                                                      ctypes.c_int),
 }
 
 # The argument structs of include/flash_prologue.h whose fields are all 8 bytes
@@ -96,6 +99,7 @@ SIGNATURES = {
 _ROWS, _ROTATION, _CACHE = "Pqqq", "PqqPqqq", "PqqqPqqqqqPqqPPq"
 GQA_ARGS = struct.Struct("@" + 8 * _ROWS + "PP" + _ROTATION + "Pqqq" + "PP" + "Pq" + "Pq" + "6q" + "d")
 APPEND_ARGS = struct.Struct("@" + 4 * _ROWS + "PP" + _ROTATION + _CACHE + "5q" + "d")
+ATTENTION_ARGS = struct.Struct("@" + 2 * _ROWS + "P" + _CACHE + "Pq" + "6q" + "d")
 NO_ROWS = (0, 0, 0, 0)
 
 MAX_PEERS = 8

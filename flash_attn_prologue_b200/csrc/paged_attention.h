@@ -1,0 +1,56 @@
+// Arguments of the paged attention kernels (paged_decode.cu, paged_prefill.cu).
+#pragma once
+
+#include "paged_host.h"
+
+namespace flash_prologue {
+
+struct AttentionArgs {
+  const void* q;
+  void* out;
+  float* lse;                // [T, Hq] natural logarithm, or null
+  int64_t q_n, q_h, out_n, out_h;
+  const void* k;
+  const void* v;
+  int64_t k_page, k_slot, k_head, v_page, v_slot, v_head;  // elements
+  PagedTarget pages;
+  int64_t tokens;
+  int heads, kv_heads, group;  // group = heads / kv_heads
+  float scale_log2;          // softmax_scale * log2(e)
+  int64_t window;            // keys a row sees at most; 0: all
+  void* workspace;
+  int64_t max_keys;          // pages.max_pages * page_size
+};
+
+// One request as the kernels see it: its new tokens and the keys it may reach.
+struct Request {
+  int64_t first;   // packed index of its first new token
+  int64_t news;    // new tokens
+  int64_t total;   // tokens in the cache
+};
+
+// Sizes are clamped to what the tensors hold, so wrong ones cannot lead outside
+// them. r == batch is the padding behind the last request: tokens without keys.
+__device__ __forceinline__ Request request_at(const PagedTarget& p, int64_t tokens, int64_t max_keys, int r,
+                                              bool* bad) {
+  Request q;
+  if (p.cu_seqlens) {
+    int64_t a = __ldg(p.cu_seqlens + r), b = r < p.batch ? (int64_t)__ldg(p.cu_seqlens + r + 1) : tokens;
+    a = a < 0 ? 0 : (a > tokens ? tokens : a);
+    b = b < a ? a : (b > tokens ? tokens : b);
+    q.first = a;
+    q.news = b - a;
+  } else {
+    q.first = r;
+    q.news = r < p.batch ? 1 : 0;
+  }
+  int64_t total = r < p.batch ? (int64_t)__ldg(p.seq_lens + r) : 0;
+  *bad = total > max_keys;
+  q.total = total < 0 ? 0 : (total > max_keys ? max_keys : total);
+  return q;
+}
+
+size_t paged_decode_workspace(int D, int sms);
+cudaError_t launch_paged_decode(const AttentionArgs& a, int dtype, int D, cudaStream_t stream);
+
+}  // namespace flash_prologue

@@ -1,6 +1,7 @@
 """Serving from a paged cache: the prologue on a step's new tokens with K and V
-appended to their pages (``append_paged_kv``). The reference ends before
-attention and has no cache.
+appended to their pages (``append_paged_kv``), and the attention of those tokens
+over the cache (``paged_attention``). The reference ends before attention and
+has no cache.
 
 A cache is two tensors ``[pages, page_size, Hk, D]`` (any strides with
 contiguous D, so ``[pages, Hk, page_size, D]`` memory is passed transposed) and,
@@ -9,13 +10,15 @@ new tokens counted). New tokens of all requests are packed along T in request
 order, split by ``cu_seqlens [B + 1]`` (int32); without it each request has one.
 Nothing is read back from the GPU, so a step can be captured in a CUDA graph.
 """
-from typing import Optional
+import ctypes
+import math
+from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
 from .fused_epilogue import _DeviceGuard
-from .gqa import check_rows, eager, flat_fp32, readable, rotation_of, rows_of
+from .gqa import MAX_HEADS, check_rows, eager, flat_fp32, readable, rotation_of, rows_of
 
 
 def _check_cache(q, heads, k_cache, v_cache, page_table, seq_lens, cu_seqlens):
@@ -115,3 +118,93 @@ def append_paged_kv(q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache,
     _no_grad("append_paged_kv", args)
     call = _append if eager(*args) else torch.ops.flash_prologue.append_paged_kv
     return call(*args, eps)
+
+
+ATTENTION_HEAD_DIMS = (64, 128)
+_WORKSPACE_BYTES = {}
+
+
+def _workspace_bytes(heads, kv_heads, dim):
+    key = (heads, kv_heads, dim, torch.cuda.current_device())
+    nbytes = _WORKSPACE_BYTES.get(key)
+    if nbytes is None:
+        out = ctypes.c_size_t(0)
+        _lib.check(_lib.load().flash_prologue_paged_attention_workspace_size(heads, kv_heads, dim, ctypes.byref(out)),
+                   "flash_prologue_paged_attention_workspace_size")
+        nbytes = _WORKSPACE_BYTES[key] = int(out.value)
+    return nbytes
+
+
+def _aligned_rows(q):
+    """q, or a copy whose rows start on 16 bytes and are contiguous along D."""
+    st = q.stride()
+    return q if st[2] == 1 and q.data_ptr() % 16 == 0 and not (st[0] | st[1]) % 8 else q.contiguous().clone()
+
+
+def _attention(q, k_cache, v_cache, page_table, seq_lens, cu_seqlens, softmax_scale, window, want_lse):
+    if q.ndim != 3:
+        raise ValueError("q must be packed [T,Hq,D]")
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("paged attention takes BF16 or FP16")
+    tokens, heads, dim = q.shape
+    if dim not in ATTENTION_HEAD_DIMS:
+        raise ValueError(f"head dimension must be one of {ATTENTION_HEAD_DIMS}")
+    kv_heads = k_cache.shape[2] if k_cache.ndim == 4 else 0
+    _check_cache(q, kv_heads, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
+    if kv_heads <= 0 or heads <= 0 or heads % kv_heads or heads > MAX_HEADS:
+        raise ValueError(f"query heads must be a multiple of the key heads and at most {MAX_HEADS}")
+    if not math.isfinite(softmax_scale):
+        raise ValueError("softmax_scale must be finite")
+    if window < 0:
+        raise ValueError("window must be 0 (all keys) or positive")
+    if q.device.type != "cuda":
+        raise ValueError("the attention kernels run on CUDA devices only")
+    q = _aligned_rows(q)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty(q.shape[:2] if want_lse else (0,), dtype=torch.float32, device=q.device)
+    if tokens:
+        with _DeviceGuard(q.device):
+            workspace = torch.empty(_workspace_bytes(heads, kv_heads, dim), dtype=torch.uint8, device=q.device)
+            args = _lib.ATTENTION_ARGS.pack(
+                *rows_of(q), *rows_of(out), lse.data_ptr() if want_lse else 0,
+                *_cache_of(k_cache, v_cache, page_table, seq_lens, cu_seqlens), workspace.data_ptr(),
+                workspace.numel(), tokens, heads, kv_heads, dim, _lib.DTYPE_CODES[q.dtype], window, softmax_scale)
+            _lib.check(_lib.load().flash_prologue_paged_attention(args, _lib.stream_of(q.device)),
+                       "flash_prologue_paged_attention")
+    return out, lse
+
+
+@torch.library.custom_op("flash_prologue::paged_attention", mutates_args=())
+def paged_attention_op(
+    q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+    seq_lens: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None, softmax_scale: float = 1.0, window: int = 0,
+    want_lse: bool = False,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    return _attention(q, k_cache, v_cache, page_table, seq_lens, cu_seqlens, softmax_scale, window, want_lse)
+
+
+@paged_attention_op.register_fake
+def _attention_fake(q, k_cache, v_cache, page_table, seq_lens, cu_seqlens=None, softmax_scale=1.0, window=0,
+                    want_lse=False):
+    return (torch.empty(q.shape, dtype=q.dtype, device=q.device),
+            torch.empty(q.shape[:2] if want_lse else (0,), dtype=torch.float32, device=q.device))
+
+
+def paged_attention(q, k_cache, v_cache, page_table, seq_lens, cu_seqlens=None, *, softmax_scale=1.0, window=0,
+                    return_lse=False):
+    """Attention of a step's new tokens over a paged cache that holds them already.
+
+    q [T,Hq,D] (BF16 or FP16, D 64 or 128; Hq a multiple of the cache's heads): the new tokens
+    of all requests as append_paged_kv returns them. A token at position p of its request
+    attends to the cached positions 0 .. p, or p - window + 1 .. p with a window; query head h
+    reads key head h // (Hq / Hk). softmax_scale multiplies the scores: 1 by default, since the
+    prologue's exp(scales) has scaled Q. Returns the rows [T,Hq,D] in q's type and, with
+    return_lse, the scores' log-sum-exp [T,Hq] in FP32. A token that sees no key gets zeros
+    (lse -inf); one whose page is outside the cache gets NaN and the device error word is set.
+    What lies in slots that a token does not see never reaches it. Not differentiable.
+    """
+    tensors = (q, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
+    _no_grad("paged_attention", tensors)
+    call = _attention if eager(*tensors) else torch.ops.flash_prologue.paged_attention
+    out, lse = call(*tensors, softmax_scale, window, return_lse)
+    return (out, lse) if return_lse else out

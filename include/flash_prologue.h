@@ -540,6 +540,34 @@ typedef struct flash_prologue_append_args {
  */
 FLASH_PROLOGUE_API int flash_prologue_append_paged(const flash_prologue_append_args* args, void* stream);
 
+typedef struct flash_prologue_attention_args {
+  flash_prologue_rows q, out;     /* packed rows of the new tokens: stride n per token */
+  float* lse;                     /* [tokens, Hq] or NULL                              */
+  flash_prologue_cache cache;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t tokens, Hq, Hk, D, dtype;
+  int64_t window;                 /* keys a token sees at most, its own included; 0: all */
+  double softmax_scale;
+} flash_prologue_attention_args;
+
+/*
+ * Attention of the new tokens over the cache (which holds them already): token
+ * i of request r has position p = seq_lens[r] - new tokens + i and
+ *   out = sum_j softmax_j(softmax_scale * <q, k_j>) v_j  over the keys j <= p,
+ * with a window over p - window < j <= p. Query head h reads key head
+ * h / (Hq / Hk). BF16 or FP16, D in {64, 128}; scores, statistics and sums are
+ * FP32. Keys that a token does not see never reach it, whatever their slots
+ * hold. A token that sees no key (position below 0, padding past the last
+ * request) gets zeros and an lse of -infinity; one that needs a page outside
+ * the cache gets NaN, and the error word. Results are the same run to run.
+ * Rows and caches are 16-byte aligned. workspace: 16-byte aligned, at least
+ * flash_prologue_paged_attention_workspace_size() bytes, no initialisation.
+ */
+FLASH_PROLOGUE_API int flash_prologue_paged_attention(const flash_prologue_attention_args* args, void* stream);
+/* Bytes of workspace for these heads on the current device, whatever the lengths. */
+FLASH_PROLOGUE_API int flash_prologue_paged_attention_workspace_size(int64_t Hq, int64_t Hk, int64_t D, size_t* bytes);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif
