@@ -51,6 +51,17 @@ __device__ __forceinline__ Request request_at(const PagedTarget& p, int64_t toke
 }
 
 size_t paged_decode_workspace(int D, int sms);
+struct PrefillPlan {
+  int tile_tokens;   // whole tokens of a 128-row tile
+  int splits;        // shares of a tile's keys
+  int64_t tiles;     // tiles there can be, all requests
+  size_t workspace;  // bytes; 0 without shares
+};
+PrefillPlan plan_paged_prefill(int64_t tokens, int64_t batch, bool ragged, int64_t kv_heads, int64_t group, int D,
+                               int64_t max_keys, int64_t window, int sms);
+// False where the cache's layout has no tensor map (the other kernel reads it).
+bool launch_paged_prefill(const AttentionArgs& a, const PrefillPlan& plan, int dtype, int D, int64_t page_size,
+                          cudaStream_t stream, cudaError_t* err);
 cudaError_t launch_paged_decode(const AttentionArgs& a, int dtype, int D, cudaStream_t stream);
 
 }  // namespace flash_prologue

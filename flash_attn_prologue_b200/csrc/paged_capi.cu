@@ -19,34 +19,56 @@ int device_sms() {
   return sms;
 }
 
-int head_checks(int64_t Hq, int64_t Hk, int64_t D) {
-  if (Hq < 0 || Hk <= 0 || Hq % Hk != 0) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
-  return Hq > kMaxGqaHeads || (D != 64 && D != 128) ? FLASH_PROLOGUE_ERR_UNSUPPORTED : FLASH_PROLOGUE_OK;
+int size_checks(const flash_prologue_attention_args* a) {
+  if (!a || a->tokens < 0 || a->window < 0 || !isfinite(a->softmax_scale) || a->Hq < 0 || a->Hk <= 0 || a->Hq % a->Hk)
+    return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
+  if ((a->dtype != FLASH_PROLOGUE_BF16 && a->dtype != FLASH_PROLOGUE_FP16) || a->Hq > kMaxGqaHeads ||
+      (a->D != 64 && a->D != 128) || a->tokens >= (int64_t(1) << 31) / kMaxGqaHeads)
+    return FLASH_PROLOGUE_ERR_UNSUPPORTED;
+  return check_cache(a->cache, a->tokens, a->dtype);
+}
+
+// Tiles of 128 rows on the tensor cores where the requests have more rows a key
+// head than the other kernel's 16-row tile on average. The tiled kernel takes
+// the maximum of the unscaled scores, so the scale has to be positive, and a
+// tile holds at least one whole token.
+bool use_prefill(const flash_prologue_attention_args* a) {
+  const int64_t group = a->Hq / a->Hk;
+  return a->tokens * group > 16 * a->cache.batch && group <= 128 && a->softmax_scale > 0;
+}
+
+PrefillPlan plan_of(const flash_prologue_attention_args* a, int sms) {
+  const flash_prologue_cache& c = a->cache;
+  return plan_paged_prefill(a->tokens, c.batch, c.cu_seqlens != nullptr, a->Hk, a->Hq / a->Hk, (int)a->D,
+                            c.max_pages * c.page_size, a->window, sms);
+}
+
+// Room for either kernel: the tiled one gives way to the other where the cache has no tensor map.
+size_t workspace_of(const flash_prologue_attention_args* a, int sms) {
+  const size_t decode = paged_decode_workspace((int)a->D, sms);
+  if (!use_prefill(a)) return decode;
+  const size_t prefill = plan_of(a, sms).workspace;
+  return prefill > decode ? prefill : decode;
 }
 
 }  // namespace
 
 extern "C" {
 
-int flash_prologue_paged_attention_workspace_size(int64_t Hq, int64_t Hk, int64_t D, size_t* bytes) {
-  if (!bytes) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
+int flash_prologue_paged_attention_workspace_size(const flash_prologue_attention_args* a, size_t* bytes) {
+  if (!a || !bytes) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
   *bytes = 0;
-  const int st = head_checks(Hq, Hk, D);
-  if (st != FLASH_PROLOGUE_OK) return st;
+  const int st = size_checks(a);
+  if (st != FLASH_PROLOGUE_OK || a->tokens == 0 || a->Hq == 0) return st;
   const int sms = device_sms();
   if (sms <= 0) return FLASH_PROLOGUE_ERR_CUDA;
-  *bytes = paged_decode_workspace((int)D, sms);
+  *bytes = workspace_of(a, sms);
   return FLASH_PROLOGUE_OK;
 }
 
 int flash_prologue_paged_attention(const flash_prologue_attention_args* a, void* stream) {
-  if (!a || a->tokens < 0 || a->window < 0 || !isfinite(a->softmax_scale)) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
-  if (a->dtype != FLASH_PROLOGUE_BF16 && a->dtype != FLASH_PROLOGUE_FP16) return FLASH_PROLOGUE_ERR_UNSUPPORTED;
-  int st = head_checks(a->Hq, a->Hk, a->D);
-  if (st != FLASH_PROLOGUE_OK) return st;
-  if (a->tokens >= (int64_t(1) << 31) / 512) return FLASH_PROLOGUE_ERR_UNSUPPORTED;
+  const int st = size_checks(a);
   const flash_prologue_cache& c = a->cache;
-  st = check_cache(c, a->tokens, a->dtype);
   if (st != FLASH_PROLOGUE_OK || a->tokens == 0 || a->Hq == 0) return st;
   if (!a->q.data || !a->out.data) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
   if ((reinterpret_cast<uintptr_t>(a->q.data) | reinterpret_cast<uintptr_t>(a->out.data)) & 15 ||
@@ -56,7 +78,7 @@ int flash_prologue_paged_attention(const flash_prologue_attention_args* a, void*
   const int sms = device_sms();
   if (sms <= 0) return FLASH_PROLOGUE_ERR_CUDA;
   if (!a->workspace || (reinterpret_cast<uintptr_t>(a->workspace) & 15) ||
-      a->workspace_bytes < (int64_t)paged_decode_workspace((int)a->D, sms))
+      a->workspace_bytes < (int64_t)workspace_of(a, sms))
     return FLASH_PROLOGUE_ERR_WORKSPACE;
   AttentionArgs g{};
   g.q = a->q.data;
@@ -83,6 +105,12 @@ int flash_prologue_paged_attention(const flash_prologue_attention_args* a, void*
   g.window = a->window;
   g.workspace = a->workspace;
   g.max_keys = c.max_pages * c.page_size;
+  if (use_prefill(a)) {
+    cudaError_t err = cudaSuccess;
+    if (launch_paged_prefill(g, plan_of(a, sms), (int)a->dtype, (int)a->D, c.page_size,
+                             static_cast<cudaStream_t>(stream), &err))
+      return err == cudaSuccess ? FLASH_PROLOGUE_OK : FLASH_PROLOGUE_ERR_CUDA;
+  }
   return launch_paged_decode(g, (int)a->dtype, (int)a->D, static_cast<cudaStream_t>(stream)) == cudaSuccess
              ? FLASH_PROLOGUE_OK
              : FLASH_PROLOGUE_ERR_CUDA;

@@ -1,0 +1,726 @@
+// Attention of chunks of new tokens over a paged cache on the tensor cores
+// (tcgen05): o_i = sum_j p_ij v_j with p the softmax of the scaled scores over
+// the keys that row i sees (causal, optional window).
+//
+// Bound by the tensor cores and, as much, by the exponentials: a block of 128
+// rows x 128 keys costs 4 * 128 * 128 * D operations (1,024 cycles of an SM's
+// tensor core at D = 128) and 128 * 128 exponentials (1,024 cycles of its 16 a
+// cycle). The chain of one tile -- scores, softmax, product with V -- cannot
+// overlap itself, so two CTAs share an SM, each with 256 of its 512
+// tensor-memory columns, and one's softmax runs beside the other's products.
+//
+// A CTA takes one tile: the rows (query heads x whole tokens) of one key head
+// that fit into 128, and its blocks of 128 keys (or a share of them where
+// there are fewer tiles than the GPU holds; paged_join adds the shares up).
+//   warps 0-3  one row a thread: scores from tensor memory, running maximum
+//              and sum, probabilities back to tensor memory over the scores
+//              they came from, output to global memory;
+//   warp 4     issues S = Q K^T (both from shared memory) and O += P V (P from
+//              tensor memory, V read transposed from shared memory);
+//   warp 5     TMA loads of K and V, one box of a page a lane;
+//   warps 6-7  clean V in blocks that some row of the tile does not see whole:
+//              zeros for slots outside the tile's keys, and for infinities and
+//              NaNs, which 0 * V would carry into rows that do not see them
+//              (the epilogue adds them to the rows that do).
+// The running maximum that scales O is only moved when a row's maximum has
+// grown by more than 2^8: until then the probabilities are at most 2^8 instead
+// of 1, which neither type nor sum minds, and O stays where it is.
+//
+// Scores, statistics, sums and O are FP32; the probabilities are rounded to the
+// cache's type for the second product (their sum is taken before the rounding),
+// an error of the size of the output's own rounding. Waits are bounded; tensor
+// memory is released on every path.
+#include "paged_attention.h"
+#include "tensor_map.h"
+#include "umma_util.cuh"
+
+namespace flash_prologue {
+namespace {
+
+constexpr int kTile = 128;             // rows of a tile, keys of a block
+constexpr int kPrefillThreads = 256;
+constexpr int kRowThreads = 128;
+constexpr int kSCol = 0, kOCol = 128;  // tensor-memory columns: scores / probabilities, output
+constexpr int kTmemCols = 256;
+constexpr int kLaunchRegs = 128, kRowRegs = 200, kOtherRegs = 56;
+static_assert(kRowThreads * kRowRegs + (kPrefillThreads - kRowThreads) * kOtherRegs <= kPrefillThreads * kLaunchRegs,
+              "register split exceeds the block's launch allocation");
+
+template <int D>
+struct Layout {
+  static constexpr int kHalves = D / 64;           // 64-column (128-byte) halves of a row
+  static constexpr int kStages = D == 64 ? 2 : 1;  // K and V blocks in flight
+  static constexpr int kOperand = kTile * D * 2;   // bytes of a Q tile, a K block or a V block
+  static constexpr int kHalfBytes = kTile * 128;
+  static constexpr size_t kSmem = 1024 + (size_t)kOperand * (1 + 2 * kStages);
+};
+
+struct Barriers {
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], v_clean[2], s_full, p_full, o_full, drain;
+  uint32_t tmem;
+  int bad, wild;
+  int64_t sums[kPrefillThreads / 32];
+  int64_t found[2];
+};
+
+struct Tile {  // what the join needs to know of a tile
+  int64_t token0;
+  int rows, kv_head, parts;
+};
+
+struct PrefillArgs {
+  AttentionArgs a;
+  int tile_tokens;       // whole tokens of a tile: 128 / group
+  int splits;            // shares a tile's blocks may be cut into
+  int box_rows;          // keys of a TMA box: page_size, at most 128
+  int64_t tiles;         // tiles the grid has room for, all requests
+  float* part_out;       // [tiles * kv_heads * splits][128][D]
+  float* part_stat;      // [...][128][2]
+  Tile* joins;           // [tiles * kv_heads]
+};
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem], issued by one thread.
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
+      ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+        "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]),
+        "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]),
+        "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Names 32 registers behind a tcgen05.wait::ld, so that no use of them moves above it.
+__device__ __forceinline__ void pin(uint32_t (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    asm volatile("" : "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3]), "+r"(v[i + 4]), "+r"(v[i + 5]),
+                      "+r"(v[i + 6]), "+r"(v[i + 7]));
+}
+// kind::f16 with A and B of one 16-bit type (format 1: BF16, 0: FP16), FP32 accumulator.
+template <typename T>
+__host__ __device__ constexpr uint32_t idesc_of(int N, bool b_mn) {
+  constexpr uint32_t f = std::is_same<T, __half>::value ? 0u : 1u;
+  return (1u << 4) | (f << 7) | (f << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) |
+         ((uint32_t)(kTile >> 4) << 24);
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+template <typename T>
+constexpr uint32_t kExponent = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+
+// The keys of a tile and the split's share of its blocks.
+struct Work {
+  Request q;
+  int r;
+  int head;
+  int64_t tile;         // of the request
+  int64_t token0;       // first token of the tile, of the request's new ones
+  int rows;             // valid rows
+  int64_t pos0, pos1;   // positions of the first and last token
+  int64_t lo, hi;       // keys that some row sees
+  int64_t first, last;  // this split's blocks (of 128 keys)
+  int parts;            // splits that have blocks
+};
+
+__device__ __forceinline__ bool partial_block(const Work& w, int64_t window, int64_t block) {
+  const int64_t kb = block * kTile;
+  return kb + kTile - 1 > w.pos0 || (window && kb < w.pos1 - window + 1);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kPrefillThreads, 2)
+    paged_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                         const __grid_constant__ PrefillArgs p) {
+  using L = Layout<D>;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ Barriers bar;
+  const AttentionArgs& a = p.a;
+  unsigned char* q_s = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  unsigned char* k_s = q_s + L::kOperand;
+  unsigned char* v_s = k_s + L::kStages * L::kOperand;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // ---- this CTA's tile: last tiles first (they have the most keys), splits innermost
+  const int64_t item = (int64_t)blockIdx.x / p.splits;
+  const int split = (int)(blockIdx.x - item * p.splits);
+  const int64_t tile_of_all = p.tiles - 1 - item / a.kv_heads;
+  const int requests = a.pages.batch + (a.pages.cu_seqlens ? 1 : 0);
+  if (threadIdx.x == 0) bar.found[0] = -1;
+  __syncthreads();
+  int64_t before = 0;
+  for (int r0 = 0; r0 < requests; r0 += kPrefillThreads) {
+    const int r = r0 + threadIdx.x;
+    int64_t n = 0;
+    if (r < requests) {
+      bool too_long;
+      const Request q = request_at(a.pages, a.tokens, a.max_keys, r, &too_long);
+      n = (q.news + p.tile_tokens - 1) / p.tile_tokens;
+      if (too_long && n) atomicOr(&g_device_error, kDeviceErrorIndex);
+    }
+    int64_t upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 31) bar.sums[warp] = upto;
+    __syncthreads();
+    int64_t start = before + upto - n, all = 0;
+#pragma unroll
+    for (int w = 0; w < kPrefillThreads / 32; ++w) {
+      if (w < warp) start += bar.sums[w];
+      all += bar.sums[w];
+    }
+    if (tile_of_all >= start && tile_of_all < start + n) {
+      bar.found[0] = r;
+      bar.found[1] = tile_of_all - start;
+    }
+    before += all;
+    __syncthreads();
+    if (before > tile_of_all) break;
+  }
+  Tile* join = p.joins ? p.joins + item : nullptr;
+  if (bar.found[0] < 0) {  // the grid has room for more tiles than there are
+    if (join && split == 0 && threadIdx.x == 0) join->parts = 0;
+    return;
+  }
+  Work w;
+  w.r = (int)bar.found[0];
+  w.tile = bar.found[1];
+  w.head = (int)(item % a.kv_heads);
+  bool too_long;
+  w.q = request_at(a.pages, a.tokens, a.max_keys, w.r, &too_long);
+  w.token0 = w.tile * p.tile_tokens;
+  const int64_t tokens = min((int64_t)p.tile_tokens, w.q.news - w.token0);
+  w.rows = (int)tokens * a.group;
+  w.pos0 = w.q.total - w.q.news + w.token0;
+  w.pos1 = w.pos0 + tokens - 1;
+  w.hi = w.pos1 + 1 > 0 ? w.pos1 + 1 : 0;
+  w.lo = a.window && w.pos0 - a.window + 1 > 0 ? w.pos0 - a.window + 1 : 0;
+  {
+    const int64_t first = w.lo / kTile, last = (w.hi + kTile - 1) / kTile;
+    const int64_t blocks = last > first ? last - first : 0;
+    // Shares of at least two blocks: a share's fixed cost is about that of two blocks.
+    int64_t share = (blocks + p.splits - 1) / p.splits;
+    if (share < 2) share = 2;
+    w.parts = blocks ? (int)((blocks + share - 1) / share) : 1;
+    w.first = first + split * share;
+    w.last = min(first + blocks, w.first + share);
+  }
+  if (join && split == 0 && threadIdx.x == 0) {
+    join->token0 = w.q.first + w.token0;
+    join->rows = w.rows;
+    join->kv_head = w.head;
+    join->parts = w.parts;
+  }
+  if (split >= w.parts) return;
+  const int blocks = w.last > w.first ? (int)(w.last - w.first) : 0;
+
+  // ---- barriers, tensor memory, Q
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bar.k_full[s], 1);
+      mbar_init(&bar.k_empty[s], 1);
+      mbar_init(&bar.v_full[s], 1);
+      mbar_init(&bar.v_empty[s], 1);
+      mbar_init(&bar.v_clean[s], 2);
+    }
+    mbar_init(&bar.s_full, 1);
+    mbar_init(&bar.p_full, kRowThreads / 32);
+    mbar_init(&bar.o_full, 1);
+    mbar_init(&bar.drain, 1);
+    bar.bad = too_long;
+    bar.wild = 0;
+    fence_mbar_init();
+  }
+  if (warp == 4) {
+    tmem_alloc(&bar.tmem, kTmemCols);
+    tmem_relinquish();
+  }
+  for (int i = threadIdx.x; i < kTile * (D / 8); i += kPrefillThreads) {
+    const int row = i / (D / 8), c = i % (D / 8);
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (row < w.rows) {
+      const int t = row / a.group, g = row - t * a.group;
+      v = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (w.q.first + w.token0 + t) * a.q_n +
+                                               (int64_t)(w.head * a.group + g) * a.q_h + c * 8));
+    }
+    *reinterpret_cast<uint4*>(q_s + (c >> 3) * L::kHalfBytes + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
+  }
+  fence_proxy_async_smem();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bar.tmem;
+
+  // Row state (warps 0-3); the row's keys are [see_lo, see_hi].
+  const int row = threadIdx.x;
+  int64_t see_hi = -1, see_lo = 0;
+  float top = -INFINITY, sum = 0.f;
+
+  if (warp >= 4) {
+    setmaxnreg_dec<kOtherRegs>();
+    if (warp == 4 && lane == 0) {
+      // ---------------- products ----------------
+      constexpr uint32_t idesc_s = idesc_of<T>(kTile, false), idesc_o = idesc_of<T>(D, true);
+      bool failed = false;
+      auto scores = [&](int j) {
+        const int s = j % L::kStages;
+        if (!mbar_wait(&bar.k_full[s], (j / L::kStages) & 1)) return false;
+        tc_fence_after();
+        const uint32_t k = smem_u32(k_s) + s * L::kOperand, q = smem_u32(q_s);
+#pragma unroll
+        for (int h = 0; h < L::kHalves; ++h) {
+          const uint64_t qd = smem_desc_k_sw128(q + h * L::kHalfBytes), kd = smem_desc_k_sw128(k + h * L::kHalfBytes);
+#pragma unroll
+          for (int c = 0; c < 4; ++c)  // 16 columns (32 bytes) a step
+            umma_bf16(tmem + kSCol, qd + 2 * c, kd + 2 * c, idesc_s, (h | c) != 0);
+        }
+        umma_commit(&bar.k_empty[s]);
+        umma_commit(&bar.s_full);
+        return true;
+      };
+      if (blocks) failed = !scores(0);
+      for (int j = 0; j < blocks && !failed; ++j) {
+        const int s = j % L::kStages;
+        if (!mbar_wait(&bar.v_clean[s], (j / L::kStages) & 1)) { failed = true; break; }
+        if (!mbar_wait(&bar.p_full, j & 1)) { failed = true; break; }
+        tc_fence_after();
+        const uint32_t v = smem_u32(v_s) + s * L::kOperand;
+        const uint64_t vd = smem_desc_mn_sw128(v, L::kHalfBytes);
+#pragma unroll
+        for (int c = 0; c < kTile / 16; ++c)  // 16 keys a step: 8 columns of P, two 8-row groups of V (2,048 bytes)
+          umma_ts(tmem + kOCol, tmem + kSCol + 8 * c, vd + 128 * c, idesc_o, (j | c) != 0);
+        umma_commit(&bar.v_empty[s]);
+        // The next scores overwrite P: products of one thread run in the order they were issued in.
+        if (j + 1 < blocks) failed = !scores(j + 1);
+        else umma_commit(&bar.o_full);
+      }
+      if (failed) {  // tensor memory is not released under products still running
+        umma_commit(&bar.drain);
+        mbar_wait(&bar.drain, 0);
+      }
+    } else if (warp == 5) {
+      // ---------------- loads ----------------
+      const int boxes = kTile / p.box_rows;
+      const int32_t* table = a.pages.page_table + (int64_t)w.r * a.pages.table_stride;
+      const int in_page = (1 << a.pages.page_log2) - 1;
+      // The page of this lane's box of a block, -1 where there is nothing to load.
+      auto page_of = [&](int j) {
+        int page = -1;
+        if (lane < boxes && j < blocks) {
+          const int64_t key = (w.first + j) * kTile + lane * p.box_rows;
+          if (key < w.hi && key + p.box_rows > w.lo) {
+            page = __ldg(table + (key >> a.pages.page_log2));
+            if (page < 0 || page >= a.pages.num_pages) {
+              page = -1;
+              bar.bad = 1;
+            }
+          }
+        }
+        return page;
+      };
+      const uint32_t box_bytes = (uint32_t)p.box_rows * 128;
+      bool ok = true;
+      auto load = [&](int j, int page, const CUtensorMap* map, unsigned char* ring, uint64_t* full, uint64_t* empty) {
+        const int s = j % L::kStages;
+        if (!__all_sync(0xffffffffu, mbar_wait(&empty[s], ((j / L::kStages) & 1) ^ 1))) return false;
+        const uint32_t count = __popc(__ballot_sync(0xffffffffu, page >= 0));
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], count * box_bytes * L::kHalves);
+        __syncwarp();
+        if (page >= 0) {
+          const int64_t key = (w.first + j) * kTile + lane * p.box_rows;
+          const uint32_t dst = smem_u32(ring) + s * L::kOperand + lane * box_bytes;
+#pragma unroll
+          for (int h = 0; h < L::kHalves; ++h)
+            tma_load_4d(dst + h * L::kHalfBytes, map, h * 64, (int)(key & in_page), w.head, page, &full[s]);
+        }
+        __syncwarp();
+        return true;
+      };
+      int page = page_of(0);
+      int j = 0;
+      for (; j < blocks && ok; ++j) {
+        const int next = page_of(j + 1);
+        ok = load(j, page, &k_map, k_s, bar.k_full, bar.k_empty) && load(j, page, &v_map, v_s, bar.v_full, bar.v_empty);
+        page = next;
+        if (!ok) break;
+      }
+      // No product's arrival on an empty barrier lands after the CTA has gone.
+      for (int e = blocks; e < blocks + L::kStages && blocks && ok; ++e) {
+        const int s = e % L::kStages;
+        ok = mbar_wait(&bar.k_empty[s], ((e / L::kStages) & 1) ^ 1) && mbar_wait(&bar.v_empty[s], ((e / L::kStages) & 1) ^ 1);
+      }
+      if (j < blocks) {  // a wait ran out: wait (bounded) for the loads still in flight
+        for (int s = 0; s < L::kStages; ++s) {
+          for (int e = j; e >= 0 && e > j - L::kStages - 1; --e)
+            if (e % L::kStages == s) {
+              mbar_wait(&bar.k_full[s], (e / L::kStages) & 1);
+              mbar_wait(&bar.v_full[s], (e / L::kStages) & 1);
+              break;
+            }
+        }
+      }
+    } else if (warp >= 6) {
+      // ---------------- cleaning ----------------
+      const int t = (warp - 6) * 32 + lane;
+      for (int j = 0; j < blocks; ++j) {
+        // Every block is passed on, so that a barrier's phases are never counted past.
+        const int s = j % L::kStages;
+        if (!__all_sync(0xffffffffu, mbar_wait(&bar.v_full[s], (j / L::kStages) & 1))) break;
+        if (!partial_block(w, a.window, w.first + j)) {
+          if (lane == 0) mbar_arrive(&bar.v_clean[s]);
+          continue;
+        }
+        const int64_t kb = (w.first + j) * kTile;
+        uint4* v = reinterpret_cast<uint4*>(v_s + s * L::kOperand);
+        bool wild = false;
+#pragma unroll 4
+        for (int i = t; i < kTile * D / 8; i += 64) {
+          const int64_t key = kb + ((i >> 3) & (kTile - 1));
+          uint4 x = v[i];
+          if (key < w.lo || key >= w.hi) {
+            v[i] = make_uint4(0, 0, 0, 0);
+            continue;
+          }
+          uint32_t* word = reinterpret_cast<uint32_t*>(&x);
+          bool changed = false;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            constexpr uint32_t m = kExponent<T>;
+            if ((word[e] & m) == m) { word[e] &= 0xffff0000u; changed = true; }
+            if ((word[e] >> 16 & m) == m) { word[e] &= 0x0000ffffu; changed = true; }
+          }
+          if (changed) {
+            v[i] = x;
+            wild = true;
+          }
+        }
+        if (wild) bar.wild = 1;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.v_clean[s]);
+      }
+    }
+  } else {
+    // ---------------- softmax ----------------
+    setmaxnreg_inc<kRowRegs>();
+    if (row < w.rows) {
+      see_hi = w.pos0 + row / a.group;
+      if (a.window && see_hi - a.window + 1 > 0) see_lo = see_hi - a.window + 1;
+    }
+    const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
+    const float scale = a.scale_log2;
+    bool ok = true;
+    for (int j = 0; j < blocks; ++j) {
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(&bar.s_full, j & 1)))) break;
+      tc_fence_after();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(mine + kSCol + 32 * c, s[c]);
+      tmem_wait_ld();
+#pragma unroll
+      for (int c = 0; c < 4; ++c) pin(s[c]);
+      const int64_t block = w.first + j;
+      if (partial_block(w, a.window, block)) {
+        const int64_t kb = block * kTile;
+        const int64_t hi64 = see_hi - kb, lo64 = see_lo - kb;
+        const int hi = hi64 > kTile ? kTile : (hi64 < -1 ? -1 : (int)hi64);
+        const int lo = lo64 > kTile ? kTile : (lo64 < 0 ? 0 : (int)lo64);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (32 * c + i > hi || 32 * c + i < lo) s[c][i] = 0xff800000u;  // -infinity
+      }
+      float most[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        most[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+        for (int i = 1; i < 32; ++i) most[c] = fmaxf(most[c], __uint_as_float(s[c][i]));
+      }
+      const float block_top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+      const float now = fmaxf(top, block_top);
+      const bool fresh = top == -INFINITY;  // nothing summed yet, O is zero
+      if (fresh) top = now;
+      const bool move = !fresh && (now - top) * scale > 8.f;
+      // O is at rest here: these scores were issued behind the last product with V.
+      if (__any_sync(0xffffffffu, move)) {
+        const float f = move ? exp2_approx((top - now) * scale) : 1.f;
+        sum *= f;
+        if (move) top = now;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(mine + kOCol + 32 * c, o);
+          tmem_wait_ld();
+          pin(o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+          tmem_st32(mine + kOCol + 32 * c, o);
+        }
+        tmem_wait_st();
+      }
+      const float from = top == -INFINITY ? 0.f : top * scale;
+      const float2 scale2 = make_float2(scale, scale), from2 = make_float2(-from, -from);
+      float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t out[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const int c = half * 2 + (i >> 4), e = (i & 15) * 2;
+          float2 x = __ffma2_rn(make_float2(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])), scale2, from2);
+          x.x = exp2_approx(x.x);
+          x.y = exp2_approx(x.y);
+          add[i & 1] = __fadd2_rn(add[i & 1], x);
+          out[i] = pack2<T>(x.x, x.y);
+        }
+        tmem_st32(mine + kSCol + 32 * half, out);
+      }
+      const float2 both = __fadd2_rn(add[0], add[1]);
+      sum += both.x + both.y;
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar.p_full);
+    }
+    if (blocks && ok) mbar_wait(&bar.o_full, 0);
+  }
+  __syncthreads();  // `bad` and `wild` are final
+
+  // ---- output
+  if (warp < 4) {
+    tc_fence_after();
+    const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
+    const bool bad = bar.bad, wild = bar.wild, whole = w.parts == 1;
+    const float nan = __int_as_float(0x7fc00000);
+    if (bad) sum = nan;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int t = row / a.group, g = row - t * a.group;
+    const int64_t token = w.q.first + w.token0 + t;
+    const int h = w.head * a.group + g;
+    const bool valid = row < w.rows;
+    const int64_t slot = item * p.splits + split;
+    const float top2 = top == -INFINITY ? top : top * a.scale_log2;
+#pragma unroll 1
+    for (int c = 0; c < D / 32; ++c) {
+      uint32_t o[32];
+      __syncwarp();
+      if (blocks) {
+        tmem_ld32(mine + kOCol + 32 * c, o);
+        tmem_wait_ld();
+        pin(o);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = 0;
+      }
+      if (wild && valid) {
+        // The infinities and NaNs taken out of V, added to a row that sees them.
+        for (int j = 0; j < blocks; ++j) {
+          if (!partial_block(w, a.window, w.first + j)) continue;
+          const int64_t kb = (w.first + j) * kTile;
+          const int64_t k0 = kb > see_lo ? kb : see_lo, k1 = min(kb + kTile - 1, see_hi);
+          for (int64_t k = k0; k <= k1; ++k) {
+            const int32_t* entry = a.pages.page_table + (int64_t)w.r * a.pages.table_stride + (k >> a.pages.page_log2);
+            const int64_t page = __ldg(entry);
+            if (page < 0 || page >= a.pages.num_pages) continue;
+            const T* v = static_cast<const T*>(a.v) + page * a.v_page +
+                         (k & ((1 << a.pages.page_log2) - 1)) * a.v_slot + w.head * a.v_head + 32 * c;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float x = (float)v[i];
+              if (!isfinite(x)) o[i] = __float_as_uint(__uint_as_float(o[i]) + x);
+            }
+          }
+        }
+      }
+      if (!valid) continue;
+      if (whole) {
+        uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + token * a.out_n + (int64_t)h * a.out_h + 32 * c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            x[e] = pack2<T>(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
+          out[i] = make_uint4(x[0], x[1], x[2], x[3]);
+        }
+      } else {
+        float4* out = reinterpret_cast<float4*>(p.part_out + (slot * kTile + row) * D + 32 * c);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          out[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
+                               __uint_as_float(o[4 * i + 3]));
+      }
+    }
+    if (valid) {
+      if (!whole) {
+        p.part_stat[(slot * kTile + row) * 2] = top2;
+        p.part_stat[(slot * kTile + row) * 2 + 1] = sum;
+      } else if (a.lse) {
+        a.lse[token * a.heads + h] = (top2 + log2f(sum)) * 0.6931471805599453f;
+      }
+    }
+  }
+  if (threadIdx.x == 0 && bar.bad) atomicOr(&g_device_error, kDeviceErrorIndex);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// Adds up the shares of a tile, a row a warp: 16 rows a CTA.
+template <typename T, int D>
+__global__ void __launch_bounds__(512) prefill_join_kernel(const PrefillArgs p) {
+  const AttentionArgs& a = p.a;
+  const int64_t item = blockIdx.x / (kTile / 16);
+  const Tile t = p.joins[item];
+  const int row = (int)(blockIdx.x % (kTile / 16)) * 16 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (t.parts <= 1 || row >= t.rows) return;
+  const int64_t slot0 = item * p.splits;
+  float m = -INFINITY;
+  for (int s = 0; s < t.parts; ++s) m = fmaxf(m, p.part_stat[((slot0 + s) * kTile + row) * 2]);
+  const float from = m == -INFINITY ? 0.f : m;
+  float o[D / 32] = {}, l = 0.f;
+  for (int s = 0; s < t.parts; ++s) {
+    const int64_t at = (slot0 + s) * kTile + row;
+    const float f = exp2_approx(p.part_stat[at * 2] - from);
+    l += f * p.part_stat[at * 2 + 1];
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) o[c] += f * p.part_out[at * D + 32 * c + lane];
+  }
+  const int token = row / a.group, h = t.kv_head * a.group + row - token * a.group;
+  T* out = static_cast<T*>(a.out) + (t.token0 + token) * a.out_n + (int64_t)h * a.out_h;
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) {
+    const float x = l == 0.f ? 0.f : o[c] / l;
+    if constexpr (std::is_same<T, __half>::value) out[32 * c + lane] = __float2half_rn(x);
+    else out[32 * c + lane] = __float2bfloat16_rn(x);
+  }
+  if (a.lse && lane == 0) a.lse[(t.token0 + token) * a.heads + h] = (m + log2f(l)) * 0.6931471805599453f;
+}
+
+// A cache as {D, slots, heads, pages}, a box of 64 columns x box_rows slots.
+bool encode_cache(CUtensorMap* map, const void* base, int dtype, int D, int64_t page_size, int64_t heads, int64_t pages,
+                  int64_t s_slot, int64_t s_head, int64_t s_page, int box_rows) {
+  const uint64_t dims[4] = {(uint64_t)D, (uint64_t)page_size, (uint64_t)heads, (uint64_t)pages};
+  // A dimension of one entry gets a stride that no address depends on.
+  const uint64_t strides[3] = {(uint64_t)(2 * s_slot), heads > 1 ? (uint64_t)(2 * s_head) : 128,
+                               pages > 1 ? (uint64_t)(2 * s_page) : 128};
+  for (uint64_t s : strides)
+    if (s == 0 || (int64_t)s < 0) return false;
+  const uint32_t box[4] = {64, (uint32_t)box_rows, 1, 1};
+  return encode_tensor_map(map, dtype == 0 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base,
+                           dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <typename T, int D>
+cudaError_t launch(const CUtensorMap& k_map, const CUtensorMap& v_map, const PrefillArgs& p, int64_t items,
+                   cudaStream_t stream) {
+  const void* fn = reinterpret_cast<const void*>(&paged_prefill_kernel<T, D>);
+  // setmaxnreg only completes where the kernel starts with kLaunchRegs a thread.
+  static const int regs = [fn] {
+    cudaFuncAttributes attr;
+    return cudaFuncGetAttributes(&attr, fn) == cudaSuccess ? attr.numRegs : 0;
+  }();
+  if (regs < kLaunchRegs) return cudaErrorInvalidConfiguration;
+  cudaError_t err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Layout<D>::kSmem);
+  if (err != cudaSuccess) return err;
+  err = launch_kernel(paged_prefill_kernel<T, D>, dim3((unsigned)(items * p.splits)), dim3(kPrefillThreads),
+                      Layout<D>::kSmem, stream, k_map, v_map, p);
+  if (err != cudaSuccess || p.splits == 1) return err;
+  return launch_kernel(prefill_join_kernel<T, D>, dim3((unsigned)(items * (kTile / 16))), dim3(512), 0, stream, p);
+}
+
+}  // namespace
+
+// Tiles, and the shares their blocks are cut into where there are fewer tiles
+// than the GPU holds CTAs (lengths are only known on the device: their bound is
+// the page table's width).
+PrefillPlan plan_paged_prefill(int64_t tokens, int64_t batch, bool ragged, int64_t kv_heads, int64_t group, int D,
+                               int64_t max_keys, int64_t window, int sms) {
+  PrefillPlan p{};
+  p.tile_tokens = (int)(kTile / group);
+  p.tiles = ragged ? (tokens + p.tile_tokens - 1) / p.tile_tokens + (tokens < batch ? tokens : batch) + 1 : tokens;
+  const int64_t items = p.tiles * kv_heads;
+  int64_t keys = window && window + p.tile_tokens < max_keys ? window + p.tile_tokens : max_keys;
+  int64_t splits = 2 * (int64_t)sms / items, most = (keys / kTile + 2) / 2;
+  if (splits > most) splits = most;
+  p.splits = (int)(splits < 1 ? 1 : splits);
+  if (p.splits > 1)
+    p.workspace = (size_t)(items * p.splits) * kTile * (size_t)(D + 2) * sizeof(float) + (size_t)items * sizeof(Tile);
+  return p;
+}
+
+bool launch_paged_prefill(const AttentionArgs& a, const PrefillPlan& plan, int dtype, int D, int64_t page_size,
+                          cudaStream_t stream, cudaError_t* err) {
+  PrefillArgs p{};
+  p.a = a;
+  p.tile_tokens = plan.tile_tokens;
+  p.splits = plan.splits;
+  p.tiles = plan.tiles;
+  p.box_rows = page_size < kTile ? (int)page_size : kTile;
+  const int64_t items = plan.tiles * a.kv_heads;
+  if (items * p.splits * (kTile / 16) >= (int64_t(1) << 31)) return false;
+  CUtensorMap k_map, v_map;
+  if (!encode_cache(&k_map, a.k, dtype, D, page_size, a.kv_heads, a.pages.num_pages, a.k_slot, a.k_head, a.k_page,
+                    p.box_rows) ||
+      !encode_cache(&v_map, a.v, dtype, D, page_size, a.kv_heads, a.pages.num_pages, a.v_slot, a.v_head, a.v_page,
+                    p.box_rows))
+    return false;
+  if (p.splits > 1) {
+    p.part_out = static_cast<float*>(a.workspace);
+    p.part_stat = p.part_out + items * p.splits * kTile * D;
+    p.joins = reinterpret_cast<Tile*>(p.part_stat + items * p.splits * kTile * 2);
+  }
+  if (D == 64)
+    *err = dtype == 0 ? launch<__nv_bfloat16, 64>(k_map, v_map, p, items, stream)
+                      : launch<__half, 64>(k_map, v_map, p, items, stream);
+  else
+    *err = dtype == 0 ? launch<__nv_bfloat16, 128>(k_map, v_map, p, items, stream)
+                      : launch<__half, 128>(k_map, v_map, p, items, stream);
+  return true;
+}
+
+cudaError_t read_paged_prefill_device_error(int* value, bool reset) {
+  cudaError_t err = cudaMemcpyFromSymbol(value, g_device_error, sizeof(int));
+  if (err != cudaSuccess || !reset) return err;
+  const int zero = 0;
+  return cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int));
+}
+
+}  // namespace flash_prologue

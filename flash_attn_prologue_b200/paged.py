@@ -124,13 +124,17 @@ ATTENTION_HEAD_DIMS = (64, 128)
 _WORKSPACE_BYTES = {}
 
 
-def _workspace_bytes(heads, kv_heads, dim):
-    key = (heads, kv_heads, dim, torch.cuda.current_device())
+def _workspace_bytes(key, args):
+    """Workspace of a call: a function of its sizes and the device (``key``), asked for once."""
+    key = (*key, torch.cuda.current_device())
     nbytes = _WORKSPACE_BYTES.get(key)
     if nbytes is None:
         out = ctypes.c_size_t(0)
-        _lib.check(_lib.load().flash_prologue_paged_attention_workspace_size(heads, kv_heads, dim, ctypes.byref(out)),
+        _lib.check(_lib.load().flash_prologue_paged_attention_workspace_size(_lib.ATTENTION_ARGS.pack(*args),
+                                                                             ctypes.byref(out)),
                    "flash_prologue_paged_attention_workspace_size")
+        if len(_WORKSPACE_BYTES) >= 4096:  # many distinct sizes: start over
+            _WORKSPACE_BYTES.clear()
         nbytes = _WORKSPACE_BYTES[key] = int(out.value)
     return nbytes
 
@@ -164,11 +168,13 @@ def _attention(q, k_cache, v_cache, page_table, seq_lens, cu_seqlens, softmax_sc
     lse = torch.empty(q.shape[:2] if want_lse else (0,), dtype=torch.float32, device=q.device)
     if tokens:
         with _DeviceGuard(q.device):
-            workspace = torch.empty(_workspace_bytes(heads, kv_heads, dim), dtype=torch.uint8, device=q.device)
-            args = _lib.ATTENTION_ARGS.pack(
-                *rows_of(q), *rows_of(out), lse.data_ptr() if want_lse else 0,
-                *_cache_of(k_cache, v_cache, page_table, seq_lens, cu_seqlens), workspace.data_ptr(),
-                workspace.numel(), tokens, heads, kv_heads, dim, _lib.DTYPE_CODES[q.dtype], window, softmax_scale)
+            head = (*rows_of(q), *rows_of(out), lse.data_ptr() if want_lse else 0,
+                    *_cache_of(k_cache, v_cache, page_table, seq_lens, cu_seqlens))
+            sizes = (tokens, heads, kv_heads, dim, _lib.DTYPE_CODES[q.dtype], window, softmax_scale)
+            nbytes = _workspace_bytes((*sizes, cu_seqlens is None, k_cache.shape[1], page_table.shape),
+                                      (*head, 0, 0, *sizes))
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+            args = _lib.ATTENTION_ARGS.pack(*head, workspace.data_ptr(), nbytes, *sizes)
             _lib.check(_lib.load().flash_prologue_paged_attention(args, _lib.stream_of(q.device)),
                        "flash_prologue_paged_attention")
     return out, lse

@@ -565,8 +565,10 @@ typedef struct flash_prologue_attention_args {
  * flash_prologue_paged_attention_workspace_size() bytes, no initialisation.
  */
 FLASH_PROLOGUE_API int flash_prologue_paged_attention(const flash_prologue_attention_args* args, void* stream);
-/* Bytes of workspace for these heads on the current device, whatever the lengths. */
-FLASH_PROLOGUE_API int flash_prologue_paged_attention_workspace_size(int64_t Hq, int64_t Hk, int64_t D, size_t* bytes);
+/* Bytes of workspace a call with these sizes needs on the current device, whatever the lengths
+ * (pointers other than cu_seqlens' presence do not matter, but are checked). */
+FLASH_PROLOGUE_API int flash_prologue_paged_attention_workspace_size(const flash_prologue_attention_args* args,
+                       size_t* bytes);
 
 #ifdef __cplusplus
 }  /* extern "C" */
