@@ -22,6 +22,11 @@ struct AttentionArgs {
   int64_t max_keys;          // pages.max_pages * page_size
 };
 
+// Lets the next kernel of the stream be placed (see launch_following), and
+// waits until the one before has ended and its writes can be read.
+__device__ __forceinline__ void start_next_kernel() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // One request as the kernels see it: its new tokens and the keys it may reach.
 struct Request {
   int64_t first;   // packed index of its first new token

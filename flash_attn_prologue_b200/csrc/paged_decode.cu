@@ -135,6 +135,7 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
   const int batch = a.pages.batch + (a.pages.cu_seqlens ? 1 : 0);
   const uint32_t ring = smem_u32(smem) + warp * kRing * kStepBytes;
 
+  start_next_kernel();
   // This CTA's run of units.
   int64_t mine = 0;
   bool bad = false;
@@ -159,8 +160,8 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
   int64_t before = 0;
   for (int r0 = 0; r0 < batch; r0 += kDecodeThreads) {
     const int r = r0 + threadIdx.x;
-    int64_t n = 0;
-    if (r < batch) {
+    int64_t n = batch <= kDecodeThreads ? mine : 0;  // one request a thread: counted already
+    if (batch > kDecodeThreads && r < batch) {
       bool b;
       const Request q = request_at(a.pages, a.tokens, a.max_keys, r, &b);
       if (q.news) n = units_of(q, a);
@@ -462,33 +463,57 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
   }
 }
 
-// Joins the parts of the item that CTA blockIdx.x of the first kernel began.
+// Joins the parts of the item that CTA blockIdx.x of the first kernel began: a
+// row a warp, its columns over the lanes, the parts' loads in flight together.
+constexpr int kJoinWarps = 4;
 template <typename T, int D>
-__global__ void __launch_bounds__(kDecodeThreads) paged_join_kernel(const AttentionArgs a, int64_t ctas) {
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const AttentionArgs a, int64_t ctas) {
+  constexpr int kCols = D / 32;  // columns of a lane
   const float* part_out = static_cast<const float*>(a.workspace);
   const float* part_stat = part_out + 2 * ctas * kRows * D;
+  wait_for_previous_kernel();
   const Part p = reinterpret_cast<const Part*>(part_stat + 2 * ctas * kRows * 2)[blockIdx.x];
-  if (p.last < 0) return;
-  for (int i = threadIdx.x; i < p.rows * D; i += kDecodeThreads) {
-    const int row = i / D, col = i % D;
-    float m = -INFINITY;
-    for (int64_t c = blockIdx.x; c <= p.last; ++c) {
-      const int64_t slot = 2 * c + (c == blockIdx.x ? 1 : 0);
-      m = fmaxf(m, part_stat[(slot * kRows + row) * 2]);
+  const int row = blockIdx.y * kJoinWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (p.last < 0 || row >= p.rows) return;
+  const int first = blockIdx.x, parts = p.last - first + 1;
+  // Part i is in the second slot of the CTA that began the item, in the first slot of the others.
+  const auto stat_of = [&](int i) {
+    const int64_t slot = 2 * (int64_t)(first + i) + (i == 0);
+    return __ldcg(reinterpret_cast<const float2*>(part_stat + (slot * kRows + row) * 2));
+  };
+  float m = -INFINITY;
+  for (int i = lane; i < parts; i += 32) m = fmaxf(m, stat_of(i).x);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float from = m == -INFINITY ? 0.f : m;
+  float o[kCols] = {}, l = 0.f;
+#pragma unroll 8
+  for (int i = 0; i < parts; ++i) {
+    const float2 st = stat_of(i);
+    const int64_t slot = 2 * (int64_t)(first + i) + (i == 0);
+    const float* src = part_out + (slot * kRows + row) * D + lane * kCols;
+    float x[kCols];
+    if constexpr (kCols == 4) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
+      x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else {
+      const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
+      x[0] = v.x; x[1] = v.y;
     }
-    const float from = m == -INFINITY ? 0.f : m;
-    float o = 0.f, l = 0.f;
-    for (int64_t c = blockIdx.x; c <= p.last; ++c) {
-      const int64_t slot = 2 * c + (c == blockIdx.x ? 1 : 0);
-      const float f = exp2_approx(part_stat[(slot * kRows + row) * 2] - from);
-      o += f * part_out[(slot * kRows + row) * D + col];
-      l += f * part_stat[(slot * kRows + row) * 2 + 1];
-    }
-    const int64_t at = p.row0 + row, token = at / a.group;
-    const int h = p.kv_head * a.group + (int)(at - token * a.group);
-    static_cast<T*>(a.out)[(p.token0 + token) * a.out_n + h * a.out_h + col] = from_float<T>(l == 0.f ? 0.f : o / l);
-    if (a.lse && col == 0) a.lse[(p.token0 + token) * a.heads + h] = (m + log2f(l)) * 0.6931471805599453f;
+    const float f = exp2_approx(st.x - from);
+    l += f * st.y;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) o[c] += f * x[c];
   }
+  const int64_t at = p.row0 + row, token = at / a.group;
+  const int h = p.kv_head * a.group + (int)(at - token * a.group);
+  uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + (p.token0 + token) * a.out_n + h * a.out_h) +
+                  lane * (kCols / 2);
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) o[c] = l == 0.f ? 0.f : o[c] / l;
+#pragma unroll
+  for (int c = 0; c < kCols / 2; ++c) out[c] = pack2<T>(o[2 * c], o[2 * c + 1]);
+  if (a.lse && lane == 0) a.lse[(p.token0 + token) * a.heads + h] = (m + log2f(l)) * 0.6931471805599453f;
 }
 
 int64_t most_ctas(int D, int sms) { return (int64_t)sms * (D == 64 ? 4 : 2); }
@@ -511,7 +536,8 @@ cudaError_t launch(const AttentionArgs& a, cudaStream_t stream) {
   if (grid <= 0) return cudaErrorInvalidConfiguration;
   err = launch_kernel(paged_decode_kernel<T, D>, dim3((unsigned)grid), dim3(kDecodeThreads), smem, stream, a);
   if (err != cudaSuccess) return err;
-  return launch_kernel(paged_join_kernel<T, D>, dim3((unsigned)grid), dim3(kDecodeThreads), 0, stream, a, grid);
+  return launch_following(paged_join_kernel<T, D>, dim3((unsigned)grid, kRows / kJoinWarps), dim3(kJoinWarps * 32), stream,
+                          a, grid);
 }
 
 }  // namespace

@@ -170,6 +170,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
   unsigned char* v_s = k_s + L::kStages * L::kOperand;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  if (p.splits > 1) start_next_kernel();
   // ---- this CTA's tile: last tiles first (they have the most keys), splits innermost
   const int64_t item = (int64_t)blockIdx.x / p.splits;
   const int split = (int)(blockIdx.x - item * p.splits);
@@ -608,6 +609,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(512) prefill_join_kernel(const PrefillArgs p) {
   const AttentionArgs& a = p.a;
   const int64_t item = blockIdx.x / (kTile / 16);
+  wait_for_previous_kernel();
   const Tile t = p.joins[item];
   const int row = (int)(blockIdx.x % (kTile / 16)) * 16 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (t.parts <= 1 || row >= t.rows) return;
@@ -616,6 +618,7 @@ __global__ void __launch_bounds__(512) prefill_join_kernel(const PrefillArgs p) 
   for (int s = 0; s < t.parts; ++s) m = fmaxf(m, p.part_stat[((slot0 + s) * kTile + row) * 2]);
   const float from = m == -INFINITY ? 0.f : m;
   float o[D / 32] = {}, l = 0.f;
+#pragma unroll 4
   for (int s = 0; s < t.parts; ++s) {
     const int64_t at = (slot0 + s) * kTile + row;
     const float f = exp2_approx(p.part_stat[at * 2] - from);
@@ -663,7 +666,7 @@ cudaError_t launch(const CUtensorMap& k_map, const CUtensorMap& v_map, const Pre
   err = launch_kernel(paged_prefill_kernel<T, D>, dim3((unsigned)(items * p.splits)), dim3(kPrefillThreads),
                       Layout<D>::kSmem, stream, k_map, v_map, p);
   if (err != cudaSuccess || p.splits == 1) return err;
-  return launch_kernel(prefill_join_kernel<T, D>, dim3((unsigned)(items * (kTile / 16))), dim3(512), 0, stream, p);
+  return launch_following(prefill_join_kernel<T, D>, dim3((unsigned)(items * (kTile / 16))), dim3(512), stream, p);
 }
 
 }  // namespace

@@ -33,6 +33,30 @@ inline cudaError_t launch_kernel(void (*fn)(P...), dim3 grid, dim3 block, size_t
       vals);
 }
 
+// As launch_kernel, for a kernel that follows one which calls start_next_kernel()
+// and begins itself with wait_for_previous_kernel(): its blocks may be placed
+// while the one before still runs, which hides the launch.
+template <typename... P, typename... A>
+inline cudaError_t launch_following(void (*fn)(P...), dim3 grid, dim3 block, cudaStream_t stream, A&&... args) {
+  static_assert(sizeof...(P) == sizeof...(A), "kernel argument count");
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = block;
+  config.stream = stream;
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  std::tuple<std::decay_t<P>...> vals(std::forward<A>(args)...);
+  return std::apply(
+      [&](auto&... v) {
+        void* ptrs[] = {static_cast<void*>(&v)..., nullptr};
+        return cudaLaunchKernelExC(&config, reinterpret_cast<const void*>(fn), ptrs);
+      },
+      vals);
+}
+
 // Index 0 = Q, 1 = K in every two-element array below.
 struct FwdArgs {
   const void* x[2];   // inputs
