@@ -95,7 +95,8 @@ GqaTables tables_of(const flash_prologue_gqa_args* a) {
 int check_cache(const flash_prologue_cache& c, int64_t tokens, int64_t dtype) {
   if (c.batch < 0 || c.num_pages < 0 || c.max_pages < 0 || c.page_size < 8 || (c.page_size & (c.page_size - 1)))
     return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
-  if (c.batch >= (1 << 24) || c.page_size > (1 << 20) || c.num_pages >= (int64_t(1) << 31))
+  if (c.batch >= (1 << 24) || c.page_size > (1 << 20) || c.num_pages >= (int64_t(1) << 31) ||
+      c.max_pages >= (int64_t(1) << 30) / c.page_size)
     return FLASH_PROLOGUE_ERR_UNSUPPORTED;
   if (!c.cu_seqlens && tokens != c.batch) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
   if (tokens == 0) return FLASH_PROLOGUE_OK;

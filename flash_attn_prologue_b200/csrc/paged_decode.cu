@@ -27,6 +27,7 @@ constexpr int kWarpKeys = 16;   // keys of a warp's step
 constexpr int kDecodeWarps = 4;
 constexpr int kDecodeThreads = kDecodeWarps * 32;
 constexpr int kBlockKeys = kWarpKeys * kDecodeWarps;
+constexpr int kNone = -(1 << 30);  // below every relative position
 constexpr int kRing = 3;        // steps of a warp's ring
 
 struct Part {  // an item that a CTA began and others go on with
@@ -240,22 +241,36 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
     if (threadIdx.x == 0) bad_page = too_long;
     __syncthreads();
 
+    // Positions relative to this warp's first key, in 32 bits (a request has fewer than 2^30 keys).
     const int steps = (int)(b1 - b0);
     const int64_t warp_key = key0 + b0 * kBlockKeys + warp * kWarpKeys;
+    const int key_lo = (int)(lo - warp_key), key_hi = (int)(hi - warp_key);
+    const int all_lo = a.window ? (int)(base + (row0 + rows - 1) / a.group - a.window + 1 - warp_key) : kNone;
+    const int all_hi = (int)(base + row0 / a.group - warp_key);  // every row sees keys all_lo .. all_hi
+    int see_lo[2], see_hi[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      see_hi[e] = row_pos[e] < 0 ? kNone : (int)(row_pos[e] - warp_key);
+      see_lo[e] = a.window ? (int)(row_pos[e] - a.window + 1 - warp_key) : kNone;
+    }
     const int32_t* table = a.pages.page_table + (int64_t)r * a.pages.table_stride;
-    int64_t page_of[2] = {0, 0};  // pages of the 16 keys of step page_step + lane (two where pages hold 8)
+    const int in_page = (1 << a.pages.page_log2) - 1;
+    // A lane's pieces of a step: rows lane / kPieces + i * kRowStep, 16 bytes at column lane % kPieces.
+    constexpr int kPieces = D / 8, kRowStep = 32 / kPieces;
+    const int64_t k_lane = head * a.k_head + lane / kPieces * a.k_slot + lane % kPieces * 8;
+    const int64_t v_lane = head * a.v_head + lane / kPieces * a.v_slot + lane % kPieces * 8;
+    int page_of[2] = {0, 0};  // pages of the 16 keys of step page_step + lane (two where pages hold 8)
     int page_step = -32;
     auto load = [&](int step) {
       if (step < steps) {
         if (step - page_step >= 32) {
           page_step = step;
-          const int64_t key = warp_key + (int64_t)(step + lane) * kBlockKeys;
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
-            const int64_t k = key + s * 8;
+            const int k = (step + lane) * kBlockKeys + s * 8;
             page_of[s] = 0;
-            if (step + lane < steps && k < hi && k + 8 > lo) {
-              page_of[s] = __ldg(table + (k >> a.pages.page_log2));
+            if (step + lane < steps && k < key_hi && k + 8 > key_lo) {
+              page_of[s] = __ldg(table + ((warp_key + k) >> a.pages.page_log2));
               if (page_of[s] < 0 || page_of[s] >= a.pages.num_pages) {
                 page_of[s] = -1;
                 bad_page = 1;
@@ -263,27 +278,32 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
             }
           }
         }
-        const int64_t page_lo = __shfl_sync(0xffffffffu, page_of[0], step - page_step);
-        const int64_t page_hi = __shfl_sync(0xffffffffu, page_of[1], step - page_step);
-        const int64_t key = warp_key + (int64_t)step * kBlockKeys;
+        const int page[2] = {__shfl_sync(0xffffffffu, page_of[0], step - page_step),
+                             __shfl_sync(0xffffffffu, page_of[1], step - page_step)};
+        const int key = step * kBlockKeys;
         const uint32_t dst = ring + (step % kRing) * kStepBytes;
+        const bool full = key >= key_lo && key + kWarpKeys <= key_hi && page[0] >= 0 && page[1] >= 0;
 #pragma unroll
-        for (int i = 0; i < kPerLane; ++i) {
-          const int piece = i * 32 + lane;
-          const int row = piece / (D / 8), c = piece % (D / 8);
-          const int64_t k = key + row;
-          const int64_t page = row < 8 ? page_lo : page_hi;
-          const int64_t slot = k & ((1 << a.pages.page_log2) - 1);
-          const bool ok = k >= lo && k < hi && page >= 0;
+        for (int s = 0; s < 2; ++s) {
+          const int64_t slot = (int)(warp_key + key + s * 8) & in_page;
           const T* kp = static_cast<const T*>(a.k);
           const T* vp = static_cast<const T*>(a.v);
-          if (ok) {
-            kp += page * a.k_page + slot * a.k_slot + head * a.k_head + c * 8;
-            vp += page * a.v_page + slot * a.v_slot + head * a.v_head + c * 8;
+          if (page[s] >= 0) {
+            kp += page[s] * a.k_page + slot * a.k_slot + k_lane;
+            vp += page[s] * a.v_page + slot * a.v_slot + v_lane;
           }
-          const uint32_t at = dst + row * kRowBytes + ((c ^ (row & 7)) * 16);
-          cp_async16(at, kp, ok);
-          cp_async16(at + kWarpKeys * kRowBytes, vp, ok);
+#pragma unroll
+          for (int i = 0; i < kPerLane / 2; ++i) {
+            const int row = s * 8 + i * kRowStep + lane / kPieces;
+            const uint32_t at = dst + row * kRowBytes + ((lane % kPieces) ^ (row & 7)) * 16;
+            const bool ok = full || (key + row >= key_lo && key + row < key_hi && page[s] >= 0);
+            cp_async16(at, kp, ok);
+            cp_async16(at + kWarpKeys * kRowBytes, vp, ok);
+            if (page[s] >= 0) {
+              kp += kRowStep * a.k_slot;
+              vp += kRowStep * a.v_slot;
+            }
+          }
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -295,8 +315,8 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
       asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
       __syncwarp();
       load(step + kRing - 1);
-      const int64_t key = warp_key + (int64_t)step * kBlockKeys;
-      if (key >= hi || key + kWarpKeys <= lo) continue;
+      const int key = step * kBlockKeys;
+      if (key >= key_hi || key + kWarpKeys <= key_lo) continue;
       const uint32_t ks = ring + (step % kRing) * kStepBytes, vs = ks + kWarpKeys * kRowBytes;
       float s[2][4] = {};
 #pragma unroll
@@ -309,7 +329,7 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
         mma16816<T>(s[1], qf[c], b[2], b[3]);
       }
       // Row e of this lane: scores s[n][2 e + x] of keys n * 8 + (lane % 4) * 2 + x.
-      bool hidden = false;
+      const bool edge = key < all_lo || key + kWarpKeys - 1 > all_hi;  // some row does not see some key
       float p[2][4];
       float scale[2];
 #pragma unroll
@@ -318,28 +338,27 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const int64_t k = key + n * 8 + (lane % 4) * 2 + x;
-            const bool sees = k <= row_pos[e] && (!a.window || k > row_pos[e] - a.window);
-            const float t = sees ? s[n][2 * e + x] * a.scale_log2 : -INFINITY;
-            hidden |= !sees && k >= lo && k < hi && row_pos[e] >= 0;
-            p[n][2 * e + x] = t;
-            most = fmaxf(most, t);
-          }
+          for (int x = 0; x < 2; ++x) p[n][2 * e + x] = s[n][2 * e + x] * a.scale_log2;
+        if (edge) {
+          const int lo_e = see_lo[e] - key - (lane % 4) * 2, hi_e = see_hi[e] - key - (lane % 4) * 2;
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              if (n * 8 + x > hi_e || n * 8 + x < lo_e) p[n][2 * e + x] = -INFINITY;
+        }
+        most = fmaxf(fmaxf(p[0][2 * e], p[0][2 * e + 1]), fmaxf(p[1][2 * e], p[1][2 * e + 1]));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
         const float now = fmaxf(top[e], most);
         const float from = now == -INFINITY ? 0.f : now;
         scale[e] = exp2_approx(top[e] - from);
         top[e] = now;
-        sum[e] *= scale[e];
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            p[n][2 * e + x] = exp2_approx(p[n][2 * e + x] - from);
-            sum[e] += p[n][2 * e + x];
-          }
+          for (int x = 0; x < 2; ++x) p[n][2 * e + x] = exp2_approx(p[n][2 * e + x] - from);
+        sum[e] = sum[e] * scale[e] + ((p[0][2 * e] + p[0][2 * e + 1]) + (p[1][2 * e] + p[1][2 * e + 1]));
       }
       if (__any_sync(0xffffffffu, scale[0] != 1.f || scale[1] != 1.f)) {
 #pragma unroll
@@ -350,16 +369,15 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
           acc[t][3] *= scale[1];
         }
       }
-      // Where a row of the tile does not see a key that others see, an infinity or NaN in
+      // Where a row of the tile does not see a key that others may, an infinity or NaN in
       // that key's V must not reach it through 0 * V: such values are taken out of the
       // product and added to the rows that see them.
-      if (__any_sync(0xffffffffu, hidden)) {
+      if (edge) {
         uint32_t* v32 = reinterpret_cast<uint32_t*>(smem + (vs - smem_u32(smem)));
         bool wild = false;
         for (int i = lane; i < kWarpKeys * D / 2; i += 32) wild |= non_finite<T>(v32[i]);
         if (__any_sync(0xffffffffu, wild)) {
           for (int j = 0; j < kWarpKeys; ++j) {
-            const int64_t k = key + j;
             const T* vrow = reinterpret_cast<const T*>(smem + (vs - smem_u32(smem)) + j * kRowBytes);
 #pragma unroll
             for (int t = 0; t < kTiles; ++t)
@@ -369,7 +387,7 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
                 if (isfinite(val)) continue;
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
-                  if (k <= row_pos[e] && (!a.window || k > row_pos[e] - a.window)) acc[t][2 * e + x] += val;
+                  if (key + j <= see_hi[e] && key + j >= see_lo[e]) acc[t][2 * e + x] += val;
               }
           }
           __syncwarp();
