@@ -481,57 +481,85 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
   }
 }
 
-// Joins the parts of the item that CTA blockIdx.x of the first kernel began: a
-// row a warp, its columns over the lanes, the parts' loads in flight together.
-constexpr int kJoinWarps = 4;
+// Joins the parts of one row of the item that CTA blockIdx.x of the first kernel
+// began: every warp takes each eighth part, its columns over the lanes.
+constexpr int kJoinWarps = 8;
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const AttentionArgs a, int64_t ctas) {
   constexpr int kCols = D / 32;  // columns of a lane
+  __shared__ float joined[kJoinWarps][D], sums[kJoinWarps], tops[kJoinWarps];
   const float* part_out = static_cast<const float*>(a.workspace);
   const float* part_stat = part_out + 2 * ctas * kRows * D;
   wait_for_previous_kernel();
   const Part p = reinterpret_cast<const Part*>(part_stat + 2 * ctas * kRows * 2)[blockIdx.x];
-  const int row = blockIdx.y * kJoinWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (p.last < 0 || row >= p.rows) return;
   const int first = blockIdx.x, parts = p.last - first + 1;
-  // Part i is in the second slot of the CTA that began the item, in the first slot of the others.
-  const auto stat_of = [&](int i) {
-    const int64_t slot = 2 * (int64_t)(first + i) + (i == 0);
-    return __ldcg(reinterpret_cast<const float2*>(part_stat + (slot * kRows + row) * 2));
-  };
-  float m = -INFINITY;
-  for (int i = lane; i < parts; i += 32) m = fmaxf(m, stat_of(i).x);
+  float top = -INFINITY, sum = 0.f, o[kCols] = {};
+  constexpr int kFlight = 4;
+  for (int i0 = warp; i0 < parts; i0 += kJoinWarps * kFlight) {
+    float2 st[kFlight];
+    float x[kFlight][kCols];
 #pragma unroll
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float from = m == -INFINITY ? 0.f : m;
-  float o[kCols] = {}, l = 0.f;
-#pragma unroll 8
-  for (int i = 0; i < parts; ++i) {
-    const float2 st = stat_of(i);
-    const int64_t slot = 2 * (int64_t)(first + i) + (i == 0);
-    const float* src = part_out + (slot * kRows + row) * D + lane * kCols;
-    float x[kCols];
-    if constexpr (kCols == 4) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
-      x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-    } else {
-      const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
-      x[0] = v.x; x[1] = v.y;
+    for (int f = 0; f < kFlight; ++f) {
+      const int i = i0 + f * kJoinWarps;
+      st[f] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) x[f][c] = 0.f;
+      if (i < parts) {
+        // Part i is in the second slot of the CTA that began the item, in the first slot of the others.
+        const int64_t at = (2 * (int64_t)(first + i) + (i == 0)) * kRows + row;
+        st[f] = __ldcg(reinterpret_cast<const float2*>(part_stat + at * 2));
+        const float* src = part_out + at * D + lane * kCols;
+        if constexpr (kCols == 4) {
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
+          x[f][0] = v.x; x[f][1] = v.y; x[f][2] = v.z; x[f][3] = v.w;
+        } else {
+          const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
+          x[f][0] = v.x; x[f][1] = v.y;
+        }
+      }
     }
-    const float f = exp2_approx(st.x - from);
-    l += f * st.y;
+    float now = top;
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) o[c] += f * x[c];
+    for (int f = 0; f < kFlight; ++f) now = fmaxf(now, st[f].x);
+    const float from = now == -INFINITY ? 0.f : now, moved = exp2_approx(top - from);
+    top = now;
+    sum *= moved;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) o[c] *= moved;
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) {
+      const float e = exp2_approx(st[f].x - from);
+      sum += e * st[f].y;
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) o[c] += e * x[f][c];
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < kCols; ++c) joined[warp][lane * kCols + c] = o[c];
+  if (lane == 0) {
+    sums[warp] = sum;
+    tops[warp] = top;
+  }
+  __syncthreads();
+  const int col = threadIdx.x;
+  if (col >= D) return;
+  float m = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) m = fmaxf(m, tops[w]);
+  const float from = m == -INFINITY ? 0.f : m;
+  float v = 0.f, l = 0.f;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) {
+    const float e = exp2_approx(tops[w] - from);
+    v += e * joined[w][col];
+    l += e * sums[w];
   }
   const int64_t at = p.row0 + row, token = at / a.group;
   const int h = p.kv_head * a.group + (int)(at - token * a.group);
-  uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + (p.token0 + token) * a.out_n + h * a.out_h) +
-                  lane * (kCols / 2);
-#pragma unroll
-  for (int c = 0; c < kCols; ++c) o[c] = l == 0.f ? 0.f : o[c] / l;
-#pragma unroll
-  for (int c = 0; c < kCols / 2; ++c) out[c] = pack2<T>(o[2 * c], o[2 * c + 1]);
-  if (a.lse && lane == 0) a.lse[(p.token0 + token) * a.heads + h] = (m + log2f(l)) * 0.6931471805599453f;
+  static_cast<T*>(a.out)[(p.token0 + token) * a.out_n + h * a.out_h + col] = from_float<T>(l == 0.f ? 0.f : v / l);
+  if (a.lse && col == 0) a.lse[(p.token0 + token) * a.heads + h] = (m + log2f(l)) * 0.6931471805599453f;
 }
 
 int64_t most_ctas(int D, int sms) { return (int64_t)sms * (D == 64 ? 4 : 2); }
@@ -554,8 +582,8 @@ cudaError_t launch(const AttentionArgs& a, cudaStream_t stream) {
   if (grid <= 0) return cudaErrorInvalidConfiguration;
   err = launch_kernel(paged_decode_kernel<T, D>, dim3((unsigned)grid), dim3(kDecodeThreads), smem, stream, a);
   if (err != cudaSuccess) return err;
-  return launch_following(paged_join_kernel<T, D>, dim3((unsigned)grid, kRows / kJoinWarps), dim3(kJoinWarps * 32), stream,
-                          a, grid);
+  const unsigned rows = a.pages.cu_seqlens || a.group > kRows ? kRows : a.group;  // rows a tile can have
+  return launch_following(paged_join_kernel<T, D>, dim3((unsigned)grid, rows), dim3(kJoinWarps * 32), stream, a, grid);
 }
 
 }  // namespace
