@@ -93,6 +93,20 @@ TmaPlan plan_tma(int64_t B, int64_t H, int64_t N, int D, int dtype, bool heads_i
   return p;
 }
 
+cudaError_t allow_shared_memory(const void* kernel, size_t bytes) {
+  static std::mutex mu;
+  static std::unordered_map<const void*, std::unordered_map<int, size_t>> allowed;
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  std::lock_guard<std::mutex> lock(mu);
+  size_t& most = allowed[kernel][dev];
+  if (bytes <= most) return cudaSuccess;
+  err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (err == cudaSuccess) most = bytes;
+  return err;
+}
+
 int64_t persistent_grid(const void* kernel, size_t smem_bytes, int64_t n_items, int threads) {
   struct Key {
     const void* fn;

@@ -244,9 +244,7 @@ const void* ready_kernel(int Hq, int D, int dtype, bool vec, size_t* smem) {
   const void* fn = bwd_kernel_for(dtype, D, vec);
   if (!fn) return nullptr;
   *smem = smem_bytes(Hq, D, dtype, vec);
-  if (*smem > 48 * 1024 &&
-      cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)*smem) != cudaSuccess)
-    return nullptr;
+  if (*smem > 48 * 1024 && allow_shared_memory(fn, *smem) != cudaSuccess) return nullptr;
   return fn;
 }
 

@@ -568,7 +568,7 @@ template <typename T, int D>
 cudaError_t launch(const AttentionArgs& a, cudaStream_t stream) {
   constexpr size_t smem = (size_t)kDecodeWarps * kRing * 2 * kWarpKeys * D * 2;
   const void* fn = reinterpret_cast<const void*>(&paged_decode_kernel<T, D>);
-  cudaError_t err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t err = allow_shared_memory(fn, smem);
   if (err != cudaSuccess) return err;
   // Never more CTAs than there can be units.
   const int64_t tiles = a.tokens * a.group / kRows + (a.tokens < a.pages.batch ? a.tokens : a.pages.batch) + 1;

@@ -661,7 +661,7 @@ cudaError_t launch(const CUtensorMap& k_map, const CUtensorMap& v_map, const Pre
     return cudaFuncGetAttributes(&attr, fn) == cudaSuccess ? attr.numRegs : 0;
   }();
   if (regs < kLaunchRegs) return cudaErrorInvalidConfiguration;
-  cudaError_t err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Layout<D>::kSmem);
+  cudaError_t err = allow_shared_memory(fn, Layout<D>::kSmem);
   if (err != cudaSuccess) return err;
   err = launch_kernel(paged_prefill_kernel<T, D>, dim3((unsigned)(items * p.splits)), dim3(kPrefillThreads),
                       Layout<D>::kSmem, stream, k_map, v_map, p);

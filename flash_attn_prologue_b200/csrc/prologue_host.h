@@ -214,6 +214,9 @@ Geometry plan_geometry(int64_t B, int64_t H, int64_t N, int D, bool heads_inner)
 int64_t persistent_grid(const void* kernel, size_t smem_bytes, int64_t n_items,
                         int threads = kThreads);
 
+// Lets `kernel` have `bytes` of dynamic shared memory on the current device (asked for once).
+cudaError_t allow_shared_memory(const void* kernel, size_t bytes);
+
 // Fixed-order sum of the [G, C] per-CTA partials into dw [two_d] and ds [C - two_d].
 cudaError_t launch_bwd_finalize(const float* partials, int64_t G, int C, int two_d, float* dw,
                                 float* ds, cudaStream_t stream);

@@ -16,7 +16,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .fused_epilogue import _DeviceGuard, _get_compact_strides, _grad_view
+from .fused_epilogue import _DeviceGuard, _grad_view
 from .functional import SUPPORTED_CUTE_HEAD_DIMS, _plain_eager
 
 MAX_HEADS = 512
@@ -28,35 +28,39 @@ def check_rows(q, k, rmsnorm_weight, scales, sin, cos, eps):
     q and k are packed [T, H, D] or dense [B, H, N, D] and agree in everything
     but the head count; rmsnorm_weight and scales may be None where the caller
     allows it."""
-    if q.ndim not in (3, 4) or k.ndim != q.ndim:
+    qs, ks, dtype = q.shape, k.shape, q.dtype
+    if len(qs) not in (3, 4) or len(ks) != len(qs):
         raise ValueError("q/k must both be packed [T,H,D] or dense [B,H,N,D]")
-    heads = 1
-    hq, hk, d = q.shape[heads], k.shape[heads], q.shape[-1]
-    if any(a != b for i, (a, b) in enumerate(zip(q.shape, k.shape)) if i != heads):
+    hq, hk, d = qs[1], ks[1], qs[-1]
+    if qs[0] != ks[0] or qs[2:] != ks[2:]:
         raise ValueError("q/k may differ in their head count only")
-    if q.dtype not in _lib.DTYPE_CODES or k.dtype != q.dtype:
+    if dtype not in _lib.DTYPE_CODES or k.dtype != dtype:
         raise ValueError("q/k must share BF16, FP16, or FP32 dtype")
     if d not in SUPPORTED_CUTE_HEAD_DIMS:
         raise ValueError(f"head dimension must be one of {SUPPORTED_CUTE_HEAD_DIMS}")
     if hk <= 0 or hq <= 0 or hq % hk or hq > MAX_HEADS:
         raise ValueError(f"query heads must be a multiple of the key heads and at most {MAX_HEADS}")
-    if not math.isfinite(eps) or eps <= 0:
+    if not 0 < eps < math.inf:
         raise ValueError("eps must be finite and positive")
-    if rmsnorm_weight is not None and rmsnorm_weight.shape != (2, 1, d):
-        raise ValueError("weight must be [2,1,D]")
-    if scales is not None and scales.shape != (hq, 1, 1):
-        raise ValueError("log-scales must be [Hq,1,1]")
+    device = q.device
+    shared = k.device == device and sin.device == device and cos.device == device
+    fp32 = sin.dtype == torch.float32 and cos.dtype == torch.float32
+    if rmsnorm_weight is not None:
+        if rmsnorm_weight.shape != (2, 1, d):
+            raise ValueError("weight must be [2,1,D]")
+        shared, fp32 = shared and rmsnorm_weight.device == device, fp32 and rmsnorm_weight.dtype == torch.float32
+    if scales is not None:
+        if scales.shape != (hq, 1, 1):
+            raise ValueError("log-scales must be [Hq,1,1]")
+        shared, fp32 = shared and scales.device == device, fp32 and scales.dtype == torch.float32
     if sin.ndim != 2 or sin.shape != cos.shape or sin.shape[1] != d // 2:
         raise ValueError("sin/cos must be matching tables [positions, D/2]")
-    for t in (rmsnorm_weight, scales, sin, cos):
-        if t is not None and t.dtype != torch.float32:
-            raise ValueError("weights, log-scales, and sin/cos must be FP32")
+    if not fp32:
+        raise ValueError("weights, log-scales, and sin/cos must be FP32")
     if sin.requires_grad or cos.requires_grad:
         raise ValueError("gradients of sin/cos are not implemented")
-    device = q.device
-    for t in (k, rmsnorm_weight, scales, sin, cos):
-        if t is not None and t.device != device:
-            raise ValueError("all tensors must share a device")
+    if not shared:
+        raise ValueError("all tensors must share a device")
     if device.type != "cuda":
         raise ValueError("the prologue kernels run on CUDA devices only")
 
@@ -77,7 +81,27 @@ def _check_positions(positions, q, sin):
 
 def eager(*tensors) -> bool:
     """An eager call on plain tensors, parameters or None (see _plain_eager)."""
-    return _plain_eager(*(t for t in tensors if t is not None and type(t) is not torch.nn.Parameter))
+    for t in tensors:
+        if t is not None and type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
+            return False
+    return _plain_eager()
+
+
+def on_device(t):
+    """A guard that makes t's device current, or None where it is already."""
+    return None if t.get_device() == torch._C._cuda_getDevice() else _DeviceGuard(t.device)
+
+
+def call_library(name, args, like):
+    """Calls entry point ``name`` on the current stream of ``like``'s device."""
+    guard = on_device(like)
+    if guard is None:
+        status = getattr(_lib.load(), name)(args, _lib.stream_of(like.device))
+    else:
+        with guard:
+            status = getattr(_lib.load(), name)(args, _lib.stream_of(like.device))
+    if status:
+        _lib.check(status, name)
 
 
 def readable(t):
@@ -114,15 +138,13 @@ def _call(name, q, k, w, s, sin, cos, positions, eps, rows, grads=(0, 0), worksp
     args = _lib.GQA_ARGS.pack(
         *rows_of(q), *rows_of(k), *rows, w.data_ptr(), s.data_ptr(), *rotation_of(sin, cos), *where, *grads,
         *workspace, *peers, B, N, q.shape[1], k.shape[1], q.shape[-1], _lib.DTYPE_CODES[q.dtype], eps)
-    _lib.check(getattr(_lib.load(), name)(args, _lib.stream_of(q.device)), name)
-
-
-def _empty_like_rows(t):
-    return torch.empty_strided(t.shape, _get_compact_strides(t.shape, t.stride()), dtype=t.dtype, device=t.device)
+    call_library(name, args, q)
 
 
 def _in_place_rows(t):
     """As ``readable``, with expanded (stride-0) activations made contiguous too."""
+    if t.is_contiguous():
+        return t
     if t.stride(-1) != 1 or any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
         return t.contiguous()
     return t
@@ -132,45 +154,46 @@ def gqa_forward(q, k, rmsnorm_weight, scales, sin, cos, positions, eps):
     check_rows(q, k, rmsnorm_weight, scales, sin, cos, eps)
     _check_positions(positions, q, sin)
     q, k = _in_place_rows(q), _in_place_rows(k)
-    q_out, k_out = _empty_like_rows(q), _empty_like_rows(k)
+    q_out, k_out = torch.empty_like(q), torch.empty_like(k)  # dense, in the inputs' memory order
     if q.numel():
-        w, s = flat_fp32(rmsnorm_weight), scales.contiguous()
-        with _DeviceGuard(q.device):
-            _call("flash_prologue_gqa_fwd", q, k, w, s, sin, cos, positions, eps,
-                  (*rows_of(q_out), *rows_of(k_out), *_lib.NO_ROWS, *_lib.NO_ROWS, *_lib.NO_ROWS, *_lib.NO_ROWS))
+        _call("flash_prologue_gqa_fwd", q, k, flat_fp32(rmsnorm_weight), scales.contiguous(), sin, cos, positions, eps,
+              (*rows_of(q_out), *rows_of(k_out), *_lib.NO_ROWS, *_lib.NO_ROWS, *_lib.NO_ROWS, *_lib.NO_ROWS))
     return q_out, k_out
 
 
 _WORKSPACE_BYTES = {}
 
 
-def _workspace_bytes(heads, dim):
-    key = (heads, dim, torch.cuda.current_device())
-    if key not in _WORKSPACE_BYTES:
+def _workspace_bytes(heads, dim, device):
+    nbytes = _WORKSPACE_BYTES.get((heads, dim, device))
+    if nbytes is None:
         out = ctypes.c_size_t(0)
-        _lib.check(_lib.load().flash_prologue_gqa_bwd_workspace_size(heads, dim, ctypes.byref(out)),
-                   "flash_prologue_gqa_bwd_workspace_size")
-        _WORKSPACE_BYTES[key] = int(out.value)
-    return _WORKSPACE_BYTES[key]
+        with _DeviceGuard(device):
+            _lib.check(_lib.load().flash_prologue_gqa_bwd_workspace_size(heads, dim, ctypes.byref(out)),
+                       "flash_prologue_gqa_bwd_workspace_size")
+        nbytes = _WORKSPACE_BYTES[(heads, dim, device)] = int(out.value)
+    return nbytes
 
 
-def gqa_backward(q, k, rmsnorm_weight, scales, sin, cos, positions, grad_q_out, grad_k_out, eps):
+def gqa_backward(q, k, rmsnorm_weight, scales, sin, cos, positions, grad_q_out, grad_k_out, eps, checked=False):
+    """``checked``: the arguments but the gradients went through gqa_forward."""
     from .distributed import active_peer_group
-    check_rows(q, k, rmsnorm_weight, scales, sin, cos, eps)
-    _check_positions(positions, q, sin)
+    if not checked:
+        check_rows(q, k, rmsnorm_weight, scales, sin, cos, eps)
+        _check_positions(positions, q, sin)
+    if grad_q_out.shape != q.shape or grad_k_out.shape != k.shape:
+        raise ValueError("upstream gradients must have the shapes of q and k")
     q, k = _in_place_rows(q), _in_place_rows(k)
-    grad_q, grad_k = _empty_like_rows(q), _empty_like_rows(k)
+    grad_q, grad_k = torch.empty_like(q), torch.empty_like(k)
     grad_w = torch.empty_like(rmsnorm_weight, memory_format=torch.contiguous_format)
     grad_s = torch.empty_like(scales, memory_format=torch.contiguous_format)
     gq, gk = _grad_view(grad_q_out, q), _grad_view(grad_k_out, k)
-    w, s = flat_fp32(rmsnorm_weight), scales.contiguous()
-    with _DeviceGuard(q.device):
-        workspace = torch.empty(_workspace_bytes(q.shape[1], q.shape[-1]), dtype=torch.uint8, device=q.device)
-        group = active_peer_group(q.device)
-        peers = (0, 0) if group is None else (ctypes.addressof(group.desc), group.next_epoch())
-        _call("flash_prologue_gqa_bwd", q, k, w, s, sin, cos, positions, eps,
-              (*_lib.NO_ROWS, *_lib.NO_ROWS, *rows_of(gq), *rows_of(gk), *rows_of(grad_q), *rows_of(grad_k)),
-              (grad_w.data_ptr(), grad_s.data_ptr()), (workspace.data_ptr(), workspace.numel()), peers)
+    workspace = grad_w.new_empty(_workspace_bytes(q.shape[1], q.shape[-1], q.device) // 4)
+    group = active_peer_group(q.device)
+    peers = (0, 0) if group is None else (ctypes.addressof(group.desc), group.next_epoch())
+    _call("flash_prologue_gqa_bwd", q, k, flat_fp32(rmsnorm_weight), scales.contiguous(), sin, cos, positions, eps,
+          (*_lib.NO_ROWS, *_lib.NO_ROWS, *rows_of(gq), *rows_of(gk), *rows_of(grad_q), *rows_of(grad_k)),
+          (grad_w.data_ptr(), grad_s.data_ptr()), (workspace.data_ptr(), 4 * workspace.numel()), peers)
     return grad_q, grad_k, grad_w, grad_s
 
 
@@ -185,7 +208,7 @@ class _GqaEager(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_q, grad_k):
-        dq, dk, dw, ds = gqa_backward(*ctx.saved_tensors, grad_q, grad_k, ctx.eps)
+        dq, dk, dw, ds = gqa_backward(*ctx.saved_tensors, grad_q, grad_k, ctx.eps, checked=True)
         return dq, dk, dw, ds, None, None, None, None
 
 
@@ -199,7 +222,7 @@ def qknorm_rope_scale_gqa_op(
 
 @qknorm_rope_scale_gqa_op.register_fake
 def _gqa_fake(q, k, rmsnorm_weight, scales, sin, cos, positions=None, eps=1e-5):
-    return _empty_like_rows(_in_place_rows(q)), _empty_like_rows(_in_place_rows(k))
+    return torch.empty_like(_in_place_rows(q)), torch.empty_like(_in_place_rows(k))
 
 
 @torch.library.custom_op("flash_prologue::qknorm_rope_scale_gqa_backward", mutates_args=())
@@ -213,7 +236,7 @@ def qknorm_rope_scale_gqa_backward_op(
 
 @qknorm_rope_scale_gqa_backward_op.register_fake
 def _gqa_backward_fake(q, k, rmsnorm_weight, scales, sin, cos, positions, grad_q_out, grad_k_out, eps=1e-5):
-    return (_empty_like_rows(_in_place_rows(q)), _empty_like_rows(_in_place_rows(k)),
+    return (torch.empty_like(_in_place_rows(q)), torch.empty_like(_in_place_rows(k)),
             torch.empty_like(rmsnorm_weight, memory_format=torch.contiguous_format),
             torch.empty_like(scales, memory_format=torch.contiguous_format))
 

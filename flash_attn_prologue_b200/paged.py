@@ -18,37 +18,39 @@ import torch
 
 from . import _lib
 from .fused_epilogue import _DeviceGuard
-from .gqa import MAX_HEADS, check_rows, eager, flat_fp32, readable, rotation_of, rows_of
+from .gqa import MAX_HEADS, call_library, check_rows, eager, flat_fp32, readable, rotation_of, rows_of
 
 
 def _check_cache(q, heads, k_cache, v_cache, page_table, seq_lens, cu_seqlens):
     """The cache and its tables, for packed rows q [T, H, D] with ``heads`` key heads."""
-    if k_cache.ndim != 4 or v_cache.shape != k_cache.shape or k_cache.shape[3] != q.shape[-1]:
+    ks, dtype, device = k_cache.shape, q.dtype, q.device
+    if len(ks) != 4 or v_cache.shape != ks or ks[3] != q.shape[2]:
         raise ValueError("caches must be matching [pages, page_size, Hk, D] tensors")
-    page_size = k_cache.shape[1]
+    page_size = ks[1]
     if page_size < 8 or page_size & (page_size - 1):
         raise ValueError("page_size must be a power of two, at least 8")
-    if k_cache.shape[2] != heads:
+    if ks[2] != heads:
         raise ValueError("caches and rows must have the same key heads")
-    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+    if k_cache.dtype != dtype or v_cache.dtype != dtype:
         raise ValueError("caches and rows must share a dtype")
     if k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
         raise ValueError("caches must be contiguous along D")
-    if page_table.ndim != 2 or seq_lens.shape != (page_table.shape[0],):
+    table = page_table.shape
+    if len(table) != 2 or seq_lens.shape != table[:1]:
         raise ValueError("page_table must be [B, max_pages] and seq_lens [B]")
-    for t in (page_table, seq_lens, cu_seqlens):
-        if t is not None and t.dtype != torch.int32:
-            raise ValueError("page_table, seq_lens and cu_seqlens must be int32")
-    if page_table.shape[1] > 1 and page_table.stride(1) != 1 or not seq_lens.is_contiguous():
+    int32 = torch.int32
+    if page_table.dtype != int32 or seq_lens.dtype != int32 or (cu_seqlens is not None and cu_seqlens.dtype != int32):
+        raise ValueError("page_table, seq_lens and cu_seqlens must be int32")
+    if (table[1] > 1 and page_table.stride(1) != 1) or not seq_lens.is_contiguous():
         raise ValueError("page_table rows and seq_lens must be contiguous")
     if cu_seqlens is None:
-        if q.shape[0] != page_table.shape[0]:
+        if q.shape[0] != table[0]:
             raise ValueError("without cu_seqlens every request has one token")
-    elif cu_seqlens.shape != (page_table.shape[0] + 1,) or not cu_seqlens.is_contiguous():
+    elif cu_seqlens.shape != (table[0] + 1,) or not cu_seqlens.is_contiguous():
         raise ValueError("cu_seqlens must be a contiguous [B + 1]")
-    for t in (k_cache, v_cache, page_table, seq_lens, cu_seqlens):
-        if t is not None and t.device != q.device:
-            raise ValueError("all tensors must share a device")
+    if (k_cache.device != device or v_cache.device != device or page_table.device != device
+            or seq_lens.device != device or (cu_seqlens is not None and cu_seqlens.device != device)):
+        raise ValueError("all tensors must share a device")
 
 
 def _cache_of(k_cache, v_cache, page_table, seq_lens, cu_seqlens):
@@ -59,9 +61,11 @@ def _cache_of(k_cache, v_cache, page_table, seq_lens, cu_seqlens):
             0 if cu_seqlens is None else cu_seqlens.data_ptr(), page_table.shape[0])
 
 
-def _no_grad(name, tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{name} is not differentiable: call it under torch.no_grad()")
+def _no_grad(name, *tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{name} is not differentiable: call it under torch.no_grad()")
 
 
 def _append(q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache, page_table, seq_lens, cu_seqlens, eps):
@@ -70,7 +74,7 @@ def _append(q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache, page_ta
     check_rows(q, k, rmsnorm_weight, scales, sin, cos, eps)
     _check_cache(q, k.shape[1], k_cache, v_cache, page_table, seq_lens, cu_seqlens)
     q, k, v = readable(q), readable(k), readable(v)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if q.shape[0]:
         w = None if rmsnorm_weight is None else flat_fp32(rmsnorm_weight)
         s = None if scales is None else scales.contiguous()
@@ -79,9 +83,7 @@ def _append(q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache, page_ta
             0 if s is None else s.data_ptr(), *rotation_of(sin, cos),
             *_cache_of(k_cache, v_cache, page_table, seq_lens, cu_seqlens),
             q.shape[0], q.shape[1], k.shape[1], q.shape[2], _lib.DTYPE_CODES[q.dtype], eps)
-        with _DeviceGuard(q.device):
-            _lib.check(_lib.load().flash_prologue_append_paged(args, _lib.stream_of(q.device)),
-                       "flash_prologue_append_paged")
+        call_library("flash_prologue_append_paged", args, q)
     return q_out
 
 
@@ -115,7 +117,7 @@ def append_paged_kv(q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache,
     the device error word. Not differentiable.
     """
     args = (q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
-    _no_grad("append_paged_kv", args)
+    _no_grad("append_paged_kv", q, k, v, rmsnorm_weight, scales, k_cache, v_cache)
     call = _append if eager(*args) else torch.ops.flash_prologue.append_paged_kv
     return call(*args, eps)
 
@@ -124,15 +126,15 @@ ATTENTION_HEAD_DIMS = (64, 128)
 _WORKSPACE_BYTES = {}
 
 
-def _workspace_bytes(key, args):
+def _workspace_bytes(key, args, device):
     """Workspace of a call: a function of its sizes and the device (``key``), asked for once."""
-    key = (*key, torch.cuda.current_device())
     nbytes = _WORKSPACE_BYTES.get(key)
     if nbytes is None:
         out = ctypes.c_size_t(0)
-        _lib.check(_lib.load().flash_prologue_paged_attention_workspace_size(_lib.ATTENTION_ARGS.pack(*args),
-                                                                             ctypes.byref(out)),
-                   "flash_prologue_paged_attention_workspace_size")
+        with _DeviceGuard(device):
+            _lib.check(_lib.load().flash_prologue_paged_attention_workspace_size(_lib.ATTENTION_ARGS.pack(*args),
+                                                                                 ctypes.byref(out)),
+                       "flash_prologue_paged_attention_workspace_size")
         if len(_WORKSPACE_BYTES) >= 4096:  # many distinct sizes: start over
             _WORKSPACE_BYTES.clear()
         nbytes = _WORKSPACE_BYTES[key] = int(out.value)
@@ -164,19 +166,17 @@ def _attention(q, k_cache, v_cache, page_table, seq_lens, cu_seqlens, softmax_sc
     if q.device.type != "cuda":
         raise ValueError("the attention kernels run on CUDA devices only")
     q = _aligned_rows(q)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:2] if want_lse else (0,), dtype=torch.float32, device=q.device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = q.new_empty((tokens, heads), dtype=torch.float32) if want_lse else None
     if tokens:
-        with _DeviceGuard(q.device):
-            head = (*rows_of(q), *rows_of(out), lse.data_ptr() if want_lse else 0,
-                    *_cache_of(k_cache, v_cache, page_table, seq_lens, cu_seqlens))
-            sizes = (tokens, heads, kv_heads, dim, _lib.DTYPE_CODES[q.dtype], window, softmax_scale)
-            nbytes = _workspace_bytes((*sizes, cu_seqlens is None, k_cache.shape[1], page_table.shape),
-                                      (*head, 0, 0, *sizes))
-            workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-            args = _lib.ATTENTION_ARGS.pack(*head, workspace.data_ptr(), nbytes, *sizes)
-            _lib.check(_lib.load().flash_prologue_paged_attention(args, _lib.stream_of(q.device)),
-                       "flash_prologue_paged_attention")
+        head = (*rows_of(q), *rows_of(out), lse.data_ptr() if want_lse else 0,
+                *_cache_of(k_cache, v_cache, page_table, seq_lens, cu_seqlens))
+        sizes = (tokens, heads, kv_heads, dim, _lib.DTYPE_CODES[q.dtype], window, softmax_scale)
+        nbytes = _workspace_bytes((*sizes, cu_seqlens is None, k_cache.shape[1], page_table.shape, q.get_device()),
+                                  (*head, 0, 0, *sizes), q.device)
+        workspace = q.new_empty((nbytes + 1) // 2)
+        call_library("flash_prologue_paged_attention",
+                     _lib.ATTENTION_ARGS.pack(*head, workspace.data_ptr(), nbytes, *sizes), q)
     return out, lse
 
 
@@ -186,7 +186,8 @@ def paged_attention_op(
     seq_lens: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None, softmax_scale: float = 1.0, window: int = 0,
     want_lse: bool = False,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
-    return _attention(q, k_cache, v_cache, page_table, seq_lens, cu_seqlens, softmax_scale, window, want_lse)
+    out, lse = _attention(q, k_cache, v_cache, page_table, seq_lens, cu_seqlens, softmax_scale, window, want_lse)
+    return out, q.new_empty(0, dtype=torch.float32) if lse is None else lse
 
 
 @paged_attention_op.register_fake
@@ -210,7 +211,7 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, cu_seqlens=None, 
     What lies in slots that a token does not see never reaches it. Not differentiable.
     """
     tensors = (q, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
-    _no_grad("paged_attention", tensors)
+    _no_grad("paged_attention", q, k_cache, v_cache)
     call = _attention if eager(*tensors) else torch.ops.flash_prologue.paged_attention
     out, lse = call(*tensors, softmax_scale, window, return_lse)
     return (out, lse) if return_lse else out
