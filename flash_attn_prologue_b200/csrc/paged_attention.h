@@ -58,7 +58,8 @@ __device__ __forceinline__ Request request_at(const PagedTarget& p, int64_t toke
 size_t paged_decode_workspace(int D, int sms);
 struct PrefillPlan {
   int tile_tokens;   // whole tokens of a 128-row tile
-  int splits;        // shares of a tile's keys
+  int splits;        // shares of the keys of the items behind whole_items
+  int64_t whole_items;
   int64_t tiles;     // tiles there can be, all requests
   size_t workspace;  // bytes; 0 without shares
 };
