@@ -29,63 +29,50 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// One row block of a warp's work: this lane's token and head.
-struct BlockCursor {
-  int64_t item;
-  int i, i1;          // head block, end of the slice
-  int64_t b, n;       // token (valid when there)
-  bool there;
-
-  __device__ __forceinline__ void enter(const GqaBwdArgs& a, int64_t items, int tp, int tslot) {
-    if (item >= items) return;
-    const int64_t group = a.p.slices == 1 ? item : item / a.p.slices;
-    i = (int)(item - group * a.p.slices) * a.p.per_slice;
-    i1 = min(i + a.p.per_slice, a.p.iters[0] + a.p.iters[1]);
-    const int64_t token = group * tp + tslot;
-    there = token < a.B * a.N;
-    b = 0;
-    n = token;
-    if (a.B > 1 && there) {
-      b = token / a.N;
-      n = token - b * a.N;
-    }
-  }
-  // Next row block; true when it is the first one of another token group.
-  __device__ __forceinline__ bool next(const GqaBwdArgs& a, int64_t items, int64_t warps, int tp, int tslot) {
-    if (++i < i1) return false;
-    item += warps;
-    enter(a, items, tp, tslot);
-    return true;
-  }
+// A warp's walk over its row blocks: for each of its token groups the slice's
+// head blocks of Q, then of K. `in` and `g` point at this lane's first columns.
+template <typename T>
+struct Walk {
+  int item;
+  int i, i1;          // head block of Q and K together, end of the slice
+  const T* in[2];
+  bool there;         // this lane's token exists (the pointers stay put where not)
 };
 
 template <typename T, int D, bool VEC>
 __global__ void __launch_bounds__(kThreads, 2) gqa_bwd_kernel(const GqaBwdArgs a) {
   constexpr int L = D / 16;
   constexpr int HALF = D / 2;
-  constexpr int kPieces = Chunk<T>::kWords / 4;             // 16-byte pieces of a chunk
-  constexpr int kStageBytes = VEC ? 4 * kPieces * 512 : 0;  // x1, x2, g1, g2 of 32 lanes
+  using C = Columns<T, D>;
+  constexpr int kStageBytes = VEC ? 4 * C::kPieces * 512 : 0;  // x1, x2, g1, g2 of 32 lanes
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  float* w_s = reinterpret_cast<float*>(smem_raw);  // [2 * D]
-  float* e_s = w_s + 2 * D;                         // [Hq]
-  float* ds_s = e_s + a.H[0];                       // [kWarps][Hq]
-  float* dw_s = ds_s + kWarps * a.H[0];             // [kWarps][2 * D]
+  float* w_s = reinterpret_cast<float*>(smem_raw);  // [q, k][half][lane of a row][8]: as the lanes own them
+  float2* e_s = reinterpret_cast<float2*>(w_s + 2 * D);  // [Hq] exp(scale), exp(-scale)
+  float* ds_s = reinterpret_cast<float*>(e_s + a.H[0]);  // [kWarps][Hq]
+  float* dw_s = ds_s + kWarps * a.H[0];                  // [kWarps][2 * D]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t floats = (uint32_t)(2 * D + a.H[0] * (kWarps + 1) + kWarps * 2 * D);
+  const uint32_t floats = (uint32_t)(2 * D + a.H[0] * (kWarps + 2) + kWarps * 2 * D);
   unsigned char* ring = smem_raw + ((floats * 4 + 15) & ~15u) + warp * kStages * kStageBytes + lane * 16;
   const uint32_t ring_u = smem_u32(ring);
-  for (int i = threadIdx.x; i < 2 * D; i += kThreads) w_s[i] = a.w[i];
-  for (int i = threadIdx.x; i < a.H[0]; i += kThreads) e_s[i] = expf(a.scales[i]);
+  for (int i = threadIdx.x; i < 2 * D; i += kThreads) {
+    const int c = i / kChunk % L, j = i % kChunk;
+    w_s[i] = a.w[i / HALF * HALF + C::of(c, j)];
+  }
+  for (int i = threadIdx.x; i < a.H[0]; i += kThreads) {
+    const float v = a.scales[i];
+    e_s[i] = make_float2(expf(v), expf(-v));
+  }
   for (int i = threadIdx.x; i < kWarps * a.H[0]; i += kThreads) ds_s[i] = 0.f;
   __syncthreads();
 
-  const int slot = lane / L;
-  const int j0 = (lane % L) * kChunk;
+  const int slot = lane / L, c_lane = lane % L;
+  const int j0 = C::first(c_lane);
   const int HS = 1 << a.p.log2_hs;
   const int TP = (32 / L) >> a.p.log2_hs;
   const int hslot = slot & (HS - 1), tslot = slot >> a.p.log2_hs;
-  const int64_t items = a.p.groups * a.p.slices;
-  const int64_t warps = (int64_t)gridDim.x * kWarps;
+  // Items, tokens and rows are counted in 32 bits (the host checks): fewer registers and no 64-bit division.
+  const int items = (int)(a.p.groups * a.p.slices), warps = gridDim.x * kWarps, tokens = (int)(a.B * a.N), N = (int)a.N;
+  const int q_iters = a.p.iters[0], all_iters = q_iters + a.p.iters[1];
 
   float2 acc[2][2][kPairs];  // d w of this lane's columns: [q, k][first, second half]
 #pragma unroll
@@ -93,34 +80,58 @@ __global__ void __launch_bounds__(kThreads, 2) gqa_bwd_kernel(const GqaBwdArgs a
 #pragma unroll
     for (int p = 0; p < kPairs; ++p) acc[t][0][p] = acc[t][1][p] = make_float2(0.f, 0.f);
 
-  BlockCursor cur, pre;
-  cur.item = (int64_t)blockIdx.x * kWarps + warp;
-  cur.enter(a, items, TP, tslot);
-  pre = cur;
+  // This lane's token of an item, and its first row of tensor t under head block it.
+  const auto token_of = [&](int item, int& b, int& n, int& i) {
+    const int group = a.p.slices == 1 ? item : item / a.p.slices;
+    i = (item - group * a.p.slices) * a.p.per_slice;
+    const int token = group * TP + tslot;
+    const bool there = token < tokens;
+    b = 0;
+    n = there ? token : 0;
+    if (a.B > 1) {
+      b = n / N;
+      n -= b * N;
+    }
+    return there;
+  };
+  Walk<T> pre;
+  int pre_b = 0, pre_n = 0;
+  const auto pre_at = [&](int t, int it) {
+    const int h = it * HS + hslot;
+    pre.in[0] = static_cast<const T*>(a.x[t]) + pre_b * a.sx[t].b + h * a.sx[t].h + pre_n * a.sx[t].n + j0;
+    pre.in[1] = static_cast<const T*>(a.gy[t]) + pre_b * a.sgy[t].b + h * a.sgy[t].h + pre_n * a.sgy[t].n + j0;
+  };
+  const auto pre_enter = [&]() {
+    if (pre.item >= items) return;
+    pre.there = token_of(pre.item, pre_b, pre_n, pre.i);
+    pre.i1 = min(pre.i + a.p.per_slice, all_iters);
+    if (pre.i < q_iters) pre_at(0, pre.i);
+    else pre_at(1, pre.i - q_iters);
+  };
+  pre.item = blockIdx.x * kWarps + warp;
+  pre_enter();
 
-  auto prefetch = [&](int stage) {
+  const auto prefetch = [&](int stage) {
     if constexpr (VEC) {
       if (pre.item < items) {
-        const int t = pre.i >= a.p.iters[0];
-        const int h = (pre.i - t * a.p.iters[0]) * HS + hslot;
-        const bool ok = pre.there && h < a.H[t];
-        const T* x = static_cast<const T*>(a.x[t]);
-        const T* g = static_cast<const T*>(a.gy[t]);
-        if (ok) {
-          x += pre.b * a.sx[t].b + h * a.sx[t].h + pre.n * a.sx[t].n + j0;
-          g += pre.b * a.sgy[t].b + h * a.sgy[t].h + pre.n * a.sgy[t].n + j0;
-        }
         const uint32_t dst = ring_u + stage * kStageBytes;
 #pragma unroll
-        for (int q = 0; q < kPieces; ++q) {
-          const int o = q * (16 / (int)sizeof(T));
-          const int half = ok ? HALF : 0;
-          cp_async16(dst + (0 * kPieces + q) * 512, x + (ok ? o : 0), ok);
-          cp_async16(dst + (1 * kPieces + q) * 512, x + (ok ? half + o : 0), ok);
-          cp_async16(dst + (2 * kPieces + q) * 512, g + (ok ? o : 0), ok);
-          cp_async16(dst + (3 * kPieces + q) * 512, g + (ok ? half + o : 0), ok);
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int q = 0; q < C::kPieces; ++q) {
+            cp_async16(dst + ((2 * s) * C::kPieces + q) * 512, pre.in[s] + q * C::kApart, pre.there);
+            cp_async16(dst + ((2 * s + 1) * C::kPieces + q) * 512, pre.in[s] + HALF + q * C::kApart, pre.there);
+          }
+        ++pre.i;
+        if (pre.i == pre.i1) {
+          pre.item += warps;
+          pre_enter();
+        } else if (pre.i == q_iters) {
+          pre_at(1, 0);
+        } else {
+          pre.in[0] += HS * (pre.i < q_iters ? a.sx[0].h : a.sx[1].h);
+          pre.in[1] += HS * (pre.i < q_iters ? a.sgy[0].h : a.sgy[1].h);
         }
-        pre.next(a, items, warps, TP, tslot);
       }
       cp_async_commit();  // an empty group past the end keeps the count
     }
@@ -128,79 +139,81 @@ __global__ void __launch_bounds__(kThreads, 2) gqa_bwd_kernel(const GqaBwdArgs a
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) prefetch(s);
 
-  float sn[kChunk], cs[kChunk];
-  bool fresh = true;
   int stage = 0;
-  while (cur.item < items) {
-    if (fresh) {
-      const int64_t pos = cur.there ? rotation_row(a.tab, cur.b, cur.n) : -1;
-      if (pos >= 0) {
-        load_table<VEC>(sn, a.tab.sin + pos * a.tab.sin_n + j0 * a.tab.sin_j, a.tab.sin_j);
-        load_table<VEC>(cs, a.tab.cos + pos * a.tab.cos_n + j0 * a.tab.cos_j, a.tab.cos_j);
-      } else {
-        const float v = cur.there ? __int_as_float(0x7fc00000) : 0.f;  // as in the forward
-#pragma unroll
-        for (int j = 0; j < kChunk; ++j) { sn[j] = v; cs[j] = v; }
-      }
-    }
-    const int t = cur.i >= a.p.iters[0];
-    const int h = (cur.i - t * a.p.iters[0]) * HS + hslot;
-    const bool ok = cur.there && h < a.H[t];
-    Chunk<T> x1, x2, g1, g2;
-    if constexpr (VEC) {
-      int ahead = stage + kStages - 1;
-      if (ahead >= kStages) ahead -= kStages;
-      prefetch(ahead);
-      cp_async_wait<kStages - 1>();
-      const uint4* src = reinterpret_cast<const uint4*>(ring + stage * kStageBytes);
-#pragma unroll
-      for (int q = 0; q < kPieces; ++q) {
-        const uint4 v0 = src[(0 * kPieces + q) * 32], v1 = src[(1 * kPieces + q) * 32];
-        const uint4 v2 = src[(2 * kPieces + q) * 32], v3 = src[(3 * kPieces + q) * 32];
-        x1.w[4 * q] = v0.x; x1.w[4 * q + 1] = v0.y; x1.w[4 * q + 2] = v0.z; x1.w[4 * q + 3] = v0.w;
-        x2.w[4 * q] = v1.x; x2.w[4 * q + 1] = v1.y; x2.w[4 * q + 2] = v1.z; x2.w[4 * q + 3] = v1.w;
-        g1.w[4 * q] = v2.x; g1.w[4 * q + 1] = v2.y; g1.w[4 * q + 2] = v2.z; g1.w[4 * q + 3] = v2.w;
-        g2.w[4 * q] = v3.x; g2.w[4 * q + 1] = v3.y; g2.w[4 * q + 2] = v3.z; g2.w[4 * q + 3] = v3.w;
-      }
-      if (++stage == kStages) stage = 0;
+  for (int item = blockIdx.x * kWarps + warp; item < items; item += warps) {
+    int b, n, i0;
+    const bool there = token_of(item, b, n, i0);
+    const int i1 = i0 + a.p.per_slice;
+    float sn[kChunk], cs[kChunk];
+    const int64_t pos = there ? rotation_row(a.tab, b, n) : -1;
+    if (pos >= 0) {
+      load_columns<T, D, VEC>(sn, a.tab.sin + pos * a.tab.sin_n + j0 * a.tab.sin_j, a.tab.sin_j);
+      load_columns<T, D, VEC>(cs, a.tab.cos + pos * a.tab.cos_n + j0 * a.tab.cos_j, a.tab.cos_j);
     } else {
-      if (ok) {
-        const T* x = static_cast<const T*>(a.x[t]) + cur.b * a.sx[t].b + h * a.sx[t].h + cur.n * a.sx[t].n + j0;
-        const T* g = static_cast<const T*>(a.gy[t]) + cur.b * a.sgy[t].b + h * a.sgy[t].h + cur.n * a.sgy[t].n + j0;
-        load_stream<T, false>(x1, x);
-        load_stream<T, false>(x2, x + HALF);
-        load_stream<T, false>(g1, g);
-        load_stream<T, false>(g2, g + HALF);
-      } else {
-        chunk_zero(x1);
-        chunk_zero(x2);
-        chunk_zero(g1);
-        chunk_zero(g2);
+      const float v = there ? __int_as_float(0x7fc00000) : 0.f;  // as in the forward
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) { sn[j] = v; cs[j] = v; }
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int begin = t ? q_iters : 0;
+      const int it0 = max(i0 - begin, 0), it1 = min(i1 - begin, a.p.iters[t]);
+      if (it0 >= it1) continue;
+      const int h0 = it0 * HS + hslot;
+      T* out = static_cast<T*>(a.dx[t]) + b * a.sdx[t].b + h0 * a.sdx[t].h + n * a.sdx[t].n + j0;
+            const float* wa = w_s + t * D + c_lane * kChunk;
+      const float* wb = wa + HALF;
+      for (int it = it0; it < it1; ++it) {
+        const int h = it * HS + hslot;
+        Chunk<T> x1, x2, g1, g2;
+        if constexpr (VEC) {
+          int ahead = stage + kStages - 1;
+          if (ahead >= kStages) ahead -= kStages;
+          prefetch(ahead);
+          cp_async_wait<kStages - 1>();
+          const uint4* src = reinterpret_cast<const uint4*>(ring + stage * kStageBytes);
+#pragma unroll
+          for (int q = 0; q < C::kPieces; ++q) {
+            const uint4 v0 = src[(0 * C::kPieces + q) * 32], v1 = src[(1 * C::kPieces + q) * 32];
+            const uint4 v2 = src[(2 * C::kPieces + q) * 32], v3 = src[(3 * C::kPieces + q) * 32];
+            x1.w[4 * q] = v0.x; x1.w[4 * q + 1] = v0.y; x1.w[4 * q + 2] = v0.z; x1.w[4 * q + 3] = v0.w;
+            x2.w[4 * q] = v1.x; x2.w[4 * q + 1] = v1.y; x2.w[4 * q + 2] = v1.z; x2.w[4 * q + 3] = v1.w;
+            g1.w[4 * q] = v2.x; g1.w[4 * q + 1] = v2.y; g1.w[4 * q + 2] = v2.z; g1.w[4 * q + 3] = v2.w;
+            g2.w[4 * q] = v3.x; g2.w[4 * q + 1] = v3.y; g2.w[4 * q + 2] = v3.z; g2.w[4 * q + 3] = v3.w;
+          }
+          if (++stage == kStages) stage = 0;
+        } else if (there) {
+          const T* x = static_cast<const T*>(a.x[t]) + b * a.sx[t].b + h * a.sx[t].h + n * a.sx[t].n + j0;
+          const T* g = static_cast<const T*>(a.gy[t]) + b * a.sgy[t].b + h * a.sgy[t].h + n * a.sgy[t].n + j0;
+          load_chunk<T, D, false>(x1, x);
+          load_chunk<T, D, false>(x2, x + HALF);
+          load_chunk<T, D, false>(g1, g);
+          load_chunk<T, D, false>(g2, g + HALF);
+        } else {
+          chunk_zero(x1);
+          chunk_zero(x2);
+          chunk_zero(g1);
+          chunk_zero(g2);
+        }
+        const float r = inv_rms_bwd<D>(row_sum<L>(lane_sumsq2(x1, x2)), a.eps);
+        const float2 e = t == 0 ? e_s[h] : make_float2(1.f, 1.f);
+        const float re = r * e.x;
+        float2 u1[kPairs], u2[kPairs], n1[kPairs], n2[kPairs];
+        const float s = row_sum<L>(
+            bwd_lane_reduce(x1, x2, g1, g2, re, wa, wb, sn, cs, acc[t][0], acc[t][1], u1, u2, n1, n2));
+        if (t == 0) {
+          float sum = s;  // over the warp's tokens of this head
+          for (int o = L * HS; o < 32; o <<= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, o));
+          if (c_lane == 0 && tslot == 0) ds_s[warp * a.H[0] + h] += sum;
+        }
+        if (there) {
+          lane_dx(n1, n2, u1, u2, re, r * (s * (1.f / D)) * e.y, x1, x2);
+          store_chunk<T, D, VEC>(out, x1);
+          store_chunk<T, D, VEC>(out + HALF, x2);
+        }
+        out += HS * a.sdx[t].h;
       }
     }
-    const float r = inv_rms_bwd<D>(row_sum<L>(lane_sumsq2(x1, x2)), a.eps);
-    const float e = t == 0 && ok ? e_s[h] : 1.f;
-    const float re = r * e;
-    const float* wa = w_s + t * D + j0;
-    const float* wb = wa + HALF;
-    float2 u1[kPairs], u2[kPairs], n1[kPairs], n2[kPairs];
-    float part;
-    if (t == 0) part = bwd_lane_reduce(x1, x2, g1, g2, re, wa, wb, sn, cs, acc[0][0], acc[0][1], u1, u2, n1, n2);
-    else part = bwd_lane_reduce(x1, x2, g1, g2, re, wa, wb, sn, cs, acc[1][0], acc[1][1], u1, u2, n1, n2);
-    const float s = row_sum<L>(part);
-    if (t == 0) {
-      float sum = s;  // over the warp's tokens of this head
-      for (int o = L * HS; o < 32; o <<= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, o));
-      if (j0 == 0 && tslot == 0 && h < a.H[0]) ds_s[warp * a.H[0] + h] += sum;
-    }
-    if (ok) {
-      T* out = static_cast<T*>(a.dx[t]) + cur.b * a.sdx[t].b + h * a.sdx[t].h + cur.n * a.sdx[t].n + j0;
-      Chunk<T> o1, o2;
-      lane_dx(n1, n2, u1, u2, re, r * (s * (1.f / D)) / e, o1, o2);
-      store_stream<T, VEC>(out, o1);
-      store_stream<T, VEC>(out + HALF, o2);
-    }
-    fresh = cur.next(a, items, warps, TP, tslot);
   }
   if constexpr (VEC) cp_async_wait<0>();
 
@@ -215,14 +228,14 @@ __global__ void __launch_bounds__(kThreads, 2) gqa_bwd_kernel(const GqaBwdArgs a
       for (int j = 0; j < kChunk; ++j) {
 #pragma unroll
         for (int o = L; o < 32; o <<= 1) v[j] = __fadd_rn(v[j], __shfl_xor_sync(0xffffffffu, v[j], o));
-        if (slot == 0) dw_s[warp * 2 * D + t * D + half * HALF + j0 + j] = v[j];
+        if (slot == 0) dw_s[warp * 2 * D + t * D + half * HALF + C::of(c_lane, j)] = v[j];
       }
     }
   }
   __syncthreads();
-  const int C = 2 * D + a.H[0];
-  float* out = a.partials + (int64_t)blockIdx.x * C;
-  for (int col = threadIdx.x; col < C; col += kThreads) {
+  const int C2 = 2 * D + a.H[0];
+  float* out = a.partials + (int64_t)blockIdx.x * C2;
+  for (int col = threadIdx.x; col < C2; col += kThreads) {
     float v = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w)
@@ -234,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, 2) gqa_bwd_kernel(const GqaBwdArgs a
 const void* bwd_kernel_for(int dtype, int D, bool vec) { FLASH_PROLOGUE_GQA_KERNEL(gqa_bwd_kernel) }
 
 size_t smem_bytes(int Hq, int D, int dtype, bool vec) {
-  const size_t floats = (size_t)2 * D + (size_t)Hq * (kWarps + 1) + (size_t)kWarps * 2 * D;
+  const size_t floats = (size_t)2 * D + (size_t)Hq * (kWarps + 2) + (size_t)kWarps * 2 * D;
   const size_t stage = vec ? (dtype == 2 ? 4096 : 2048) : 0;
   return ((floats * 4 + 15) & ~(size_t)15) + kWarps * kStages * stage;
 }

@@ -68,7 +68,8 @@ bool heads_inner(const flash_prologue_rows& q, int64_t H, int64_t N) {
 int gqa_checks(const flash_prologue_gqa_args* a) {
   if (!a || a->B < 0 || a->N < 0 || a->Hq < 0 || a->Hk < 0) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
   if (!(a->eps > 0) || !isfinite(a->eps)) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
-  if (!supported(a->D, a->dtype) || a->Hq > kMaxGqaHeads || a->B >= (int64_t(1) << 31) || a->N >= (int64_t(1) << 31))
+  if (!supported(a->D, a->dtype) || a->Hq > kMaxGqaHeads || a->B >= (int64_t(1) << 31) || a->N >= (int64_t(1) << 31) ||
+      a->B * a->N >= (int64_t(1) << 31) - (1 << 20))
     return FLASH_PROLOGUE_ERR_UNSUPPORTED;
   if (a->Hk > 0 ? a->Hq % a->Hk != 0 : a->Hq != 0) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
   if (a->B * a->N * a->Hq == 0) return FLASH_PROLOGUE_OK;
@@ -224,7 +225,7 @@ int flash_prologue_gqa_bwd(const flash_prologue_gqa_args* a, void* stream) {
 int flash_prologue_append_paged(const flash_prologue_append_args* a, void* stream) {
   if (!a || a->tokens < 0 || a->Hq < 0 || a->Hk < 0) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
   if (!(a->eps > 0) || !isfinite(a->eps)) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
-  if (!supported(a->D, a->dtype) || a->Hq > kMaxGqaHeads || a->tokens >= (int64_t(1) << 31))
+  if (!supported(a->D, a->dtype) || a->Hq > kMaxGqaHeads || a->tokens >= (int64_t(1) << 31) - (1 << 20))
     return FLASH_PROLOGUE_ERR_UNSUPPORTED;
   if (a->Hk > 0 ? a->Hq % a->Hk != 0 : a->Hq != 0) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
   const flash_prologue_cache& c = a->cache;

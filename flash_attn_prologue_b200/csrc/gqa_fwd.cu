@@ -34,24 +34,24 @@ __global__ void __launch_bounds__(kThreads) gqa_fwd_kernel(const GqaFwdArgs a) {
   constexpr int HALF = D / 2;
   const int lane = threadIdx.x & 31;
   const int slot = lane / L;
-  const int j0 = (lane % L) * kChunk;
+  const int j0 = Columns<T, D>::first(lane % L);
   const int HS = 1 << a.p.log2_hs;
   const int TP = (32 / L) >> a.p.log2_hs;
   const int hslot = slot & (HS - 1), tslot = slot >> a.p.log2_hs;
-  const int64_t items = a.p.groups * a.p.slices;
-  const int64_t warps = (int64_t)gridDim.x * kWarps;
-  const int all_iters = a.p.iters[0] + a.p.iters[1] + a.p.iters[2];
+  // Items, tokens and rows are counted in 32 bits (the host checks): fewer registers and no 64-bit division.
+  const int items = (int)(a.p.groups * a.p.slices), warps = gridDim.x * kWarps, tokens = (int)(a.B * a.N), N = (int)a.N;
+  const bool paged = a.paged.page_table != nullptr;
 
-  for (int64_t item = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); item < items; item += warps) {
-    const int64_t group = a.p.slices == 1 ? item : item / a.p.slices;
-    const int i0 = (int)(item - group * a.p.slices) * a.p.per_slice;
-    const int i1 = min(i0 + a.p.per_slice, all_iters);
-    const int64_t token = group * TP + tslot;
+  for (int item = blockIdx.x * kWarps + (threadIdx.x >> 5); item < items; item += warps) {
+    const int group = a.p.slices == 1 ? item : item / a.p.slices;
+    const int i0 = (item - group * a.p.slices) * a.p.per_slice, i1 = i0 + a.p.per_slice;
+    const int token = group * TP + tslot;
     // Where this lane's token lies, and the row of the tables that turns it.
-    bool there = token < a.B * a.N;
-    int64_t b = 0, n = token, pos = -1, page = 0, in_page = 0;
+    const bool there = token < tokens;
+    int b = 0, n = there ? token : 0, page = 0, in_page = 0;
+    int64_t pos = -1;
     if (there) {
-      if (a.paged.page_table) {
+      if (paged) {
         const PagedTarget& pg = a.paged;
         int64_t first = token, count = 1;
         int64_t r = token;
@@ -70,88 +70,88 @@ __global__ void __launch_bounds__(kThreads) gqa_fwd_kernel(const GqaFwdArgs a) {
           }
           if (ok) {
             pos = at;
-            in_page = at & ((1 << pg.page_log2) - 1);
+            in_page = (int)at & ((1 << pg.page_log2) - 1);
           } else {
             atomicOr(&g_device_error, kDeviceErrorIndex);
           }
         }
       } else {
         if (a.B > 1) {
-          b = token / a.N;
-          n = token - b * a.N;
+          b = token / N;
+          n = token - b * N;
         }
         pos = rotation_row(a.tab, b, n);
       }
     }
+    const bool placed = pos >= 0;
     float sn[kChunk], cs[kChunk];
-    if (pos >= 0) {
-      load_table<VEC>(sn, a.tab.sin + pos * a.tab.sin_n + j0 * a.tab.sin_j, a.tab.sin_j);
-      load_table<VEC>(cs, a.tab.cos + pos * a.tab.cos_n + j0 * a.tab.cos_j, a.tab.cos_j);
+    if (placed) {
+      load_columns<T, D, VEC>(sn, a.tab.sin + pos * a.tab.sin_n + j0 * a.tab.sin_j, a.tab.sin_j);
+      load_columns<T, D, VEC>(cs, a.tab.cos + pos * a.tab.cos_n + j0 * a.tab.cos_j, a.tab.cos_j);
     } else {
       // A position out of range rotates by NaN (dense rows); a token without a place gives zeros.
-      const float v = a.paged.page_table ? 0.f : __int_as_float(0x7fc00000);
+      const float v = paged ? 0.f : __int_as_float(0x7fc00000);
 #pragma unroll
       for (int j = 0; j < kChunk; ++j) { sn[j] = v; cs[j] = v; }
     }
 
-    float wa[kChunk], wb[kChunk];
-    int w_of = -1;
-    for (int i = i0; i < i1; i += kAhead) {
-      Chunk<T> x1[kAhead], x2[kAhead];
+    // The slice's row blocks of Q, then K, then V; HS divides their heads.
+    int begin = 0;
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        int t = 0, it = i + k;
-        if (it >= a.p.iters[0]) { it -= a.p.iters[0]; t = 1; }
-        if (t == 1 && it >= a.p.iters[1]) { it -= a.p.iters[1]; t = 2; }
-        const int h = it * HS + hslot;
-        if (there && i + k < i1 && h < a.H[t]) {
-          const T* p = static_cast<const T*>(a.x[t]) + b * a.sx[t].b + h * a.sx[t].h + n * a.sx[t].n + j0;
-          load_stream<T, VEC>(x1[k], p);
-          load_stream<T, VEC>(x2[k], p + HALF);
+    for (int t = 0; t < 3; ++t) {
+      const int it0 = max(i0 - begin, 0), it1 = min(i1 - begin, a.p.iters[t]);
+      begin += a.p.iters[t];
+      if (it0 >= it1) continue;
+      const int h0 = it0 * HS + hslot;
+      const bool to_cache = t != 0 && paged;
+      const T* in = static_cast<const T*>(a.x[t]) + b * a.sx[t].b + h0 * a.sx[t].h + n * a.sx[t].n + j0;
+      T* out = static_cast<T*>(a.y[t]) + h0 * a.sy[t].h + j0 +
+               (to_cache ? page * a.sy[t].b + in_page * a.sy[t].n : b * a.sy[t].b + n * a.sy[t].n);
+      const bool store = there && (placed || !to_cache);
+      float wa[kChunk], wb[kChunk];
+      const float* scales = t == 0 ? a.scales : nullptr;
+      if (t != 2) {
+        if (a.w) {
+          load_columns<T, D, true>(wa, a.w + t * D + j0, 1);
+          load_columns<T, D, true>(wb, a.w + t * D + HALF + j0, 1);
         } else {
-          chunk_zero(x1[k]);
-          chunk_zero(x2[k]);
+#pragma unroll
+          for (int j = 0; j < kChunk; ++j) wa[j] = wb[j] = 1.f;
         }
       }
+      for (int it = it0; it < it1; it += kAhead) {
+        Chunk<T> x1[kAhead], x2[kAhead];
+        float e[kAhead];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        if (i + k >= i1) break;
-        int t = 0, it = i + k;
-        if (it >= a.p.iters[0]) { it -= a.p.iters[0]; t = 1; }
-        if (t == 1 && it >= a.p.iters[1]) { it -= a.p.iters[1]; t = 2; }
-        const int h = it * HS + hslot;
-        const bool ok = there && h < a.H[t];
-        const bool to_cache = t != 0 && a.paged.page_table;
-        T* out = static_cast<T*>(a.y[t]) + h * a.sy[t].h + j0 +
-                 (to_cache ? page * a.sy[t].b + in_page * a.sy[t].n : b * a.sy[t].b + n * a.sy[t].n);
-        const bool store = ok && !(to_cache && pos < 0);
-        if (t == 2) {
+        for (int k = 0; k < kAhead; ++k) {
+          if (there && it + k < it1) {
+            load_chunk<T, D, VEC>(x1[k], in);
+            load_chunk<T, D, VEC>(x2[k], in + HALF);
+            e[k] = scales ? __ldg(scales + (it + k) * HS + hslot) : 0.f;
+            in += HS * a.sx[t].h;
+          } else {
+            chunk_zero(x1[k]);
+            chunk_zero(x2[k]);
+            e[k] = 0.f;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          if (it + k >= it1) break;
+          if (t != 2) {
+            const float r = a.w ? inv_rms<D>(row_sum<L>(lane_sumsq(x1[k], x2[k])), a.eps) : 1.f;
+            fwd_lane(x1[k], x2[k], r, wa, wb, sn, cs, scales != nullptr, scales ? expf(e[k]) : 1.f, x1[k], x2[k]);
+            if (!placed && paged) {  // also where the row holds infinities
+              chunk_zero(x1[k]);
+              chunk_zero(x2[k]);
+            }
+          }
           if (store) {
-            store_stream<T, VEC>(out, x1[k]);
-            store_stream<T, VEC>(out + HALF, x2[k]);
+            store_chunk<T, D, VEC>(out, x1[k]);
+            store_chunk<T, D, VEC>(out + HALF, x2[k]);
           }
-          continue;
+          out += HS * a.sy[t].h;
         }
-        if (w_of != t) {
-          w_of = t;
-#pragma unroll
-          for (int j = 0; j < kChunk; ++j) {
-            wa[j] = a.w ? __ldg(a.w + t * D + j0 + j) : 1.f;
-            wb[j] = a.w ? __ldg(a.w + t * D + HALF + j0 + j) : 1.f;
-          }
-        }
-        float r = 1.f;
-        if (a.w) r = inv_rms<D>(row_sum<L>(lane_sumsq(x1[k], x2[k])), a.eps);
-        if (!store) continue;  // after the shuffles: every lane took part in them
-        const bool scale = t == 0 && a.scales;
-        Chunk<T> o1, o2;
-        fwd_lane(x1[k], x2[k], r, wa, wb, sn, cs, scale, scale ? expf(__ldg(a.scales + h)) : 1.f, o1, o2);
-        if (pos < 0 && a.paged.page_table) {  // also where the row holds infinities
-          chunk_zero(o1);
-          chunk_zero(o2);
-        }
-        store_stream<T, VEC>(out, o1);
-        store_stream<T, VEC>(out + HALF, o2);
       }
     }
   }
@@ -173,9 +173,9 @@ RowsPlan plan_rows(int64_t tokens, int Hq, int Hk, int Hv, int D, bool heads_inn
     ++p.log2_hs;
   }
   const int tp = slots / hs;
-  p.iters[0] = (Hq + hs - 1) / hs;
-  p.iters[1] = (Hk + hs - 1) / hs;
-  p.iters[2] = (Hv + hs - 1) / hs;
+  p.iters[0] = Hq / hs;
+  p.iters[1] = Hk / hs;
+  p.iters[2] = Hv / hs;
   p.groups = (tokens + tp - 1) / tp;
   const int all = p.iters[0] + p.iters[1] + p.iters[2];
   int64_t slices = p.groups > 0 ? (want_warps + p.groups - 1) / p.groups : 1;

@@ -112,6 +112,66 @@ __device__ __forceinline__ void chunk_zero(Chunk<T>& c) {
   for (int i = 0; i < Chunk<T>::kWords; ++i) c.w[i] = 0;
 }
 
+// Columns of a half row that lane c of the row's L owns: 8 of them, in 16-byte
+// pieces that lie next to the other lanes' (one piece of a 16-bit type, two of
+// FP32: with 32 bytes a lane every access would touch twice the sectors).
+template <typename T, int D>
+struct Columns {
+  static constexpr int kPieces = sizeof(T) == 4 ? 2 : 1;
+  static constexpr int kPer = kChunk / kPieces;           // columns of a piece
+  static constexpr int kApart = D / 2 / kPieces;          // columns from one piece to the next
+  static __device__ __forceinline__ int first(int c) { return c * kPer; }
+  static __device__ __forceinline__ int of(int c, int j) { return j / kPer * kApart + c * kPer + j % kPer; }
+};
+
+// The lane's chunk of a half row; `half` points at the half's first piece of the lane.
+template <typename T, int D, bool VEC>
+__device__ __forceinline__ void load_chunk(Chunk<T>& x, const T* half) {
+  using C = Columns<T, D>;
+  if constexpr (VEC) {
+#pragma unroll
+    for (int q = 0; q < C::kPieces; ++q) {
+      const uint4 v = __ldcs(reinterpret_cast<const uint4*>(half + q * C::kApart));
+      x.w[4 * q] = v.x; x.w[4 * q + 1] = v.y; x.w[4 * q + 2] = v.z; x.w[4 * q + 3] = v.w;
+    }
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) x.w[j] = reinterpret_cast<const uint32_t*>(half)[C::of(0, j)];
+  } else {
+    load_stream<T, false>(x, half);
+  }
+}
+template <typename T, int D, bool VEC>
+__device__ __forceinline__ void store_chunk(T* half, const Chunk<T>& x) {
+  using C = Columns<T, D>;
+  if constexpr (VEC) {
+#pragma unroll
+    for (int q = 0; q < C::kPieces; ++q)
+      *reinterpret_cast<uint4*>(half + q * C::kApart) =
+          make_uint4(x.w[4 * q], x.w[4 * q + 1], x.w[4 * q + 2], x.w[4 * q + 3]);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) reinterpret_cast<uint32_t*>(half)[C::of(0, j)] = x.w[j];
+  } else {
+    store_stream<T, false>(half, x);
+  }
+}
+// The lane's 8 values of an FP32 table row or parameter (`half`: as above, in floats).
+template <typename T, int D, bool VEC>
+__device__ __forceinline__ void load_columns(float (&v)[kChunk], const float* half, int64_t stride) {
+  using C = Columns<T, D>;
+  if constexpr (VEC) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const float4 x = __ldg(reinterpret_cast<const float4*>(half + C::of(0, 4 * q)));
+      v[4 * q] = x.x; v[4 * q + 1] = x.y; v[4 * q + 2] = x.z; v[4 * q + 3] = x.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) v[j] = __ldg(half + C::of(0, j) * stride);
+  }
+}
+
 // A kernel for each activation type, head dimension and access width.
 #define FLASH_PROLOGUE_GQA_DIMS(T, KERNEL)                                                        \
   switch (D) {                                                                                    \
