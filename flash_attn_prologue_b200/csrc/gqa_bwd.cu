@@ -19,16 +19,6 @@ namespace {
 
 constexpr int kStages = 3;
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
-  const int bytes = ok ? 16 : 0;  // 0: the 16 bytes are filled with zeros, src is not read
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // A warp's walk over its row blocks: for each of its token groups the slice's
 // head blocks of Q, then of K. `in` and `g` point at this lane's first columns.
 template <typename T>

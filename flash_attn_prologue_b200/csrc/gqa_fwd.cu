@@ -8,18 +8,17 @@
 // Bound by HBM: every row is read and written once, the tables once a token.
 // A lane owns one chunk pair of a row (rotation partners in one lane) and a
 // warp owns a token group: HS heads x TP tokens at a time, the token's sin/cos
-// kept in registers while it walks the heads of Q, K and V; a few row blocks are
-// loaded before the first is used.
+// kept in registers while it walks the heads of Q, K and V. Its loads go through
+// a ring in shared memory: each lane copies its own chunks with cp.async,
+// kStages - 1 row blocks ahead, and reads back only what it copied.
 #include "gqa_rows.cuh"
 
 namespace flash_prologue {
 namespace {
 
-// Row blocks whose loads are in flight together: 4 of a 16-bit type (65,536
-// tokens x 40 heads x 128: forward 25 us faster than with 2), 2 of FP32 (8,188
-// tokens x 34 heads x 128: 3 us faster than 4, which leave two CTAs an SM).
-template <typename T>
-constexpr int kAheadOf = sizeof(T) == 4 ? 2 : 4;
+// Slots of the ring. 65,536 tokens x 40 heads x 128 BF16, forward and backward:
+// 553 us with the ring, 569 with four row blocks loaded into registers at a time.
+constexpr int kStages = 4;
 
 // Request of packed token `u`: the last b with cu[b] <= u (requests without
 // new tokens share a start with the next one).
@@ -33,11 +32,15 @@ __device__ __forceinline__ int request_of(const int32_t* cu, int batch, int64_t 
 }
 
 template <typename T, int D, bool VEC>
-__global__ void __launch_bounds__(kThreads) gqa_fwd_kernel(const GqaFwdArgs a) {
+__global__ void __launch_bounds__(kThreads, 3) gqa_fwd_kernel(const GqaFwdArgs a) {
   constexpr int L = D / 16;
   constexpr int HALF = D / 2;
-  constexpr int kAhead = kAheadOf<T>;
+  using C = Columns<T, D>;
+  constexpr int kStageBytes = VEC ? 2 * C::kPieces * 512 : 0;  // x1, x2 of 32 lanes
+  extern __shared__ __align__(16) unsigned char smem_raw[];
   const int lane = threadIdx.x & 31;
+  unsigned char* ring = smem_raw + (threadIdx.x >> 5) * kStages * kStageBytes + lane * 16;
+  const uint32_t ring_u = smem_u32(ring);
   const int slot = lane / L;
   const int j0 = Columns<T, D>::first(lane % L);
   const int HS = 1 << a.p.log2_hs;
@@ -46,6 +49,63 @@ __global__ void __launch_bounds__(kThreads) gqa_fwd_kernel(const GqaFwdArgs a) {
   // Items, tokens and rows are counted in 32 bits (the host checks): fewer registers and no 64-bit division.
   const int items = (int)(a.p.groups * a.p.slices), warps = gridDim.x * kWarps, tokens = (int)(a.B * a.N), N = (int)a.N;
   const bool paged = a.paged.page_table != nullptr;
+  const int q_iters = a.p.iters[0], qk_iters = q_iters + a.p.iters[1], all_iters = qk_iters + a.p.iters[2];
+
+  // The loads' walk over the warp's row blocks: for each of its token groups the
+  // slice's head blocks of Q, K and V. `pre_in` points at this lane's first columns.
+  int pre_item = blockIdx.x * kWarps + (threadIdx.x >> 5), pre_i = 0, pre_i1 = 0, pre_b = 0, pre_n = 0;
+  bool pre_there = false;
+  const T* pre_in = nullptr;
+  const auto pre_at = [&](int t, int it) {
+    pre_in = static_cast<const T*>(a.x[t]) + pre_b * a.sx[t].b + (it * HS + hslot) * a.sx[t].h + pre_n * a.sx[t].n + j0;
+  };
+  const auto pre_enter = [&]() {
+    if (pre_item >= items) return;
+    const int group = a.p.slices == 1 ? pre_item : pre_item / a.p.slices;
+    pre_i = (pre_item - group * a.p.slices) * a.p.per_slice;
+    pre_i1 = min(pre_i + a.p.per_slice, all_iters);
+    const int token = group * TP + tslot;
+    pre_there = token < tokens;  // the pointer stays at a token that exists
+    pre_b = 0;
+    pre_n = pre_there ? token : 0;
+    if (a.B > 1) {
+      pre_b = pre_n / N;
+      pre_n -= pre_b * N;
+    }
+    if (pre_i < q_iters) pre_at(0, pre_i);
+    else if (pre_i < qk_iters) pre_at(1, pre_i - q_iters);
+    else pre_at(2, pre_i - qk_iters);
+  };
+  const auto prefetch = [&](int stage) {
+    if constexpr (VEC) {
+      if (pre_item < items) {
+        const uint32_t dst = ring_u + stage * kStageBytes;
+#pragma unroll
+        for (int q = 0; q < C::kPieces; ++q) {
+          cp_async16(dst + q * 512, pre_in + q * C::kApart, pre_there);
+          cp_async16(dst + (C::kPieces + q) * 512, pre_in + HALF + q * C::kApart, pre_there);
+        }
+        ++pre_i;
+        if (pre_i == pre_i1) {
+          pre_item += warps;
+          pre_enter();
+        } else if (pre_i == q_iters) {
+          pre_at(1, 0);
+        } else if (pre_i == qk_iters) {
+          pre_at(2, 0);
+        } else {
+          pre_in += HS * (pre_i < q_iters ? a.sx[0].h : pre_i < qk_iters ? a.sx[1].h : a.sx[2].h);
+        }
+      }
+      cp_async_commit();  // an empty group past the end keeps the count
+    }
+  };
+  if constexpr (VEC) {
+    pre_enter();
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) prefetch(s);
+  }
+  int stage = 0;
 
   for (int item = blockIdx.x * kWarps + (threadIdx.x >> 5); item < items; item += warps) {
     const int group = a.p.slices == 1 ? item : item / a.p.slices;
@@ -124,42 +184,45 @@ __global__ void __launch_bounds__(kThreads) gqa_fwd_kernel(const GqaFwdArgs a) {
           for (int j = 0; j < kChunk; ++j) wa[j] = wb[j] = 1.f;
         }
       }
-      for (int it = it0; it < it1; it += kAhead) {
-        Chunk<T> x1[kAhead], x2[kAhead];
-        float e[kAhead];
+      for (int it = it0; it < it1; ++it) {
+        Chunk<T> x1, x2;
+        if constexpr (VEC) {
+          prefetch(stage == 0 ? kStages - 1 : stage - 1);
+          cp_async_wait<kStages - 1>();
+          const uint4* src = reinterpret_cast<const uint4*>(ring + stage * kStageBytes);
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-          if (there && it + k < it1) {
-            load_chunk<T, D, VEC>(x1[k], in);
-            load_chunk<T, D, VEC>(x2[k], in + HALF);
-            e[k] = scales ? __ldg(scales + (it + k) * HS + hslot) : 0.f;
-            in += HS * a.sx[t].h;
-          } else {
-            chunk_zero(x1[k]);
-            chunk_zero(x2[k]);
-            e[k] = 0.f;
+          for (int q = 0; q < C::kPieces; ++q) {
+            const uint4 v0 = src[q * 32], v1 = src[(C::kPieces + q) * 32];
+            x1.w[4 * q] = v0.x; x1.w[4 * q + 1] = v0.y; x1.w[4 * q + 2] = v0.z; x1.w[4 * q + 3] = v0.w;
+            x2.w[4 * q] = v1.x; x2.w[4 * q + 1] = v1.y; x2.w[4 * q + 2] = v1.z; x2.w[4 * q + 3] = v1.w;
+          }
+          if (++stage == kStages) stage = 0;
+        } else if (there) {
+          load_chunk<T, D, false>(x1, in);
+          load_chunk<T, D, false>(x2, in + HALF);
+          in += HS * a.sx[t].h;
+        } else {
+          chunk_zero(x1);
+          chunk_zero(x2);
+        }
+        if (t != 2) {
+          const float r = a.w ? inv_rms<D>(row_sum<L>(lane_sumsq(x1, x2)), a.eps) : 1.f;
+          const float e = scales ? expf(__ldg(scales + it * HS + hslot)) : 1.f;
+          fwd_lane(x1, x2, r, wa, wb, sn, cs, scales != nullptr, e, x1, x2);
+          if (!placed && paged) {  // also where the row holds infinities
+            chunk_zero(x1);
+            chunk_zero(x2);
           }
         }
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-          if (it + k >= it1) break;
-          if (t != 2) {
-            const float r = a.w ? inv_rms<D>(row_sum<L>(lane_sumsq(x1[k], x2[k])), a.eps) : 1.f;
-            fwd_lane(x1[k], x2[k], r, wa, wb, sn, cs, scales != nullptr, scales ? expf(e[k]) : 1.f, x1[k], x2[k]);
-            if (!placed && paged) {  // also where the row holds infinities
-              chunk_zero(x1[k]);
-              chunk_zero(x2[k]);
-            }
-          }
-          if (store) {
-            store_chunk<T, D, VEC>(out, x1[k]);
-            store_chunk<T, D, VEC>(out + HALF, x2[k]);
-          }
-          out += HS * a.sy[t].h;
+        if (store) {
+          store_chunk<T, D, VEC>(out, x1);
+          store_chunk<T, D, VEC>(out + HALF, x2);
         }
+        out += HS * a.sy[t].h;
       }
     }
   }
+  if constexpr (VEC) cp_async_wait<0>();
 }
 
 const void* fwd_kernel_for(int dtype, int D, bool vec) { FLASH_PROLOGUE_GQA_KERNEL(gqa_fwd_kernel) }
@@ -194,11 +257,16 @@ RowsPlan plan_rows(int64_t tokens, int Hq, int Hk, int Hv, int D, bool heads_inn
 cudaError_t launch_gqa_fwd(const GqaFwdArgs& a, int dtype, int D, bool vec, cudaStream_t stream) {
   const void* fn = fwd_kernel_for(dtype, D, vec);
   if (!fn) return cudaErrorInvalidValue;
-  const int64_t grid = persistent_grid(fn, 0, (a.p.groups * a.p.slices + kWarps - 1) / kWarps);
+  const size_t smem = vec ? (size_t)kWarps * kStages * (dtype == 2 ? 2048 : 1024) : 0;
+  if (smem > 48 * 1024) {
+    const cudaError_t err = allow_shared_memory(fn, smem);
+    if (err != cudaSuccess) return err;
+  }
+  const int64_t grid = persistent_grid(fn, smem, (a.p.groups * a.p.slices + kWarps - 1) / kWarps);
   if (grid <= 0) return cudaErrorInvalidConfiguration;
   GqaFwdArgs args = a;
   void* params[] = {&args};
-  return cudaLaunchKernel(fn, dim3((unsigned)grid), dim3(kThreads), params, 0, stream);
+  return cudaLaunchKernel(fn, dim3((unsigned)grid), dim3(kThreads), params, smem, stream);
 }
 
 cudaError_t read_gqa_fwd_device_error(int* value, bool reset) {

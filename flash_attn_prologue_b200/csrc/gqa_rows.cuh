@@ -91,6 +91,17 @@ int64_t gqa_bwd_grid(const RowsPlan& p, int Hq, int D, int dtype, bool vec);
 cudaError_t launch_gqa_bwd(const GqaBwdArgs& a, float* dw, float* ds, int dtype, int D, bool vec,
                            const BwdReduce& red, cudaStream_t stream);
 
+// Copies of 16 bytes that a lane makes into shared memory for itself.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
+  const int bytes = ok ? 16 : 0;  // 0: the 16 bytes are filled with zeros, src is not read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // Rotation row of token (b, n); -1 (and the error word) when it is out of range.
 __device__ __forceinline__ int64_t rotation_row(const GqaTables& t, int64_t b, int64_t n) {
   int64_t pos = n;

@@ -5,24 +5,26 @@
 // Bound by the tensor cores and, as much, by the exponentials: 128 rows x 128
 // keys cost 4 * 128 * 128 * D operations (1,024 cycles of an SM's tensor core
 // at D = 128) and 128 * 128 exponentials (1,024 cycles of its 16 a cycle). So
-// neither may wait for the other: the scores of the next block of 64 keys are
-// computed into a second buffer while the softmax of this one runs, and two
-// CTAs share an SM, each with 256 of its 512 tensor-memory columns (two score
-// buffers, the output), so that two warps a scheduler do softmax all the time.
-// (Blocks of 128 keys in one buffer, softmax and products taking turns within
-// a CTA, measured 101 us where this form takes 82 for ragged chunks of up to
-// 2,000 tokens with a window of 1,024 keys, 16/4 heads x 64.)
+// neither may wait for the other. Keys come in blocks of 64: a block's scores
+// (64 columns of tensor memory) are free as soon as the rows have them in
+// registers, so the next block's scores are computed beside this one's softmax,
+// and the probabilities have two buffers, so the product with V runs beside the
+// next softmax. With the output that is 256 columns of the 512, so two CTAs share
+// an SM and two warps a scheduler do softmax. Ragged chunks of up to 2,000 tokens
+// with a window of 1,024 keys, 16/4 heads x 64 FP16: 81 us; probabilities over
+// the scores they came from, with two buffers for both: 83 us; one such buffer
+// of 128 keys: 101 us.
 //
 // A CTA takes one tile: the rows (query heads x whole tokens) of one key head
 // that fit into 128, and its blocks of keys (or a share of them where there
 // are fewer tiles than the GPU holds; a second kernel adds the shares up).
 //   warps 0-3  one row a thread: scores from tensor memory, running maximum
-//              and sum, probabilities back to tensor memory over the scores
-//              they came from, output to global memory;
-//   warp 4     issues S = Q K^T (both from shared memory) and O += P V (P from
-//              tensor memory, V read transposed from shared memory);
+//              and sum, probabilities to tensor memory, output to global memory;
+//   warp 4     issues S = Q K^T (both from shared memory);
+//   warp 6     issues O += P V (P from tensor memory, V read transposed from
+//              shared memory);
 //   warp 5     TMA loads of K and V, one box of a page a lane;
-//   warps 6-7  clean V in blocks that some row of the tile does not see whole:
+//   warp 7     cleans V in blocks that some row of the tile does not see whole:
 //              zeros for slots outside the tile's keys, and for infinities and
 //              NaNs, which 0 * V would carry into rows that do not see them
 //              (the epilogue adds them to the rows that do).
@@ -45,7 +47,6 @@ constexpr int kTile = 128;             // rows of a tile
 constexpr int kKeys = 64;              // keys of a block
 constexpr int kPrefillThreads = 256;
 constexpr int kRowThreads = 128;
-constexpr int kSCol = 0, kOCol = 128;  // tensor-memory columns: scores / probabilities (two buffers), output
 constexpr int kTmemCols = 256;
 
 template <int D>
@@ -54,13 +55,17 @@ struct Layout {
   static constexpr int kStages = D == 64 ? 4 : 2;  // K and V blocks in flight
   static constexpr int kQ = kTile * D * 2, kQHalf = kTile * 128;      // bytes of the Q tile, of its halves
   static constexpr int kBlock = kKeys * D * 2, kHalf = kKeys * 128;   // of a K or V block
+  // Tensor-memory columns: blocks of scores (two where there is room), two of probabilities, the output.
+  static constexpr int kScores = D == 64 ? 2 : 1;
+  static constexpr int kSCol = 0, kPCol = kScores * kKeys, kOCol = kPCol + kKeys;
+  static_assert(kOCol + D <= kTmemCols, "tensor memory");
   static constexpr size_t kSmem = 1024 + (size_t)kQ + (size_t)kBlock * 2 * kStages;
 };
 
 constexpr int kMaxStages = 4;
 struct Barriers {
-  uint64_t k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages], v_clean[kMaxStages];
-  uint64_t s_full[2], p_full[2], o_done[2], drain;
+  uint64_t k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages];
+  uint64_t s_full[2], s_read[2], p_full[2], o_done[2], clean_ask, v_clean, drain[2];
   uint32_t tmem;
   int bad, wild;
   int64_t sums[kPrefillThreads / 32];
@@ -91,6 +96,34 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       " [%0], [%1, {%2, %3, %4, %5}], [%6];"
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
       : "memory");
+}
+// mbar_wait without the suspend hint, whose try takes twice as long where the
+// phase is complete (102 cycles instead of 51) and wakes later where it is not
+// (a round trip of two warps: 434 cycles instead of 289); bounded by the clock.
+__device__ __forceinline__ bool phase_done(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done != 0;
+}
+__device__ __forceinline__ bool phase_wait(uint64_t* bar, uint32_t parity) {
+  constexpr long long kMostCycles = 8000000000ll;  // about 4 s
+  const uint32_t a = smem_u32(bar);
+  if (phase_done(a, parity)) return true;
+  const long long start = clock64();
+  do {
+    if (phase_done(a, parity)) return true;
+  } while (clock64() - start < kMostCycles);
+  atomicOr(&g_device_error, kDeviceErrorTimeout);
+  return false;
+}
+// One lane of the (whole) warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
 }
 // D[tmem] (+)= A[tmem] * B[smem], issued by one thread.
 __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -182,7 +215,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
   unsigned char* q_s = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* k_s = q_s + L::kQ;
   unsigned char* v_s = k_s + L::kStages * L::kBlock;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (p.splits > 1) start_next_kernel();
   // ---- this CTA's tile: last tiles first (they have the most keys), splits innermost
@@ -270,14 +303,17 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       mbar_init(&bar.k_empty[s], 1);
       mbar_init(&bar.v_full[s], 1);
       mbar_init(&bar.v_empty[s], 1);
-      mbar_init(&bar.v_clean[s], 2);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bar.s_full[b], 1);
+      mbar_init(&bar.s_read[b], kRowThreads / 32);
       mbar_init(&bar.p_full[b], kRowThreads / 32);
       mbar_init(&bar.o_done[b], 1);
     }
-    mbar_init(&bar.drain, 1);
+    mbar_init(&bar.clean_ask, 1);
+    mbar_init(&bar.v_clean, 1);
+    mbar_init(&bar.drain[0], 1);
+    mbar_init(&bar.drain[1], 1);
     bar.bad = too_long;
     bar.wild = 0;
     fence_mbar_init();
@@ -308,45 +344,72 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
   float top = -INFINITY, sum = 0.f;
 
   if (warp >= 4) {
-    if (warp == 4 && lane == 0) {
-      // ---------------- products ----------------
-      constexpr uint32_t idesc_s = idesc_of<T>(kKeys, false), idesc_o = idesc_of<T>(D, true);
+    // The issuing warps walk the blocks whole, with values the compiler knows to be the same
+    // in all lanes, and one lane issues. Each has one product: a warp that issued both, with
+    // its waits, took longer for a block than its softmax does.
+    const int n = __shfl_sync(0xffffffffu, blocks, 0);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    if (warp == 4) {
+      // ---------------- scores ----------------
+      constexpr uint32_t idesc = idesc_of<T>(kKeys, false);
+      const uint64_t q_desc = smem_desc_k_sw128(smem_u32(q_s));
       bool failed = false;
-      auto scores = [&](int j) {
-        const int s = j % L::kStages;
-        if (!mbar_wait(&bar.k_full[s], (j / L::kStages) & 1)) return false;
-        tc_fence_after();
-        const uint32_t k = smem_u32(k_s) + s * L::kBlock, q = smem_u32(q_s);
-#pragma unroll
-        for (int h = 0; h < L::kHalves; ++h) {
-          const uint64_t qd = smem_desc_k_sw128(q + h * L::kQHalf), kd = smem_desc_k_sw128(k + h * L::kHalf);
-#pragma unroll
-          for (int c = 0; c < 4; ++c)  // 16 columns (32 bytes) a step
-            umma_bf16(tmem + kSCol + (j & 1) * kKeys, qd + 2 * c, kd + 2 * c, idesc_s, (h | c) != 0);
+      for (int j = 0; j < n; ++j) {
+        const int s = j % L::kStages, b = j % L::kScores, before = j - L::kScores;
+        // The last scores of this buffer are in the rows' registers, K is here.
+        if (!__all_sync(0xffffffffu, (before < 0 || phase_wait(&bar.s_read[b], (before / L::kScores) & 1)) &&
+                                         phase_wait(&bar.k_full[s], (j / L::kStages) & 1))) {
+          failed = true;
+          break;
         }
-        umma_commit(&bar.k_empty[s]);
-        umma_commit(&bar.s_full[j & 1]);
-        return true;
-      };
-      if (blocks) failed = !scores(0);
-      if (blocks > 1 && !failed) failed = !scores(1);
-      for (int j = 0; j < blocks && !failed; ++j) {
-        const int s = j % L::kStages;
-        if (!mbar_wait(&bar.v_clean[s], (j / L::kStages) & 1)) { failed = true; break; }
-        if (!mbar_wait(&bar.p_full[j & 1], (j >> 1) & 1)) { failed = true; break; }
         tc_fence_after();
-        const uint64_t vd = smem_desc_mn_sw128(smem_u32(v_s) + s * L::kBlock, L::kHalf);
+        const uint64_t k_desc = smem_desc_k_sw128(smem_u32(k_s) + s * L::kBlock);
+        if (elect_one()) {
 #pragma unroll
-        for (int c = 0; c < kKeys / 16; ++c)  // 16 keys a step: 8 columns of P, two 8-row groups of V (2,048 bytes)
-          umma_ts(tmem + kOCol, tmem + kSCol + (j & 1) * kKeys + 8 * c, vd + 128 * c, idesc_o, (j | c) != 0);
-        umma_commit(&bar.v_empty[s]);
-        umma_commit(&bar.o_done[j & 1]);
-        // These scores overwrite the P just read: products of one thread run in the order they were issued in.
-        if (j + 2 < blocks) failed = !scores(j + 2);
+          for (int h = 0; h < L::kHalves; ++h)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)  // 16 columns (32 bytes) a step
+              umma_bf16(tm + L::kSCol + b * kKeys, q_desc + h * (L::kQHalf / 16) + 2 * c,
+                        k_desc + h * (L::kHalf / 16) + 2 * c, idesc, (h | c) != 0);
+          umma_commit(&bar.k_empty[s]);
+          umma_commit(&bar.s_full[b]);
+        }
+        __syncwarp();
       }
       if (failed) {  // tensor memory is not released under products still running
-        umma_commit(&bar.drain);
-        mbar_wait(&bar.drain, 0);
+        if (elect_one()) umma_commit(&bar.drain[0]);
+        phase_wait(&bar.drain[0], 0);
+      }
+    } else if (warp == 6) {
+      // ---------------- output ----------------
+      constexpr uint32_t idesc = idesc_of<T>(D, true);
+      bool failed = false;
+      uint32_t cleaned = 0;
+      for (int j = 0; j < n; ++j) {
+        const int s = j % L::kStages;
+        bool ok = phase_wait(&bar.v_full[s], (j / L::kStages) & 1);
+        const bool partial = partial_block(w, a.window, w.first + j);
+        if (partial && lane == 0) mbar_arrive(&bar.clean_ask);  // cleaned beside the block's softmax
+        ok = ok && (!partial || phase_wait(&bar.v_clean, cleaned & 1)) && phase_wait(&bar.p_full[j & 1], (j >> 1) & 1);
+        cleaned += partial;
+        if (!__all_sync(0xffffffffu, ok)) {
+          failed = true;
+          break;
+        }
+        tc_fence_after();
+        const uint64_t v_desc = smem_desc_mn_sw128(smem_u32(v_s) + s * L::kBlock, L::kHalf);
+        if (elect_one()) {
+#pragma unroll
+          for (int c = 0; c < kKeys / 16; ++c)  // 16 keys a step: 8 columns of P, two 8-row groups of V (2,048 bytes)
+            umma_ts(tm + L::kOCol, tm + L::kPCol + (j & 1) * (kKeys / 2) + 8 * c, v_desc + 128 * c, idesc, (j | c) != 0);
+          umma_commit(&bar.v_empty[s]);
+          umma_commit(&bar.o_done[j & 1]);
+        }
+        __syncwarp();
+      }
+      if (failed) {
+        if (elect_one()) umma_commit(&bar.drain[1]);
+        phase_wait(&bar.drain[1], 0);
       }
     } else if (warp == 5) {
       // ---------------- loads ----------------
@@ -372,7 +435,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       bool ok = true;
       auto load = [&](int j, int page, const CUtensorMap* map, unsigned char* ring, uint64_t* full, uint64_t* empty) {
         const int s = j % L::kStages;
-        if (!__all_sync(0xffffffffu, mbar_wait(&empty[s], ((j / L::kStages) & 1) ^ 1))) return false;
+        if (!__all_sync(0xffffffffu, phase_wait(&empty[s], ((j / L::kStages) & 1) ^ 1))) return false;
         const uint32_t count = __popc(__ballot_sync(0xffffffffu, page >= 0));
         if (lane == 0) mbar_arrive_expect_tx(&full[s], count * box_bytes * L::kHalves);
         __syncwarp();
@@ -397,34 +460,31 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       // No product's arrival on an empty barrier lands after the CTA has gone.
       for (int e = blocks; e < blocks + L::kStages && blocks && ok; ++e) {
         const int s = e % L::kStages;
-        ok = mbar_wait(&bar.k_empty[s], ((e / L::kStages) & 1) ^ 1) && mbar_wait(&bar.v_empty[s], ((e / L::kStages) & 1) ^ 1);
+        ok = phase_wait(&bar.k_empty[s], ((e / L::kStages) & 1) ^ 1) && phase_wait(&bar.v_empty[s], ((e / L::kStages) & 1) ^ 1);
       }
       if (j < blocks) {  // a wait ran out: wait (bounded) for the loads still in flight
         for (int s = 0; s < L::kStages; ++s) {
           for (int e = j; e >= 0 && e > j - L::kStages - 1; --e)
             if (e % L::kStages == s) {
-              mbar_wait(&bar.k_full[s], (e / L::kStages) & 1);
-              mbar_wait(&bar.v_full[s], (e / L::kStages) & 1);
+              phase_wait(&bar.k_full[s], (e / L::kStages) & 1);
+              phase_wait(&bar.v_full[s], (e / L::kStages) & 1);
               break;
             }
         }
       }
-    } else if (warp >= 6) {
+    } else {
       // ---------------- cleaning ----------------
-      const int t = (warp - 6) * 32 + lane;
+      uint32_t asked = 0;
       for (int j = 0; j < blocks; ++j) {
-        // Every block is passed on, so that a barrier's phases are never counted past.
+        if (!partial_block(w, a.window, w.first + j)) continue;
         const int s = j % L::kStages;
-        if (!__all_sync(0xffffffffu, mbar_wait(&bar.v_full[s], (j / L::kStages) & 1))) break;
-        if (!partial_block(w, a.window, w.first + j)) {
-          if (lane == 0) mbar_arrive(&bar.v_clean[s]);
-          continue;
-        }
+        // Asked by the warp that has seen the block arrive.
+        if (!__all_sync(0xffffffffu, phase_wait(&bar.clean_ask, asked++ & 1))) break;
         const int64_t kb = (w.first + j) * kKeys;
         uint4* v = reinterpret_cast<uint4*>(v_s + s * L::kBlock);
         bool wild = false;
 #pragma unroll 4
-        for (int i = t; i < kKeys * D / 8; i += 64) {
+        for (int i = lane; i < kKeys * D / 8; i += 32) {
           const int64_t key = kb + ((i >> 3) & (kKeys - 1));
           uint4 x = v[i];
           if (key < w.lo || key >= w.hi) {
@@ -447,7 +507,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
         if (wild) bar.wild = 1;
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.v_clean[s]);
+        if (lane == 0) mbar_arrive(&bar.v_clean);
       }
     }
   } else {
@@ -460,15 +520,17 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
     const float scale = a.scale_log2;
     bool ok = true;
     for (int j = 0; j < blocks; ++j) {
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait(&bar.s_full[j & 1], (j >> 1) & 1)))) break;
+      if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.s_full[j % L::kScores], (j / L::kScores) & 1)))) break;
       tc_fence_after();
-      const uint32_t scores = mine + kSCol + (j & 1) * kKeys;
       uint32_t s[2][32];
-      tmem_ld32(scores, s[0]);
-      tmem_ld32(scores + 32, s[1]);
+      tmem_ld32(mine + L::kSCol + j % L::kScores * kKeys, s[0]);
+      tmem_ld32(mine + L::kSCol + j % L::kScores * kKeys + 32, s[1]);
       tmem_wait_ld();
       pin(s[0]);
       pin(s[1]);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar.s_read[j % L::kScores]);
       const int64_t block = w.first + j;
       if (partial_block(w, a.window, block)) {
         const int64_t kb = block * kKeys;
@@ -495,8 +557,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       if (fresh) top = now;
       const bool move = !fresh && (now - top) * scale > 8.f;
       if (__any_sync(0xffffffffu, move)) {
-        // O has to be at rest: the last product with V done, the next one waits for this block's P.
-        if (!(ok = __all_sync(0xffffffffu, mbar_wait(&bar.o_done[(j - 1) & 1], ((j - 1) >> 1) & 1)))) break;
+        // O has to be at rest: the last product with V done; the next one waits for this block's P.
+        if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.o_done[(j - 1) & 1], ((j - 1) >> 1) & 1)))) break;
         tc_fence_after();
         const float f = move ? exp2_approx((top - now) * scale) : 1.f;
         sum *= f;
@@ -504,12 +566,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
 #pragma unroll 1
         for (int c = 0; c < D / 16; ++c) {
           uint32_t o[16];
-          tmem_ld16(mine + kOCol + 16 * c, o);
+          tmem_ld16(mine + L::kOCol + 16 * c, o);
           tmem_wait_ld();
           pin(o);
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-          tmem_st16(mine + kOCol + 16 * c, o);
+          tmem_st16(mine + L::kOCol + 16 * c, o);
         }
       }
       const float from = top == -INFINITY ? 0.f : top * scale;
@@ -525,7 +587,10 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
         add[i & 3] = __fadd2_rn(add[i & 3], x);
         out[i] = pack2<T>(x.x, x.y);
       }
-      tmem_st32(scores, out);
+      // The buffer's last P has to be used up.
+      if (j >= 2 && !(ok = __all_sync(0xffffffffu, phase_wait(&bar.o_done[j & 1], ((j - 2) >> 1) & 1)))) break;
+      tc_fence_after();
+      tmem_st32(mine + L::kPCol + (j & 1) * (kKeys / 2), out);
       const float2 both = __fadd2_rn(__fadd2_rn(add[0], add[1]), __fadd2_rn(add[2], add[3]));
       sum += both.x + both.y;
       tmem_wait_st();
@@ -533,7 +598,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.p_full[j & 1]);
     }
-    if (blocks && ok) mbar_wait(&bar.o_done[(blocks - 1) & 1], ((blocks - 1) >> 1) & 1);
+    if (blocks && ok) phase_wait(&bar.o_done[(blocks - 1) & 1], ((blocks - 1) >> 1) & 1);
   }
   __syncthreads();  // `bad` and `wild` are final
 
@@ -556,7 +621,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       uint32_t o[32];
       __syncwarp();
       if (blocks) {
-        tmem_ld32(mine + kOCol + 32 * c, o);
+        tmem_ld32(mine + L::kOCol + 32 * c, o);
         tmem_wait_ld();
         pin(o);
       } else {
