@@ -14,12 +14,12 @@ struct AttentionArgs {
   const void* v;
   int64_t k_page, k_slot, k_head, v_page, v_slot, v_head;  // elements
   PagedTarget pages;
-  int64_t tokens;
+  int tokens;
   int heads, kv_heads, group;  // group = heads / kv_heads
   float scale_log2;          // softmax_scale * log2(e)
-  int64_t window;            // keys a row sees at most; 0: all
+  int window;                // keys a row sees at most; 0: all
   void* workspace;
-  int64_t max_keys;          // pages.max_pages * page_size
+  int max_keys;              // pages.max_pages * page_size
 };
 
 // Lets the next kernel of the stream be placed (see launch_following), and
@@ -29,29 +29,27 @@ __device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("gridd
 
 // One request as the kernels see it: its new tokens and the keys it may reach.
 struct Request {
-  int64_t first;   // packed index of its first new token
-  int64_t news;    // new tokens
-  int64_t total;   // tokens in the cache
+  int first;   // packed index of its first new token
+  int news;    // new tokens
+  int total;   // tokens in the cache
 };
 
 // Sizes are clamped to what the tensors hold, so wrong ones cannot lead outside
 // them. r == batch is the padding behind the last request: tokens without keys.
-__device__ __forceinline__ Request request_at(const PagedTarget& p, int64_t tokens, int64_t max_keys, int r,
-                                              bool* bad) {
+// The host keeps tokens x heads below 2^31 and max_keys below 2^30.
+__device__ __forceinline__ Request request_at(const PagedTarget& p, int tokens, int max_keys, int r, bool* too_long) {
   Request q;
+  const int total = r < p.batch ? __ldg(p.seq_lens + r) : 0;
   if (p.cu_seqlens) {
-    int64_t a = __ldg(p.cu_seqlens + r), b = r < p.batch ? (int64_t)__ldg(p.cu_seqlens + r + 1) : tokens;
-    a = a < 0 ? 0 : (a > tokens ? tokens : a);
-    b = b < a ? a : (b > tokens ? tokens : b);
-    q.first = a;
-    q.news = b - a;
+    const int a = __ldg(p.cu_seqlens + r), b = r < p.batch ? __ldg(p.cu_seqlens + r + 1) : tokens;
+    q.first = min(max(a, 0), tokens);
+    q.news = min(max(b, q.first), tokens) - q.first;
   } else {
     q.first = r;
     q.news = r < p.batch ? 1 : 0;
   }
-  int64_t total = r < p.batch ? (int64_t)__ldg(p.seq_lens + r) : 0;
-  *bad = total > max_keys;
-  q.total = total < 0 ? 0 : (total > max_keys ? max_keys : total);
+  *too_long = total > max_keys;
+  q.total = min(max(total, 0), max_keys);
   return q;
 }
 

@@ -97,14 +97,14 @@ int flash_prologue_paged_attention(const flash_prologue_attention_args* a, void*
   g.v_slot = c.v_slot;
   g.v_head = c.v_head;
   g.pages = paged_target(c);
-  g.tokens = a->tokens;
+  g.tokens = (int)a->tokens;
   g.heads = (int)a->Hq;
   g.kv_heads = (int)a->Hk;
   g.group = g.heads / g.kv_heads;
   g.scale_log2 = (float)(a->softmax_scale * 1.4426950408889634);
   g.workspace = a->workspace;
-  g.max_keys = c.max_pages * c.page_size;
-  g.window = a->window < g.max_keys ? a->window : 0;  // as long as any request: all keys
+  g.max_keys = (int)(c.max_pages * c.page_size);
+  g.window = a->window < g.max_keys ? (int)a->window : 0;  // as long as any request: all keys
   if (use_prefill(a)) {
     cudaError_t err = cudaSuccess;
     if (launch_paged_prefill(g, plan_of(a, sms), (int)a->dtype, (int)a->D, c.page_size,

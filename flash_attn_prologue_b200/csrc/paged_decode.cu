@@ -95,17 +95,16 @@ __device__ __forceinline__ T from_float(float v) {
 }
 
 // Blocks of keys from the first that the request's first new token sees to its last key.
-__device__ __forceinline__ int64_t first_key(const Request& q, int64_t window) {
-  const int64_t at = q.total - q.news - window + 1;
-  return window && at > 0 ? at : 0;
+__device__ __forceinline__ int first_key(const Request& q, int window) {
+  return window ? max(q.total - q.news - window + 1, 0) : 0;
 }
-__device__ __forceinline__ int64_t blocks_of(const Request& q, int64_t window) {
-  const int64_t lo = first_key(q, window) / kBlockKeys, hi = (q.total + kBlockKeys - 1) / kBlockKeys;
-  return hi > lo ? hi - lo : 1;  // one at least: it writes the zeros of rows without keys
+__device__ __forceinline__ int blocks_of(const Request& q, int window) {
+  const int lo = first_key(q, window) / kBlockKeys, hi = (q.total + kBlockKeys - 1) / kBlockKeys;
+  return max(hi - lo, 1);  // one at least: it writes the zeros of rows without keys
 }
 __device__ __forceinline__ int64_t units_of(const Request& q, const AttentionArgs& a) {
-  const int64_t tiles = (q.news * a.group + kRows - 1) / kRows;
-  return tiles * a.kv_heads * blocks_of(q, a.window);
+  const int tiles = (q.news * a.group + kRows - 1) / kRows;
+  return (int64_t)tiles * a.kv_heads * blocks_of(q, a.window);
 }
 
 // Sum over the CTA (every thread gets it).
@@ -571,7 +570,7 @@ cudaError_t launch(const AttentionArgs& a, cudaStream_t stream) {
   cudaError_t err = allow_shared_memory(fn, smem);
   if (err != cudaSuccess) return err;
   // Never more CTAs than there can be units.
-  const int64_t tiles = a.tokens * a.group / kRows + (a.tokens < a.pages.batch ? a.tokens : a.pages.batch) + 1;
+  const int64_t tiles = (int64_t)a.tokens * a.group / kRows + (a.tokens < a.pages.batch ? a.tokens : a.pages.batch) + 1;
   const int64_t blocks = a.max_keys / kBlockKeys + 1;
   int dev = 0, sms = 0;
   if ((err = cudaGetDevice(&dev)) != cudaSuccess ||

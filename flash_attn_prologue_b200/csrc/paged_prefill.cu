@@ -68,22 +68,22 @@ struct Barriers {
   uint64_t s_full[2], s_read[2], p_full[2], o_done[2], clean_ask, v_clean, drain[2];
   uint32_t tmem;
   int bad, wild;
-  int64_t sums[kPrefillThreads / 32];
-  int64_t found[2];
+  int sums[kPrefillThreads / 32];
+  int found, found_tile;  // request of the CTA's tile (-1: none), its tile of it
+  Request request;
 };
 
 struct Tile {  // what the join needs to know of a tile
-  int64_t token0;
-  int rows, kv_head, parts;
+  int token0, rows, kv_head, parts;
 };
 
 struct PrefillArgs {
   AttentionArgs a;
   int tile_tokens;       // whole tokens of a tile: 128 / group
   int splits;            // shares that the blocks of the last items may be cut into
-  int64_t whole_items;   // items (tile, key head) before those
+  int whole_items;       // items (tile, key head) before those
   int box_rows;          // keys of a TMA box: page_size, at most 64
-  int64_t tiles;         // tiles the grid has room for, all requests
+  int tiles;             // tiles the grid has room for, all requests
   float* part_out;       // [cut items * splits][128][D]
   float* part_stat;      // [...][128][2]
   Tile* joins;           // [cut items]
@@ -190,17 +190,16 @@ struct Work {
   Request q;
   int r;
   int head;
-  int64_t tile;         // of the request
-  int64_t token0;       // first token of the tile, of the request's new ones
-  int rows;             // valid rows
-  int64_t pos0, pos1;   // positions of the first and last token
-  int64_t lo, hi;       // keys that some row sees
-  int64_t first, last;  // this split's blocks (of 64 keys)
-  int parts;            // splits that have blocks
+  int token0;       // first token of the tile, of the request's new ones
+  int rows;         // valid rows
+  int pos0, pos1;   // positions of the first and last token
+  int lo, hi;       // keys that some row sees
+  int first, last;  // this split's blocks (of 64 keys)
+  int parts;        // splits that have blocks
 };
 
-__device__ __forceinline__ bool partial_block(const Work& w, int64_t window, int64_t block) {
-  const int64_t kb = block * kKeys;
+__device__ __forceinline__ bool partial_block(const Work& w, int window, int block) {
+  const int kb = block * kKeys;
   return kb + kKeys - 1 > w.pos0 || (window && kb < w.pos1 - window + 1);
 }
 
@@ -219,84 +218,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
 
   if (p.splits > 1) start_next_kernel();
   // ---- this CTA's tile: last tiles first (they have the most keys), splits innermost
-  const int64_t cut = (int64_t)blockIdx.x - p.whole_items;  // CTAs of the items that are cut
+  const int cut = (int)blockIdx.x - p.whole_items;  // CTAs of the items that are cut
   const int splits = cut < 0 ? 1 : p.splits;
-  const int64_t item = cut < 0 ? (int64_t)blockIdx.x : p.whole_items + cut / p.splits;
-  const int split = cut < 0 ? 0 : (int)(cut % p.splits);
-  const int64_t tile_of_all = p.tiles - 1 - item / a.kv_heads;
+  const int item = cut < 0 ? (int)blockIdx.x : p.whole_items + cut / p.splits;
+  const int split = cut < 0 ? 0 : cut % p.splits;
+  const int tile_of_all = p.tiles - 1 - item / a.kv_heads;
   const int requests = a.pages.batch + (a.pages.cu_seqlens ? 1 : 0);
-  if (threadIdx.x == 0) bar.found[0] = -1;
-  __syncthreads();
-  int64_t before = 0;
-  for (int r0 = 0; r0 < requests; r0 += kPrefillThreads) {
-    const int r = r0 + threadIdx.x;
-    int64_t n = 0;
-    if (r < requests) {
-      bool too_long;
-      const Request q = request_at(a.pages, a.tokens, a.max_keys, r, &too_long);
-      n = (q.news + p.tile_tokens - 1) / p.tile_tokens;
-      if (too_long && n) atomicOr(&g_device_error, kDeviceErrorIndex);
-    }
-    int64_t upto = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += v;
-    }
-    if (lane == 31) bar.sums[warp] = upto;
-    __syncthreads();
-    int64_t start = before + upto - n, all = 0;
-#pragma unroll
-    for (int w = 0; w < kPrefillThreads / 32; ++w) {
-      if (w < warp) start += bar.sums[w];
-      all += bar.sums[w];
-    }
-    if (tile_of_all >= start && tile_of_all < start + n) {
-      bar.found[0] = r;
-      bar.found[1] = tile_of_all - start;
-    }
-    before += all;
-    __syncthreads();
-    if (before > tile_of_all) break;
-  }
-  Tile* join = splits > 1 ? p.joins + (item - p.whole_items) : nullptr;
-  if (bar.found[0] < 0) {  // the grid has room for more tiles than there are
-    if (join && split == 0 && threadIdx.x == 0) join->parts = 0;
-    return;
-  }
-  Work w;
-  w.r = (int)bar.found[0];
-  w.tile = bar.found[1];
-  w.head = (int)(item % a.kv_heads);
-  bool too_long;
-  w.q = request_at(a.pages, a.tokens, a.max_keys, w.r, &too_long);
-  w.token0 = w.tile * p.tile_tokens;
-  const int64_t tokens = min((int64_t)p.tile_tokens, w.q.news - w.token0);
-  w.rows = (int)tokens * a.group;
-  w.pos0 = w.q.total - w.q.news + w.token0;
-  w.pos1 = w.pos0 + tokens - 1;
-  w.hi = w.pos1 + 1 > 0 ? w.pos1 + 1 : 0;
-  w.lo = a.window && w.pos0 - a.window + 1 > 0 ? w.pos0 - a.window + 1 : 0;
-  {
-    const int64_t first = w.lo / kKeys, last = (w.hi + kKeys - 1) / kKeys;
-    const int64_t blocks = last > first ? last - first : 0;
-    // Shares of at least four blocks: a share's fixed cost is about theirs.
-    int64_t share = (blocks + splits - 1) / splits;
-    if (share < 4 && splits > 1) share = 4;
-    w.parts = blocks ? (int)((blocks + share - 1) / share) : 1;
-    w.first = first + split * share;
-    w.last = min(first + blocks, w.first + share);
-  }
-  if (join && split == 0 && threadIdx.x == 0) {
-    join->token0 = w.q.first + w.token0;
-    join->rows = w.rows;
-    join->kv_head = w.head;
-    join->parts = w.parts;
-  }
-  if (split >= w.parts) return;
-  const int blocks = w.last > w.first ? (int)(w.last - w.first) : 0;
-
-  // ---- barriers, tensor memory, Q
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::kStages; ++s) {
       mbar_init(&bar.k_full[s], 1);
@@ -314,13 +241,125 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
     mbar_init(&bar.v_clean, 1);
     mbar_init(&bar.drain[0], 1);
     mbar_init(&bar.drain[1], 1);
-    bar.bad = too_long;
+    bar.found = -1;
+    bar.bad = 0;
     bar.wild = 0;
     fence_mbar_init();
   }
+  int before = 0;
+  for (int r0 = 0; r0 < requests; r0 += kPrefillThreads) {
+    const int r = r0 + threadIdx.x;
+    Request q{0, 0, 0};
+    bool too_long = false;
+    if (r < requests) q = request_at(a.pages, a.tokens, a.max_keys, r, &too_long);
+    const int n = (q.news + p.tile_tokens - 1) / p.tile_tokens;
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 31) bar.sums[warp] = upto;
+    __syncthreads();
+    int start = before + upto - n, all = 0;
+#pragma unroll
+    for (int w = 0; w < kPrefillThreads / 32; ++w) {
+      if (w < warp) start += bar.sums[w];
+      all += bar.sums[w];
+    }
+    if (tile_of_all >= start && tile_of_all < start + n) {
+      bar.found = r;
+      bar.found_tile = tile_of_all - start;
+      bar.request = q;
+      bar.bad = too_long;
+    }
+    before += all;
+    __syncthreads();
+    if (before > tile_of_all) break;
+  }
+  Tile* join = splits > 1 ? p.joins + (item - p.whole_items) : nullptr;
+  if (bar.found < 0) {  // the grid has room for more tiles than there are
+    if (join && split == 0 && threadIdx.x == 0) join->parts = 0;
+    return;
+  }
+  Work w;
+  w.r = bar.found;
+  w.head = item % a.kv_heads;
+  w.q = bar.request;
+  w.token0 = bar.found_tile * p.tile_tokens;
+  const int tokens = min(p.tile_tokens, w.q.news - w.token0);
+  w.rows = tokens * a.group;
+  w.pos0 = w.q.total - w.q.news + w.token0;
+  w.pos1 = w.pos0 + tokens - 1;
+  w.hi = max(w.pos1 + 1, 0);
+  w.lo = a.window ? max(w.pos0 - a.window + 1, 0) : 0;
+  {
+    const int first = w.lo / kKeys, blocks = max((w.hi + kKeys - 1) / kKeys - first, 0);
+    // Shares of at least four blocks: a share's fixed cost is about theirs.
+    int share = blocks;
+    if (splits > 1) share = max((blocks + splits - 1) / splits, 4);
+    w.parts = blocks && splits > 1 ? (blocks + share - 1) / share : 1;
+    w.first = first + split * share;
+    w.last = min(first + blocks, w.first + share);
+  }
+  if (join && split == 0 && threadIdx.x == 0) {
+    join->token0 = w.q.first + w.token0;
+    join->rows = w.rows;
+    join->kv_head = w.head;
+    join->parts = w.parts;
+  }
+  if (split >= w.parts) return;
+  const int blocks = max(w.last - w.first, 0);
+
+  // ---- tensor memory, Q
   if (warp == 4) {
     tmem_alloc(&bar.tmem, kTmemCols);
     tmem_relinquish();
+  }
+  // The loads begin before the other warps have Q in shared memory.
+  const int boxes = kKeys / p.box_rows, in_page = (1 << a.pages.page_log2) - 1;
+  const uint32_t box_bytes = (uint32_t)p.box_rows * 128;
+  // The page of this lane's box of a block, -1 where there is nothing to load.
+  const auto page_of = [&](int j) {
+    int page = -1;
+    if (lane < boxes && j < blocks) {
+      const int key = (w.first + j) * kKeys + lane * p.box_rows;
+      if (key < w.hi && key + p.box_rows > w.lo) {
+        page = __ldg(a.pages.page_table + w.r * a.pages.table_stride + (key >> a.pages.page_log2));
+        if (page < 0 || page >= a.pages.num_pages) {
+          page = -1;
+          bar.bad = 1;
+        }
+      }
+    }
+    return page;
+  };
+  const auto load = [&](int j, int page, const CUtensorMap* map, unsigned char* ring, uint64_t* full) {
+    const int s = j % L::kStages;
+    const uint32_t count = __popc(__ballot_sync(0xffffffffu, page >= 0));
+    if (lane == 0) mbar_arrive_expect_tx(&full[s], count * box_bytes * L::kHalves);
+    __syncwarp();
+    if (page >= 0) {
+      const int key = (w.first + j) * kKeys + lane * p.box_rows;
+      const uint32_t dst = smem_u32(ring) + s * L::kBlock + lane * box_bytes;
+#pragma unroll
+      for (int h = 0; h < L::kHalves; ++h)
+        tma_load_4d(dst + h * L::kHalf, map, h * 64, key & in_page, w.head, page, &full[s]);
+    }
+    __syncwarp();
+  };
+  int next_page = -1;  // of the first block that the loop below loads
+  if (warp == 5) {
+    int page[L::kStages];
+#pragma unroll
+    for (int j = 0; j < L::kStages; ++j) page[j] = page_of(j);
+    next_page = page_of(L::kStages);
+#pragma unroll
+    for (int j = 0; j < L::kStages; ++j)
+      if (j < blocks) {
+        load(j, page[j], &k_map, k_s, bar.k_full);
+        load(j, page[j], &v_map, v_s, bar.v_full);
+      }
   }
   for (int i = threadIdx.x; i < kTile * (D / 8); i += kPrefillThreads) {
     const int row = i / (D / 8), c = i % (D / 8);
@@ -328,7 +367,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
     if (row < w.rows) {
       const int t = row / a.group, g = row - t * a.group;
       v = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (w.q.first + w.token0 + t) * a.q_n +
-                                               (int64_t)(w.head * a.group + g) * a.q_h + c * 8));
+                                               (w.head * a.group + g) * a.q_h + c * 8));
     }
     *reinterpret_cast<uint4*>(q_s + (c >> 3) * L::kQHalf + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
   }
@@ -340,7 +379,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
 
   // Row state (warps 0-3); the row's keys are [see_lo, see_hi].
   const int row = threadIdx.x;
-  int64_t see_hi = -1, see_lo = 0;
+  int see_hi = -1, see_lo = 0;
   float top = -INFINITY, sum = 0.f;
 
   if (warp >= 4) {
@@ -413,49 +452,16 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       }
     } else if (warp == 5) {
       // ---------------- loads ----------------
-      const int boxes = kKeys / p.box_rows;
-      const int32_t* table = a.pages.page_table + (int64_t)w.r * a.pages.table_stride;
-      const int in_page = (1 << a.pages.page_log2) - 1;
-      // The page of this lane's box of a block, -1 where there is nothing to load.
-      auto page_of = [&](int j) {
-        int page = -1;
-        if (lane < boxes && j < blocks) {
-          const int64_t key = (w.first + j) * kKeys + lane * p.box_rows;
-          if (key < w.hi && key + p.box_rows > w.lo) {
-            page = __ldg(table + (key >> a.pages.page_log2));
-            if (page < 0 || page >= a.pages.num_pages) {
-              page = -1;
-              bar.bad = 1;
-            }
-          }
-        }
-        return page;
-      };
-      const uint32_t box_bytes = (uint32_t)p.box_rows * 128;
       bool ok = true;
-      auto load = [&](int j, int page, const CUtensorMap* map, unsigned char* ring, uint64_t* full, uint64_t* empty) {
-        const int s = j % L::kStages;
-        if (!__all_sync(0xffffffffu, phase_wait(&empty[s], ((j / L::kStages) & 1) ^ 1))) return false;
-        const uint32_t count = __popc(__ballot_sync(0xffffffffu, page >= 0));
-        if (lane == 0) mbar_arrive_expect_tx(&full[s], count * box_bytes * L::kHalves);
-        __syncwarp();
-        if (page >= 0) {
-          const int64_t key = (w.first + j) * kKeys + lane * p.box_rows;
-          const uint32_t dst = smem_u32(ring) + s * L::kBlock + lane * box_bytes;
-#pragma unroll
-          for (int h = 0; h < L::kHalves; ++h)
-            tma_load_4d(dst + h * L::kHalf, map, h * 64, (int)(key & in_page), w.head, page, &full[s]);
-        }
-        __syncwarp();
-        return true;
-      };
-      int page = page_of(0);
-      int j = 0;
-      for (; j < blocks && ok; ++j) {
-        const int next = page_of(j + 1);
-        ok = load(j, page, &k_map, k_s, bar.k_full, bar.k_empty) && load(j, page, &v_map, v_s, bar.v_full, bar.v_empty);
+      int j = L::kStages;
+      for (int page = next_page; j < blocks; ++j) {
+        const int s = j % L::kStages, next = page_of(j + 1);
+        const uint32_t parity = ((j / L::kStages) & 1) ^ 1;
+        if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.k_empty[s], parity)))) break;
+        load(j, page, &k_map, k_s, bar.k_full);
+        if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.v_empty[s], parity)))) break;
+        load(j, page, &v_map, v_s, bar.v_full);
         page = next;
-        if (!ok) break;
       }
       // No product's arrival on an empty barrier lands after the CTA has gone.
       for (int e = blocks; e < blocks + L::kStages && blocks && ok; ++e) {
@@ -480,12 +486,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
         const int s = j % L::kStages;
         // Asked by the warp that has seen the block arrive.
         if (!__all_sync(0xffffffffu, phase_wait(&bar.clean_ask, asked++ & 1))) break;
-        const int64_t kb = (w.first + j) * kKeys;
+        const int kb = (w.first + j) * kKeys;
         uint4* v = reinterpret_cast<uint4*>(v_s + s * L::kBlock);
         bool wild = false;
 #pragma unroll 4
         for (int i = lane; i < kKeys * D / 8; i += 32) {
-          const int64_t key = kb + ((i >> 3) & (kKeys - 1));
+          const int key = kb + ((i >> 3) & (kKeys - 1));
           uint4 x = v[i];
           if (key < w.lo || key >= w.hi) {
             v[i] = make_uint4(0, 0, 0, 0);
@@ -531,12 +537,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.s_read[j % L::kScores]);
-      const int64_t block = w.first + j;
+      const int block = w.first + j;
       if (partial_block(w, a.window, block)) {
-        const int64_t kb = block * kKeys;
-        const int64_t hi64 = see_hi - kb, lo64 = see_lo - kb;
-        const int hi = hi64 > kKeys ? kKeys : (hi64 < -1 ? -1 : (int)hi64);
-        const int lo = lo64 > kKeys ? kKeys : (lo64 < 0 ? 0 : (int)lo64);
+        const int hi = see_hi - block * kKeys, lo = see_lo - block * kKeys;
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -611,10 +614,10 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
     if (bad) sum = nan;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const int t = row / a.group, g = row - t * a.group;
-    const int64_t token = w.q.first + w.token0 + t;
+    const int token = w.q.first + w.token0 + t;
     const int h = w.head * a.group + g;
     const bool valid = row < w.rows;
-    const int64_t slot = cut;
+    const int64_t slot = cut;  // of the cut items' shares
     const float top2 = top == -INFINITY ? top : top * a.scale_log2;
 #pragma unroll 1
     for (int c = 0; c < D / 32; ++c) {
@@ -632,9 +635,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
         // The infinities and NaNs taken out of V, added to a row that sees them.
         for (int j = 0; j < blocks; ++j) {
           if (!partial_block(w, a.window, w.first + j)) continue;
-          const int64_t kb = (w.first + j) * kKeys;
-          const int64_t k0 = kb > see_lo ? kb : see_lo, k1 = min(kb + kKeys - 1, see_hi);
-          for (int64_t k = k0; k <= k1; ++k) {
+          const int kb = (w.first + j) * kKeys;
+          for (int k = max(kb, see_lo); k <= min(kb + kKeys - 1, see_hi); ++k) {
             const int32_t* entry = a.pages.page_table + (int64_t)w.r * a.pages.table_stride + (k >> a.pages.page_log2);
             const int64_t page = __ldg(entry);
             if (page < 0 || page >= a.pages.num_pages) continue;
@@ -672,7 +674,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
         p.part_stat[(slot * kTile + row) * 2] = top2;
         p.part_stat[(slot * kTile + row) * 2 + 1] = sum;
       } else if (a.lse) {
-        a.lse[token * a.heads + h] = (top2 + log2f(sum)) * 0.6931471805599453f;
+        a.lse[(int64_t)token * a.heads + h] = (top2 + log2f(sum)) * 0.6931471805599453f;
       }
     }
   }
@@ -715,7 +717,7 @@ __global__ void __launch_bounds__(512) prefill_join_kernel(const PrefillArgs p) 
     if constexpr (std::is_same<T, __half>::value) out[32 * c + lane] = __float2half_rn(x);
     else out[32 * c + lane] = __float2bfloat16_rn(x);
   }
-  if (a.lse && lane == 0) a.lse[(t.token0 + token) * a.heads + h] = (m + log2f(l)) * 0.6931471805599453f;
+  if (a.lse && lane == 0) a.lse[(int64_t)(t.token0 + token) * a.heads + h] = (m + log2f(l)) * 0.6931471805599453f;
 }
 
 // A cache as {D, slots, heads, pages}, a box of 64 columns x box_rows slots.
@@ -784,11 +786,11 @@ bool launch_paged_prefill(const AttentionArgs& a, const PrefillPlan& plan, int d
   p.a = a;
   p.tile_tokens = plan.tile_tokens;
   p.splits = plan.splits;
-  p.whole_items = plan.whole_items;
-  p.tiles = plan.tiles;
+  p.whole_items = (int)plan.whole_items;
+  p.tiles = (int)plan.tiles;
   p.box_rows = page_size < kKeys ? (int)page_size : kKeys;
   const int64_t items = plan.tiles * a.kv_heads;
-  if (items * p.splits * (kTile / 16) >= (int64_t(1) << 31)) return false;
+  if (items * plan.splits * (kTile / 16) >= (int64_t(1) << 31)) return false;
   CUtensorMap k_map, v_map;
   if (!encode_cache(&k_map, a.k, dtype, D, page_size, a.kv_heads, a.pages.num_pages, a.k_slot, a.k_head, a.k_page,
                     p.box_rows) ||
