@@ -31,7 +31,7 @@ constexpr int kNone = -(1 << 30);  // below every relative position
 constexpr int kRing = 3;        // steps of a warp's ring
 
 struct Part {  // an item that a CTA began and others go on with
-  int64_t token0;  // packed index of its first row's request
+  int token0;  // packed index of its first row's request
   int row0, rows;  // rows of the tile that exist
   int kv_head;
   int last;        // CTA that ends it; -1: nothing to join
@@ -154,7 +154,9 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
   if (threadIdx.x == 0) parts[cta].last = -1;
   const int64_t ctas = min((int64_t)gridDim.x, units);  // every one of these has a unit at least
   if (cta >= ctas) return;
-  const int64_t begin = cta * units / ctas, end = (cta + 1) * units / ctas;
+  const bool small = units < (int64_t(1) << 31) / 1024;  // the products below fit 32 bits
+  const int64_t begin = small ? (int)cta * (int)units / (int)ctas : cta * units / ctas;
+  const int64_t end = small ? ((int)cta + 1) * (int)units / (int)ctas : (cta + 1) * units / ctas;
 
   // The request that `begin` falls into: one scan over the requests, a CTA's width at a time.
   int64_t before = 0;
@@ -202,27 +204,27 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
       q = request_at(a.pages, a.tokens, a.max_keys, r, &too_long);
       in_request = q.news ? units_of(q, a) : 0;
     }
-    const int64_t blocks = blocks_of(q, a.window);
-    const int64_t item = (unit - start) / blocks;
-    const int64_t item_start = start + item * blocks;
-    const int64_t b0 = unit - item_start, b1 = min(blocks, end - item_start);
-    const int head = (int)(item % a.kv_heads);
-    const int64_t row0 = item / a.kv_heads * kRows;       // of the request's news * group rows
-    const int rows = (int)min((int64_t)kRows, q.news * a.group - row0);
-    const int64_t base = q.total - q.news;                // position of new token 0
-    const int64_t key0 = first_key(q, a.window) / kBlockKeys * kBlockKeys;
+    const int blocks = blocks_of(q, a.window);
+    const int64_t in = unit - start;
+    const int item = in >> 31 ? (int)(in / blocks) : (int)in / blocks;  // tiles x heads stay below 2^31
+    const int64_t item_start = start + (int64_t)item * blocks;
+    const int b0 = (int)(unit - item_start), b1 = (int)min((int64_t)blocks, end - item_start);
+    const int head = item % a.kv_heads;
+    const int row0 = item / a.kv_heads * kRows;       // of the request's news * group rows
+    const int rows = min(kRows, q.news * a.group - row0);
+    const int base = q.total - q.news;                // position of new token 0
+    const int key0 = first_key(q, a.window) / kBlockKeys * kBlockKeys;
     // Keys that a row of this tile sees.
-    const int64_t hi = base + (row0 + rows - 1) / a.group + 1;
-    int64_t lo = a.window ? base + row0 / a.group - a.window + 1 : 0;
-    if (lo < 0) lo = 0;
+    const int hi = base + (row0 + rows - 1) / a.group + 1;
+    const int lo = a.window ? max(base + row0 / a.group - a.window + 1, 0) : 0;
 
     // The tile's Q as operand fragments: rows lane / 4 and lane / 4 + 8.
     uint32_t qf[D / 16][4];
-    int64_t row_pos[2];
+    int row_pos[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const int row = lane / 4 + s * 8;
-      const int64_t at = row0 + row, i = at / a.group;
+      const int at = row0 + row, i = at / a.group;
       row_pos[s] = row < rows ? base + i : -1;
       const T* p = static_cast<const T*>(a.q) + (q.first + i) * a.q_n +
                    (head * a.group + (at - i * a.group)) * a.q_h + (lane % 4) * 2;
@@ -241,16 +243,16 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
     __syncthreads();
 
     // Positions relative to this warp's first key, in 32 bits (a request has fewer than 2^30 keys).
-    const int steps = (int)(b1 - b0);
-    const int64_t warp_key = key0 + b0 * kBlockKeys + warp * kWarpKeys;
-    const int key_lo = (int)(lo - warp_key), key_hi = (int)(hi - warp_key);
-    const int all_lo = a.window ? (int)(base + (row0 + rows - 1) / a.group - a.window + 1 - warp_key) : kNone;
-    const int all_hi = (int)(base + row0 / a.group - warp_key);  // every row sees keys all_lo .. all_hi
+    const int steps = b1 - b0;
+    const int warp_key = key0 + b0 * kBlockKeys + warp * kWarpKeys;
+    const int key_lo = lo - warp_key, key_hi = hi - warp_key;
+    const int all_lo = a.window ? base + (row0 + rows - 1) / a.group - a.window + 1 - warp_key : kNone;
+    const int all_hi = base + row0 / a.group - warp_key;  // every row sees keys all_lo .. all_hi
     int see_lo[2], see_hi[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      see_hi[e] = row_pos[e] < 0 ? kNone : (int)(row_pos[e] - warp_key);
-      see_lo[e] = a.window ? (int)(row_pos[e] - a.window + 1 - warp_key) : kNone;
+      see_hi[e] = row_pos[e] < 0 ? kNone : row_pos[e] - warp_key;
+      see_lo[e] = a.window ? row_pos[e] - a.window + 1 - warp_key : kNone;
     }
     const int32_t* table = a.pages.page_table + (int64_t)r * a.pages.table_stride;
     const int in_page = (1 << a.pages.page_log2) - 1;
@@ -284,7 +286,7 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
         const bool full = key >= key_lo && key + kWarpKeys <= key_hi && page[0] >= 0 && page[1] >= 0;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          const int64_t slot = (int)(warp_key + key + s * 8) & in_page;
+          const int slot = (warp_key + key + s * 8) & in_page;
           const T* kp = static_cast<const T*>(a.k);
           const T* vp = static_cast<const T*>(a.v);
           if (page[s] >= 0) {
@@ -452,12 +454,12 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
       }
       if (bad_page) l = o = __int_as_float(0x7fc00000);
       if (whole) {
-        const int64_t at = row0 + row, token = at / a.group;
-        const int h = head * a.group + (int)(at - token * a.group);
+        const int at = row0 + row, token = at / a.group;
+        const int h = head * a.group + (at - token * a.group);
         static_cast<T*>(a.out)[(q.first + token) * a.out_n + h * a.out_h + col] =
             from_float<T>(l == 0.f ? 0.f : o / l);
         if (a.lse && col == 0)
-          a.lse[(q.first + token) * a.heads + h] = (m + log2f(l)) * 0.6931471805599453f;
+          a.lse[(int64_t)(q.first + token) * a.heads + h] = (m + log2f(l)) * 0.6931471805599453f;
       } else {
         part_out[(slot * kRows + row) * D + col] = o;
         if (col == 0) {
@@ -469,7 +471,7 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
     if (threadIdx.x == 0 && b0 == 0 && b1 < blocks) {
       Part p;
       p.token0 = q.first;
-      p.row0 = (int)row0;
+      p.row0 = row0;
       p.rows = rows;
       p.kv_head = head;
       p.last = (int)(((item_start + blocks) * ctas - 1) / units);
@@ -555,10 +557,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Atten
     v += e * joined[w][col];
     l += e * sums[w];
   }
-  const int64_t at = p.row0 + row, token = at / a.group;
-  const int h = p.kv_head * a.group + (int)(at - token * a.group);
+  const int at = p.row0 + row, token = at / a.group;
+  const int h = p.kv_head * a.group + (at - token * a.group);
   static_cast<T*>(a.out)[(p.token0 + token) * a.out_n + h * a.out_h + col] = from_float<T>(l == 0.f ? 0.f : v / l);
-  if (a.lse && col == 0) a.lse[(p.token0 + token) * a.heads + h] = (m + log2f(l)) * 0.6931471805599453f;
+  if (a.lse && col == 0) a.lse[(int64_t)(p.token0 + token) * a.heads + h] = (m + log2f(l)) * 0.6931471805599453f;
 }
 
 int64_t most_ctas(int D, int sms) { return (int64_t)sms * (D == 64 ? 4 : 2); }
