@@ -19,6 +19,7 @@ struct AttentionArgs {
   float scale_log2;          // softmax_scale * log2(e)
   int window;                // keys a row sees at most; 0: all
   void* workspace;
+  int whole;                 // single-token kernel: items are not split (set at launch)
   int max_keys;              // pages.max_pages * page_size
 };
 
@@ -53,13 +54,14 @@ __device__ __forceinline__ Request request_at(const PagedTarget& p, int tokens, 
   return q;
 }
 
+// Workspace bytes that cover every call of the kernel on a device of `sms` SMs.
 size_t paged_decode_workspace(int D, int sms);
+size_t paged_prefill_workspace(int D, int sms);
 struct PrefillPlan {
   int tile_tokens;   // whole tokens of a 128-row tile
   int splits;        // shares of the keys of the items behind whole_items
   int64_t whole_items;
   int64_t tiles;     // tiles there can be, all requests
-  size_t workspace;  // bytes; 0 without shares
 };
 PrefillPlan plan_paged_prefill(int64_t tokens, int64_t batch, bool ragged, int64_t kv_heads, int64_t group, int D,
                                int64_t max_keys, int64_t window, int sms);

@@ -37,17 +37,8 @@ bool use_prefill(const flash_prologue_attention_args* a) {
   return a->tokens * group > 16 * a->cache.batch && group <= 128 && a->softmax_scale > 0;
 }
 
-PrefillPlan plan_of(const flash_prologue_attention_args* a, int sms) {
-  const flash_prologue_cache& c = a->cache;
-  return plan_paged_prefill(a->tokens, c.batch, c.cu_seqlens != nullptr, a->Hk, a->Hq / a->Hk, (int)a->D,
-                            c.max_pages * c.page_size, a->window, sms);
-}
-
-// Room for either kernel: the tiled one gives way to the other where the cache has no tensor map.
-size_t workspace_of(const flash_prologue_attention_args* a, int sms) {
-  const size_t decode = paged_decode_workspace((int)a->D, sms);
-  if (!use_prefill(a)) return decode;
-  const size_t prefill = plan_of(a, sms).workspace;
+size_t workspace_of(int64_t D, int sms) {
+  const size_t decode = paged_decode_workspace((int)D, sms), prefill = paged_prefill_workspace((int)D, sms);
   return prefill > decode ? prefill : decode;
 }
 
@@ -55,14 +46,13 @@ size_t workspace_of(const flash_prologue_attention_args* a, int sms) {
 
 extern "C" {
 
-int flash_prologue_paged_attention_workspace_size(const flash_prologue_attention_args* a, size_t* bytes) {
-  if (!a || !bytes) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
+int flash_prologue_paged_attention_workspace_size(int64_t D, size_t* bytes) {
+  if (!bytes) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
   *bytes = 0;
-  const int st = size_checks(a);
-  if (st != FLASH_PROLOGUE_OK || a->tokens == 0 || a->Hq == 0) return st;
+  if (D != 64 && D != 128) return FLASH_PROLOGUE_ERR_UNSUPPORTED;
   const int sms = device_sms();
   if (sms <= 0) return FLASH_PROLOGUE_ERR_CUDA;
-  *bytes = workspace_of(a, sms);
+  *bytes = workspace_of(D, sms);
   return FLASH_PROLOGUE_OK;
 }
 
@@ -78,7 +68,7 @@ int flash_prologue_paged_attention(const flash_prologue_attention_args* a, void*
   const int sms = device_sms();
   if (sms <= 0) return FLASH_PROLOGUE_ERR_CUDA;
   if (!a->workspace || (reinterpret_cast<uintptr_t>(a->workspace) & 15) ||
-      a->workspace_bytes < (int64_t)workspace_of(a, sms))
+      a->workspace_bytes < (int64_t)workspace_of(a->D, sms))
     return FLASH_PROLOGUE_ERR_WORKSPACE;
   AttentionArgs g{};
   g.q = a->q.data;
@@ -106,8 +96,10 @@ int flash_prologue_paged_attention(const flash_prologue_attention_args* a, void*
   g.max_keys = (int)(c.max_pages * c.page_size);
   g.window = a->window < g.max_keys ? (int)a->window : 0;  // as long as any request: all keys
   if (use_prefill(a)) {
+    const PrefillPlan plan = plan_paged_prefill(a->tokens, c.batch, c.cu_seqlens != nullptr, a->Hk, g.group, (int)a->D,
+                                                g.max_keys, g.window, sms);
     cudaError_t err = cudaSuccess;
-    if (launch_paged_prefill(g, plan_of(a, sms), (int)a->dtype, (int)a->D, c.page_size,
+    if (launch_paged_prefill(g, plan, (int)a->dtype, (int)a->D, c.page_size,
                              static_cast<cudaStream_t>(stream), &err))
       return err == cudaSuccess ? FLASH_PROLOGUE_OK : FLASH_PROLOGUE_ERR_CUDA;
   }

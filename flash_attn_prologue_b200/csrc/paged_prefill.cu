@@ -775,9 +775,12 @@ PrefillPlan plan_paged_prefill(int64_t tokens, int64_t batch, bool ragged, int64
     if (splits > 1) p.splits = (int)splits;
   }
   if (p.splits == 1) p.whole_items = items;
-  else
-    p.workspace = (size_t)(cut * p.splits) * kTile * (size_t)(D + 2) * sizeof(float) + (size_t)cut * sizeof(Tile);
   return p;
+}
+
+// At most one share a CTA that the device holds.
+size_t paged_prefill_workspace(int D, int sms) {
+  return (size_t)(2 * sms) * (kTile * (size_t)(D + 2) * sizeof(float) + sizeof(Tile));
 }
 
 bool launch_paged_prefill(const AttentionArgs& a, const PrefillPlan& plan, int dtype, int D, int64_t page_size,

@@ -42,17 +42,18 @@ def check_rows(q, k, rmsnorm_weight, scales, sin, cos, eps):
         raise ValueError(f"query heads must be a multiple of the key heads and at most {MAX_HEADS}")
     if not 0 < eps < math.inf:
         raise ValueError("eps must be finite and positive")
+    float32 = torch.float32
     device = q.device
     shared = k.device == device and sin.device == device and cos.device == device
-    fp32 = sin.dtype == torch.float32 and cos.dtype == torch.float32
+    fp32 = sin.dtype is float32 and cos.dtype is float32
     if rmsnorm_weight is not None:
         if rmsnorm_weight.shape != (2, 1, d):
             raise ValueError("weight must be [2,1,D]")
-        shared, fp32 = shared and rmsnorm_weight.device == device, fp32 and rmsnorm_weight.dtype == torch.float32
+        shared, fp32 = shared and rmsnorm_weight.device == device, fp32 and rmsnorm_weight.dtype is float32
     if scales is not None:
         if scales.shape != (hq, 1, 1):
             raise ValueError("log-scales must be [Hq,1,1]")
-        shared, fp32 = shared and scales.device == device, fp32 and scales.dtype == torch.float32
+        shared, fp32 = shared and scales.device == device, fp32 and scales.dtype is float32
     if sin.ndim != 2 or sin.shape != cos.shape or sin.shape[1] != d // 2:
         raise ValueError("sin/cos must be matching tables [positions, D/2]")
     if not fp32:
@@ -87,19 +88,14 @@ def eager(*tensors) -> bool:
     return _plain_eager()
 
 
-def on_device(t):
-    """A guard that makes t's device current, or None where it is already."""
-    return None if t.get_device() == torch._C._cuda_getDevice() else _DeviceGuard(t.device)
-
-
-def call_library(name, args, like):
-    """Calls entry point ``name`` on the current stream of ``like``'s device."""
-    guard = on_device(like)
-    if guard is None:
-        status = getattr(_lib.load(), name)(args, _lib.stream_of(like.device))
+def call_library(name, args, device):
+    """Calls entry point ``name`` on ``device``'s current stream, with the device current."""
+    function = getattr(_lib.load(), name)
+    if device.index == torch._C._cuda_getDevice():
+        status = function(args, _lib.stream_of(device))
     else:
-        with guard:
-            status = getattr(_lib.load(), name)(args, _lib.stream_of(like.device))
+        with _DeviceGuard(device):
+            status = function(args, _lib.stream_of(device))
     if status:
         _lib.check(status, name)
 
@@ -138,7 +134,7 @@ def _call(name, q, k, w, s, sin, cos, positions, eps, rows, grads=(0, 0), worksp
     args = _lib.GQA_ARGS.pack(
         *rows_of(q), *rows_of(k), *rows, w.data_ptr(), s.data_ptr(), *rotation_of(sin, cos), *where, *grads,
         *workspace, *peers, B, N, q.shape[1], k.shape[1], q.shape[-1], _lib.DTYPE_CODES[q.dtype], eps)
-    call_library(name, args, q)
+    call_library(name, args, q.device)
 
 
 def _in_place_rows(t):

@@ -21,44 +21,48 @@ from .fused_epilogue import _DeviceGuard
 from .gqa import MAX_HEADS, call_library, check_rows, eager, flat_fp32, readable, rotation_of, rows_of
 
 
-def _check_cache(q, heads, k_cache, v_cache, page_table, seq_lens, cu_seqlens):
-    """The cache and its tables, for packed rows q [T, H, D] with ``heads`` key heads."""
+def _checked_cache(q, heads, k_cache, v_cache, page_table, seq_lens, cu_seqlens):
+    """flash_prologue_cache of the cache and its tables, once they fit the packed rows
+    q [T, H, D] with ``heads`` key heads."""
     ks, dtype, device = k_cache.shape, q.dtype, q.device
     if len(ks) != 4 or v_cache.shape != ks or ks[3] != q.shape[2]:
         raise ValueError("caches must be matching [pages, page_size, Hk, D] tensors")
-    page_size = ks[1]
+    pages, page_size, kv_heads, _ = ks
     if page_size < 8 or page_size & (page_size - 1):
         raise ValueError("page_size must be a power of two, at least 8")
-    if ks[2] != heads:
+    if kv_heads != heads:
         raise ValueError("caches and rows must have the same key heads")
-    if k_cache.dtype != dtype or v_cache.dtype != dtype:
+    if k_cache.dtype is not dtype or v_cache.dtype is not dtype:
         raise ValueError("caches and rows must share a dtype")
-    if k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
+    a, b = k_cache.stride(), v_cache.stride()
+    if a[3] != 1 or b[3] != 1:
         raise ValueError("caches must be contiguous along D")
-    table = page_table.shape
+    table, rows = page_table.shape, page_table.stride()
     if len(table) != 2 or seq_lens.shape != table[:1]:
         raise ValueError("page_table must be [B, max_pages] and seq_lens [B]")
+    batch, width = table
     int32 = torch.int32
-    if page_table.dtype != int32 or seq_lens.dtype != int32 or (cu_seqlens is not None and cu_seqlens.dtype != int32):
+    if page_table.dtype is not int32 or seq_lens.dtype is not int32:
         raise ValueError("page_table, seq_lens and cu_seqlens must be int32")
-    if (table[1] > 1 and page_table.stride(1) != 1) or not seq_lens.is_contiguous():
+    if (width > 1 and rows[1] != 1) or not seq_lens.is_contiguous():
         raise ValueError("page_table rows and seq_lens must be contiguous")
+    shared = (k_cache.device == device and v_cache.device == device and page_table.device == device
+              and seq_lens.device == device)
     if cu_seqlens is None:
-        if q.shape[0] != table[0]:
+        if q.shape[0] != batch:
             raise ValueError("without cu_seqlens every request has one token")
-    elif cu_seqlens.shape != (table[0] + 1,) or not cu_seqlens.is_contiguous():
-        raise ValueError("cu_seqlens must be a contiguous [B + 1]")
-    if (k_cache.device != device or v_cache.device != device or page_table.device != device
-            or seq_lens.device != device or (cu_seqlens is not None and cu_seqlens.device != device)):
+        starts = 0
+    else:
+        if cu_seqlens.dtype is not int32:
+            raise ValueError("page_table, seq_lens and cu_seqlens must be int32")
+        if cu_seqlens.shape != (batch + 1,) or not cu_seqlens.is_contiguous():
+            raise ValueError("cu_seqlens must be a contiguous [B + 1]")
+        shared = shared and cu_seqlens.device == device
+        starts = cu_seqlens.data_ptr()
+    if not shared:
         raise ValueError("all tensors must share a device")
-
-
-def _cache_of(k_cache, v_cache, page_table, seq_lens, cu_seqlens):
-    """flash_prologue_cache."""
-    a, b = k_cache.stride(), v_cache.stride()
-    return (k_cache.data_ptr(), a[0], a[1], a[2], v_cache.data_ptr(), b[0], b[1], b[2], k_cache.shape[0],
-            k_cache.shape[1], page_table.data_ptr(), page_table.stride(0), page_table.shape[1], seq_lens.data_ptr(),
-            0 if cu_seqlens is None else cu_seqlens.data_ptr(), page_table.shape[0])
+    return (k_cache.data_ptr(), a[0], a[1], a[2], v_cache.data_ptr(), b[0], b[1], b[2], pages, page_size,
+            page_table.data_ptr(), rows[0], width, seq_lens.data_ptr(), starts, batch)
 
 
 def _no_grad(name, *tensors):
@@ -72,18 +76,18 @@ def _append(q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache, page_ta
     if q.ndim != 3 or v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
         raise ValueError("q, k and v must be packed [T,Hq,D], [T,Hk,D], [T,Hk,D]")
     check_rows(q, k, rmsnorm_weight, scales, sin, cos, eps)
-    _check_cache(q, k.shape[1], k_cache, v_cache, page_table, seq_lens, cu_seqlens)
+    cache = _checked_cache(q, k.shape[1], k_cache, v_cache, page_table, seq_lens, cu_seqlens)
     q, k, v = readable(q), readable(k), readable(v)
     q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    if q.shape[0]:
+    tokens, heads, dim = q.shape
+    if tokens:
         w = None if rmsnorm_weight is None else flat_fp32(rmsnorm_weight)
         s = None if scales is None else scales.contiguous()
         args = _lib.APPEND_ARGS.pack(
-            *rows_of(q), *rows_of(k), *rows_of(v), *rows_of(q_out), 0 if w is None else w.data_ptr(),
-            0 if s is None else s.data_ptr(), *rotation_of(sin, cos),
-            *_cache_of(k_cache, v_cache, page_table, seq_lens, cu_seqlens),
-            q.shape[0], q.shape[1], k.shape[1], q.shape[2], _lib.DTYPE_CODES[q.dtype], eps)
-        call_library("flash_prologue_append_paged", args, q)
+            *rows_of(q), *rows_of(k), *rows_of(v), q_out.data_ptr(), 0, dim, heads * dim,
+            0 if w is None else w.data_ptr(), 0 if s is None else s.data_ptr(), *rotation_of(sin, cos), *cache, tokens,
+            heads, k.shape[1], dim, _lib.DTYPE_CODES[q.dtype], eps)
+        call_library("flash_prologue_append_paged", args, q.device)
     return q_out
 
 
@@ -126,57 +130,55 @@ ATTENTION_HEAD_DIMS = (64, 128)
 _WORKSPACE_BYTES = {}
 
 
-def _workspace_bytes(key, args, device):
-    """Workspace of a call: a function of its sizes and the device (``key``), asked for once."""
-    nbytes = _WORKSPACE_BYTES.get(key)
-    if nbytes is None:
-        out = ctypes.c_size_t(0)
-        with _DeviceGuard(device):
-            _lib.check(_lib.load().flash_prologue_paged_attention_workspace_size(_lib.ATTENTION_ARGS.pack(*args),
-                                                                                 ctypes.byref(out)),
-                       "flash_prologue_paged_attention_workspace_size")
-        if len(_WORKSPACE_BYTES) >= 4096:  # many distinct sizes: start over
-            _WORKSPACE_BYTES.clear()
-        nbytes = _WORKSPACE_BYTES[key] = int(out.value)
-    return nbytes
+def _workspace_bytes(dim, device):
+    out = ctypes.c_size_t(0)
+    with _DeviceGuard(device):
+        _lib.check(_lib.load().flash_prologue_paged_attention_workspace_size(dim, ctypes.byref(out)),
+                   "flash_prologue_paged_attention_workspace_size")
+    _WORKSPACE_BYTES[dim, device.index] = int(out.value)
+    return int(out.value)
 
 
-def _aligned_rows(q):
+def _aligned_rows(q, stride):
     """q, or a copy whose rows start on 16 bytes and are contiguous along D."""
-    st = q.stride()
-    return q if st[2] == 1 and q.data_ptr() % 16 == 0 and not (st[0] | st[1]) % 8 else q.contiguous().clone()
+    if stride[2] == 1 and not (stride[0] | stride[1]) & 7 and not q.data_ptr() & 15:
+        return q
+    return q.contiguous().clone()
 
 
 def _attention(q, k_cache, v_cache, page_table, seq_lens, cu_seqlens, softmax_scale, window, want_lse):
-    if q.ndim != 3:
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 3:
         raise ValueError("q must be packed [T,Hq,D]")
-    if q.dtype not in (torch.bfloat16, torch.float16):
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise ValueError("paged attention takes BF16 or FP16")
-    tokens, heads, dim = q.shape
+    tokens, heads, dim = shape
     if dim not in ATTENTION_HEAD_DIMS:
         raise ValueError(f"head dimension must be one of {ATTENTION_HEAD_DIMS}")
     kv_heads = k_cache.shape[2] if k_cache.ndim == 4 else 0
-    _check_cache(q, kv_heads, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
+    cache = _checked_cache(q, kv_heads, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
     if kv_heads <= 0 or heads <= 0 or heads % kv_heads or heads > MAX_HEADS:
         raise ValueError(f"query heads must be a multiple of the key heads and at most {MAX_HEADS}")
-    if not math.isfinite(softmax_scale):
+    if not -math.inf < softmax_scale < math.inf:
         raise ValueError("softmax_scale must be finite")
     if window < 0:
         raise ValueError("window must be 0 (all keys) or positive")
-    if q.device.type != "cuda":
+    device = q.device
+    if device.type != "cuda":
         raise ValueError("the attention kernels run on CUDA devices only")
-    q = _aligned_rows(q)
+    stride = q.stride()
+    q = _aligned_rows(q, stride)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = q.new_empty((tokens, heads), dtype=torch.float32) if want_lse else None
     if tokens:
-        head = (*rows_of(q), *rows_of(out), lse.data_ptr() if want_lse else 0,
-                *_cache_of(k_cache, v_cache, page_table, seq_lens, cu_seqlens))
-        sizes = (tokens, heads, kv_heads, dim, _lib.DTYPE_CODES[q.dtype], window, softmax_scale)
-        nbytes = _workspace_bytes((*sizes, cu_seqlens is None, k_cache.shape[1], page_table.shape, q.get_device()),
-                                  (*head, 0, 0, *sizes), q.device)
+        stride = q.stride()
+        nbytes = _WORKSPACE_BYTES.get((dim, device.index)) or _workspace_bytes(dim, device)
         workspace = q.new_empty((nbytes + 1) // 2)
-        call_library("flash_prologue_paged_attention",
-                     _lib.ATTENTION_ARGS.pack(*head, workspace.data_ptr(), nbytes, *sizes), q)
+        args = _lib.ATTENTION_ARGS.pack(
+            q.data_ptr(), 0, stride[1], stride[0], out.data_ptr(), 0, dim, heads * dim,
+            lse.data_ptr() if want_lse else 0, *cache, workspace.data_ptr(), nbytes, tokens, heads, kv_heads, dim,
+            _lib.DTYPE_CODES[dtype], window, softmax_scale)
+        call_library("flash_prologue_paged_attention", args, device)
     return out, lse
 
 

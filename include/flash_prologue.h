@@ -565,10 +565,8 @@ typedef struct flash_prologue_attention_args {
  * flash_prologue_paged_attention_workspace_size() bytes, no initialisation.
  */
 FLASH_PROLOGUE_API int flash_prologue_paged_attention(const flash_prologue_attention_args* args, void* stream);
-/* Bytes of workspace a call with these sizes needs on the current device, whatever the lengths
- * (pointers other than cu_seqlens' presence do not matter, but are checked). */
-FLASH_PROLOGUE_API int flash_prologue_paged_attention_workspace_size(const flash_prologue_attention_args* args,
-                       size_t* bytes);
+/* Bytes of workspace that cover every call with head dimension D on the current device. */
+FLASH_PROLOGUE_API int flash_prologue_paged_attention_workspace_size(int64_t D, size_t* bytes);
 
 #ifdef __cplusplus
 }  /* extern "C" */
