@@ -93,7 +93,7 @@ TmaPlan plan_tma(int64_t B, int64_t H, int64_t N, int D, int dtype, bool heads_i
   return p;
 }
 
-cudaError_t allow_shared_memory(const void* kernel, size_t bytes) {
+cudaError_t allow_shared_memory(const void* kernel, size_t bytes) try {
   static std::mutex mu;
   static std::unordered_map<const void*, std::unordered_map<int, size_t>> allowed;
   int dev = 0;
@@ -105,6 +105,8 @@ cudaError_t allow_shared_memory(const void* kernel, size_t bytes) {
   err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
   if (err == cudaSuccess) most = bytes;
   return err;
+} catch (...) {  // no room for the note: nothing leaves through the C entry points
+  return cudaErrorMemoryAllocation;
 }
 
 int64_t persistent_grid(const void* kernel, size_t smem_bytes, int64_t n_items, int threads) {

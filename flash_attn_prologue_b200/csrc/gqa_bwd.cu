@@ -50,7 +50,8 @@ __global__ void __launch_bounds__(kThreads, 2) gqa_bwd_kernel(const GqaBwdArgs a
   }
   for (int i = threadIdx.x; i < a.H[0]; i += kThreads) {
     const float v = a.scales[i];
-    e_s[i] = make_float2(expf(v), expf(-v));
+    // Below e^-80 the gradients are under 1e-34 and exp(-v) may be infinite: without the second, 0 * inf cannot arise.
+    e_s[i] = make_float2(expf(v), v < -80.f ? 0.f : expf(-v));
   }
   for (int i = threadIdx.x; i < kWarps * a.H[0]; i += kThreads) ds_s[i] = 0.f;
   __syncthreads();

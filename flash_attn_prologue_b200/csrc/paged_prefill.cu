@@ -485,7 +485,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
         if (!partial_block(w, a.window, w.first + j)) continue;
         const int s = j % L::kStages;
         // Asked by the warp that has seen the block arrive.
-        if (!__all_sync(0xffffffffu, phase_wait(&bar.clean_ask, asked++ & 1))) break;
+        if (!__all_sync(0xffffffffu, phase_wait(&bar.clean_ask, asked++ & 1) &&
+                                         phase_wait(&bar.v_full[s], (j / L::kStages) & 1)))
+          break;
         const int kb = (w.first + j) * kKeys;
         uint4* v = reinterpret_cast<uint4*>(v_s + s * L::kBlock);
         bool wild = false;

@@ -151,6 +151,48 @@ def test_repeats_bit_for_bit_and_on_another_stream():
 
 
 @pytest.mark.gpu
+def test_very_small_query_scales():
+    """exp(scale) underflows: zero rows and zero gradients, no NaN."""
+    q, k, w, s, sin, cos, _, up = _problem("packed", 1, 9, 4, 2, 64, FP32, None)
+    s = torch.tensor([-200.0, -85.0, -60.0, 0.0], device="cuda").view(4, 1, 1)
+    args = [t.detach().requires_grad_() for t in (q, k, w, s)]
+    got = fap.qknorm_rope_scale_gqa(*args, sin, cos)
+    grads = torch.autograd.grad(got, args, up)
+    assert all(t.isfinite().all() for t in (*got, *grads))
+    assert not got[0][:, 0].any() and not grads[0][:, 0].any() and grads[0][:, 3].any()
+
+
+@pytest.mark.gpu
+def test_sums_over_a_peer_group_of_one_rank():
+    """Inside reducing() the backward takes the group's reduction: one epoch a call, the plain call's bits."""
+    import ctypes
+    from types import SimpleNamespace
+    from flash_attn_prologue_b200 import distributed
+    nd, nf = ctypes.c_size_t(), ctypes.c_size_t()
+    assert _lib.load().flash_prologue_peer_buffer_bytes(1, 160, ctypes.byref(nd), ctypes.byref(nf)) == 0
+    data = torch.zeros(nd.value // 4, device="cuda")
+    flags = torch.zeros(nf.value // 4, dtype=torch.int32, device="cuda")
+    desc = _lib.PeersDesc()
+    desc.world, desc.rank, desc.max_cols, desc.wait_ms = 1, 0, 160, 1000
+    desc.data[0], desc.flags[0] = data.data_ptr(), flags.data_ptr()
+    epochs = iter(range(1, 10))
+    group = SimpleNamespace(desc=desc, next_epoch=lambda: next(epochs))
+    q, k, w, s, sin, cos, _, up = _problem("packed", 1, 300, 16, 4, 64, BF16, None)
+    args = [t.detach().requires_grad_() for t in (q, k, w, s)]
+    plain = torch.autograd.grad(fap.qknorm_rope_scale_gqa(*args, sin, cos), args, up)
+    index = torch.cuda.current_device()
+    distributed._ACTIVE_PEER_GROUPS[index] = group
+    try:
+        for _ in range(2):
+            grads = torch.autograd.grad(fap.qknorm_rope_scale_gqa(*args, sin, cos), args, up)
+            assert all(torch.equal(a, b) for a, b in zip(plain, grads))
+    finally:
+        distributed._ACTIVE_PEER_GROUPS.pop(index)
+    torch.cuda.synchronize()
+    assert next(epochs) == 3 and _lib.device_error() == 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("shape", [(0, 8, 64), (2, 8, 0, 64)])
 def test_no_tokens(shape):
     q = torch.randn(shape, device="cuda", requires_grad=True)

@@ -82,6 +82,20 @@ def test_single_tokens(Hq, Hk, page, window, D, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("news,totals", [
+    ([1] * 9, [1, 64, 100, 128, 129, 192, 200, 255, 256]),
+    ([2, 0, 1, 3], [200, 256, 1, 3]),
+    ([1] * 400, [1 + i % 250 for i in range(400)]),
+])
+@pytest.mark.parametrize("Hq,Hk,D,window", [(8, 2, 128, 0), (16, 16, 64, 70), (48, 2, 64, 0)])
+def test_short_caches(news, totals, Hq, Hk, D, window):
+    """Caches that one CTA an item reads whole."""
+    req = Requests(news, totals, Hq, Hk, D, 64, FP16)
+    assert req.table.shape[1] * 64 <= 256
+    _check(req, req.q.half(), window=window, rows=list(range(0, sum(news), 1 + sum(news) // 60)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("news,totals", [
     ([1], [40000]),                      # split over the whole GPU
     ([1, 1], [70001, 3]),
     ([5], [20000]),
