@@ -16,6 +16,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
+from .distributed import active_peer_group
 from .fused_epilogue import _DeviceGuard, _grad_view
 from .functional import SUPPORTED_CUTE_HEAD_DIMS, _plain_eager
 
@@ -173,7 +174,6 @@ def _workspace_bytes(heads, dim, device):
 
 def gqa_backward(q, k, rmsnorm_weight, scales, sin, cos, positions, grad_q_out, grad_k_out, eps, checked=False):
     """``checked``: the arguments but the gradients went through gqa_forward."""
-    from .distributed import active_peer_group
     if not checked:
         check_rows(q, k, rmsnorm_weight, scales, sin, cos, eps)
         _check_positions(positions, q, sin)
