@@ -5,6 +5,13 @@
 
 namespace flash_prologue {
 
+// Probabilities of FP16 caches are 2^7 times as large while they are multiplied
+// with V (and summed): those down to 2^-21 of the largest then keep all of their
+// bits, where unscaled ones below 2^-14 would lose them. The largest may be 2^8
+// (paged_prefill.cu), which is 2^15 so, inside the type. BF16 has FP32's range.
+template <typename T>
+constexpr float kProbabilityShift = std::is_same<T, __half>::value ? 7.f : 0.f;
+
 struct AttentionArgs {
   const void* q;
   void* out;

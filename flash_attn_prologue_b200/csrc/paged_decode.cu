@@ -359,7 +359,8 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int x = 0; x < 2; ++x) p[n][2 * e + x] = exp2_approx(p[n][2 * e + x] - from);
+          for (int x = 0; x < 2; ++x)
+            p[n][2 * e + x] = exp2_approx(p[n][2 * e + x] - (from - kProbabilityShift<T>));
         sum[e] = sum[e] * scale[e] + ((p[0][2 * e] + p[0][2 * e + 1]) + (p[1][2 * e] + p[1][2 * e + 1]));
       }
       if (__any_sync(0xffffffffu, scale[0] != 1.f || scale[1] != 1.f)) {
@@ -460,7 +461,7 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
         static_cast<T*>(a.out)[(q.first + token) * a.out_n + h * a.out_h + col] =
             from_float<T>(l == 0.f ? 0.f : o / l);
         if (a.lse && col == 0)
-          a.lse[(int64_t)(q.first + token) * a.heads + h] = (m + log2f(l)) * 0.6931471805599453f;
+          a.lse[(int64_t)(q.first + token) * a.heads + h] = (m + log2f(l) - kProbabilityShift<T>) * 0.6931471805599453f;
       } else {
         part_out[(slot * kRows + row) * D + col] = o;
         if (col == 0) {
@@ -561,7 +562,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Atten
   const int at = p.row0 + row, token = at / a.group;
   const int h = p.kv_head * a.group + (at - token * a.group);
   static_cast<T*>(a.out)[(p.token0 + token) * a.out_n + h * a.out_h + col] = from_float<T>(l == 0.f ? 0.f : v / l);
-  if (a.lse && col == 0) a.lse[(int64_t)(p.token0 + token) * a.heads + h] = (m + log2f(l)) * 0.6931471805599453f;
+  if (a.lse && col == 0) a.lse[(int64_t)(p.token0 + token) * a.heads + h] = (m + log2f(l) - kProbabilityShift<T>) * 0.6931471805599453f;
 }
 
 int64_t most_ctas(int D, int sms) { return (int64_t)sms * (D == 64 ? 4 : 2); }

@@ -579,7 +579,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
           tmem_st16(mine + L::kOCol + 16 * c, o);
         }
       }
-      const float from = top == -INFINITY ? 0.f : top * scale;
+      const float from = (top == -INFINITY ? 0.f : top * scale) - kProbabilityShift<T>;
       const float2 scale2 = make_float2(scale, scale), from2 = make_float2(-from, -from);
       float2 add[4] = {};
       uint32_t out[32];
@@ -676,7 +676,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
         p.part_stat[(slot * kTile + row) * 2] = top2;
         p.part_stat[(slot * kTile + row) * 2 + 1] = sum;
       } else if (a.lse) {
-        a.lse[(int64_t)token * a.heads + h] = (top2 + log2f(sum)) * 0.6931471805599453f;
+        a.lse[(int64_t)token * a.heads + h] = (top2 + log2f(sum) - kProbabilityShift<T>) * 0.6931471805599453f;
       }
     }
   }
@@ -719,7 +719,7 @@ __global__ void __launch_bounds__(512) prefill_join_kernel(const PrefillArgs p) 
     if constexpr (std::is_same<T, __half>::value) out[32 * c + lane] = __float2half_rn(x);
     else out[32 * c + lane] = __float2bfloat16_rn(x);
   }
-  if (a.lse && lane == 0) a.lse[(int64_t)(t.token0 + token) * a.heads + h] = (m + log2f(l)) * 0.6931471805599453f;
+  if (a.lse && lane == 0) a.lse[(int64_t)(t.token0 + token) * a.heads + h] = (m + log2f(l) - kProbabilityShift<T>) * 0.6931471805599453f;
 }
 
 // A cache as {D, slots, heads, pages}, a box of 64 columns x box_rows slots.
