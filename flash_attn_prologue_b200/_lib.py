@@ -237,6 +237,11 @@ def ptr(t: torch.Tensor):
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
+def raw_stream(index: int) -> int:
+    """The current CUDA stream of device ``index`` as an integer."""
+    return torch.cuda.current_stream(index).cuda_stream if _raw_stream is None else _raw_stream(index)
+
+
 def stream_of(device: torch.device):
     """The current CUDA stream of ``device`` as a cudaStream_t (a direct query
     of the raw handle where torch exposes one: a few microseconds less per call

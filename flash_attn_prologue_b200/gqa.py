@@ -18,7 +18,7 @@ import torch
 from . import _lib
 from .distributed import active_peer_group
 from .fused_epilogue import _DeviceGuard, _grad_view
-from .functional import SUPPORTED_CUTE_HEAD_DIMS, _plain_eager
+from .functional import SUPPORTED_CUTE_HEAD_DIMS
 
 MAX_HEADS = 512
 
@@ -81,22 +81,27 @@ def _check_positions(positions, q, sin):
         raise ValueError("all tensors must share a device")
 
 
+_functorch_active = getattr(torch._C, "_are_functorch_transforms_active", lambda: False)
+
+
 def eager(*tensors) -> bool:
-    """An eager call on plain tensors, parameters or None (see _plain_eager)."""
+    """An eager call on plain tensors, parameters or None (functional._plain_eager, which takes no parameters)."""
+    if torch.compiler.is_compiling() or torch._C._is_tracing() or _functorch_active():
+        return False
     for t in tensors:
         if t is not None and type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
             return False
-    return _plain_eager()
+    return True
 
 
 def call_library(name, args, device):
     """Calls entry point ``name`` on ``device``'s current stream, with the device current."""
     function = getattr(_lib.load(), name)
     if device.index == torch._C._cuda_getDevice():
-        status = function(args, _lib.stream_of(device))
+        status = function(args, _lib.raw_stream(device.index))
     else:
         with _DeviceGuard(device):
-            status = function(args, _lib.stream_of(device))
+            status = function(args, _lib.raw_stream(device.index))
     if status:
         _lib.check(status, name)
 
@@ -121,7 +126,7 @@ def rotation_of(sin, cos):
 def flat_fp32(t):
     """A parameter as the contiguous, 16-byte aligned array the kernels read."""
     t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    return t if not t.data_ptr() & 15 else t.clone()
 
 
 def _call(name, q, k, w, s, sin, cos, positions, eps, rows, grads=(0, 0), workspace=(0, 0), peers=(0, 0)):
@@ -262,5 +267,8 @@ def qknorm_rope_scale_gqa(q, k, rmsnorm_weight, scales, sin, cos, positions=None
     in q, k, rmsnorm_weight and scales; outputs and gradients keep the inputs' memory order.
     """
     if eager(q, k, rmsnorm_weight, scales, sin, cos, positions):
+        if not torch.is_grad_enabled() or not (q.requires_grad or k.requires_grad or rmsnorm_weight.requires_grad
+                                               or scales.requires_grad):
+            return gqa_forward(q, k, rmsnorm_weight, scales, sin, cos, positions, eps)
         return _GqaEager.apply(q, k, rmsnorm_weight, scales, sin, cos, positions, eps)
     return torch.ops.flash_prologue.qknorm_rope_scale_gqa(q, k, rmsnorm_weight, scales, sin, cos, positions, eps)
