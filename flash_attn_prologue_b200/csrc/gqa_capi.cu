@@ -235,6 +235,9 @@ int flash_prologue_append_paged(const flash_prologue_append_args* a, void* strea
     return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
   if (!aligned(a->rmsnorm_weight, 16)) return FLASH_PROLOGUE_ERR_ALIGNMENT;
   if (expanded(a->q_out, 1, a->Hq, a->tokens)) return FLASH_PROLOGUE_ERR_EXPANDED;
+  if (c.k_slot == 0 || c.v_slot == 0 || (c.num_pages > 1 && (c.k_page == 0 || c.v_page == 0)) ||
+      (a->Hk > 1 && (c.k_head == 0 || c.v_head == 0)))
+    return FLASH_PROLOGUE_ERR_EXPANDED;  // slots that are written must be apart
   const size_t es = elem_size(a->dtype);
   const bool vec = rows_vec(a->q, es) && rows_vec(a->k, es) && rows_vec(a->v, es) && rows_vec(a->q_out, es) &&
                    rotation_vec(a->rotation);

@@ -189,6 +189,10 @@ def test_refused_caches(change, text):
     args = {n: t.cuda() for n, t in {**_cpu_step(), **change}.items()}
     with pytest.raises(ValueError, match=text):
         fap.append_paged_kv(**args)
+    with pytest.raises(ValueError, match="expanded"):
+        good = {n: t.cuda() for n, t in _cpu_step().items()}
+        good["v_cache"] = good["v_cache"][:, :, :1].expand(-1, -1, 2, -1)
+        fap.append_paged_kv(**good)
     with pytest.raises(ValueError, match="contiguous along D"):
         good = {n: t.cuda() for n, t in _cpu_step().items()}
         good["k_cache"] = good["k_cache"].transpose(0, 3).contiguous().transpose(0, 3)
