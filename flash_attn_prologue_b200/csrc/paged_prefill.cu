@@ -603,7 +603,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.p_full[j & 1]);
     }
-    if (blocks && ok) phase_wait(&bar.o_done[(blocks - 1) & 1], ((blocks - 1) >> 1) & 1);
+    if (blocks && ok) ok = phase_wait(&bar.o_done[(blocks - 1) & 1], ((blocks - 1) >> 1) & 1);
+    if (!ok) sum = __int_as_float(0x7fc00000);  // a wait ran out: no output that could pass for one
   }
   __syncthreads();  // `bad` and `wild` are final
 
