@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kThreads, 2) gqa_bwd_kernel(const GqaBwdArgs a
       if (it0 >= it1) continue;
       const int h0 = it0 * HS + hslot;
       T* out = static_cast<T*>(a.dx[t]) + b * a.sdx[t].b + h0 * a.sdx[t].h + n * a.sdx[t].n + j0;
-            const float* wa = w_s + t * D + c_lane * kChunk;
+      const float* wa = w_s + t * D + c_lane * kChunk;
       const float* wb = wa + HALF;
       for (int it = it0; it < it1; ++it) {
         const int h = it * HS + hslot;

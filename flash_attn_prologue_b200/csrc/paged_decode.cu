@@ -8,11 +8,12 @@
 // and both products run on 16 x 8 x 16 matrix instructions, far from their
 // limit. Work is counted in blocks of 64 keys over all requests, row tiles and
 // key heads, and every CTA of a full GPU takes an equal run of them, whatever
-// the requests' lengths; where a run ends inside an item its part goes to the
-// workspace (row maximum, sum and unscaled output, FP32) and a second kernel
-// joins the parts in order. A warp takes 16 of a block's keys and loads them
-// with cp.async into a ring of its own, two blocks ahead, so no barrier stands
-// between a load and its use; the four warps join at an item's end.
+// the requests' lengths (with few items, a piece of one: cut_of). Where a run
+// ends inside an item its part goes to the workspace (row maximum, sum and
+// unscaled output, FP32) and a second kernel joins the parts in order. A warp
+// takes 16 of a block's keys and loads them with cp.async into a ring of its
+// own, two blocks ahead, so no barrier stands between a load and its use; the
+// four warps join at an item's end.
 //
 // Scores, softmax statistics and outputs are FP32; the probabilities are
 // rounded to the cache's type for the second product (their sum is taken
@@ -103,22 +104,55 @@ __device__ __forceinline__ int blocks_of(const Request& q, int window) {
   const int lo = first_key(q, window) / kBlockKeys, hi = (q.total + kBlockKeys - 1) / kBlockKeys;
   return max(hi - lo, 1);  // one at least: it writes the zeros of rows without keys
 }
-__device__ __forceinline__ int64_t units_of(const Request& q, const AttentionArgs& a) {
-  const int tiles = (q.news * a.group + kRows - 1) / kRows;
-  return (int64_t)tiles * a.kv_heads * (a.whole ? 1 : blocks_of(q, a.window));
+// Row tiles times key heads, each an item of blocks_of() blocks.
+__device__ __forceinline__ int64_t items_of(const Request& q, const AttentionArgs& a) {
+  return (int64_t)((q.news * a.group + kRows - 1) / kRows) * a.kv_heads;
+}
+// Units of an item: `cut` blocks at most in each.
+__device__ __forceinline__ int units_of_item(int blocks, int cut) {
+  return cut == 1 ? blocks : (blocks + cut - 1) / cut;
 }
 
-// Sum over the CTA (every thread gets it).
-__device__ __forceinline__ int64_t cta_sum(int64_t v, int64_t* scratch) {
+// Sums of two values over the CTA (every thread gets them).
+__device__ __forceinline__ void cta_sum(int64_t (&v)[2], int64_t (*scratch)[2]) {
+  if (__all_sync(0xffffffffu, (v[0] | v[1]) >> 24 == 0)) {
+    v[0] = __reduce_add_sync(0xffffffffu, (unsigned)v[0]);
+    v[1] = __reduce_add_sync(0xffffffffu, (unsigned)v[1]);
+  } else {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0;
+    for (int o = 16; o; o >>= 1)
 #pragma unroll
-  for (int w = 0; w < kDecodeWarps; ++w) v += scratch[w];
-  return v;
+      for (int i = 0; i < 2; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  }
+  if ((threadIdx.x & 31) == 0) {
+    scratch[threadIdx.x >> 5][0] = v[0];
+    scratch[threadIdx.x >> 5][1] = v[1];
+  }
+  __syncthreads();
+  v[0] = v[1] = 0;
+#pragma unroll
+  for (int w = 0; w < kDecodeWarps; ++w) {
+    v[0] += scratch[w][0];
+    v[1] += scratch[w][1];
+  }
+}
+
+// Blocks of a unit. 1: every CTA takes an equal run of units, which may begin
+// and end inside items. Where a run crosses an item's border its CTA fills and
+// empties its pipeline twice; with fewer items than CTAs, items can be cut into
+// pieces of a CTA each instead, longer than the runs. Worth it up to about a
+// quarter more and 3 blocks: pieces (runs) of 6 requests x 8,192 keys, 32/8 x
+// 128: 39.7 (43.1) us; 16 x up to 6 tokens, 4,096 keys, 16/4 x 64: 17.6 (19.6);
+// not taken, pieces half as long again: 32 x 4,096 keys, 16/4 x 64: 27.4 (26.0).
+// (kAll: an item is a unit.)
+constexpr int kAll = 1 << 30;
+__device__ __forceinline__ int cut_of(const AttentionArgs& a, int64_t blocks, int64_t items) {
+  const int64_t grid = gridDim.x;
+  if (a.whole) return kAll;
+  if (blocks <= grid || items >= grid || blocks >= int64_t(1) << 30) return 1;
+  // The sum of ceil(b / cut) over the items is below blocks / cut + items <= grid.
+  const int cut = (int)(blocks + grid - items - 1) / (int)(grid - items), run = (int)blocks / (int)grid;
+  return cut <= run + run / 4 + 3 ? cut : 1;
 }
 
 template <typename T, int D>
@@ -128,7 +162,7 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
   constexpr int kPerLane = kWarpKeys * (D / 8) / 32;     // 16-byte pieces of K (and of V) a lane loads
   constexpr int kTiles = D / 8;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ int64_t scratch[kDecodeWarps];
+  __shared__ int64_t scratch[kDecodeWarps], sums[kDecodeWarps][2];
   __shared__ int64_t found[2];  // request of the CTA's next unit, units before it
   __shared__ float stat[kDecodeWarps][kRows][2];
   __shared__ int bad_page;
@@ -138,16 +172,24 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
 
   if (!a.whole) start_next_kernel();
   // This CTA's run of units.
-  int64_t mine = 0;
+  int64_t total[2] = {0, 0}, my_items = 0;  // blocks and items of all requests; items of this thread's last one
+  int my_blocks = 0;
   bool bad = false;
   for (int r = threadIdx.x; r < batch; r += kDecodeThreads) {
     bool b;
     const Request q = request_at(a.pages, a.tokens, a.max_keys, r, &b);
     bad |= b;
-    if (q.news) mine += units_of(q, a);
+    my_items = items_of(q, a);
+    my_blocks = blocks_of(q, a.window);
+    total[0] += my_items * my_blocks;
+    total[1] += my_items;
   }
   if (bad) atomicOr(&g_device_error, kDeviceErrorIndex);
-  const int64_t units = cta_sum(mine, scratch);
+  if (threadIdx.x == 0) found[0] = -1;
+  cta_sum(total, sums);
+  const int cut = cut_of(a, total[0], total[1]);
+  const bool pieces = cut > 1 && !a.whole;  // a CTA has one unit
+  const int64_t units = a.whole ? total[1] : total[0];  // where CTAs have runs of them
   const int64_t slots = 2 * (int64_t)gridDim.x, cta = blockIdx.x;
   float* part_out = static_cast<float*>(a.workspace);                    // [slots][kRows][D]
   float* part_stat = part_out + slots * kRows * D;                       // [slots][kRows][2]
@@ -156,24 +198,37 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
   const int64_t ctas = min((int64_t)gridDim.x, units);  // every one of these has a unit at least
   if (cta >= ctas) return;
   const bool small = units < (int64_t(1) << 31) / 1024;  // the products below fit 32 bits
-  const int64_t begin = small ? (int)cta * (int)units / (int)ctas : cta * units / ctas;
-  const int64_t end = small ? ((int)cta + 1) * (int)units / (int)ctas : (cta + 1) * units / ctas;
+  const int64_t begin = pieces ? cta : small ? (int)cta * (int)units / (int)ctas : cta * units / ctas;
+  const int64_t end = pieces ? cta + 1 : small ? ((int)cta + 1) * (int)units / (int)ctas : (cta + 1) * units / ctas;
 
   // The request that `begin` falls into: one scan over the requests, a CTA's width at a time.
   int64_t before = 0;
   for (int r0 = 0; r0 < batch; r0 += kDecodeThreads) {
     const int r = r0 + threadIdx.x;
-    int64_t n = batch <= kDecodeThreads ? mine : 0;  // one request a thread: counted already
-    if (batch > kDecodeThreads && r < batch) {
-      bool b;
-      const Request q = request_at(a.pages, a.tokens, a.max_keys, r, &b);
-      if (q.news) n = units_of(q, a);
+    int64_t n = my_items * units_of_item(my_blocks, cut);  // one request a thread: read already
+    if (batch > kDecodeThreads) {
+      n = 0;
+      if (r < batch) {
+        bool b;
+        const Request q = request_at(a.pages, a.tokens, a.max_keys, r, &b);
+        n = items_of(q, a) * units_of_item(blocks_of(q, a.window), cut);
+      }
     }
     int64_t upto = n;  // inclusive sum within the warp
+    if (small) {
+      int low = (int)n;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += v;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, low, o);
+        if (lane >= o) low += v;
+      }
+      upto = low;
+    } else {
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
     }
     __syncthreads();
     if (lane == 31) scratch[warp] = upto;
@@ -192,24 +247,27 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
     if (before > begin) break;  // the same for every thread
   }
   __syncthreads();
+  if (found[0] < 0) return;  // fewer pieces than CTAs
   int r = (int)found[0];
   int64_t start = found[1];
 
   for (int64_t unit = begin; unit < end;) {
     bool too_long;  // more tokens than the page table has room for
     Request q = request_at(a.pages, a.tokens, a.max_keys, r, &too_long);
-    int64_t in_request = q.news ? units_of(q, a) : 0;
+    int64_t in_request = items_of(q, a) * units_of_item(blocks_of(q, a.window), cut);
     while (unit >= start + in_request) {
       start += in_request;
       ++r;
       q = request_at(a.pages, a.tokens, a.max_keys, r, &too_long);
-      in_request = q.news ? units_of(q, a) : 0;
+      in_request = items_of(q, a) * units_of_item(blocks_of(q, a.window), cut);
     }
-    const int blocks = blocks_of(q, a.window), per_item = a.whole ? 1 : blocks;
+    const int blocks = blocks_of(q, a.window), per_item = units_of_item(blocks, cut);
+    const int size = cut == 1 ? 1 : (blocks + per_item - 1) / per_item;  // blocks of a unit, evenly
     const int64_t in = unit - start;
     const int item = in >> 31 ? (int)(in / per_item) : (int)in / per_item;  // tiles x heads stay below 2^31
     const int64_t item_start = start + (int64_t)item * per_item;
-    const int b0 = (int)(unit - item_start), b1 = a.whole ? blocks : (int)min((int64_t)blocks, end - item_start);
+    const int u0 = (int)(unit - item_start), u1 = (int)min((int64_t)per_item, end - item_start);
+    const int b0 = u0 * size, b1 = min(u1 * size, blocks);
     const int head = item % a.kv_heads;
     const int row0 = item / a.kv_heads * kRows;       // of the request's news * group rows
     const int rows = min(kRows, q.news * a.group - row0);
@@ -476,10 +534,10 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
       p.row0 = row0;
       p.rows = rows;
       p.kv_head = head;
-      p.last = (int)(((item_start + blocks) * ctas - 1) / units);
+      p.last = (int)(pieces ? item_start + per_item - 1 : ((item_start + per_item) * ctas - 1) / units);
       parts[cta] = p;
     }
-    unit = item_start + (a.whole ? 1 : b1);
+    unit = item_start + u1;
     __syncthreads();
   }
 }

@@ -112,6 +112,20 @@ def test_long_and_many(news, totals, window):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("news,totals", [
+    ([1, 1, 1], [9000, 30, 20001]),
+    ([3, 0, 5, 1], [20000, 7000, 12345, 5]),
+    ([1] * 140, [300 + 7 * i for i in range(140)]),  # more requests than threads
+    ([2, 1, 0, 3] * 35, [300 + 9 * i for i in range(140)]),
+])
+@pytest.mark.parametrize("Hq,Hk,D,window", [(8, 2, 64, 0), (3, 1, 128, 0), (4, 1, 64, 5000), (12, 4, 128, 300)])
+def test_few_items_over_many_ctas(news, totals, Hq, Hk, D, window):
+    """Key heads times row tiles are fewer than a full GPU's CTAs, or about as many."""
+    req = Requests(news, totals, Hq, Hk, D, 32, BF16)
+    _check(req, req.q.to(BF16), window=window)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("news,totals", [([4, 3], [2, 5]), ([6, 2], [0, 2]), ([40], [10])])
 def test_rows_without_keys_are_zero(news, totals):
     req = Requests(news, totals, 8, 2, 64, 8, BF16)
