@@ -11,19 +11,24 @@
 // and the probabilities have two buffers, so the product with V runs beside the
 // next softmax. With the output that is 256 columns of the 512, so two CTAs share
 // an SM and two warps a scheduler do softmax. Ragged chunks of up to 2,000 tokens
-// with a window of 1,024 keys, 16/4 heads x 64 FP16: 81 us; probabilities over
-// the scores they came from, with two buffers for both: 83 us; one such buffer
-// of 128 keys: 101 us.
+// with a window of 1,024 keys, 16/4 heads x 64 FP16, a CTA a tile: 78 us;
+// probabilities over the scores they came from, with two buffers for both: 80 us;
+// one such buffer of 128 keys: 98 us.
 //
-// A CTA takes one tile: the rows (query heads x whole tokens) of one key head
-// that fit into 128, and its blocks of keys (or a share of them where there
-// are fewer tiles than the GPU holds; a second kernel adds the shares up).
+// A tile is the rows (query heads x whole tokens) of one key head that fit into
+// 128, and its blocks of keys (or a share of them where there are fewer tiles
+// than the GPU holds; a second kernel adds the shares up). There is a CTA a tile
+// in the grid, but one that runs takes over the tiles of those that have not
+// started (cluster launch control), so the start of a tile -- finding its
+// request, the pages' indices, the first loads and scores -- runs beside the last
+// softmax and output of the one before: about 2 us a tile instead of 7, and 65 us
+// for the chunks above. All buffers and their phases go on from tile to tile.
 //   warps 0-3  one row a thread: scores from tensor memory, running maximum
 //              and sum, probabilities to tensor memory, output to global memory;
 //   warp 4     issues S = Q K^T (both from shared memory);
 //   warp 6     issues O += P V (P from tensor memory, V read transposed from
 //              shared memory);
-//   warp 5     TMA loads of K and V, one box of a page a lane;
+//   warp 5     finds the tiles and loads Q, K and V by TMA, one box of a page a lane;
 //   warp 7     cleans V in blocks that some row of the tile does not see whole:
 //              zeros for slots outside the tile's keys, and for infinities and
 //              NaNs, which 0 * V would carry into rows that do not see them
@@ -62,15 +67,29 @@ struct Layout {
   static constexpr size_t kSmem = 1024 + (size_t)kQ + (size_t)kBlock * 2 * kStages;
 };
 
+// A tile and the split's share of its blocks.
+struct Work {
+  int first_token;  // packed index of its first row's token
+  int r;
+  int head;
+  int rows;         // valid rows; -1: no more tiles
+  int pos0, pos1;   // positions of the first and last token
+  int lo, hi;       // keys that some row sees
+  int first, blocks;  // this split's blocks (of 64 keys)
+  int parts;        // splits that have blocks
+  int share;        // where an item that is cut keeps this share
+  int bad, wild;    // an index was out of range; V held infinities or NaNs in partial blocks
+};
+
 constexpr int kMaxStages = 4;
 struct Barriers {
   uint64_t k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages];
   uint64_t s_full[2], s_read[2], p_full[2], o_done[2], clean_ask, v_clean, drain[2];
+  uint64_t q_full, q_empty, work_full[2], work_empty[2], next_here;
   uint32_t tmem;
-  int bad, wild;
   int sums[kPrefillThreads / 32];
-  int found, found_tile;  // request of the CTA's tile (-1: none), its tile of it
-  Request request;
+  int found, found_start;  // request of the CTA's first tile (-1: none), tiles before it
+  Work work[2];            // the tile that the warps are at and the next
 };
 
 struct Tile {  // what the join needs to know of a tile
@@ -96,6 +115,29 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       " [%0], [%1, {%2, %3, %4, %5}], [%6];"
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
       : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+      : "memory");
+}
+// Asks for a CTA of the grid that has not started, to do its work here; the
+// answer (16 bytes) arrives at `bar`. After an answer without one, not to be called again.
+__device__ __forceinline__ void ask_next_cta(void* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+               ::"r"(smem_u32(answer)), "r"(smem_u32(bar)) : "memory");
+}
+// Its index, -1 if there is none.
+__device__ __forceinline__ int next_cta(const void* answer) {
+  uint32_t got, x;
+  asm volatile(
+      "{\n .reg .b128 h;\n .reg .pred p;\n ld.shared.b128 h, [%2];\n mov.u32 %1, 0;\n"
+      " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n selp.u32 %0, 1, 0, p;\n"
+      " @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n}\n"
+      : "=r"(got), "=r"(x) : "r"(smem_u32(answer)) : "memory");
+  return got ? (int)x : -1;
 }
 // mbar_wait without the suspend hint, whose try takes twice as long where the
 // phase is complete (102 cycles instead of 51) and wakes later where it is not
@@ -185,19 +227,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 template <typename T>
 constexpr uint32_t kExponent = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
 
-// The keys of a tile and the split's share of its blocks.
-struct Work {
-  Request q;
-  int r;
-  int head;
-  int token0;       // first token of the tile, of the request's new ones
-  int rows;         // valid rows
-  int pos0, pos1;   // positions of the first and last token
-  int lo, hi;       // keys that some row sees
-  int first, last;  // this split's blocks (of 64 keys)
-  int parts;        // splits that have blocks
-};
-
 __device__ __forceinline__ bool partial_block(const Work& w, int window, int block) {
   const int kb = block * kKeys;
   return kb + kKeys - 1 > w.pos0 || (window && kb < w.pos1 - window + 1);
@@ -205,11 +234,12 @@ __device__ __forceinline__ bool partial_block(const Work& w, int window, int blo
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kPrefillThreads, 2)
-    paged_prefill_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
-                         const __grid_constant__ PrefillArgs p) {
+    paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                         const __grid_constant__ CUtensorMap v_map, const __grid_constant__ PrefillArgs p) {
   using L = Layout<D>;
   extern __shared__ unsigned char smem_raw[];
   __shared__ Barriers bar;
+  __shared__ __align__(16) unsigned char answer[16];
   const AttentionArgs& a = p.a;
   unsigned char* q_s = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* k_s = q_s + L::kQ;
@@ -217,12 +247,6 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (p.splits > 1) start_next_kernel();
-  // ---- this CTA's tile: last tiles first (they have the most keys), splits innermost
-  const int cut = (int)blockIdx.x - p.whole_items;  // CTAs of the items that are cut
-  const int splits = cut < 0 ? 1 : p.splits;
-  const int item = cut < 0 ? (int)blockIdx.x : p.whole_items + cut / p.splits;
-  const int split = cut < 0 ? 0 : cut % p.splits;
-  const int tile_of_all = p.tiles - 1 - item / a.kv_heads;
   const int requests = a.pages.batch + (a.pages.cu_seqlens ? 1 : 0);
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::kStages; ++s) {
@@ -236,171 +260,96 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       mbar_init(&bar.s_read[b], kRowThreads / 32);
       mbar_init(&bar.p_full[b], kRowThreads / 32);
       mbar_init(&bar.o_done[b], 1);
+      mbar_init(&bar.work_full[b], 1);
+      mbar_init(&bar.work_empty[b], kRowThreads / 32 + 3);
+      mbar_init(&bar.drain[b], 1);
     }
     mbar_init(&bar.clean_ask, 1);
     mbar_init(&bar.v_clean, 1);
-    mbar_init(&bar.drain[0], 1);
-    mbar_init(&bar.drain[1], 1);
+    mbar_init(&bar.q_full, 1);
+    mbar_init(&bar.q_empty, 1);
+    mbar_init(&bar.next_here, 1);
     bar.found = -1;
-    bar.bad = 0;
-    bar.wild = 0;
     fence_mbar_init();
   }
-  int before = 0;
-  for (int r0 = 0; r0 < requests; r0 += kPrefillThreads) {
-    const int r = r0 + threadIdx.x;
-    Request q{0, 0, 0};
-    bool too_long = false;
-    if (r < requests) q = request_at(a.pages, a.tokens, a.max_keys, r, &too_long);
-    const int n = (q.news + p.tile_tokens - 1) / p.tile_tokens;
-    int upto = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += v;
-    }
-    if (lane == 31) bar.sums[warp] = upto;
-    __syncthreads();
-    int start = before + upto - n, all = 0;
-#pragma unroll
-    for (int w = 0; w < kPrefillThreads / 32; ++w) {
-      if (w < warp) start += bar.sums[w];
-      all += bar.sums[w];
-    }
-    if (tile_of_all >= start && tile_of_all < start + n) {
-      bar.found = r;
-      bar.found_tile = tile_of_all - start;
-      bar.request = q;
-      bar.bad = too_long;
-    }
-    before += all;
-    __syncthreads();
-    if (before > tile_of_all) break;
-  }
-  Tile* join = splits > 1 ? p.joins + (item - p.whole_items) : nullptr;
-  if (bar.found < 0) {  // the grid has room for more tiles than there are
-    if (join && split == 0 && threadIdx.x == 0) join->parts = 0;
-    return;
-  }
-  Work w;
-  w.r = bar.found;
-  w.head = item % a.kv_heads;
-  w.q = bar.request;
-  w.token0 = bar.found_tile * p.tile_tokens;
-  const int tokens = min(p.tile_tokens, w.q.news - w.token0);
-  w.rows = tokens * a.group;
-  w.pos0 = w.q.total - w.q.news + w.token0;
-  w.pos1 = w.pos0 + tokens - 1;
-  w.hi = max(w.pos1 + 1, 0);
-  w.lo = a.window ? max(w.pos0 - a.window + 1, 0) : 0;
+  // The request of the first tile; later ones are found from there.
+  const auto tiles_of = [&](const Request& q) { return (q.news + p.tile_tokens - 1) / p.tile_tokens; };
+  // Last tiles first (they have the most keys), splits innermost.
+  const auto tile_at = [&](int index) {
+    return p.tiles - 1 - (index < p.whole_items ? index : p.whole_items + (index - p.whole_items) / p.splits) / a.kv_heads;
+  };
+  int all_tiles = 0;
   {
-    const int first = w.lo / kKeys, blocks = max((w.hi + kKeys - 1) / kKeys - first, 0);
-    // Shares of at least four blocks: a share's fixed cost is about theirs.
-    int share = blocks;
-    if (splits > 1) share = max((blocks + splits - 1) / splits, 4);
-    w.parts = blocks && splits > 1 ? (blocks + share - 1) / share : 1;
-    w.first = first + split * share;
-    w.last = min(first + blocks, w.first + share);
+    const int tile = tile_at(blockIdx.x);
+    for (int r0 = 0; r0 < requests; r0 += kPrefillThreads) {
+      const int r = r0 + threadIdx.x;
+      Request q{0, 0, 0};
+      bool too_long;
+      if (r < requests) q = request_at(a.pages, a.tokens, a.max_keys, r, &too_long);
+      const int n = tiles_of(q);
+      int upto = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      if (lane == 31) bar.sums[warp] = upto;
+      __syncthreads();
+      int start = all_tiles + upto - n;
+#pragma unroll
+      for (int w = 0; w < kPrefillThreads / 32; ++w) {
+        if (w < warp) start += bar.sums[w];
+        all_tiles += bar.sums[w];
+      }
+      if (tile >= start && tile < start + n) {
+        bar.found = r;
+        bar.found_start = start;
+      }
+      __syncthreads();
+    }
   }
-  if (join && split == 0 && threadIdx.x == 0) {
-    join->token0 = w.q.first + w.token0;
-    join->rows = w.rows;
-    join->kv_head = w.head;
-    join->parts = w.parts;
-  }
-  if (split >= w.parts) return;
-  const int blocks = max(w.last - w.first, 0);
-
-  // ---- tensor memory, Q
   if (warp == 4) {
     tmem_alloc(&bar.tmem, kTmemCols);
     tmem_relinquish();
   }
-  // The loads begin before the other warps have Q in shared memory.
-  const int boxes = kKeys / p.box_rows, in_page = (1 << a.pages.page_log2) - 1;
-  const uint32_t box_bytes = (uint32_t)p.box_rows * 128;
-  // The page of this lane's box of a block, -1 where there is nothing to load.
-  const auto page_of = [&](int j) {
-    int page = -1;
-    if (lane < boxes && j < blocks) {
-      const int key = (w.first + j) * kKeys + lane * p.box_rows;
-      if (key < w.hi && key + p.box_rows > w.lo) {
-        page = __ldg(a.pages.page_table + w.r * a.pages.table_stride + (key >> a.pages.page_log2));
-        if (page < 0 || page >= a.pages.num_pages) {
-          page = -1;
-          bar.bad = 1;
-        }
-      }
-    }
-    return page;
-  };
-  const auto load = [&](int j, int page, const CUtensorMap* map, unsigned char* ring, uint64_t* full) {
-    const int s = j % L::kStages;
-    const uint32_t count = __popc(__ballot_sync(0xffffffffu, page >= 0));
-    if (lane == 0) mbar_arrive_expect_tx(&full[s], count * box_bytes * L::kHalves);
-    __syncwarp();
-    if (page >= 0) {
-      const int key = (w.first + j) * kKeys + lane * p.box_rows;
-      const uint32_t dst = smem_u32(ring) + s * L::kBlock + lane * box_bytes;
-#pragma unroll
-      for (int h = 0; h < L::kHalves; ++h)
-        tma_load_4d(dst + h * L::kHalf, map, h * 64, key & in_page, w.head, page, &full[s]);
-    }
-    __syncwarp();
-  };
-  int next_page = -1;  // of the first block that the loop below loads
-  if (warp == 5) {
-    int page[L::kStages];
-#pragma unroll
-    for (int j = 0; j < L::kStages; ++j) page[j] = page_of(j);
-    next_page = page_of(L::kStages);
-#pragma unroll
-    for (int j = 0; j < L::kStages; ++j)
-      if (j < blocks) {
-        load(j, page[j], &k_map, k_s, bar.k_full);
-        load(j, page[j], &v_map, v_s, bar.v_full);
-      }
-  }
-  for (int i = threadIdx.x; i < kTile * (D / 8); i += kPrefillThreads) {
-    const int row = i / (D / 8), c = i % (D / 8);
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (row < w.rows) {
-      const int t = row / a.group, g = row - t * a.group;
-      v = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (w.q.first + w.token0 + t) * a.q_n +
-                                               (w.head * a.group + g) * a.q_h + c * 8));
-    }
-    *reinterpret_cast<uint4*>(q_s + (c >> 3) * L::kQHalf + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
-  }
-  fence_proxy_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bar.tmem;
 
-  // Row state (warps 0-3); the row's keys are [see_lo, see_hi].
-  const int row = threadIdx.x;
-  int see_hi = -1, see_lo = 0;
-  float top = -INFINITY, sum = 0.f;
+  // Every warp walks the CTA's tiles; `g` counts its blocks over all of them (buffers and
+  // phases go on from tile to tile), `t` the tiles. Where a wait runs out a warp leaves.
+  uint32_t g = 0;
+  const auto next_work = [&](uint32_t t) {
+    return __all_sync(0xffffffffu, phase_wait(&bar.work_full[t & 1], (t >> 1) & 1));
+  };
+  const auto done_with = [&](uint32_t t) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bar.work_empty[t & 1]);
+  };
 
-  if (warp >= 4) {
+  if (warp == 4) {
+    // ---------------- scores ----------------
     // The issuing warps walk the blocks whole, with values the compiler knows to be the same
     // in all lanes, and one lane issues. Each has one product: a warp that issued both, with
     // its waits, took longer for a block than its softmax does.
-    const int n = __shfl_sync(0xffffffffu, blocks, 0);
+    constexpr uint32_t idesc = idesc_of<T>(kKeys, false);
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-    if (warp == 4) {
-      // ---------------- scores ----------------
-      constexpr uint32_t idesc = idesc_of<T>(kKeys, false);
-      const uint64_t q_desc = smem_desc_k_sw128(smem_u32(q_s));
-      bool failed = false;
-      for (int j = 0; j < n; ++j) {
-        const int s = j % L::kStages, b = j % L::kScores, before = j - L::kScores;
+    const uint64_t q_desc = smem_desc_k_sw128(smem_u32(q_s));
+    bool ok = true;
+    uint32_t queries = 0;
+    for (uint32_t t = 0; ok; ++t) {
+      if (!(ok = next_work(t))) break;
+      const Work& w = bar.work[t & 1];
+      const int n = __shfl_sync(0xffffffffu, w.blocks, 0);
+      if (w.rows < 0) break;
+      if (n) ok = __all_sync(0xffffffffu, phase_wait(&bar.q_full, queries++ & 1));
+      for (int j = 0; j < n && ok; ++j, ++g) {
+        const uint32_t s = g % L::kStages, b = g % L::kScores;
         // The last scores of this buffer are in the rows' registers, K is here.
-        if (!__all_sync(0xffffffffu, (before < 0 || phase_wait(&bar.s_read[b], (before / L::kScores) & 1)) &&
-                                         phase_wait(&bar.k_full[s], (j / L::kStages) & 1))) {
-          failed = true;
+        if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.s_read[b], ((g / L::kScores) & 1) ^ 1) &&
+                                               phase_wait(&bar.k_full[s], (g / L::kStages) & 1))))
           break;
-        }
         tc_fence_after();
         const uint64_t k_desc = smem_desc_k_sw128(smem_u32(k_s) + s * L::kBlock);
         if (elect_one()) {
@@ -412,90 +361,253 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
                         k_desc + h * (L::kHalf / 16) + 2 * c, idesc, (h | c) != 0);
           umma_commit(&bar.k_empty[s]);
           umma_commit(&bar.s_full[b]);
+          if (j == n - 1) umma_commit(&bar.q_empty);
         }
         __syncwarp();
       }
-      if (failed) {  // tensor memory is not released under products still running
-        if (elect_one()) umma_commit(&bar.drain[0]);
-        phase_wait(&bar.drain[0], 0);
-      }
-    } else if (warp == 6) {
-      // ---------------- output ----------------
-      constexpr uint32_t idesc = idesc_of<T>(D, true);
-      bool failed = false;
-      uint32_t cleaned = 0;
-      for (int j = 0; j < n; ++j) {
-        const int s = j % L::kStages;
-        bool ok = phase_wait(&bar.v_full[s], (j / L::kStages) & 1);
+      done_with(t);
+    }
+    if (!ok) {  // tensor memory is not released under products still running
+      if (elect_one()) umma_commit(&bar.drain[0]);
+      phase_wait(&bar.drain[0], 0);
+    }
+  } else if (warp == 6) {
+    // ---------------- output ----------------
+    constexpr uint32_t idesc = idesc_of<T>(D, true);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    bool ok = true;
+    uint32_t cleaned = 0;
+    for (uint32_t t = 0; ok; ++t) {
+      if (!(ok = next_work(t))) break;
+      const Work& w = bar.work[t & 1];
+      const int n = __shfl_sync(0xffffffffu, w.blocks, 0);
+      if (w.rows < 0) break;
+      for (int j = 0; j < n; ++j, ++g) {
+        const uint32_t s = g % L::kStages;
+        ok = phase_wait(&bar.v_full[s], (g / L::kStages) & 1);
         const bool partial = partial_block(w, a.window, w.first + j);
         if (partial && lane == 0) mbar_arrive(&bar.clean_ask);  // cleaned beside the block's softmax
-        ok = ok && (!partial || phase_wait(&bar.v_clean, cleaned & 1)) && phase_wait(&bar.p_full[j & 1], (j >> 1) & 1);
+        ok = ok && (!partial || phase_wait(&bar.v_clean, cleaned & 1)) && phase_wait(&bar.p_full[g & 1], (g >> 1) & 1);
         cleaned += partial;
-        if (!__all_sync(0xffffffffu, ok)) {
-          failed = true;
-          break;
-        }
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
         tc_fence_after();
         const uint64_t v_desc = smem_desc_mn_sw128(smem_u32(v_s) + s * L::kBlock, L::kHalf);
         if (elect_one()) {
 #pragma unroll
           for (int c = 0; c < kKeys / 16; ++c)  // 16 keys a step: 8 columns of P, two 8-row groups of V (2,048 bytes)
-            umma_ts(tm + L::kOCol, tm + L::kPCol + (j & 1) * (kKeys / 2) + 8 * c, v_desc + 128 * c, idesc, (j | c) != 0);
+            umma_ts(tm + L::kOCol, tm + L::kPCol + (g & 1) * (kKeys / 2) + 8 * c, v_desc + 128 * c, idesc, (j | c) != 0);
           umma_commit(&bar.v_empty[s]);
-          umma_commit(&bar.o_done[j & 1]);
+          umma_commit(&bar.o_done[g & 1]);
         }
         __syncwarp();
       }
-      if (failed) {
-        if (elect_one()) umma_commit(&bar.drain[1]);
-        phase_wait(&bar.drain[1], 0);
+      done_with(t);
+    }
+    if (!ok) {
+      if (elect_one()) umma_commit(&bar.drain[1]);
+      phase_wait(&bar.drain[1], 0);
+    }
+  } else if (warp == 5) {
+    // ---------------- tiles and loads ----------------
+    const int in_page = (1 << a.pages.page_log2) - 1, boxes = kKeys / p.box_rows;
+    const uint32_t box_bytes = (uint32_t)p.box_rows * 128;
+    // The last tile's request: `r` with `before` tiles of others in front of it.
+    int r = requests, before = all_tiles;
+    Request q{0, 0, 0};
+    bool too_long = false;
+    if (bar.found >= 0) {
+      r = bar.found;
+      before = bar.found_start;
+      q = request_at(a.pages, a.tokens, a.max_keys, r, &too_long);
+    }
+    // The work of CTA `index`; false where it has none.
+    const auto describe = [&](int index, Work& w) {
+      const int cut = index - p.whole_items, splits = cut < 0 ? 1 : p.splits, split = cut < 0 ? 0 : cut % p.splits;
+      const int item = cut < 0 ? index : p.whole_items + cut / p.splits, tile = tile_at(index);
+      if (tile >= before + tiles_of(q)) {  // not before the last one: from the end
+        r = requests;
+        before = all_tiles;
+        q = Request{0, 0, 0};
       }
-    } else if (warp == 5) {
-      // ---------------- loads ----------------
-      bool ok = true;
-      int j = L::kStages;
-      for (int page = next_page; j < blocks; ++j) {
-        const int s = j % L::kStages, next = page_of(j + 1);
-        const uint32_t parity = ((j / L::kStages) & 1) ^ 1;
-        if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.k_empty[s], parity)))) break;
-        load(j, page, &k_map, k_s, bar.k_full);
-        if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.v_empty[s], parity)))) break;
-        load(j, page, &v_map, v_s, bar.v_full);
-        page = next;
+      while (tile < before && r > 0) {  // 32 requests back
+        const int at = r - 1 - lane;
+        Request mine{0, 0, 0};
+        bool over = false;
+        if (at >= 0) mine = request_at(a.pages, a.tokens, a.max_keys, at, &over);
+        const int n = tiles_of(mine);
+        int upto = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += v;
+        }
+        const uint32_t here = __ballot_sync(0xffffffffu, tile >= before - upto && tile < before - upto + n);
+        const int src = here ? __ffs(here) - 1 : 31;
+        r = here ? r - 1 - src : max(r - 32, 0);
+        before -= __shfl_sync(0xffffffffu, upto, src);
+        q.first = __shfl_sync(0xffffffffu, mine.first, src);
+        q.news = here ? __shfl_sync(0xffffffffu, mine.news, src) : 0;
+        q.total = __shfl_sync(0xffffffffu, mine.total, src);
+        too_long = __shfl_sync(0xffffffffu, (int)over, src);
+        if (here) break;
       }
-      // No product's arrival on an empty barrier lands after the CTA has gone.
-      for (int e = blocks; e < blocks + L::kStages && blocks && ok; ++e) {
-        const int s = e % L::kStages;
-        ok = phase_wait(&bar.k_empty[s], ((e / L::kStages) & 1) ^ 1) && phase_wait(&bar.v_empty[s], ((e / L::kStages) & 1) ^ 1);
+      Tile* join = splits > 1 && split == 0 && lane == 0 ? p.joins + (item - p.whole_items) : nullptr;
+      if (tile < before || tile >= before + tiles_of(q)) {  // the grid has room for more tiles than there are
+        if (join) join->parts = 0;
+        return false;
       }
-      if (j < blocks) {  // a wait ran out: wait (bounded) for the loads still in flight
-        for (int s = 0; s < L::kStages; ++s) {
-          for (int e = j; e >= 0 && e > j - L::kStages - 1; --e)
-            if (e % L::kStages == s) {
-              phase_wait(&bar.k_full[s], (e / L::kStages) & 1);
-              phase_wait(&bar.v_full[s], (e / L::kStages) & 1);
-              break;
-            }
+      const int token0 = (tile - before) * p.tile_tokens, tokens = min(p.tile_tokens, q.news - token0);
+      w.r = r;
+      w.head = item % a.kv_heads;
+      w.first_token = q.first + token0;
+      w.rows = tokens * a.group;
+      w.pos0 = q.total - q.news + token0;
+      w.pos1 = w.pos0 + tokens - 1;
+      w.hi = max(w.pos1 + 1, 0);
+      w.lo = a.window ? max(w.pos0 - a.window + 1, 0) : 0;
+      const int first = w.lo / kKeys, blocks = max((w.hi + kKeys - 1) / kKeys - first, 0);
+      // Shares of at least four blocks: a share's fixed cost is about theirs.
+      int share = blocks;
+      if (splits > 1) share = max((blocks + splits - 1) / splits, 4);
+      w.parts = blocks && splits > 1 ? (blocks + share - 1) / share : 1;
+      w.first = first + split * share;
+      w.blocks = max(min(first + blocks, w.first + share) - w.first, 0);
+      w.share = cut;
+      w.bad = too_long;
+      w.wild = 0;
+      if (join) {
+        join->token0 = w.first_token;
+        join->rows = w.rows;
+        join->kv_head = w.head;
+        join->parts = w.parts;
+      }
+      return split < w.parts;
+    };
+    // The page of this lane's box of a block, -1 where there is nothing to load.
+    const auto page_of = [&](const Work& w, int j, int* bad) {
+      int page = -1;
+      if (lane < boxes && j < w.blocks) {
+        const int key = (w.first + j) * kKeys + lane * p.box_rows;
+        if (key < w.hi && key + p.box_rows > w.lo) {
+          page = __ldg(a.pages.page_table + w.r * a.pages.table_stride + (key >> a.pages.page_log2));
+          if (page < 0 || page >= a.pages.num_pages) {
+            page = -1;
+            *bad = 1;
+          }
         }
       }
+      return page;
+    };
+    const auto load = [&](const Work& w, int j, int page, const CUtensorMap* map, unsigned char* ring, uint64_t* full) {
+      const uint32_t s = g % L::kStages, count = __popc(__ballot_sync(0xffffffffu, page >= 0));
+      if (lane == 0) mbar_arrive_expect_tx(&full[s], count * box_bytes * L::kHalves);
+      __syncwarp();
+      if (page >= 0) {
+        const int key = (w.first + j) * kKeys + lane * p.box_rows;
+        const uint32_t dst = smem_u32(ring) + s * L::kBlock + lane * box_bytes;
+#pragma unroll
+        for (int h = 0; h < L::kHalves; ++h)
+          tma_load_4d(dst + h * L::kHalf, map, h * 64, key & in_page, w.head, page, &full[s]);
+      }
+      __syncwarp();
+    };
+    bool ok = true;
+    uint32_t t = 0, queries = 0, asked = 0;
+    uint32_t k_loads = 0, v_loads = 0, q_loads = 0;  // begun
+    for (int index = blockIdx.x; index >= 0;) {
+      Work w;
+      if (describe(index, w)) {
+        Work& slot = bar.work[t & 1];
+        int page = page_of(w, 0, &w.bad);
+        w.bad = __any_sync(0xffffffffu, w.bad);
+        if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.work_empty[t & 1], ((t >> 1) & 1) ^ 1)))) break;
+        if (lane == 0) {
+          slot = w;
+          mbar_arrive(&bar.work_full[t & 1]);
+        }
+        __syncwarp();
+        ++t;
+        for (int j = 0; j < w.blocks; ++j, ++g) {
+          const uint32_t s = g % L::kStages, parity = ((g / L::kStages) & 1) ^ 1;
+          const int next = page_of(w, j + 1, &slot.bad);
+          if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.k_empty[s], parity)))) break;
+          load(w, j, page, &k_map, k_s, bar.k_full);
+          ++k_loads;
+          if (j == 0) {
+            // The last tile's scores have been computed: its Q can go.
+            if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.q_empty, (queries & 1) ^ 1)))) break;
+            ++queries;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&bar.q_full, p.tile_tokens * a.group * 128 * L::kHalves);
+#pragma unroll
+              for (int h = 0; h < L::kHalves; ++h)
+                tma_load_3d(smem_u32(q_s) + h * L::kQHalf, &q_map, h * 64, w.head * a.group, w.first_token, &bar.q_full);
+            }
+            __syncwarp();
+            ++q_loads;
+          }
+          if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.v_empty[s], parity)))) break;
+          load(w, j, page, &v_map, v_s, bar.v_full);
+          ++v_loads;
+          page = next;
+        }
+        if (!ok) break;
+      }
+      // Asked for late, while the last blocks are computed, so that an idle CTA is not left without.
+      if (lane == 0) {
+        fence_proxy_async_smem();  // the last answer has been read
+        mbar_arrive_expect_tx(&bar.next_here, 16);
+        ask_next_cta(answer, &bar.next_here);
+      }
+      __syncwarp();
+      if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.next_here, asked++ & 1)))) break;
+      index = __shfl_sync(0xffffffffu, next_cta(answer), 0);
+    }
+    if (ok) {
+      if (__all_sync(0xffffffffu, phase_wait(&bar.work_empty[t & 1], ((t >> 1) & 1) ^ 1)) && lane == 0) {
+        bar.work[t & 1].rows = -1;
+        bar.work[t & 1].blocks = 0;
+        mbar_arrive(&bar.work_full[t & 1]);
+      }
+      __syncwarp();
+      // No product's arrival on an empty barrier lands after the CTA has gone.
+      for (uint32_t e = g; e < g + L::kStages && ok; ++e) {
+        const uint32_t s = e % L::kStages, parity = ((e / L::kStages) & 1) ^ 1;
+        ok = phase_wait(&bar.k_empty[s], parity) && phase_wait(&bar.v_empty[s], parity);
+      }
+      if (ok) phase_wait(&bar.q_empty, (queries & 1) ^ 1);
     } else {
-      // ---------------- cleaning ----------------
-      uint32_t asked = 0;
-      for (int j = 0; j < blocks; ++j) {
+      // A wait ran out: wait (bounded) for what is still on its way to shared memory.
+      if (asked) phase_wait(&bar.next_here, (asked - 1) & 1);
+      if (q_loads) phase_wait(&bar.q_full, (q_loads - 1) & 1);
+      for (uint32_t back = 1; back <= L::kStages; ++back) {
+        if (k_loads >= back) phase_wait(&bar.k_full[(k_loads - back) % L::kStages], ((k_loads - back) / L::kStages) & 1);
+        if (v_loads >= back) phase_wait(&bar.v_full[(v_loads - back) % L::kStages], ((v_loads - back) / L::kStages) & 1);
+      }
+    }
+  } else if (warp == 7) {
+    // ---------------- cleaning ----------------
+    uint32_t asked = 0;
+    bool ok = true;
+    for (uint32_t t = 0; ok; ++t) {
+      if (!(ok = next_work(t))) break;
+      Work& w = bar.work[t & 1];
+      if (w.rows < 0) break;
+      for (int j = 0; j < w.blocks; ++j, ++g) {
         if (!partial_block(w, a.window, w.first + j)) continue;
-        const int s = j % L::kStages;
+        const uint32_t s = g % L::kStages;
         // Asked by the warp that has seen the block arrive.
-        if (!__all_sync(0xffffffffu, phase_wait(&bar.clean_ask, asked++ & 1) &&
-                                         phase_wait(&bar.v_full[s], (j / L::kStages) & 1)))
+        if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.clean_ask, asked++ & 1) &&
+                                               phase_wait(&bar.v_full[s], (g / L::kStages) & 1))))
           break;
-        const int kb = (w.first + j) * kKeys;
+        const int kb = (w.first + j) * kKeys, lo = w.lo - kb, hi = w.hi - kb;
         uint4* v = reinterpret_cast<uint4*>(v_s + s * L::kBlock);
         bool wild = false;
 #pragma unroll 4
         for (int i = lane; i < kKeys * D / 8; i += 32) {
-          const int key = kb + ((i >> 3) & (kKeys - 1));
+          const int key = (i >> 3) & (kKeys - 1);
           uint4 x = v[i];
-          if (key < w.lo || key >= w.hi) {
+          if (key < lo || key >= hi) {
             v[i] = make_uint4(0, 0, 0, 0);
             continue;
           }
@@ -512,176 +624,185 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
             wild = true;
           }
         }
-        if (wild) bar.wild = 1;
+        if (wild) w.wild = 1;
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar.v_clean);
       }
+      done_with(t);
     }
   } else {
-    // ---------------- softmax ----------------
-    if (row < w.rows) {
-      see_hi = w.pos0 + row / a.group;
-      if (a.window && see_hi - a.window + 1 > 0) see_lo = see_hi - a.window + 1;
-    }
+    // ---------------- softmax and output rows ----------------
+    const int row = threadIdx.x;
     const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
     const float scale = a.scale_log2;
     bool ok = true;
-    for (int j = 0; j < blocks; ++j) {
-      if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.s_full[j % L::kScores], (j / L::kScores) & 1)))) break;
-      tc_fence_after();
-      uint32_t s[2][32];
-      tmem_ld32(mine + L::kSCol + j % L::kScores * kKeys, s[0]);
-      tmem_ld32(mine + L::kSCol + j % L::kScores * kKeys + 32, s[1]);
-      tmem_wait_ld();
-      pin(s[0]);
-      pin(s[1]);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar.s_read[j % L::kScores]);
-      const int block = w.first + j;
-      if (partial_block(w, a.window, block)) {
-        const int hi = see_hi - block * kKeys, lo = see_lo - block * kKeys;
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (32 * c + i > hi || 32 * c + i < lo) s[c][i] = 0xff800000u;  // -infinity
+    for (uint32_t t = 0; ok; ++t) {
+      if (!(ok = next_work(t))) break;
+      const Work& w = bar.work[t & 1];
+      if (w.rows < 0) break;
+      // Row state; the row's keys are [see_lo, see_hi].
+      const int blocks = w.blocks;
+      int see_hi = -1, see_lo = 0;
+      float top = -INFINITY, sum = 0.f;
+      if (row < w.rows) {
+        see_hi = w.pos0 + row / a.group;
+        if (a.window && see_hi - a.window + 1 > 0) see_lo = see_hi - a.window + 1;
       }
-      float most[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) most[i] = __uint_as_float(s[0][i]);
-#pragma unroll
-      for (int i = 8; i < kKeys; i += 8)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) most[e] = fmaxf(most[e], __uint_as_float(s[(i + e) >> 5][(i + e) & 31]));
-      const float block_top = fmaxf(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])),
-                                    fmaxf(fmaxf(most[4], most[5]), fmaxf(most[6], most[7])));
-      const float now = fmaxf(top, block_top);
-      const bool fresh = top == -INFINITY;  // nothing summed yet, O is zero
-      if (fresh) top = now;
-      const bool move = !fresh && (now - top) * scale > 8.f;
-      if (__any_sync(0xffffffffu, move)) {
-        // O has to be at rest: the last product with V done; the next one waits for this block's P.
-        if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.o_done[(j - 1) & 1], ((j - 1) >> 1) & 1)))) break;
+      for (int j = 0; j < blocks; ++j, ++g) {
+        const uint32_t b = g % L::kScores;
+        if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.s_full[b], (g / L::kScores) & 1)))) break;
         tc_fence_after();
-        const float f = move ? exp2_approx((top - now) * scale) : 1.f;
-        sum *= f;
-        if (move) top = now;
+        uint32_t s[2][32];
+        tmem_ld32(mine + L::kSCol + b * kKeys, s[0]);
+        tmem_ld32(mine + L::kSCol + b * kKeys + 32, s[1]);
+        tmem_wait_ld();
+        pin(s[0]);
+        pin(s[1]);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.s_read[b]);
+        const int block = w.first + j;
+        if (partial_block(w, a.window, block)) {
+          const int hi = see_hi - block * kKeys, lo = see_lo - block * kKeys;
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (32 * c + i > hi || 32 * c + i < lo) s[c][i] = 0xff800000u;  // -infinity
+        }
+        float most[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most[i] = __uint_as_float(s[0][i]);
+#pragma unroll
+        for (int i = 8; i < kKeys; i += 8)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) most[e] = fmaxf(most[e], __uint_as_float(s[(i + e) >> 5][(i + e) & 31]));
+        const float block_top = fmaxf(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])),
+                                      fmaxf(fmaxf(most[4], most[5]), fmaxf(most[6], most[7])));
+        const float now = fmaxf(top, block_top);
+        const bool fresh = top == -INFINITY;  // nothing summed yet, O is zero
+        if (fresh) top = now;
+        const bool move = !fresh && (now - top) * scale > 8.f;
+        if (__any_sync(0xffffffffu, move)) {
+          // O has to be at rest: the last product with V done; the next one waits for this block's P.
+          if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1)))) break;
+          tc_fence_after();
+          const float f = move ? exp2_approx((top - now) * scale) : 1.f;
+          sum *= f;
+          if (move) top = now;
 #pragma unroll 1
-        for (int c = 0; c < D / 16; ++c) {
-          uint32_t o[16];
-          tmem_ld16(mine + L::kOCol + 16 * c, o);
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld16(mine + L::kOCol + 16 * c, o);
+            tmem_wait_ld();
+            pin(o);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st16(mine + L::kOCol + 16 * c, o);
+          }
+        }
+        const float from = (top == -INFINITY ? 0.f : top * scale) - kProbabilityShift<T>;
+        const float2 scale2 = make_float2(scale, scale), from2 = make_float2(-from, -from);
+        float2 add[4] = {};
+        uint32_t out[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const int c = i >> 4, e = (i & 15) * 2;
+          float2 x = __ffma2_rn(make_float2(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])), scale2, from2);
+          x.x = exp2_approx(x.x);
+          x.y = exp2_approx(x.y);
+          add[i & 3] = __fadd2_rn(add[i & 3], x);
+          out[i] = pack2<T>(x.x, x.y);
+        }
+        // The buffer's last P has to be used up.
+        if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.o_done[g & 1], ((g >> 1) & 1) ^ 1)))) break;
+        tc_fence_after();
+        tmem_st32(mine + L::kPCol + (g & 1) * (kKeys / 2), out);
+        const float2 both = __fadd2_rn(__fadd2_rn(add[0], add[1]), __fadd2_rn(add[2], add[3]));
+        sum += both.x + both.y;
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.p_full[g & 1]);
+      }
+      if (blocks && ok) ok = phase_wait(&bar.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) sum = __int_as_float(0x7fc00000);  // a wait ran out: no output that could pass for one
+
+      // ---- the tile's output
+      tc_fence_after();
+      const bool bad = w.bad, wild = w.wild, whole = w.parts == 1;
+      if (bad) sum = __int_as_float(0x7fc00000);
+      if (bad && row == 0) atomicOr(&g_device_error, kDeviceErrorIndex);
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const int i_token = row / a.group, token = w.first_token + i_token;
+      const int h = w.head * a.group + row - i_token * a.group;
+      const bool valid = row < w.rows;
+      const int64_t share = w.share;
+      const float top2 = top == -INFINITY ? top : top * scale;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        __syncwarp();
+        if (blocks) {
+          tmem_ld32(mine + L::kOCol + 32 * c, o);
           tmem_wait_ld();
           pin(o);
+        } else {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-          tmem_st16(mine + L::kOCol + 16 * c, o);
+          for (int i = 0; i < 32; ++i) o[i] = 0;
         }
-      }
-      const float from = (top == -INFINITY ? 0.f : top * scale) - kProbabilityShift<T>;
-      const float2 scale2 = make_float2(scale, scale), from2 = make_float2(-from, -from);
-      float2 add[4] = {};
-      uint32_t out[32];
+        if (wild && valid) {
+          // The infinities and NaNs taken out of V, added to a row that sees them.
+          for (int j = 0; j < blocks; ++j) {
+            if (!partial_block(w, a.window, w.first + j)) continue;
+            const int kb = (w.first + j) * kKeys;
+            for (int k = max(kb, see_lo); k <= min(kb + kKeys - 1, see_hi); ++k) {
+              const int32_t* entry = a.pages.page_table + (int64_t)w.r * a.pages.table_stride + (k >> a.pages.page_log2);
+              const int64_t page = __ldg(entry);
+              if (page < 0 || page >= a.pages.num_pages) continue;
+              const T* v = static_cast<const T*>(a.v) + page * a.v_page +
+                           (k & ((1 << a.pages.page_log2) - 1)) * a.v_slot + w.head * a.v_head + 32 * c;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const int c = i >> 4, e = (i & 15) * 2;
-        float2 x = __ffma2_rn(make_float2(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])), scale2, from2);
-        x.x = exp2_approx(x.x);
-        x.y = exp2_approx(x.y);
-        add[i & 3] = __fadd2_rn(add[i & 3], x);
-        out[i] = pack2<T>(x.x, x.y);
-      }
-      // The buffer's last P has to be used up.
-      if (j >= 2 && !(ok = __all_sync(0xffffffffu, phase_wait(&bar.o_done[j & 1], ((j - 2) >> 1) & 1)))) break;
-      tc_fence_after();
-      tmem_st32(mine + L::kPCol + (j & 1) * (kKeys / 2), out);
-      const float2 both = __fadd2_rn(__fadd2_rn(add[0], add[1]), __fadd2_rn(add[2], add[3]));
-      sum += both.x + both.y;
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar.p_full[j & 1]);
-    }
-    if (blocks && ok) ok = phase_wait(&bar.o_done[(blocks - 1) & 1], ((blocks - 1) >> 1) & 1);
-    if (!ok) sum = __int_as_float(0x7fc00000);  // a wait ran out: no output that could pass for one
-  }
-  __syncthreads();  // `bad` and `wild` are final
-
-  // ---- output
-  if (warp < 4) {
-    tc_fence_after();
-    const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
-    const bool bad = bar.bad, wild = bar.wild, whole = w.parts == 1;
-    const float nan = __int_as_float(0x7fc00000);
-    if (bad) sum = nan;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int t = row / a.group, g = row - t * a.group;
-    const int token = w.q.first + w.token0 + t;
-    const int h = w.head * a.group + g;
-    const bool valid = row < w.rows;
-    const int64_t slot = cut;  // of the cut items' shares
-    const float top2 = top == -INFINITY ? top : top * a.scale_log2;
-#pragma unroll 1
-    for (int c = 0; c < D / 32; ++c) {
-      uint32_t o[32];
-      __syncwarp();
-      if (blocks) {
-        tmem_ld32(mine + L::kOCol + 32 * c, o);
-        tmem_wait_ld();
-        pin(o);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = 0;
-      }
-      if (wild && valid) {
-        // The infinities and NaNs taken out of V, added to a row that sees them.
-        for (int j = 0; j < blocks; ++j) {
-          if (!partial_block(w, a.window, w.first + j)) continue;
-          const int kb = (w.first + j) * kKeys;
-          for (int k = max(kb, see_lo); k <= min(kb + kKeys - 1, see_hi); ++k) {
-            const int32_t* entry = a.pages.page_table + (int64_t)w.r * a.pages.table_stride + (k >> a.pages.page_log2);
-            const int64_t page = __ldg(entry);
-            if (page < 0 || page >= a.pages.num_pages) continue;
-            const T* v = static_cast<const T*>(a.v) + page * a.v_page +
-                         (k & ((1 << a.pages.page_log2) - 1)) * a.v_slot + w.head * a.v_head + 32 * c;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float x = (float)v[i];
-              if (!isfinite(x)) o[i] = __float_as_uint(__uint_as_float(o[i]) + x);
+              for (int i = 0; i < 32; ++i) {
+                const float x = (float)v[i];
+                if (!isfinite(x)) o[i] = __float_as_uint(__uint_as_float(o[i]) + x);
+              }
             }
           }
         }
-      }
-      if (!valid) continue;
-      if (whole) {
-        uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + token * a.out_n + (int64_t)h * a.out_h + 32 * c);
+        if (!valid) continue;
+        if (whole) {
+          uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + token * a.out_n + (int64_t)h * a.out_h + 32 * c);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t x[4];
+          for (int i = 0; i < 4; ++i) {
+            uint32_t x[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            x[e] = pack2<T>(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
-          out[i] = make_uint4(x[0], x[1], x[2], x[3]);
+            for (int e = 0; e < 4; ++e)
+              x[e] = pack2<T>(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv);
+            out[i] = make_uint4(x[0], x[1], x[2], x[3]);
+          }
+        } else {
+          float4* out = reinterpret_cast<float4*>(p.part_out + (share * kTile + row) * D + 32 * c);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            out[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
+                                 __uint_as_float(o[4 * i + 3]));
         }
-      } else {
-        float4* out = reinterpret_cast<float4*>(p.part_out + (slot * kTile + row) * D + 32 * c);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          out[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
-                               __uint_as_float(o[4 * i + 3]));
       }
-    }
-    if (valid) {
-      if (!whole) {
-        p.part_stat[(slot * kTile + row) * 2] = top2;
-        p.part_stat[(slot * kTile + row) * 2 + 1] = sum;
-      } else if (a.lse) {
-        a.lse[(int64_t)token * a.heads + h] = (top2 + log2f(sum) - kProbabilityShift<T>) * 0.6931471805599453f;
+      if (valid) {
+        if (!whole) {
+          p.part_stat[(share * kTile + row) * 2] = top2;
+          p.part_stat[(share * kTile + row) * 2 + 1] = sum;
+        } else if (a.lse) {
+          a.lse[(int64_t)token * a.heads + h] = (top2 + log2f(sum) - kProbabilityShift<T>) * 0.6931471805599453f;
+        }
       }
+      tc_fence_before();
+      done_with(t);
     }
   }
-  if (threadIdx.x == 0 && bar.bad) atomicOr(&g_device_error, kDeviceErrorIndex);
   tc_fence_before();
   __syncthreads();
   if (warp == 4) {
@@ -737,15 +858,27 @@ bool encode_cache(CUtensorMap* map, const void* base, int dtype, int D, int64_t 
                            dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// The rows as {D, heads, tokens}, a box of 64 columns x the query heads of a key head x a tile's tokens.
+bool encode_rows(CUtensorMap* map, const void* base, int dtype, int D, int64_t heads, int64_t tokens, int64_t s_head,
+                 int64_t s_token, int64_t group, int64_t tile_tokens) {
+  const uint64_t dims[3] = {(uint64_t)D, (uint64_t)heads, (uint64_t)tokens};
+  const uint64_t strides[2] = {heads > 1 ? (uint64_t)(2 * s_head) : 128, tokens > 1 ? (uint64_t)(2 * s_token) : 128};
+  for (uint64_t s : strides)
+    if (s == 0 || (int64_t)s < 0) return false;
+  const uint32_t box[3] = {64, (uint32_t)group, (uint32_t)tile_tokens};
+  return encode_tensor_map(map, dtype == 0 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base,
+                           dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 template <typename T, int D>
-cudaError_t launch(const CUtensorMap& k_map, const CUtensorMap& v_map, const PrefillArgs& p, int64_t items,
+cudaError_t launch(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map, const PrefillArgs& p, int64_t items,
                    cudaStream_t stream) {
   const void* fn = reinterpret_cast<const void*>(&paged_prefill_kernel<T, D>);
   cudaError_t err = allow_shared_memory(fn, Layout<D>::kSmem);
   if (err != cudaSuccess) return err;
   const int64_t cut = items - p.whole_items;
   err = launch_kernel(paged_prefill_kernel<T, D>, dim3((unsigned)(p.whole_items + cut * p.splits)), dim3(kPrefillThreads),
-                      Layout<D>::kSmem, stream, k_map, v_map, p);
+                      Layout<D>::kSmem, stream, q_map, k_map, v_map, p);
   if (err != cudaSuccess || p.splits == 1) return err;
   return launch_following(prefill_join_kernel<T, D>, dim3((unsigned)(cut * (kTile / 16))), dim3(512), stream, p);
 }
@@ -797,8 +930,9 @@ bool launch_paged_prefill(const AttentionArgs& a, const PrefillPlan& plan, int d
   p.box_rows = page_size < kKeys ? (int)page_size : kKeys;
   const int64_t items = plan.tiles * a.kv_heads;
   if (items * plan.splits * (kTile / 16) >= (int64_t(1) << 31)) return false;
-  CUtensorMap k_map, v_map;
-  if (!encode_cache(&k_map, a.k, dtype, D, page_size, a.kv_heads, a.pages.num_pages, a.k_slot, a.k_head, a.k_page,
+  CUtensorMap q_map, k_map, v_map;
+  if (!encode_rows(&q_map, a.q, dtype, D, a.heads, a.tokens, a.q_h, a.q_n, a.group, plan.tile_tokens) ||
+      !encode_cache(&k_map, a.k, dtype, D, page_size, a.kv_heads, a.pages.num_pages, a.k_slot, a.k_head, a.k_page,
                     p.box_rows) ||
       !encode_cache(&v_map, a.v, dtype, D, page_size, a.kv_heads, a.pages.num_pages, a.v_slot, a.v_head, a.v_page,
                     p.box_rows))
@@ -810,11 +944,11 @@ bool launch_paged_prefill(const AttentionArgs& a, const PrefillPlan& plan, int d
     p.joins = reinterpret_cast<Tile*>(p.part_stat + shares * kTile * 2);
   }
   if (D == 64)
-    *err = dtype == 0 ? launch<__nv_bfloat16, 64>(k_map, v_map, p, items, stream)
-                      : launch<__half, 64>(k_map, v_map, p, items, stream);
+    *err = dtype == 0 ? launch<__nv_bfloat16, 64>(q_map, k_map, v_map, p, items, stream)
+                      : launch<__half, 64>(q_map, k_map, v_map, p, items, stream);
   else
-    *err = dtype == 0 ? launch<__nv_bfloat16, 128>(k_map, v_map, p, items, stream)
-                      : launch<__half, 128>(k_map, v_map, p, items, stream);
+    *err = dtype == 0 ? launch<__nv_bfloat16, 128>(q_map, k_map, v_map, p, items, stream)
+                      : launch<__half, 128>(q_map, k_map, v_map, p, items, stream);
   return true;
 }
 
