@@ -11,9 +11,9 @@
 // and the probabilities have two buffers, so the product with V runs beside the
 // next softmax. With the output that is 256 columns of the 512, so two CTAs share
 // an SM and two warps a scheduler do softmax. Ragged chunks of up to 2,000 tokens
-// with a window of 1,024 keys, 16/4 heads x 64 FP16, a CTA a tile: 78 us;
-// probabilities over the scores they came from, with two buffers for both: 80 us;
-// one such buffer of 128 keys: 98 us.
+// with a window of 1,024 keys, 16/4 heads x 64 FP16, a CTA a tile: 81 us;
+// probabilities over the scores they came from, with two buffers for both: 83 us;
+// one such buffer of 128 keys: 101 us.
 //
 // A tile is the rows (query heads x whole tokens) of one key head that fit into
 // 128, and its blocks of keys (or a share of them where there are fewer tiles
@@ -21,8 +21,8 @@
 // in the grid, but one that runs takes over the tiles of those that have not
 // started (cluster launch control), so the start of a tile -- finding its
 // request, the pages' indices, the first loads and scores -- runs beside the last
-// softmax and output of the one before: about 2 us a tile instead of 7, and 65 us
-// for the chunks above. All buffers and their phases go on from tile to tile.
+// softmax and output of the one before: about 2 us a tile instead of 7 (78 to
+// 61 us for the chunks above). All buffers and their phases go on from tile to tile.
 //   warps 0-3  one row a thread: scores from tensor memory, running maximum
 //              and sum, probabilities to tensor memory, output to global memory;
 //   warp 4     issues S = Q K^T (both from shared memory);
@@ -76,6 +76,7 @@ struct Work {
   int pos0, pos1;   // positions of the first and last token
   int lo, hi;       // keys that some row sees
   int first, blocks;  // this split's blocks (of 64 keys)
+  int full0, full1;   // of them, those that every row sees whole: [full0, full1)
   int parts;        // splits that have blocks
   int share;        // where an item that is cut keeps this share
   int bad, wild;    // an index was out of range; V held infinities or NaNs in partial blocks
@@ -227,11 +228,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 template <typename T>
 constexpr uint32_t kExponent = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
 
-__device__ __forceinline__ bool partial_block(const Work& w, int window, int block) {
-  const int kb = block * kKeys;
-  return kb + kKeys - 1 > w.pos0 || (window && kb < w.pos1 - window + 1);
-}
-
 template <typename T, int D>
 __global__ void __launch_bounds__(kPrefillThreads, 2)
     paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
@@ -380,12 +376,13 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
     for (uint32_t t = 0; ok; ++t) {
       if (!(ok = next_work(t))) break;
       const Work& w = bar.work[t & 1];
-      const int n = __shfl_sync(0xffffffffu, w.blocks, 0);
+      const int n = __shfl_sync(0xffffffffu, w.blocks, 0), full0 = __shfl_sync(0xffffffffu, w.full0, 0),
+                full1 = __shfl_sync(0xffffffffu, w.full1, 0);
       if (w.rows < 0) break;
       for (int j = 0; j < n; ++j, ++g) {
         const uint32_t s = g % L::kStages;
         ok = phase_wait(&bar.v_full[s], (g / L::kStages) & 1);
-        const bool partial = partial_block(w, a.window, w.first + j);
+        const bool partial = j < full0 || j >= full1;
         if (partial && lane == 0) mbar_arrive(&bar.clean_ask);  // cleaned beside the block's softmax
         ok = ok && (!partial || phase_wait(&bar.v_clean, cleaned & 1)) && phase_wait(&bar.p_full[g & 1], (g >> 1) & 1);
         cleaned += partial;
@@ -472,6 +469,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       w.parts = blocks && splits > 1 ? (blocks + share - 1) / share : 1;
       w.first = first + split * share;
       w.blocks = max(min(first + blocks, w.first + share) - w.first, 0);
+      w.full0 = a.window ? max((max(w.pos1 - a.window + 1, 0) + kKeys - 1) / kKeys - w.first, 0) : 0;
+      w.full1 = (w.pos0 + 1) / kKeys - w.first;
       w.share = cut;
       w.bad = too_long;
       w.wild = 0;
@@ -483,20 +482,21 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       }
       return split < w.parts;
     };
-    // The page of this lane's box of a block, -1 where there is nothing to load.
-    const auto page_of = [&](const Work& w, int j, int* bad) {
-      int page = -1;
-      if (lane < boxes && j < w.blocks) {
-        const int key = (w.first + j) * kKeys + lane * p.box_rows;
-        if (key < w.hi && key + p.box_rows > w.lo) {
-          page = __ldg(a.pages.page_table + w.r * a.pages.table_stride + (key >> a.pages.page_log2));
-          if (page < 0 || page >= a.pages.num_pages) {
-            page = -1;
-            *bad = 1;
-          }
-        }
-      }
-      return page;
+    // This lane has a box of the block to load.
+    const auto has_box = [&](const Work& w, int j) {
+      const int key = (w.first + j) * kKeys + lane * p.box_rows;
+      return lane < boxes && j < w.blocks && key < w.hi && key + p.box_rows > w.lo;
+    };
+    // Its entry of the page table, read a block ahead and checked when the box is loaded (-1: nothing to load).
+    const auto entry_of = [&](const Work& w, int j) {
+      const int key = (w.first + j) * kKeys + lane * p.box_rows;
+      return has_box(w, j) ? __ldg(a.pages.page_table + w.r * a.pages.table_stride + (key >> a.pages.page_log2)) : -1;
+    };
+    const auto page_of = [&](const Work& w, int j, int entry, int* bad) {
+      if (!has_box(w, j)) return -1;
+      if (entry >= 0 && entry < a.pages.num_pages) return entry;
+      *bad = 1;
+      return -1;
     };
     const auto load = [&](const Work& w, int j, int page, const CUtensorMap* map, unsigned char* ring, uint64_t* full) {
       const uint32_t s = g % L::kStages, count = __popc(__ballot_sync(0xffffffffu, page >= 0));
@@ -518,8 +518,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       Work w;
       if (describe(index, w)) {
         Work& slot = bar.work[t & 1];
-        int page = page_of(w, 0, &w.bad);
-        w.bad = __any_sync(0xffffffffu, w.bad);
+        int entry = entry_of(w, 0);
         if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.work_empty[t & 1], ((t >> 1) & 1) ^ 1)))) break;
         if (lane == 0) {
           slot = w;
@@ -529,7 +528,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
         ++t;
         for (int j = 0; j < w.blocks; ++j, ++g) {
           const uint32_t s = g % L::kStages, parity = ((g / L::kStages) & 1) ^ 1;
-          const int next = page_of(w, j + 1, &slot.bad);
+          const int page = page_of(w, j, entry, &slot.bad);
+          entry = entry_of(w, j + 1);
           if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.k_empty[s], parity)))) break;
           load(w, j, page, &k_map, k_s, bar.k_full);
           ++k_loads;
@@ -549,7 +549,6 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
           if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.v_empty[s], parity)))) break;
           load(w, j, page, &v_map, v_s, bar.v_full);
           ++v_loads;
-          page = next;
         }
         if (!ok) break;
       }
@@ -593,8 +592,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       if (!(ok = next_work(t))) break;
       Work& w = bar.work[t & 1];
       if (w.rows < 0) break;
-      for (int j = 0; j < w.blocks; ++j, ++g) {
-        if (!partial_block(w, a.window, w.first + j)) continue;
+      const int n = w.blocks, full0 = w.full0, full1 = w.full1;
+      for (int j = 0; j < n; ++j, ++g) {
+        if (j >= full0 && j < full1) continue;
         const uint32_t s = g % L::kStages;
         // Asked by the warp that has seen the block arrive.
         if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.clean_ask, asked++ & 1) &&
@@ -642,7 +642,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       const Work& w = bar.work[t & 1];
       if (w.rows < 0) break;
       // Row state; the row's keys are [see_lo, see_hi].
-      const int blocks = w.blocks;
+      const int blocks = w.blocks, first = w.first, full0 = w.full0, full1 = w.full1;
       int see_hi = -1, see_lo = 0;
       float top = -INFINITY, sum = 0.f;
       if (row < w.rows) {
@@ -662,9 +662,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar.s_read[b]);
-        const int block = w.first + j;
-        if (partial_block(w, a.window, block)) {
-          const int hi = see_hi - block * kKeys, lo = see_lo - block * kKeys;
+        if (j < full0 || j >= full1) {
+          const int hi = see_hi - (first + j) * kKeys, lo = see_lo - (first + j) * kKeys;
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -756,8 +755,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
         if (wild && valid) {
           // The infinities and NaNs taken out of V, added to a row that sees them.
           for (int j = 0; j < blocks; ++j) {
-            if (!partial_block(w, a.window, w.first + j)) continue;
-            const int kb = (w.first + j) * kKeys;
+            if (j >= full0 && j < full1) continue;
+            const int kb = (first + j) * kKeys;
             for (int k = max(kb, see_lo); k <= min(kb + kKeys - 1, see_hi); ++k) {
               const int32_t* entry = a.pages.page_table + (int64_t)w.r * a.pages.table_stride + (k >> a.pages.page_log2);
               const int64_t page = __ldg(entry);
