@@ -884,11 +884,15 @@ cudaError_t launch(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUt
 
 }  // namespace
 
+constexpr int kMostShares = 2;  // for each CTA that the device holds
+
 // Tiles, and the shares that blocks are cut into. The GPU holds 2 CTAs an SM;
 // the items that would leave its last round partly empty (all of them, where
-// there are few) are cut so that they fill it. Lengths are only known on the
-// device: the bound on the shares is the page table's width. 4,096 tokens over
-// 16,384 keys, 32/8 heads x 128 (1,024 items, 3.46 rounds): 1,075 us with whole items, 1,046 us so.
+// there are few) are cut where the rounds of their shares are shorter together.
+// Lengths are only known on the device: the bound on the shares is the page
+// table's width. 32/8 heads x 128, whole items against shares: 4,096 tokens over
+// 16,384 keys (1,024 items, 3.46 rounds) 1,075 and 1,046 us; 16 requests of 4,096
+// keys, 6 tokens each (128 items) 78 and 57 us, 64 tokens each (256) 96 and 84 us.
 PrefillPlan plan_paged_prefill(int64_t tokens, int64_t batch, bool ragged, int64_t kv_heads, int64_t group, int D,
                                int64_t max_keys, int64_t window, int sms) {
   PrefillPlan p{};
@@ -899,23 +903,32 @@ PrefillPlan plan_paged_prefill(int64_t tokens, int64_t batch, bool ragged, int64
     const int64_t ends = (tokens < batch ? tokens : batch) + 1;
     p.tiles = (tokens + ends * (p.tile_tokens - 1)) / p.tile_tokens;
   }
+  // Tiles that there are likely to be (requests of the same size): those beyond them come first and end at once.
+  const int64_t asked = tokens < batch ? tokens : batch, each = (tokens + asked - 1) / asked;
+  const int64_t likely = asked * ((each + p.tile_tokens - 1) / p.tile_tokens);
   const int64_t items = p.tiles * kv_heads, slots = 2 * (int64_t)sms;
-  const int64_t cut = items % slots;
+  const int64_t real = likely < p.tiles ? likely * kv_heads : items, cut = real % slots;
   p.whole_items = items - cut;
   p.splits = 1;
   if (cut) {
     const int64_t keys = window && window + p.tile_tokens < max_keys ? window + p.tile_tokens : max_keys;
-    const int64_t most = (keys / kKeys + 5) / 4;  // shares of at least four blocks
-    const int64_t splits = slots / cut < most ? slots / cut : most;
-    if (splits > 1) p.splits = (int)splits;
+    const int64_t blocks = keys / kKeys + 1, most = (blocks + 4) / 4;  // shares of at least four blocks
+    // Rounds times a share's blocks, with about 3 for its start and end and 3 for the join.
+    int64_t least = blocks + 3;
+    for (int64_t s = 2; s <= most && cut * s <= kMostShares * slots; ++s) {
+      const int64_t cost = (cut * s + slots - 1) / slots * ((blocks + s - 1) / s + 3) + 3;
+      if (cost < least) {
+        least = cost;
+        p.splits = (int)s;
+      }
+    }
   }
   if (p.splits == 1) p.whole_items = items;
   return p;
 }
 
-// At most one share a CTA that the device holds.
 size_t paged_prefill_workspace(int D, int sms) {
-  return (size_t)(2 * sms) * (kTile * (size_t)(D + 2) * sizeof(float) + sizeof(Tile));
+  return (size_t)(kMostShares * 2 * sms) * (kTile * (size_t)(D + 2) * sizeof(float) + sizeof(Tile));
 }
 
 bool launch_paged_prefill(const AttentionArgs& a, const PrefillPlan& plan, int dtype, int D, int64_t page_size,
