@@ -227,6 +227,18 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 }
 template <typename T>
 constexpr uint32_t kExponent = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+// Bits 15 and 31 of the result: infinity or NaN in either half of a pair of 16-bit values.
+template <typename T>
+__device__ __forceinline__ uint32_t non_finite(uint32_t pair) {
+  constexpr uint32_t step = 0x8000u - kExponent<T>;  // carries an exponent of ones into the sign's place
+  return ((pair & 0x7fff7fffu) + (step << 16 | step)) & 0x80008000u;
+}
+// The pair with such values replaced by zero.
+template <typename T>
+__device__ __forceinline__ uint32_t finite_only(uint32_t pair) {
+  const uint32_t n = non_finite<T>(pair);
+  return pair & ~((n >> 15) * 0xffffu);
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kPrefillThreads, 2)
@@ -603,25 +615,22 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
         const int kb = (w.first + j) * kKeys, lo = w.lo - kb, hi = w.hi - kb;
         uint4* v = reinterpret_cast<uint4*>(v_s + s * L::kBlock);
         bool wild = false;
-#pragma unroll 4
-        for (int i = lane; i < kKeys * D / 8; i += 32) {
-          const int key = (i >> 3) & (kKeys - 1);
-          uint4 x = v[i];
-          if (key < lo || key >= hi) {
-            v[i] = make_uint4(0, 0, 0, 0);
-            continue;
-          }
-          uint32_t* word = reinterpret_cast<uint32_t*>(&x);
-          bool changed = false;
+        constexpr int kFlight = 8;
+#pragma unroll 1
+        for (int i0 = lane; i0 < kKeys * D / 8; i0 += 32 * kFlight) {
+          uint4 x[kFlight];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            constexpr uint32_t m = kExponent<T>;
-            if ((word[e] & m) == m) { word[e] &= 0xffff0000u; changed = true; }
-            if ((word[e] >> 16 & m) == m) { word[e] &= 0x0000ffffu; changed = true; }
-          }
-          if (changed) {
-            v[i] = x;
-            wild = true;
+          for (int f = 0; f < kFlight; ++f) x[f] = v[i0 + 32 * f];
+#pragma unroll
+          for (int f = 0; f < kFlight; ++f) {
+            const int i = i0 + 32 * f, key = (i >> 3) & (kKeys - 1);
+            if (key < lo || key >= hi) {
+              v[i] = make_uint4(0, 0, 0, 0);
+            } else if (non_finite<T>(x[f].x) | non_finite<T>(x[f].y) | non_finite<T>(x[f].z) | non_finite<T>(x[f].w)) {
+              v[i] = make_uint4(finite_only<T>(x[f].x), finite_only<T>(x[f].y), finite_only<T>(x[f].z),
+                                finite_only<T>(x[f].w));
+              wild = true;
+            }
           }
         }
         if (wild) w.wild = 1;
