@@ -893,7 +893,7 @@ cudaError_t launch(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUt
 
 }  // namespace
 
-constexpr int kMostShares = 2;  // for each CTA that the device holds
+constexpr int kMostShares = 3;  // for each CTA that the device holds
 
 // Tiles, and the shares that blocks are cut into. The GPU holds 2 CTAs an SM;
 // the items that would leave its last round partly empty (all of them, where
@@ -917,14 +917,16 @@ PrefillPlan plan_paged_prefill(int64_t tokens, int64_t batch, bool ragged, int64
   const int64_t likely = asked * ((each + p.tile_tokens - 1) / p.tile_tokens);
   const int64_t items = p.tiles * kv_heads, slots = 2 * (int64_t)sms;
   const int64_t real = likely < p.tiles ? likely * kv_heads : items, cut = real % slots;
-  p.whole_items = items - cut;
+  // Where all may run at once, none is left whole: it would take as long as all its keys.
+  const int64_t room = real < slots ? items : cut;
+  p.whole_items = items - room;
   p.splits = 1;
   if (cut) {
     const int64_t keys = window && window + p.tile_tokens < max_keys ? window + p.tile_tokens : max_keys;
     const int64_t blocks = keys / kKeys + 1, most = (blocks + 4) / 4;  // shares of at least four blocks
     // Rounds times a share's blocks, with about 3 for its start and end and 3 for the join.
     int64_t least = blocks + 3;
-    for (int64_t s = 2; s <= most && cut * s <= kMostShares * slots; ++s) {
+    for (int64_t s = 2; s <= most && room * s <= kMostShares * slots; ++s) {
       const int64_t cost = (cut * s + slots - 1) / slots * ((blocks + s - 1) / s + 3) + 3;
       if (cost < least) {
         least = cost;

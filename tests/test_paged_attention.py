@@ -126,6 +126,19 @@ def test_few_items_over_many_ctas(news, totals, Hq, Hk, D, window):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("news,totals", [
+    ([900, 0, 1300, 5], [900, 40, 2000, 1100]),   # more tiles than the GPU holds at once
+    ([1] * 300 + [1500], [9] * 300 + [1500]),     # most of them of other requests than the last
+    ([40, 3, 25, 1], [3000, 2500, 2900, 900]),    # few, of uneven requests: keys shared out
+])
+@pytest.mark.parametrize("Hq,Hk,D,dtype,window", [(32, 2, 64, FP16, 0), (32, 2, 128, BF16, 100), (12, 4, 128, FP16, 0)])
+def test_many_and_few_tiles(news, totals, Hq, Hk, D, dtype, window):
+    req = Requests(news, totals, Hq, Hk, D, 16, dtype)
+    rows = None if sum(news) <= 350 else list(range(0, sum(news), 37)) + [sum(news) - 1]
+    _check(req, req.q.to(dtype), window=window, rows=rows)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("news,totals", [([4, 3], [2, 5]), ([6, 2], [0, 2]), ([40], [10])])
 def test_rows_without_keys_are_zero(news, totals):
     req = Requests(news, totals, 8, 2, 64, 8, BF16)
