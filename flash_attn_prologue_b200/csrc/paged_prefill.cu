@@ -21,7 +21,7 @@
 // in the grid, but one that runs takes over the tiles of those that have not
 // started (cluster launch control), so the start of a tile -- finding its
 // request, the pages' indices, the first loads and scores -- runs beside the last
-// softmax and output of the one before: about 2 us a tile instead of 7 (78 to
+// softmax and output of the one before: 2 to 3 us a tile instead of 7 (78 to
 // 61 us for the chunks above). All buffers and their phases go on from tile to tile.
 //   warps 0-3  one row a thread: scores from tensor memory, running maximum
 //              and sum, probabilities to tensor memory, output to global memory;
@@ -39,8 +39,9 @@
 //
 // Scores, statistics, sums and O are FP32; the probabilities are rounded to the
 // cache's type for the second product (their sum is taken before the rounding),
-// an error of the size of the output's own rounding. Waits are bounded; tensor
-// memory is released on every path.
+// an error of the size of the output's own rounding. Waits are bounded: where one
+// runs out the error word is set, the tile's rows are NaN, and the CTA ends (a tile
+// that it had taken over may stay unwritten). Tensor memory is released on every path.
 #include "paged_attention.h"
 #include "tensor_map.h"
 #include "umma_util.cuh"
