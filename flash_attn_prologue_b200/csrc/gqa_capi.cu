@@ -258,6 +258,7 @@ int flash_prologue_append_paged(const flash_prologue_append_args* a, void* strea
   g.w = a->rmsnorm_weight;
   g.scales = a->scales;
   g.tab = tables_of(a->rotation);
+  g.append = true;
   g.paged = paged_target(c);
   g.B = 1;
   g.N = a->tokens;

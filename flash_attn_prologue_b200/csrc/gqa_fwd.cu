@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(kThreads, 3) gqa_fwd_kernel(const GqaFwdArgs a
   const int hslot = slot & (HS - 1), tslot = slot >> a.p.log2_hs;
   // Items, tokens and rows are counted in 32 bits (the host checks): fewer registers and no 64-bit division.
   const int items = (int)(a.p.groups * a.p.slices), warps = gridDim.x * kWarps, tokens = (int)(a.B * a.N), N = (int)a.N;
-  const bool paged = a.paged.page_table != nullptr;
+  const bool paged = a.append;  // the table may be null: one without columns has no address
   const int q_iters = a.p.iters[0], qk_iters = q_iters + a.p.iters[1], all_iters = qk_iters + a.p.iters[2];
 
   // The loads' walk over the warp's row blocks: for each of its token groups the

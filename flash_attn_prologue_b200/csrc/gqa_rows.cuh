@@ -56,7 +56,8 @@ struct GqaFwdArgs {
   const float* w;      // [2, D] or null (rotation only)
   const float* scales; // [Hq] or null
   GqaTables tab;
-  PagedTarget paged;   // page_table null: dense k_out
+  bool append;         // K and V go to the pages of `paged`, else to dense outputs
+  PagedTarget paged;
   int64_t B, N;
   int H[3];
   float eps;

@@ -108,6 +108,30 @@ def test_indices_out_of_range_are_not_followed():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("ragged", [True, False])
+@pytest.mark.parametrize("pages", [5, 0])
+def test_requests_without_pages_write_nothing(pages, ragged):
+    """A page table without columns (its tensor has no address), with and without a cache behind it."""
+    g = torch.Generator(device="cuda").manual_seed(0)
+    news = [4, 0, 2] if ragged else [1, 1, 1]
+    q, k, v = (torch.randn(sum(news), h, 64, generator=g, device="cuda").to(BF16) for h in (8, 2, 2))
+    w, s = torch.ones(2, 1, 64, device="cuda"), torch.zeros(8, 1, 1, device="cuda")
+    caches = [torch.randn(pages, 16, 2, 64, generator=g, device="cuda").to(BF16) for _ in range(2)]
+    kept = [c.clone() for c in caches]
+    table = torch.zeros(3, 0, dtype=torch.int32, device="cuda")
+    lens = torch.tensor(news, dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0] + news).cumsum(0).to(torch.int32).cuda() if ragged else None
+    _lib.device_error()
+    got = fap.append_paged_kv(q, k, v, w, s, *tables(8, 64), *caches, table, lens, cu)
+    assert _lib.device_error() == 2
+    assert got.shape == q.shape and not got.any()
+    assert all(torch.equal(a, b) for a, b in zip(caches, kept))
+    out, lse = fap.paged_attention(q, *caches, table, lens, cu, return_lse=True)
+    assert _lib.device_error() == 2
+    assert out.isnan().all() and lse.isnan().all()
+
+
+@pytest.mark.gpu
 def test_padding_tokens_come_back_as_zeros():
     req = Requests([4, 3, 2], [20, 3, 9], 8, 2, 64, 8, BF16)
     args = _inputs(req, 8, 2, 64, BF16)
