@@ -42,14 +42,20 @@ struct Request {
   int total;   // tokens in the cache
 };
 
+// Requests that a kernel goes through: split by cu_seqlens, two more than there
+// are, for the rows behind the last request and before the first.
+__device__ __forceinline__ int requests_of(const PagedTarget& p) { return p.batch + (p.cu_seqlens ? 2 : 0); }
+
 // Sizes are clamped to what the tensors hold, so wrong ones cannot lead outside
-// them. r == batch is the padding behind the last request: tokens without keys.
+// them. r == batch is the padding behind the last request, r == batch + 1 that
+// before the first: tokens without keys.
 // The host keeps tokens x heads below 2^31 and max_keys below 2^30.
 __device__ __forceinline__ Request request_at(const PagedTarget& p, int tokens, int max_keys, int r, bool* too_long) {
   Request q;
   const int total = r < p.batch ? __ldg(p.seq_lens + r) : 0;
   if (p.cu_seqlens) {
-    const int a = __ldg(p.cu_seqlens + r), b = r < p.batch ? __ldg(p.cu_seqlens + r + 1) : tokens;
+    const int a = r <= p.batch ? __ldg(p.cu_seqlens + r) : 0;
+    const int b = r < p.batch ? __ldg(p.cu_seqlens + r + 1) : r == p.batch ? tokens : __ldg(p.cu_seqlens);
     q.first = min(max(a, 0), tokens);
     q.news = min(max(b, q.first), tokens) - q.first;
   } else {

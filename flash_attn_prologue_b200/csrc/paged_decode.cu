@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
   __shared__ float stat[kDecodeWarps][kRows][2];
   __shared__ int bad_page;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int batch = a.pages.batch + (a.pages.cu_seqlens ? 1 : 0);
+  const int batch = requests_of(a.pages);
   const uint32_t ring = smem_u32(smem) + warp * kRing * kStepBytes;
 
   if (!a.whole) start_next_kernel();
@@ -636,7 +636,7 @@ cudaError_t launch(AttentionArgs a, cudaStream_t stream) {
   cudaError_t err = allow_shared_memory(fn, smem);
   if (err != cudaSuccess) return err;
   // Never more CTAs than there can be units.
-  const int64_t tiles = (int64_t)a.tokens * a.group / kRows + (a.tokens < a.pages.batch ? a.tokens : a.pages.batch) + 1;
+  const int64_t tiles = (int64_t)a.tokens * a.group / kRows + (a.tokens < a.pages.batch + 2 ? a.tokens : a.pages.batch + 2);
   const int64_t blocks = a.whole ? 1 : a.max_keys / kBlockKeys + 1;
   int dev = 0, sms = 0;
   if ((err = cudaGetDevice(&dev)) != cudaSuccess ||

@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (p.splits > 1) start_next_kernel();
-  const int requests = a.pages.batch + (a.pages.cu_seqlens ? 1 : 0);
+  const int requests = requests_of(a.pages);
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::kStages; ++s) {
       mbar_init(&bar.k_full[s], 1);
@@ -909,8 +909,8 @@ PrefillPlan plan_paged_prefill(int64_t tokens, int64_t batch, bool ragged, int64
   p.tile_tokens = (int)(kTile / group);
   p.tiles = tokens;
   if (ragged) {
-    // Every request (and the padding) may leave its last tile partly empty.
-    const int64_t ends = (tokens < batch ? tokens : batch) + 1;
+    // Every request (and the padding on either side) may leave its last tile partly empty.
+    const int64_t ends = tokens < batch + 2 ? tokens : batch + 2;
     p.tiles = (tokens + ends * (p.tile_tokens - 1)) / p.tile_tokens;
   }
   // Tiles that there are likely to be (requests of the same size): those beyond them come first and end at once.

@@ -535,7 +535,7 @@ typedef struct flash_prologue_append_args {
 /*
  * The prologue on a step's new tokens, each turned by its position in its
  * request, with K and V written to the cache and Q to q_out. Tokens past the
- * last request get zero Q rows and no cache write, like tokens whose position,
+ * last request or before the first get zero Q rows and no cache write, like tokens whose position,
  * page or table row is out of range (which also set the error word).
  */
 FLASH_PROLOGUE_API int flash_prologue_append_paged(const flash_prologue_append_args* args, void* stream);
@@ -559,7 +559,7 @@ typedef struct flash_prologue_attention_args {
  * h / (Hq / Hk). BF16 or FP16, D in {64, 128}; scores, statistics and sums are
  * FP32. Keys that a token does not see never reach it, whatever their slots
  * hold. A token that sees no key (position below 0, padding past the last
- * request) gets zeros and an lse of -infinity; one that needs a page outside
+ * request or before the first) gets zeros and an lse of -infinity; one that needs a page outside
  * the cache gets NaN, and the error word. Results are the same run to run.
  * Rows and caches are 16-byte aligned. workspace: 16-byte aligned, at least
  * flash_prologue_paged_attention_workspace_size() bytes, no initialisation.

@@ -234,6 +234,30 @@ def test_padding_rows_are_zero(chunk):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("news,totals,ahead", [
+    ([1, 0, 1, 3, 1, 1], [40, 9, 1, 250, 66, 130], 5),      # single-token kernel, short caches
+    ([2, 1, 0, 1, 1, 1], [3000, 70, 4, 900, 64, 333], 7),   # split over CTAs
+    ([60, 2], [90, 9], 5),                                  # 128-row tiles
+    ([70, 2], [1500, 2], 300),                              # keys shared out
+])
+@pytest.mark.parametrize("D,window", [(64, 0), (128, 50)])
+def test_rows_before_the_first_request_are_zero(news, totals, ahead, D, window):
+    """cu_seqlens that begin behind 0, as append_paged_kv takes them."""
+    req = Requests(news, totals, 8, 2, D, 16, BF16)
+    q = torch.cat((torch.ones(ahead, 8, D, device="cuda"), req.q, torch.ones(2, 8, D, device="cuda"))).to(BF16)
+    torch.full((4, *q.shape), math.nan, dtype=BF16, device="cuda")  # what an unwritten output may come to lie in
+    scale = D ** -0.5
+    out, lse = fap.paged_attention(q, req.k, req.v, req.table, req.seq_lens, req.cu + ahead, softmax_scale=scale,
+                                   window=window, return_lse=True)
+    for rows in (slice(0, ahead), slice(-2, None)):
+        assert (out[rows] == 0).all() and (lse[rows] == -math.inf).all()
+    exact, size, exact_lse = _exact(req, q[ahead:-2], scale, window)
+    u = HALF_ULP[BF16]
+    assert ((out[ahead:-2].double() - exact).abs() <= u * exact.abs() + (u + SCORE) * size + 1e-30).all()
+    assert ((lse[ahead:-2].double() - exact_lse).abs() <= SCORE).all()
+
+
+@pytest.mark.gpu
 def test_wrong_splits_stay_inside_the_rows():
     """cu_seqlens that run backwards or past the rows are cut to them; nothing faults."""
     req = Requests([20, 20], [50, 50], 8, 2, 64, 16, BF16)
