@@ -1,5 +1,6 @@
 // C ABI of paged attention: argument checks and the choice of kernel.
 // Declarations: include/flash_prologue.h.
+#include <float.h>
 #include <math.h>
 
 #include "paged_attention.h"
@@ -19,8 +20,12 @@ int device_sms() {
   return sms;
 }
 
+// The factor of the scores' base-2 exponentials.
+double scale_log2_of(const flash_prologue_attention_args* a) { return a->softmax_scale * 1.4426950408889634; }
+
 int size_checks(const flash_prologue_attention_args* a) {
-  if (!a || a->tokens < 0 || a->window < 0 || !isfinite(a->softmax_scale) || a->Hq < 0 || a->Hk <= 0 || a->Hq % a->Hk)
+  if (!a || a->tokens < 0 || a->window < 0 || !(fabs(scale_log2_of(a)) <= FLT_MAX) || a->Hq < 0 || a->Hk <= 0 ||
+      a->Hq % a->Hk)
     return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
   if ((a->dtype != FLASH_PROLOGUE_BF16 && a->dtype != FLASH_PROLOGUE_FP16) || a->Hq > kMaxGqaHeads ||
       (a->D != 64 && a->D != 128) || a->tokens >= (int64_t(1) << 31) / kMaxGqaHeads)
@@ -30,11 +35,12 @@ int size_checks(const flash_prologue_attention_args* a) {
 
 // Tiles of 128 rows on the tensor cores where the requests have more rows a key
 // head than the other kernel's 16-row tile on average. The tiled kernel takes
-// the maximum of the unscaled scores, so the scale has to be positive, and a
-// tile holds at least one whole token.
-bool use_prefill(const flash_prologue_attention_args* a) {
+// the maximum of the unscaled scores and multiplies masked ones (-infinity) by the
+// scale, so the FP32 scale has to be positive (and normal), and a tile holds at
+// least one whole token.
+bool use_prefill(const flash_prologue_attention_args* a, float scale_log2) {
   const int64_t group = a->Hq / a->Hk;
-  return a->tokens * group > 16 * a->cache.batch && group <= 128 && a->softmax_scale > 0;
+  return a->tokens * group > 16 * a->cache.batch && group <= 128 && scale_log2 >= FLT_MIN;
 }
 
 size_t workspace_of(int64_t D, int sms) {
@@ -58,8 +64,8 @@ int flash_prologue_paged_attention_workspace_size(int64_t D, size_t* bytes) {
 
 int flash_prologue_paged_attention(const flash_prologue_attention_args* a, void* stream) {
   const int st = size_checks(a);
-  const flash_prologue_cache& c = a->cache;
   if (st != FLASH_PROLOGUE_OK || a->tokens == 0 || a->Hq == 0) return st;
+  const flash_prologue_cache& c = a->cache;
   if (!a->q.data || !a->out.data) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
   if ((reinterpret_cast<uintptr_t>(a->q.data) | reinterpret_cast<uintptr_t>(a->out.data)) & 15 ||
       ((a->q.n | a->q.h | a->out.n | a->out.h) & 7))
@@ -91,11 +97,11 @@ int flash_prologue_paged_attention(const flash_prologue_attention_args* a, void*
   g.heads = (int)a->Hq;
   g.kv_heads = (int)a->Hk;
   g.group = g.heads / g.kv_heads;
-  g.scale_log2 = (float)(a->softmax_scale * 1.4426950408889634);
+  g.scale_log2 = (float)scale_log2_of(a);
   g.workspace = a->workspace;
   g.max_keys = (int)(c.max_pages * c.page_size);
   g.window = a->window < g.max_keys ? (int)a->window : 0;  // as long as any request: all keys
-  if (use_prefill(a)) {
+  if (use_prefill(a, g.scale_log2)) {
     const PrefillPlan plan = plan_paged_prefill(a->tokens, c.batch, c.cu_seqlens != nullptr, a->Hk, g.group, (int)a->D,
                                                 g.max_keys, g.window, sms);
     cudaError_t err = cudaSuccess;

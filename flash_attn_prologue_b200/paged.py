@@ -127,6 +127,7 @@ def append_paged_kv(q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache,
 
 
 ATTENTION_HEAD_DIMS = (64, 128)
+LARGEST_SCALE = 2.0 ** 127  # times log2(e) it is still an FP32 number
 _WORKSPACE_BYTES = {}
 
 
@@ -159,8 +160,8 @@ def _attention(q, k_cache, v_cache, page_table, seq_lens, cu_seqlens, softmax_sc
     cache = _checked_cache(q, kv_heads, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
     if kv_heads <= 0 or heads <= 0 or heads % kv_heads or heads > MAX_HEADS:
         raise ValueError(f"query heads must be a multiple of the key heads and at most {MAX_HEADS}")
-    if not -math.inf < softmax_scale < math.inf:
-        raise ValueError("softmax_scale must be finite")
+    if not -LARGEST_SCALE < softmax_scale < LARGEST_SCALE:
+        raise ValueError("softmax_scale must be finite, and in FP32 too")
     if window < 0:
         raise ValueError("window must be 0 (all keys) or positive")
     device = q.device

@@ -193,6 +193,15 @@ def test_large_scores_pick_one_key_and_scales():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("news", [[3, 1], [40, 3]])
+@pytest.mark.parametrize("scale", [1e-50, 1e-44, 1e-39, 1e-37, -1e-50])
+def test_scales_that_vanish_in_fp32(scale, news):
+    """Equal weights, whether the scale rounds to 0, to a subnormal number or to a very small one."""
+    req = Requests(news, [45, 400], 8, 2, 64, 16, BF16)
+    _check(req, req.q.to(BF16), scale=scale)
+
+
+@pytest.mark.gpu
 def test_requests_share_pages_and_strided_rows():
     req = Requests([1, 1, 50], [40, 33, 90], 8, 2, 128, 16, BF16, share=True)
     wide = torch.randn(52, 14, 128, device="cuda").to(BF16)
@@ -376,6 +385,8 @@ def _cpu_call(**change):
     (dict(seq_lens=torch.ones(3, dtype=torch.int64)), "int32"),
     (dict(cu_seqlens=torch.zeros(3, dtype=torch.int32)), "cu_seqlens must be"),
     (dict(softmax_scale=math.nan), "softmax_scale"),
+    (dict(softmax_scale=3e38), "softmax_scale"),
+    (dict(softmax_scale=-1e300), "softmax_scale"),
     (dict(window=-1), "window"),
     (dict(q=torch.zeros(3, 8, 64, dtype=BF16, requires_grad=True)), "not differentiable"),
     (dict(), "CUDA devices only"),
@@ -396,7 +407,7 @@ def test_c_abi_refusals():
 
     assert call(T=0, batch=0, ptr=0) == _lib.OK
     for wrong, status in ((dict(dtype=2), 2), (dict(D=32), 2), (dict(Hk=3), 1), (dict(Hk=0), 1), (dict(Hq=1024), 2),
-                          (dict(window=-1), 1), (dict(scale=math.inf), 1), (dict(page=24), 1), (dict(page=4), 1),
+                          (dict(window=-1), 1), (dict(scale=math.inf), 1), (dict(scale=3e38), 1), (dict(scale=math.nan), 1), (dict(page=24), 1), (dict(page=4), 1),
                           (dict(slot=129), _lib.ERR_ALIGNMENT), (dict(k=72), _lib.ERR_ALIGNMENT), (dict(k=0), 1),
                           (dict(batch=2), 1), (dict(ptr=0), 1), (dict(ptr=68), _lib.ERR_ALIGNMENT),
                           (dict(n=513), _lib.ERR_ALIGNMENT), (dict(T=-1), 1), (dict(batch=-1, cu=64), 1)):
