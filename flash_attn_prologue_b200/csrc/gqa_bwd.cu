@@ -18,6 +18,7 @@ namespace flash_prologue {
 namespace {
 
 constexpr int kStages = 3;
+constexpr float kSmallScale = 0x1p-115f;
 
 // A warp's walk over its row blocks: for each of its token groups the slice's
 // head blocks of Q, then of K. `in` and `g` point at this lane's first columns.
@@ -37,7 +38,7 @@ __global__ void __launch_bounds__(kThreads, 2) gqa_bwd_kernel(const GqaBwdArgs a
   constexpr int kStageBytes = VEC ? 4 * C::kPieces * 512 : 0;  // x1, x2, g1, g2 of 32 lanes
   extern __shared__ __align__(16) unsigned char smem_raw[];
   float* w_s = reinterpret_cast<float*>(smem_raw);  // [q, k][half][lane of a row][8]: as the lanes own them
-  float2* e_s = reinterpret_cast<float2*>(w_s + 2 * D);  // [Hq] exp(scale), exp(-scale)
+  float2* e_s = reinterpret_cast<float2*>(w_s + 2 * D);  // [Hq] e = exp(scale), 1 / e
   float* ds_s = reinterpret_cast<float*>(e_s + a.H[0]);  // [kWarps][Hq]
   float* dw_s = ds_s + kWarps * a.H[0];                  // [kWarps][2 * D]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -50,8 +51,9 @@ __global__ void __launch_bounds__(kThreads, 2) gqa_bwd_kernel(const GqaBwdArgs a
   }
   for (int i = threadIdx.x; i < a.H[0]; i += kThreads) {
     const float v = a.scales[i];
-    // Below e^-80 the gradients are under 1e-34 and exp(-v) may be infinite: without the second, 0 * inf cannot arise.
-    e_s[i] = make_float2(expf(v), v < -80.f ? 0.f : expf(-v));
+    const float e = expf(v);
+    // Where 1 / e may be infinite it is kept as 2^-32 / e (0 where e has vanished), and s is 2^32 times as large beside it.
+    e_s[i] = make_float2(e, e >= kSmallScale ? expf(-v) : e > 0.f ? 0x1p-32f / e : 0.f);
   }
   for (int i = threadIdx.x; i < kWarps * a.H[0]; i += kThreads) ds_s[i] = 0.f;
   __syncthreads();
@@ -198,7 +200,8 @@ __global__ void __launch_bounds__(kThreads, 2) gqa_bwd_kernel(const GqaBwdArgs a
           if (c_lane == 0 && tslot == 0) ds_s[warp * a.H[0] + h] += sum;
         }
         if (there) {
-          lane_dx(n1, n2, u1, u2, re, r * (s * (1.f / D)) * e.y, x1, x2);
+          const float lift = e.x >= kSmallScale ? 1.f : 0x1p32f;
+          lane_dx(n1, n2, u1, u2, re, r * (s * lift * (1.f / D)) * e.y, x1, x2);
           store_chunk<T, D, VEC>(out, x1);
           store_chunk<T, D, VEC>(out + HALF, x2);
         }

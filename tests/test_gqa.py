@@ -6,7 +6,7 @@ import torch
 
 import flash_attn_prologue_b200 as fap
 from flash_attn_prologue_b200 import _lib
-from tests._paged import assert_within, rotate64, tables
+from tests._paged import BAND, HALF_ULP, TINY, assert_within, rotate64, tables
 
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
 
@@ -160,6 +160,24 @@ def test_very_small_query_scales():
     grads = torch.autograd.grad(got, args, up)
     assert all(t.isfinite().all() for t in (*got, *grads))
     assert not got[0][:, 0].any() and not grads[0][:, 0].any() and grads[0][:, 3].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout,D", [("packed", 64), ("odd", 128), ("packed", 256)])
+def test_gradients_of_small_query_scales(layout, D):
+    """exp(scale) far below 1: FP32 gradients are right to their last bits down to 2^-126, and to a few of FP32's
+    smallest steps below."""
+    q, k, w, _, sin, cos, _, up = _problem(layout, 1, 11, 6, 2, D, FP32, None)
+    s = torch.tensor([-95.0, -86.0, -84.0, -80.5, -79.0, -1.0], device="cuda").view(6, 1, 1)
+    args = [t.detach().requires_grad_() for t in (q, k, w, s)]
+    grads = torch.autograd.grad(fap.qknorm_rope_scale_gqa(*args, sin, cos), args, up)
+    _, dx, _, (ds, ds_size) = _exact(q, k, w, s, sin, cos, None, up)
+    for i, name in enumerate("qk"):
+        # as elsewhere, and 64 half steps of FP32's subnormal numbers for the products of the terms (|x|, |u| < 8)
+        off = (grads[i].double() - dx[i][0]).abs()
+        bound = HALF_ULP[FP32] * dx[i][0].abs() + 2 * BAND * dx[i][1] + 64 * TINY[FP32]
+        assert (off <= bound).all(), f"d{name}: {float((off / bound).max())}"
+    assert ((grads[3].double() - ds).abs() <= (128 + 16) * 2.0 ** -24 * ds_size + 2 * D * 11 * 64 * TINY[FP32]).all()
 
 
 @pytest.mark.gpu
