@@ -90,6 +90,7 @@ SIGNATURES = {
     "flash_prologue_gqa_bwd_workspace_size": ([_i64, _i64, ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
     "flash_prologue_append_paged": ([ctypes.c_char_p, _vp], ctypes.c_int),
     "flash_prologue_paged_attention": ([ctypes.c_char_p, _vp], ctypes.c_int),
+    "flash_prologue_selftest_attention_waits": ([ctypes.c_char_p, _i64, _vp], ctypes.c_int),
     "flash_prologue_paged_attention_workspace_size": ([_i64, ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
 }
 

@@ -78,9 +78,10 @@ struct PrefillPlan {
 };
 PrefillPlan plan_paged_prefill(int64_t tokens, int64_t batch, bool ragged, int64_t kv_heads, int64_t group, int D,
                                int64_t max_keys, int64_t window, int sms);
-// False where the cache's layout has no tensor map (the other kernel reads it).
+// False where the cache's layout has no tensor map (the other kernel reads it). wait_cycles: 0, or
+// (self-test, BF16) the limit of the kernel's waits, but for those for copies and products under way.
 bool launch_paged_prefill(const AttentionArgs& a, const PrefillPlan& plan, int dtype, int D, int64_t page_size,
-                          cudaStream_t stream, cudaError_t* err);
+                          long long wait_cycles, cudaStream_t stream, cudaError_t* err);
 cudaError_t launch_paged_decode(const AttentionArgs& a, int dtype, int D, cudaStream_t stream);
 
 }  // namespace flash_prologue

@@ -48,21 +48,8 @@ size_t workspace_of(int64_t D, int sms) {
   return prefill > decode ? prefill : decode;
 }
 
-}  // namespace
-
-extern "C" {
-
-int flash_prologue_paged_attention_workspace_size(int64_t D, size_t* bytes) {
-  if (!bytes) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
-  *bytes = 0;
-  if (D != 64 && D != 128) return FLASH_PROLOGUE_ERR_UNSUPPORTED;
-  const int sms = device_sms();
-  if (sms <= 0) return FLASH_PROLOGUE_ERR_CUDA;
-  *bytes = workspace_of(D, sms);
-  return FLASH_PROLOGUE_OK;
-}
-
-int flash_prologue_paged_attention(const flash_prologue_attention_args* a, void* stream) {
+// wait_cycles: 0, or the limit of the tiled kernel's waits (self-test), and no other kernel is taken.
+int attention(const flash_prologue_attention_args* a, int64_t wait_cycles, void* stream) {
   const int st = size_checks(a);
   if (st != FLASH_PROLOGUE_OK || a->tokens == 0 || a->Hq == 0) return st;
   const flash_prologue_cache& c = a->cache;
@@ -106,12 +93,37 @@ int flash_prologue_paged_attention(const flash_prologue_attention_args* a, void*
                                                 g.max_keys, g.window, sms);
     cudaError_t err = cudaSuccess;
     if (launch_paged_prefill(g, plan, (int)a->dtype, (int)a->D, c.page_size,
-                             static_cast<cudaStream_t>(stream), &err))
+                             wait_cycles, static_cast<cudaStream_t>(stream), &err))
       return err == cudaSuccess ? FLASH_PROLOGUE_OK : FLASH_PROLOGUE_ERR_CUDA;
   }
+  if (wait_cycles) return FLASH_PROLOGUE_ERR_UNSUPPORTED;
   return launch_paged_decode(g, (int)a->dtype, (int)a->D, static_cast<cudaStream_t>(stream)) == cudaSuccess
              ? FLASH_PROLOGUE_OK
              : FLASH_PROLOGUE_ERR_CUDA;
+}
+
+}  // namespace
+
+extern "C" {
+
+int flash_prologue_paged_attention_workspace_size(int64_t D, size_t* bytes) {
+  if (!bytes) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
+  *bytes = 0;
+  if (D != 64 && D != 128) return FLASH_PROLOGUE_ERR_UNSUPPORTED;
+  const int sms = device_sms();
+  if (sms <= 0) return FLASH_PROLOGUE_ERR_CUDA;
+  *bytes = workspace_of(D, sms);
+  return FLASH_PROLOGUE_OK;
+}
+
+int flash_prologue_paged_attention(const flash_prologue_attention_args* a, void* stream) {
+  return attention(a, 0, stream);
+}
+
+int flash_prologue_selftest_attention_waits(const flash_prologue_attention_args* a, int64_t wait_cycles, void* stream) {
+  if (!a || wait_cycles < 1 || wait_cycles > (int64_t(1) << 33)) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
+  if (a->dtype != FLASH_PROLOGUE_BF16) return FLASH_PROLOGUE_ERR_UNSUPPORTED;
+  return attention(a, wait_cycles, stream);
 }
 
 }  // extern "C"

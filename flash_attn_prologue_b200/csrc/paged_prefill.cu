@@ -40,8 +40,10 @@
 // Scores, statistics, sums and O are FP32; the probabilities are rounded to the
 // cache's type for the second product (their sum is taken before the rounding),
 // an error of the size of the output's own rounding. Waits are bounded: where one
-// runs out the error word is set, the tile's rows are NaN, and the CTA ends (a tile
-// that it had taken over may stay unwritten). Tensor memory is released on every path.
+// runs out the error word is set, the rows that the CTA was at or had taken over
+// are NaN, and it ends once its copies and products are done. (Only a tile whose
+// index does not come back within twice the limit stays unwritten.) Tensor memory
+// is released on every path.
 #include "paged_attention.h"
 #include "tensor_map.h"
 #include "umma_util.cuh"
@@ -92,6 +94,10 @@ struct Barriers {
   int sums[kPrefillThreads / 32];
   int found, found_start;  // request of the CTA's first tile (-1: none), tiles before it
   Work work[2];            // the tile that the warps are at and the next
+  // Where a wait ran out: the tiles that were put into work, and one that was taken over and not put there.
+  uint32_t posted;
+  int has_left;
+  Work left;
 };
 
 struct Tile {  // what the join needs to know of a tile
@@ -108,6 +114,7 @@ struct PrefillArgs {
   float* part_out;       // [cut items * splits][128][D]
   float* part_stat;      // [...][128][2]
   Tile* joins;           // [cut items]
+  long long wait_cycles; // self-test: limit of a wait
 };
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3,
@@ -160,6 +167,20 @@ __device__ __forceinline__ bool phase_wait(uint64_t* bar, uint32_t parity) {
   do {
     if (phase_done(a, parity)) return true;
   } while (clock64() - start < kMostCycles);
+  atomicOr(&g_device_error, kDeviceErrorTimeout);
+  return false;
+}
+// The self-test's wait: polls that do not suspend, so that a limit of any length can run out.
+__device__ __forceinline__ bool short_wait(uint64_t* bar, uint32_t parity, long long most_cycles) {
+  const long long start = clock64();
+  do {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    if (done) return true;
+  } while (clock64() - start < most_cycles);
   atomicOr(&g_device_error, kDeviceErrorTimeout);
   return false;
 }
@@ -241,7 +262,24 @@ __device__ __forceinline__ uint32_t finite_only(uint32_t pair) {
   return pair & ~((n >> 15) * 0xffffu);
 }
 
+// NaN for row `row` of a tile (or of this share of it) that was not computed.
 template <typename T, int D>
+__device__ __noinline__ void void_row(const PrefillArgs& p, const Work& w, int row) {
+  if (row >= w.rows) return;
+  const float nan = __int_as_float(0x7fc00000);
+  if (w.parts > 1) {
+    float* stat = p.part_stat + ((int64_t)w.share * kTile + row) * 2;
+    stat[0] = -INFINITY;
+    stat[1] = nan;
+    return;
+  }
+  const int token = w.first_token + row / p.a.group, h = w.head * p.a.group + row % p.a.group;
+  T* out = static_cast<T*>(p.a.out) + token * p.a.out_n + (int64_t)h * p.a.out_h;
+  for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(out + c) = make_uint4(~0u, ~0u, ~0u, ~0u);
+  if (p.a.lse) p.a.lse[(int64_t)token * p.a.heads + h] = nan;
+}
+
+template <typename T, int D, bool kSelfTest = false>
 __global__ void __launch_bounds__(kPrefillThreads, 2)
     paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                          const __grid_constant__ CUtensorMap v_map, const __grid_constant__ PrefillArgs p) {
@@ -250,6 +288,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
   __shared__ Barriers bar;
   __shared__ __align__(16) unsigned char answer[16];
   const AttentionArgs& a = p.a;
+  const auto wait_for = [&](uint64_t* b, uint32_t parity) {
+    if constexpr (kSelfTest) return short_wait(b, parity, p.wait_cycles);
+    else return phase_wait(b, parity);
+  };
+  // For copies and products under way, which end by themselves: never cut short.
+  const auto drain = [](uint64_t* b, uint32_t parity) { return phase_wait(b, parity); };
   unsigned char* q_s = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char* k_s = q_s + L::kQ;
   unsigned char* v_s = k_s + L::kStages * L::kBlock;
@@ -279,6 +323,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
     mbar_init(&bar.q_empty, 1);
     mbar_init(&bar.next_here, 1);
     bar.found = -1;
+    bar.has_left = 0;
     fence_mbar_init();
   }
   // The request of the first tile; later ones are found from there.
@@ -328,9 +373,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
 
   // Every warp walks the CTA's tiles; `g` counts its blocks over all of them (buffers and
   // phases go on from tile to tile), `t` the tiles. Where a wait runs out a warp leaves.
-  uint32_t g = 0;
+  uint32_t g = 0, rows_done = 0;  // rows_done: tiles whose rows this warp has written
   const auto next_work = [&](uint32_t t) {
-    return __all_sync(0xffffffffu, phase_wait(&bar.work_full[t & 1], (t >> 1) & 1));
+    return __all_sync(0xffffffffu, wait_for(&bar.work_full[t & 1], (t >> 1) & 1));
   };
   const auto done_with = [&](uint32_t t) {
     __syncwarp();
@@ -352,12 +397,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       const Work& w = bar.work[t & 1];
       const int n = __shfl_sync(0xffffffffu, w.blocks, 0);
       if (w.rows < 0) break;
-      if (n) ok = __all_sync(0xffffffffu, phase_wait(&bar.q_full, queries++ & 1));
+      if (n) ok = __all_sync(0xffffffffu, wait_for(&bar.q_full, queries++ & 1));
       for (int j = 0; j < n && ok; ++j, ++g) {
         const uint32_t s = g % L::kStages, b = g % L::kScores;
         // The last scores of this buffer are in the rows' registers, K is here.
-        if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.s_read[b], ((g / L::kScores) & 1) ^ 1) &&
-                                               phase_wait(&bar.k_full[s], (g / L::kStages) & 1))))
+        if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.s_read[b], ((g / L::kScores) & 1) ^ 1) &&
+                                               wait_for(&bar.k_full[s], (g / L::kStages) & 1))))
           break;
         tc_fence_after();
         const uint64_t k_desc = smem_desc_k_sw128(smem_u32(k_s) + s * L::kBlock);
@@ -376,10 +421,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       }
       done_with(t);
     }
-    if (!ok) {  // tensor memory is not released under products still running
-      if (elect_one()) umma_commit(&bar.drain[0]);
-      phase_wait(&bar.drain[0], 0);
-    }
+    // Neither tensor memory nor the tiles are released under products still running.
+    if (elect_one()) umma_commit(&bar.drain[0]);
+    drain(&bar.drain[0], 0);
   } else if (warp == 6) {
     // ---------------- output ----------------
     constexpr uint32_t idesc = idesc_of<T>(D, true);
@@ -394,10 +438,10 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       if (w.rows < 0) break;
       for (int j = 0; j < n; ++j, ++g) {
         const uint32_t s = g % L::kStages;
-        ok = phase_wait(&bar.v_full[s], (g / L::kStages) & 1);
+        ok = wait_for(&bar.v_full[s], (g / L::kStages) & 1);
         const bool partial = j < full0 || j >= full1;
         if (partial && lane == 0) mbar_arrive(&bar.clean_ask);  // cleaned beside the block's softmax
-        ok = ok && (!partial || phase_wait(&bar.v_clean, cleaned & 1)) && phase_wait(&bar.p_full[g & 1], (g >> 1) & 1);
+        ok = ok && (!partial || wait_for(&bar.v_clean, cleaned & 1)) && wait_for(&bar.p_full[g & 1], (g >> 1) & 1);
         cleaned += partial;
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         tc_fence_after();
@@ -413,10 +457,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       }
       done_with(t);
     }
-    if (!ok) {
-      if (elect_one()) umma_commit(&bar.drain[1]);
-      phase_wait(&bar.drain[1], 0);
-    }
+    if (elect_one()) umma_commit(&bar.drain[1]);
+    drain(&bar.drain[1], 0);
   } else if (warp == 5) {
     // ---------------- tiles and loads ----------------
     const int in_page = (1 << a.pages.page_log2) - 1, boxes = kKeys / p.box_rows;
@@ -524,7 +566,13 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       }
       __syncwarp();
     };
-    bool ok = true;
+    const auto leave = [&](const Work& w) {
+      if (lane == 0) {
+        bar.left = w;
+        bar.has_left = 1;
+      }
+    };
+    bool ok = true, asking = false;
     uint32_t t = 0, queries = 0, asked = 0;
     uint32_t k_loads = 0, v_loads = 0, q_loads = 0;  // begun
     for (int index = blockIdx.x; index >= 0;) {
@@ -532,7 +580,10 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       if (describe(index, w)) {
         Work& slot = bar.work[t & 1];
         int entry = entry_of(w, 0);
-        if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.work_empty[t & 1], ((t >> 1) & 1) ^ 1)))) break;
+        if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.work_empty[t & 1], ((t >> 1) & 1) ^ 1)))) {
+          leave(w);
+          break;
+        }
         if (lane == 0) {
           slot = w;
           mbar_arrive(&bar.work_full[t & 1]);
@@ -543,12 +594,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
           const uint32_t s = g % L::kStages, parity = ((g / L::kStages) & 1) ^ 1;
           const int page = page_of(w, j, entry, &slot.bad);
           entry = entry_of(w, j + 1);
-          if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.k_empty[s], parity)))) break;
+          if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.k_empty[s], parity)))) break;
           load(w, j, page, &k_map, k_s, bar.k_full);
           ++k_loads;
           if (j == 0) {
             // The last tile's scores have been computed: its Q can go.
-            if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.q_empty, (queries & 1) ^ 1)))) break;
+            if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.q_empty, (queries & 1) ^ 1)))) break;
             ++queries;
             if (lane == 0) {
               mbar_arrive_expect_tx(&bar.q_full, p.tile_tokens * a.group * 128 * L::kHalves);
@@ -559,7 +610,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
             __syncwarp();
             ++q_loads;
           }
-          if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.v_empty[s], parity)))) break;
+          if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.v_empty[s], parity)))) break;
           load(w, j, page, &v_map, v_s, bar.v_full);
           ++v_loads;
         }
@@ -572,11 +623,15 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
         ask_next_cta(answer, &bar.next_here);
       }
       __syncwarp();
-      if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.next_here, asked++ & 1)))) break;
+      asking = true;
+      if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.next_here, asked++ & 1)))) break;
+      asking = false;
       index = __shfl_sync(0xffffffffu, next_cta(answer), 0);
     }
+    if (lane == 0) bar.posted = t;
     if (ok) {
-      if (__all_sync(0xffffffffu, phase_wait(&bar.work_empty[t & 1], ((t >> 1) & 1) ^ 1)) && lane == 0) {
+      ok = __all_sync(0xffffffffu, wait_for(&bar.work_empty[t & 1], ((t >> 1) & 1) ^ 1));
+      if (ok && lane == 0) {
         bar.work[t & 1].rows = -1;
         bar.work[t & 1].blocks = 0;
         mbar_arrive(&bar.work_full[t & 1]);
@@ -585,16 +640,21 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       // No product's arrival on an empty barrier lands after the CTA has gone.
       for (uint32_t e = g; e < g + L::kStages && ok; ++e) {
         const uint32_t s = e % L::kStages, parity = ((e / L::kStages) & 1) ^ 1;
-        ok = phase_wait(&bar.k_empty[s], parity) && phase_wait(&bar.v_empty[s], parity);
+        ok = __all_sync(0xffffffffu, wait_for(&bar.k_empty[s], parity) && wait_for(&bar.v_empty[s], parity));
       }
-      if (ok) phase_wait(&bar.q_empty, (queries & 1) ^ 1);
-    } else {
-      // A wait ran out: wait (bounded) for what is still on its way to shared memory.
-      if (asked) phase_wait(&bar.next_here, (asked - 1) & 1);
-      if (q_loads) phase_wait(&bar.q_full, (q_loads - 1) & 1);
+      if (ok) ok = __all_sync(0xffffffffu, wait_for(&bar.q_empty, (queries & 1) ^ 1));
+    }
+    if (!ok) {
+      // A wait ran out: what is still on its way to shared memory has to arrive. A tile that does is not computed.
+      if (asking && __all_sync(0xffffffffu, drain(&bar.next_here, (asked - 1) & 1))) {
+        const int index = __shfl_sync(0xffffffffu, next_cta(answer), 0);
+        Work w;
+        if (index >= 0 && describe(index, w)) leave(w);
+      }
+      if (q_loads) drain(&bar.q_full, (q_loads - 1) & 1);
       for (uint32_t back = 1; back <= L::kStages; ++back) {
-        if (k_loads >= back) phase_wait(&bar.k_full[(k_loads - back) % L::kStages], ((k_loads - back) / L::kStages) & 1);
-        if (v_loads >= back) phase_wait(&bar.v_full[(v_loads - back) % L::kStages], ((v_loads - back) / L::kStages) & 1);
+        if (k_loads >= back) drain(&bar.k_full[(k_loads - back) % L::kStages], ((k_loads - back) / L::kStages) & 1);
+        if (v_loads >= back) drain(&bar.v_full[(v_loads - back) % L::kStages], ((v_loads - back) / L::kStages) & 1);
       }
     }
   } else if (warp == 7) {
@@ -610,8 +670,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
         if (j >= full0 && j < full1) continue;
         const uint32_t s = g % L::kStages;
         // Asked by the warp that has seen the block arrive.
-        if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.clean_ask, asked++ & 1) &&
-                                               phase_wait(&bar.v_full[s], (g / L::kStages) & 1))))
+        if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.clean_ask, asked++ & 1) &&
+                                               wait_for(&bar.v_full[s], (g / L::kStages) & 1))))
           break;
         const int kb = (w.first + j) * kKeys, lo = w.lo - kb, hi = w.hi - kb;
         uint4* v = reinterpret_cast<uint4*>(v_s + s * L::kBlock);
@@ -647,7 +707,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
     const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
     const float scale = a.scale_log2;
     bool ok = true;
-    for (uint32_t t = 0; ok; ++t) {
+    for (; ok; ++rows_done) {
+      const uint32_t t = rows_done;
       if (!(ok = next_work(t))) break;
       const Work& w = bar.work[t & 1];
       if (w.rows < 0) break;
@@ -661,7 +722,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       }
       for (int j = 0; j < blocks; ++j, ++g) {
         const uint32_t b = g % L::kScores;
-        if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.s_full[b], (g / L::kScores) & 1)))) break;
+        if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.s_full[b], (g / L::kScores) & 1)))) break;
         tc_fence_after();
         uint32_t s[2][32];
         tmem_ld32(mine + L::kSCol + b * kKeys, s[0]);
@@ -695,7 +756,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
         const bool move = !fresh && (now - top) * scale > 8.f;
         if (__any_sync(0xffffffffu, move)) {
           // O has to be at rest: the last product with V done; the next one waits for this block's P.
-          if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1)))) break;
+          if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1)))) break;
           tc_fence_after();
           const float f = move ? exp2_approx((top - now) * scale) : 1.f;
           sum *= f;
@@ -725,7 +786,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
           out[i] = pack2<T>(x.x, x.y);
         }
         // The buffer's last P has to be used up.
-        if (!(ok = __all_sync(0xffffffffu, phase_wait(&bar.o_done[g & 1], ((g >> 1) & 1) ^ 1)))) break;
+        if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.o_done[g & 1], ((g >> 1) & 1) ^ 1)))) break;
         tc_fence_after();
         tmem_st32(mine + L::kPCol + (g & 1) * (kKeys / 2), out);
         const float2 both = __fadd2_rn(__fadd2_rn(add[0], add[1]), __fadd2_rn(add[2], add[3]));
@@ -735,7 +796,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
         __syncwarp();
         if (lane == 0) mbar_arrive(&bar.p_full[g & 1]);
       }
-      if (blocks && ok) ok = phase_wait(&bar.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
+      if (blocks && ok) ok = wait_for(&bar.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) sum = __int_as_float(0x7fc00000);  // a wait ran out: no output that could pass for one
 
@@ -811,12 +872,18 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       tc_fence_before();
       done_with(t);
     }
+    tmem_wait_st();  // where a wait ran out between a store and its use
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 4) {
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
+  }
+  // Tiles that were left where a wait ran out (at most the two that are in work, and one more).
+  if (warp < 4) {
+    for (; rows_done < bar.posted; ++rows_done) void_row<T, D>(p, bar.work[rows_done & 1], threadIdx.x);
+    if (bar.has_left) void_row<T, D>(p, bar.left, threadIdx.x);
   }
 }
 
@@ -829,6 +896,10 @@ __global__ void __launch_bounds__(512) prefill_join_kernel(const PrefillArgs p) 
   const Tile t = p.joins[item];
   const int row = (int)(blockIdx.x % (kTile / 16)) * 16 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (t.parts <= 1 || row >= t.rows) return;
+  // What no CTA wrote (a wait ran out) may be anything.
+  if (t.parts > p.splits || t.rows > kTile || t.kv_head < 0 || t.kv_head >= a.kv_heads || t.token0 < 0 ||
+      t.token0 >= a.tokens - (t.rows - 1) / a.group)
+    return;
   const int64_t slot0 = item * p.splits;
   float m = -INFINITY;
   for (int s = 0; s < t.parts; ++s) m = fmaxf(m, p.part_stat[((slot0 + s) * kTile + row) * 2]);
@@ -879,14 +950,14 @@ bool encode_rows(CUtensorMap* map, const void* base, int dtype, int D, int64_t h
                            dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool kSelfTest = false>
 cudaError_t launch(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map, const PrefillArgs& p, int64_t items,
                    cudaStream_t stream) {
-  const void* fn = reinterpret_cast<const void*>(&paged_prefill_kernel<T, D>);
+  const void* fn = reinterpret_cast<const void*>(&paged_prefill_kernel<T, D, kSelfTest>);
   cudaError_t err = allow_shared_memory(fn, Layout<D>::kSmem);
   if (err != cudaSuccess) return err;
   const int64_t cut = items - p.whole_items;
-  err = launch_kernel(paged_prefill_kernel<T, D>, dim3((unsigned)(p.whole_items + cut * p.splits)), dim3(kPrefillThreads),
+  err = launch_kernel(paged_prefill_kernel<T, D, kSelfTest>, dim3((unsigned)(p.whole_items + cut * p.splits)), dim3(kPrefillThreads),
                       Layout<D>::kSmem, stream, q_map, k_map, v_map, p);
   if (err != cudaSuccess || p.splits == 1) return err;
   return launch_following(prefill_join_kernel<T, D>, dim3((unsigned)(cut * (kTile / 16))), dim3(512), stream, p);
@@ -944,9 +1015,10 @@ size_t paged_prefill_workspace(int D, int sms) {
 }
 
 bool launch_paged_prefill(const AttentionArgs& a, const PrefillPlan& plan, int dtype, int D, int64_t page_size,
-                          cudaStream_t stream, cudaError_t* err) {
+                          long long wait_cycles, cudaStream_t stream, cudaError_t* err) {
   PrefillArgs p{};
   p.a = a;
+  p.wait_cycles = wait_cycles;
   p.tile_tokens = plan.tile_tokens;
   p.splits = plan.splits;
   p.whole_items = (int)plan.whole_items;
@@ -967,7 +1039,10 @@ bool launch_paged_prefill(const AttentionArgs& a, const PrefillPlan& plan, int d
     p.part_stat = p.part_out + shares * kTile * D;
     p.joins = reinterpret_cast<Tile*>(p.part_stat + shares * kTile * 2);
   }
-  if (D == 64)
+  if (wait_cycles)
+    *err = D == 64 ? launch<__nv_bfloat16, 64, true>(q_map, k_map, v_map, p, items, stream)
+                   : launch<__nv_bfloat16, 128, true>(q_map, k_map, v_map, p, items, stream);
+  else if (D == 64)
     *err = dtype == 0 ? launch<__nv_bfloat16, 64>(q_map, k_map, v_map, p, items, stream)
                       : launch<__half, 64>(q_map, k_map, v_map, p, items, stream);
   else

@@ -565,6 +565,15 @@ typedef struct flash_prologue_attention_args {
  * flash_prologue_paged_attention_workspace_size() bytes, no initialisation.
  */
 FLASH_PROLOGUE_API int flash_prologue_paged_attention(const flash_prologue_attention_args* args, void* stream);
+/*
+ * Self-test of failure detection: a call (BF16) whose waits inside the tiled
+ * kernel (chunks) give up after `wait_cycles` clock cycles (1 .. 2^33) instead
+ * of about 4 s. Rows whose tile was given up are NaN, all others are right, and
+ * the error word has bit 0 set; the context stays usable. Calls that another
+ * kernel serves are refused (FLASH_PROLOGUE_ERR_UNSUPPORTED).
+ */
+FLASH_PROLOGUE_API int flash_prologue_selftest_attention_waits(const flash_prologue_attention_args* args,
+                                                               int64_t wait_cycles, void* stream);
 /* Bytes of workspace that cover every call with head dimension D on the current device. */
 FLASH_PROLOGUE_API int flash_prologue_paged_attention_workspace_size(int64_t D, size_t* bytes);
 

@@ -233,6 +233,48 @@ def test_pages_out_of_range_give_nan_and_the_error_word(news):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("news,totals,window", [
+    ([700, 0, 900, 5], [900, 40, 2000, 1100], 0),   # whole tiles, more than the GPU holds at once
+    ([1500, 40], [1500, 4000], 300),
+    ([70, 3, 25], [6000, 2500, 2900], 0),           # keys shared out
+])
+@pytest.mark.parametrize("D", [64, 128])
+def test_waits_that_run_out(news, totals, window, D, monkeypatch):
+    """Tiles given up come out as NaN with the error word set, shares of a tile included; the rest has its bits."""
+    req = Requests(news, totals, 32, 4, D, 16, BF16)
+    other = Requests(news, totals, 32, 4, D, 16, BF16, seed=1)
+
+    def call(r):
+        return fap.paged_attention(r.q.to(BF16), r.k, r.v, r.table, r.seq_lens, r.cu, softmax_scale=0.1, window=window,
+                                   return_lse=True)
+
+    def bounded(cycles):
+        def run(name, args, device):
+            status = _lib.load().flash_prologue_selftest_attention_waits(args, cycles, _lib.raw_stream(device.index))
+            _lib.check(status, "flash_prologue_selftest_attention_waits")
+        return run
+
+    clean, clean_lse = call(req)
+    _lib.device_error()
+    given_up = 0
+    for cycles in (1, 200, 600, 1000, 2000, 4000, 8000, 20000, 100000, 2 ** 32):
+        call(other)  # leaves other rows and shares where this call's may come to lie
+        torch.cuda.synchronize()
+        with monkeypatch.context() as m:
+            m.setattr(fap.paged, "call_library", bounded(cycles))
+            got, lse = call(req)
+        error = _lib.device_error()
+        lost = got.isnan().all(-1)
+        assert torch.equal(got.isnan().any(-1), lost) and torch.equal(lse.isnan(), lost)
+        assert torch.equal(got[~lost], clean[~lost]) and torch.equal(lse[~lost], clean_lse[~lost])
+        assert error == 1 if lost.any() else error in (0, 1)
+        given_up += int(lost.sum())
+    assert error == 0 and not lost.any()  # the limit of a call
+    assert given_up
+    assert all(torch.equal(a, b) for a, b in zip(call(req), (clean, clean_lse)))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("chunk", [1, 60])
 def test_padding_rows_are_zero(chunk):
     req = Requests([chunk, 2], [chunk + 30, 9], 8, 2, 64, 16, BF16)
@@ -406,6 +448,8 @@ def test_c_abi_refusals():
             ptr, 0, 64, n, ptr, 0, 64, n, 0, *cache, 0, 0, T, Hq, Hk, D, dtype, window, scale), None)
 
     assert call(T=0, batch=0, ptr=0) == _lib.OK
+    for cycles in (0, -1, 10 ** 10):
+        assert lib.flash_prologue_selftest_attention_waits(bytes(_lib.ATTENTION_ARGS.size), cycles, None) == 1
     for wrong, status in ((dict(dtype=2), 2), (dict(D=32), 2), (dict(Hk=3), 1), (dict(Hk=0), 1), (dict(Hq=1024), 2),
                           (dict(window=-1), 1), (dict(scale=math.inf), 1), (dict(scale=3e38), 1), (dict(scale=math.nan), 1), (dict(page=24), 1), (dict(page=4), 1),
                           (dict(slot=129), _lib.ERR_ALIGNMENT), (dict(k=72), _lib.ERR_ALIGNMENT), (dict(k=0), 1),
