@@ -152,9 +152,11 @@ class _CuteEager(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_q, grad_k):
-        from .fused_epilogue import cute_backward
+        from .fused_epilogue import cute_backward, qknorm_rope_scale_cute_backward_op
         q, k, rmsnorm_weight, scales, sin, cos = ctx.saved_tensors
-        dq, dk, dw, ds = cute_backward(q, k, rmsnorm_weight, scales, sin, cos, grad_q, grad_k, ctx.eps)
+        # create_graph: the registered op, which refuses second derivatives
+        backward = qknorm_rope_scale_cute_backward_op if torch.is_grad_enabled() else cute_backward
+        dq, dk, dw, ds = backward(q, k, rmsnorm_weight, scales, sin, cos, grad_q, grad_k, ctx.eps)
         return dq, dk, dw, ds, None, None, None
 
 

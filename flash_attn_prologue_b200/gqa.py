@@ -209,7 +209,10 @@ class _GqaEager(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_q, grad_k):
-        dq, dk, dw, ds = gqa_backward(*ctx.saved_tensors, grad_q, grad_k, ctx.eps, checked=True)
+        if torch.is_grad_enabled():  # create_graph: the registered op, which refuses second derivatives
+            dq, dk, dw, ds = qknorm_rope_scale_gqa_backward_op(*ctx.saved_tensors, grad_q, grad_k, ctx.eps)
+        else:
+            dq, dk, dw, ds = gqa_backward(*ctx.saved_tensors, grad_q, grad_k, ctx.eps, checked=True)
         return dq, dk, dw, ds, None, None, None, None
 
 
