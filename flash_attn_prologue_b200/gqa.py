@@ -14,6 +14,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .distributed import active_peer_group
@@ -92,6 +93,15 @@ def eager(*tensors) -> bool:
         if t is not None and type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
             return False
     return True
+
+
+def refuse_tangents(name, *tensors):
+    """Forward-mode derivatives would be lost without a word: neither the kernels nor a
+    registered operator (without a rule for them) hands tangents on."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
 def call_library(name, args, device):
@@ -221,6 +231,7 @@ def qknorm_rope_scale_gqa_op(
     q: torch.Tensor, k: torch.Tensor, rmsnorm_weight: torch.Tensor, scales: torch.Tensor, sin: torch.Tensor,
     cos: torch.Tensor, positions: Optional[torch.Tensor] = None, eps: float = 1e-5,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
+    refuse_tangents("qknorm_rope_scale_gqa", q, k, rmsnorm_weight, scales, sin, cos)
     return gqa_forward(q, k, rmsnorm_weight, scales, sin, cos, positions, eps)
 
 
@@ -235,6 +246,7 @@ def qknorm_rope_scale_gqa_backward_op(
     cos: torch.Tensor, positions: Optional[torch.Tensor], grad_q_out: torch.Tensor, grad_k_out: torch.Tensor,
     eps: float = 1e-5,
 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    refuse_tangents("qknorm_rope_scale_gqa_backward", q, k, rmsnorm_weight, scales, sin, cos, grad_q_out, grad_k_out)
     return gqa_backward(q, k, rmsnorm_weight, scales, sin, cos, positions, grad_q_out, grad_k_out, eps)
 
 
@@ -269,6 +281,7 @@ def qknorm_rope_scale_gqa(q, k, rmsnorm_weight, scales, sin, cos, positions=None
     the device error word. All arithmetic through the final cast is FP32. Differentiable
     in q, k, rmsnorm_weight and scales; outputs and gradients keep the inputs' memory order.
     """
+    refuse_tangents("qknorm_rope_scale_gqa", q, k, rmsnorm_weight, scales, sin, cos)
     if eager(q, k, rmsnorm_weight, scales, sin, cos, positions):
         if not torch.is_grad_enabled() or not (q.requires_grad or k.requires_grad or rmsnorm_weight.requires_grad
                                                or scales.requires_grad):

@@ -18,7 +18,7 @@ import torch
 
 from . import _lib
 from .fused_epilogue import _DeviceGuard
-from .gqa import MAX_HEADS, call_library, check_rows, eager, flat_fp32, readable, rotation_of, rows_of
+from .gqa import MAX_HEADS, call_library, check_rows, eager, flat_fp32, readable, refuse_tangents, rotation_of, rows_of
 
 
 def _checked_cache(q, heads, k_cache, v_cache, page_table, seq_lens, cu_seqlens):
@@ -66,6 +66,7 @@ def _checked_cache(q, heads, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
 
 
 def _no_grad(name, *tensors):
+    refuse_tangents(name, *tensors)
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
@@ -121,7 +122,7 @@ def append_paged_kv(q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache,
     the device error word. Not differentiable.
     """
     args = (q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
-    _no_grad("append_paged_kv", q, k, v, rmsnorm_weight, scales, k_cache, v_cache)
+    _no_grad("append_paged_kv", q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache)
     call = _append if eager(q, k, v, rmsnorm_weight, sin, k_cache) else torch.ops.flash_prologue.append_paged_kv
     return call(*args, eps)
 
@@ -189,6 +190,7 @@ def paged_attention_op(
     seq_lens: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None, softmax_scale: float = 1.0, window: int = 0,
     want_lse: bool = False,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
+    refuse_tangents("paged_attention", q, k_cache, v_cache)
     out, lse = _attention(q, k_cache, v_cache, page_table, seq_lens, cu_seqlens, softmax_scale, window, want_lse)
     return out, q.new_empty(0, dtype=torch.float32) if lse is None else lse
 

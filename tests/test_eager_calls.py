@@ -4,9 +4,10 @@ The kernels are replaced by plain functions where only the host's path matters, 
 this runs on the CPU."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import flash_attn_prologue_b200 as fap
-from flash_attn_prologue_b200 import functional, fused_epilogue, gqa
+from flash_attn_prologue_b200 import functional, fused_epilogue, gqa, paged
 from tests._paged import tables
 
 OPS = torch.ops.flash_prologue
@@ -27,6 +28,22 @@ def plain_gqa(monkeypatch):
         return 2 * q * grad_q, 3 * grad_k, torch.zeros_like(w), torch.zeros_like(s)
 
     monkeypatch.setattr(gqa, "gqa_backward", backward)
+
+
+def _step(device="cpu"):
+    """append_paged_kv's arguments, and paged_attention's."""
+    q, k, w, s, sin, cos = _rows(device)
+    caches = [torch.zeros(4, 16, 2, 64, device=device) for _ in range(2)]
+    table = torch.arange(3, dtype=torch.int32, device=device)[:, None]
+    lens = torch.ones(3, dtype=torch.int32, device=device)
+    return [q, k, k.clone(), w, s, sin, cos, *caches, table, lens, None], [q, *caches, table, lens, None]
+
+
+@pytest.fixture
+def plain_step(monkeypatch):
+    """append_paged_kv and paged_attention with 2 q in place of the kernels' results."""
+    monkeypatch.setattr(paged, "_append", lambda q, *rest: 2 * q)
+    monkeypatch.setattr(paged, "_attention", lambda q, *rest: (2 * q, None))
 
 
 def _differentiate_twice(call, q):
@@ -69,3 +86,45 @@ def test_second_derivatives_on_the_gpu():
         assert torch.equal(first, again)
         with pytest.raises(RuntimeError, match="differentiate twice|no autograd formula"):
             _differentiate_twice(call, leaf)
+
+
+def _refuses_tangents(call, args, at):
+    with forward_ad.dual_level():
+        duals = list(args)
+        duals[at] = forward_ad.make_dual(args[at], torch.ones_like(args[at]))
+        with pytest.raises(NotImplementedError, match="forward"):
+            call(*duals)
+        call(*args)  # no tangents in a call: nothing to lose
+
+
+@pytest.mark.parametrize("at", range(6))
+@pytest.mark.parametrize("needs_grad", [False, True])
+@pytest.mark.parametrize("call", [fap.qknorm_rope_scale_gqa, lambda *a: OPS.qknorm_rope_scale_gqa(*a, None, 1e-5)])
+def test_forward_mode_is_refused(call, needs_grad, at, plain_gqa):
+    args = list(_rows())
+    if needs_grad:
+        args[2 if at != 2 else 3].requires_grad_()
+    _refuses_tangents(call, args, at)
+
+
+@pytest.mark.parametrize("at", range(9))
+def test_forward_mode_is_refused_by_the_append(at, plain_step):
+    args = _step()[0]
+    with torch.no_grad():
+        _refuses_tangents(fap.append_paged_kv, args, at)
+    _refuses_tangents(fap.append_paged_kv, args, at)
+
+
+@pytest.mark.parametrize("at", [0, 1, 2])
+@pytest.mark.parametrize("call", [fap.paged_attention, OPS.paged_attention])
+def test_forward_mode_is_refused_by_the_attention(call, at, plain_step):
+    _refuses_tangents(call, _step()[1], at)
+
+
+def test_forward_mode_transform_is_refused(plain_gqa, plain_step):
+    q, *rest = _rows()
+    with pytest.raises(NotImplementedError, match="forward"):
+        torch.func.jvp(lambda q: fap.qknorm_rope_scale_gqa(q, *rest), (q,), (torch.ones_like(q),))
+    q, *rest = _step()[1]
+    with pytest.raises(NotImplementedError, match="forward"):
+        torch.func.jvp(lambda q: fap.paged_attention(q, *rest), (q,), (torch.ones_like(q),))
