@@ -125,16 +125,21 @@ def qknorm_rope_scale(q, k, rmsnorm_weight, scales, sin, cos, eps=1e-5, *, backe
             transform(k, rmsnorm_weight[1]).to(k.dtype))
 
 
+_functorch_active = getattr(torch._C, "_are_functorch_transforms_active", lambda: False)
+
+
+def _recorded() -> bool:
+    """The registered custom op must be what is called: under torch.compile, torch.jit.trace,
+    a functorch transform or a dispatch mode (make_fx, a fake mode, a profiler of operators),
+    which see operators and not the library's calls."""
+    return (torch.compiler.is_compiling() or torch._C._is_tracing() or _functorch_active()
+            or torch._C._len_torch_dispatch_stack() > 0)
+
+
 def _plain_eager(*tensors) -> bool:
-    """True for an eager call on plain tensors: not compiled, traced, under a
-    functorch transform or on tensor subclasses (fake, meta wrappers, DTensor),
-    where the registered custom op must be what is recorded."""
-    if torch.compiler.is_compiling() or torch.jit.is_tracing():
-        return False
-    active = getattr(torch._C, "_are_functorch_transforms_active", None)
-    if active is not None and active():
-        return False
-    return all(type(t) is torch.Tensor for t in tensors)
+    """True for an eager call on plain tensors: not recorded, nor on tensor
+    subclasses (fake, meta wrappers, DTensor)."""
+    return not _recorded() and all(type(t) is torch.Tensor for t in tensors)
 
 
 class _CuteEager(torch.autograd.Function):

@@ -19,7 +19,7 @@ from torch.autograd import forward_ad
 from . import _lib
 from .distributed import active_peer_group
 from .fused_epilogue import _DeviceGuard, _grad_view
-from .functional import SUPPORTED_CUTE_HEAD_DIMS
+from .functional import SUPPORTED_CUTE_HEAD_DIMS, _recorded
 
 MAX_HEADS = 512
 
@@ -82,12 +82,9 @@ def _check_positions(positions, q, sin):
         raise ValueError("all tensors must share a device")
 
 
-_functorch_active = getattr(torch._C, "_are_functorch_transforms_active", lambda: False)
-
-
 def eager(*tensors) -> bool:
     """An eager call on plain tensors, parameters or None (functional._plain_eager, which takes no parameters)."""
-    if torch.compiler.is_compiling() or torch._C._is_tracing() or _functorch_active():
+    if _recorded():
         return False
     for t in tensors:
         if t is not None and type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:

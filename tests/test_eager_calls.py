@@ -5,6 +5,8 @@ this runs on the CPU."""
 import pytest
 import torch
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
+from torch.utils._python_dispatch import TorchDispatchMode
 
 import flash_attn_prologue_b200 as fap
 from flash_attn_prologue_b200 import functional, fused_epilogue, gqa, paged
@@ -32,10 +34,12 @@ def plain_gqa(monkeypatch):
 
 def _step(device="cpu"):
     """append_paged_kv's arguments, and paged_attention's."""
-    q, k, w, s, sin, cos = _rows(device)
-    caches = [torch.zeros(4, 16, 2, 64, device=device) for _ in range(2)]
+    q, k, w, s, _, _ = _rows(device)
+    sin, cos = tables(16, 64, device)
+    g = torch.Generator().manual_seed(1)
+    caches = [torch.randn(4, 16, 2, 64, generator=g).to(device) for _ in range(2)]
     table = torch.arange(3, dtype=torch.int32, device=device)[:, None]
-    lens = torch.ones(3, dtype=torch.int32, device=device)
+    lens = torch.full((3,), 9, dtype=torch.int32, device=device)
     return [q, k, k.clone(), w, s, sin, cos, *caches, table, lens, None], [q, *caches, table, lens, None]
 
 
@@ -128,3 +132,51 @@ def test_forward_mode_transform_is_refused(plain_gqa, plain_step):
     q, *rest = _step()[1]
     with pytest.raises(NotImplementedError, match="forward"):
         torch.func.jvp(lambda q: fap.paged_attention(q, *rest), (q,), (torch.ones_like(q),))
+
+
+class _Names(TorchDispatchMode):
+    """Notes the operators called under it."""
+
+    def __init__(self):
+        super().__init__()
+        self.names = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        self.names.append(func.name())
+        return func(*args, **(kwargs or {}))
+
+
+def _calls(device):
+    rows = _rows(device)
+    cute = [rows[0], rows[1].repeat_interleave(2, 1), *rows[2:]]
+    append, attend = _step(device)
+    if device == "cuda":
+        append, attend = ([t.bfloat16() if t is not None and t.ndim >= 3 and t.shape[-1] == 64 and t.shape[0] > 2 else t
+                           for t in args] for args in (append, attend))
+    return [("qknorm_rope_scale_gqa", fap.qknorm_rope_scale_gqa, rows),
+            ("qknorm_rope_scale_cute", lambda *a: fap.qknorm_rope_scale(*a, backend="cute"), cute),
+            ("append_paged_kv", fap.append_paged_kv, append), ("paged_attention", fap.paged_attention, attend)]
+
+
+@pytest.mark.parametrize("which", [0, 2, 3])
+def test_dispatch_modes_and_traces_see_the_operators(which, plain_gqa, plain_step):
+    name, call, args = _calls("cpu")[which]
+    with _Names() as seen:
+        call(*args)
+    assert f"flash_prologue::{name}" in seen.names
+    graph = make_fx(lambda *a: call(*a))(*args)
+    assert name in graph.code
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", range(4))
+def test_a_trace_of_real_tensors_replays(which):
+    """make_fx on real tensors records the operator, and its graph computes new results from new inputs."""
+    name, call, args = _calls("cuda")[which]
+    fresh = lambda: [t.clone() if t is not None else None for t in args]  # noqa: E731
+    graph = make_fx(lambda *a: call(*a))(*fresh())
+    assert name in graph.code
+    args = [args[0] * 2 + 1, *args[1:]]
+    a, b = call(*fresh()), graph(*fresh())
+    for x, y in zip(a if isinstance(a, tuple) else (a,), b if isinstance(b, tuple) else (b,)):
+        assert torch.equal(x, y) and x.any()
