@@ -15,6 +15,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .fused_epilogue import _DeviceGuard
@@ -123,8 +124,11 @@ def append_paged_kv(q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache,
     """
     args = (q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
     _no_grad("append_paged_kv", q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache)
-    call = _append if eager(q, k, v, rmsnorm_weight, sin, k_cache) else torch.ops.flash_prologue.append_paged_kv
-    return call(*args, eps)
+    if not eager(q, k, v, rmsnorm_weight, sin, k_cache):
+        return torch.ops.flash_prologue.append_paged_kv(*args, eps)
+    out = _append(*args, eps)
+    increment_version((k_cache, v_cache))  # as the registered op: autograd refuses what it saved of the caches before
+    return out
 
 
 ATTENTION_HEAD_DIMS = (64, 128)

@@ -180,3 +180,32 @@ def test_a_trace_of_real_tensors_replays(which):
     a, b = call(*fresh()), graph(*fresh())
     for x, y in zip(a if isinstance(a, tuple) else (a,), b if isinstance(b, tuple) else (b,)):
         assert torch.equal(x, y) and x.any()
+
+
+@pytest.mark.parametrize("call", [fap.append_paged_kv, lambda *a: OPS.append_paged_kv(*a, 1e-5)])
+def test_an_append_counts_as_a_change_of_the_caches(call, plain_step):
+    args = _step()[0]
+    caches = args[7:9]
+    weight = torch.ones(64, requires_grad=True)
+    saved = [(c * weight).sum() for c in caches]  # the caches are kept for the backward
+    with torch.no_grad():
+        call(*args)
+    assert [c._version for c in caches] == [1, 1]
+    for loss in saved:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():
+        args = _step()[0]
+        call(*args)  # inference tensors have no version to count
+
+
+@pytest.mark.gpu
+def test_an_append_on_the_gpu_counts_as_a_change():
+    _, call, args = _calls("cuda")[2]
+    weight = torch.ones(64, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    loss = (args[8][1:] * weight).sum()  # a view's counter is its base's
+    call(*args)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        call(*[t.clone() if t is not None else None for t in args])
