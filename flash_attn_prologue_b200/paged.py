@@ -124,7 +124,7 @@ def append_paged_kv(q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache,
     """
     args = (q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
     _no_grad("append_paged_kv", q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache)
-    if not eager(q, k, v, rmsnorm_weight, sin, k_cache):
+    if not eager(*args):
         return torch.ops.flash_prologue.append_paged_kv(*args, eps)
     out = _append(*args, eps)
     increment_version((k_cache, v_cache))  # as the registered op: autograd refuses what it saved of the caches before
@@ -221,6 +221,6 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, cu_seqlens=None, 
     """
     tensors = (q, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
     _no_grad("paged_attention", q, k_cache, v_cache)
-    call = _attention if eager(q, k_cache, page_table) else torch.ops.flash_prologue.paged_attention
+    call = _attention if eager(*tensors) else torch.ops.flash_prologue.paged_attention
     out, lse = call(*tensors, softmax_scale, window, return_lse)
     return (out, lse) if return_lse else out

@@ -209,3 +209,26 @@ def test_an_append_on_the_gpu_counts_as_a_change():
         loss.backward()
     with torch.inference_mode():
         call(*[t.clone() if t is not None else None for t in args])
+
+
+class _Noting(torch.Tensor):
+    """A tensor subclass that notes the operators called with it."""
+
+    names = []
+
+    @classmethod
+    def __torch_function__(cls, func, types, args=(), kwargs=None):
+        cls.names.append(str(func))
+        return super().__torch_function__(func, types, args, kwargs or {})
+
+
+@pytest.mark.parametrize("which,at", [(w, i) for w, n in ((0, 6), (2, 12), (3, 6)) for i in range(n)])
+def test_a_tensor_subclass_in_any_place_takes_the_operator(which, at, plain_gqa, plain_step):
+    name, call, args = _calls("cpu")[which]
+    args = list(args)
+    if args[at] is None:  # cu_seqlens
+        args[at] = torch.arange(4, dtype=torch.int32)
+    args[at] = args[at].as_subclass(_Noting)
+    _Noting.names.clear()
+    call(*args)
+    assert any(f"flash_prologue.{name}" in n for n in _Noting.names)
