@@ -629,7 +629,8 @@ template <typename T, int D>
 cudaError_t launch(AttentionArgs a, cudaStream_t stream) {
   // Short caches: a CTA does whole items, which takes it a few steps more and saves the
   // second kernel. 32/8 heads x 128, 64 requests of 128 and 256 keys: 14.5 and 19.0 us,
-  // split 20.2 and 24.2; one request of 256 and 512 keys: 9.4 and 12.8 us, split 8.2.
+  // split 20.2 and 24.2. The rule knows the table's width, not the lengths: one request of
+  // 256 keys loses by it (9.4 us, split 8.2), and so do many short ones under a wide table.
   a.whole = a.max_keys <= kWholeKeys;
   constexpr size_t smem = (size_t)kDecodeWarps * kRing * 2 * kWarpKeys * D * 2;
   const void* fn = reinterpret_cast<const void*>(&paged_decode_kernel<T, D>);

@@ -276,7 +276,8 @@ def qknorm_rope_scale_gqa(q, k, rmsnorm_weight, scales, sin, cos, positions=None
     (int32 or int64; [T], or [N] / [B,N] for dense rows) names each token's row, and
     without it token n has row n. A position outside the tables gives NaN rows and sets
     the device error word. All arithmetic through the final cast is FP32. Differentiable
-    in q, k, rmsnorm_weight and scales; outputs and gradients keep the inputs' memory order.
+    in q, k, rmsnorm_weight and scales, once: second and forward-mode derivatives are refused.
+    Outputs and gradients keep the inputs' memory order.
     """
     refuse_tangents("qknorm_rope_scale_gqa", q, k, rmsnorm_weight, scales, sin, cos)
     if eager(q, k, rmsnorm_weight, scales, sin, cos, positions):

@@ -118,9 +118,10 @@ def append_paged_kv(q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache,
     index among them, which is also where it is written: slot ``position % page_size`` of page
     ``page_table[request, position // page_size]``. rmsnorm_weight [2,1,D] or None (rotation
     only), scales [Hq,1,1] or None, sin/cos FP32 tables [positions, D/2] as in
-    qknorm_rope_scale_gqa. Tokens past the last request come back as zeros and are not
-    written; so are tokens whose position, page or table row is out of range, which also set
-    the device error word. Not differentiable.
+    qknorm_rope_scale_gqa. Tokens past the last request, or before the first where cu_seqlens
+    begin above 0, come back as zeros and are not written; so are tokens whose position, page or table row is out of range, which also set
+    the device error word. Counts as an in-place change of both caches. Not differentiable:
+    tensors that require gradients (where they are enabled) or carry tangents are refused.
     """
     args = (q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
     _no_grad("append_paged_kv", q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache)
@@ -214,10 +215,12 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, cu_seqlens=None, 
     of all requests as append_paged_kv returns them. A token at position p of its request
     attends to the cached positions 0 .. p, or p - window + 1 .. p with a window; query head h
     reads key head h // (Hq / Hk). softmax_scale multiplies the scores: 1 by default, since the
-    prologue's exp(scales) has scaled Q. Returns the rows [T,Hq,D] in q's type and, with
-    return_lse, the scores' log-sum-exp [T,Hq] in FP32. A token that sees no key gets zeros
-    (lse -inf); one whose page is outside the cache gets NaN and the device error word is set.
-    What lies in slots that a token does not see never reaches it. Not differentiable.
+    prologue's exp(scales) has scaled Q (it has to be finite in FP32). Returns the rows [T,Hq,D] in q's type and, with
+    return_lse, the scores' log-sum-exp [T,Hq] in FP32. A token that sees no key, padding on
+    either side of the requests included, gets zeros (lse -inf); one whose page is outside the
+    cache gets NaN, as may tokens of its request near it, and the device error word is set.
+    What lies in slots that a token does not see never reaches it. Not differentiable: as
+    append_paged_kv.
     """
     tensors = (q, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
     _no_grad("paged_attention", q, k_cache, v_cache)

@@ -559,10 +559,12 @@ typedef struct flash_prologue_attention_args {
  * h / (Hq / Hk). BF16 or FP16, D in {64, 128}; scores, statistics and sums are
  * FP32. Keys that a token does not see never reach it, whatever their slots
  * hold. A token that sees no key (position below 0, padding past the last
- * request or before the first) gets zeros and an lse of -infinity; one that needs a page outside
- * the cache gets NaN, and the error word. Results are the same run to run.
- * Rows and caches are 16-byte aligned. workspace: 16-byte aligned, at least
- * flash_prologue_paged_attention_workspace_size() bytes, no initialisation.
+ * request or before the first) gets zeros and an lse of -infinity; one that needs
+ * a page outside the cache gets NaN, as may rows of its request in the same tile,
+ * and the error word. softmax_scale * log2(e) has to be finite in FP32. Results
+ * are the same run to run. Rows and caches are 16-byte aligned. workspace: 16-byte
+ * aligned, at least flash_prologue_paged_attention_workspace_size() bytes, no
+ * initialisation.
  */
 FLASH_PROLOGUE_API int flash_prologue_paged_attention(const flash_prologue_attention_args* args, void* stream);
 /*
