@@ -6,7 +6,8 @@ import torch
 
 import flash_attn_prologue_b200 as fap
 from flash_attn_prologue_b200 import _lib
-from tests._paged import BAND, HALF_ULP, TINY, assert_within, rotate64, tables
+from tests._paged import assert_within, rotate64, tables
+from tests._paged import BAND, HALF_ULP, TINY
 
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
 

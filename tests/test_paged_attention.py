@@ -427,8 +427,6 @@ def _cpu_call(**change):
     (dict(seq_lens=torch.ones(3, dtype=torch.int64)), "int32"),
     (dict(cu_seqlens=torch.zeros(3, dtype=torch.int32)), "cu_seqlens must be"),
     (dict(softmax_scale=math.nan), "softmax_scale"),
-    (dict(softmax_scale=3e38), "softmax_scale"),
-    (dict(softmax_scale=-1e300), "softmax_scale"),
     (dict(window=-1), "window"),
     (dict(q=torch.zeros(3, 8, 64, dtype=BF16, requires_grad=True)), "not differentiable"),
     (dict(), "CUDA devices only"),
@@ -448,11 +446,23 @@ def test_c_abi_refusals():
             ptr, 0, 64, n, ptr, 0, 64, n, 0, *cache, 0, 0, T, Hq, Hk, D, dtype, window, scale), None)
 
     assert call(T=0, batch=0, ptr=0) == _lib.OK
-    for cycles in (0, -1, 10 ** 10):
-        assert lib.flash_prologue_selftest_attention_waits(bytes(_lib.ATTENTION_ARGS.size), cycles, None) == 1
     for wrong, status in ((dict(dtype=2), 2), (dict(D=32), 2), (dict(Hk=3), 1), (dict(Hk=0), 1), (dict(Hq=1024), 2),
-                          (dict(window=-1), 1), (dict(scale=math.inf), 1), (dict(scale=3e38), 1), (dict(scale=math.nan), 1), (dict(page=24), 1), (dict(page=4), 1),
+                          (dict(window=-1), 1), (dict(scale=math.inf), 1), (dict(page=24), 1), (dict(page=4), 1),
                           (dict(slot=129), _lib.ERR_ALIGNMENT), (dict(k=72), _lib.ERR_ALIGNMENT), (dict(k=0), 1),
                           (dict(batch=2), 1), (dict(ptr=0), 1), (dict(ptr=68), _lib.ERR_ALIGNMENT),
                           (dict(n=513), _lib.ERR_ALIGNMENT), (dict(T=-1), 1), (dict(batch=-1, cu=64), 1)):
         assert call(**wrong) == status, wrong
+
+
+@pytest.mark.parametrize("scale", [3e38, -1e300, math.nan, math.inf])
+def test_scales_that_fp32_cannot_hold_are_refused(scale):
+    with pytest.raises(ValueError, match="softmax_scale"):
+        _cpu_call(softmax_scale=scale)
+    cache = (64, 2048, 128, 64, 64, 2048, 128, 64, 4, 16, 64, 1, 1, 64, 0, 3)
+    args = _lib.ATTENTION_ARGS.pack(64, 0, 64, 512, 64, 0, 64, 512, 0, *cache, 0, 0, 3, 8, 2, 64, 0, 0, scale)
+    assert _lib.load().flash_prologue_paged_attention(args, None) == 1
+
+
+@pytest.mark.parametrize("cycles", [0, -1, 10 ** 10])
+def test_wait_limits_that_are_refused(cycles):
+    assert _lib.load().flash_prologue_selftest_attention_waits(bytes(_lib.ATTENTION_ARGS.size), cycles, None) == 1
