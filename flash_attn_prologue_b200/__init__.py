@@ -30,6 +30,11 @@ _LAZY = {
     "qknorm_rope_scale_gqa": ("gqa", "qknorm_rope_scale_gqa"),
     "append_paged_kv": ("paged", "append_paged_kv"),
     "paged_attention": ("paged", "paged_attention"),
+    "rotary_axes": ("gqa", "rotary_axes"),
+    "append_paged_kv_int4": ("int4", "append_paged_kv_int4"),
+    "unpack_int4": ("int4", "unpack_int4"),
+    "int4_cache": ("int4", "int4_cache"),
+    "plan_paged_step": ("plan", "plan_paged_step"),
 }
 __all__ = ["qknorm_rope_scale", "qknorm_rope_scale_qkv", "prepare_backend", "RMSNormRoPEScale", "FusedQKV",
            *_LAZY]

@@ -92,6 +92,12 @@ SIGNATURES = {
     "flash_prologue_paged_attention": ([ctypes.c_char_p, _vp], ctypes.c_int),
     "flash_prologue_selftest_attention_waits": ([ctypes.c_char_p, _i64, _vp], ctypes.c_int),
     "flash_prologue_paged_attention_workspace_size": ([_i64, ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
+    "flash_prologue_gqa_fwd_axes": ([ctypes.c_char_p, ctypes.c_char_p, _vp], ctypes.c_int),
+    "flash_prologue_gqa_bwd_axes": ([ctypes.c_char_p, ctypes.c_char_p, _vp], ctypes.c_int),
+    "flash_prologue_append_paged_axes": ([ctypes.c_char_p, ctypes.c_char_p, _vp], ctypes.c_int),
+    "flash_prologue_append_paged_int4": ([ctypes.c_char_p, ctypes.c_char_p, ctypes.c_char_p, _vp], ctypes.c_int),
+    "flash_prologue_unpack_int4": ([_vp, _vp, _vp, _i64, _i64, _i64, _vp], ctypes.c_int),
+    "flash_prologue_plan_paged_step": ([ctypes.c_char_p, _vp], ctypes.c_int),
 }
 
 # The argument structs of include/flash_prologue.h whose fields are all 8 bytes
@@ -100,6 +106,9 @@ _ROWS, _ROTATION, _CACHE = "Pqqq", "PqqPqqq", "PqqqPqqqqqPqqPPq"
 GQA_ARGS = struct.Struct("@" + 8 * _ROWS + "PP" + _ROTATION + "Pqqq" + "PP" + "Pq" + "Pq" + "6q" + "d")
 APPEND_ARGS = struct.Struct("@" + 4 * _ROWS + "PP" + _ROTATION + _CACHE + "5q" + "d")
 ATTENTION_ARGS = struct.Struct("@" + 2 * _ROWS + "P" + _CACHE + "Pq" + "6q" + "d")
+AXES_ARGS = struct.Struct("@Pqqqqq4Q")
+SCALES_ARGS = struct.Struct("@PqqqPqqq")
+PLAN_ARGS = struct.Struct("@PqqPPPPqPPPPPPP3q")
 NO_ROWS = (0, 0, 0, 0)
 
 MAX_PEERS = 8

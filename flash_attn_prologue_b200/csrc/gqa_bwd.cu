@@ -30,7 +30,7 @@ struct Walk {
   bool there;         // this lane's token exists (the pointers stay put where not)
 };
 
-template <typename T, int D, bool VEC>
+template <typename T, int D, bool VEC, bool AXES>
 __global__ void __launch_bounds__(kThreads, 2) gqa_bwd_kernel(const GqaBwdArgs a) {
   constexpr int L = D / 16;
   constexpr int HALF = D / 2;
@@ -138,10 +138,18 @@ __global__ void __launch_bounds__(kThreads, 2) gqa_bwd_kernel(const GqaBwdArgs a
     const bool there = token_of(item, b, n, i0);
     const int i1 = i0 + a.p.per_slice;
     float sn[kChunk], cs[kChunk];
-    const int64_t pos = there ? rotation_row(a.tab, b, n) : -1;
+    int64_t pos;
+    [[maybe_unused]] int rows[4];
+    if constexpr (AXES) pos = there && rotation_rows(a.tab, b, n, rows) ? 0 : -1;
+    else pos = there ? rotation_row(a.tab, b, n) : -1;
     if (pos >= 0) {
-      load_columns<T, D, VEC>(sn, a.tab.sin + pos * a.tab.sin_n + j0 * a.tab.sin_j, a.tab.sin_j);
-      load_columns<T, D, VEC>(cs, a.tab.cos + pos * a.tab.cos_n + j0 * a.tab.cos_j, a.tab.cos_j);
+      if constexpr (AXES) {
+        load_turned<T, D, VEC>(sn, a.tab.sin, a.tab.sin_n, a.tab.sin_j, a.tab, rows, j0);
+        load_turned<T, D, VEC>(cs, a.tab.cos, a.tab.cos_n, a.tab.cos_j, a.tab, rows, j0);
+      } else {
+        load_columns<T, D, VEC>(sn, a.tab.sin + pos * a.tab.sin_n + j0 * a.tab.sin_j, a.tab.sin_j);
+        load_columns<T, D, VEC>(cs, a.tab.cos + pos * a.tab.cos_n + j0 * a.tab.cos_j, a.tab.cos_j);
+      }
     } else {
       const float v = there ? __int_as_float(0x7fc00000) : 0.f;  // as in the forward
 #pragma unroll
@@ -238,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, 2) gqa_bwd_kernel(const GqaBwdArgs a
   }
 }
 
-const void* bwd_kernel_for(int dtype, int D, bool vec) { FLASH_PROLOGUE_GQA_KERNEL(gqa_bwd_kernel) }
+const void* bwd_kernel_for(int dtype, int D, bool vec, bool axes) { FLASH_PROLOGUE_GQA_KERNEL(gqa_bwd_kernel) }
 
 size_t smem_bytes(int Hq, int D, int dtype, bool vec) {
   const size_t floats = (size_t)2 * D + (size_t)Hq * (kWarps + 2) + (size_t)kWarps * 2 * D;
@@ -247,8 +255,8 @@ size_t smem_bytes(int Hq, int D, int dtype, bool vec) {
 }
 
 // The kernel with its shared memory allowed (above 48 KB it has to be asked for).
-const void* ready_kernel(int Hq, int D, int dtype, bool vec, size_t* smem) {
-  const void* fn = bwd_kernel_for(dtype, D, vec);
+const void* ready_kernel(int Hq, int D, int dtype, bool vec, bool axes, size_t* smem) {
+  const void* fn = bwd_kernel_for(dtype, D, vec, axes);
   if (!fn) return nullptr;
   *smem = smem_bytes(Hq, D, dtype, vec);
   if (*smem > 48 * 1024 && allow_shared_memory(fn, *smem) != cudaSuccess) return nullptr;
@@ -257,9 +265,9 @@ const void* ready_kernel(int Hq, int D, int dtype, bool vec, size_t* smem) {
 
 }  // namespace
 
-int64_t gqa_bwd_grid(const RowsPlan& p, int Hq, int D, int dtype, bool vec) {
+int64_t gqa_bwd_grid(const RowsPlan& p, int Hq, int D, int dtype, bool vec, bool axes) {
   size_t smem = 0;
-  const void* fn = ready_kernel(Hq, D, dtype, vec, &smem);
+  const void* fn = ready_kernel(Hq, D, dtype, vec, axes, &smem);
   if (!fn) return -1;
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess ||
@@ -272,8 +280,8 @@ int64_t gqa_bwd_grid(const RowsPlan& p, int Hq, int D, int dtype, bool vec) {
 cudaError_t launch_gqa_bwd(const GqaBwdArgs& a, float* dw, float* ds, int dtype, int D, bool vec,
                            const BwdReduce& red, cudaStream_t stream) {
   size_t smem = 0;
-  const void* fn = ready_kernel(a.H[0], D, dtype, vec, &smem);
-  const int64_t grid = gqa_bwd_grid(a.p, a.H[0], D, dtype, vec);
+  const void* fn = ready_kernel(a.H[0], D, dtype, vec, a.tab.axes != 0, &smem);
+  const int64_t grid = gqa_bwd_grid(a.p, a.H[0], D, dtype, vec, a.tab.axes != 0);
   if (!fn || grid <= 0) return cudaErrorInvalidConfiguration;
   GqaBwdArgs args = a;
   void* params[] = {&args};

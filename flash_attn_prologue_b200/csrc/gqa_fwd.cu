@@ -3,7 +3,8 @@
 // scale, written to dense outputs, or with K and V going to the pages of a
 // cache (append). Per row
 //   y = x / sqrt(mean(x^2) + eps) * w;  o = R(pos) y;  Q: o *= exp(scale[h])
-// with the arithmetic (and rounding order) of the equal-heads forward.
+// with the arithmetic (and rounding order) of the equal-heads forward. Into a
+// cache of 4 bits K and V go as codes and scales (int4_rows.cuh), from FP32.
 //
 // Bound by HBM: every row is read and written once, the tables once a token.
 // A lane owns one chunk pair of a row (rotation partners in one lane) and a
@@ -12,6 +13,7 @@
 // a ring in shared memory: each lane copies its own chunks with cp.async,
 // kStages - 1 row blocks ahead, and reads back only what it copied.
 #include "gqa_rows.cuh"
+#include "int4_rows.cuh"
 
 namespace flash_prologue {
 namespace {
@@ -31,7 +33,23 @@ __device__ __forceinline__ int request_of(const int32_t* cu, int batch, int64_t 
   return lo;
 }
 
-template <typename T, int D, bool VEC>
+// 1 / sqrt(mean + eps) in 64 bits, rounded once: where a row is rounded to codes, those do
+// not depend on the order of its sum.
+template <typename T, int D, int L>
+__device__ __forceinline__ float inv_rms_exact(const Chunk<T>& x1, const Chunk<T>& x2, float eps) {
+  double sum = 0;
+#pragma unroll
+  for (int p = 0; p < kPairs; ++p) {
+    const float2 a = chunk_get2(x1, p), b = chunk_get2(x2, p);
+    sum = fma((double)a.x, (double)a.x, fma((double)a.y, (double)a.y, sum));
+    sum = fma((double)b.x, (double)b.x, fma((double)b.y, (double)b.y, sum));
+  }
+#pragma unroll
+  for (int o = 1; o < L; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return (float)(1.0 / sqrt(sum * (1.0 / D) + (double)eps));
+}
+
+template <typename T, int D, bool VEC, bool AXES, bool INT4 = false>
 __global__ void __launch_bounds__(kThreads, 3) gqa_fwd_kernel(const GqaFwdArgs a) {
   constexpr int L = D / 16;
   constexpr int HALF = D / 2;
@@ -115,6 +133,7 @@ __global__ void __launch_bounds__(kThreads, 3) gqa_fwd_kernel(const GqaFwdArgs a
     const bool there = token < tokens;
     int b = 0, n = there ? token : 0, page = 0, in_page = 0;
     int64_t pos = -1;
+    [[maybe_unused]] int rows[4];  // AXES: pos only says whether the token is turned and placed
     if (there) {
       if (paged) {
         const PagedTarget& pg = a.paged;
@@ -128,10 +147,13 @@ __global__ void __launch_bounds__(kThreads, 3) gqa_fwd_kernel(const GqaFwdArgs a
         // Tokens past the last request (padding) belong to none: their Q rows come out as zeros.
         if (token >= first && token < first + count) {
           const int64_t at = (int64_t)__ldg(pg.seq_lens + r) - count + (token - first);
-          bool ok = at >= 0 && at < a.tab.rows && (at >> pg.page_log2) < pg.max_pages;
+          bool ok = at >= 0 && (AXES || at < a.tab.rows) && (at >> pg.page_log2) < pg.max_pages;
           if (ok) {
             page = __ldg(pg.page_table + r * pg.table_stride + (at >> pg.page_log2));
             ok = page >= 0 && page < pg.num_pages;
+          }
+          if constexpr (AXES) {
+            if (ok) ok = rotation_rows(a.tab, 0, token, rows);
           }
           if (ok) {
             pos = at;
@@ -145,14 +167,20 @@ __global__ void __launch_bounds__(kThreads, 3) gqa_fwd_kernel(const GqaFwdArgs a
           b = token / N;
           n = token - b * N;
         }
-        pos = rotation_row(a.tab, b, n);
+        if constexpr (AXES) pos = rotation_rows(a.tab, b, n, rows) ? 0 : -1;
+        else pos = rotation_row(a.tab, b, n);
       }
     }
     const bool placed = pos >= 0;
     float sn[kChunk], cs[kChunk];
     if (placed) {
-      load_columns<T, D, VEC>(sn, a.tab.sin + pos * a.tab.sin_n + j0 * a.tab.sin_j, a.tab.sin_j);
-      load_columns<T, D, VEC>(cs, a.tab.cos + pos * a.tab.cos_n + j0 * a.tab.cos_j, a.tab.cos_j);
+      if constexpr (AXES) {
+        load_turned<T, D, VEC>(sn, a.tab.sin, a.tab.sin_n, a.tab.sin_j, a.tab, rows, j0);
+        load_turned<T, D, VEC>(cs, a.tab.cos, a.tab.cos_n, a.tab.cos_j, a.tab, rows, j0);
+      } else {
+        load_columns<T, D, VEC>(sn, a.tab.sin + pos * a.tab.sin_n + j0 * a.tab.sin_j, a.tab.sin_j);
+        load_columns<T, D, VEC>(cs, a.tab.cos + pos * a.tab.cos_n + j0 * a.tab.cos_j, a.tab.cos_j);
+      }
     } else {
       // A position out of range rotates by NaN (dense rows); a token without a place gives zeros.
       const float v = paged ? 0.f : __int_as_float(0x7fc00000);
@@ -173,6 +201,16 @@ __global__ void __launch_bounds__(kThreads, 3) gqa_fwd_kernel(const GqaFwdArgs a
       T* out = static_cast<T*>(a.y[t]) + h0 * a.sy[t].h + j0 +
                (to_cache ? page * a.sy[t].b + in_page * a.sy[t].n : b * a.sy[t].b + n * a.sy[t].n);
       const bool store = there && (placed || !to_cache);
+      // A cache of 4 bits: this lane's word of a row's first half, its scale (one of two lanes writes it).
+      unsigned char* codes = nullptr;
+      uint16_t* scale = nullptr;
+      if constexpr (INT4) {
+        if (t != 0) {
+          codes = static_cast<unsigned char*>(a.y[t]) + h0 * a.sy[t].h + page * a.sy[t].b + in_page * a.sy[t].n +
+                  lane % L * 4;
+          scale = a.scale[t - 1] + h0 * a.ss[t - 1].h + page * a.ss[t - 1].b + in_page * a.ss[t - 1].n + lane % L;
+        }
+      }
       float wa[kChunk], wb[kChunk];
       const float* scales = t == 0 ? a.scales : nullptr;
       if (t != 2) {
@@ -205,6 +243,32 @@ __global__ void __launch_bounds__(kThreads, 3) gqa_fwd_kernel(const GqaFwdArgs a
           chunk_zero(x1);
           chunk_zero(x2);
         }
+        if constexpr (INT4) {
+          if (t != 0) {
+            float2 o1[kPairs], o2[kPairs];
+            if (t == 1) {
+              const float r = a.w ? inv_rms_exact<T, D, L>(x1, x2, a.eps) : 1.f;
+              fwd_lane_values(x1, x2, r, wa, wb, sn, cs, false, 1.f, o1, o2);
+            } else {
+#pragma unroll
+              for (int p = 0; p < kPairs; ++p) {
+                o1[p] = chunk_get2(x1, p);
+                o2[p] = chunk_get2(x2, p);
+              }
+            }
+            uint32_t w1, w2;
+            uint16_t s;
+            int4_encode<T, L>(o1, o2, w1, w2, s);
+            if (store) {
+              *reinterpret_cast<uint32_t*>(codes) = w1;
+              *reinterpret_cast<uint32_t*>(codes + D / 4) = w2;
+              if (lane % L < L / 2) *scale = s;
+            }
+            codes += HS * a.sy[t].h;
+            scale += HS * a.ss[t - 1].h;
+            continue;
+          }
+        }
         if (t != 2) {
           const float r = a.w ? inv_rms<D>(row_sum<L>(lane_sumsq(x1, x2)), a.eps) : 1.f;
           const float e = scales ? expf(__ldg(scales + it * HS + hslot)) : 1.f;
@@ -225,7 +289,20 @@ __global__ void __launch_bounds__(kThreads, 3) gqa_fwd_kernel(const GqaFwdArgs a
   if constexpr (VEC) cp_async_wait<0>();
 }
 
-const void* fwd_kernel_for(int dtype, int D, bool vec) { FLASH_PROLOGUE_GQA_KERNEL(gqa_fwd_kernel) }
+const void* fwd_kernel_for(int dtype, int D, bool vec, bool axes) { FLASH_PROLOGUE_GQA_KERNEL(gqa_fwd_kernel) }
+
+template <typename T, bool AXES>
+const void* int4_kernel_of(int D, bool vec) {
+  if (D == 64)
+    return vec ? reinterpret_cast<const void*>(&gqa_fwd_kernel<T, 64, true, AXES, true>)
+               : reinterpret_cast<const void*>(&gqa_fwd_kernel<T, 64, false, AXES, true>);
+  return vec ? reinterpret_cast<const void*>(&gqa_fwd_kernel<T, 128, true, AXES, true>)
+             : reinterpret_cast<const void*>(&gqa_fwd_kernel<T, 128, false, AXES, true>);
+}
+const void* int4_kernel_for(int dtype, int D, bool vec, bool axes) {
+  if (axes) return dtype == 0 ? int4_kernel_of<__nv_bfloat16, true>(D, vec) : int4_kernel_of<__half, true>(D, vec);
+  return dtype == 0 ? int4_kernel_of<__nv_bfloat16, false>(D, vec) : int4_kernel_of<__half, false>(D, vec);
+}
 
 }  // namespace
 
@@ -255,7 +332,8 @@ RowsPlan plan_rows(int64_t tokens, int Hq, int Hk, int Hv, int D, bool heads_inn
 }
 
 cudaError_t launch_gqa_fwd(const GqaFwdArgs& a, int dtype, int D, bool vec, cudaStream_t stream) {
-  const void* fn = fwd_kernel_for(dtype, D, vec);
+  const bool axes = a.tab.axes != 0;
+  const void* fn = a.scale[0] ? int4_kernel_for(dtype, D, vec, axes) : fwd_kernel_for(dtype, D, vec, axes);
   if (!fn) return cudaErrorInvalidValue;
   const size_t smem = vec ? (size_t)kWarps * kStages * (dtype == 2 ? 2048 : 1024) : 0;
   if (smem > 48 * 1024) {

@@ -36,6 +36,11 @@ struct GqaTables {
   const void* positions;               // null: row n of the tables; else int32 / int64 [b, n]
   int64_t pos_b, pos_n;
   int pos_is64;
+  // Several axes (axes > 0): positions [axes, b, n], and the axis of pair j in bits
+  // 2 * (j % 32) of word j / 32, so a byte holds the axes of four neighbouring pairs.
+  int axes;
+  int64_t pos_axis;
+  uint64_t pair_axes[4];
 };
 
 struct PagedTarget {
@@ -57,6 +62,8 @@ struct GqaFwdArgs {
   const float* scales; // [Hq] or null
   GqaTables tab;
   bool append;         // K and V go to the pages of `paged`, else to dense outputs
+  uint16_t* scale[2];  // a cache of 4 bits: the scales of K and V (else null); y, sy: codes, in bytes
+  RowStrides ss[2];
   PagedTarget paged;
   int64_t B, N;
   int H[3];
@@ -88,7 +95,7 @@ inline bool valid_peers(const flash_prologue_peers* peers, int64_t epoch, int64_
 
 RowsPlan plan_rows(int64_t tokens, int Hq, int Hk, int Hv, int D, bool heads_inner, int64_t want_warps);
 cudaError_t launch_gqa_fwd(const GqaFwdArgs& a, int dtype, int D, bool vec, cudaStream_t stream);
-int64_t gqa_bwd_grid(const RowsPlan& p, int Hq, int D, int dtype, bool vec);
+int64_t gqa_bwd_grid(const RowsPlan& p, int Hq, int D, int dtype, bool vec, bool axes);
 cudaError_t launch_gqa_bwd(const GqaBwdArgs& a, float* dw, float* ds, int dtype, int D, bool vec,
                            const BwdReduce& red, cudaStream_t stream);
 
@@ -116,6 +123,23 @@ __device__ __forceinline__ int64_t rotation_row(const GqaTables& t, int64_t b, i
     return -1;
   }
   return pos;
+}
+
+// Rotation row of token (b, n) on each axis (the first again where there are fewer than
+// four); false, with the error word set, where one is out of range.
+__device__ __forceinline__ bool rotation_rows(const GqaTables& t, int64_t b, int64_t n, int (&row)[4]) {
+  const int64_t i = b * t.pos_b + n * t.pos_n;
+  bool ok = true;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const int64_t at = i + (x < t.axes ? x * t.pos_axis : 0);
+    const int64_t pos = t.pos_is64 ? static_cast<const int64_t*>(t.positions)[at]
+                                   : (int64_t) static_cast<const int32_t*>(t.positions)[at];
+    ok = ok && pos >= 0 && pos < t.rows;
+    row[x] = (int)pos;  // tables of axes have fewer than 2^31 rows (the host checks)
+  }
+  if (!ok) atomicOr(&g_device_error, kDeviceErrorIndex);
+  return ok;
 }
 
 template <typename T>
@@ -184,17 +208,45 @@ __device__ __forceinline__ void load_columns(float (&v)[kChunk], const float* ha
   }
 }
 
-// A kernel for each activation type, head dimension and access width.
+// The lane's 8 values of the rows that turn its pairs, each by its axis. Four pairs of
+// one axis are read at once; mixed ones (interleaved axes) one by one, from rows that
+// the warp's other lanes read too. First column of the lane: j0.
+template <typename T, int D, bool VEC>
+__device__ __forceinline__ void load_turned(float (&v)[kChunk], const float* table, int64_t s_row, int64_t s_col,
+                                            const GqaTables& t, const int (&row)[4], int j0) {
+  using C = Columns<T, D>;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int col = j0 + C::of(0, 4 * q);
+    const uint32_t byte = (uint32_t)(t.pair_axes[col >> 5] >> (2 * (col & 31))) & 0xffu;
+    const auto row_of = [&](uint32_t axis) {
+      return table + (int64_t)(axis == 0 ? row[0] : axis == 1 ? row[1] : axis == 2 ? row[2] : row[3]) * s_row;
+    };
+    if (VEC && byte == (byte & 3u) * 0x55u) {
+      const float4 x = __ldg(reinterpret_cast<const float4*>(row_of(byte & 3u) + col));
+      v[4 * q] = x.x; v[4 * q + 1] = x.y; v[4 * q + 2] = x.z; v[4 * q + 3] = x.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * q + e] = __ldg(row_of(byte >> (2 * e) & 3u) + (col + e) * s_col);
+    }
+  }
+}
+
+// A kernel for each activation type, head dimension, access width, and whether pairs
+// turn by several axes (kernels of their own: the others keep their registers).
+#define FLASH_PROLOGUE_GQA_AXES(T, DIM, VEC, KERNEL)                                              \
+  (axes ? reinterpret_cast<const void*>(&KERNEL<T, DIM, VEC, true>)                               \
+        : reinterpret_cast<const void*>(&KERNEL<T, DIM, VEC, false>))
 #define FLASH_PROLOGUE_GQA_DIMS(T, KERNEL)                                                        \
   switch (D) {                                                                                    \
-    case 32: return vec ? reinterpret_cast<const void*>(&KERNEL<T, 32, true>)                     \
-                        : reinterpret_cast<const void*>(&KERNEL<T, 32, false>);                   \
-    case 64: return vec ? reinterpret_cast<const void*>(&KERNEL<T, 64, true>)                     \
-                        : reinterpret_cast<const void*>(&KERNEL<T, 64, false>);                   \
-    case 128: return vec ? reinterpret_cast<const void*>(&KERNEL<T, 128, true>)                   \
-                         : reinterpret_cast<const void*>(&KERNEL<T, 128, false>);                 \
-    case 256: return vec ? reinterpret_cast<const void*>(&KERNEL<T, 256, true>)                   \
-                         : reinterpret_cast<const void*>(&KERNEL<T, 256, false>);                 \
+    case 32: return vec ? FLASH_PROLOGUE_GQA_AXES(T, 32, true, KERNEL)                            \
+                        : FLASH_PROLOGUE_GQA_AXES(T, 32, false, KERNEL);                          \
+    case 64: return vec ? FLASH_PROLOGUE_GQA_AXES(T, 64, true, KERNEL)                            \
+                        : FLASH_PROLOGUE_GQA_AXES(T, 64, false, KERNEL);                          \
+    case 128: return vec ? FLASH_PROLOGUE_GQA_AXES(T, 128, true, KERNEL)                          \
+                         : FLASH_PROLOGUE_GQA_AXES(T, 128, false, KERNEL);                        \
+    case 256: return vec ? FLASH_PROLOGUE_GQA_AXES(T, 256, true, KERNEL)                          \
+                         : FLASH_PROLOGUE_GQA_AXES(T, 256, false, KERNEL);                        \
     default: return nullptr;                                                                      \
   }
 #define FLASH_PROLOGUE_GQA_KERNEL(KERNEL)                                                         \

@@ -30,7 +30,7 @@ int size_checks(const flash_prologue_attention_args* a) {
   if ((a->dtype != FLASH_PROLOGUE_BF16 && a->dtype != FLASH_PROLOGUE_FP16) || a->Hq > kMaxGqaHeads ||
       (a->D != 64 && a->D != 128) || a->tokens >= (int64_t(1) << 31) / kMaxGqaHeads)
     return FLASH_PROLOGUE_ERR_UNSUPPORTED;
-  return check_cache(a->cache, a->tokens, a->dtype);
+  return check_cache(a->cache, a->tokens, 2);
 }
 
 // Tiles of 128 rows on the tensor cores where the requests have more rows a key

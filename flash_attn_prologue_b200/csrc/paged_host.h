@@ -6,8 +6,10 @@
 
 namespace flash_prologue {
 
-// Sizes, pointers and alignment of a cache and its tables (status code).
-int check_cache(const flash_prologue_cache& c, int64_t tokens, int64_t dtype);
+// Sizes, pointers and alignment of a cache (elements of `es` bytes) and its tables (status code).
+int check_cache(const flash_prologue_cache& c, int64_t tokens, size_t es);
+// Pointers and alignment of a 4-bit cache's scales.
+int check_scales(const flash_prologue_scales& s, const flash_prologue_cache& c, int64_t D);
 
 inline PagedTarget paged_target(const flash_prologue_cache& c) {
   PagedTarget t{};

@@ -319,12 +319,11 @@ __device__ __forceinline__ float lane_sumsq2(const Chunk<T>& x1, const Chunk<T>&
 // Every product and sum rounds separately, as in the eager formulation
 // (a - b is computed as a + (-b), which rounds identically).
 template <typename T>
-__device__ __forceinline__ void fwd_lane(const Chunk<T>& x1, const Chunk<T>& x2, float r,
-                                         const float* wa, const float* wb, const float (&sn)[kChunk],
-                                         const float (&cs)[kChunk], bool scale, float e,
-                                         Chunk<T>& out1, Chunk<T>& out2) {
+__device__ __forceinline__ void fwd_lane_values(const Chunk<T>& x1, const Chunk<T>& x2, float r,
+                                                const float* wa, const float* wb, const float (&sn)[kChunk],
+                                                const float (&cs)[kChunk], bool scale, float e,
+                                                float2 (&o1)[kPairs], float2 (&o2)[kPairs]) {
   const float2 r2 = splat2(r), e2 = splat2(e);
-  float2 o1[kPairs], o2[kPairs];
 #pragma unroll
   for (int p = 0; p < kPairs; ++p) {
     const float2 c2 = make_float2(cs[2 * p], cs[2 * p + 1]);
@@ -338,6 +337,15 @@ __device__ __forceinline__ void fwd_lane(const Chunk<T>& x1, const Chunk<T>& x2,
       o2[p] = __fmul2_rn(o2[p], e2);
     }
   }
+}
+// The same, rounded to T.
+template <typename T>
+__device__ __forceinline__ void fwd_lane(const Chunk<T>& x1, const Chunk<T>& x2, float r,
+                                         const float* wa, const float* wb, const float (&sn)[kChunk],
+                                         const float (&cs)[kChunk], bool scale, float e,
+                                         Chunk<T>& out1, Chunk<T>& out2) {
+  float2 o1[kPairs], o2[kPairs];
+  fwd_lane_values(x1, x2, r, wa, wb, sn, cs, scale, e, o1, o2);
   chunk_set2(out1, o1);
   chunk_set2(out2, o2);
 }

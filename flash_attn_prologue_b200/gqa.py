@@ -7,11 +7,14 @@ by exp(scales), with its backward; registered as
 prologue has equal Q and K heads and takes sin/cos rows in token order
 (flash_attn_prologue/functional.py:29-70); the arithmetic and the layouts are
 its own. The kernels (csrc/gqa_fwd.cu, csrc/gqa_bwd.cu) read strided views in
-place.
+place. With ``axes`` each rotation pair is turned by the position on an axis of
+its own (time, height and width of images and video); ``rotary_axes`` lays out
+the usual patterns.
 """
 import ctypes
+import functools
 import math
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple
 
 import torch
 from torch.autograd import forward_ad
@@ -68,6 +71,67 @@ def check_rows(q, k, rmsnorm_weight, scales, sin, cos, eps):
         raise ValueError("the prologue kernels run on CUDA devices only")
 
 
+MAX_AXES = 4
+
+
+def rotary_axes(sections, interleaved=False):
+    """The axis of each rotation pair, for ``axes=``: sections[a] of the D / 2 pairs turn by axis a.
+
+    In blocks (all pairs of axis 0, then those of axis 1, ...), or interleaved: the axes in
+    turn, 0, 1, 2, 0, 1, 2, ..., each as long as it has pairs left."""
+    sections = [int(n) for n in sections]
+    if not 1 <= len(sections) <= MAX_AXES or min(sections) < 0:
+        raise ValueError(f"sections must be 1 to {MAX_AXES} counts of pairs")
+    if not interleaved:
+        return tuple(a for a, n in enumerate(sections) for _ in range(n))
+    left, out = list(sections), []
+    while any(left):
+        for a, n in enumerate(left):
+            if n:
+                out.append(a)
+                left[a] -= 1
+    return tuple(out)
+
+
+@functools.lru_cache(maxsize=64)
+def _packed_axes(axes, half):
+    """``pairs`` of flash_prologue_axes, and one more than the last axis."""
+    if len(axes) != half:
+        raise ValueError("axes must name the axis of each of the D / 2 rotation pairs")
+    if min(axes) < 0 or max(axes) >= MAX_AXES:
+        raise ValueError(f"axes must be in 0 .. {MAX_AXES - 1}")
+    words = [0] * 4
+    for j, a in enumerate(axes):
+        words[j // 32] |= int(a) << 2 * (j % 32)
+    return tuple(words), max(axes) + 1
+
+
+def axes_of(axes, positions, q, rows):
+    """flash_prologue_axes of rows q packed [T, H, D] or dense [B, H, N, D] and tables of ``rows`` rows; axes None:
+    all pairs by the one position a token that positions has."""
+    half = q.shape[-1] // 2
+    if positions is None:
+        raise ValueError("axes take positions")
+    dtype, shape, st = positions.dtype, positions.shape, positions.stride()
+    if dtype is not torch.int32 and dtype is not torch.int64:
+        raise ValueError("positions must be int32 or int64")
+    tokens = q.shape[:1] if q.ndim == 3 else (q.shape[0], q.shape[2])
+    if axes is None:
+        words, count, named = (0, 0, 0, 0), 1, 1
+        shape, st = (1, *shape), (0, *st)
+    else:
+        words, named = _packed_axes(tuple(axes), half)
+        count = shape[0] if shape else 0
+    if shape[1:] != tokens and shape[1:] != tokens[1:] or not named <= count <= MAX_AXES or len(shape) < 2:
+        raise ValueError("positions must be [axes,T] for packed rows, [axes,N] or [axes,B,N] for dense rows")
+    if positions.device != q.device:
+        raise ValueError("all tensors must share a device")
+    if rows >= 1 << 31:
+        raise ValueError("sin/cos tables of several axes must have fewer than 2^31 rows")
+    return _lib.AXES_ARGS.pack(positions.data_ptr(), st[0], st[1] if len(st) == 3 else 0, st[-1],
+                               64 if dtype is torch.int64 else 32, count, *words)
+
+
 def _check_positions(positions, q, sin):
     n = q.shape[0] if q.ndim == 3 else q.shape[2]
     if positions is None:
@@ -101,14 +165,14 @@ def refuse_tangents(name, *tensors):
                 raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
-def call_library(name, args, device):
+def call_library(name, args, device, *more):
     """Calls entry point ``name`` on ``device``'s current stream, with the device current."""
     function = getattr(_lib.load(), name)
     if device.index == torch._C._cuda_getDevice():
-        status = function(args, _lib.raw_stream(device.index))
+        status = function(args, *more, _lib.raw_stream(device.index))
     else:
         with _DeviceGuard(device):
-            status = function(args, _lib.raw_stream(device.index))
+            status = function(args, *more, _lib.raw_stream(device.index))
     if status:
         _lib.check(status, name)
 
@@ -136,9 +200,9 @@ def flat_fp32(t):
     return t if not t.data_ptr() & 15 else t.clone()
 
 
-def _call(name, q, k, w, s, sin, cos, positions, eps, rows, grads=(0, 0), workspace=(0, 0), peers=(0, 0)):
+def _call(name, q, k, w, s, sin, cos, positions, eps, axes, rows, grads=(0, 0), workspace=(0, 0), peers=(0, 0)):
     B, N = (1, q.shape[0]) if q.ndim == 3 else (q.shape[0], q.shape[2])
-    if positions is None:
+    if positions is None or axes is not None:
         where = (0, 0, 0, 64)
     else:
         st = positions.stride()
@@ -147,7 +211,10 @@ def _call(name, q, k, w, s, sin, cos, positions, eps, rows, grads=(0, 0), worksp
     args = _lib.GQA_ARGS.pack(
         *rows_of(q), *rows_of(k), *rows, w.data_ptr(), s.data_ptr(), *rotation_of(sin, cos), *where, *grads,
         *workspace, *peers, B, N, q.shape[1], k.shape[1], q.shape[-1], _lib.DTYPE_CODES[q.dtype], eps)
-    call_library(name, args, q.device)
+    if axes is None:
+        call_library(name, args, q.device)
+    else:
+        call_library(name + "_axes", args, q.device, axes)
 
 
 def _in_place_rows(t):
@@ -159,14 +226,22 @@ def _in_place_rows(t):
     return t
 
 
-def gqa_forward(q, k, rmsnorm_weight, scales, sin, cos, positions, eps):
+def _turned(axes, positions, q, sin):
+    """flash_prologue_axes, or None where the one-axis call takes the (checked) positions."""
+    if axes is None:
+        _check_positions(positions, q, sin)
+        return None
+    return axes_of(axes, positions, q, sin.shape[0])
+
+
+def gqa_forward(q, k, rmsnorm_weight, scales, sin, cos, positions, eps, axes=None):
     check_rows(q, k, rmsnorm_weight, scales, sin, cos, eps)
-    _check_positions(positions, q, sin)
+    turn = _turned(axes, positions, q, sin)
     q, k = _in_place_rows(q), _in_place_rows(k)
     q_out, k_out = torch.empty_like(q), torch.empty_like(k)  # dense, in the inputs' memory order
     if q.numel():
         _call("flash_prologue_gqa_fwd", q, k, flat_fp32(rmsnorm_weight), scales.contiguous(), sin, cos, positions, eps,
-              (*rows_of(q_out), *rows_of(k_out), *_lib.NO_ROWS, *_lib.NO_ROWS, *_lib.NO_ROWS, *_lib.NO_ROWS))
+              turn, (*rows_of(q_out), *rows_of(k_out), *_lib.NO_ROWS, *_lib.NO_ROWS, *_lib.NO_ROWS, *_lib.NO_ROWS))
     return q_out, k_out
 
 
@@ -184,11 +259,15 @@ def _workspace_bytes(heads, dim, device):
     return nbytes
 
 
-def gqa_backward(q, k, rmsnorm_weight, scales, sin, cos, positions, grad_q_out, grad_k_out, eps, checked=False):
+def gqa_backward(q, k, rmsnorm_weight, scales, sin, cos, positions, grad_q_out, grad_k_out, eps, checked=False,
+                 axes=None):
     """``checked``: the arguments but the gradients went through gqa_forward."""
+    turn = None
     if not checked:
         check_rows(q, k, rmsnorm_weight, scales, sin, cos, eps)
-        _check_positions(positions, q, sin)
+        turn = _turned(axes, positions, q, sin)
+    elif axes is not None:
+        turn = axes_of(axes, positions, q, sin.shape[0])
     if grad_q_out.shape != q.shape or grad_k_out.shape != k.shape:
         raise ValueError("upstream gradients must have the shapes of q and k")
     q, k = _in_place_rows(q), _in_place_rows(k)
@@ -200,40 +279,47 @@ def gqa_backward(q, k, rmsnorm_weight, scales, sin, cos, positions, grad_q_out, 
     group = active_peer_group(q.device)
     peers = (0, 0) if group is None else (ctypes.addressof(group.desc), group.next_epoch())
     _call("flash_prologue_gqa_bwd", q, k, flat_fp32(rmsnorm_weight), scales.contiguous(), sin, cos, positions, eps,
-          (*_lib.NO_ROWS, *_lib.NO_ROWS, *rows_of(gq), *rows_of(gk), *rows_of(grad_q), *rows_of(grad_k)),
+          turn, (*_lib.NO_ROWS, *_lib.NO_ROWS, *rows_of(gq), *rows_of(gk), *rows_of(grad_q), *rows_of(grad_k)),
           (grad_w.data_ptr(), grad_s.data_ptr()), (workspace.data_ptr(), 4 * workspace.numel()), peers)
     return grad_q, grad_k, grad_w, grad_s
+
+
+def _forward(q, k, rmsnorm_weight, scales, sin, cos, positions, eps, axes):
+    args = (q, k, rmsnorm_weight, scales, sin, cos, positions, eps)
+    return gqa_forward(*args) if axes is None else gqa_forward(*args, axes=axes)
 
 
 class _GqaEager(torch.autograd.Function):
     """The op for eager calls, without the custom-op dispatch layers (as _CuteEager)."""
 
     @staticmethod
-    def forward(ctx, q, k, rmsnorm_weight, scales, sin, cos, positions, eps):
+    def forward(ctx, q, k, rmsnorm_weight, scales, sin, cos, positions, eps, axes):
         ctx.save_for_backward(q, k, rmsnorm_weight, scales, sin, cos, positions)
-        ctx.eps = eps
-        return gqa_forward(q, k, rmsnorm_weight, scales, sin, cos, positions, eps)
+        ctx.eps, ctx.axes = eps, axes
+        return _forward(q, k, rmsnorm_weight, scales, sin, cos, positions, eps, axes)
 
     @staticmethod
     def backward(ctx, grad_q, grad_k):
         if torch.is_grad_enabled():  # create_graph: the registered op, which refuses second derivatives
-            dq, dk, dw, ds = qknorm_rope_scale_gqa_backward_op(*ctx.saved_tensors, grad_q, grad_k, ctx.eps)
+            dq, dk, dw, ds = qknorm_rope_scale_gqa_backward_op(*ctx.saved_tensors, grad_q, grad_k, ctx.eps, ctx.axes)
         else:
-            dq, dk, dw, ds = gqa_backward(*ctx.saved_tensors, grad_q, grad_k, ctx.eps, checked=True)
-        return dq, dk, dw, ds, None, None, None, None
+            more = {} if ctx.axes is None else {"axes": ctx.axes}
+            dq, dk, dw, ds = gqa_backward(*ctx.saved_tensors, grad_q, grad_k, ctx.eps, checked=True, **more)
+        return dq, dk, dw, ds, None, None, None, None, None
 
 
 @torch.library.custom_op("flash_prologue::qknorm_rope_scale_gqa", mutates_args=())
 def qknorm_rope_scale_gqa_op(
     q: torch.Tensor, k: torch.Tensor, rmsnorm_weight: torch.Tensor, scales: torch.Tensor, sin: torch.Tensor,
     cos: torch.Tensor, positions: Optional[torch.Tensor] = None, eps: float = 1e-5,
+    axes: Optional[Sequence[int]] = None,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     refuse_tangents("qknorm_rope_scale_gqa", q, k, rmsnorm_weight, scales, sin, cos)
-    return gqa_forward(q, k, rmsnorm_weight, scales, sin, cos, positions, eps)
+    return _forward(q, k, rmsnorm_weight, scales, sin, cos, positions, eps, axes)
 
 
 @qknorm_rope_scale_gqa_op.register_fake
-def _gqa_fake(q, k, rmsnorm_weight, scales, sin, cos, positions=None, eps=1e-5):
+def _gqa_fake(q, k, rmsnorm_weight, scales, sin, cos, positions=None, eps=1e-5, axes=None):
     return torch.empty_like(_in_place_rows(q)), torch.empty_like(_in_place_rows(k))
 
 
@@ -241,14 +327,15 @@ def _gqa_fake(q, k, rmsnorm_weight, scales, sin, cos, positions=None, eps=1e-5):
 def qknorm_rope_scale_gqa_backward_op(
     q: torch.Tensor, k: torch.Tensor, rmsnorm_weight: torch.Tensor, scales: torch.Tensor, sin: torch.Tensor,
     cos: torch.Tensor, positions: Optional[torch.Tensor], grad_q_out: torch.Tensor, grad_k_out: torch.Tensor,
-    eps: float = 1e-5,
+    eps: float = 1e-5, axes: Optional[Sequence[int]] = None,
 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     refuse_tangents("qknorm_rope_scale_gqa_backward", q, k, rmsnorm_weight, scales, sin, cos, grad_q_out, grad_k_out)
-    return gqa_backward(q, k, rmsnorm_weight, scales, sin, cos, positions, grad_q_out, grad_k_out, eps)
+    more = {} if axes is None else {"axes": axes}
+    return gqa_backward(q, k, rmsnorm_weight, scales, sin, cos, positions, grad_q_out, grad_k_out, eps, **more)
 
 
 @qknorm_rope_scale_gqa_backward_op.register_fake
-def _gqa_backward_fake(q, k, rmsnorm_weight, scales, sin, cos, positions, grad_q_out, grad_k_out, eps=1e-5):
+def _gqa_backward_fake(q, k, rmsnorm_weight, scales, sin, cos, positions, grad_q_out, grad_k_out, eps=1e-5, axes=None):
     return (torch.empty_like(_in_place_rows(q)), torch.empty_like(_in_place_rows(k)),
             torch.empty_like(rmsnorm_weight, memory_format=torch.contiguous_format),
             torch.empty_like(scales, memory_format=torch.contiguous_format))
@@ -256,18 +343,18 @@ def _gqa_backward_fake(q, k, rmsnorm_weight, scales, sin, cos, positions, grad_q
 
 def _setup_context(ctx, inputs, output):
     ctx.save_for_backward(*inputs[:7])
-    ctx.eps = inputs[7]
+    ctx.eps, ctx.axes = inputs[7:]
 
 
 def _backward(ctx, grad_q, grad_k):
-    dq, dk, dw, ds = qknorm_rope_scale_gqa_backward_op(*ctx.saved_tensors, grad_q, grad_k, ctx.eps)
-    return dq, dk, dw, ds, None, None, None, None
+    dq, dk, dw, ds = qknorm_rope_scale_gqa_backward_op(*ctx.saved_tensors, grad_q, grad_k, ctx.eps, ctx.axes)
+    return dq, dk, dw, ds, None, None, None, None, None
 
 
 torch.library.register_autograd("flash_prologue::qknorm_rope_scale_gqa", _backward, setup_context=_setup_context)
 
 
-def qknorm_rope_scale_gqa(q, k, rmsnorm_weight, scales, sin, cos, positions=None, eps=1e-5):
+def qknorm_rope_scale_gqa(q, k, rmsnorm_weight, scales, sin, cos, positions=None, eps=1e-5, axes=None):
     """qknorm_rope_scale with Hq query heads on Hk key heads and a position per token.
 
     q/k: packed [T,Hq,D] / [T,Hk,D] or dense [B,Hq,N,D] / [B,Hk,N,D], BF16/FP16/FP32,
@@ -278,11 +365,16 @@ def qknorm_rope_scale_gqa(q, k, rmsnorm_weight, scales, sin, cos, positions=None
     the device error word. All arithmetic through the final cast is FP32. Differentiable
     in q, k, rmsnorm_weight and scales, once: second and forward-mode derivatives are refused.
     Outputs and gradients keep the inputs' memory order.
+
+    ``axes``: up to four positions a token ([axes,T], [axes,N] or [axes,B,N]), and axes[j], a
+    number in 0 .. 3, says which of them turns rotation pair j (channels j and j + D/2) of every
+    head; rotary_axes makes the usual patterns. A token with any of its positions outside the
+    tables gives NaN rows.
     """
     refuse_tangents("qknorm_rope_scale_gqa", q, k, rmsnorm_weight, scales, sin, cos)
     if eager(q, k, rmsnorm_weight, scales, sin, cos, positions):
         if not torch.is_grad_enabled() or not (q.requires_grad or k.requires_grad or rmsnorm_weight.requires_grad
                                                or scales.requires_grad):
-            return gqa_forward(q, k, rmsnorm_weight, scales, sin, cos, positions, eps)
-        return _GqaEager.apply(q, k, rmsnorm_weight, scales, sin, cos, positions, eps)
-    return torch.ops.flash_prologue.qknorm_rope_scale_gqa(q, k, rmsnorm_weight, scales, sin, cos, positions, eps)
+            return _forward(q, k, rmsnorm_weight, scales, sin, cos, positions, eps, axes)
+        return _GqaEager.apply(q, k, rmsnorm_weight, scales, sin, cos, positions, eps, axes)
+    return torch.ops.flash_prologue.qknorm_rope_scale_gqa(q, k, rmsnorm_weight, scales, sin, cos, positions, eps, axes)

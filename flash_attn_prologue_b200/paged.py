@@ -12,29 +12,35 @@ Nothing is read back from the GPU, so a step can be captured in a CUDA graph.
 """
 import ctypes
 import math
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple
 
 import torch
 from torch.autograd.graph import increment_version
 
 from . import _lib
 from .fused_epilogue import _DeviceGuard
-from .gqa import MAX_HEADS, call_library, check_rows, eager, flat_fp32, readable, refuse_tangents, rotation_of, rows_of
+from .gqa import (MAX_HEADS, axes_of, call_library, check_rows, eager, flat_fp32, readable, refuse_tangents, rotation_of,
+                  rows_of)
 
 
-def _checked_cache(q, heads, k_cache, v_cache, page_table, seq_lens, cu_seqlens):
+def checked_cache(q, heads, k_cache, v_cache, page_table, seq_lens, cu_seqlens, dtype=None):
     """flash_prologue_cache of the cache and its tables, once they fit the packed rows
-    q [T, H, D] with ``heads`` key heads."""
-    ks, dtype, device = k_cache.shape, q.dtype, q.device
-    if len(ks) != 4 or v_cache.shape != ks or ks[3] != q.shape[2]:
-        raise ValueError("caches must be matching [pages, page_size, Hk, D] tensors")
+    q [T, H, D] with ``heads`` key heads; dtype uint8: codes of 4 bits."""
+    ks, device = k_cache.shape, q.device
+    if dtype is None:
+        dtype, dim = q.dtype, q.shape[2]
+    else:
+        dim = q.shape[2] // 2
+    if len(ks) != 4 or v_cache.shape != ks or ks[3] != dim:
+        raise ValueError("caches must be matching [pages, page_size, Hk, D] tensors" if dtype is not torch.uint8
+                         else "caches must be matching [pages, page_size, Hk, D / 2] tensors")
     pages, page_size, kv_heads, _ = ks
     if page_size < 8 or page_size & (page_size - 1):
         raise ValueError("page_size must be a power of two, at least 8")
     if kv_heads != heads:
         raise ValueError("caches and rows must have the same key heads")
     if k_cache.dtype is not dtype or v_cache.dtype is not dtype:
-        raise ValueError("caches and rows must share a dtype")
+        raise ValueError("caches and rows must share a dtype" if dtype is not torch.uint8 else "caches must be uint8")
     a, b = k_cache.stride(), v_cache.stride()
     if a[3] != 1 or b[3] != 1:
         raise ValueError("caches must be contiguous along D")
@@ -66,7 +72,7 @@ def _checked_cache(q, heads, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
             page_table.data_ptr(), rows[0], width, seq_lens.data_ptr(), starts, batch)
 
 
-def _no_grad(name, *tensors):
+def no_grad(name, *tensors):
     refuse_tangents(name, *tensors)
     if torch.is_grad_enabled():
         for t in tensors:
@@ -74,22 +80,37 @@ def _no_grad(name, *tensors):
                 raise ValueError(f"{name} is not differentiable: call it under torch.no_grad()")
 
 
-def _append(q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache, page_table, seq_lens, cu_seqlens, eps):
+def append_args(q, k, v, rmsnorm_weight, scales, sin, cos, cache, q_out, eps):
+    """flash_prologue_append_args, and the tensors that have to live until the call."""
+    tokens, heads, dim = q.shape
+    w = None if rmsnorm_weight is None else flat_fp32(rmsnorm_weight)
+    s = None if scales is None else scales.contiguous()
+    return _lib.APPEND_ARGS.pack(
+        *rows_of(q), *rows_of(k), *rows_of(v), q_out.data_ptr(), 0, dim, heads * dim,
+        0 if w is None else w.data_ptr(), 0 if s is None else s.data_ptr(), *rotation_of(sin, cos), *cache, tokens,
+        heads, k.shape[1], dim, _lib.DTYPE_CODES[q.dtype], eps), (w, s)
+
+
+def check_step(q, k, v, rmsnorm_weight, scales, sin, cos, eps):
+    """The rows of a step's new tokens, and what turns and scales them."""
     if q.ndim != 3 or v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
         raise ValueError("q, k and v must be packed [T,Hq,D], [T,Hk,D], [T,Hk,D]")
     check_rows(q, k, rmsnorm_weight, scales, sin, cos, eps)
-    cache = _checked_cache(q, k.shape[1], k_cache, v_cache, page_table, seq_lens, cu_seqlens)
+
+
+def _append(q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache, page_table, seq_lens, cu_seqlens, eps,
+            positions=None, axes=None):
+    check_step(q, k, v, rmsnorm_weight, scales, sin, cos, eps)
+    cache = checked_cache(q, k.shape[1], k_cache, v_cache, page_table, seq_lens, cu_seqlens)
+    turn = None if positions is None and axes is None else axes_of(axes, positions, q, sin.shape[0])
     q, k, v = readable(q), readable(k), readable(v)
     q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    tokens, heads, dim = q.shape
-    if tokens:
-        w = None if rmsnorm_weight is None else flat_fp32(rmsnorm_weight)
-        s = None if scales is None else scales.contiguous()
-        args = _lib.APPEND_ARGS.pack(
-            *rows_of(q), *rows_of(k), *rows_of(v), q_out.data_ptr(), 0, dim, heads * dim,
-            0 if w is None else w.data_ptr(), 0 if s is None else s.data_ptr(), *rotation_of(sin, cos), *cache, tokens,
-            heads, k.shape[1], dim, _lib.DTYPE_CODES[q.dtype], eps)
-        call_library("flash_prologue_append_paged", args, q.device)
+    if q.shape[0]:
+        args, _alive = append_args(q, k, v, rmsnorm_weight, scales, sin, cos, cache, q_out, eps)
+        if turn is None:
+            call_library("flash_prologue_append_paged", args, q.device)
+        else:
+            call_library("flash_prologue_append_paged_axes", args, q.device, turn)
     return q_out
 
 
@@ -98,19 +119,21 @@ def append_paged_kv_op(
     q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rmsnorm_weight: Optional[torch.Tensor],
     scales: Optional[torch.Tensor], sin: torch.Tensor, cos: torch.Tensor, k_cache: torch.Tensor,
     v_cache: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
-    cu_seqlens: Optional[torch.Tensor] = None, eps: float = 1e-5,
+    cu_seqlens: Optional[torch.Tensor] = None, eps: float = 1e-5, positions: Optional[torch.Tensor] = None,
+    axes: Optional[Sequence[int]] = None,
 ) -> torch.Tensor:
-    return _append(q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache, page_table, seq_lens, cu_seqlens, eps)
+    return _append(q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache, page_table, seq_lens, cu_seqlens, eps,
+                   positions, axes)
 
 
 @append_paged_kv_op.register_fake
 def _append_fake(q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache, page_table, seq_lens,
-                 cu_seqlens=None, eps=1e-5):
+                 cu_seqlens=None, eps=1e-5, positions=None, axes=None):
     return torch.empty(q.shape, dtype=q.dtype, device=q.device)
 
 
 def append_paged_kv(q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache, page_table, seq_lens,
-                    cu_seqlens=None, eps=1e-5):
+                    cu_seqlens=None, eps=1e-5, positions=None, axes=None):
     """The prologue on a step's new tokens; K and V go to the cache, the Q rows come back.
 
     q [T,Hq,D], k and v [T,Hk,D] (views of one projection are read in place; BF16, FP16 or
@@ -118,16 +141,18 @@ def append_paged_kv(q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache,
     index among them, which is also where it is written: slot ``position % page_size`` of page
     ``page_table[request, position // page_size]``. rmsnorm_weight [2,1,D] or None (rotation
     only), scales [Hq,1,1] or None, sin/cos FP32 tables [positions, D/2] as in
-    qknorm_rope_scale_gqa. Tokens past the last request, or before the first where cu_seqlens
+    qknorm_rope_scale_gqa. ``positions`` [T] turns tokens by other positions than those they are
+    written at, and with ``axes`` (as in qknorm_rope_scale_gqa) positions are [axes,T].
+    Tokens past the last request, or before the first where cu_seqlens
     begin above 0, come back as zeros and are not written; so are tokens whose position, page or table row is out of range, which also set
     the device error word. Counts as an in-place change of both caches. Not differentiable:
     tensors that require gradients (where they are enabled) or carry tangents are refused.
     """
     args = (q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
-    _no_grad("append_paged_kv", q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache)
-    if not eager(*args):
-        return torch.ops.flash_prologue.append_paged_kv(*args, eps)
-    out = _append(*args, eps)
+    no_grad("append_paged_kv", q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_cache)
+    if not eager(*args, positions):
+        return torch.ops.flash_prologue.append_paged_kv(*args, eps, positions, axes)
+    out = _append(*args, eps, positions, axes)
     increment_version((k_cache, v_cache))  # as the registered op: autograd refuses what it saved of the caches before
     return out
 
@@ -146,7 +171,7 @@ def _workspace_bytes(dim, device):
     return int(out.value)
 
 
-def _aligned_rows(q, stride):
+def aligned_rows(q, stride):
     """q, or a copy whose rows start on 16 bytes and are contiguous along D."""
     if stride[2] == 1 and not (stride[0] | stride[1]) & 7 and not q.data_ptr() & 15:
         return q
@@ -163,7 +188,7 @@ def _attention(q, k_cache, v_cache, page_table, seq_lens, cu_seqlens, softmax_sc
     if dim not in ATTENTION_HEAD_DIMS:
         raise ValueError(f"head dimension must be one of {ATTENTION_HEAD_DIMS}")
     kv_heads = k_cache.shape[2] if k_cache.ndim == 4 else 0
-    cache = _checked_cache(q, kv_heads, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
+    cache = checked_cache(q, kv_heads, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
     if kv_heads <= 0 or heads <= 0 or heads % kv_heads or heads > MAX_HEADS:
         raise ValueError(f"query heads must be a multiple of the key heads and at most {MAX_HEADS}")
     if not -LARGEST_SCALE < softmax_scale < LARGEST_SCALE:
@@ -174,7 +199,7 @@ def _attention(q, k_cache, v_cache, page_table, seq_lens, cu_seqlens, softmax_sc
     if device.type != "cuda":
         raise ValueError("the attention kernels run on CUDA devices only")
     stride = q.stride()
-    q = _aligned_rows(q, stride)
+    q = aligned_rows(q, stride)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = q.new_empty((tokens, heads), dtype=torch.float32) if want_lse else None
     if tokens:
@@ -223,7 +248,7 @@ def paged_attention(q, k_cache, v_cache, page_table, seq_lens, cu_seqlens=None, 
     append_paged_kv.
     """
     tensors = (q, k_cache, v_cache, page_table, seq_lens, cu_seqlens)
-    _no_grad("paged_attention", q, k_cache, v_cache)
+    no_grad("paged_attention", q, k_cache, v_cache)
     call = _attention if eager(*tensors) else torch.ops.flash_prologue.paged_attention
     out, lse = call(*tensors, softmax_scale, window, return_lse)
     return (out, lse) if return_lse else out

@@ -579,6 +579,100 @@ FLASH_PROLOGUE_API int flash_prologue_selftest_attention_waits(const flash_prolo
 /* Bytes of workspace that cover every call with head dimension D on the current device. */
 FLASH_PROLOGUE_API int flash_prologue_paged_attention_workspace_size(int64_t D, size_t* bytes);
 
+/*
+ * ---------------------------------------------------------------------------
+ * Positions with several axes (time, height, width, ...): rotation pair j of a
+ * token (channels j and j + D / 2) is turned by row positions[axis of j][b, n]
+ * of the tables. `pairs` holds two bits a pair: pair j's axis in bits
+ * 2 * (j % 32) of word j / 32. A token with any of its `count` positions
+ * outside the tables is one whose position is out of range.
+ */
+typedef struct flash_prologue_axes {
+  const void* positions;                               /* [count, B, N] */
+  int64_t position_axis, position_b, position_n;       /* element strides */
+  int64_t position_bits;                               /* 32 or 64 */
+  int64_t count;                                       /* 1 .. 4; no pair names an axis beyond */
+  uint64_t pairs[4];
+} flash_prologue_axes;
+
+/* As the calls without axes, whose `positions` field these ignore. */
+FLASH_PROLOGUE_API int flash_prologue_gqa_fwd_axes(const flash_prologue_gqa_args* args, const flash_prologue_axes* axes,
+                                                   void* stream);
+FLASH_PROLOGUE_API int flash_prologue_gqa_bwd_axes(const flash_prologue_gqa_args* args, const flash_prologue_axes* axes,
+                                                   void* stream);
+/* Tokens are written where they belong in their request and turned by `axes` (B is 1, N the packed tokens). */
+FLASH_PROLOGUE_API int flash_prologue_append_paged_axes(const flash_prologue_append_args* args,
+                                                        const flash_prologue_axes* axes, void* stream);
+
+/*
+ * ---------------------------------------------------------------------------
+ * A paged cache held in 4 bits (D 64 or 128). A row's channels are in D / 32
+ * groups of 32: group g has the channels c with (c / 8) % (D / 32) == g. A group
+ * has a scale s, a BF16 number of at most five significant bits: -1/8 of the
+ * value of largest magnitude (of x and -x: x), cut towards zero. Channel c has
+ * the code clamp(rint(x / s), -8, 7) and stands for s * code, which is exact in
+ * BF16. For FP16 rows |s| is kept within 2^-20 .. 7936 (then s * code is exact in
+ * FP16 too), for BF16 rows at 2^-100 at least; a group of zeros has s = 0. A group
+ * that holds an infinity or NaN has a NaN scale: it stands for NaN.
+ * In memory: D / 2 bytes of codes, a 32-bit word for each 8 channels in order;
+ * in a word, codes + 8 of the even channels 0, 2, 4, 6 in bits 0, 4, 8, 12 and of
+ * the odd ones 1, 3, 5, 7 in bits 16, 20, 24, 28. Scales: D / 32 BF16, by group.
+ * In flash_prologue_cache `k` and `v` are the codes and the strides count bytes;
+ * they are multiples of 16 (codes are 16-byte aligned).
+ */
+typedef struct flash_prologue_scales {
+  void* k;
+  int64_t k_page, k_slot, k_head; /* element strides (BF16), multiples of D / 32; aligned to D / 16 bytes */
+  void* v;
+  int64_t v_page, v_slot, v_head;
+} flash_prologue_scales;
+
+/* flash_prologue_append_paged with K and V rounded to 4 bits (from FP32); BF16 or FP16 rows; axes may be NULL. */
+FLASH_PROLOGUE_API int flash_prologue_append_paged_int4(const flash_prologue_append_args* args,
+                                                        const flash_prologue_scales* scales,
+                                                        const flash_prologue_axes* axes, void* stream);
+/* What `rows` rows of codes and scales stand for, as BF16 or FP16 rows [rows, D]; all contiguous, 16-byte aligned. */
+FLASH_PROLOGUE_API int flash_prologue_unpack_int4(const void* codes, const void* scales, void* out, int64_t rows, int64_t D,
+                                                  int64_t dtype, void* stream);
+
+/*
+ * ---------------------------------------------------------------------------
+ * A step's page tables, lengths, positions and slots from its requests' lengths.
+ * Request r holds seq_lens[r] tokens and gets new_lens[r] more; below 0 it has
+ * ended: its pages (but the first keep[r]) go on top of the stack of free pages,
+ * request by request, and it is empty. Then requests take the pages that they
+ * grow by from the top of the stack, in order, into page_table. seq_lens_out are
+ * the lengths after the step, cu_seqlens the running sum of the new tokens,
+ * free_count_out the pages left on the stack. requests, positions, slots: of each
+ * of `tokens` packed new tokens its request, its position in it and page *
+ * page_size + slot; -1, 0 and -1 behind the last. Inputs other than page_table and
+ * free_pages stay as they are, and these may not overlap the outputs.
+ * Where pages run out the table's entries are -1 and the tokens' slots too; where
+ * the stack has no room returned pages are lost; a length that the table has no
+ * room for leaves slots of -1. All of these set bit 1 of the device error word,
+ * as do lengths out of range.
+ */
+typedef struct flash_prologue_plan_args {
+  int32_t* page_table;            /* [batch, max_pages], rows table_stride apart */
+  int64_t table_stride, max_pages;
+  const int32_t* seq_lens;        /* [batch] */
+  const int32_t* new_lens;        /* [batch] */
+  const int32_t* keep;            /* [batch] or NULL */
+  int32_t* free_pages;            /* [free_size] */
+  int64_t free_size;
+  const int32_t* free_count;      /* [1] */
+  int32_t* seq_lens_out;          /* [batch] */
+  int32_t* cu_seqlens;            /* [batch + 1] */
+  int32_t* free_count_out;        /* [1] */
+  int32_t* positions;             /* [tokens] */
+  int64_t* slots;                 /* [tokens] */
+  int32_t* requests;              /* [tokens] */
+  int64_t tokens, batch, page_size;
+} flash_prologue_plan_args;
+
+/* batch is at most 8192; page_size a power of two, at least 8. */
+FLASH_PROLOGUE_API int flash_prologue_plan_paged_step(const flash_prologue_plan_args* args, void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif
