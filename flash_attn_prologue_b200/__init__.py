@@ -32,6 +32,7 @@ _LAZY = {
     "paged_attention": ("paged", "paged_attention"),
     "rotary_axes": ("gqa", "rotary_axes"),
     "append_paged_kv_int4": ("int4", "append_paged_kv_int4"),
+    "paged_attention_int4": ("int4", "paged_attention_int4"),
     "unpack_int4": ("int4", "unpack_int4"),
     "int4_cache": ("int4", "int4_cache"),
     "plan_paged_step": ("plan", "plan_paged_step"),

@@ -279,7 +279,8 @@ FLASH_PROLOGUE_API int flash_prologue_device_error(int* value, int reset) {
   using Reader = cudaError_t (*)(int*, bool);
   const Reader readers[] = {read_device_error,         read_gemm_device_error,    read_gemm_bwd_device_error,
                             read_peer_device_error,    read_gqa_fwd_device_error, read_gqa_bwd_device_error,
-                            read_paged_decode_device_error, read_paged_prefill_device_error, read_paged_plan_device_error};
+                            read_paged_decode_device_error, read_paged_prefill_device_error, read_paged_plan_device_error,
+                            read_paged_int4_decode_device_error};
   int all = 0;
   for (Reader read : readers) {
     int word = 0;

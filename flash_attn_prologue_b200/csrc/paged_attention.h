@@ -83,5 +83,9 @@ PrefillPlan plan_paged_prefill(int64_t tokens, int64_t batch, bool ragged, int64
 bool launch_paged_prefill(const AttentionArgs& a, const PrefillPlan& plan, int dtype, int D, int64_t page_size,
                           long long wait_cycles, cudaStream_t stream, cudaError_t* err);
 cudaError_t launch_paged_decode(const AttentionArgs& a, int dtype, int D, cudaStream_t stream);
+// The same over a cache of 4 bits (a.k, a.v: codes, strides in bytes).
+size_t paged_int4_decode_workspace(int D, int sms);
+cudaError_t launch_paged_int4_decode(const AttentionArgs& a, const flash_prologue_scales& s, int dtype, int D,
+                                     cudaStream_t stream);
 
 }  // namespace flash_prologue

@@ -23,14 +23,14 @@ int device_sms() {
 // The factor of the scores' base-2 exponentials.
 double scale_log2_of(const flash_prologue_attention_args* a) { return a->softmax_scale * 1.4426950408889634; }
 
-int size_checks(const flash_prologue_attention_args* a) {
+int size_checks(const flash_prologue_attention_args* a, bool int4) {
   if (!a || a->tokens < 0 || a->window < 0 || !(fabs(scale_log2_of(a)) <= FLT_MAX) || a->Hq < 0 || a->Hk <= 0 ||
       a->Hq % a->Hk)
     return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
   if ((a->dtype != FLASH_PROLOGUE_BF16 && a->dtype != FLASH_PROLOGUE_FP16) || a->Hq > kMaxGqaHeads ||
       (a->D != 64 && a->D != 128) || a->tokens >= (int64_t(1) << 31) / kMaxGqaHeads)
     return FLASH_PROLOGUE_ERR_UNSUPPORTED;
-  return check_cache(a->cache, a->tokens, 2);
+  return check_cache(a->cache, a->tokens, int4 ? 1 : 2);
 }
 
 // Tiles of 128 rows on the tensor cores where the requests have more rows a key
@@ -43,15 +43,20 @@ bool use_prefill(const flash_prologue_attention_args* a, float scale_log2) {
   return a->tokens * group > 16 * a->cache.batch && group <= 128 && scale_log2 >= FLT_MIN;
 }
 
+size_t int4_workspace_of(int64_t D, int sms) { return paged_int4_decode_workspace((int)D, sms); }
+
 size_t workspace_of(int64_t D, int sms) {
   const size_t decode = paged_decode_workspace((int)D, sms), prefill = paged_prefill_workspace((int)D, sms);
   return prefill > decode ? prefill : decode;
 }
 
 // wait_cycles: 0, or the limit of the tiled kernel's waits (self-test), and no other kernel is taken.
-int attention(const flash_prologue_attention_args* a, int64_t wait_cycles, void* stream) {
-  const int st = size_checks(a);
+// scales: null, or the cache is one of 4 bits.
+int attention(const flash_prologue_attention_args* a, const flash_prologue_scales* scales, int64_t wait_cycles,
+              void* stream) {
+  int st = size_checks(a, scales != nullptr);
   if (st != FLASH_PROLOGUE_OK || a->tokens == 0 || a->Hq == 0) return st;
+  if (scales && (st = check_scales(*scales, a->cache, a->D)) != FLASH_PROLOGUE_OK) return st;
   const flash_prologue_cache& c = a->cache;
   if (!a->q.data || !a->out.data) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
   if ((reinterpret_cast<uintptr_t>(a->q.data) | reinterpret_cast<uintptr_t>(a->out.data)) & 15 ||
@@ -61,7 +66,7 @@ int attention(const flash_prologue_attention_args* a, int64_t wait_cycles, void*
   const int sms = device_sms();
   if (sms <= 0) return FLASH_PROLOGUE_ERR_CUDA;
   if (!a->workspace || (reinterpret_cast<uintptr_t>(a->workspace) & 15) ||
-      a->workspace_bytes < (int64_t)workspace_of(a->D, sms))
+      a->workspace_bytes < (int64_t)(scales ? int4_workspace_of(a->D, sms) : workspace_of(a->D, sms)))
     return FLASH_PROLOGUE_ERR_WORKSPACE;
   AttentionArgs g{};
   g.q = a->q.data;
@@ -88,6 +93,10 @@ int attention(const flash_prologue_attention_args* a, int64_t wait_cycles, void*
   g.workspace = a->workspace;
   g.max_keys = (int)(c.max_pages * c.page_size);
   g.window = a->window < g.max_keys ? (int)a->window : 0;  // as long as any request: all keys
+  if (scales)
+    return launch_paged_int4_decode(g, *scales, (int)a->dtype, (int)a->D, static_cast<cudaStream_t>(stream)) == cudaSuccess
+               ? FLASH_PROLOGUE_OK
+               : FLASH_PROLOGUE_ERR_CUDA;
   if (use_prefill(a, g.scale_log2)) {
     const PrefillPlan plan = plan_paged_prefill(a->tokens, c.batch, c.cu_seqlens != nullptr, a->Hk, g.group, (int)a->D,
                                                 g.max_keys, g.window, sms);
@@ -117,13 +126,28 @@ int flash_prologue_paged_attention_workspace_size(int64_t D, size_t* bytes) {
 }
 
 int flash_prologue_paged_attention(const flash_prologue_attention_args* a, void* stream) {
-  return attention(a, 0, stream);
+  return attention(a, nullptr, 0, stream);
+}
+
+int flash_prologue_paged_attention_int4_workspace_size(int64_t D, size_t* bytes) {
+  if (!bytes) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
+  *bytes = 0;
+  if (D != 64 && D != 128) return FLASH_PROLOGUE_ERR_UNSUPPORTED;
+  const int sms = device_sms();
+  if (sms <= 0) return FLASH_PROLOGUE_ERR_CUDA;
+  *bytes = int4_workspace_of(D, sms);
+  return FLASH_PROLOGUE_OK;
+}
+
+int flash_prologue_paged_attention_int4(const flash_prologue_attention_args* a, const flash_prologue_scales* scales,
+                                        void* stream) {
+  return scales ? attention(a, scales, 0, stream) : FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
 }
 
 int flash_prologue_selftest_attention_waits(const flash_prologue_attention_args* a, int64_t wait_cycles, void* stream) {
   if (!a || wait_cycles < 1 || wait_cycles > (int64_t(1) << 33)) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
   if (a->dtype != FLASH_PROLOGUE_BF16) return FLASH_PROLOGUE_ERR_UNSUPPORTED;
-  return attention(a, wait_cycles, stream);
+  return attention(a, nullptr, wait_cycles, stream);
 }
 
 }  // extern "C"

@@ -18,26 +18,13 @@
 // Scores, softmax statistics and outputs are FP32; the probabilities are
 // rounded to the cache's type for the second product (their sum is taken
 // before the rounding), an error of the size of the output's own rounding.
-#include "paged_attention.h"
+#include "paged_runs.cuh"
 
 namespace flash_prologue {
 namespace {
 
 constexpr int kRows = 16;       // rows of a tile
-constexpr int kWarpKeys = 16;   // keys of a warp's step
-constexpr int kDecodeWarps = 4;
-constexpr int kDecodeThreads = kDecodeWarps * 32;
-constexpr int kBlockKeys = kWarpKeys * kDecodeWarps;
-constexpr int kNone = -(1 << 30);  // below every relative position
-constexpr int kWholeKeys = 256; // longest caches whose items are never split
 constexpr int kRing = 3;        // steps of a warp's ring
-
-struct Part {  // an item that a CTA began and others go on with
-  int token0;  // packed index of its first row's request
-  int row0, rows;  // rows of the tile that exist
-  int kv_head;
-  int last;        // CTA that ends it; -1: nothing to join
-};
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
   const int bytes = ok ? 16 : 0;  // 0: zeros, src is not read
@@ -64,11 +51,6 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   if constexpr (std::is_same<T, __half>::value) {
@@ -90,71 +72,6 @@ __device__ __forceinline__ float to_float(T v) {
   if constexpr (std::is_same<T, __half>::value) return __half2float(v);
   else return __bfloat162float(v);
 }
-template <typename T>
-__device__ __forceinline__ T from_float(float v) {
-  if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
-  else return __float2bfloat16_rn(v);
-}
-
-// Blocks of keys from the first that the request's first new token sees to its last key.
-__device__ __forceinline__ int first_key(const Request& q, int window) {
-  return window ? max(q.total - q.news - window + 1, 0) : 0;
-}
-__device__ __forceinline__ int blocks_of(const Request& q, int window) {
-  const int lo = first_key(q, window) / kBlockKeys, hi = (q.total + kBlockKeys - 1) / kBlockKeys;
-  return max(hi - lo, 1);  // one at least: it writes the zeros of rows without keys
-}
-// Row tiles times key heads, each an item of blocks_of() blocks.
-__device__ __forceinline__ int64_t items_of(const Request& q, const AttentionArgs& a) {
-  return (int64_t)((q.news * a.group + kRows - 1) / kRows) * a.kv_heads;
-}
-// Units of an item: `cut` blocks at most in each.
-__device__ __forceinline__ int units_of_item(int blocks, int cut) {
-  return cut == 1 ? blocks : (blocks + cut - 1) / cut;
-}
-
-// Sums of two values over the CTA (every thread gets them).
-__device__ __forceinline__ void cta_sum(int64_t (&v)[2], int64_t (*scratch)[2]) {
-  if (__all_sync(0xffffffffu, (v[0] | v[1]) >> 24 == 0)) {
-    v[0] = __reduce_add_sync(0xffffffffu, (unsigned)v[0]);
-    v[1] = __reduce_add_sync(0xffffffffu, (unsigned)v[1]);
-  } else {
-#pragma unroll
-    for (int o = 16; o; o >>= 1)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
-  }
-  if ((threadIdx.x & 31) == 0) {
-    scratch[threadIdx.x >> 5][0] = v[0];
-    scratch[threadIdx.x >> 5][1] = v[1];
-  }
-  __syncthreads();
-  v[0] = v[1] = 0;
-#pragma unroll
-  for (int w = 0; w < kDecodeWarps; ++w) {
-    v[0] += scratch[w][0];
-    v[1] += scratch[w][1];
-  }
-}
-
-// Blocks of a unit. 1: every CTA takes an equal run of units, which may begin
-// and end inside items. Where a run crosses an item's border its CTA fills and
-// empties its pipeline twice; with fewer items than CTAs, items can be cut into
-// pieces of a CTA each instead, longer than the runs. Worth it up to about a
-// quarter more and 3 blocks: pieces (runs) of 6 requests x 8,192 keys, 32/8 x
-// 128: 39.7 (43.1) us; 16 x up to 6 tokens, 4,096 keys, 16/4 x 64: 17.6 (19.6);
-// not taken, pieces half as long again: 32 x 4,096 keys, 16/4 x 64: 27.4 (26.0).
-// (kAll: an item is a unit.)
-constexpr int kAll = 1 << 30;
-__device__ __forceinline__ int cut_of(const AttentionArgs& a, int64_t blocks, int64_t items) {
-  const int64_t grid = gridDim.x;
-  if (a.whole) return kAll;
-  if (blocks <= grid || items >= grid || blocks >= int64_t(1) << 30) return 1;
-  // The sum of ceil(b / cut) over the items is below blocks / cut + items <= grid.
-  const int cut = (int)(blocks + grid - items - 1) / (int)(grid - items), run = (int)blocks / (int)grid;
-  return cut <= run + run / 4 + 3 ? cut : 1;
-}
-
 template <typename T, int D>
 __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const AttentionArgs a) {
   constexpr int kRowBytes = D * 2;
@@ -162,120 +79,26 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
   constexpr int kPerLane = kWarpKeys * (D / 8) / 32;     // 16-byte pieces of K (and of V) a lane loads
   constexpr int kTiles = D / 8;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ int64_t scratch[kDecodeWarps], sums[kDecodeWarps][2];
-  __shared__ int64_t found[2];  // request of the CTA's next unit, units before it
+  __shared__ RunScratch shared;
   __shared__ float stat[kDecodeWarps][kRows][2];
   __shared__ int bad_page;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int batch = requests_of(a.pages);
   const uint32_t ring = smem_u32(smem) + warp * kRing * kStepBytes;
 
   if (!a.whole) start_next_kernel();
-  // This CTA's run of units.
-  int64_t total[2] = {0, 0}, my_items = 0;  // blocks and items of all requests; items of this thread's last one
-  int my_blocks = 0;
-  bool bad = false;
-  for (int r = threadIdx.x; r < batch; r += kDecodeThreads) {
-    bool b;
-    const Request q = request_at(a.pages, a.tokens, a.max_keys, r, &b);
-    bad |= b;
-    my_items = items_of(q, a);
-    my_blocks = blocks_of(q, a.window);
-    total[0] += my_items * my_blocks;
-    total[1] += my_items;
-  }
-  if (bad) atomicOr(&g_device_error, kDeviceErrorIndex);
-  if (threadIdx.x == 0) found[0] = -1;
-  cta_sum(total, sums);
-  const int cut = cut_of(a, total[0], total[1]);
-  const bool pieces = cut > 1 && !a.whole;  // a CTA has one unit
-  const int64_t units = a.whole ? total[1] : total[0];  // where CTAs have runs of them
   const int64_t slots = 2 * (int64_t)gridDim.x, cta = blockIdx.x;
   float* part_out = static_cast<float*>(a.workspace);                    // [slots][kRows][D]
   float* part_stat = part_out + slots * kRows * D;                       // [slots][kRows][2]
   Part* parts = reinterpret_cast<Part*>(part_stat + slots * kRows * 2);  // [grid]
-  if (threadIdx.x == 0 && !a.whole) parts[cta].last = -1;
-  const int64_t ctas = min((int64_t)gridDim.x, units);  // every one of these has a unit at least
-  if (cta >= ctas) return;
-  const bool small = units < (int64_t(1) << 31) / 1024;  // the products below fit 32 bits
-  const int64_t begin = pieces ? cta : small ? (int)cta * (int)units / (int)ctas : cta * units / ctas;
-  const int64_t end = pieces ? cta + 1 : small ? ((int)cta + 1) * (int)units / (int)ctas : (cta + 1) * units / ctas;
+  Run run;
+  if (!find_run<kRows>(a, shared, parts, run)) return;
 
-  // The request that `begin` falls into: one scan over the requests, a CTA's width at a time.
-  int64_t before = 0;
-  for (int r0 = 0; r0 < batch; r0 += kDecodeThreads) {
-    const int r = r0 + threadIdx.x;
-    int64_t n = my_items * units_of_item(my_blocks, cut);  // one request a thread: read already
-    if (batch > kDecodeThreads) {
-      n = 0;
-      if (r < batch) {
-        bool b;
-        const Request q = request_at(a.pages, a.tokens, a.max_keys, r, &b);
-        n = items_of(q, a) * units_of_item(blocks_of(q, a.window), cut);
-      }
-    }
-    int64_t upto = n;  // inclusive sum within the warp
-    if (small) {
-      int low = (int)n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, low, o);
-        if (lane >= o) low += v;
-      }
-      upto = low;
-    } else {
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += v;
-      }
-    }
-    __syncthreads();
-    if (lane == 31) scratch[warp] = upto;
-    __syncthreads();
-    int64_t start = before + upto - n, all = 0;
-#pragma unroll
-    for (int w = 0; w < kDecodeWarps; ++w) {
-      if (w < warp) start += scratch[w];
-      all += scratch[w];
-    }
-    if (begin >= start && begin < start + n) {
-      found[0] = r;
-      found[1] = start;
-    }
-    before += all;
-    if (before > begin) break;  // the same for every thread
-  }
-  __syncthreads();
-  if (found[0] < 0) return;  // fewer pieces than CTAs
-  int r = (int)found[0];
-  int64_t start = found[1];
-
-  for (int64_t unit = begin; unit < end;) {
-    bool too_long;  // more tokens than the page table has room for
-    Request q = request_at(a.pages, a.tokens, a.max_keys, r, &too_long);
-    int64_t in_request = items_of(q, a) * units_of_item(blocks_of(q, a.window), cut);
-    while (unit >= start + in_request) {
-      start += in_request;
-      ++r;
-      q = request_at(a.pages, a.tokens, a.max_keys, r, &too_long);
-      in_request = items_of(q, a) * units_of_item(blocks_of(q, a.window), cut);
-    }
-    const int blocks = blocks_of(q, a.window), per_item = units_of_item(blocks, cut);
-    const int size = cut == 1 ? 1 : (blocks + per_item - 1) / per_item;  // blocks of a unit, evenly
-    const int64_t in = unit - start;
-    const int item = in >> 31 ? (int)(in / per_item) : (int)in / per_item;  // tiles x heads stay below 2^31
-    const int64_t item_start = start + (int64_t)item * per_item;
-    const int u0 = (int)(unit - item_start), u1 = (int)min((int64_t)per_item, end - item_start);
-    const int b0 = u0 * size, b1 = min(u1 * size, blocks);
-    const int head = item % a.kv_heads;
-    const int row0 = item / a.kv_heads * kRows;       // of the request's news * group rows
-    const int rows = min(kRows, q.news * a.group - row0);
-    const int base = q.total - q.news;                // position of new token 0
-    const int key0 = first_key(q, a.window) / kBlockKeys * kBlockKeys;
-    // Keys that a row of this tile sees.
-    const int hi = base + (row0 + rows - 1) / a.group + 1;
-    const int lo = a.window ? max(base + row0 / a.group - a.window + 1, 0) : 0;
+  for (int64_t unit = run.begin; unit < run.end;) {
+    Item it;
+    find_item<kRows>(a, run, unit, it);
+    const Request& q = it.q;
+    const int b0 = it.b0, b1 = it.b1, blocks = it.blocks, head = it.head, row0 = it.row0, rows = it.rows, base = it.base,
+              key0 = it.key0, hi = it.hi, lo = it.lo;
 
     // The tile's Q as operand fragments: rows lane / 4 and lane / 4 + 8.
     uint32_t qf[D / 16][4];
@@ -298,7 +121,7 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
     for (int t = 0; t < kTiles; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[t][e] = 0.f;
-    if (threadIdx.x == 0) bad_page = too_long;
+    if (threadIdx.x == 0) bad_page = it.too_long;
     __syncthreads();
 
     // Positions relative to this warp's first key, in 32 bits (a request has fewer than 2^30 keys).
@@ -313,7 +136,7 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
       see_hi[e] = row_pos[e] < 0 ? kNone : row_pos[e] - warp_key;
       see_lo[e] = a.window ? row_pos[e] - a.window + 1 - warp_key : kNone;
     }
-    const int32_t* table = a.pages.page_table + (int64_t)r * a.pages.table_stride;
+    const int32_t* table = a.pages.page_table + (int64_t)it.r * a.pages.table_stride;
     const int in_page = (1 << a.pages.page_log2) - 1;
     // A lane's pieces of a step: rows lane / kPieces + i * kRowStep, 16 bytes at column lane % kPieces.
     constexpr int kPieces = D / 8, kRowStep = 32 / kPieces;
@@ -528,99 +351,10 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
         }
       }
     }
-    if (threadIdx.x == 0 && b0 == 0 && b1 < blocks) {
-      Part p;
-      p.token0 = q.first;
-      p.row0 = row0;
-      p.rows = rows;
-      p.kv_head = head;
-      p.last = (int)(pieces ? item_start + per_item - 1 : ((item_start + per_item) * ctas - 1) / units);
-      parts[cta] = p;
-    }
-    unit = item_start + u1;
+    if (threadIdx.x == 0 && b0 == 0 && b1 < blocks) parts[cta] = part_of(run, it);
+    unit = it.item_start + it.u1;
     __syncthreads();
   }
-}
-
-// Joins the parts of one row of the item that CTA blockIdx.x of the first kernel
-// began: every warp takes each eighth part, its columns over the lanes.
-constexpr int kJoinWarps = 8;
-template <typename T, int D>
-__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const AttentionArgs a, int64_t ctas) {
-  constexpr int kCols = D / 32;  // columns of a lane
-  __shared__ float joined[kJoinWarps][D], sums[kJoinWarps], tops[kJoinWarps];
-  const float* part_out = static_cast<const float*>(a.workspace);
-  const float* part_stat = part_out + 2 * ctas * kRows * D;
-  wait_for_previous_kernel();
-  const Part p = reinterpret_cast<const Part*>(part_stat + 2 * ctas * kRows * 2)[blockIdx.x];
-  const int row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (p.last < 0 || row >= p.rows) return;
-  const int first = blockIdx.x, parts = p.last - first + 1;
-  float top = -INFINITY, sum = 0.f, o[kCols] = {};
-  constexpr int kFlight = 4;
-  for (int i0 = warp; i0 < parts; i0 += kJoinWarps * kFlight) {
-    float2 st[kFlight];
-    float x[kFlight][kCols];
-#pragma unroll
-    for (int f = 0; f < kFlight; ++f) {
-      const int i = i0 + f * kJoinWarps;
-      st[f] = make_float2(-INFINITY, 0.f);
-#pragma unroll
-      for (int c = 0; c < kCols; ++c) x[f][c] = 0.f;
-      if (i < parts) {
-        // Part i is in the second slot of the CTA that began the item, in the first slot of the others.
-        const int64_t at = (2 * (int64_t)(first + i) + (i == 0)) * kRows + row;
-        st[f] = __ldcg(reinterpret_cast<const float2*>(part_stat + at * 2));
-        const float* src = part_out + at * D + lane * kCols;
-        if constexpr (kCols == 4) {
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
-          x[f][0] = v.x; x[f][1] = v.y; x[f][2] = v.z; x[f][3] = v.w;
-        } else {
-          const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
-          x[f][0] = v.x; x[f][1] = v.y;
-        }
-      }
-    }
-    float now = top;
-#pragma unroll
-    for (int f = 0; f < kFlight; ++f) now = fmaxf(now, st[f].x);
-    const float from = now == -INFINITY ? 0.f : now, moved = exp2_approx(top - from);
-    top = now;
-    sum *= moved;
-#pragma unroll
-    for (int c = 0; c < kCols; ++c) o[c] *= moved;
-#pragma unroll
-    for (int f = 0; f < kFlight; ++f) {
-      const float e = exp2_approx(st[f].x - from);
-      sum += e * st[f].y;
-#pragma unroll
-      for (int c = 0; c < kCols; ++c) o[c] += e * x[f][c];
-    }
-  }
-#pragma unroll
-  for (int c = 0; c < kCols; ++c) joined[warp][lane * kCols + c] = o[c];
-  if (lane == 0) {
-    sums[warp] = sum;
-    tops[warp] = top;
-  }
-  __syncthreads();
-  const int col = threadIdx.x;
-  if (col >= D) return;
-  float m = -INFINITY;
-#pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) m = fmaxf(m, tops[w]);
-  const float from = m == -INFINITY ? 0.f : m;
-  float v = 0.f, l = 0.f;
-#pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) {
-    const float e = exp2_approx(tops[w] - from);
-    v += e * joined[w][col];
-    l += e * sums[w];
-  }
-  const int at = p.row0 + row, token = at / a.group;
-  const int h = p.kv_head * a.group + (at - token * a.group);
-  static_cast<T*>(a.out)[(p.token0 + token) * a.out_n + h * a.out_h + col] = from_float<T>(l == 0.f ? 0.f : v / l);
-  if (a.lse && col == 0) a.lse[(int64_t)(p.token0 + token) * a.heads + h] = (m + log2f(l) - kProbabilityShift<T>) * 0.6931471805599453f;
 }
 
 int64_t most_ctas(int D, int sms) { return (int64_t)sms * (D == 64 ? 4 : 2); }
@@ -649,7 +383,7 @@ cudaError_t launch(AttentionArgs a, cudaStream_t stream) {
   err = launch_kernel(paged_decode_kernel<T, D>, dim3((unsigned)grid), dim3(kDecodeThreads), smem, stream, a);
   if (err != cudaSuccess || a.whole) return err;
   const unsigned rows = a.pages.cu_seqlens || a.group > kRows ? kRows : a.group;  // rows a tile can have
-  return launch_following(paged_join_kernel<T, D>, dim3((unsigned)grid, rows), dim3(kJoinWarps * 32), stream, a, grid);
+  return launch_following(paged_join_kernel<T, D, kRows, kProbabilityShift<T> != 0>, dim3((unsigned)grid, rows), dim3(kJoinWarps * 32), stream, a, grid);
 }
 
 }  // namespace

@@ -1,0 +1,556 @@
+// Attention of a few new tokens a request over a paged cache held in 4 bits:
+// o_i = sum_j p_ij v_j with p the softmax of the scaled scores over the keys that
+// row i sees, k and v the products s * (u - 8) of scales s and stored codes u.
+//
+// Bound by HBM in bytes (72 a row at D = 128), but each byte holds two values, so
+// the instructions that bring codes to the matrix units count as much. Few are
+// needed: the 16 bits u have the value u * 2^-24 as an FP16 number, and 16 u the
+// value u * 2^-20, so an AND takes two codes of a word (four bits each, 16 bits
+// apart) to an operand register, with no arithmetic at all. The powers of two go
+// into the other operand and the results; scales and the 8 come in afterwards,
+// exactly:
+//   S_ij = sum_g s_jg (sum_{c in g} q_ic u_jc - 8 sum_{c in g} q_ic)
+//   O_id = sum_j (p_ij s_jg) u_jd - 8 sum_j (p_ij s_jg),   g the group of d.
+// The first sums start at -8 sum q instead of 0; the last one is a matrix product
+// with a constant. Keys (then channels) are the 16 rows of the instructions and
+// query rows their 8 columns: a group of up to 8 query heads fills them with one
+// product where 16-row tiles of Q would leave half empty.
+//
+// Q is FP16 for the product, scaled by a power of two a row so that its largest
+// value is 2^14 to 2^15 (what falls below 2^-24 is 2^-39 of that). The weights
+// p s are rounded to FP16 once, scaled by 2^7 and the power of two sigma above the
+// largest scale that the row has seen, so that they are at most 2^15; an error of the size
+// of a 16-bit output's rounding. Scores, statistics and sums are FP32. The maximum
+// that scales a row of O moves only when the row's has grown by more than 2^8.
+//
+// Work is shared out as in paged_decode.cu (paged_runs.cuh): a warp takes 16 of a
+// block's 64 keys and loads them with cp.async into a ring of its own.
+#include "paged_runs.cuh"
+
+namespace flash_prologue {
+namespace {
+
+constexpr int kRing = 5;             // steps of a warp's ring
+constexpr int kCtasPerSm = 4;
+constexpr int kLeastScale = -80;     // least exponent of sigma: sums of 2^(15 + 80) stay inside FP32
+constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
+
+template <int BYTES>
+__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, bool ok) {
+  const int bytes = ok ? BYTES : 0;  // 0: zeros, src is not read
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+// d = a b + c of 16 x 16 and 16 x 8 FP16 fragments.
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1, float c0, float c1, float c2, float c3) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+               "{%10, %11, %12, %13};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t a) {  // of an 8 x 8 matrix of 16-bit values over the warp
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 floats_of(uint32_t half2) { return __half22float2(*reinterpret_cast<__half2*>(&half2)); }
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }  // -126 .. 127
+// The two BF16 numbers of a word.
+__device__ __forceinline__ float low_bf16(uint32_t x) { return __uint_as_float(x << 16); }
+__device__ __forceinline__ float high_bf16(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
+
+// A row's scales: G of them in G / 2 words.
+template <int G>
+struct Scales {
+  uint32_t w[G / 2];
+  __device__ __forceinline__ void load(uint32_t addr) {
+    if constexpr (G == 4) {
+      const uint2 v = lds64(addr);
+      w[0] = v.x;
+      w[1] = v.y;
+    } else {
+      w[0] = lds32(addr);
+    }
+  }
+  __device__ __forceinline__ float get(int g) const { return g & 1 ? high_bf16(w[g / 2]) : low_bf16(w[g / 2]); }
+};
+// G words of a row's piece.
+template <int G>
+__device__ __forceinline__ void load_words(uint32_t (&w)[G], uint32_t addr) {
+  if constexpr (G == 4) {
+    const uint4 v = lds128(addr);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  } else {
+    const uint2 v = lds64(addr);
+    w[0] = v.x; w[1] = v.y;
+  }
+}
+
+// A step's 16 keys of one row of codes each. Slot k of the products (rows of S, columns of
+// V^T) is key key_of(k): with it the 8 lanes (16 at D = 64) that read shared memory at once
+// find their pieces in different banks, both for K (4 pieces of neighbouring slots) and for
+// V (few pieces of every other slot), where pieces lie as at() says.
+__device__ __forceinline__ int key_of(int slot) { return slot ^ (slot >> 1 & 1); }
+template <int D>
+__device__ __forceinline__ int at(int key, int piece) {  // bytes; piece 0 .. 3 of a row
+  if constexpr (D == 128) return key * 64 + ((piece ^ (key >> 1 & 2)) * 16);
+  else return (key ^ (key >> 2 & 1)) * 32 + piece * 8;
+}
+
+template <int D>
+struct Step {
+  static constexpr int kCodes = kWarpKeys * D / 2, kScale = kWarpKeys * D / 16;
+  static constexpr int kV = kCodes, kKScale = 2 * kCodes, kVScale = 2 * kCodes + kScale, kBytes = 2 * (kCodes + kScale);
+};
+
+struct Int4Args {
+  AttentionArgs a;  // k, v: codes, strides in bytes
+  const uint16_t* k_scale;
+  const uint16_t* v_scale;
+  int64_t ks_page, ks_slot, ks_head, vs_page, vs_slot, vs_head;
+};
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kDecodeThreads) paged_int4_decode_kernel(const Int4Args args) {
+  const AttentionArgs& a = args.a;
+  constexpr int kRows = 8 * NT;
+  constexpr int G = D / 32;  // groups of channels; words of a piece
+  using S = Step<D>;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ RunScratch shared;
+  __shared__ float stat[kDecodeWarps][kRows][2];
+  __shared__ int bad_page;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t ring = smem_u32(smem) + warp * kRing * S::kBytes;
+
+  if (!a.whole) start_next_kernel();
+  const int64_t slots = 2 * (int64_t)gridDim.x, cta = blockIdx.x;
+  float* part_out = static_cast<float*>(a.workspace);                    // [slots][kRows][D]
+  float* part_stat = part_out + slots * kRows * D;                       // [slots][kRows][2]
+  Part* parts = reinterpret_cast<Part*>(part_stat + slots * kRows * 2);  // [grid]
+  Run run;
+  if (!find_run<kRows>(a, shared, parts, run)) return;
+
+  // This lane's places in the products. K: slots j and j + 8, piece p of the row. V: piece and
+  // half (even or odd channels) of the words, slots 2 p, 2 p + 1 and 8 more.
+  const int j = lane / 4, p = lane % 4;
+  const int k_at = at<D>(key_of(j), p);  // key + 8: kWarpKeys * D / 4 bytes on
+  const int v_at[2] = {at<D>(key_of(2 * p), j % 4), at<D>(key_of(2 * p + 1), j % 4)};
+  constexpr int kEight = kWarpKeys * D / 4;
+  const uint32_t half_of = j / 4 ? 0x7632u : 0x5410u;
+
+  for (int64_t unit = run.begin; unit < run.end;) {
+    Item it;
+    find_item<kRows>(a, run, unit, it);
+    const Request& q = it.q;
+    const int b0 = it.b0, b1 = it.b1, row0 = it.row0, rows = it.rows, base = it.base;
+
+    // Q: row 8 n + j of the tile, this lane's channels 8 (p G + g) .. + 7 of each group, times a power of two.
+    uint32_t qf[NT][G][4];
+    float start[NT][G][2];   // -8 sum of q over a group, of this lane's two columns 2 p and 2 p + 1
+    float row_scale[NT][2];  // takes their sums to base-2 scores
+    int see_hi[NT][2];       // last position that they see
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int row = 8 * n + j, of = row0 + row, i = of / a.group;
+      uint4 x[G];
+      float most = 0.f;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        x[g] = make_uint4(0, 0, 0, 0);
+        if (row < rows)
+          x[g] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (q.first + i) * a.q_n +
+                                                      (it.head * a.group + (of - i * a.group)) * a.q_h + 8 * (p * G + g)));
+        const T* v = reinterpret_cast<const T*>(&x[g]);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) most = fmaxf(most, fabsf((float)v[c]));
+      }
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      // The factor 2^(14 - exponent), in two steps: it may be beyond FP32's range.
+      const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -126), 127);
+      const float f0 = power_of_two((14 - e) / 2), f1 = power_of_two((14 - e) - (14 - e) / 2);
+      float sum[G];
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const T* v = reinterpret_cast<const T*>(&x[g]);
+        sum[g] = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float f2 = c & 1 ? 0.0625f : 1.f;  // beside codes of 16 u
+          qf[n][g][c] = half2_of((float)v[2 * c] * f0 * f1 * f2, (float)v[2 * c + 1] * f0 * f1 * f2);
+          const float2 got = floats_of(qf[n][g][c]);
+          sum[g] += (got.x + got.y) * (c & 1 ? 16.f : 1.f);
+        }
+        sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
+        sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int from = (2 * p + x) * 4;
+#pragma unroll
+        for (int g = 0; g < G; ++g) start[n][g][x] = -8.f * 0x1p-24f * __shfl_sync(0xffffffffu, sum[g], from);
+        // 2^24 of the codes, 2^(e - 14) of the row
+        const int up = __shfl_sync(0xffffffffu, e, from) + 10;
+        row_scale[n][x] = a.scale_log2 * power_of_two(up / 2) * power_of_two(up - up / 2);
+        const int at_row = 8 * n + 2 * p + x;
+        see_hi[n][x] = at_row < rows ? base + (row0 + at_row) / a.group : -1;
+      }
+    }
+    float acc[NT][G][2][4], eights[NT][G][4], top[NT][2], sum[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) acc[n][g][0][x] = acc[n][g][1][x] = eights[n][g][x] = 0.f;
+      top[n][0] = top[n][1] = -INFINITY;
+      sum[n][0] = sum[n][1] = 0.f;
+    }
+    int sigma[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) sigma[n][0] = sigma[n][1] = kLeastScale;
+    uint32_t limit = (uint32_t)(kLeastScale + 127) << 7;  // 2^(least sigma of the lane's columns) as a BF16 number
+    if (threadIdx.x == 0) bad_page = it.too_long;
+    __syncthreads();
+
+    // Positions relative to this warp's first key, in 32 bits (a request has fewer than 2^30 keys).
+    const int steps = b1 - b0;
+    const int warp_key = it.key0 + b0 * kBlockKeys + warp * kWarpKeys;
+    const int key_lo = it.lo - warp_key, key_hi = it.hi - warp_key;
+    const int all_lo = a.window ? base + (row0 + rows - 1) / a.group - a.window + 1 - warp_key : kNone;
+    const int all_hi = base + row0 / a.group - warp_key;  // every row sees keys all_lo .. all_hi
+    const int32_t* table = a.pages.page_table + (int64_t)it.r * a.pages.table_stride;
+    const int in_page = (1 << a.pages.page_log2) - 1;
+    int page_of[2] = {0, 0};  // pages of the 16 keys of step page_step + lane (two where pages hold 8)
+    int page_step = -32;
+    const auto load = [&](int step) {
+      if (step < steps) {
+        if (step - page_step >= 32) {
+          page_step = step;
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const int k = (step + lane) * kBlockKeys + s * 8;
+            page_of[s] = 0;
+            if (step + lane < steps && k < key_hi && k + 8 > key_lo) {
+              page_of[s] = __ldg(table + ((warp_key + k) >> a.pages.page_log2));
+              if (page_of[s] < 0 || page_of[s] >= a.pages.num_pages) {
+                page_of[s] = -1;
+                bad_page = 1;
+              }
+            }
+          }
+        }
+        const int page[2] = {__shfl_sync(0xffffffffu, page_of[0], step - page_step),
+                             __shfl_sync(0xffffffffu, page_of[1], step - page_step)};
+        const int key = step * kBlockKeys;
+        const uint32_t dst = ring + (step % kRing) * S::kBytes;
+        const int slot[2] = {(warp_key + key) & in_page, (warp_key + key + 8) & in_page};
+        // Codes of slots outside the tile's keys are whatever they are: their scales are zeros.
+        constexpr int kChunks = D / 32;  // 16 bytes of a row
+#pragma unroll
+        for (int i = 0; i < kChunks / 2; ++i) {
+          const int row = i * 32 / kChunks + lane / kChunks, chunk = lane % kChunks, s = row >> 3;
+          const int64_t there = page[s] >= 0 ? page[s] : 0, in = slot[s] + (row & 7);
+          // (a piece is half a chunk at D = 64)
+          const uint32_t to = dst + at<D>(row, chunk * (4 / kChunks));
+          cp_async16(to, static_cast<const unsigned char*>(a.k) + there * a.k_page + in * a.k_slot + it.head * a.k_head + chunk * 16,
+                     page[s] >= 0);
+          cp_async16(to + S::kV, static_cast<const unsigned char*>(a.v) + there * a.v_page + in * a.v_slot +
+                                     it.head * a.v_head + chunk * 16, page[s] >= 0);
+        }
+        const int row = lane & 15, s = row >> 3;
+        const bool ok = page[s] >= 0 && key + row >= key_lo && key + row < key_hi;
+        const int64_t there = page[s] >= 0 ? page[s] : 0, in = slot[s] + (row & 7);
+        const uint16_t* from = lane < 16 ? args.k_scale + there * args.ks_page + in * args.ks_slot + it.head * args.ks_head
+                                         : args.v_scale + there * args.vs_page + in * args.vs_slot + it.head * args.vs_head;
+        cp_async_small<D / 16>(dst + (lane < 16 ? S::kKScale : S::kVScale) + row * (D / 16), from, ok);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int s = 0; s < kRing - 1; ++s) load(s);
+
+    for (int step = 0; step < steps; ++step) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+      __syncwarp();
+      load(step + kRing - 1);
+      const int key = step * kBlockKeys;
+      if (key >= key_hi || key + kWarpKeys <= key_lo) continue;
+      const uint32_t here = ring + (step % kRing) * S::kBytes;
+
+      // Scores of keys key_of(j) and 8 more (x / 2), columns 2 p and 2 p + 1 (x % 2).
+      float s[NT][4] = {};
+      {
+        uint32_t wa[G], wb[G];
+        load_words<G>(wa, here + k_at);
+        load_words<G>(wb, here + k_at + kEight);
+        Scales<G> sa, sb;
+        sa.load(here + S::kKScale + key_of(j) * (D / 16));
+        sb.load(here + S::kKScale + (key_of(j) + 8) * (D / 16));
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const uint32_t ua = wa[g] >> 8, ub = wb[g] >> 8;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float c[4];
+            mma_f16(c, wa[g] & kLow, wb[g] & kLow, wa[g] & kHigh, wb[g] & kHigh, qf[n][g][0], qf[n][g][1], start[n][g][0],
+                    start[n][g][1], start[n][g][0], start[n][g][1]);
+            mma_f16(c, ua & kLow, ub & kLow, ua & kHigh, ub & kHigh, qf[n][g][2], qf[n][g][3], c[0], c[1], c[2], c[3]);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) s[n][x] += c[x] * (x < 2 ? sa.get(g) : sb.get(g));
+          }
+        }
+      }
+      const bool edge = key < all_lo || key + kWarpKeys - 1 > all_hi;  // some row does not see some key
+      bool move = false;
+      bool sees[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          s[n][x] *= row_scale[n][x & 1];
+          sees[n][x] = true;
+          if (edge) {
+            const int k = warp_key + key + key_of(j) + (x / 2) * 8, hi = see_hi[n][x & 1];
+            sees[n][x] = k <= hi && (!a.window || k > hi - a.window);
+            if (!sees[n][x]) s[n][x] = -INFINITY;
+          }
+          move |= s[n][x] > top[n][x & 1] + 8.f;
+        }
+      Scales<G> va, vb;
+      va.load(here + S::kVScale + key_of(j) * (D / 16));
+      vb.load(here + S::kVScale + (key_of(j) + 8) * (D / 16));
+      uint32_t largest = 0;  // magnitudes of the lane's V scales, as pairs of 16 bits
+#pragma unroll
+      for (int i = 0; i < G / 2; ++i)
+        largest = __vmaxu2(largest, __vmaxu2(va.w[i] & 0x7fff7fffu, vb.w[i] & 0x7fff7fffu));
+      move |= edge || (largest >> 16) >= limit || (largest & 0xffffu) >= limit;
+      if (__any_sync(0xffffffffu, move)) {
+        // A row's maximum or its largest scale may have moved: its O and sums follow. Each row goes by
+        // the keys that it sees, so what others see does not change its bits.
+        uint32_t size[2] = {0, 0};  // this lane's keys
+#pragma unroll
+        for (int i = 0; i < G / 2; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t x = va.w[i] >> 16 * h & 0x7fffu, y = vb.w[i] >> 16 * h & 0x7fffu;
+            if (x < 0x7f80u) size[0] = max(size[0], x);  // infinities and NaNs lose their own group only
+            if (y < 0x7f80u) size[1] = max(size[1], y);
+          }
+        int least = 127;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            float most = fmaxf(s[n][x], s[n][x + 2]);
+            uint32_t big = max(sees[n][x] ? size[0] : 0u, sees[n][x + 2] ? size[1] : 0u);
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+              most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+              big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+            }
+            const float was = top[n][x];
+            const int sigma_was = sigma[n][x];
+            if (most > was + 8.f) top[n][x] = most;
+            sigma[n][x] = min(max(sigma_was, (int)(big >> 7) - 126), 127);
+            least = min(least, sigma[n][x]);
+            const float f = top[n][x] == -INFINITY ? 1.f
+                                                   : exp2_approx(fmaxf(was - top[n][x], -300.f) + (float)(sigma_was - sigma[n][x]));
+            sum[n][x] *= f;
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                acc[n][g][0][2 * r + x] *= f;
+                acc[n][g][1][2 * r + x] *= f;
+                eights[n][g][2 * r + x] *= f;
+              }
+          }
+        limit = (uint32_t)(least + 127) << 7;
+      }
+      float w[NT][4];  // probabilities times 2^(7 - sigma)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const float from = top[n][x] == -INFINITY ? 0.f : top[n][x], up = (float)(7 - sigma[n][x]);
+          w[n][x] = exp2_approx((s[n][x] - from) + up);
+          w[n][x + 2] = exp2_approx((s[n][x + 2] - from) + up);
+          sum[n][x] += w[n][x] + w[n][x + 2];
+        }
+
+      // Channels of this lane: words j % 4 of the four keys, even or odd ones.
+      uint32_t w0[G], w1[G], w8[G], w9[G];
+      load_words<G>(w0, here + S::kV + v_at[0]);
+      load_words<G>(w1, here + S::kV + v_at[1]);
+      load_words<G>(w8, here + S::kV + v_at[0] + kEight);
+      load_words<G>(w9, here + S::kV + v_at[1] + kEight);
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const uint32_t x = __byte_perm(w0[g], w1[g], half_of), y = __byte_perm(w8[g], w9[g], half_of);
+        const uint32_t x8 = x >> 8, y8 = y >> 8;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float z[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            z[i] = w[n][i] * (i < 2 ? va.get(g) : vb.get(g));
+            if (edge && !sees[n][i]) z[i] = 0.f;  // whatever the scale is
+          }
+          const uint32_t w_lo = transposed(half2_of(z[0], z[1])), w_hi = transposed(half2_of(z[2], z[3]));
+          float (&o0)[4] = acc[n][g][0], (&o1)[4] = acc[n][g][1], (&e)[4] = eights[n][g];
+          mma_f16(o0, x & kLow, x & kHigh, y & kLow, y & kHigh, w_lo, w_hi, o0[0], o0[1], o0[2], o0[3]);
+          mma_f16(o1, x8 & kLow, x8 & kHigh, y8 & kLow, y8 & kHigh, w_lo, w_hi, o1[0], o1[1], o1[2], o1[3]);
+          mma_f16(e, 0x00080008u, 0x00800080u, 0x00080008u, 0x00800080u, w_lo, w_hi, e[0], e[1], e[2], e[3]);
+        }
+      }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+
+    // The four warps' sums over their keys, joined.
+    float* joined = reinterpret_cast<float*>(smem) + warp * kRows * D;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        float l = sum[n][x];
+        l += __shfl_xor_sync(0xffffffffu, l, 4);
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        const int row = 8 * n + 2 * p + x;
+        const float down = power_of_two(sigma[n][x] - 7);
+        if (j == 0) {
+          stat[warp][row][0] = top[n][x];
+          stat[warp][row][1] = l * down;
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int channel = 8 * (j % 4 * G + g) + 4 * t + j / 4;
+            joined[row * D + channel] = (acc[n][g][t][x] - eights[n][g][x]) * down * 0x1p24f;
+            joined[row * D + channel + 2] = (acc[n][g][t][2 + x] - eights[n][g][2 + x]) * down * 0x1p20f;
+          }
+      }
+    __syncthreads();
+    const bool whole = b0 == 0 && b1 == it.blocks;
+    const int64_t slot = 2 * cta + (b0 == 0 ? 1 : 0);
+    if (threadIdx.x == 0 && bad_page) atomicOr(&g_device_error, kDeviceErrorIndex);
+    for (int i = threadIdx.x; i < rows * D; i += kDecodeThreads) {
+      const int row = i / D, col = i % D;
+      float m = -INFINITY;
+#pragma unroll
+      for (int v = 0; v < kDecodeWarps; ++v) m = fmaxf(m, stat[v][row][0]);
+      const float from = m == -INFINITY ? 0.f : m;
+      float o = 0.f, l = 0.f;
+#pragma unroll
+      for (int v = 0; v < kDecodeWarps; ++v) {
+        const float f = exp2_approx(stat[v][row][0] - from);
+        o += f * reinterpret_cast<float*>(smem)[(v * kRows + row) * D + col];
+        l += f * stat[v][row][1];
+      }
+      if (bad_page) l = o = __int_as_float(0x7fc00000);
+      if (whole) {
+        const int of = row0 + row, token = of / a.group;
+        const int h = it.head * a.group + (of - token * a.group);
+        static_cast<T*>(a.out)[(q.first + token) * a.out_n + h * a.out_h + col] = from_float<T>(l == 0.f ? 0.f : o / l);
+        if (a.lse && col == 0) a.lse[(int64_t)(q.first + token) * a.heads + h] = (m + log2f(l)) * 0.6931471805599453f;
+      } else {
+        part_out[(slot * kRows + row) * D + col] = o;
+        if (col == 0) {
+          part_stat[(slot * kRows + row) * 2] = m;
+          part_stat[(slot * kRows + row) * 2 + 1] = l;
+        }
+      }
+    }
+    if (threadIdx.x == 0 && b0 == 0 && b1 < it.blocks) parts[cta] = part_of(run, it);
+    unit = it.item_start + it.u1;
+    __syncthreads();
+  }
+}
+
+template <typename T, int D, int NT>
+cudaError_t launch(Int4Args args, cudaStream_t stream) {
+  AttentionArgs& a = args.a;
+  constexpr int kRows = 8 * NT;
+  a.whole = a.max_keys <= kWholeKeys;
+  constexpr size_t ring = (size_t)kDecodeWarps * kRing * Step<D>::kBytes, joined = (size_t)kDecodeWarps * kRows * D * 4;
+  constexpr size_t smem = ring > joined ? ring : joined;
+  const void* fn = reinterpret_cast<const void*>(&paged_int4_decode_kernel<T, D, NT>);
+  cudaError_t err = allow_shared_memory(fn, smem);
+  if (err != cudaSuccess) return err;
+  // Never more CTAs than there can be units.
+  const int64_t tiles = (int64_t)a.tokens * a.group / kRows + (a.tokens < a.pages.batch + 2 ? a.tokens : a.pages.batch + 2);
+  const int64_t blocks = a.whole ? 1 : a.max_keys / kBlockKeys + 1;
+  int dev = 0, sms = 0;
+  if ((err = cudaGetDevice(&dev)) != cudaSuccess ||
+      (err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess)
+    return err;
+  const int64_t want = tiles * a.kv_heads * blocks, most = (int64_t)sms * kCtasPerSm;
+  const int64_t grid = persistent_grid(fn, smem, want < most ? want : most, kDecodeThreads);
+  if (grid <= 0) return cudaErrorInvalidConfiguration;
+  err = launch_kernel(paged_int4_decode_kernel<T, D, NT>, dim3((unsigned)grid), dim3(kDecodeThreads), smem, stream, args);
+  if (err != cudaSuccess || a.whole) return err;
+  const unsigned rows = a.pages.cu_seqlens || a.group > kRows ? kRows : a.group;  // rows a tile can have
+  return launch_following(paged_join_kernel<T, D, kRows, false>, dim3((unsigned)grid, rows), dim3(kJoinWarps * 32), stream, a,
+                          grid);
+}
+
+template <typename T, int D>
+cudaError_t launch_rows(const Int4Args& args, cudaStream_t stream) {
+  // Tiles of 8 rows where the requests have no more a key head on average, else of 16.
+  return (int64_t)args.a.tokens * args.a.group <= 8 * (int64_t)args.a.pages.batch ? launch<T, D, 1>(args, stream)
+                                                                                  : launch<T, D, 2>(args, stream);
+}
+
+}  // namespace
+
+size_t paged_int4_decode_workspace(int D, int sms) {
+  return (size_t)sms * kCtasPerSm * (2 * 16 * (size_t)(D + 2) * sizeof(float) + sizeof(Part));
+}
+
+cudaError_t launch_paged_int4_decode(const AttentionArgs& a, const flash_prologue_scales& s, int dtype, int D,
+                                     cudaStream_t stream) {
+  Int4Args args{};
+  args.a = a;
+  args.k_scale = static_cast<const uint16_t*>(s.k);
+  args.v_scale = static_cast<const uint16_t*>(s.v);
+  args.ks_page = s.k_page;
+  args.ks_slot = s.k_slot;
+  args.ks_head = s.k_head;
+  args.vs_page = s.v_page;
+  args.vs_slot = s.v_slot;
+  args.vs_head = s.v_head;
+  if (D == 64) return dtype == 0 ? launch_rows<__nv_bfloat16, 64>(args, stream) : launch_rows<__half, 64>(args, stream);
+  return dtype == 0 ? launch_rows<__nv_bfloat16, 128>(args, stream) : launch_rows<__half, 128>(args, stream);
+}
+
+cudaError_t read_paged_int4_decode_device_error(int* value, bool reset) {
+  cudaError_t err = cudaMemcpyFromSymbol(value, g_device_error, sizeof(int));
+  if (err != cudaSuccess || !reset) return err;
+  const int zero = 0;
+  return cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int));
+}
+
+}  // namespace flash_prologue

@@ -199,6 +199,7 @@ cudaError_t read_gqa_bwd_device_error(int* value, bool reset);
 cudaError_t read_paged_decode_device_error(int* value, bool reset);
 cudaError_t read_paged_prefill_device_error(int* value, bool reset);
 cudaError_t read_paged_plan_device_error(int* value, bool reset);
+cudaError_t read_paged_int4_decode_device_error(int* value, bool reset);
 // One thread waits (bounded by `tries` polls) on a barrier nothing arrives at.
 cudaError_t launch_selftest_wait_timeout(uint32_t tries, cudaStream_t stream);
 int64_t tma_grid(bool bwd, const TmaPlan& p, int H, int D, int dtype, bool inv = false);

@@ -1,5 +1,6 @@
-"""A paged cache held in 4 bits: the prologue that writes it (``append_paged_kv_int4``) and what
-it stands for (``unpack_int4``). The reference has no cache.
+"""A paged cache held in 4 bits: the prologue that writes it (``append_paged_kv_int4``), the
+attention that reads it (``paged_attention_int4``) and what it stands for (``unpack_int4``).
+The reference has no cache.
 
 A cache is four tensors (``int4_cache`` makes them): codes ``[pages, page_size, Hk, D/2]`` uint8
 and scales ``[pages, page_size, Hk, D/32]`` bfloat16 of K and of V, 72 bytes a row at D = 128
@@ -7,15 +8,16 @@ instead of 256. Pages, tables and lengths are those of flash_attn_prologue_b200.
 channels are in D/32 groups of 32 (channel c in group (c // 8) % (D/32)), each with a scale s of
 five significant bits; a channel is rounded to s times a whole number from -8 to 7.
 """
-from typing import Optional, Sequence
+import ctypes
+from typing import Optional, Sequence, Tuple
 
 import torch
 from torch.autograd.graph import increment_version
 
 from . import _lib
 from .fused_epilogue import _DeviceGuard
-from .gqa import axes_of, call_library, eager, readable, refuse_tangents
-from .paged import ATTENTION_HEAD_DIMS, append_args, check_step, checked_cache, no_grad
+from .gqa import MAX_HEADS, axes_of, call_library, eager, readable, refuse_tangents
+from .paged import ATTENTION_HEAD_DIMS, LARGEST_SCALE, aligned_rows, append_args, check_step, checked_cache, no_grad
 
 
 def int4_cache(pages, page_size, kv_heads, dim, device="cuda"):
@@ -102,6 +104,81 @@ def append_paged_kv_int4(q, k, v, rmsnorm_weight, scales, sin, cos, k_cache, v_c
     out = _append(*args, eps, positions, axes)
     increment_version((k_cache, v_cache, k_scale, v_scale))
     return out
+
+
+_WORKSPACE_BYTES = {}
+
+
+def _workspace_bytes(dim, device):
+    out = ctypes.c_size_t(0)
+    with _DeviceGuard(device):
+        _lib.check(_lib.load().flash_prologue_paged_attention_int4_workspace_size(dim, ctypes.byref(out)),
+                   "flash_prologue_paged_attention_int4_workspace_size")
+    _WORKSPACE_BYTES[dim, device.index] = int(out.value)
+    return int(out.value)
+
+
+def _attention(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, cu_seqlens, softmax_scale, window, want_lse):
+    _check_rows(q)
+    tokens, heads, dim = q.shape
+    kv_heads = k_cache.shape[2] if k_cache.ndim == 4 else 0
+    cache = checked_cache(q, kv_heads, k_cache, v_cache, page_table, seq_lens, cu_seqlens, torch.uint8)
+    scale_args = _checked_scales(k_cache, k_scale, v_scale, dim)
+    if kv_heads <= 0 or heads <= 0 or heads % kv_heads or heads > MAX_HEADS:
+        raise ValueError(f"query heads must be a multiple of the key heads and at most {MAX_HEADS}")
+    if not -LARGEST_SCALE < softmax_scale < LARGEST_SCALE:
+        raise ValueError("softmax_scale must be finite, and in FP32 too")
+    if window < 0:
+        raise ValueError("window must be 0 (all keys) or positive")
+    device = q.device
+    if device.type != "cuda":
+        raise ValueError("the attention kernels run on CUDA devices only")
+    q = aligned_rows(q, q.stride())
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = q.new_empty((tokens, heads), dtype=torch.float32) if want_lse else None
+    if tokens:
+        stride = q.stride()
+        nbytes = _WORKSPACE_BYTES.get((dim, device.index)) or _workspace_bytes(dim, device)
+        workspace = q.new_empty((nbytes + 1) // 2)
+        args = _lib.ATTENTION_ARGS.pack(
+            q.data_ptr(), 0, stride[1], stride[0], out.data_ptr(), 0, dim, heads * dim,
+            lse.data_ptr() if want_lse else 0, *cache, workspace.data_ptr(), nbytes, tokens, heads, kv_heads, dim,
+            _lib.DTYPE_CODES[q.dtype], window, softmax_scale)
+        call_library("flash_prologue_paged_attention_int4", args, device, scale_args)
+    return out, lse
+
+
+@torch.library.custom_op("flash_prologue::paged_attention_int4", mutates_args=())
+def paged_attention_int4_op(
+    q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+    page_table: torch.Tensor, seq_lens: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None,
+    softmax_scale: float = 1.0, window: int = 0, want_lse: bool = False,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    refuse_tangents("paged_attention_int4", q, k_scale, v_scale)
+    out, lse = _attention(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, cu_seqlens, softmax_scale, window,
+                          want_lse)
+    return out, q.new_empty(0, dtype=torch.float32) if lse is None else lse
+
+
+@paged_attention_int4_op.register_fake
+def _attention_fake(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, cu_seqlens=None, softmax_scale=1.0,
+                    window=0, want_lse=False):
+    return (torch.empty(q.shape, dtype=q.dtype, device=q.device),
+            torch.empty(q.shape[:2] if want_lse else (0,), dtype=torch.float32, device=q.device))
+
+
+def paged_attention_int4(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, cu_seqlens=None, *,
+                         softmax_scale=1.0, window=0, return_lse=False):
+    """paged_attention over a cache held in 4 bits, with the exact values that it stands for.
+
+    Arguments, masks, windows, rows without keys, indices out of range and derivatives as in
+    paged_attention. A scale that is NaN makes the rows that see its slot NaN, and no others.
+    """
+    tensors = (q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, cu_seqlens)
+    no_grad("paged_attention_int4", q, k_scale, v_scale)
+    call = _attention if eager(*tensors) else torch.ops.flash_prologue.paged_attention_int4
+    out, lse = call(*tensors, softmax_scale, window, return_lse)
+    return (out, lse) if return_lse else out
 
 
 def _unpack(cache, scale, dtype):

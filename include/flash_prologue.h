@@ -631,6 +631,11 @@ typedef struct flash_prologue_scales {
 FLASH_PROLOGUE_API int flash_prologue_append_paged_int4(const flash_prologue_append_args* args,
                                                         const flash_prologue_scales* scales,
                                                         const flash_prologue_axes* axes, void* stream);
+/* flash_prologue_paged_attention over such a cache. */
+FLASH_PROLOGUE_API int flash_prologue_paged_attention_int4(const flash_prologue_attention_args* args,
+                                                           const flash_prologue_scales* scales, void* stream);
+/* Bytes of workspace that cover every call of it with head dimension D on the current device. */
+FLASH_PROLOGUE_API int flash_prologue_paged_attention_int4_workspace_size(int64_t D, size_t* bytes);
 /* What `rows` rows of codes and scales stand for, as BF16 or FP16 rows [rows, D]; all contiguous, 16-byte aligned. */
 FLASH_PROLOGUE_API int flash_prologue_unpack_int4(const void* codes, const void* scales, void* out, int64_t rows, int64_t D,
                                                   int64_t dtype, void* stream);
