@@ -24,6 +24,8 @@ namespace flash_prologue {
 namespace {
 
 constexpr int kRows = 16;       // rows of a tile
+constexpr int kBlockKeys = kWarpKeys * kDecodeWarps;
+using Tiles = Tiling<kRows, kBlockKeys, 1>;
 constexpr int kRing = 3;        // steps of a warp's ring
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
@@ -91,11 +93,11 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_decode_kernel(const Atte
   float* part_stat = part_out + slots * kRows * D;                       // [slots][kRows][2]
   Part* parts = reinterpret_cast<Part*>(part_stat + slots * kRows * 2);  // [grid]
   Run run;
-  if (!find_run<kRows>(a, shared, parts, run)) return;
+  if (!find_run<Tiles>(a, shared, parts, run)) return;
 
   for (int64_t unit = run.begin; unit < run.end;) {
     Item it;
-    find_item<kRows>(a, run, unit, it);
+    find_item<Tiles>(a, run, unit, it);
     const Request& q = it.q;
     const int b0 = it.b0, b1 = it.b1, blocks = it.blocks, head = it.head, row0 = it.row0, rows = it.rows, base = it.base,
               key0 = it.key0, hi = it.hi, lo = it.lo;

@@ -23,16 +23,19 @@
 // of a 16-bit output's rounding. Scores, statistics and sums are FP32. The maximum
 // that scales a row of O moves only when the row's has grown by more than 2^8.
 //
-// Work is shared out as in paged_decode.cu (paged_runs.cuh): a warp takes 16 of a
-// block's 64 keys and loads them with cp.async into a ring of its own.
+// Work is shared out as in paged_decode.cu (paged_runs.cuh). A warp takes 16 keys of
+// one key head a step and loads them with cp.async into a ring of its own; a CTA's
+// four warps take neighbouring heads of the same keys where there are such, since
+// their rows lie next to each other.
 #include "paged_runs.cuh"
 
 namespace flash_prologue {
 namespace {
 
-constexpr int kRing = 5;             // steps of a warp's ring
+constexpr int kRing = 4;             // steps of a warp's ring
 constexpr int kCtasPerSm = 4;
 constexpr int kLeastScale = -80;     // least exponent of sigma: sums of 2^(15 + 80) stay inside FP32
+constexpr float kNoTop = -3e38f;      // the maximum of a row that has seen no key
 constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
 
 template <int BYTES>
@@ -129,11 +132,13 @@ struct Int4Args {
   int64_t ks_page, ks_slot, ks_head, vs_page, vs_slot, vs_head;
 };
 
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kDecodeThreads) paged_int4_decode_kernel(const Int4Args args) {
+// NT tiles of 8 rows; HEADS key heads a CTA, so 4 / HEADS warps share a head's keys.
+template <typename T, int D, int NT, int HEADS>
+__global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 128 ? 3 : 4 : 2) paged_int4_decode_kernel(const Int4Args args) {
   const AttentionArgs& a = args.a;
-  constexpr int kRows = 8 * NT;
+  constexpr int kRows = 8 * NT, kSplit = kDecodeWarps / HEADS, kBlockKeys = kWarpKeys * kSplit;
   constexpr int G = D / 32;  // groups of channels; words of a piece
+  using Tiles = Tiling<kRows, kBlockKeys, HEADS>;
   using S = Step<D>;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ RunScratch shared;
@@ -144,25 +149,36 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_int4_decode_kernel(const
 
   if (!a.whole) start_next_kernel();
   const int64_t slots = 2 * (int64_t)gridDim.x, cta = blockIdx.x;
-  float* part_out = static_cast<float*>(a.workspace);                    // [slots][kRows][D]
-  float* part_stat = part_out + slots * kRows * D;                       // [slots][kRows][2]
-  Part* parts = reinterpret_cast<Part*>(part_stat + slots * kRows * 2);  // [grid]
+  float* part_out = static_cast<float*>(a.workspace);                            // [slots][HEADS][kRows][D]
+  float* part_stat = part_out + slots * HEADS * kRows * D;                       // [slots][HEADS][kRows][2]
+  Part* parts = reinterpret_cast<Part*>(part_stat + slots * HEADS * kRows * 2);  // [grid]
   Run run;
-  if (!find_run<kRows>(a, shared, parts, run)) return;
+  if (!find_run<Tiles>(a, shared, parts, run)) return;
 
   // This lane's places in the products. K: slots j and j + 8, piece p of the row. V: piece and
   // half (even or odd channels) of the words, slots 2 p, 2 p + 1 and 8 more.
   const int j = lane / 4, p = lane % 4;
-  const int k_at = at<D>(key_of(j), p);  // key + 8: kWarpKeys * D / 4 bytes on
-  const int v_at[2] = {at<D>(key_of(2 * p), j % 4), at<D>(key_of(2 * p + 1), j % 4)};
+  const uint32_t k_at = at<D>(key_of(j), p);  // key + 8: kWarpKeys * D / 4 bytes on
+  const uint32_t v_at[2] = {(uint32_t)at<D>(key_of(2 * p), j % 4) + S::kV, (uint32_t)at<D>(key_of(2 * p + 1), j % 4) + S::kV};
+  const uint32_t scale_at = S::kKScale + key_of(j) * (D / 16);
   constexpr int kEight = kWarpKeys * D / 4;
   const uint32_t half_of = j / 4 ? 0x7632u : 0x5410u;
+  // Its places in the loads: a 16-byte chunk of K and of V in each pass over a step's rows, a row's
+  // scales of K (lanes 0 .. 15) or V.
+  constexpr int kChunks = D / 32, kPasses = kChunks / 2;
+  const int load_row = lane / kChunks, chunk = lane % kChunks;
+  const uint32_t load_at = at<D>(load_row, chunk * (4 / kChunks));  // (a piece is half a chunk at D = 64)
+  const uint32_t scale_to = (lane < 16 ? S::kKScale : S::kVScale) + (lane & 15) * (D / 16);
+  const bool wide = a.pages.page_log2 >= 4;  // a step's keys are in one page
+  const int in_page = (1 << a.pages.page_log2) - 1;
 
   for (int64_t unit = run.begin; unit < run.end;) {
     Item it;
-    find_item<kRows>(a, run, unit, it);
+    find_item<Tiles>(a, run, unit, it);
     const Request& q = it.q;
     const int b0 = it.b0, b1 = it.b1, row0 = it.row0, rows = it.rows, base = it.base;
+    const int head = it.head + warp % HEADS;
+    const bool idle = HEADS > 1 && head >= a.kv_heads;
 
     // Q: row 8 n + j of the tile, this lane's channels 8 (p G + g) .. + 7 of each group, times a power of two.
     uint32_t qf[NT][G][4];
@@ -177,9 +193,9 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_int4_decode_kernel(const
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         x[g] = make_uint4(0, 0, 0, 0);
-        if (row < rows)
+        if (row < rows && !idle)
           x[g] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (q.first + i) * a.q_n +
-                                                      (it.head * a.group + (of - i * a.group)) * a.q_h + 8 * (p * G + g)));
+                                                      (head * a.group + (of - i * a.group)) * a.q_h + 8 * (p * G + g)));
         const T* v = reinterpret_cast<const T*>(&x[g]);
 #pragma unroll
         for (int c = 0; c < 8; ++c) most = fmaxf(most, fabsf((float)v[c]));
@@ -216,32 +232,40 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_int4_decode_kernel(const
         see_hi[n][x] = at_row < rows ? base + (row0 + at_row) / a.group : -1;
       }
     }
-    float acc[NT][G][2][4], eights[NT][G][4], top[NT][2], sum[NT][2];
+    // Of a column: probabilities are 2^(score - from), from = top + sigma - 7 (whole numbers: no
+    // rounding); `over` is what they reach 2^8 above top, `limit` 2^(least sigma).
+    float acc[NT][G][2][4], eights[NT][G][4], top[NT][2], from[NT][2], over[NT][2], sum[NT][2], limit = power_of_two(kLeastScale);
+    int sigma[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int g = 0; g < G; ++g)
 #pragma unroll
         for (int x = 0; x < 4; ++x) acc[n][g][0][x] = acc[n][g][1][x] = eights[n][g][x] = 0.f;
-      top[n][0] = top[n][1] = -INFINITY;
-      sum[n][0] = sum[n][1] = 0.f;
-    }
-    int sigma[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) sigma[n][0] = sigma[n][1] = kLeastScale;
-    uint32_t limit = (uint32_t)(kLeastScale + 127) << 7;  // 2^(least sigma of the lane's columns) as a BF16 number
+      for (int x = 0; x < 2; ++x) {
+        top[n][x] = from[n][x] = kNoTop;
+        over[n][x] = 0.f;
+        sum[n][x] = 0.f;
+        sigma[n][x] = kLeastScale;
+      }
+    }
     if (threadIdx.x == 0) bad_page = it.too_long;
     __syncthreads();
 
     // Positions relative to this warp's first key, in 32 bits (a request has fewer than 2^30 keys).
-    const int steps = b1 - b0;
-    const int warp_key = it.key0 + b0 * kBlockKeys + warp * kWarpKeys;
+    const int steps = idle ? 0 : b1 - b0;
+    const int warp_key = it.key0 + b0 * kBlockKeys + warp / HEADS * kWarpKeys;
     const int key_lo = it.lo - warp_key, key_hi = it.hi - warp_key;
     const int all_lo = a.window ? base + (row0 + rows - 1) / a.group - a.window + 1 - warp_key : kNone;
     const int all_hi = base + row0 / a.group - warp_key;  // every row sees keys all_lo .. all_hi
     const int32_t* table = a.pages.page_table + (int64_t)it.r * a.pages.table_stride;
-    const int in_page = (1 << a.pages.page_log2) - 1;
-    int page_of[2] = {0, 0};  // pages of the 16 keys of step page_step + lane (two where pages hold 8)
+    const unsigned char* k_lane = static_cast<const unsigned char*>(a.k) + head * a.k_head + (load_row & 7) * a.k_slot + chunk * 16;
+    const unsigned char* v_lane = static_cast<const unsigned char*>(a.v) + head * a.v_head + (load_row & 7) * a.v_slot + chunk * 16;
+    const uint16_t* s_lane = lane < 16 ? args.k_scale + head * args.ks_head + (lane & 7) * args.ks_slot
+                                       : args.v_scale + head * args.vs_head + (lane & 7) * args.vs_slot;
+    const int64_t s_page = lane < 16 ? args.ks_page : args.vs_page, s_slot = lane < 16 ? args.ks_slot : args.vs_slot;
+    int page_of[2] = {0, 0};  // page of the keys of step page_step + lane (pages of 8 slots: of either half)
     int page_step = -32;
     const auto load = [&](int step) {
       if (step < steps) {
@@ -251,7 +275,7 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_int4_decode_kernel(const
           for (int s = 0; s < 2; ++s) {
             const int k = (step + lane) * kBlockKeys + s * 8;
             page_of[s] = 0;
-            if (step + lane < steps && k < key_hi && k + 8 > key_lo) {
+            if (step + lane < steps && k < key_hi && k + (wide ? 16 : 8) > key_lo) {
               page_of[s] = __ldg(table + ((warp_key + k) >> a.pages.page_log2));
               if (page_of[s] < 0 || page_of[s] >= a.pages.num_pages) {
                 page_of[s] = -1;
@@ -260,56 +284,60 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_int4_decode_kernel(const
             }
           }
         }
-        const int page[2] = {__shfl_sync(0xffffffffu, page_of[0], step - page_step),
-                             __shfl_sync(0xffffffffu, page_of[1], step - page_step)};
         const int key = step * kBlockKeys;
-        const uint32_t dst = ring + (step % kRing) * S::kBytes;
-        const int slot[2] = {(warp_key + key) & in_page, (warp_key + key + 8) & in_page};
+        const uint32_t dst = ring + step % kRing * S::kBytes;
+        const int page0 = __shfl_sync(0xffffffffu, page_of[0], step - page_step), slot0 = (warp_key + key) & in_page;
         // Codes of slots outside the tile's keys are whatever they are: their scales are zeros.
-        constexpr int kChunks = D / 32;  // 16 bytes of a row
+        const int row = lane & 15;
+        if (wide && page0 >= 0) {
+          const unsigned char* k = k_lane + page0 * a.k_page + slot0 * a.k_slot;
+          const unsigned char* v = v_lane + page0 * a.v_page + slot0 * a.v_slot;
+          if constexpr (kPasses == 1) {
+            if (load_row >= 8) {
+              k += 8 * a.k_slot;
+              v += 8 * a.v_slot;
+            }
+          }
 #pragma unroll
-        for (int i = 0; i < kChunks / 2; ++i) {
-          const int row = i * 32 / kChunks + lane / kChunks, chunk = lane % kChunks, s = row >> 3;
-          const int64_t there = page[s] >= 0 ? page[s] : 0, in = slot[s] + (row & 7);
-          // (a piece is half a chunk at D = 64)
-          const uint32_t to = dst + at<D>(row, chunk * (4 / kChunks));
-          cp_async16(to, static_cast<const unsigned char*>(a.k) + there * a.k_page + in * a.k_slot + it.head * a.k_head + chunk * 16,
-                     page[s] >= 0);
-          cp_async16(to + S::kV, static_cast<const unsigned char*>(a.v) + there * a.v_page + in * a.v_slot +
-                                     it.head * a.v_head + chunk * 16, page[s] >= 0);
+          for (int i = 0; i < kPasses; ++i) {
+            cp_async16(dst + load_at + i * kEight, k + i * (8 * a.k_slot), true);
+            cp_async16(dst + load_at + S::kV + i * kEight, v + i * (8 * a.v_slot), true);
+          }
+          const bool ok = key + row >= key_lo && key + row < key_hi;
+          cp_async_small<D / 16>(dst + scale_to, s_lane + page0 * s_page + (slot0 + (row & 8)) * s_slot, ok);
+        } else {
+          // Pages of 8 slots, or one that is outside the cache.
+          const int page1 = __shfl_sync(0xffffffffu, page_of[1], step - page_step), slot1 = (warp_key + key + 8) & in_page;
+#pragma unroll
+          for (int i = 0; i < kPasses; ++i) {
+            const bool second = kPasses == 1 ? load_row >= 8 : i == 1;
+            const int page = second ? page1 : page0, slot = second ? slot1 : slot0, there = max(page, 0);
+            cp_async16(dst + load_at + i * kEight, k_lane + there * a.k_page + slot * a.k_slot, page >= 0);
+            cp_async16(dst + load_at + S::kV + i * kEight, v_lane + there * a.v_page + slot * a.v_slot, page >= 0);
+          }
+          const int page = row & 8 ? page1 : page0, slot = row & 8 ? slot1 : slot0;
+          const bool ok = page >= 0 && key + row >= key_lo && key + row < key_hi;
+          cp_async_small<D / 16>(dst + scale_to, s_lane + max(page, 0) * s_page + slot * s_slot, ok);
         }
-        const int row = lane & 15, s = row >> 3;
-        const bool ok = page[s] >= 0 && key + row >= key_lo && key + row < key_hi;
-        const int64_t there = page[s] >= 0 ? page[s] : 0, in = slot[s] + (row & 7);
-        const uint16_t* from = lane < 16 ? args.k_scale + there * args.ks_page + in * args.ks_slot + it.head * args.ks_head
-                                         : args.v_scale + there * args.vs_page + in * args.vs_slot + it.head * args.vs_head;
-        cp_async_small<D / 16>(dst + (lane < 16 ? S::kKScale : S::kVScale) + row * (D / 16), from, ok);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-#pragma unroll
-    for (int s = 0; s < kRing - 1; ++s) load(s);
-
-    for (int step = 0; step < steps; ++step) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
-      __syncwarp();
-      load(step + kRing - 1);
-      const int key = step * kBlockKeys;
-      if (key >= key_hi || key + kWarpKeys <= key_lo) continue;
-      const uint32_t here = ring + (step % kRing) * S::kBytes;
-
-      // Scores of keys key_of(j) and 8 more (x / 2), columns 2 p and 2 p + 1 (x % 2).
+    // A step's scores, probabilities and product; EDGE: some row does not see some key.
+    const auto compute = [&](auto edge, uint32_t here, int key) {
+      constexpr bool EDGE = decltype(edge)::value;
+      // Sums of keys key_of(j) and 8 more (x / 2), columns 2 p and 2 p + 1 (x % 2).
       float s[NT][4] = {};
       {
         uint32_t wa[G], wb[G];
         load_words<G>(wa, here + k_at);
         load_words<G>(wb, here + k_at + kEight);
         Scales<G> sa, sb;
-        sa.load(here + S::kKScale + key_of(j) * (D / 16));
-        sb.load(here + S::kKScale + (key_of(j) + 8) * (D / 16));
+        sa.load(here + scale_at);
+        sb.load(here + scale_at + 8 * (D / 16));
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           const uint32_t ua = wa[g] >> 8, ub = wb[g] >> 8;
+          const float fa = sa.get(g), fb = sb.get(g);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             float c[4];
@@ -317,65 +345,71 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_int4_decode_kernel(const
                     start[n][g][1], start[n][g][0], start[n][g][1]);
             mma_f16(c, ua & kLow, ub & kLow, ua & kHigh, ub & kHigh, qf[n][g][2], qf[n][g][3], c[0], c[1], c[2], c[3]);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) s[n][x] += c[x] * (x < 2 ? sa.get(g) : sb.get(g));
+            for (int x = 0; x < 4; ++x) s[n][x] = fmaf(c[x], x < 2 ? fa : fb, s[n][x]);
           }
         }
       }
-      const bool edge = key < all_lo || key + kWarpKeys - 1 > all_hi;  // some row does not see some key
-      bool move = false;
-      bool sees[NT][4];
+      Scales<G> va, vb;
+      va.load(here + scale_at + S::kVScale - S::kKScale);
+      vb.load(here + scale_at + S::kVScale - S::kKScale + 8 * (D / 16));
+      float fa[G], fb[G], largest = 0.f;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int g = 0; g < G; ++g) {
+        fa[g] = va.get(g);
+        fb[g] = vb.get(g);
+        largest = fmaxf(largest, fmaxf(fabsf(fa[g]), fabsf(fb[g])));
+      }
+      [[maybe_unused]] bool sees[NT][4];
+      float w[NT][4];  // probabilities times 2^(7 - sigma)
+      bool move = EDGE || largest >= limit;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          s[n][x] *= row_scale[n][x & 1];
-          sees[n][x] = true;
-          if (edge) {
+          if constexpr (EDGE) {
             const int k = warp_key + key + key_of(j) + (x / 2) * 8, hi = see_hi[n][x & 1];
             sees[n][x] = k <= hi && (!a.window || k > hi - a.window);
-            if (!sees[n][x]) s[n][x] = -INFINITY;
           }
-          move |= s[n][x] > top[n][x & 1] + 8.f;
+          w[n][x] = exp2_approx(fmaf(s[n][x], row_scale[n][x & 1], -from[n][x & 1]));
         }
-      Scales<G> va, vb;
-      va.load(here + S::kVScale + key_of(j) * (D / 16));
-      vb.load(here + S::kVScale + (key_of(j) + 8) * (D / 16));
-      uint32_t largest = 0;  // magnitudes of the lane's V scales, as pairs of 16 bits
-#pragma unroll
-      for (int i = 0; i < G / 2; ++i)
-        largest = __vmaxu2(largest, __vmaxu2(va.w[i] & 0x7fff7fffu, vb.w[i] & 0x7fff7fffu));
-      move |= edge || (largest >> 16) >= limit || (largest & 0xffffu) >= limit;
+        move |= fmaxf(w[n][0], w[n][2]) > over[n][0] || fmaxf(w[n][1], w[n][3]) > over[n][1];
+      }
       if (__any_sync(0xffffffffu, move)) {
         // A row's maximum or its largest scale may have moved: its O and sums follow. Each row goes by
         // the keys that it sees, so what others see does not change its bits.
-        uint32_t size[2] = {0, 0};  // this lane's keys
+        float size[2] = {0.f, 0.f};  // largest scale of this lane's keys; infinities and NaNs lose their own group only
 #pragma unroll
-        for (int i = 0; i < G / 2; ++i)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t x = va.w[i] >> 16 * h & 0x7fffu, y = vb.w[i] >> 16 * h & 0x7fffu;
-            if (x < 0x7f80u) size[0] = max(size[0], x);  // infinities and NaNs lose their own group only
-            if (y < 0x7f80u) size[1] = max(size[1], y);
-          }
+        for (int g = 0; g < G; ++g) {
+          if (fabsf(fa[g]) < INFINITY) size[0] = fmaxf(size[0], fabsf(fa[g]));
+          if (fabsf(fb[g]) < INFINITY) size[1] = fmaxf(size[1], fabsf(fb[g]));
+        }
         int least = 127;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            float most = fmaxf(s[n][x], s[n][x + 2]);
-            uint32_t big = max(sees[n][x] ? size[0] : 0u, sees[n][x + 2] ? size[1] : 0u);
+            float most = kNoTop, big = 0.f;
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              if constexpr (EDGE) {
+                if (!sees[n][x + 2 * y]) continue;
+              }
+              most = fmaxf(most, s[n][x + 2 * y] * row_scale[n][x]);
+              big = fmaxf(big, size[y]);
+            }
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) {
               most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-              big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+              big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
             }
             const float was = top[n][x];
             const int sigma_was = sigma[n][x];
-            if (most > was + 8.f) top[n][x] = most;
-            sigma[n][x] = min(max(sigma_was, (int)(big >> 7) - 126), 127);
+            if (most > was + 8.f) top[n][x] = ceilf(most);
+            sigma[n][x] = min(max(sigma_was, (int)(__float_as_uint(big) >> 23) - 126), 127);
             least = min(least, sigma[n][x]);
-            const float f = top[n][x] == -INFINITY ? 1.f
-                                                   : exp2_approx(fmaxf(was - top[n][x], -300.f) + (float)(sigma_was - sigma[n][x]));
+            from[n][x] = top[n][x] + (float)(sigma[n][x] - 7);
+            over[n][x] = power_of_two(min(15 - sigma[n][x], 127));
+            const float f = exp2_approx(fmaxf(was - top[n][x], -300.f) + (float)(sigma_was - sigma[n][x]));
             sum[n][x] *= f;
 #pragma unroll
             for (int g = 0; g < G; ++g)
@@ -385,26 +419,28 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_int4_decode_kernel(const
                 acc[n][g][1][2 * r + x] *= f;
                 eights[n][g][2 * r + x] *= f;
               }
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+              w[n][x + 2 * y] = exp2_approx(fmaf(s[n][x + 2 * y], row_scale[n][x], -from[n][x]));
           }
-        limit = (uint32_t)(least + 127) << 7;
+        limit = power_of_two(least);
       }
-      float w[NT][4];  // probabilities times 2^(7 - sigma)
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const float from = top[n][x] == -INFINITY ? 0.f : top[n][x], up = (float)(7 - sigma[n][x]);
-          w[n][x] = exp2_approx((s[n][x] - from) + up);
-          w[n][x + 2] = exp2_approx((s[n][x + 2] - from) + up);
-          sum[n][x] += w[n][x] + w[n][x + 2];
+        for (int x = 0; x < 4; ++x) {
+          if constexpr (EDGE) {
+            if (!sees[n][x]) w[n][x] = 0.f;
+          }
+          sum[n][x & 1] += w[n][x];
         }
 
       // Channels of this lane: words j % 4 of the four keys, even or odd ones.
       uint32_t w0[G], w1[G], w8[G], w9[G];
-      load_words<G>(w0, here + S::kV + v_at[0]);
-      load_words<G>(w1, here + S::kV + v_at[1]);
-      load_words<G>(w8, here + S::kV + v_at[0] + kEight);
-      load_words<G>(w9, here + S::kV + v_at[1] + kEight);
+      load_words<G>(w0, here + v_at[0]);
+      load_words<G>(w1, here + v_at[1]);
+      load_words<G>(w8, here + v_at[0] + kEight);
+      load_words<G>(w9, here + v_at[1] + kEight);
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         const uint32_t x = __byte_perm(w0[g], w1[g], half_of), y = __byte_perm(w8[g], w9[g], half_of);
@@ -414,8 +450,10 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_int4_decode_kernel(const
           float z[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            z[i] = w[n][i] * (i < 2 ? va.get(g) : vb.get(g));
-            if (edge && !sees[n][i]) z[i] = 0.f;  // whatever the scale is
+            z[i] = w[n][i] * (i < 2 ? fa[g] : fb[g]);
+            if constexpr (EDGE) {
+              if (!sees[n][i]) z[i] = 0.f;  // whatever the scale is
+            }
           }
           const uint32_t w_lo = transposed(half2_of(z[0], z[1])), w_hi = transposed(half2_of(z[2], z[3]));
           float (&o0)[4] = acc[n][g][0], (&o1)[4] = acc[n][g][1], (&e)[4] = eights[n][g];
@@ -424,11 +462,23 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_int4_decode_kernel(const
           mma_f16(e, 0x00080008u, 0x00800080u, 0x00080008u, 0x00800080u, w_lo, w_hi, e[0], e[1], e[2], e[3]);
         }
       }
+    };
+#pragma unroll
+    for (int s = 0; s < kRing - 1; ++s) load(s);
+
+    for (int step = 0; step < steps; ++step) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+      __syncwarp();
+      load(step + kRing - 1);
+      const int key = step * kBlockKeys;
+      const uint32_t here = ring + step % kRing * S::kBytes;
+      if (key >= all_lo && key + kWarpKeys - 1 <= all_hi) compute(std::false_type{}, here, key);
+      else if (key < key_hi && key + kWarpKeys > key_lo) compute(std::true_type{}, here, key);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
 
-    // The four warps' sums over their keys, joined.
+    // The sums of the warps that share a head's keys, joined.
     float* joined = reinterpret_cast<float*>(smem) + warp * kRows * D;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -441,7 +491,7 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_int4_decode_kernel(const
         const int row = 8 * n + 2 * p + x;
         const float down = power_of_two(sigma[n][x] - 7);
         if (j == 0) {
-          stat[warp][row][0] = top[n][x];
+          stat[warp][row][0] = top[n][x] == kNoTop ? -INFINITY : top[n][x];
           stat[warp][row][1] = l * down;
         }
 #pragma unroll
@@ -457,30 +507,32 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_int4_decode_kernel(const
     const bool whole = b0 == 0 && b1 == it.blocks;
     const int64_t slot = 2 * cta + (b0 == 0 ? 1 : 0);
     if (threadIdx.x == 0 && bad_page) atomicOr(&g_device_error, kDeviceErrorIndex);
-    for (int i = threadIdx.x; i < rows * D; i += kDecodeThreads) {
-      const int row = i / D, col = i % D;
+    const int heads = min(HEADS, a.kv_heads - it.head);
+    for (int i = threadIdx.x; i < heads * rows * D; i += kDecodeThreads) {
+      const int col = i % D, h_row = i / D, hh = HEADS == 1 ? 0 : h_row / rows, row = h_row - hh * rows;
       float m = -INFINITY;
 #pragma unroll
-      for (int v = 0; v < kDecodeWarps; ++v) m = fmaxf(m, stat[v][row][0]);
-      const float from = m == -INFINITY ? 0.f : m;
+      for (int v = 0; v < kSplit; ++v) m = fmaxf(m, stat[v * HEADS + hh][row][0]);
+      const float top_of = m == -INFINITY ? 0.f : m;
       float o = 0.f, l = 0.f;
 #pragma unroll
-      for (int v = 0; v < kDecodeWarps; ++v) {
-        const float f = exp2_approx(stat[v][row][0] - from);
-        o += f * reinterpret_cast<float*>(smem)[(v * kRows + row) * D + col];
-        l += f * stat[v][row][1];
+      for (int v = 0; v < kSplit; ++v) {
+        const float f = exp2_approx(stat[v * HEADS + hh][row][0] - top_of);
+        o += f * reinterpret_cast<float*>(smem)[((v * HEADS + hh) * kRows + row) * D + col];
+        l += f * stat[v * HEADS + hh][row][1];
       }
       if (bad_page) l = o = __int_as_float(0x7fc00000);
       if (whole) {
         const int of = row0 + row, token = of / a.group;
-        const int h = it.head * a.group + (of - token * a.group);
+        const int h = (it.head + hh) * a.group + (of - token * a.group);
         static_cast<T*>(a.out)[(q.first + token) * a.out_n + h * a.out_h + col] = from_float<T>(l == 0.f ? 0.f : o / l);
         if (a.lse && col == 0) a.lse[(int64_t)(q.first + token) * a.heads + h] = (m + log2f(l)) * 0.6931471805599453f;
       } else {
-        part_out[(slot * kRows + row) * D + col] = o;
+        const int64_t to = (slot * HEADS + hh) * kRows + row;
+        part_out[to * D + col] = o;
         if (col == 0) {
-          part_stat[(slot * kRows + row) * 2] = m;
-          part_stat[(slot * kRows + row) * 2 + 1] = l;
+          part_stat[to * 2] = m;
+          part_stat[to * 2 + 1] = l;
         }
       }
     }
@@ -490,14 +542,14 @@ __global__ void __launch_bounds__(kDecodeThreads) paged_int4_decode_kernel(const
   }
 }
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, int HEADS>
 cudaError_t launch(Int4Args args, cudaStream_t stream) {
   AttentionArgs& a = args.a;
-  constexpr int kRows = 8 * NT;
-  a.whole = a.max_keys <= kWholeKeys;
+  constexpr int kRows = 8 * NT, kBlockKeys = kWarpKeys * kDecodeWarps / HEADS;
+  a.whole = a.max_keys <= kWholeKeys / HEADS;
   constexpr size_t ring = (size_t)kDecodeWarps * kRing * Step<D>::kBytes, joined = (size_t)kDecodeWarps * kRows * D * 4;
   constexpr size_t smem = ring > joined ? ring : joined;
-  const void* fn = reinterpret_cast<const void*>(&paged_int4_decode_kernel<T, D, NT>);
+  const void* fn = reinterpret_cast<const void*>(&paged_int4_decode_kernel<T, D, NT, HEADS>);
   cudaError_t err = allow_shared_memory(fn, smem);
   if (err != cudaSuccess) return err;
   // Never more CTAs than there can be units.
@@ -507,27 +559,36 @@ cudaError_t launch(Int4Args args, cudaStream_t stream) {
   if ((err = cudaGetDevice(&dev)) != cudaSuccess ||
       (err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess)
     return err;
-  const int64_t want = tiles * a.kv_heads * blocks, most = (int64_t)sms * kCtasPerSm;
+  const int64_t want = tiles * ((a.kv_heads + HEADS - 1) / HEADS) * blocks, most = (int64_t)sms * kCtasPerSm;
   const int64_t grid = persistent_grid(fn, smem, want < most ? want : most, kDecodeThreads);
   if (grid <= 0) return cudaErrorInvalidConfiguration;
-  err = launch_kernel(paged_int4_decode_kernel<T, D, NT>, dim3((unsigned)grid), dim3(kDecodeThreads), smem, stream, args);
+  err = launch_kernel(paged_int4_decode_kernel<T, D, NT, HEADS>, dim3((unsigned)grid), dim3(kDecodeThreads), smem, stream, args);
   if (err != cudaSuccess || a.whole) return err;
   const unsigned rows = a.pages.cu_seqlens || a.group > kRows ? kRows : a.group;  // rows a tile can have
-  return launch_following(paged_join_kernel<T, D, kRows, false>, dim3((unsigned)grid, rows), dim3(kJoinWarps * 32), stream, a,
-                          grid);
+  return launch_following(paged_join_kernel<T, D, kRows, false, HEADS>, dim3((unsigned)grid, rows, HEADS), dim3(kJoinWarps * 32),
+                          stream, a, grid);
+}
+
+// Key heads of a CTA: a cache line holds the scales of several heads' slots, and is fetched
+// once where one CTA reads them together. Four at a time, two, or one where most of four would idle.
+template <typename T, int D, int NT>
+cudaError_t launch_heads(const Int4Args& args, cudaStream_t stream) {
+  const int heads = args.a.kv_heads;
+  if (heads % 4 == 0 || heads % 4 == 3) return launch<T, D, NT, 4>(args, stream);
+  return heads % 2 == 0 ? launch<T, D, NT, 2>(args, stream) : launch<T, D, NT, 1>(args, stream);
 }
 
 template <typename T, int D>
 cudaError_t launch_rows(const Int4Args& args, cudaStream_t stream) {
   // Tiles of 8 rows where the requests have no more a key head on average, else of 16.
-  return (int64_t)args.a.tokens * args.a.group <= 8 * (int64_t)args.a.pages.batch ? launch<T, D, 1>(args, stream)
-                                                                                  : launch<T, D, 2>(args, stream);
+  return (int64_t)args.a.tokens * args.a.group <= 8 * (int64_t)args.a.pages.batch ? launch_heads<T, D, 1>(args, stream)
+                                                                                  : launch_heads<T, D, 2>(args, stream);
 }
 
 }  // namespace
 
 size_t paged_int4_decode_workspace(int D, int sms) {
-  return (size_t)sms * kCtasPerSm * (2 * 16 * (size_t)(D + 2) * sizeof(float) + sizeof(Part));
+  return (size_t)sms * kCtasPerSm * (2 * 4 * 16 * (size_t)(D + 2) * sizeof(float) + sizeof(Part));
 }
 
 cudaError_t launch_paged_int4_decode(const AttentionArgs& a, const flash_prologue_scales& s, int dtype, int D,

@@ -1,7 +1,7 @@
 // How the kernels for few new tokens a request (paged_decode.cu, paged_int4_decode.cu)
 // share out their work: items (a tile of ROWS rows of a key head's query heads x new
-// tokens, over the request's keys) of blocks of 64 keys, counted over all requests.
-// Every CTA of a full GPU takes an equal run of blocks, or with few items a piece of
+// tokens, over the request's keys, for HEADS key heads next to each other) of blocks
+// of KEYS keys, counted over all requests. Every CTA of a full GPU takes an equal run of blocks, or with few items a piece of
 // one; items that several CTAs have are joined by a second kernel, in order.
 #pragma once
 
@@ -13,7 +13,12 @@ namespace {
 constexpr int kDecodeWarps = 4;
 constexpr int kDecodeThreads = kDecodeWarps * 32;
 constexpr int kWarpKeys = 16;   // keys of a warp's step
-constexpr int kBlockKeys = kWarpKeys * kDecodeWarps;
+template <int ROWS_, int KEYS_, int HEADS_>
+struct Tiling {
+  static constexpr int ROWS = ROWS_, KEYS = KEYS_, HEADS = HEADS_;
+  // Head groups (the last may have fewer heads).
+  static __device__ __forceinline__ int groups(const AttentionArgs& a) { return HEADS == 1 ? a.kv_heads : (a.kv_heads + HEADS - 1) / HEADS; }
+};
 constexpr int kNone = -(1 << 30);  // below every relative position
 constexpr int kWholeKeys = 256; // longest caches whose items are never split
 
@@ -39,14 +44,15 @@ __device__ __forceinline__ T from_float(float v) {
 __device__ __forceinline__ int first_key(const Request& q, int window) {
   return window ? max(q.total - q.news - window + 1, 0) : 0;
 }
+template <class B>
 __device__ __forceinline__ int blocks_of(const Request& q, int window) {
-  const int lo = first_key(q, window) / kBlockKeys, hi = (q.total + kBlockKeys - 1) / kBlockKeys;
+  const int lo = first_key(q, window) / B::KEYS, hi = (q.total + B::KEYS - 1) / B::KEYS;
   return max(hi - lo, 1);  // one at least: it writes the zeros of rows without keys
 }
-// Row tiles times key heads, each an item of blocks_of() blocks.
-template <int ROWS>
+// Row tiles times head groups, each an item of blocks_of() blocks.
+template <class B>
 __device__ __forceinline__ int64_t items_of(const Request& q, const AttentionArgs& a) {
-  return (int64_t)((q.news * a.group + ROWS - 1) / ROWS) * a.kv_heads;
+  return (int64_t)((q.news * a.group + B::ROWS - 1) / B::ROWS) * B::groups(a);
 }
 // Units of an item: `cut` blocks at most in each.
 __device__ __forceinline__ int units_of_item(int blocks, int cut) {
@@ -110,7 +116,7 @@ struct Run {
 };
 
 // This CTA's run; false where it has none. parts[cta] is marked as nothing to join.
-template <int ROWS>
+template <class B>
 __device__ __forceinline__ bool find_run(const AttentionArgs& a, RunScratch& shared, Part* parts, Run& run) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int batch = requests_of(a.pages);
@@ -123,8 +129,8 @@ __device__ __forceinline__ bool find_run(const AttentionArgs& a, RunScratch& sha
     bool b;
     const Request q = request_at(a.pages, a.tokens, a.max_keys, r, &b);
     bad |= b;
-    my_items = items_of<ROWS>(q, a);
-    my_blocks = blocks_of(q, a.window);
+    my_items = items_of<B>(q, a);
+    my_blocks = blocks_of<B>(q, a.window);
     total[0] += my_items * my_blocks;
     total[1] += my_items;
   }
@@ -151,7 +157,7 @@ __device__ __forceinline__ bool find_run(const AttentionArgs& a, RunScratch& sha
       if (r < batch) {
         bool b;
         const Request q = request_at(a.pages, a.tokens, a.max_keys, r, &b);
-        n = items_of<ROWS>(q, a) * units_of_item(blocks_of(q, a.window), cut);
+        n = items_of<B>(q, a) * units_of_item(blocks_of<B>(q, a.window), cut);
       }
     }
     int64_t upto = n;  // inclusive sum within the warp
@@ -207,12 +213,13 @@ struct Item {
   int per_item, u1;     // units of the item, the end of this CTA's
   int64_t item_start;   // units before the item
   int blocks, b0, b1;   // blocks of the item, this CTA's
-  int head, row0, rows; // of the request's news * group rows
+  int head;             // first key head
+  int row0, rows;       // of the request's news * group rows
   int base;             // position of new token 0
   int key0, lo, hi;     // first key of block 0; keys that a row of this tile sees
 };
 
-template <int ROWS>
+template <class B>
 __device__ __forceinline__ void find_item(const AttentionArgs& a, Run& run, int64_t unit, Item& it) {
   bool too_long;
   int r = run.r;
@@ -220,25 +227,25 @@ __device__ __forceinline__ void find_item(const AttentionArgs& a, Run& run, int6
   const int cut = run.cut;
   const int64_t end = run.end;
   Request q = request_at(a.pages, a.tokens, a.max_keys, r, &too_long);
-  int64_t in_request = items_of<ROWS>(q, a) * units_of_item(blocks_of(q, a.window), cut);
+  int64_t in_request = items_of<B>(q, a) * units_of_item(blocks_of<B>(q, a.window), cut);
   while (unit >= start + in_request) {
     start += in_request;
     ++r;
     q = request_at(a.pages, a.tokens, a.max_keys, r, &too_long);
-    in_request = items_of<ROWS>(q, a) * units_of_item(blocks_of(q, a.window), cut);
+    in_request = items_of<B>(q, a) * units_of_item(blocks_of<B>(q, a.window), cut);
   }
-  const int blocks = blocks_of(q, a.window), per_item = units_of_item(blocks, cut);
+  const int blocks = blocks_of<B>(q, a.window), per_item = units_of_item(blocks, cut);
   const int size = cut == 1 ? 1 : (blocks + per_item - 1) / per_item;  // blocks of a unit, evenly
   const int64_t in = unit - start;
   const int item = in >> 31 ? (int)(in / per_item) : (int)in / per_item;  // tiles x heads stay below 2^31
   const int64_t item_start = start + (int64_t)item * per_item;
   const int u0 = (int)(unit - item_start), u1 = (int)min((int64_t)per_item, end - item_start);
   const int b0 = u0 * size, b1 = min(u1 * size, blocks);
-  const int head = item % a.kv_heads;
-  const int row0 = item / a.kv_heads * ROWS;       // of the request's news * group rows
-  const int rows = min(ROWS, q.news * a.group - row0);
+  const int groups = B::groups(a), head = item % groups * B::HEADS;
+  const int row0 = item / groups * B::ROWS;         // of the request's news * group rows
+  const int rows = min(B::ROWS, q.news * a.group - row0);
   const int base = q.total - q.news;                // position of new token 0
-  const int key0 = first_key(q, a.window) / kBlockKeys * kBlockKeys;
+  const int key0 = first_key(q, a.window) / B::KEYS * B::KEYS;
   // Keys that a row of this tile sees.
   const int hi = base + (row0 + rows - 1) / a.group + 1;
   const int lo = a.window ? max(base + row0 / a.group - a.window + 1, 0) : 0;
@@ -273,19 +280,19 @@ __device__ __forceinline__ Part part_of(const Run& run, const Item& it) {
   return p;
 }
 
-// Joins the parts of one row of the item that CTA blockIdx.x of the first kernel
+// Joins the parts of one row (and head) of the item that CTA blockIdx.x of the first kernel
 // began: every warp takes each eighth part, its columns over the lanes.
 constexpr int kJoinWarps = 8;
-template <typename T, int D, int ROWS, bool SHIFTED>
+template <typename T, int D, int ROWS, bool SHIFTED, int HEADS = 1>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const AttentionArgs a, int64_t ctas) {
   constexpr int kCols = D / 32;  // columns of a lane
   __shared__ float joined[kJoinWarps][D], sums[kJoinWarps], tops[kJoinWarps];
   const float* part_out = static_cast<const float*>(a.workspace);
-  const float* part_stat = part_out + 2 * ctas * ROWS * D;
+  const float* part_stat = part_out + 2 * ctas * HEADS * ROWS * D;
   wait_for_previous_kernel();
-  const Part p = reinterpret_cast<const Part*>(part_stat + 2 * ctas * ROWS * 2)[blockIdx.x];
-  const int row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (p.last < 0 || row >= p.rows) return;
+  const Part p = reinterpret_cast<const Part*>(part_stat + 2 * ctas * HEADS * ROWS * 2)[blockIdx.x];
+  const int head = HEADS == 1 ? 0 : blockIdx.z, row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (p.last < 0 || row >= p.rows || (HEADS > 1 && p.kv_head + head >= a.kv_heads)) return;
   const int first = blockIdx.x, parts = p.last - first + 1;
   float top = -INFINITY, sum = 0.f, o[kCols] = {};
   constexpr int kFlight = 4;
@@ -300,7 +307,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Atten
       for (int c = 0; c < kCols; ++c) x[f][c] = 0.f;
       if (i < parts) {
         // Part i is in the second slot of the CTA that began the item, in the first slot of the others.
-        const int64_t at = (2 * (int64_t)(first + i) + (i == 0)) * ROWS + row;
+        const int64_t at = ((2 * (int64_t)(first + i) + (i == 0)) * HEADS + head) * ROWS + row;
         st[f] = __ldcg(reinterpret_cast<const float2*>(part_stat + at * 2));
         const float* src = part_out + at * D + lane * kCols;
         if constexpr (kCols == 4) {
@@ -349,7 +356,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Atten
     l += e * sums[w];
   }
   const int at = p.row0 + row, token = at / a.group;
-  const int h = p.kv_head * a.group + (at - token * a.group);
+  const int h = (p.kv_head + head) * a.group + (at - token * a.group);
   static_cast<T*>(a.out)[(p.token0 + token) * a.out_n + h * a.out_h + col] = from_float<T>(l == 0.f ? 0.f : v / l);
   if (a.lse && col == 0) a.lse[(int64_t)(p.token0 + token) * a.heads + h] = (m + log2f(l) - (SHIFTED ? kProbabilityShift<T> : 0.f)) * 0.6931471805599453f;
 }

@@ -262,7 +262,10 @@ def test_pages_out_of_range_give_nan_and_the_error_word(news):
     lens[1] = 10 ** 6  # more tokens than its pages hold
     got = fap.paged_attention_int4(q, *req.cache, req.table, lens, req.cu)
     assert _lib.device_error() == 2
-    assert got[news[0]:-news[2]].isnan().all() and torch.equal(got[:news[0]], clean[:news[0]])
+    assert got[news[0]:-news[2]].isnan().all()
+    # other lengths move the borders at which the work is cut, and with them the order of sums: right, not equal
+    exact, bound, _ = _bound(req, q, 1.0, 0)
+    assert ((got[:news[0]].double() - exact[:news[0]]).abs() <= bound[:news[0]]).all()
 
 
 @pytest.mark.gpu
