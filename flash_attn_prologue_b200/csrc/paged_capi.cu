@@ -56,7 +56,13 @@ int attention(const flash_prologue_attention_args* a, const flash_prologue_scale
               void* stream) {
   int st = size_checks(a, scales != nullptr);
   if (st != FLASH_PROLOGUE_OK || a->tokens == 0 || a->Hq == 0) return st;
-  if (scales && (st = check_scales(*scales, a->cache, a->D)) != FLASH_PROLOGUE_OK) return st;
+  if (scales) {
+    if ((st = check_scales(*scales, a->cache, a->D)) != FLASH_PROLOGUE_OK) return st;
+    // The kernels multiply pages and slots by strides of 31 bits.
+    for (int64_t s : {a->cache.k_page, a->cache.k_slot, a->cache.v_page, a->cache.v_slot, 2 * scales->k_page,
+                      2 * scales->k_slot, 2 * scales->v_page, 2 * scales->v_slot})
+      if (s > INT32_MAX || s < INT32_MIN) return FLASH_PROLOGUE_ERR_UNSUPPORTED;
+  }
   const flash_prologue_cache& c = a->cache;
   if (!a->q.data || !a->out.data) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
   if ((reinterpret_cast<uintptr_t>(a->q.data) | reinterpret_cast<uintptr_t>(a->out.data)) & 15 ||

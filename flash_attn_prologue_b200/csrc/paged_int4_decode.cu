@@ -32,6 +32,8 @@
 namespace flash_prologue {
 namespace {
 
+constexpr int kHalves = 1;           // 16-key halves of a warp's step
+constexpr int kStepKeys = kHalves * kWarpKeys;
 constexpr int kRing = 4;             // steps of a warp's ring
 constexpr int kCtasPerSm = 4;
 constexpr int kLeastScale = -80;     // least exponent of sigma: sums of 2^(15 + 80) stay inside FP32
@@ -108,7 +110,7 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[G], uint32_t addr) {
   }
 }
 
-// A step's 16 keys of one row of codes each. Slot k of the products (rows of S, columns of
+// A half step's 16 keys of one row of codes each. Slot k of the products (rows of S, columns of
 // V^T) is key key_of(k): with it the 8 lanes (16 at D = 64) that read shared memory at once
 // find their pieces in different banks, both for K (4 pieces of neighbouring slots) and for
 // V (few pieces of every other slot), where pieces lie as at() says.
@@ -120,7 +122,7 @@ __device__ __forceinline__ int at(int key, int piece) {  // bytes; piece 0 .. 3 
 }
 
 template <int D>
-struct Step {
+struct Half {
   static constexpr int kCodes = kWarpKeys * D / 2, kScale = kWarpKeys * D / 16;
   static constexpr int kV = kCodes, kKScale = 2 * kCodes, kVScale = 2 * kCodes + kScale, kBytes = 2 * (kCodes + kScale);
 };
@@ -129,23 +131,24 @@ struct Int4Args {
   AttentionArgs a;  // k, v: codes, strides in bytes
   const uint16_t* k_scale;
   const uint16_t* v_scale;
-  int64_t ks_page, ks_slot, ks_head, vs_page, vs_slot, vs_head;
+  int64_t ks_page, ks_slot, ks_head, vs_page, vs_slot, vs_head;  // elements
 };
 
 // NT tiles of 8 rows; HEADS key heads a CTA, so 4 / HEADS warps share a head's keys.
 template <typename T, int D, int NT, int HEADS>
 __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 128 ? 3 : 4 : 2) paged_int4_decode_kernel(const Int4Args args) {
   const AttentionArgs& a = args.a;
-  constexpr int kRows = 8 * NT, kSplit = kDecodeWarps / HEADS, kBlockKeys = kWarpKeys * kSplit;
+  constexpr int kRows = 8 * NT, kSplit = kDecodeWarps / HEADS, kBlockKeys = kStepKeys * kSplit;
   constexpr int G = D / 32;  // groups of channels; words of a piece
   using Tiles = Tiling<kRows, kBlockKeys, HEADS>;
-  using S = Step<D>;
+  using S = Half<D>;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ RunScratch shared;
   __shared__ float stat[kDecodeWarps][kRows][2];
   __shared__ int bad_page;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t ring = smem_u32(smem) + warp * kRing * S::kBytes;
+  constexpr uint32_t kStage = kHalves * S::kBytes;
+  const uint32_t ring = smem_u32(smem) + warp * kRing * kStage, ring_end = ring + kRing * kStage;
 
   if (!a.whole) start_next_kernel();
   const int64_t slots = 2 * (int64_t)gridDim.x, cta = blockIdx.x;
@@ -233,9 +236,9 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 128 ? 3 : 4 : 2
       }
     }
     // Of a column: probabilities are 2^(score - from), from = top + sigma - 7 (whole numbers: no
-    // rounding); `over` is what they reach 2^8 above top, `limit` 2^(least sigma).
-    float acc[NT][G][2][4], eights[NT][G][4], top[NT][2], from[NT][2], over[NT][2], sum[NT][2], limit = power_of_two(kLeastScale);
-    int sigma[NT][2];
+    // rounding); `over` is what they reach 2^8 above top, 2^(15 - sigma); `limit` is 2^(least sigma).
+    float acc[NT][G][2][4], eights[NT][G][4], from[NT][2], over[NT][2], sum[NT][2], limit = power_of_two(kLeastScale);
+    const auto sigma_of = [](float over) { return 15 - ((int)(__float_as_uint(over) >> 23) - 127); };
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -244,10 +247,9 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 128 ? 3 : 4 : 2
         for (int x = 0; x < 4; ++x) acc[n][g][0][x] = acc[n][g][1][x] = eights[n][g][x] = 0.f;
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        top[n][x] = from[n][x] = kNoTop;
-        over[n][x] = 0.f;
+        from[n][x] = kNoTop;
+        over[n][x] = power_of_two(15 - kLeastScale);
         sum[n][x] = 0.f;
-        sigma[n][x] = kLeastScale;
       }
     }
     if (threadIdx.x == 0) bad_page = it.too_long;
@@ -255,85 +257,96 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 128 ? 3 : 4 : 2
 
     // Positions relative to this warp's first key, in 32 bits (a request has fewer than 2^30 keys).
     const int steps = idle ? 0 : b1 - b0;
-    const int warp_key = it.key0 + b0 * kBlockKeys + warp / HEADS * kWarpKeys;
+    const int warp_key = it.key0 + b0 * kBlockKeys + warp / HEADS * kStepKeys;
     const int key_lo = it.lo - warp_key, key_hi = it.hi - warp_key;
     const int all_lo = a.window ? base + (row0 + rows - 1) / a.group - a.window + 1 - warp_key : kNone;
     const int all_hi = base + row0 / a.group - warp_key;  // every row sees keys all_lo .. all_hi
     const int32_t* table = a.pages.page_table + (int64_t)it.r * a.pages.table_stride;
+    // Strides of slots and pages take 31 bits (the host checks): a product and a sum in one instruction.
     const unsigned char* k_lane = static_cast<const unsigned char*>(a.k) + head * a.k_head + (load_row & 7) * a.k_slot + chunk * 16;
     const unsigned char* v_lane = static_cast<const unsigned char*>(a.v) + head * a.v_head + (load_row & 7) * a.v_slot + chunk * 16;
-    const uint16_t* s_lane = lane < 16 ? args.k_scale + head * args.ks_head + (lane & 7) * args.ks_slot
-                                       : args.v_scale + head * args.vs_head + (lane & 7) * args.vs_slot;
-    const int64_t s_page = lane < 16 ? args.ks_page : args.vs_page, s_slot = lane < 16 ? args.ks_slot : args.vs_slot;
-    int page_of[2] = {0, 0};  // page of the keys of step page_step + lane (pages of 8 slots: of either half)
-    int page_step = -32;
+    const unsigned char* s_lane = reinterpret_cast<const unsigned char*>(
+        lane < 16 ? args.k_scale + head * args.ks_head + (lane & 7) * args.ks_slot
+                  : args.v_scale + head * args.vs_head + (lane & 7) * args.vs_slot);
+    const int k_page = (int)a.k_page, k_slot = (int)a.k_slot, v_page = (int)a.v_page, v_slot = (int)a.v_slot;
+    const int s_page = 2 * (int)(lane < 16 ? args.ks_page : args.vs_page), s_slot = 2 * (int)(lane < 16 ? args.ks_slot : args.vs_slot);
+    const auto along = [](const unsigned char* from, int n, int stride) { return from + (int64_t)n * stride; };
+    // Pages of the keys of step page_step + lane, eight by eight (sixteen where they are in one page); -1: none.
+    int page_of[2 * kHalves];
+    int page_left = 0;  // steps that they still cover
+    uint32_t to = ring;
     const auto load = [&](int step) {
       if (step < steps) {
-        if (step - page_step >= 32) {
-          page_step = step;
+        if (page_left == 0) {
+          page_left = 32;
 #pragma unroll
-          for (int s = 0; s < 2; ++s) {
+          for (int s = 0; s < 2 * kHalves; ++s) {
             const int k = (step + lane) * kBlockKeys + s * 8;
-            page_of[s] = 0;
+            page_of[s] = -1;
+            if (wide && s % 2) continue;
             if (step + lane < steps && k < key_hi && k + (wide ? 16 : 8) > key_lo) {
-              page_of[s] = __ldg(table + ((warp_key + k) >> a.pages.page_log2));
-              if (page_of[s] < 0 || page_of[s] >= a.pages.num_pages) {
-                page_of[s] = -1;
-                bad_page = 1;
-              }
+              const int page = __ldg(table + ((warp_key + k) >> a.pages.page_log2));
+              if (page >= 0 && page < a.pages.num_pages) page_of[s] = page;
+              else bad_page = 1;
             }
           }
         }
-        const int key = step * kBlockKeys;
-        const uint32_t dst = ring + step % kRing * S::kBytes;
-        const int page0 = __shfl_sync(0xffffffffu, page_of[0], step - page_step), slot0 = (warp_key + key) & in_page;
+        const int from = 32 - page_left--;
+        const int key = step * kBlockKeys, row = lane & 15;
+        const bool inside = key >= key_lo && key + kStepKeys <= key_hi;
         // Codes of slots outside the tile's keys are whatever they are: their scales are zeros.
-        const int row = lane & 15;
-        if (wide && page0 >= 0) {
-          const unsigned char* k = k_lane + page0 * a.k_page + slot0 * a.k_slot;
-          const unsigned char* v = v_lane + page0 * a.v_page + slot0 * a.v_slot;
-          if constexpr (kPasses == 1) {
-            if (load_row >= 8) {
-              k += 8 * a.k_slot;
-              v += 8 * a.v_slot;
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+          const uint32_t dst = to + h * S::kBytes;
+          const int first = key + h * kWarpKeys;
+          const int page0 = __shfl_sync(0xffffffffu, page_of[2 * h], from), slot0 = (warp_key + first) & in_page;
+          const bool ok = inside || (first + row >= key_lo && first + row < key_hi);
+          if (wide && page0 >= 0) {
+            const unsigned char* k = along(along(k_lane, page0, k_page), slot0, k_slot);
+            const unsigned char* v = along(along(v_lane, page0, v_page), slot0, v_slot);
+            if constexpr (kPasses == 1) {
+              k = along(k, load_row & 8, k_slot);
+              v = along(v, load_row & 8, v_slot);
             }
-          }
 #pragma unroll
-          for (int i = 0; i < kPasses; ++i) {
-            cp_async16(dst + load_at + i * kEight, k + i * (8 * a.k_slot), true);
-            cp_async16(dst + load_at + S::kV + i * kEight, v + i * (8 * a.v_slot), true);
-          }
-          const bool ok = key + row >= key_lo && key + row < key_hi;
-          cp_async_small<D / 16>(dst + scale_to, s_lane + page0 * s_page + (slot0 + (row & 8)) * s_slot, ok);
-        } else {
-          // Pages of 8 slots, or one that is outside the cache.
-          const int page1 = __shfl_sync(0xffffffffu, page_of[1], step - page_step), slot1 = (warp_key + key + 8) & in_page;
+            for (int i = 0; i < kPasses; ++i) {
+              cp_async16(dst + load_at + i * kEight, along(k, 8 * i, k_slot), true);
+              cp_async16(dst + load_at + S::kV + i * kEight, along(v, 8 * i, v_slot), true);
+            }
+            cp_async_small<D / 16>(dst + scale_to, along(along(s_lane, page0, s_page), slot0 + (row & 8), s_slot), ok);
+          } else {
+            // Pages of 8 slots, or none.
+            const int page1 = __shfl_sync(0xffffffffu, page_of[2 * h + 1], from), slot1 = (warp_key + first + 8) & in_page;
 #pragma unroll
-          for (int i = 0; i < kPasses; ++i) {
-            const bool second = kPasses == 1 ? load_row >= 8 : i == 1;
-            const int page = second ? page1 : page0, slot = second ? slot1 : slot0, there = max(page, 0);
-            cp_async16(dst + load_at + i * kEight, k_lane + there * a.k_page + slot * a.k_slot, page >= 0);
-            cp_async16(dst + load_at + S::kV + i * kEight, v_lane + there * a.v_page + slot * a.v_slot, page >= 0);
+            for (int i = 0; i < kPasses; ++i) {
+              const bool second = kPasses == 1 ? load_row >= 8 : i == 1;
+              const int page = second ? page1 : page0, slot = second ? slot1 : slot0, there = max(page, 0);
+              cp_async16(dst + load_at + i * kEight, along(along(k_lane, there, k_page), slot, k_slot), page >= 0);
+              cp_async16(dst + load_at + S::kV + i * kEight, along(along(v_lane, there, v_page), slot, v_slot), page >= 0);
+            }
+            const int page = row & 8 ? page1 : page0, slot = row & 8 ? slot1 : slot0;
+            cp_async_small<D / 16>(dst + scale_to, along(along(s_lane, max(page, 0), s_page), slot, s_slot), page >= 0 && ok);
           }
-          const int page = row & 8 ? page1 : page0, slot = row & 8 ? slot1 : slot0;
-          const bool ok = page >= 0 && key + row >= key_lo && key + row < key_hi;
-          cp_async_small<D / 16>(dst + scale_to, s_lane + max(page, 0) * s_page + slot * s_slot, ok);
         }
+        to += kStage;
+        if (to == ring_end) to = ring;
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
     // A step's scores, probabilities and product; EDGE: some row does not see some key.
     const auto compute = [&](auto edge, uint32_t here, int key) {
       constexpr bool EDGE = decltype(edge)::value;
-      // Sums of keys key_of(j) and 8 more (x / 2), columns 2 p and 2 p + 1 (x % 2).
-      float s[NT][4] = {};
-      {
+      // Sums of a half's keys key_of(j) and 8 more (x / 2), columns 2 p and 2 p + 1 (x % 2).
+      float s[kHalves][NT][4] = {};
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) {
+        const uint32_t at_half = here + h * S::kBytes;
         uint32_t wa[G], wb[G];
-        load_words<G>(wa, here + k_at);
-        load_words<G>(wb, here + k_at + kEight);
+        load_words<G>(wa, at_half + k_at);
+        load_words<G>(wb, at_half + k_at + kEight);
         Scales<G> sa, sb;
-        sa.load(here + scale_at);
-        sb.load(here + scale_at + 8 * (D / 16));
+        sa.load(at_half + scale_at);
+        sb.load(at_half + scale_at + 8 * (D / 16));
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           const uint32_t ua = wa[g] >> 8, ub = wb[g] >> 8;
@@ -345,44 +358,50 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 128 ? 3 : 4 : 2
                     start[n][g][1], start[n][g][0], start[n][g][1]);
             mma_f16(c, ua & kLow, ub & kLow, ua & kHigh, ub & kHigh, qf[n][g][2], qf[n][g][3], c[0], c[1], c[2], c[3]);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) s[n][x] = fmaf(c[x], x < 2 ? fa : fb, s[n][x]);
+            for (int x = 0; x < 4; ++x) s[h][n][x] = fmaf(c[x], x < 2 ? fa : fb, s[h][n][x]);
           }
         }
       }
-      Scales<G> va, vb;
-      va.load(here + scale_at + S::kVScale - S::kKScale);
-      vb.load(here + scale_at + S::kVScale - S::kKScale + 8 * (D / 16));
-      float fa[G], fb[G], largest = 0.f;
+      Scales<G> va[kHalves], vb[kHalves];
+      float largest = 0.f;
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        fa[g] = va.get(g);
-        fb[g] = vb.get(g);
-        largest = fmaxf(largest, fmaxf(fabsf(fa[g]), fabsf(fb[g])));
+      for (int h = 0; h < kHalves; ++h) {
+        const uint32_t at_scales = here + h * S::kBytes + scale_at + S::kVScale - S::kKScale;
+        va[h].load(at_scales);
+        vb[h].load(at_scales + 8 * (D / 16));
+#pragma unroll
+        for (int g = 0; g < G; ++g) largest = fmaxf(largest, fmaxf(fabsf(va[h].get(g)), fabsf(vb[h].get(g))));
       }
-      [[maybe_unused]] bool sees[NT][4];
-      float w[NT][4];  // probabilities times 2^(7 - sigma)
+      const auto sees = [&](int h, int n, int x) {
+        const int k = warp_key + key + h * kWarpKeys + key_of(j) + (x / 2) * 8, hi = see_hi[n][x & 1];
+        return k <= hi && (!a.window || k > hi - a.window);
+      };
+      float w[kHalves][NT][4];  // probabilities times 2^(7 - sigma)
       bool move = EDGE || largest >= limit;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
+        float most[2] = {0.f, 0.f};
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          if constexpr (EDGE) {
-            const int k = warp_key + key + key_of(j) + (x / 2) * 8, hi = see_hi[n][x & 1];
-            sees[n][x] = k <= hi && (!a.window || k > hi - a.window);
+        for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            w[h][n][x] = exp2_approx(fmaf(s[h][n][x], row_scale[n][x & 1], -from[n][x & 1]));
+            most[x & 1] = fmaxf(most[x & 1], w[h][n][x]);
           }
-          w[n][x] = exp2_approx(fmaf(s[n][x], row_scale[n][x & 1], -from[n][x & 1]));
-        }
-        move |= fmaxf(w[n][0], w[n][2]) > over[n][0] || fmaxf(w[n][1], w[n][3]) > over[n][1];
+        move |= most[0] > over[n][0] || most[1] > over[n][1];
       }
       if (__any_sync(0xffffffffu, move)) {
         // A row's maximum or its largest scale may have moved: its O and sums follow. Each row goes by
         // the keys that it sees, so what others see does not change its bits.
-        float size[2] = {0.f, 0.f};  // largest scale of this lane's keys; infinities and NaNs lose their own group only
+        float size[kHalves][2] = {};  // largest scale of this lane's keys; infinities and NaNs lose their own group only
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          if (fabsf(fa[g]) < INFINITY) size[0] = fmaxf(size[0], fabsf(fa[g]));
-          if (fabsf(fb[g]) < INFINITY) size[1] = fmaxf(size[1], fabsf(fb[g]));
-        }
+        for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            const float x = fabsf(va[h].get(g)), y = fabsf(vb[h].get(g));
+            if (x < INFINITY) size[h][0] = fmaxf(size[h][0], x);
+            if (y < INFINITY) size[h][1] = fmaxf(size[h][1], y);
+          }
         int least = 127;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -390,26 +409,24 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 128 ? 3 : 4 : 2
           for (int x = 0; x < 2; ++x) {
             float most = kNoTop, big = 0.f;
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              if constexpr (EDGE) {
-                if (!sees[n][x + 2 * y]) continue;
+            for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+              for (int y = 0; y < 2; ++y) {
+                if (EDGE && !sees(h, n, x + 2 * y)) continue;
+                most = fmaxf(most, s[h][n][x + 2 * y] * row_scale[n][x]);
+                big = fmaxf(big, size[h][y]);
               }
-              most = fmaxf(most, s[n][x + 2 * y] * row_scale[n][x]);
-              big = fmaxf(big, size[y]);
-            }
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) {
               most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
               big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
             }
-            const float was = top[n][x];
-            const int sigma_was = sigma[n][x];
-            if (most > was + 8.f) top[n][x] = ceilf(most);
-            sigma[n][x] = min(max(sigma_was, (int)(__float_as_uint(big) >> 23) - 126), 127);
-            least = min(least, sigma[n][x]);
-            from[n][x] = top[n][x] + (float)(sigma[n][x] - 7);
-            over[n][x] = power_of_two(min(15 - sigma[n][x], 127));
-            const float f = exp2_approx(fmaxf(was - top[n][x], -300.f) + (float)(sigma_was - sigma[n][x]));
+            const int sigma_was = sigma_of(over[n][x]), sigma = min(max(sigma_was, (int)(__float_as_uint(big) >> 23) - 126), 127);
+            const float was = from[n][x] - (float)(sigma_was - 7), top = most > was + 8.f ? ceilf(most) : was;
+            least = min(least, sigma);
+            from[n][x] = top + (float)(sigma - 7);
+            over[n][x] = power_of_two(15 - sigma);
+            const float f = exp2_approx(fmaxf(was - top, -300.f) + (float)(sigma_was - sigma));
             sum[n][x] *= f;
 #pragma unroll
             for (int g = 0; g < G; ++g)
@@ -420,60 +437,64 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 128 ? 3 : 4 : 2
                 eights[n][g][2 * r + x] *= f;
               }
 #pragma unroll
-            for (int y = 0; y < 2; ++y)
-              w[n][x + 2 * y] = exp2_approx(fmaf(s[n][x + 2 * y], row_scale[n][x], -from[n][x]));
+            for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+              for (int y = 0; y < 2; ++y)
+                w[h][n][x + 2 * y] = exp2_approx(fmaf(s[h][n][x + 2 * y], row_scale[n][x], -from[n][x]));
           }
         limit = power_of_two(least);
       }
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int h = 0; h < kHalves; ++h) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          if constexpr (EDGE) {
-            if (!sees[n][x]) w[n][x] = 0.f;
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            if (EDGE && !sees(h, n, x)) w[h][n][x] = 0.f;
+            sum[n][x & 1] += w[h][n][x];
           }
-          sum[n][x & 1] += w[n][x];
-        }
-
-      // Channels of this lane: words j % 4 of the four keys, even or odd ones.
-      uint32_t w0[G], w1[G], w8[G], w9[G];
-      load_words<G>(w0, here + v_at[0]);
-      load_words<G>(w1, here + v_at[1]);
-      load_words<G>(w8, here + v_at[0] + kEight);
-      load_words<G>(w9, here + v_at[1] + kEight);
+        // Channels of this lane: words j % 4 of the four keys, even or odd ones.
+        const uint32_t at_half = here + h * S::kBytes;
+        uint32_t w0[G], w1[G], w8[G], w9[G];
+        load_words<G>(w0, at_half + v_at[0]);
+        load_words<G>(w1, at_half + v_at[1]);
+        load_words<G>(w8, at_half + v_at[0] + kEight);
+        load_words<G>(w9, at_half + v_at[1] + kEight);
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const uint32_t x = __byte_perm(w0[g], w1[g], half_of), y = __byte_perm(w8[g], w9[g], half_of);
-        const uint32_t x8 = x >> 8, y8 = y >> 8;
+        for (int g = 0; g < G; ++g) {
+          const uint32_t x = __byte_perm(w0[g], w1[g], half_of), y = __byte_perm(w8[g], w9[g], half_of);
+          const uint32_t x8 = x >> 8, y8 = y >> 8;
+          const float fa = va[h].get(g), fb = vb[h].get(g);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float z[4];
+          for (int n = 0; n < NT; ++n) {
+            float z[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            z[i] = w[n][i] * (i < 2 ? fa[g] : fb[g]);
-            if constexpr (EDGE) {
-              if (!sees[n][i]) z[i] = 0.f;  // whatever the scale is
+            for (int i = 0; i < 4; ++i) {
+              z[i] = w[h][n][i] * (i < 2 ? fa : fb);
+              if (EDGE && !sees(h, n, i)) z[i] = 0.f;  // whatever the scale is
             }
+            const uint32_t w_lo = transposed(half2_of(z[0], z[1])), w_hi = transposed(half2_of(z[2], z[3]));
+            float (&o0)[4] = acc[n][g][0], (&o1)[4] = acc[n][g][1], (&e)[4] = eights[n][g];
+            mma_f16(o0, x & kLow, x & kHigh, y & kLow, y & kHigh, w_lo, w_hi, o0[0], o0[1], o0[2], o0[3]);
+            mma_f16(o1, x8 & kLow, x8 & kHigh, y8 & kLow, y8 & kHigh, w_lo, w_hi, o1[0], o1[1], o1[2], o1[3]);
+            mma_f16(e, 0x00080008u, 0x00800080u, 0x00080008u, 0x00800080u, w_lo, w_hi, e[0], e[1], e[2], e[3]);
           }
-          const uint32_t w_lo = transposed(half2_of(z[0], z[1])), w_hi = transposed(half2_of(z[2], z[3]));
-          float (&o0)[4] = acc[n][g][0], (&o1)[4] = acc[n][g][1], (&e)[4] = eights[n][g];
-          mma_f16(o0, x & kLow, x & kHigh, y & kLow, y & kHigh, w_lo, w_hi, o0[0], o0[1], o0[2], o0[3]);
-          mma_f16(o1, x8 & kLow, x8 & kHigh, y8 & kLow, y8 & kHigh, w_lo, w_hi, o1[0], o1[1], o1[2], o1[3]);
-          mma_f16(e, 0x00080008u, 0x00800080u, 0x00080008u, 0x00800080u, w_lo, w_hi, e[0], e[1], e[2], e[3]);
         }
       }
     };
 #pragma unroll
     for (int s = 0; s < kRing - 1; ++s) load(s);
 
+    uint32_t here = ring;
     for (int step = 0; step < steps; ++step) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
       __syncwarp();
       load(step + kRing - 1);
       const int key = step * kBlockKeys;
-      const uint32_t here = ring + step % kRing * S::kBytes;
-      if (key >= all_lo && key + kWarpKeys - 1 <= all_hi) compute(std::false_type{}, here, key);
-      else if (key < key_hi && key + kWarpKeys > key_lo) compute(std::true_type{}, here, key);
+      if (key >= all_lo && key + kStepKeys - 1 <= all_hi) compute(std::false_type{}, here, key);
+      else if (key < key_hi && key + kStepKeys > key_lo) compute(std::true_type{}, here, key);
+      here += kStage;
+      if (here == ring_end) here = ring;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
@@ -489,9 +510,10 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 128 ? 3 : 4 : 2
         l += __shfl_xor_sync(0xffffffffu, l, 8);
         l += __shfl_xor_sync(0xffffffffu, l, 16);
         const int row = 8 * n + 2 * p + x;
-        const float down = power_of_two(sigma[n][x] - 7);
+        const int sigma = sigma_of(over[n][x]);
+        const float down = power_of_two(sigma - 7), top = from[n][x] - (float)(sigma - 7);
         if (j == 0) {
-          stat[warp][row][0] = top[n][x] == kNoTop ? -INFINITY : top[n][x];
+          stat[warp][row][0] = top == kNoTop ? -INFINITY : top;
           stat[warp][row][1] = l * down;
         }
 #pragma unroll
@@ -545,9 +567,9 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 128 ? 3 : 4 : 2
 template <typename T, int D, int NT, int HEADS>
 cudaError_t launch(Int4Args args, cudaStream_t stream) {
   AttentionArgs& a = args.a;
-  constexpr int kRows = 8 * NT, kBlockKeys = kWarpKeys * kDecodeWarps / HEADS;
+  constexpr int kRows = 8 * NT, kBlockKeys = kStepKeys * kDecodeWarps / HEADS;
   a.whole = a.max_keys <= kWholeKeys / HEADS;
-  constexpr size_t ring = (size_t)kDecodeWarps * kRing * Step<D>::kBytes, joined = (size_t)kDecodeWarps * kRows * D * 4;
+  constexpr size_t ring = (size_t)kDecodeWarps * kRing * kHalves * Half<D>::kBytes, joined = (size_t)kDecodeWarps * kRows * D * 4;
   constexpr size_t smem = ring > joined ? ring : joined;
   const void* fn = reinterpret_cast<const void*>(&paged_int4_decode_kernel<T, D, NT, HEADS>);
   cudaError_t err = allow_shared_memory(fn, smem);
