@@ -25,8 +25,8 @@ __device__ __forceinline__ float int4_scale(float high, float low) {
   float s = -0.125f * (high >= -low ? high : low);
   s = __int_as_float(__float_as_int(s) & ~0x7ffff);
   constexpr bool kHalf = std::is_same<T, __half>::value;
-  // FP16: s * code inside its range, and no bit of it below 2^-24. BF16: 1 / s is a normal number.
-  const float size = fminf(fmaxf(fabsf(s), kHalf ? 0x1p-20f : 0x1p-100f), kHalf ? 7936.f : 0x1p126f);
+  // FP16: s * code inside its range, and no bit of it below 2^-24. BF16: 1 / s and 24 s are normal numbers.
+  const float size = fminf(fmaxf(fabsf(s), kHalf ? 0x1p-20f : 0x1p-100f), kHalf ? 7936.f : 0x1p122f);
   const float kept = s == 0.f ? 0.f : copysignf(size, s);
   return high - high == 0.f && low - low == 0.f ? kept : __int_as_float(0x7fc00000);
 }

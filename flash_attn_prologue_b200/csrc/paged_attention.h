@@ -80,8 +80,9 @@ PrefillPlan plan_paged_prefill(int64_t tokens, int64_t batch, bool ragged, int64
                                int64_t max_keys, int64_t window, int sms);
 // False where the cache's layout has no tensor map (the other kernel reads it). wait_cycles: 0, or
 // (self-test, BF16) the limit of the kernel's waits, but for those for copies and products under way.
-bool launch_paged_prefill(const AttentionArgs& a, const PrefillPlan& plan, int dtype, int D, int64_t page_size,
-                          long long wait_cycles, cudaStream_t stream, cudaError_t* err);
+// scales: null, or the cache is one of 4 bits (a.k, a.v: codes, strides in bytes).
+bool launch_paged_prefill(const AttentionArgs& a, const PrefillPlan& plan, const flash_prologue_scales* scales, int dtype,
+                          int D, int64_t page_size, long long wait_cycles, cudaStream_t stream, cudaError_t* err);
 cudaError_t launch_paged_decode(const AttentionArgs& a, int dtype, int D, cudaStream_t stream);
 // The same over a cache of 4 bits (a.k, a.v: codes, strides in bytes).
 size_t paged_int4_decode_workspace(int D, int sms);

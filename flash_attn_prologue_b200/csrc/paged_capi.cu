@@ -43,7 +43,10 @@ bool use_prefill(const flash_prologue_attention_args* a, float scale_log2) {
   return a->tokens * group > 16 * a->cache.batch && group <= 128 && scale_log2 >= FLT_MIN;
 }
 
-size_t int4_workspace_of(int64_t D, int sms) { return paged_int4_decode_workspace((int)D, sms); }
+size_t int4_workspace_of(int64_t D, int sms) {
+  const size_t decode = paged_int4_decode_workspace((int)D, sms), prefill = paged_prefill_workspace((int)D, sms);
+  return prefill > decode ? prefill : decode;
+}
 
 size_t workspace_of(int64_t D, int sms) {
   const size_t decode = paged_decode_workspace((int)D, sms), prefill = paged_prefill_workspace((int)D, sms);
@@ -99,19 +102,19 @@ int attention(const flash_prologue_attention_args* a, const flash_prologue_scale
   g.workspace = a->workspace;
   g.max_keys = (int)(c.max_pages * c.page_size);
   g.window = a->window < g.max_keys ? (int)a->window : 0;  // as long as any request: all keys
-  if (scales)
-    return launch_paged_int4_decode(g, *scales, (int)a->dtype, (int)a->D, static_cast<cudaStream_t>(stream)) == cudaSuccess
-               ? FLASH_PROLOGUE_OK
-               : FLASH_PROLOGUE_ERR_CUDA;
   if (use_prefill(a, g.scale_log2)) {
     const PrefillPlan plan = plan_paged_prefill(a->tokens, c.batch, c.cu_seqlens != nullptr, a->Hk, g.group, (int)a->D,
                                                 g.max_keys, g.window, sms);
     cudaError_t err = cudaSuccess;
-    if (launch_paged_prefill(g, plan, (int)a->dtype, (int)a->D, c.page_size,
+    if (launch_paged_prefill(g, plan, scales, (int)a->dtype, (int)a->D, c.page_size,
                              wait_cycles, static_cast<cudaStream_t>(stream), &err))
       return err == cudaSuccess ? FLASH_PROLOGUE_OK : FLASH_PROLOGUE_ERR_CUDA;
   }
   if (wait_cycles) return FLASH_PROLOGUE_ERR_UNSUPPORTED;
+  if (scales)
+    return launch_paged_int4_decode(g, *scales, (int)a->dtype, (int)a->D, static_cast<cudaStream_t>(stream)) == cudaSuccess
+               ? FLASH_PROLOGUE_OK
+               : FLASH_PROLOGUE_ERR_CUDA;
   return launch_paged_decode(g, (int)a->dtype, (int)a->D, static_cast<cudaStream_t>(stream)) == cudaSuccess
              ? FLASH_PROLOGUE_OK
              : FLASH_PROLOGUE_ERR_CUDA;
@@ -150,10 +153,18 @@ int flash_prologue_paged_attention_int4(const flash_prologue_attention_args* a, 
   return scales ? attention(a, scales, 0, stream) : FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
 }
 
-int flash_prologue_selftest_attention_waits(const flash_prologue_attention_args* a, int64_t wait_cycles, void* stream) {
+static int attention_waits(const flash_prologue_attention_args* a, const flash_prologue_scales* scales, int64_t wait_cycles,
+                           void* stream) {
   if (!a || wait_cycles < 1 || wait_cycles > (int64_t(1) << 33)) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
   if (a->dtype != FLASH_PROLOGUE_BF16) return FLASH_PROLOGUE_ERR_UNSUPPORTED;
-  return attention(a, nullptr, wait_cycles, stream);
+  return attention(a, scales, wait_cycles, stream);
+}
+int flash_prologue_selftest_attention_waits(const flash_prologue_attention_args* a, int64_t wait_cycles, void* stream) {
+  return attention_waits(a, nullptr, wait_cycles, stream);
+}
+int flash_prologue_selftest_attention_int4_waits(const flash_prologue_attention_args* a, const flash_prologue_scales* scales,
+                                                 int64_t wait_cycles, void* stream) {
+  return scales ? attention_waits(a, scales, wait_cycles, stream) : FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
 }
 
 }  // extern "C"

@@ -54,6 +54,7 @@ namespace {
 constexpr int kTile = 128;             // rows of a tile
 constexpr int kKeys = 64;              // keys of a block
 constexpr int kPrefillThreads = 256;
+constexpr int kInt4Threads = kPrefillThreads + 128;  // four more warps turn codes into values
 constexpr int kRowThreads = 128;
 constexpr int kTmemCols = 256;
 
@@ -91,7 +92,7 @@ struct Barriers {
   uint64_t s_full[2], s_read[2], p_full[2], o_done[2], clean_ask, v_clean, drain[2];
   uint64_t q_full, q_empty, work_full[2], work_empty[2], next_here;
   uint32_t tmem;
-  int sums[kPrefillThreads / 32];
+  int sums[kInt4Threads / 32];
   int found, found_start;  // request of the CTA's first tile (-1: none), tiles before it
   Work work[2];            // the tile that the warps are at and the next
   // Where a wait ran out: the tiles that were put into work, and one that was taken over and not put there.
@@ -115,6 +116,10 @@ struct PrefillArgs {
   float* part_stat;      // [...][128][2]
   Tile* joins;           // [cut items]
   long long wait_cycles; // self-test: limit of a wait
+  // A cache of 4 bits (a.k, a.v: codes, strides in bytes): its scales, strides in elements.
+  const uint16_t* k_scale;
+  const uint16_t* v_scale;
+  int64_t ks_page, ks_slot, ks_head, vs_page, vs_slot, vs_head;
 };
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3,
@@ -279,8 +284,43 @@ __device__ __noinline__ void void_row(const PrefillArgs& p, const Work& w, int r
   if (p.a.lse) p.a.lse[(int64_t)token * p.a.heads + h] = nan;
 }
 
-template <typename T, int D, bool kSelfTest = false>
-__global__ void __launch_bounds__(kPrefillThreads, 2)
+// The two 16-bit values s * (u - 8) of codes u at bits 4 i and 16 + 4 i of a word, exactly. BF16: u goes
+// next to the exponent of 16, and (16 + u) s - 24 s has no rounding, since s has five significant
+// bits. FP16, where 24 s may be beyond its range: 1024 + u (or 16 u) less 1032, times s.
+template <typename T>
+__device__ __forceinline__ void int4_values(uint32_t word, uint32_t s, uint32_t s24, uint32_t (&out)[4]) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const auto h2 = [](uint32_t x) { return *reinterpret_cast<__half2*>(&x); };
+    const uint32_t low = 0x000f000fu, high = 0x00f000f0u, big = 0x64006400u, w8 = word >> 8;
+    const __half2 eight = __float2half2_rn(-1032.f), part = __float2half2_rn(0.0625f), sixteen = __float2half2_rn(-72.f);
+    const __half2 v[4] = {__hadd2(h2(word & low | big), eight), __hfma2(h2(word & high | big), part, sixteen),
+                          __hadd2(h2(w8 & low | big), eight), __hfma2(h2(w8 & high | big), part, sixteen)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 x = __hmul2(v[i], h2(s));
+      out[i] = *reinterpret_cast<const uint32_t*>(&x);
+    }
+  } else {
+    const auto b2 = [](uint32_t x) { return *reinterpret_cast<__nv_bfloat162*>(&x); };
+    const uint32_t at[4] = {word << 3, word >> 1, word >> 5, word >> 9};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 x = __hfma2(b2(at[i] & 0x00780078u | 0x41804180u), b2(s), b2(s24));
+      out[i] = *reinterpret_cast<const uint32_t*>(&x);
+    }
+  }
+}
+
+template <int N>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+// 384 threads at 80 registers each, split among the three warpgroups.
+constexpr int kRowRegisters = 120, kIssueRegisters = 56, kCodeRegisters = 64;
+static_assert(kRowRegisters + kIssueRegisters + kCodeRegisters == 3 * 80, "registers of a CTA");
+
+template <typename T, int D, bool kSelfTest = false, bool kInt4 = false>
+__global__ void __launch_bounds__(kInt4 ? kInt4Threads : kPrefillThreads, 2)
     paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                          const __grid_constant__ CUtensorMap v_map, const __grid_constant__ PrefillArgs p) {
   using L = Layout<D>;
@@ -303,9 +343,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
   const int requests = requests_of(a.pages);
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::kStages; ++s) {
-      mbar_init(&bar.k_full[s], 1);
+      mbar_init(&bar.k_full[s], kInt4 ? 4 : 1);
       mbar_init(&bar.k_empty[s], 1);
-      mbar_init(&bar.v_full[s], 1);
+      mbar_init(&bar.v_full[s], kInt4 ? 4 : 1);
       mbar_init(&bar.v_empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -314,7 +354,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       mbar_init(&bar.p_full[b], kRowThreads / 32);
       mbar_init(&bar.o_done[b], 1);
       mbar_init(&bar.work_full[b], 1);
-      mbar_init(&bar.work_empty[b], kRowThreads / 32 + 3);
+      mbar_init(&bar.work_empty[b], kRowThreads / 32 + (kInt4 ? 6 : 3));
       mbar_init(&bar.drain[b], 1);
     }
     mbar_init(&bar.clean_ask, 1);
@@ -335,7 +375,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
   int all_tiles = 0;
   {
     const int tile = tile_at(blockIdx.x);
-    for (int r0 = 0; r0 < requests; r0 += kPrefillThreads) {
+    constexpr int kThreadsHere = kInt4 ? kInt4Threads : kPrefillThreads;
+    for (int r0 = 0; r0 < requests; r0 += kThreadsHere) {
       const int r = r0 + threadIdx.x;
       Request q{0, 0, 0};
       bool too_long;
@@ -351,7 +392,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
       __syncthreads();
       int start = all_tiles + upto - n;
 #pragma unroll
-      for (int w = 0; w < kPrefillThreads / 32; ++w) {
+      for (int w = 0; w < kThreadsHere / 32; ++w) {
         if (w < warp) start += bar.sums[w];
         all_tiles += bar.sums[w];
       }
@@ -382,326 +423,456 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
     if (lane == 0) mbar_arrive(&bar.work_empty[t & 1]);
   };
 
-  if (warp == 4) {
-    // ---------------- scores ----------------
-    // The issuing warps walk the blocks whole, with values the compiler knows to be the same
-    // in all lanes, and one lane issues. Each has one product: a warp that issued both, with
-    // its waits, took longer for a block than its softmax does.
-    constexpr uint32_t idesc = idesc_of<T>(kKeys, false);
-    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-    const uint64_t q_desc = smem_desc_k_sw128(smem_u32(q_s));
-    bool ok = true;
-    uint32_t queries = 0;
-    for (uint32_t t = 0; ok; ++t) {
-      if (!(ok = next_work(t))) break;
-      const Work& w = bar.work[t & 1];
-      const int n = __shfl_sync(0xffffffffu, w.blocks, 0);
-      if (w.rows < 0) break;
-      if (n) ok = __all_sync(0xffffffffu, wait_for(&bar.q_full, queries++ & 1));
-      for (int j = 0; j < n && ok; ++j, ++g) {
-        const uint32_t s = g % L::kStages, b = g % L::kScores;
-        // The last scores of this buffer are in the rows' registers, K is here.
-        if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.s_read[b], ((g / L::kScores) & 1) ^ 1) &&
-                                               wait_for(&bar.k_full[s], (g / L::kStages) & 1))))
-          break;
-        tc_fence_after();
-        const uint64_t k_desc = smem_desc_k_sw128(smem_u32(k_s) + s * L::kBlock);
-        if (elect_one()) {
-#pragma unroll
-          for (int h = 0; h < L::kHalves; ++h)
-#pragma unroll
-            for (int c = 0; c < 4; ++c)  // 16 columns (32 bytes) a step
-              umma_bf16(tm + L::kSCol + b * kKeys, q_desc + h * (L::kQHalf / 16) + 2 * c,
-                        k_desc + h * (L::kHalf / 16) + 2 * c, idesc, (h | c) != 0);
-          umma_commit(&bar.k_empty[s]);
-          umma_commit(&bar.s_full[b]);
-          if (j == n - 1) umma_commit(&bar.q_empty);
-        }
-        __syncwarp();
-      }
-      done_with(t);
-    }
-    // Neither tensor memory nor the tiles are released under products still running.
-    if (elect_one()) umma_commit(&bar.drain[0]);
-    drain(&bar.drain[0], 0);
-  } else if (warp == 6) {
-    // ---------------- output ----------------
-    constexpr uint32_t idesc = idesc_of<T>(D, true);
-    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-    bool ok = true;
-    uint32_t cleaned = 0;
-    for (uint32_t t = 0; ok; ++t) {
-      if (!(ok = next_work(t))) break;
-      const Work& w = bar.work[t & 1];
-      const int n = __shfl_sync(0xffffffffu, w.blocks, 0), full0 = __shfl_sync(0xffffffffu, w.full0, 0),
-                full1 = __shfl_sync(0xffffffffu, w.full1, 0);
-      if (w.rows < 0) break;
-      for (int j = 0; j < n; ++j, ++g) {
-        const uint32_t s = g % L::kStages;
-        ok = wait_for(&bar.v_full[s], (g / L::kStages) & 1);
-        const bool partial = j < full0 || j >= full1;
-        if (partial && lane == 0) mbar_arrive(&bar.clean_ask);  // cleaned beside the block's softmax
-        ok = ok && (!partial || wait_for(&bar.v_clean, cleaned & 1)) && wait_for(&bar.p_full[g & 1], (g >> 1) & 1);
-        cleaned += partial;
-        if (!(ok = __all_sync(0xffffffffu, ok))) break;
-        tc_fence_after();
-        const uint64_t v_desc = smem_desc_mn_sw128(smem_u32(v_s) + s * L::kBlock, L::kHalf);
-        if (elect_one()) {
-#pragma unroll
-          for (int c = 0; c < kKeys / 16; ++c)  // 16 keys a step: 8 columns of P, two 8-row groups of V (2,048 bytes)
-            umma_ts(tm + L::kOCol, tm + L::kPCol + (g & 1) * (kKeys / 2) + 8 * c, v_desc + 128 * c, idesc, (j | c) != 0);
-          umma_commit(&bar.v_empty[s]);
-          umma_commit(&bar.o_done[g & 1]);
-        }
-        __syncwarp();
-      }
-      done_with(t);
-    }
-    if (elect_one()) umma_commit(&bar.drain[1]);
-    drain(&bar.drain[1], 0);
-  } else if (warp == 5) {
-    // ---------------- tiles and loads ----------------
-    const int in_page = (1 << a.pages.page_log2) - 1, boxes = kKeys / p.box_rows;
-    const uint32_t box_bytes = (uint32_t)p.box_rows * 128;
-    // The last tile's request: `r` with `before` tiles of others in front of it.
-    int r = requests, before = all_tiles;
-    Request q{0, 0, 0};
-    bool too_long = false;
-    if (bar.found >= 0) {
-      r = bar.found;
-      before = bar.found_start;
-      q = request_at(a.pages, a.tokens, a.max_keys, r, &too_long);
-    }
-    // The work of CTA `index`; false where it has none.
-    const auto describe = [&](int index, Work& w) {
-      const int cut = index - p.whole_items, splits = cut < 0 ? 1 : p.splits, split = cut < 0 ? 0 : cut % p.splits;
-      const int item = cut < 0 ? index : p.whole_items + cut / p.splits, tile = tile_at(index);
-      if (tile >= before + tiles_of(q)) {  // not before the last one: from the end
-        r = requests;
-        before = all_tiles;
-        q = Request{0, 0, 0};
-      }
-      while (tile < before && r > 0) {  // 32 requests back
-        const int at = r - 1 - lane;
-        Request mine{0, 0, 0};
-        bool over = false;
-        if (at >= 0) mine = request_at(a.pages, a.tokens, a.max_keys, at, &over);
-        const int n = tiles_of(mine);
-        int upto = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int v = __shfl_up_sync(0xffffffffu, upto, o);
-          if (lane >= o) upto += v;
-        }
-        const uint32_t here = __ballot_sync(0xffffffffu, tile >= before - upto && tile < before - upto + n);
-        const int src = here ? __ffs(here) - 1 : 31;
-        r = here ? r - 1 - src : max(r - 32, 0);
-        before -= __shfl_sync(0xffffffffu, upto, src);
-        q.first = __shfl_sync(0xffffffffu, mine.first, src);
-        q.news = here ? __shfl_sync(0xffffffffu, mine.news, src) : 0;
-        q.total = __shfl_sync(0xffffffffu, mine.total, src);
-        too_long = __shfl_sync(0xffffffffu, (int)over, src);
-        if (here) break;
-      }
-      Tile* join = splits > 1 && split == 0 && lane == 0 ? p.joins + (item - p.whole_items) : nullptr;
-      if (tile < before || tile >= before + tiles_of(q)) {  // the grid has room for more tiles than there are
-        if (join) join->parts = 0;
-        return false;
-      }
-      const int token0 = (tile - before) * p.tile_tokens, tokens = min(p.tile_tokens, q.news - token0);
-      w.r = r;
-      w.head = item % a.kv_heads;
-      w.first_token = q.first + token0;
-      w.rows = tokens * a.group;
-      w.pos0 = q.total - q.news + token0;
-      w.pos1 = w.pos0 + tokens - 1;
-      w.hi = max(w.pos1 + 1, 0);
-      w.lo = a.window ? max(w.pos0 - a.window + 1, 0) : 0;
-      const int first = w.lo / kKeys, blocks = max((w.hi + kKeys - 1) / kKeys - first, 0);
-      // Shares of at least four blocks: a share's fixed cost is about theirs.
-      int share = blocks;
-      if (splits > 1) share = max((blocks + splits - 1) / splits, 4);
-      w.parts = blocks && splits > 1 ? (blocks + share - 1) / share : 1;
-      w.first = first + split * share;
-      w.blocks = max(min(first + blocks, w.first + share) - w.first, 0);
-      w.full0 = a.window ? max((max(w.pos1 - a.window + 1, 0) + kKeys - 1) / kKeys - w.first, 0) : 0;
-      w.full1 = (w.pos0 + 1) / kKeys - w.first;
-      w.share = cut;
-      w.bad = too_long;
-      w.wild = 0;
-      if (join) {
-        join->token0 = w.first_token;
-        join->rows = w.rows;
-        join->kv_head = w.head;
-        join->parts = w.parts;
-      }
-      return split < w.parts;
+  if (kInt4 && warp >= 8) {
+    fewer_registers<kCodeRegisters>();
+    // ---------------- codes to values ----------------
+    // A thread has a key of the block and half its words (D = 128: all of a 64-column half), loads them
+    // a block ahead and writes them as the tensor maps of a 16-bit cache would: rows of 128 bytes,
+    // 16-byte pieces swizzled by the row.
+    constexpr int G = D / 32, kWords = D / 16;
+    const int key_row = threadIdx.x & 63, part = (threadIdx.x >> 6) & 1;
+    const int in_page = (1 << a.pages.page_log2) - 1;
+    unsigned char* const to = k_s + (D == 128 ? part * L::kHalf : 0) + key_row * 128;
+    const int swizzle = key_row & 7, piece0 = D == 128 ? 0 : 4 * part;
+    struct Codes {
+      uint32_t w[kWords];
+      uint32_t s[G / 2];
     };
-    // This lane has a box of the block to load.
-    const auto has_box = [&](const Work& w, int j) {
-      const int key = (w.first + j) * kKeys + lane * p.box_rows;
-      return lane < boxes && j < w.blocks && key < w.hi && key + p.box_rows > w.lo;
-    };
-    // Its entry of the page table, read a block ahead and checked when the box is loaded (-1: nothing to load).
-    const auto entry_of = [&](const Work& w, int j) {
-      const int key = (w.first + j) * kKeys + lane * p.box_rows;
-      return has_box(w, j) ? __ldg(a.pages.page_table + w.r * a.pages.table_stride + (key >> a.pages.page_log2)) : -1;
-    };
-    const auto page_of = [&](const Work& w, int j, int entry, int* bad) {
-      if (!has_box(w, j)) return -1;
-      if (entry >= 0 && entry < a.pages.num_pages) return entry;
-      *bad = 1;
-      return -1;
-    };
-    const auto load = [&](const Work& w, int j, int page, const CUtensorMap* map, unsigned char* ring, uint64_t* full) {
-      const uint32_t s = g % L::kStages, count = __popc(__ballot_sync(0xffffffffu, page >= 0));
-      if (lane == 0) mbar_arrive_expect_tx(&full[s], count * box_bytes * L::kHalves);
-      __syncwarp();
-      if (page >= 0) {
-        const int key = (w.first + j) * kKeys + lane * p.box_rows;
-        const uint32_t dst = smem_u32(ring) + s * L::kBlock + lane * box_bytes;
-#pragma unroll
-        for (int h = 0; h < L::kHalves; ++h)
-          tma_load_4d(dst + h * L::kHalf, map, h * 64, key & in_page, w.head, page, &full[s]);
-      }
-      __syncwarp();
-    };
-    const auto leave = [&](const Work& w) {
-      if (lane == 0) {
-        bar.left = w;
-        bar.has_left = 1;
-      }
-    };
-    bool ok = true, asking = false;
-    uint32_t t = 0, queries = 0, asked = 0;
-    uint32_t k_loads = 0, v_loads = 0, q_loads = 0;  // begun
-    for (int index = blockIdx.x; index >= 0;) {
-      Work w;
-      if (describe(index, w)) {
-        Work& slot = bar.work[t & 1];
-        int entry = entry_of(w, 0);
-        if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.work_empty[t & 1], ((t >> 1) & 1) ^ 1)))) {
-          leave(w);
-          break;
-        }
-        if (lane == 0) {
-          slot = w;
-          mbar_arrive(&bar.work_full[t & 1]);
-        }
-        __syncwarp();
-        ++t;
-        for (int j = 0; j < w.blocks; ++j, ++g) {
-          const uint32_t s = g % L::kStages, parity = ((g / L::kStages) & 1) ^ 1;
-          const int page = page_of(w, j, entry, &slot.bad);
-          entry = entry_of(w, j + 1);
-          if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.k_empty[s], parity)))) break;
-          load(w, j, page, &k_map, k_s, bar.k_full);
-          ++k_loads;
-          if (j == 0) {
-            // The last tile's scores have been computed: its Q can go.
-            if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.q_empty, (queries & 1) ^ 1)))) break;
-            ++queries;
-            if (lane == 0) {
-              mbar_arrive_expect_tx(&bar.q_full, p.tile_tokens * a.group * 128 * L::kHalves);
-#pragma unroll
-              for (int h = 0; h < L::kHalves; ++h)
-                tma_load_3d(smem_u32(q_s) + h * L::kQHalf, &q_map, h * 64, w.head * a.group, w.first_token, &bar.q_full);
-            }
-            __syncwarp();
-            ++q_loads;
-          }
-          if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.v_empty[s], parity)))) break;
-          load(w, j, page, &v_map, v_s, bar.v_full);
-          ++v_loads;
-        }
-        if (!ok) break;
-      }
-      // Asked for late, while the last blocks are computed, so that an idle CTA is not left without.
-      if (lane == 0) {
-        fence_proxy_async_smem();  // the last answer has been read
-        mbar_arrive_expect_tx(&bar.next_here, 16);
-        ask_next_cta(answer, &bar.next_here);
-      }
-      __syncwarp();
-      asking = true;
-      if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.next_here, asked++ & 1)))) break;
-      asking = false;
-      index = __shfl_sync(0xffffffffu, next_cta(answer), 0);
-    }
-    if (lane == 0) bar.posted = t;
-    if (ok) {
-      ok = __all_sync(0xffffffffu, wait_for(&bar.work_empty[t & 1], ((t >> 1) & 1) ^ 1));
-      if (ok && lane == 0) {
-        bar.work[t & 1].rows = -1;
-        bar.work[t & 1].blocks = 0;
-        mbar_arrive(&bar.work_full[t & 1]);
-      }
-      __syncwarp();
-      // No product's arrival on an empty barrier lands after the CTA has gone.
-      for (uint32_t e = g; e < g + L::kStages && ok; ++e) {
-        const uint32_t s = e % L::kStages, parity = ((e / L::kStages) & 1) ^ 1;
-        ok = __all_sync(0xffffffffu, wait_for(&bar.k_empty[s], parity) && wait_for(&bar.v_empty[s], parity));
-      }
-      if (ok) ok = __all_sync(0xffffffffu, wait_for(&bar.q_empty, (queries & 1) ^ 1));
-    }
-    if (!ok) {
-      // A wait ran out: what is still on its way to shared memory has to arrive. A tile that does is not computed.
-      if (asking && __all_sync(0xffffffffu, drain(&bar.next_here, (asked - 1) & 1))) {
-        const int index = __shfl_sync(0xffffffffu, next_cta(answer), 0);
-        Work w;
-        if (index >= 0 && describe(index, w)) leave(w);
-      }
-      if (q_loads) drain(&bar.q_full, (q_loads - 1) & 1);
-      for (uint32_t back = 1; back <= L::kStages; ++back) {
-        if (k_loads >= back) drain(&bar.k_full[(k_loads - back) % L::kStages], ((k_loads - back) / L::kStages) & 1);
-        if (v_loads >= back) drain(&bar.v_full[(v_loads - back) % L::kStages], ((v_loads - back) / L::kStages) & 1);
-      }
-    }
-  } else if (warp == 7) {
-    // ---------------- cleaning ----------------
-    uint32_t asked = 0;
     bool ok = true;
     for (uint32_t t = 0; ok; ++t) {
       if (!(ok = next_work(t))) break;
       Work& w = bar.work[t & 1];
       if (w.rows < 0) break;
-      const int n = w.blocks, full0 = w.full0, full1 = w.full1;
+      const int n = w.blocks, full0 = w.full0, full1 = w.full1, first = w.first, hi = w.hi, lo = w.lo, head = w.head;
+      const int32_t* table = a.pages.page_table + (int64_t)w.r * a.pages.table_stride;
+      // The page of this thread's key in block j: -1 where it has none that counts.
+      const auto page_at = [&](int j) {
+        const int key = (first + j) * kKeys + key_row;
+        if (j >= n || key < lo || key >= hi) return -1;
+        const int page = __ldg(table + (key >> a.pages.page_log2));
+        if (page >= 0 && page < a.pages.num_pages) return page;
+        w.bad = 1;
+        return -1;
+      };
+      const auto fetch = [&](Codes& c, int j, int page, const void* codes, int64_t c_page, int64_t c_slot, int64_t c_head,
+                             const uint16_t* scales, int64_t s_page, int64_t s_slot, int64_t s_head) {
+        const int slot = ((first + j) * kKeys + key_row) & in_page;
+#pragma unroll
+        for (int i = 0; i < G / 2; ++i) c.s[i] = 0;  // zeros
+        if (page < 0) return;
+        const uint4* from = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(codes) + page * c_page + slot * c_slot +
+                                                           head * c_head + part * (kWords * 4));
+#pragma unroll
+        for (int i = 0; i < kWords / 4; ++i) {
+          const uint4 x = __ldg(from + i);
+          c.w[4 * i] = x.x; c.w[4 * i + 1] = x.y; c.w[4 * i + 2] = x.z; c.w[4 * i + 3] = x.w;
+        }
+        const uint16_t* s = scales + page * s_page + slot * s_slot + head * s_head;
+        if constexpr (G == 4) {
+          const uint2 x = __ldg(reinterpret_cast<const uint2*>(s));
+          c.s[0] = x.x; c.s[1] = x.y;
+        } else {
+          c.s[0] = __ldg(reinterpret_cast<const uint32_t*>(s));
+        }
+      };
+      const auto put = [&](const Codes& c, unsigned char* dst) {
+        uint32_t s2[G], s24[G];
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+          const uint32_t s = i & 1 ? c.s[i / 2] >> 16 : c.s[i / 2] & 0xffffu;
+          if constexpr (std::is_same<T, __half>::value) {
+            const __half2 h = __float2half2_rn(__uint_as_float(s << 16));
+            s2[i] = *reinterpret_cast<const uint32_t*>(&h);
+            s24[i] = 0;
+          } else {
+            s2[i] = s | s << 16;
+            const __nv_bfloat162 x = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&s2[i]), __float2bfloat162_rn(-24.f));
+            s24[i] = *reinterpret_cast<const uint32_t*>(&x);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+          uint32_t v[4];
+          int4_values<T>(c.w[i], s2[i % G], s24[i % G], v);
+          *reinterpret_cast<uint4*>(dst + ((piece0 + i) ^ swizzle) * 16) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+      };
+      Codes k, v;
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) k.w[i] = v.w[i] = 0;
+      int page = page_at(0);
+      fetch(k, 0, page, a.k, a.k_page, a.k_slot, a.k_head, p.k_scale, p.ks_page, p.ks_slot, p.ks_head);
+      fetch(v, 0, page, a.v, a.v_page, a.v_slot, a.v_head, p.v_scale, p.vs_page, p.vs_slot, p.vs_head);
+      page = page_at(1);
       for (int j = 0; j < n; ++j, ++g) {
-        if (j >= full0 && j < full1) continue;
-        const uint32_t s = g % L::kStages;
-        // Asked by the warp that has seen the block arrive.
-        if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.clean_ask, asked++ & 1) &&
-                                               wait_for(&bar.v_full[s], (g / L::kStages) & 1))))
-          break;
-        const int kb = (w.first + j) * kKeys, lo = w.lo - kb, hi = w.hi - kb;
-        uint4* v = reinterpret_cast<uint4*>(v_s + s * L::kBlock);
-        bool wild = false;
-        constexpr int kFlight = 8;
-#pragma unroll 1
-        for (int i0 = lane; i0 < kKeys * D / 8; i0 += 32 * kFlight) {
-          uint4 x[kFlight];
+        const uint32_t s = g % L::kStages, parity = ((g / L::kStages) & 1) ^ 1;
+        if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.k_empty[s], parity)))) break;
+        put(k, to + s * L::kBlock);
+        if (lane == 0) mbar_arrive(&bar.k_full[s]);
+        fetch(k, j + 1, page, a.k, a.k_page, a.k_slot, a.k_head, p.k_scale, p.ks_page, p.ks_slot, p.ks_head);
+        if (j < full0 || j >= full1) {
+          // Some row does not see some key: scales that are no numbers are taken out (0 * NaN), and the
+          // epilogue adds NaN to the rows that see them.
 #pragma unroll
-          for (int f = 0; f < kFlight; ++f) x[f] = v[i0 + 32 * f];
-#pragma unroll
-          for (int f = 0; f < kFlight; ++f) {
-            const int i = i0 + 32 * f, key = (i >> 3) & (kKeys - 1);
-            if (key < lo || key >= hi) {
-              v[i] = make_uint4(0, 0, 0, 0);
-            } else if (non_finite<T>(x[f].x) | non_finite<T>(x[f].y) | non_finite<T>(x[f].z) | non_finite<T>(x[f].w)) {
-              v[i] = make_uint4(finite_only<T>(x[f].x), finite_only<T>(x[f].y), finite_only<T>(x[f].z),
-                                finite_only<T>(x[f].w));
-              wild = true;
+          for (int i = 0; i < G / 2; ++i) {
+            if (non_finite<__nv_bfloat16>(v.s[i])) {
+              v.s[i] = finite_only<__nv_bfloat16>(v.s[i]);
+              w.wild = 1;
             }
           }
         }
-        if (wild) w.wild = 1;
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.v_clean);
+        if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.v_empty[s], parity)))) break;
+        put(v, to + (v_s - k_s) + s * L::kBlock);
+        if (lane == 0) mbar_arrive(&bar.v_full[s]);
+        fetch(v, j + 1, page, a.v, a.v_page, a.v_slot, a.v_head, p.v_scale, p.vs_page, p.vs_slot, p.vs_head);
+        page = page_at(j + 2);
       }
       done_with(t);
     }
+  } else if (warp >= 4) {
+    if constexpr (kInt4) fewer_registers<kIssueRegisters>();
+    if (warp == 4) {
+      // ---------------- scores ----------------
+      // The issuing warps walk the blocks whole, with values the compiler knows to be the same
+      // in all lanes, and one lane issues. Each has one product: a warp that issued both, with
+      // its waits, took longer for a block than its softmax does.
+      constexpr uint32_t idesc = idesc_of<T>(kKeys, false);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint64_t q_desc = smem_desc_k_sw128(smem_u32(q_s));
+      bool ok = true;
+      uint32_t queries = 0;
+      for (uint32_t t = 0; ok; ++t) {
+        if (!(ok = next_work(t))) break;
+        const Work& w = bar.work[t & 1];
+        const int n = __shfl_sync(0xffffffffu, w.blocks, 0);
+        if (w.rows < 0) break;
+        if (n) ok = __all_sync(0xffffffffu, wait_for(&bar.q_full, queries++ & 1));
+        for (int j = 0; j < n && ok; ++j, ++g) {
+          const uint32_t s = g % L::kStages, b = g % L::kScores;
+          // The last scores of this buffer are in the rows' registers, K is here.
+          if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.s_read[b], ((g / L::kScores) & 1) ^ 1) &&
+                                                 wait_for(&bar.k_full[s], (g / L::kStages) & 1))))
+            break;
+          tc_fence_after();
+          const uint64_t k_desc = smem_desc_k_sw128(smem_u32(k_s) + s * L::kBlock);
+          if (elect_one()) {
+#pragma unroll
+            for (int h = 0; h < L::kHalves; ++h)
+#pragma unroll
+              for (int c = 0; c < 4; ++c)  // 16 columns (32 bytes) a step
+                umma_bf16(tm + L::kSCol + b * kKeys, q_desc + h * (L::kQHalf / 16) + 2 * c,
+                          k_desc + h * (L::kHalf / 16) + 2 * c, idesc, (h | c) != 0);
+            umma_commit(&bar.k_empty[s]);
+            umma_commit(&bar.s_full[b]);
+            if (j == n - 1) umma_commit(&bar.q_empty);
+          }
+          __syncwarp();
+        }
+        done_with(t);
+      }
+      // Neither tensor memory nor the tiles are released under products still running.
+      if (elect_one()) umma_commit(&bar.drain[0]);
+      drain(&bar.drain[0], 0);
+    } else if (warp == 6) {
+      // ---------------- output ----------------
+      constexpr uint32_t idesc = idesc_of<T>(D, true);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      bool ok = true;
+      uint32_t cleaned = 0;
+      for (uint32_t t = 0; ok; ++t) {
+        if (!(ok = next_work(t))) break;
+        const Work& w = bar.work[t & 1];
+        const int n = __shfl_sync(0xffffffffu, w.blocks, 0), full0 = __shfl_sync(0xffffffffu, w.full0, 0),
+                  full1 = __shfl_sync(0xffffffffu, w.full1, 0);
+        if (w.rows < 0) break;
+        for (int j = 0; j < n; ++j, ++g) {
+          const uint32_t s = g % L::kStages;
+          ok = wait_for(&bar.v_full[s], (g / L::kStages) & 1);
+          const bool partial = !kInt4 && (j < full0 || j >= full1);
+          if (partial && lane == 0) mbar_arrive(&bar.clean_ask);  // cleaned beside the block's softmax
+          ok = ok && (!partial || wait_for(&bar.v_clean, cleaned & 1)) && wait_for(&bar.p_full[g & 1], (g >> 1) & 1);
+          cleaned += partial;
+          if (!(ok = __all_sync(0xffffffffu, ok))) break;
+          tc_fence_after();
+          const uint64_t v_desc = smem_desc_mn_sw128(smem_u32(v_s) + s * L::kBlock, L::kHalf);
+          if (elect_one()) {
+#pragma unroll
+            for (int c = 0; c < kKeys / 16; ++c)  // 16 keys a step: 8 columns of P, two 8-row groups of V (2,048 bytes)
+              umma_ts(tm + L::kOCol, tm + L::kPCol + (g & 1) * (kKeys / 2) + 8 * c, v_desc + 128 * c, idesc, (j | c) != 0);
+            umma_commit(&bar.v_empty[s]);
+            umma_commit(&bar.o_done[g & 1]);
+          }
+          __syncwarp();
+        }
+        done_with(t);
+      }
+      if (elect_one()) umma_commit(&bar.drain[1]);
+      drain(&bar.drain[1], 0);
+    } else if (warp == 5) {
+      // ---------------- tiles and loads ----------------
+      const int in_page = (1 << a.pages.page_log2) - 1, boxes = kKeys / p.box_rows;
+      const uint32_t box_bytes = (uint32_t)p.box_rows * 128;
+      // The last tile's request: `r` with `before` tiles of others in front of it.
+      int r = requests, before = all_tiles;
+      Request q{0, 0, 0};
+      bool too_long = false;
+      if (bar.found >= 0) {
+        r = bar.found;
+        before = bar.found_start;
+        q = request_at(a.pages, a.tokens, a.max_keys, r, &too_long);
+      }
+      // The work of CTA `index`; false where it has none.
+      const auto describe = [&](int index, Work& w) {
+        const int cut = index - p.whole_items, splits = cut < 0 ? 1 : p.splits, split = cut < 0 ? 0 : cut % p.splits;
+        const int item = cut < 0 ? index : p.whole_items + cut / p.splits, tile = tile_at(index);
+        if (tile >= before + tiles_of(q)) {  // not before the last one: from the end
+          r = requests;
+          before = all_tiles;
+          q = Request{0, 0, 0};
+        }
+        while (tile < before && r > 0) {  // 32 requests back
+          const int at = r - 1 - lane;
+          Request mine{0, 0, 0};
+          bool over = false;
+          if (at >= 0) mine = request_at(a.pages, a.tokens, a.max_keys, at, &over);
+          const int n = tiles_of(mine);
+          int upto = n;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+          }
+          const uint32_t here = __ballot_sync(0xffffffffu, tile >= before - upto && tile < before - upto + n);
+          const int src = here ? __ffs(here) - 1 : 31;
+          r = here ? r - 1 - src : max(r - 32, 0);
+          before -= __shfl_sync(0xffffffffu, upto, src);
+          q.first = __shfl_sync(0xffffffffu, mine.first, src);
+          q.news = here ? __shfl_sync(0xffffffffu, mine.news, src) : 0;
+          q.total = __shfl_sync(0xffffffffu, mine.total, src);
+          too_long = __shfl_sync(0xffffffffu, (int)over, src);
+          if (here) break;
+        }
+        Tile* join = splits > 1 && split == 0 && lane == 0 ? p.joins + (item - p.whole_items) : nullptr;
+        if (tile < before || tile >= before + tiles_of(q)) {  // the grid has room for more tiles than there are
+          if (join) join->parts = 0;
+          return false;
+        }
+        const int token0 = (tile - before) * p.tile_tokens, tokens = min(p.tile_tokens, q.news - token0);
+        w.r = r;
+        w.head = item % a.kv_heads;
+        w.first_token = q.first + token0;
+        w.rows = tokens * a.group;
+        w.pos0 = q.total - q.news + token0;
+        w.pos1 = w.pos0 + tokens - 1;
+        w.hi = max(w.pos1 + 1, 0);
+        w.lo = a.window ? max(w.pos0 - a.window + 1, 0) : 0;
+        const int first = w.lo / kKeys, blocks = max((w.hi + kKeys - 1) / kKeys - first, 0);
+        // Shares of at least four blocks: a share's fixed cost is about theirs.
+        int share = blocks;
+        if (splits > 1) share = max((blocks + splits - 1) / splits, 4);
+        w.parts = blocks && splits > 1 ? (blocks + share - 1) / share : 1;
+        w.first = first + split * share;
+        w.blocks = max(min(first + blocks, w.first + share) - w.first, 0);
+        w.full0 = a.window ? max((max(w.pos1 - a.window + 1, 0) + kKeys - 1) / kKeys - w.first, 0) : 0;
+        w.full1 = (w.pos0 + 1) / kKeys - w.first;
+        w.share = cut;
+        w.bad = too_long;
+        w.wild = 0;
+        if (join) {
+          join->token0 = w.first_token;
+          join->rows = w.rows;
+          join->kv_head = w.head;
+          join->parts = w.parts;
+        }
+        return split < w.parts;
+      };
+      // This lane has a box of the block to load.
+      const auto has_box = [&](const Work& w, int j) {
+        const int key = (w.first + j) * kKeys + lane * p.box_rows;
+        return lane < boxes && j < w.blocks && key < w.hi && key + p.box_rows > w.lo;
+      };
+      // Its entry of the page table, read a block ahead and checked when the box is loaded (-1: nothing to load).
+      const auto entry_of = [&](const Work& w, int j) {
+        const int key = (w.first + j) * kKeys + lane * p.box_rows;
+        return has_box(w, j) ? __ldg(a.pages.page_table + w.r * a.pages.table_stride + (key >> a.pages.page_log2)) : -1;
+      };
+      const auto page_of = [&](const Work& w, int j, int entry, int* bad) {
+        if (!has_box(w, j)) return -1;
+        if (entry >= 0 && entry < a.pages.num_pages) return entry;
+        *bad = 1;
+        return -1;
+      };
+      const auto load = [&](const Work& w, int j, int page, const CUtensorMap* map, unsigned char* ring, uint64_t* full) {
+        const uint32_t s = g % L::kStages, count = __popc(__ballot_sync(0xffffffffu, page >= 0));
+        if (lane == 0) mbar_arrive_expect_tx(&full[s], count * box_bytes * L::kHalves);
+        __syncwarp();
+        if (page >= 0) {
+          const int key = (w.first + j) * kKeys + lane * p.box_rows;
+          const uint32_t dst = smem_u32(ring) + s * L::kBlock + lane * box_bytes;
+#pragma unroll
+          for (int h = 0; h < L::kHalves; ++h)
+            tma_load_4d(dst + h * L::kHalf, map, h * 64, key & in_page, w.head, page, &full[s]);
+        }
+        __syncwarp();
+      };
+      const auto leave = [&](const Work& w) {
+        if (lane == 0) {
+          bar.left = w;
+          bar.has_left = 1;
+        }
+      };
+      bool ok = true, asking = false;
+      uint32_t t = 0, queries = 0, asked = 0;
+      uint32_t k_loads = 0, v_loads = 0, q_loads = 0;  // begun
+      for (int index = blockIdx.x; index >= 0;) {
+        Work w;
+        if (describe(index, w)) {
+          Work& slot = bar.work[t & 1];
+          int entry = kInt4 ? -1 : entry_of(w, 0);
+          if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.work_empty[t & 1], ((t >> 1) & 1) ^ 1)))) {
+            leave(w);
+            break;
+          }
+          if (lane == 0) {
+            slot = w;
+            mbar_arrive(&bar.work_full[t & 1]);
+          }
+          __syncwarp();
+          ++t;
+          if constexpr (kInt4) {
+            // K and V are other warps' work here.
+            if (w.blocks) {
+              if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.q_empty, (queries & 1) ^ 1)))) break;
+              ++queries;
+              if (lane == 0) {
+                mbar_arrive_expect_tx(&bar.q_full, p.tile_tokens * a.group * 128 * L::kHalves);
+#pragma unroll
+                for (int h = 0; h < L::kHalves; ++h)
+                  tma_load_3d(smem_u32(q_s) + h * L::kQHalf, &q_map, h * 64, w.head * a.group, w.first_token, &bar.q_full);
+              }
+              __syncwarp();
+              ++q_loads;
+            }
+            g += w.blocks;
+          }
+          for (int j = 0; j < w.blocks && !kInt4; ++j, ++g) {
+            const uint32_t s = g % L::kStages, parity = ((g / L::kStages) & 1) ^ 1;
+            const int page = page_of(w, j, entry, &slot.bad);
+            entry = entry_of(w, j + 1);
+            if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.k_empty[s], parity)))) break;
+            load(w, j, page, &k_map, k_s, bar.k_full);
+            ++k_loads;
+            if (j == 0) {
+              // The last tile's scores have been computed: its Q can go.
+              if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.q_empty, (queries & 1) ^ 1)))) break;
+              ++queries;
+              if (lane == 0) {
+                mbar_arrive_expect_tx(&bar.q_full, p.tile_tokens * a.group * 128 * L::kHalves);
+#pragma unroll
+                for (int h = 0; h < L::kHalves; ++h)
+                  tma_load_3d(smem_u32(q_s) + h * L::kQHalf, &q_map, h * 64, w.head * a.group, w.first_token, &bar.q_full);
+              }
+              __syncwarp();
+              ++q_loads;
+            }
+            if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.v_empty[s], parity)))) break;
+            load(w, j, page, &v_map, v_s, bar.v_full);
+            ++v_loads;
+          }
+          if (!ok) break;
+        }
+        // Asked for late, while the last blocks are computed, so that an idle CTA is not left without.
+        if (lane == 0) {
+          fence_proxy_async_smem();  // the last answer has been read
+          mbar_arrive_expect_tx(&bar.next_here, 16);
+          ask_next_cta(answer, &bar.next_here);
+        }
+        __syncwarp();
+        asking = true;
+        if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.next_here, asked++ & 1)))) break;
+        asking = false;
+        index = __shfl_sync(0xffffffffu, next_cta(answer), 0);
+      }
+      if (lane == 0) bar.posted = t;
+      if (ok) {
+        ok = __all_sync(0xffffffffu, wait_for(&bar.work_empty[t & 1], ((t >> 1) & 1) ^ 1));
+        if (ok && lane == 0) {
+          bar.work[t & 1].rows = -1;
+          bar.work[t & 1].blocks = 0;
+          mbar_arrive(&bar.work_full[t & 1]);
+        }
+        __syncwarp();
+        // No product's arrival on an empty barrier lands after the CTA has gone.
+        for (uint32_t e = g; e < g + L::kStages && ok; ++e) {
+          const uint32_t s = e % L::kStages, parity = ((e / L::kStages) & 1) ^ 1;
+          ok = __all_sync(0xffffffffu, wait_for(&bar.k_empty[s], parity) && wait_for(&bar.v_empty[s], parity));
+        }
+        if (ok) ok = __all_sync(0xffffffffu, wait_for(&bar.q_empty, (queries & 1) ^ 1));
+      }
+      if (!ok) {
+        // A wait ran out: what is still on its way to shared memory has to arrive. A tile that does is not computed.
+        if (asking && __all_sync(0xffffffffu, drain(&bar.next_here, (asked - 1) & 1))) {
+          const int index = __shfl_sync(0xffffffffu, next_cta(answer), 0);
+          Work w;
+          if (index >= 0 && describe(index, w)) leave(w);
+        }
+        if (q_loads) drain(&bar.q_full, (q_loads - 1) & 1);
+        for (uint32_t back = 1; back <= L::kStages; ++back) {
+          if (k_loads >= back) drain(&bar.k_full[(k_loads - back) % L::kStages], ((k_loads - back) / L::kStages) & 1);
+          if (v_loads >= back) drain(&bar.v_full[(v_loads - back) % L::kStages], ((v_loads - back) / L::kStages) & 1);
+        }
+      }
+    } else if (kInt4 && warp == 7) {
+      // (no cleaning: scales are looked at where they are turned into values)
+    } else if (warp == 7) {
+      // ---------------- cleaning ----------------
+      uint32_t asked = 0;
+      bool ok = true;
+      for (uint32_t t = 0; ok; ++t) {
+        if (!(ok = next_work(t))) break;
+        Work& w = bar.work[t & 1];
+        if (w.rows < 0) break;
+        const int n = w.blocks, full0 = w.full0, full1 = w.full1;
+        for (int j = 0; j < n; ++j, ++g) {
+          if (j >= full0 && j < full1) continue;
+          const uint32_t s = g % L::kStages;
+          // Asked by the warp that has seen the block arrive.
+          if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.clean_ask, asked++ & 1) &&
+                                                 wait_for(&bar.v_full[s], (g / L::kStages) & 1))))
+            break;
+          const int kb = (w.first + j) * kKeys, lo = w.lo - kb, hi = w.hi - kb;
+          uint4* v = reinterpret_cast<uint4*>(v_s + s * L::kBlock);
+          bool wild = false;
+          constexpr int kFlight = 8;
+#pragma unroll 1
+          for (int i0 = lane; i0 < kKeys * D / 8; i0 += 32 * kFlight) {
+            uint4 x[kFlight];
+#pragma unroll
+            for (int f = 0; f < kFlight; ++f) x[f] = v[i0 + 32 * f];
+#pragma unroll
+            for (int f = 0; f < kFlight; ++f) {
+              const int i = i0 + 32 * f, key = (i >> 3) & (kKeys - 1);
+              if (key < lo || key >= hi) {
+                v[i] = make_uint4(0, 0, 0, 0);
+              } else if (non_finite<T>(x[f].x) | non_finite<T>(x[f].y) | non_finite<T>(x[f].z) | non_finite<T>(x[f].w)) {
+                v[i] = make_uint4(finite_only<T>(x[f].x), finite_only<T>(x[f].y), finite_only<T>(x[f].z),
+                                  finite_only<T>(x[f].w));
+                wild = true;
+              }
+            }
+          }
+          if (wild) w.wild = 1;
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar.v_clean);
+        }
+        done_with(t);
+      }
+    }
   } else {
+    if constexpr (kInt4) more_registers<kRowRegisters>();
     // ---------------- softmax and output rows ----------------
     const int row = threadIdx.x;
     const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
@@ -832,12 +1003,23 @@ __global__ void __launch_bounds__(kPrefillThreads, 2)
               const int32_t* entry = a.pages.page_table + (int64_t)w.r * a.pages.table_stride + (k >> a.pages.page_log2);
               const int64_t page = __ldg(entry);
               if (page < 0 || page >= a.pages.num_pages) continue;
-              const T* v = static_cast<const T*>(a.v) + page * a.v_page +
-                           (k & ((1 << a.pages.page_log2) - 1)) * a.v_slot + w.head * a.v_head + 32 * c;
+              if constexpr (kInt4) {
+                const uint16_t* s = p.v_scale + page * p.vs_page + (k & ((1 << a.pages.page_log2) - 1)) * p.vs_slot +
+                                    w.head * p.vs_head;
 #pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                const float x = (float)v[i];
-                if (!isfinite(x)) o[i] = __float_as_uint(__uint_as_float(o[i]) + x);
+                for (int i = 0; i < 4; ++i)
+                  if ((s[i % (D / 32)] & 0x7f80u) == 0x7f80u) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) o[8 * i + e] = 0x7fc00000u;
+                  }
+              } else {
+                const T* v = static_cast<const T*>(a.v) + page * a.v_page +
+                             (k & ((1 << a.pages.page_log2) - 1)) * a.v_slot + w.head * a.v_head + 32 * c;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                  const float x = (float)v[i];
+                  if (!isfinite(x)) o[i] = __float_as_uint(__uint_as_float(o[i]) + x);
+                }
               }
             }
           }
@@ -950,14 +1132,14 @@ bool encode_rows(CUtensorMap* map, const void* base, int dtype, int D, int64_t h
                            dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <typename T, int D, bool kSelfTest = false>
+template <typename T, int D, bool kSelfTest = false, bool kInt4 = false>
 cudaError_t launch(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map, const PrefillArgs& p, int64_t items,
                    cudaStream_t stream) {
-  const void* fn = reinterpret_cast<const void*>(&paged_prefill_kernel<T, D, kSelfTest>);
+  const void* fn = reinterpret_cast<const void*>(&paged_prefill_kernel<T, D, kSelfTest, kInt4>);
   cudaError_t err = allow_shared_memory(fn, Layout<D>::kSmem);
   if (err != cudaSuccess) return err;
   const int64_t cut = items - p.whole_items;
-  err = launch_kernel(paged_prefill_kernel<T, D, kSelfTest>, dim3((unsigned)(p.whole_items + cut * p.splits)), dim3(kPrefillThreads),
+  err = launch_kernel(paged_prefill_kernel<T, D, kSelfTest, kInt4>, dim3((unsigned)(p.whole_items + cut * p.splits)), dim3(kInt4 ? kInt4Threads : kPrefillThreads),
                       Layout<D>::kSmem, stream, q_map, k_map, v_map, p);
   if (err != cudaSuccess || p.splits == 1) return err;
   return launch_following(prefill_join_kernel<T, D>, dim3((unsigned)(cut * (kTile / 16))), dim3(512), stream, p);
@@ -1014,8 +1196,8 @@ size_t paged_prefill_workspace(int D, int sms) {
   return (size_t)(kMostShares * 2 * sms) * (kTile * (size_t)(D + 2) * sizeof(float) + sizeof(Tile));
 }
 
-bool launch_paged_prefill(const AttentionArgs& a, const PrefillPlan& plan, int dtype, int D, int64_t page_size,
-                          long long wait_cycles, cudaStream_t stream, cudaError_t* err) {
+bool launch_paged_prefill(const AttentionArgs& a, const PrefillPlan& plan, const flash_prologue_scales* scales, int dtype,
+                          int D, int64_t page_size, long long wait_cycles, cudaStream_t stream, cudaError_t* err) {
   PrefillArgs p{};
   p.a = a;
   p.wait_cycles = wait_cycles;
@@ -1026,8 +1208,18 @@ bool launch_paged_prefill(const AttentionArgs& a, const PrefillPlan& plan, int d
   p.box_rows = page_size < kKeys ? (int)page_size : kKeys;
   const int64_t items = plan.tiles * a.kv_heads;
   if (items * plan.splits * (kTile / 16) >= (int64_t(1) << 31)) return false;
-  CUtensorMap q_map, k_map, v_map;
-  if (!encode_rows(&q_map, a.q, dtype, D, a.heads, a.tokens, a.q_h, a.q_n, a.group, plan.tile_tokens) ||
+  CUtensorMap q_map, k_map{}, v_map{};
+  if (!encode_rows(&q_map, a.q, dtype, D, a.heads, a.tokens, a.q_h, a.q_n, a.group, plan.tile_tokens)) return false;
+  if (scales) {
+    p.k_scale = static_cast<const uint16_t*>(scales->k);
+    p.v_scale = static_cast<const uint16_t*>(scales->v);
+    p.ks_page = scales->k_page;
+    p.ks_slot = scales->k_slot;
+    p.ks_head = scales->k_head;
+    p.vs_page = scales->v_page;
+    p.vs_slot = scales->v_slot;
+    p.vs_head = scales->v_head;
+  } else if (
       !encode_cache(&k_map, a.k, dtype, D, page_size, a.kv_heads, a.pages.num_pages, a.k_slot, a.k_head, a.k_page,
                     p.box_rows) ||
       !encode_cache(&v_map, a.v, dtype, D, page_size, a.kv_heads, a.pages.num_pages, a.v_slot, a.v_head, a.v_page,
@@ -1039,7 +1231,16 @@ bool launch_paged_prefill(const AttentionArgs& a, const PrefillPlan& plan, int d
     p.part_stat = p.part_out + shares * kTile * D;
     p.joins = reinterpret_cast<Tile*>(p.part_stat + shares * kTile * 2);
   }
-  if (wait_cycles)
+  if (scales && wait_cycles)
+    *err = D == 64 ? launch<__nv_bfloat16, 64, true, true>(q_map, k_map, v_map, p, items, stream)
+                   : launch<__nv_bfloat16, 128, true, true>(q_map, k_map, v_map, p, items, stream);
+  else if (scales && D == 64)
+    *err = dtype == 0 ? launch<__nv_bfloat16, 64, false, true>(q_map, k_map, v_map, p, items, stream)
+                      : launch<__half, 64, false, true>(q_map, k_map, v_map, p, items, stream);
+  else if (scales)
+    *err = dtype == 0 ? launch<__nv_bfloat16, 128, false, true>(q_map, k_map, v_map, p, items, stream)
+                      : launch<__half, 128, false, true>(q_map, k_map, v_map, p, items, stream);
+  else if (wait_cycles)
     *err = D == 64 ? launch<__nv_bfloat16, 64, true>(q_map, k_map, v_map, p, items, stream)
                    : launch<__nv_bfloat16, 128, true>(q_map, k_map, v_map, p, items, stream);
   else if (D == 64)

@@ -612,7 +612,7 @@ FLASH_PROLOGUE_API int flash_prologue_append_paged_axes(const flash_prologue_app
  * value of largest magnitude (of x and -x: x), cut towards zero. Channel c has
  * the code clamp(rint(x / s), -8, 7) and stands for s * code, which is exact in
  * BF16. For FP16 rows |s| is kept within 2^-20 .. 7936 (then s * code is exact in
- * FP16 too), for BF16 rows at 2^-100 at least; a group of zeros has s = 0. A group
+ * FP16 too), for BF16 rows within 2^-100 .. 2^122; a group of zeros has s = 0. A group
  * that holds an infinity or NaN has a NaN scale: it stands for NaN.
  * In memory: D / 2 bytes of codes, a 32-bit word for each 8 channels in order;
  * in a word, codes + 8 of the even channels 0, 2, 4, 6 in bits 0, 4, 8, 12 and of
@@ -634,6 +634,10 @@ FLASH_PROLOGUE_API int flash_prologue_append_paged_int4(const flash_prologue_app
 /* flash_prologue_paged_attention over such a cache. */
 FLASH_PROLOGUE_API int flash_prologue_paged_attention_int4(const flash_prologue_attention_args* args,
                                                            const flash_prologue_scales* scales, void* stream);
+/* flash_prologue_selftest_attention_waits over such a cache. */
+FLASH_PROLOGUE_API int flash_prologue_selftest_attention_int4_waits(const flash_prologue_attention_args* args,
+                                                                    const flash_prologue_scales* scales,
+                                                                    int64_t wait_cycles, void* stream);
 /* Bytes of workspace that cover every call of it with head dimension D on the current device. */
 FLASH_PROLOGUE_API int flash_prologue_paged_attention_int4_workspace_size(int64_t D, size_t* bytes);
 /* What `rows` rows of codes and scales stand for, as BF16 or FP16 rows [rows, D]; all contiguous, 16-byte aligned. */

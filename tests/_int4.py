@@ -13,7 +13,7 @@ def cut(e, half):
     e = e.double() / 8
     power = torch.exp2(torch.floor(torch.log2(e.abs().clamp(min=2.0 ** -140))) - 4)
     s = -e.sign() * torch.floor(e.abs() / power) * power
-    least, most = (2.0 ** -20, 7936.0) if half else (2.0 ** -100, float("inf"))
+    least, most = (2.0 ** -20, 7936.0) if half else (2.0 ** -100, 2.0 ** 122)
     return torch.where(s == 0, 0, s.sign() * s.abs().clamp(least, most))
 
 

@@ -269,6 +269,47 @@ def test_pages_out_of_range_give_nan_and_the_error_word(news):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("news,totals,window", [
+    ([700, 0, 900, 5], [900, 40, 2000, 1100], 0),   # whole tiles, more than the GPU holds at once
+    ([70, 3, 25], [6000, 2500, 2900], 0),           # keys shared out
+])
+@pytest.mark.parametrize("D", [64, 128])
+def test_waits_that_run_out(news, totals, window, D, monkeypatch):
+    """Tiles given up come out as NaN with the error word set, shares of a tile included; the rest has its bits."""
+    req = Requests4(news, totals, 32, 4, D, 16, BF16)
+    other = Requests4(news, totals, 32, 4, D, 16, BF16, seed=1)
+
+    def call(r):
+        return _attend(r, r.q.to(BF16), softmax_scale=0.1, window=window, return_lse=True)
+
+    def bounded(cycles):
+        def run(name, args, device, scales):
+            status = _lib.load().flash_prologue_selftest_attention_int4_waits(args, scales, cycles,
+                                                                              _lib.raw_stream(device.index))
+            _lib.check(status, "flash_prologue_selftest_attention_int4_waits")
+        return run
+
+    clean, clean_lse = call(req)
+    _lib.device_error()
+    given_up = 0
+    for cycles in (1, 200, 600, 1000, 2000, 4000, 8000, 20000, 100000, 2 ** 32):
+        call(other)  # leaves other rows and shares where this call's may come to lie
+        torch.cuda.synchronize()
+        with monkeypatch.context() as m:
+            m.setattr(fap.int4, "call_library", bounded(cycles))
+            got, lse = call(req)
+        error = _lib.device_error()
+        lost = got.isnan().all(-1)
+        assert torch.equal(got.isnan().any(-1), lost) and torch.equal(lse.isnan(), lost)
+        assert torch.equal(got[~lost], clean[~lost]) and torch.equal(lse[~lost], clean_lse[~lost])
+        assert error == 1 if lost.any() else error in (0, 1)
+        given_up += int(lost.sum())
+    assert error == 0 and not lost.any()  # the limit of a call
+    assert given_up
+    assert all(torch.equal(a, b) for a, b in zip(call(req), (clean, clean_lse)))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("news,totals,ahead", [
     ([1, 0, 1, 3, 1, 1], [40, 9, 1, 250, 66, 130], 5),
     ([2, 1, 0, 1, 1, 1], [3000, 70, 4, 900, 64, 333], 7),
