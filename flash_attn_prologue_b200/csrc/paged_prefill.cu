@@ -54,7 +54,7 @@ namespace {
 constexpr int kTile = 128;             // rows of a tile
 constexpr int kKeys = 64;              // keys of a block
 constexpr int kPrefillThreads = 256;
-constexpr int kInt4Threads = kPrefillThreads + 128;  // four more warps turn codes into values
+constexpr int kInt4Threads = kPrefillThreads + 256;  // eight more warps turn codes into values
 constexpr int kRowThreads = 128;
 constexpr int kTmemCols = 256;
 
@@ -172,6 +172,20 @@ __device__ __forceinline__ bool phase_wait(uint64_t* bar, uint32_t parity) {
   do {
     if (phase_done(a, parity)) return true;
   } while (clock64() - start < kMostCycles);
+  atomicOr(&g_device_error, kDeviceErrorTimeout);
+  return false;
+}
+// A wait whose end nobody is in a hurry for, in suspended tries (mbar_wait's limit) that leave the issue slots to others.
+__device__ __forceinline__ bool idle_wait(uint64_t* bar, uint32_t parity) {
+  const uint32_t a = smem_u32(bar);
+  for (uint32_t i = 0; i < kMaxWaitTries; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2, %3;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done) : "r"(a), "r"(parity), "r"(kSuspendHintNs) : "memory");
+    if (done) return true;
+  }
   atomicOr(&g_device_error, kDeviceErrorTimeout);
   return false;
 }
@@ -315,9 +329,9 @@ template <int N>
 __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-// 384 threads at 80 registers each, split among the three warpgroups.
-constexpr int kRowRegisters = 120, kIssueRegisters = 56, kCodeRegisters = 64;
-static_assert(kRowRegisters + kIssueRegisters + kCodeRegisters == 3 * 80, "registers of a CTA");
+// 512 threads at 64 registers each, split among the four warpgroups.
+constexpr int kRowRegisters = 112, kOtherRegisters = 48;
+static_assert(kRowRegisters + 3 * kOtherRegisters == 4 * 64, "registers of a CTA");
 
 template <typename T, int D, bool kSelfTest = false, bool kInt4 = false>
 __global__ void __launch_bounds__(kInt4 ? kInt4Threads : kPrefillThreads, 2)
@@ -331,6 +345,11 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads : kPrefillThreads, 2)
   const auto wait_for = [&](uint64_t* b, uint32_t parity) {
     if constexpr (kSelfTest) return short_wait(b, parity, p.wait_cycles);
     else return phase_wait(b, parity);
+  };
+  // Where K and V are values made here, warps that only hand out tiles wait for a whole tile's time.
+  const auto wait_idle = [&](uint64_t* b, uint32_t parity) {
+    if constexpr (kInt4 && !kSelfTest) return idle_wait(b, parity);
+    else return wait_for(b, parity);
   };
   // For copies and products under way, which end by themselves: never cut short.
   const auto drain = [](uint64_t* b, uint32_t parity) { return phase_wait(b, parity); };
@@ -354,7 +373,7 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads : kPrefillThreads, 2)
       mbar_init(&bar.p_full[b], kRowThreads / 32);
       mbar_init(&bar.o_done[b], 1);
       mbar_init(&bar.work_full[b], 1);
-      mbar_init(&bar.work_empty[b], kRowThreads / 32 + (kInt4 ? 6 : 3));
+      mbar_init(&bar.work_empty[b], kRowThreads / 32 + (kInt4 ? 10 : 3));
       mbar_init(&bar.drain[b], 1);
     }
     mbar_init(&bar.clean_ask, 1);
@@ -424,115 +443,119 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads : kPrefillThreads, 2)
   };
 
   if (kInt4 && warp >= 8) {
-    fewer_registers<kCodeRegisters>();
+    fewer_registers<kOtherRegisters>();
     // ---------------- codes to values ----------------
-    // A thread has a key of the block and half its words (D = 128: all of a 64-column half), loads them
-    // a block ahead and writes them as the tensor maps of a 16-bit cache would: rows of 128 bytes,
-    // 16-byte pieces swizzled by the row.
-    constexpr int G = D / 32, kWords = D / 16;
-    const int key_row = threadIdx.x & 63, part = (threadIdx.x >> 6) & 1;
+    // Warps 8-11 make K, warps 12-15 V. A thread has a key of the block and half its words (at D = 128 those
+    // of one 64-column half), loads them a block ahead and writes the values as the tensor maps of a 16-bit
+    // cache would: rows of 128 bytes, 16-byte chunks swizzled by the row. (At D = 128 the two threads of a
+    // row go through their words in different orders, so that eight lanes write to eight banks.)
+    constexpr int G = D / 32, kPieces = D / 64;  // 16-byte pieces of a thread
+    const bool values = warp >= 12;
+    const int key_row = threadIdx.x % 128 / 2, part = threadIdx.x & 1, turn = D == 128 ? part : 0;
     const int in_page = (1 << a.pages.page_log2) - 1;
-    unsigned char* const to = k_s + (D == 128 ? part * L::kHalf : 0) + key_row * 128;
-    const int swizzle = key_row & 7, piece0 = D == 128 ? 0 : 4 * part;
-    struct Codes {
-      uint32_t w[kWords];
-      uint32_t s[G / 2];
-    };
+    unsigned char* const to = (values ? v_s : k_s) + (D == 128 ? part * L::kHalf : 0) + key_row * 128;
+    const int swizzle = key_row & 7, chunk0 = D == 128 ? 0 : 4 * part;
+    uint64_t* const full = values ? bar.v_full : bar.k_full;
+    uint64_t* const empty = values ? bar.v_empty : bar.k_empty;
+    // Strides of pages and slots take 31 bits (the host checks).
+    const int c_page = (int)(values ? a.v_page : a.k_page), c_slot = (int)(values ? a.v_slot : a.k_slot);
+    const int s_page = (int)(values ? p.vs_page : p.ks_page), s_slot = (int)(values ? p.vs_slot : p.ks_slot);
     bool ok = true;
     for (uint32_t t = 0; ok; ++t) {
       if (!(ok = next_work(t))) break;
       Work& w = bar.work[t & 1];
       if (w.rows < 0) break;
-      const int n = w.blocks, full0 = w.full0, full1 = w.full1, first = w.first, hi = w.hi, lo = w.lo, head = w.head;
+      const int n = w.blocks;
+      // This thread's key in block 0, and the keys that count.
+      const int key0 = w.first * kKeys + key_row, hi = w.hi, lo = w.lo;
       const int32_t* table = a.pages.page_table + (int64_t)w.r * a.pages.table_stride;
-      // The page of this thread's key in block j: -1 where it has none that counts.
-      const auto page_at = [&](int j) {
-        const int key = (first + j) * kKeys + key_row;
-        if (j >= n || key < lo || key >= hi) return -1;
-        const int page = __ldg(table + (key >> a.pages.page_log2));
-        if (page >= 0 && page < a.pages.num_pages) return page;
-        w.bad = 1;
-        return -1;
+      const unsigned char* codes = static_cast<const unsigned char*>(values ? a.v : a.k) +
+                                   w.head * (values ? a.v_head : a.k_head) + part * (kPieces * 16);
+      const uint16_t* scales = values ? p.v_scale + w.head * p.vs_head : p.k_scale + w.head * p.ks_head;
+      uint4 c[kPieces];
+      uint32_t c_scale[G / 2];
+      int page = 0;
+      const auto counts = [&](int j) {
+        const int key = key0 + j * kKeys;
+        return j < n && key >= lo && key < hi;
       };
-      const auto fetch = [&](Codes& c, int j, int page, const void* codes, int64_t c_page, int64_t c_slot, int64_t c_head,
-                             const uint16_t* scales, int64_t s_page, int64_t s_slot, int64_t s_head) {
-        const int slot = ((first + j) * kKeys + key_row) & in_page;
+      // The page of this thread's key in block j, looked at when it is used, a block later.
+      const auto find = [&](int j) {
+        if (counts(j)) page = __ldg(table + ((key0 + j * kKeys) >> a.pages.page_log2));
+      };
+      const auto fetch = [&](int j) {
 #pragma unroll
-        for (int i = 0; i < G / 2; ++i) c.s[i] = 0;  // zeros
-        if (page < 0) return;
-        const uint4* from = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(codes) + page * c_page + slot * c_slot +
-                                                           head * c_head + part * (kWords * 4));
-#pragma unroll
-        for (int i = 0; i < kWords / 4; ++i) {
-          const uint4 x = __ldg(from + i);
-          c.w[4 * i] = x.x; c.w[4 * i + 1] = x.y; c.w[4 * i + 2] = x.z; c.w[4 * i + 3] = x.w;
+        for (int g = 0; g < G / 2; ++g) c_scale[g] = 0;  // zeros
+        if (!counts(j)) return;
+        if (page < 0 || page >= a.pages.num_pages) {
+          w.bad = 1;
+          return;
         }
-        const uint16_t* s = scales + page * s_page + slot * s_slot + head * s_head;
+        const int slot = (key0 + j * kKeys) & in_page;
+        const unsigned char* from = codes + (int64_t)page * c_page + (int64_t)slot * c_slot;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) c[i] = __ldg(reinterpret_cast<const uint4*>(from + (i ^ turn) * 16));
+        const uint16_t* s = scales + (int64_t)page * s_page + (int64_t)slot * s_slot;
         if constexpr (G == 4) {
           const uint2 x = __ldg(reinterpret_cast<const uint2*>(s));
-          c.s[0] = x.x; c.s[1] = x.y;
+          c_scale[0] = x.x;
+          c_scale[1] = x.y;
         } else {
-          c.s[0] = __ldg(reinterpret_cast<const uint32_t*>(s));
+          c_scale[0] = __ldg(reinterpret_cast<const uint32_t*>(s));
         }
       };
-      const auto put = [&](const Codes& c, unsigned char* dst) {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) c[i] = make_uint4(0, 0, 0, 0);
+      find(0);
+      fetch(0);
+      find(1);
+      for (int j = 0; j < n; ++j, ++g) {
+        const uint32_t stage = g % L::kStages;
+        if (values && (j < w.full0 || j >= w.full1)) {
+          // Some row does not see some key: scales that are no numbers are taken out (0 * NaN), and the
+          // epilogue adds NaN to the rows that see them.
+#pragma unroll
+          for (int i = 0; i < G / 2; ++i)
+            if (non_finite<__nv_bfloat16>(c_scale[i])) {
+              c_scale[i] = finite_only<__nv_bfloat16>(c_scale[i]);
+              w.wild = 1;
+            }
+        }
         uint32_t s2[G], s24[G];
 #pragma unroll
         for (int i = 0; i < G; ++i) {
-          const uint32_t s = i & 1 ? c.s[i / 2] >> 16 : c.s[i / 2] & 0xffffu;
           if constexpr (std::is_same<T, __half>::value) {
-            const __half2 h = __float2half2_rn(__uint_as_float(s << 16));
+            const __half2 h = __float2half2_rn(__uint_as_float(i & 1 ? c_scale[i / 2] & 0xffff0000u : c_scale[i / 2] << 16));
             s2[i] = *reinterpret_cast<const uint32_t*>(&h);
             s24[i] = 0;
           } else {
-            s2[i] = s | s << 16;
+            s2[i] = __byte_perm(c_scale[i / 2], 0, i & 1 ? 0x3232 : 0x1010);
             const __nv_bfloat162 x = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&s2[i]), __float2bfloat162_rn(-24.f));
             s24[i] = *reinterpret_cast<const uint32_t*>(&x);
           }
         }
+        if (!(ok = __all_sync(0xffffffffu, wait_for(&empty[stage], ((g / L::kStages) & 1) ^ 1)))) break;
+        unsigned char* dst = to + stage * L::kBlock;
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) {
-          uint32_t v[4];
-          int4_values<T>(c.w[i], s2[i % G], s24[i % G], v);
-          *reinterpret_cast<uint4*>(dst + ((piece0 + i) ^ swizzle) * 16) = make_uint4(v[0], v[1], v[2], v[3]);
+        for (int i = 0; i < kPieces; ++i) {
+          const uint32_t word[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t v[4];
+            int4_values<T>(word[e], s2[e % G], s24[e % G], v);
+            *reinterpret_cast<uint4*>(dst + ((chunk0 + 4 * (i ^ turn) + e) ^ swizzle) * 16) = make_uint4(v[0], v[1], v[2], v[3]);
+          }
         }
         fence_proxy_async_smem();
         __syncwarp();
-      };
-      Codes k, v;
-#pragma unroll
-      for (int i = 0; i < kWords; ++i) k.w[i] = v.w[i] = 0;
-      int page = page_at(0);
-      fetch(k, 0, page, a.k, a.k_page, a.k_slot, a.k_head, p.k_scale, p.ks_page, p.ks_slot, p.ks_head);
-      fetch(v, 0, page, a.v, a.v_page, a.v_slot, a.v_head, p.v_scale, p.vs_page, p.vs_slot, p.vs_head);
-      page = page_at(1);
-      for (int j = 0; j < n; ++j, ++g) {
-        const uint32_t s = g % L::kStages, parity = ((g / L::kStages) & 1) ^ 1;
-        if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.k_empty[s], parity)))) break;
-        put(k, to + s * L::kBlock);
-        if (lane == 0) mbar_arrive(&bar.k_full[s]);
-        fetch(k, j + 1, page, a.k, a.k_page, a.k_slot, a.k_head, p.k_scale, p.ks_page, p.ks_slot, p.ks_head);
-        if (j < full0 || j >= full1) {
-          // Some row does not see some key: scales that are no numbers are taken out (0 * NaN), and the
-          // epilogue adds NaN to the rows that see them.
-#pragma unroll
-          for (int i = 0; i < G / 2; ++i) {
-            if (non_finite<__nv_bfloat16>(v.s[i])) {
-              v.s[i] = finite_only<__nv_bfloat16>(v.s[i]);
-              w.wild = 1;
-            }
-          }
-        }
-        if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.v_empty[s], parity)))) break;
-        put(v, to + (v_s - k_s) + s * L::kBlock);
-        if (lane == 0) mbar_arrive(&bar.v_full[s]);
-        fetch(v, j + 1, page, a.v, a.v_page, a.v_slot, a.v_head, p.v_scale, p.vs_page, p.vs_slot, p.vs_head);
-        page = page_at(j + 2);
+        if (lane == 0) mbar_arrive(&full[stage]);
+        fetch(j + 1);
+        find(j + 2);
       }
       done_with(t);
     }
   } else if (warp >= 4) {
-    if constexpr (kInt4) fewer_registers<kIssueRegisters>();
+    if constexpr (kInt4) fewer_registers<kOtherRegisters>();
     if (warp == 4) {
       // ---------------- scores ----------------
       // The issuing warps walk the blocks whole, with values the compiler knows to be the same
@@ -731,7 +754,7 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads : kPrefillThreads, 2)
         if (describe(index, w)) {
           Work& slot = bar.work[t & 1];
           int entry = kInt4 ? -1 : entry_of(w, 0);
-          if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.work_empty[t & 1], ((t >> 1) & 1) ^ 1)))) {
+          if (!(ok = __all_sync(0xffffffffu, wait_idle(&bar.work_empty[t & 1], ((t >> 1) & 1) ^ 1)))) {
             leave(w);
             break;
           }
@@ -744,7 +767,7 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads : kPrefillThreads, 2)
           if constexpr (kInt4) {
             // K and V are other warps' work here.
             if (w.blocks) {
-              if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.q_empty, (queries & 1) ^ 1)))) break;
+              if (!(ok = __all_sync(0xffffffffu, wait_idle(&bar.q_empty, (queries & 1) ^ 1)))) break;
               ++queries;
               if (lane == 0) {
                 mbar_arrive_expect_tx(&bar.q_full, p.tile_tokens * a.group * 128 * L::kHalves);
@@ -791,7 +814,7 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads : kPrefillThreads, 2)
         }
         __syncwarp();
         asking = true;
-        if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.next_here, asked++ & 1)))) break;
+        if (!(ok = __all_sync(0xffffffffu, wait_idle(&bar.next_here, asked++ & 1)))) break;
         asking = false;
         index = __shfl_sync(0xffffffffu, next_cta(answer), 0);
       }
