@@ -28,13 +28,15 @@
 // four warps take neighbouring heads of the same keys where there are such, since
 // their rows lie next to each other.
 #include "paged_runs.cuh"
+#include "tensor_map.h"
+#include "umma_util.cuh"
 
 namespace flash_prologue {
 namespace {
 
-constexpr int kHalves = 1;           // 16-key halves of a warp's step
-constexpr int kStepKeys = kHalves * kWarpKeys;
-constexpr int kRing = 4;             // steps of a warp's ring
+constexpr int kRing = 4;             // steps of a ring
+constexpr int kAhead = 2;            // steps that a CTA's common ring is loaded ahead
+constexpr int kBlockKeys = kWarpKeys * kDecodeWarps;
 constexpr int kCtasPerSm = 4;
 constexpr int kLeastScale = -80;     // least exponent of sigma: sums of 2^(15 + 80) stay inside FP32
 constexpr float kNoTop = -3e38f;      // the maximum of a row that has seen no key
@@ -110,22 +112,66 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[G], uint32_t addr) {
   }
 }
 
-// A half step's 16 keys of one row of codes each. Slot k of the products (rows of S, columns of
-// V^T) is key key_of(k): with it the 8 lanes (16 at D = 64) that read shared memory at once
-// find their pieces in different banks, both for K (4 pieces of neighbouring slots) and for
-// V (few pieces of every other slot), where pieces lie as at() says.
-__device__ __forceinline__ int key_of(int slot) { return slot ^ (slot >> 1 & 1); }
+// A step's 16 keys of a head, one row of codes each. Slot k of the products (rows of S, columns of
+// V^T) is key key_of(k), and a row's pieces lie as at() says, which is how a tensor map with 64-byte
+// (32-byte) swizzle lays out rows of 64 (32) bytes. So the 8 lanes (16 at D = 64) that read shared memory
+// at once find their pieces in different banks, both for K (4 pieces of neighbouring slots) and for V
+// (few pieces of every other slot).
+template <int D>
+__device__ __forceinline__ int key_of(int slot) { return slot ^ (D == 128 ? slot >> 1 & 1 : slot >> 2 & 1); }
 template <int D>
 __device__ __forceinline__ int at(int key, int piece) {  // bytes; piece 0 .. 3 of a row
-  if constexpr (D == 128) return key * 64 + ((piece ^ (key >> 1 & 2)) * 16);
-  else return (key ^ (key >> 2 & 1)) * 32 + piece * 8;
+  if constexpr (D == 128) return key * 64 + ((piece ^ (key >> 1 & 3)) * 16);
+  else return key * 32 + (((piece >> 1) ^ (key >> 2 & 1)) * 16) + (piece & 1) * 8;
 }
 
 template <int D>
-struct Half {
-  static constexpr int kCodes = kWarpKeys * D / 2, kScale = kWarpKeys * D / 16;
-  static constexpr int kV = kCodes, kKScale = 2 * kCodes, kVScale = 2 * kCodes + kScale, kBytes = 2 * (kCodes + kScale);
+struct Step {  // bytes of a head's step: K, V, scales of K, scales of V
+  static constexpr int kCodes = kWarpKeys * D / 2, kScale = kWarpKeys * D / 16, kBytes = 2 * (kCodes + kScale);
 };
+
+// A cache as the copies of a CTA's four heads see it (HEADS 4, pages of 16 slots at least, scales next to each
+// other along the heads or along the slots).
+struct Maps {
+  CUtensorMap k, v, k_scale, v_scale;
+  int scales_by_slot;  // a step's scales lie [head][slot] in memory, else [slot][head]
+};
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+      : "memory");
+}
+// True when the phase is complete; false (and the error word) after about 4 s.
+__device__ __forceinline__ bool phase_wait(uint64_t* bar, uint32_t parity) {
+  constexpr long long kMostCycles = 8000000000ll;
+  const uint32_t b = smem_u32(bar);
+  const auto done = [&] {
+    uint32_t d;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(d) : "r"(b), "r"(parity) : "memory");
+    return d != 0;
+  };
+  if (done()) return true;
+  const long long start = clock64();
+  do {
+    if (done()) return true;
+  } while (clock64() - start < kMostCycles);
+  atomicOr(&g_device_error, kDeviceErrorTimeout);
+  return false;
+}
 
 struct Int4Args {
   AttentionArgs a;  // k, v: codes, strides in bytes
@@ -134,23 +180,38 @@ struct Int4Args {
   int64_t ks_page, ks_slot, ks_head, vs_page, vs_slot, vs_head;  // elements
 };
 
-// NT tiles of 8 rows; HEADS key heads a CTA, so 4 / HEADS warps share a head's keys.
-template <typename T, int D, int NT, int HEADS>
-__global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 128 ? 3 : 4 : 2) paged_int4_decode_kernel(const Int4Args args) {
+// NT tiles of 8 rows; HEADS key heads a CTA, so 4 / HEADS warps share a head's keys. TMA: the four heads'
+// steps come by tensor copies into a ring of the CTA, issued by its warps in turn; else every warp loads its
+// own with cp.async.
+template <typename T, int D, int NT, int HEADS, bool TMA>
+__global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
+    paged_int4_decode_kernel(const Int4Args args, const __grid_constant__ Maps maps) {
   const AttentionArgs& a = args.a;
-  constexpr int kRows = 8 * NT, kSplit = kDecodeWarps / HEADS, kBlockKeys = kStepKeys * kSplit;
+  static_assert(!TMA || HEADS == kDecodeWarps, "a warp a head");
+  constexpr int kRows = 8 * NT, kSplit = kDecodeWarps / HEADS, kStepKeys = kWarpKeys * kSplit;  // keys of a CTA's step
   constexpr int G = D / 32;  // groups of channels; words of a piece
+  constexpr int kPerBlock = kBlockKeys / kStepKeys;
   using Tiles = Tiling<kRows, kBlockKeys, HEADS>;
-  using S = Half<D>;
-  extern __shared__ __align__(128) unsigned char smem[];
+  using S = Step<D>;
+  extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ RunScratch shared;
   __shared__ float stat[kDecodeWarps][kRows][2];
   __shared__ int bad_page;
+  __shared__ uint64_t full[kRing], empty[kRing];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr uint32_t kStage = kHalves * S::kBytes;
-  const uint32_t ring = smem_u32(smem) + warp * kRing * kStage, ring_end = ring + kRing * kStage;
+  constexpr uint32_t kStage = TMA ? kDecodeWarps * S::kBytes : S::kBytes;
+  const uint32_t ring = smem_u32(smem) + (TMA ? 0 : warp * kRing * kStage), ring_end = ring + kRing * kStage;
 
   if (!a.whole) start_next_kernel();
+  if constexpr (TMA) {
+    if (threadIdx.x == 0) {
+      for (int s = 0; s < kRing; ++s) {
+        mbar_init(&full[s], 1);
+        mbar_init(&empty[s], kDecodeWarps);
+      }
+      fence_mbar_init();
+    }
+  }
   const int64_t slots = 2 * (int64_t)gridDim.x, cta = blockIdx.x;
   float* part_out = static_cast<float*>(a.workspace);                            // [slots][HEADS][kRows][D]
   float* part_stat = part_out + slots * HEADS * kRows * D;                       // [slots][HEADS][kRows][2]
@@ -159,21 +220,22 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 128 ? 3 : 4 : 2
   if (!find_run<Tiles>(a, shared, parts, run)) return;
 
   // This lane's places in the products. K: slots j and j + 8, piece p of the row. V: piece and
-  // half (even or odd channels) of the words, slots 2 p, 2 p + 1 and 8 more.
+  // half (even or odd channels) of the words, slots 2 p, 2 p + 1 and 8 more. In bytes of a stage.
   const int j = lane / 4, p = lane % 4;
-  const uint32_t k_at = at<D>(key_of(j), p);  // key + 8: kWarpKeys * D / 4 bytes on
-  const uint32_t v_at[2] = {(uint32_t)at<D>(key_of(2 * p), j % 4) + S::kV, (uint32_t)at<D>(key_of(2 * p + 1), j % 4) + S::kV};
-  const uint32_t scale_at = S::kKScale + key_of(j) * (D / 16);
-  constexpr int kEight = kWarpKeys * D / 4;
+  constexpr int kEight = kWarpKeys * D / 4;  // 8 keys on
+  const uint32_t codes_at = TMA ? warp * S::kCodes : 0, v_codes = (TMA ? kDecodeWarps : 1) * S::kCodes + codes_at;
+  const uint32_t k_at = codes_at + at<D>(key_of<D>(j), p);
+  const uint32_t v_at[2] = {v_codes + at<D>(key_of<D>(2 * p), j % 4), v_codes + at<D>(key_of<D>(2 * p + 1), j % 4)};
   const uint32_t half_of = j / 4 ? 0x7632u : 0x5410u;
-  // Its places in the loads: a 16-byte chunk of K and of V in each pass over a step's rows, a row's
-  // scales of K (lanes 0 .. 15) or V.
-  constexpr int kChunks = D / 32, kPasses = kChunks / 2;
-  const int load_row = lane / kChunks, chunk = lane % kChunks;
-  const uint32_t load_at = at<D>(load_row, chunk * (4 / kChunks));  // (a piece is half a chunk at D = 64)
-  const uint32_t scale_to = (lane < 16 ? S::kKScale : S::kVScale) + (lane & 15) * (D / 16);
+  const bool by_head = TMA && !maps.scales_by_slot;  // [slot][head]
+  const uint32_t scale_pitch = by_head ? kDecodeWarps * D / 16 : D / 16, scale_eight = 8 * scale_pitch;
+  const uint32_t ks_at = (TMA ? 2 * kDecodeWarps : 2) * S::kCodes + (!TMA ? 0 : by_head ? warp * (D / 16) : warp * S::kScale) +
+                         key_of<D>(j) * scale_pitch;
+  const uint32_t vs_at = ks_at + (TMA ? kDecodeWarps : 1) * S::kScale;
   const bool wide = a.pages.page_log2 >= 4;  // a step's keys are in one page
   const int in_page = (1 << a.pages.page_log2) - 1;
+  [[maybe_unused]] uint32_t loads = 0;  // steps of the CTA's items before this one (stages and phases go on)
+  [[maybe_unused]] bool lost = false;   // a wait ran out: no more copies or products
 
   for (int64_t unit = run.begin; unit < run.end;) {
     Item it;
@@ -256,97 +318,24 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 128 ? 3 : 4 : 2
     __syncthreads();
 
     // Positions relative to this warp's first key, in 32 bits (a request has fewer than 2^30 keys).
-    const int steps = idle ? 0 : b1 - b0;
-    const int warp_key = it.key0 + b0 * kBlockKeys + warp / HEADS * kStepKeys;
+    const int steps = idle ? 0 : (b1 - b0) * kPerBlock;
+    const int warp_key = it.key0 + b0 * kBlockKeys + warp / HEADS * kWarpKeys;
     const int key_lo = it.lo - warp_key, key_hi = it.hi - warp_key;
     const int all_lo = a.window ? base + (row0 + rows - 1) / a.group - a.window + 1 - warp_key : kNone;
     const int all_hi = base + row0 / a.group - warp_key;  // every row sees keys all_lo .. all_hi
     const int32_t* table = a.pages.page_table + (int64_t)it.r * a.pages.table_stride;
-    // Strides of slots and pages take 31 bits (the host checks): a product and a sum in one instruction.
-    const unsigned char* k_lane = static_cast<const unsigned char*>(a.k) + head * a.k_head + (load_row & 7) * a.k_slot + chunk * 16;
-    const unsigned char* v_lane = static_cast<const unsigned char*>(a.v) + head * a.v_head + (load_row & 7) * a.v_slot + chunk * 16;
-    const unsigned char* s_lane = reinterpret_cast<const unsigned char*>(
-        lane < 16 ? args.k_scale + head * args.ks_head + (lane & 7) * args.ks_slot
-                  : args.v_scale + head * args.vs_head + (lane & 7) * args.vs_slot);
-    const int k_page = (int)a.k_page, k_slot = (int)a.k_slot, v_page = (int)a.v_page, v_slot = (int)a.v_slot;
-    const int s_page = 2 * (int)(lane < 16 ? args.ks_page : args.vs_page), s_slot = 2 * (int)(lane < 16 ? args.ks_slot : args.vs_slot);
-    const auto along = [](const unsigned char* from, int n, int stride) { return from + (int64_t)n * stride; };
-    // Pages of the keys of step page_step + lane, eight by eight (sixteen where they are in one page); -1: none.
-    int page_of[2 * kHalves];
-    int page_left = 0;  // steps that they still cover
-    uint32_t to = ring;
-    const auto load = [&](int step) {
-      if (step < steps) {
-        if (page_left == 0) {
-          page_left = 32;
-#pragma unroll
-          for (int s = 0; s < 2 * kHalves; ++s) {
-            const int k = (step + lane) * kBlockKeys + s * 8;
-            page_of[s] = -1;
-            if (wide && s % 2) continue;
-            if (step + lane < steps && k < key_hi && k + (wide ? 16 : 8) > key_lo) {
-              const int page = __ldg(table + ((warp_key + k) >> a.pages.page_log2));
-              if (page >= 0 && page < a.pages.num_pages) page_of[s] = page;
-              else bad_page = 1;
-            }
-          }
-        }
-        const int from = 32 - page_left--;
-        const int key = step * kBlockKeys, row = lane & 15;
-        const bool inside = key >= key_lo && key + kStepKeys <= key_hi;
-        // Codes of slots outside the tile's keys are whatever they are: their scales are zeros.
-#pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-          const uint32_t dst = to + h * S::kBytes;
-          const int first = key + h * kWarpKeys;
-          const int page0 = __shfl_sync(0xffffffffu, page_of[2 * h], from), slot0 = (warp_key + first) & in_page;
-          const bool ok = inside || (first + row >= key_lo && first + row < key_hi);
-          if (wide && page0 >= 0) {
-            const unsigned char* k = along(along(k_lane, page0, k_page), slot0, k_slot);
-            const unsigned char* v = along(along(v_lane, page0, v_page), slot0, v_slot);
-            if constexpr (kPasses == 1) {
-              k = along(k, load_row & 8, k_slot);
-              v = along(v, load_row & 8, v_slot);
-            }
-#pragma unroll
-            for (int i = 0; i < kPasses; ++i) {
-              cp_async16(dst + load_at + i * kEight, along(k, 8 * i, k_slot), true);
-              cp_async16(dst + load_at + S::kV + i * kEight, along(v, 8 * i, v_slot), true);
-            }
-            cp_async_small<D / 16>(dst + scale_to, along(along(s_lane, page0, s_page), slot0 + (row & 8), s_slot), ok);
-          } else {
-            // Pages of 8 slots, or none.
-            const int page1 = __shfl_sync(0xffffffffu, page_of[2 * h + 1], from), slot1 = (warp_key + first + 8) & in_page;
-#pragma unroll
-            for (int i = 0; i < kPasses; ++i) {
-              const bool second = kPasses == 1 ? load_row >= 8 : i == 1;
-              const int page = second ? page1 : page0, slot = second ? slot1 : slot0, there = max(page, 0);
-              cp_async16(dst + load_at + i * kEight, along(along(k_lane, there, k_page), slot, k_slot), page >= 0);
-              cp_async16(dst + load_at + S::kV + i * kEight, along(along(v_lane, there, v_page), slot, v_slot), page >= 0);
-            }
-            const int page = row & 8 ? page1 : page0, slot = row & 8 ? slot1 : slot0;
-            cp_async_small<D / 16>(dst + scale_to, along(along(s_lane, max(page, 0), s_page), slot, s_slot), page >= 0 && ok);
-          }
-        }
-        to += kStage;
-        if (to == ring_end) to = ring;
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
     // A step's scores, probabilities and product; EDGE: some row does not see some key.
     const auto compute = [&](auto edge, uint32_t here, int key) {
       constexpr bool EDGE = decltype(edge)::value;
-      // Sums of a half's keys key_of(j) and 8 more (x / 2), columns 2 p and 2 p + 1 (x % 2).
-      float s[kHalves][NT][4] = {};
-#pragma unroll
-      for (int h = 0; h < kHalves; ++h) {
-        const uint32_t at_half = here + h * S::kBytes;
+      // Sums of keys key_of(j) and 8 more (x / 2), columns 2 p and 2 p + 1 (x % 2).
+      float s[NT][4] = {};
+      {
         uint32_t wa[G], wb[G];
-        load_words<G>(wa, at_half + k_at);
-        load_words<G>(wb, at_half + k_at + kEight);
+        load_words<G>(wa, here + k_at);
+        load_words<G>(wb, here + k_at + kEight);
         Scales<G> sa, sb;
-        sa.load(at_half + scale_at);
-        sb.load(at_half + scale_at + 8 * (D / 16));
+        sa.load(here + ks_at);
+        sb.load(here + ks_at + scale_eight);
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           const uint32_t ua = wa[g] >> 8, ub = wb[g] >> 8;
@@ -358,50 +347,42 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 128 ? 3 : 4 : 2
                     start[n][g][1], start[n][g][0], start[n][g][1]);
             mma_f16(c, ua & kLow, ub & kLow, ua & kHigh, ub & kHigh, qf[n][g][2], qf[n][g][3], c[0], c[1], c[2], c[3]);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) s[h][n][x] = fmaf(c[x], x < 2 ? fa : fb, s[h][n][x]);
+            for (int x = 0; x < 4; ++x) s[n][x] = fmaf(c[x], x < 2 ? fa : fb, s[n][x]);
           }
         }
       }
-      Scales<G> va[kHalves], vb[kHalves];
-      float largest = 0.f;
+      Scales<G> va, vb;
+      va.load(here + vs_at);
+      vb.load(here + vs_at + scale_eight);
+      float fa[G], fb[G], largest = 0.f;
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) {
-        const uint32_t at_scales = here + h * S::kBytes + scale_at + S::kVScale - S::kKScale;
-        va[h].load(at_scales);
-        vb[h].load(at_scales + 8 * (D / 16));
-#pragma unroll
-        for (int g = 0; g < G; ++g) largest = fmaxf(largest, fmaxf(fabsf(va[h].get(g)), fabsf(vb[h].get(g))));
+      for (int g = 0; g < G; ++g) {
+        fa[g] = va.get(g);
+        fb[g] = vb.get(g);
+        largest = fmaxf(largest, fmaxf(fabsf(fa[g]), fabsf(fb[g])));
       }
-      const auto sees = [&](int h, int n, int x) {
-        const int k = warp_key + key + h * kWarpKeys + key_of(j) + (x / 2) * 8, hi = see_hi[n][x & 1];
+      const auto sees = [&](int n, int x) {
+        const int k = warp_key + key + key_of<D>(j) + (x / 2) * 8, hi = see_hi[n][x & 1];
         return k <= hi && (!a.window || k > hi - a.window);
       };
-      float w[kHalves][NT][4];  // probabilities times 2^(7 - sigma)
+      float w[NT][4];  // probabilities times 2^(7 - sigma)
       bool move = EDGE || largest >= limit;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        float most[2] = {0.f, 0.f};
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            w[h][n][x] = exp2_approx(fmaf(s[h][n][x], row_scale[n][x & 1], -from[n][x & 1]));
-            most[x & 1] = fmaxf(most[x & 1], w[h][n][x]);
-          }
-        move |= most[0] > over[n][0] || most[1] > over[n][1];
+        for (int x = 0; x < 4; ++x) w[n][x] = exp2_approx(fmaf(s[n][x], row_scale[n][x & 1], -from[n][x & 1]));
+        move |= fmaxf(w[n][0], w[n][2]) > over[n][0] || fmaxf(w[n][1], w[n][3]) > over[n][1];
       }
       if (__any_sync(0xffffffffu, move)) {
         // A row's maximum or its largest scale may have moved: its O and sums follow. Each row goes by
         // the keys that it sees, so what others see does not change its bits.
-        float size[kHalves][2] = {};  // largest scale of this lane's keys; infinities and NaNs lose their own group only
+        float size[2] = {0.f, 0.f};  // largest scale of this lane's keys; infinities and NaNs lose their own group only
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h)
-#pragma unroll
-          for (int g = 0; g < G; ++g) {
-            const float x = fabsf(va[h].get(g)), y = fabsf(vb[h].get(g));
-            if (x < INFINITY) size[h][0] = fmaxf(size[h][0], x);
-            if (y < INFINITY) size[h][1] = fmaxf(size[h][1], y);
-          }
+        for (int g = 0; g < G; ++g) {
+          const float x = fabsf(fa[g]), y = fabsf(fb[g]);
+          if (x < INFINITY) size[0] = fmaxf(size[0], x);
+          if (y < INFINITY) size[1] = fmaxf(size[1], y);
+        }
         int least = 127;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -409,13 +390,11 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 128 ? 3 : 4 : 2
           for (int x = 0; x < 2; ++x) {
             float most = kNoTop, big = 0.f;
 #pragma unroll
-            for (int h = 0; h < kHalves; ++h)
-#pragma unroll
-              for (int y = 0; y < 2; ++y) {
-                if (EDGE && !sees(h, n, x + 2 * y)) continue;
-                most = fmaxf(most, s[h][n][x + 2 * y] * row_scale[n][x]);
-                big = fmaxf(big, size[h][y]);
-              }
+            for (int y = 0; y < 2; ++y) {
+              if (EDGE && !sees(n, x + 2 * y)) continue;
+              most = fmaxf(most, s[n][x + 2 * y] * row_scale[n][x]);
+              big = fmaxf(big, size[y]);
+            }
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) {
               most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
@@ -437,66 +416,183 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 128 ? 3 : 4 : 2
                 eights[n][g][2 * r + x] *= f;
               }
 #pragma unroll
-            for (int h = 0; h < kHalves; ++h)
-#pragma unroll
-              for (int y = 0; y < 2; ++y)
-                w[h][n][x + 2 * y] = exp2_approx(fmaf(s[h][n][x + 2 * y], row_scale[n][x], -from[n][x]));
+            for (int y = 0; y < 2; ++y)
+              w[n][x + 2 * y] = exp2_approx(fmaf(s[n][x + 2 * y], row_scale[n][x], -from[n][x]));
           }
         limit = power_of_two(least);
       }
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) {
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int x = 0; x < 4; ++x) {
+          if (EDGE && !sees(n, x)) w[n][x] = 0.f;
+          sum[n][x & 1] += w[n][x];
+        }
+      // Channels of this lane: words j % 4 of the four keys, even or odd ones.
+      uint32_t w0[G], w1[G], w8[G], w9[G];
+      load_words<G>(w0, here + v_at[0]);
+      load_words<G>(w1, here + v_at[1]);
+      load_words<G>(w8, here + v_at[0] + kEight);
+      load_words<G>(w9, here + v_at[1] + kEight);
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            if (EDGE && !sees(h, n, x)) w[h][n][x] = 0.f;
-            sum[n][x & 1] += w[h][n][x];
+      for (int g = 0; g < G; ++g) {
+        const uint32_t x = __byte_perm(w0[g], w1[g], half_of), y = __byte_perm(w8[g], w9[g], half_of);
+        const uint32_t x8 = x >> 8, y8 = y >> 8;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float z[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            z[i] = w[n][i] * (i < 2 ? fa[g] : fb[g]);
+            if (EDGE && !sees(n, i)) z[i] = 0.f;  // whatever the scale is
           }
-        // Channels of this lane: words j % 4 of the four keys, even or odd ones.
-        const uint32_t at_half = here + h * S::kBytes;
-        uint32_t w0[G], w1[G], w8[G], w9[G];
-        load_words<G>(w0, at_half + v_at[0]);
-        load_words<G>(w1, at_half + v_at[1]);
-        load_words<G>(w8, at_half + v_at[0] + kEight);
-        load_words<G>(w9, at_half + v_at[1] + kEight);
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-          const uint32_t x = __byte_perm(w0[g], w1[g], half_of), y = __byte_perm(w8[g], w9[g], half_of);
-          const uint32_t x8 = x >> 8, y8 = y >> 8;
-          const float fa = va[h].get(g), fb = vb[h].get(g);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float z[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              z[i] = w[h][n][i] * (i < 2 ? fa : fb);
-              if (EDGE && !sees(h, n, i)) z[i] = 0.f;  // whatever the scale is
-            }
-            const uint32_t w_lo = transposed(half2_of(z[0], z[1])), w_hi = transposed(half2_of(z[2], z[3]));
-            float (&o0)[4] = acc[n][g][0], (&o1)[4] = acc[n][g][1], (&e)[4] = eights[n][g];
-            mma_f16(o0, x & kLow, x & kHigh, y & kLow, y & kHigh, w_lo, w_hi, o0[0], o0[1], o0[2], o0[3]);
-            mma_f16(o1, x8 & kLow, x8 & kHigh, y8 & kLow, y8 & kHigh, w_lo, w_hi, o1[0], o1[1], o1[2], o1[3]);
-            mma_f16(e, 0x00080008u, 0x00800080u, 0x00080008u, 0x00800080u, w_lo, w_hi, e[0], e[1], e[2], e[3]);
-          }
+          const uint32_t w_lo = transposed(half2_of(z[0], z[1])), w_hi = transposed(half2_of(z[2], z[3]));
+          float (&o0)[4] = acc[n][g][0], (&o1)[4] = acc[n][g][1], (&e)[4] = eights[n][g];
+          mma_f16(o0, x & kLow, x & kHigh, y & kLow, y & kHigh, w_lo, w_hi, o0[0], o0[1], o0[2], o0[3]);
+          mma_f16(o1, x8 & kLow, x8 & kHigh, y8 & kLow, y8 & kHigh, w_lo, w_hi, o1[0], o1[1], o1[2], o1[3]);
+          mma_f16(e, 0x00080008u, 0x00800080u, 0x00080008u, 0x00800080u, w_lo, w_hi, e[0], e[1], e[2], e[3]);
         }
       }
     };
+    const auto products = [&](uint32_t here, int key) {
+      if (key >= all_lo && key + kWarpKeys - 1 <= all_hi) compute(std::false_type{}, here, key);
+      else if (key < key_hi && key + kWarpKeys > key_lo) compute(std::true_type{}, here, key);
+    };
+    if constexpr (TMA) {
+      // Steps with keys that some row sees; warp i % 4 has the copies of step i.
+      const int step0 = max(key_lo, 0) / kWarpKeys, count = max(min(steps, (key_hi + kWarpKeys - 1) / kWarpKeys) - step0, 0);
+      int page_of = -1;  // page of step 4 (lane + 32 n) + warp
+      uint32_t issued = loads, load = loads;  // this warp's last copies, the step that is waited for
+      const auto issue = [&](int i) {
+        if (i >= count || (i & 3) != warp || lost) return;
+        const int mine = i >> 2;
+        if ((mine & 31) == 0) {
+          const int step = (mine + lane) * 4 + warp;
+          page_of = step < count ? __ldg(table + ((warp_key + (step0 + step) * kWarpKeys) >> a.pages.page_log2)) : -1;
+        }
+        const int page = __shfl_sync(0xffffffffu, page_of, mine & 31), slot = (warp_key + (step0 + i) * kWarpKeys) & in_page;
+        const uint32_t load = loads + i, s = load % kRing, dst = ring + s * kStage;
+        issued = load;
+        if (!(lost = !__all_sync(0xffffffffu, phase_wait(&empty[s], (load / kRing & 1) ^ 1)))) {
+          if (lane == 0) {
+            if (page >= 0 && page < a.pages.num_pages) {
+              mbar_arrive_expect_tx(&full[s], kStage);
+              tma_load_4d(dst, &maps.k, 0, slot, it.head, page, &full[s]);
+              tma_load_4d(dst + kDecodeWarps * S::kCodes, &maps.v, 0, slot, it.head, page, &full[s]);
+              const uint32_t scales = dst + 2 * kDecodeWarps * S::kCodes;
+              const int c0 = by_head ? it.head * G : slot * G, c1 = by_head ? slot : it.head;
+              tma_load_3d(scales, &maps.k_scale, c0, c1, page, &full[s]);
+              tma_load_3d(scales + kDecodeWarps * S::kScale, &maps.v_scale, c0, c1, page, &full[s]);
+            } else {
+              bad_page = 1;
+              mbar_arrive(&full[s]);
+            }
+          }
+          __syncwarp();
+        }
+      };
 #pragma unroll
-    for (int s = 0; s < kRing - 1; ++s) load(s);
-
-    uint32_t here = ring;
-    for (int step = 0; step < steps; ++step) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
-      __syncwarp();
-      load(step + kRing - 1);
-      const int key = step * kBlockKeys;
-      if (key >= all_lo && key + kStepKeys - 1 <= all_hi) compute(std::false_type{}, here, key);
-      else if (key < key_hi && key + kStepKeys > key_lo) compute(std::true_type{}, here, key);
-      here += kStage;
-      if (here == ring_end) here = ring;
+      for (int i = 0; i < kAhead; ++i) issue(i);
+      for (int i = 0; i < count && !lost; ++i) {
+        issue(i + kAhead);
+        load = loads + i;
+        const uint32_t s = load % kRing;
+        if (lost || (lost = !__all_sync(0xffffffffu, phase_wait(&full[s], load / kRing & 1)))) break;
+        products(ring + s * kStage, (step0 + i) * kWarpKeys);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[s]);
+      }
+      loads += count;
+      if (lost) {
+        bad_page = 1;  // rows without their keys are NaN
+        // Copies of this warp that are under way have to arrive before the CTA goes on or ends.
+        for (; load <= issued; ++load) phase_wait(&full[load % kRing], load / kRing & 1);
+      }
+    } else {
+      // Its places in the loads: a 16-byte chunk of K and of V in each pass over a step's rows, a row's scales of
+      // K (lanes 0 .. 15) or V. Strides of slots and pages take 31 bits (the host checks): a product and a sum
+      // in one instruction.
+      constexpr int kChunks = D / 32, kPasses = kChunks / 2;
+      const int load_row = lane / kChunks, chunk = lane % kChunks;
+      const uint32_t load_at = at<D>(load_row, chunk * (4 / kChunks));  // (a piece is half a chunk at D = 64)
+      const uint32_t scale_to = 2 * S::kCodes + (lane < 16 ? 0 : S::kScale) + (lane & 15) * (D / 16);
+      const unsigned char* k_lane = static_cast<const unsigned char*>(a.k) + head * a.k_head + (load_row & 7) * a.k_slot + chunk * 16;
+      const unsigned char* v_lane = static_cast<const unsigned char*>(a.v) + head * a.v_head + (load_row & 7) * a.v_slot + chunk * 16;
+      const unsigned char* s_lane = reinterpret_cast<const unsigned char*>(
+          lane < 16 ? args.k_scale + head * args.ks_head + (lane & 7) * args.ks_slot
+                    : args.v_scale + head * args.vs_head + (lane & 7) * args.vs_slot);
+      const int k_page = (int)a.k_page, k_slot = (int)a.k_slot, v_page = (int)a.v_page, v_slot = (int)a.v_slot;
+      const int s_page = 2 * (int)(lane < 16 ? args.ks_page : args.vs_page), s_slot = 2 * (int)(lane < 16 ? args.ks_slot : args.vs_slot);
+      const auto along = [](const unsigned char* from, int n, int stride) { return from + (int64_t)n * stride; };
+      // Pages of the keys of step page_step + lane, sixteen keys or (pages of 8) either half of them; -1: none.
+      int page_of[2] = {-1, -1};
+      int page_left = 0;  // steps that they still cover
+      uint32_t to = ring;
+      const auto load = [&](int step) {
+        if (step < steps) {
+          if (page_left == 0) {
+            page_left = 32;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              const int k = (step + lane) * kStepKeys + s * 8;
+              page_of[s] = -1;
+              if (wide && s) continue;
+              if (step + lane < steps && k < key_hi && k + (wide ? 16 : 8) > key_lo) {
+                const int page = __ldg(table + ((warp_key + k) >> a.pages.page_log2));
+                if (page >= 0 && page < a.pages.num_pages) page_of[s] = page;
+                else bad_page = 1;
+              }
+            }
+          }
+          const int from_lane = 32 - page_left--;
+          const int key = step * kStepKeys, row = lane & 15;
+          // Codes of slots outside the tile's keys are whatever they are: their scales are zeros.
+          const int page0 = __shfl_sync(0xffffffffu, page_of[0], from_lane), slot0 = (warp_key + key) & in_page;
+          const bool ok = key + row >= key_lo && key + row < key_hi;
+          if (wide && page0 >= 0) {
+            const unsigned char* k = along(along(k_lane, page0, k_page), slot0, k_slot);
+            const unsigned char* v = along(along(v_lane, page0, v_page), slot0, v_slot);
+            if constexpr (kPasses == 1) {
+              k = along(k, load_row & 8, k_slot);
+              v = along(v, load_row & 8, v_slot);
+            }
+#pragma unroll
+            for (int i = 0; i < kPasses; ++i) {
+              cp_async16(to + load_at + i * kEight, along(k, 8 * i, k_slot), true);
+              cp_async16(to + load_at + S::kCodes + i * kEight, along(v, 8 * i, v_slot), true);
+            }
+            cp_async_small<D / 16>(to + scale_to, along(along(s_lane, page0, s_page), slot0 + (row & 8), s_slot), ok);
+          } else {
+            // Pages of 8 slots, or none.
+            const int page1 = __shfl_sync(0xffffffffu, page_of[1], from_lane), slot1 = (warp_key + key + 8) & in_page;
+#pragma unroll
+            for (int i = 0; i < kPasses; ++i) {
+              const bool second = kPasses == 1 ? load_row >= 8 : i == 1;
+              const int page = second ? page1 : page0, slot = second ? slot1 : slot0, there = max(page, 0);
+              cp_async16(to + load_at + i * kEight, along(along(k_lane, there, k_page), slot, k_slot), page >= 0);
+              cp_async16(to + load_at + S::kCodes + i * kEight, along(along(v_lane, there, v_page), slot, v_slot), page >= 0);
+            }
+            const int page = row & 8 ? page1 : page0, slot = row & 8 ? slot1 : slot0;
+            cp_async_small<D / 16>(to + scale_to, along(along(s_lane, max(page, 0), s_page), slot, s_slot), page >= 0 && ok);
+          }
+          to += kStage;
+          if (to == ring_end) to = ring;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+#pragma unroll
+      for (int s = 0; s < kRing - 1; ++s) load(s);
+      uint32_t here = ring;
+      for (int step = 0; step < steps; ++step) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+        __syncwarp();
+        load(step + kRing - 1);
+        products(here, step * kStepKeys);
+        here += kStage;
+        if (here == ring_end) here = ring;
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
 
     // The sums of the warps that share a head's keys, joined.
@@ -560,18 +656,19 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 128 ? 3 : 4 : 2
     }
     if (threadIdx.x == 0 && b0 == 0 && b1 < it.blocks) parts[cta] = part_of(run, it);
     unit = it.item_start + it.u1;
+    if constexpr (TMA) fence_proxy_async_smem();  // the next copies come to lie where the sums were
     __syncthreads();
   }
 }
 
-template <typename T, int D, int NT, int HEADS>
-cudaError_t launch(Int4Args args, cudaStream_t stream) {
+template <typename T, int D, int NT, int HEADS, bool TMA>
+cudaError_t launch(Int4Args args, const Maps& maps, cudaStream_t stream) {
   AttentionArgs& a = args.a;
-  constexpr int kRows = 8 * NT, kBlockKeys = kStepKeys * kDecodeWarps / HEADS;
-  a.whole = a.max_keys <= kWholeKeys / HEADS;
-  constexpr size_t ring = (size_t)kDecodeWarps * kRing * kHalves * Half<D>::kBytes, joined = (size_t)kDecodeWarps * kRows * D * 4;
+  constexpr int kRows = 8 * NT;
+  a.whole = a.max_keys <= kWholeKeys;
+  constexpr size_t ring = (size_t)kDecodeWarps * kRing * Step<D>::kBytes, joined = (size_t)kDecodeWarps * kRows * D * 4;
   constexpr size_t smem = ring > joined ? ring : joined;
-  const void* fn = reinterpret_cast<const void*>(&paged_int4_decode_kernel<T, D, NT, HEADS>);
+  const void* fn = reinterpret_cast<const void*>(&paged_int4_decode_kernel<T, D, NT, HEADS, TMA>);
   cudaError_t err = allow_shared_memory(fn, smem);
   if (err != cudaSuccess) return err;
   // Never more CTAs than there can be units.
@@ -584,11 +681,44 @@ cudaError_t launch(Int4Args args, cudaStream_t stream) {
   const int64_t want = tiles * ((a.kv_heads + HEADS - 1) / HEADS) * blocks, most = (int64_t)sms * kCtasPerSm;
   const int64_t grid = persistent_grid(fn, smem, want < most ? want : most, kDecodeThreads);
   if (grid <= 0) return cudaErrorInvalidConfiguration;
-  err = launch_kernel(paged_int4_decode_kernel<T, D, NT, HEADS>, dim3((unsigned)grid), dim3(kDecodeThreads), smem, stream, args);
+  err = launch_kernel(paged_int4_decode_kernel<T, D, NT, HEADS, TMA>, dim3((unsigned)grid), dim3(kDecodeThreads), smem, stream,
+                      args, maps);
   if (err != cudaSuccess || a.whole) return err;
   const unsigned rows = a.pages.cu_seqlens || a.group > kRows ? kRows : a.group;  // rows a tile can have
   return launch_following(paged_join_kernel<T, D, kRows, false, HEADS>, dim3((unsigned)grid, rows, HEADS), dim3(kJoinWarps * 32),
                           stream, a, grid);
+}
+
+// The maps of a cache that the copies of four heads can take: pages of 16 slots, four heads (or a multiple), scales
+// contiguous along the heads or along the slots, and what tensor maps want of strides.
+bool make_maps(const Int4Args& args, int D, Maps* maps) {
+  const AttentionArgs& a = args.a;
+  const uint64_t slots = (uint64_t)1 << a.pages.page_log2, heads = (uint64_t)a.kv_heads, pages = (uint64_t)a.pages.num_pages;
+  if (slots < kWarpKeys || heads % kDecodeWarps || pages == 0) return false;
+  const int G = D / 32;
+  const bool by_head = args.ks_head == G && args.vs_head == G, by_slot = args.ks_slot == G && args.vs_slot == G;
+  if (!by_head && !by_slot) return false;
+  maps->scales_by_slot = !by_head;
+  const auto positive = [](int64_t bytes) { return bytes > 0; };
+  const auto codes = [&](CUtensorMap* map, const void* base, int64_t slot, int64_t head, int64_t page) {
+    const uint64_t dims[4] = {(uint64_t)D / 2, slots, heads, pages};
+    const uint64_t strides[3] = {(uint64_t)slot, (uint64_t)head, pages > 1 ? (uint64_t)page : 128};
+    const uint32_t box[4] = {(uint32_t)D / 2, kWarpKeys, kDecodeWarps, 1};
+    return positive(slot) && positive(head) && (pages == 1 || positive(page)) &&
+           encode_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, base, dims, strides, box,
+                             D == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
+  };
+  const auto scales = [&](CUtensorMap* map, const void* base, int64_t slot, int64_t head, int64_t page) {
+    const uint64_t dims[3] = {(by_head ? heads : slots) * G, by_head ? slots : heads, pages};
+    const int64_t along = 2 * (by_head ? slot : head);
+    const uint64_t strides[2] = {(uint64_t)along, pages > 1 ? (uint64_t)(2 * page) : 128};
+    const uint32_t box[3] = {(uint32_t)((by_head ? kDecodeWarps : kWarpKeys) * G), (uint32_t)(by_head ? kWarpKeys : kDecodeWarps), 1};
+    return positive(along) && (pages == 1 || positive(page)) &&
+           encode_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+  };
+  return codes(&maps->k, a.k, a.k_slot, a.k_head, a.k_page) && codes(&maps->v, a.v, a.v_slot, a.v_head, a.v_page) &&
+         scales(&maps->k_scale, args.k_scale, args.ks_slot, args.ks_head, args.ks_page) &&
+         scales(&maps->v_scale, args.v_scale, args.vs_slot, args.vs_head, args.vs_page);
 }
 
 // Key heads of a CTA: a cache line holds the scales of several heads' slots, and is fetched
@@ -596,8 +726,10 @@ cudaError_t launch(Int4Args args, cudaStream_t stream) {
 template <typename T, int D, int NT>
 cudaError_t launch_heads(const Int4Args& args, cudaStream_t stream) {
   const int heads = args.a.kv_heads;
-  if (heads % 4 == 0 || heads % 4 == 3) return launch<T, D, NT, 4>(args, stream);
-  return heads % 2 == 0 ? launch<T, D, NT, 2>(args, stream) : launch<T, D, NT, 1>(args, stream);
+  Maps maps{};
+  if (make_maps(args, D, &maps)) return launch<T, D, NT, 4, true>(args, maps, stream);
+  if (heads % 4 == 0 || heads % 4 == 3) return launch<T, D, NT, 4, false>(args, maps, stream);
+  return heads % 2 == 0 ? launch<T, D, NT, 2, false>(args, maps, stream) : launch<T, D, NT, 1, false>(args, maps, stream);
 }
 
 template <typename T, int D>
