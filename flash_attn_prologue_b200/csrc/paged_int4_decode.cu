@@ -250,9 +250,10 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
     float start[NT][G][2];   // -8 sum of q over a group, of this lane's two columns 2 p and 2 p + 1
     float row_scale[NT][2];  // takes their sums to base-2 scores
     int see_hi[NT][2];       // last position that they see
+    const auto token_of = [&](int row) { return q.news == 1 ? 0 : (row0 + row) / a.group; };  // (a division)
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int row = 8 * n + j, of = row0 + row, i = of / a.group;
+      const int row = 8 * n + j, i = token_of(row);
       uint4 x[G];
       float most = 0.f;
 #pragma unroll
@@ -260,41 +261,36 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
         x[g] = make_uint4(0, 0, 0, 0);
         if (row < rows && !idle)
           x[g] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (q.first + i) * a.q_n +
-                                                      (head * a.group + (of - i * a.group)) * a.q_h + 8 * (p * G + g)));
+                                                      (head * a.group + (row0 + row - i * a.group)) * a.q_h + 8 * (p * G + g)));
         const T* v = reinterpret_cast<const T*>(&x[g]);
 #pragma unroll
         for (int c = 0; c < 8; ++c) most = fmaxf(most, fabsf((float)v[c]));
       }
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
       most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-      // The factor 2^(14 - exponent), in two steps: it may be beyond FP32's range.
-      const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -126), 127);
-      const float f0 = power_of_two((14 - e) / 2), f1 = power_of_two((14 - e) - (14 - e) / 2);
-      float sum[G];
+      // (rows below 2^-113 come out smaller: the factor is an FP32 number)
+      const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -113), 127);
+      const float f = power_of_two(14 - e), f16 = f * 0.0625f;  // the latter beside codes of 16 u
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         const T* v = reinterpret_cast<const T*>(&x[g]);
-        sum[g] = 0.f;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float f2 = c & 1 ? 0.0625f : 1.f;  // beside codes of 16 u
-          qf[n][g][c] = half2_of((float)v[2 * c] * f0 * f1 * f2, (float)v[2 * c + 1] * f0 * f1 * f2);
-          const float2 got = floats_of(qf[n][g][c]);
-          sum[g] += (got.x + got.y) * (c & 1 ? 16.f : 1.f);
-        }
-        sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 1);
-        sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
+        for (int c = 0; c < 4; ++c)
+          qf[n][g][c] = half2_of((float)v[2 * c] * (c & 1 ? f16 : f), (float)v[2 * c + 1] * (c & 1 ? f16 : f));
+        // As keys whose codes are all 8.
+        float c[4];
+        mma_f16(c, 0x00080008u, 0x00080008u, 0x00800080u, 0x00800080u, qf[n][g][0], qf[n][g][1], 0.f, 0.f, 0.f, 0.f);
+        mma_f16(c, 0x00080008u, 0x00080008u, 0x00800080u, 0x00800080u, qf[n][g][2], qf[n][g][3], c[0], c[1], c[2], c[3]);
+        start[n][g][0] = -c[0];
+        start[n][g][1] = -c[1];
       }
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int from = (2 * p + x) * 4;
-#pragma unroll
-        for (int g = 0; g < G; ++g) start[n][g][x] = -8.f * 0x1p-24f * __shfl_sync(0xffffffffu, sum[g], from);
+      for (int x2 = 0; x2 < 2; ++x2) {
         // 2^24 of the codes, 2^(e - 14) of the row
-        const int up = __shfl_sync(0xffffffffu, e, from) + 10;
-        row_scale[n][x] = a.scale_log2 * power_of_two(up / 2) * power_of_two(up - up / 2);
-        const int at_row = 8 * n + 2 * p + x;
-        see_hi[n][x] = at_row < rows ? base + (row0 + at_row) / a.group : -1;
+        const int up = __shfl_sync(0xffffffffu, e, (2 * p + x2) * 4) + 10;
+        row_scale[n][x2] = a.scale_log2 * power_of_two(up / 2) * power_of_two(up - up / 2);
+        const int at_row = 8 * n + 2 * p + x2;
+        see_hi[n][x2] = at_row < rows ? base + token_of(at_row) : -1;
       }
     }
     // Of a column: probabilities are 2^(score - from), from = top + sigma - 7 (whole numbers: no
@@ -625,30 +621,41 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
     const bool whole = b0 == 0 && b1 == it.blocks;
     const int64_t slot = 2 * cta + (b0 == 0 ? 1 : 0);
     if (threadIdx.x == 0 && bad_page) atomicOr(&g_device_error, kDeviceErrorIndex);
+    // A row of a head a warp, kCols columns a lane.
+    constexpr int kCols = D / 32;
     const int heads = min(HEADS, a.kv_heads - it.head);
-    for (int i = threadIdx.x; i < heads * rows * D; i += kDecodeThreads) {
-      const int col = i % D, h_row = i / D, hh = HEADS == 1 ? 0 : h_row / rows, row = h_row - hh * rows;
+    for (int i = warp; i < HEADS * rows; i += kDecodeWarps) {
+      const int hh = i % HEADS, row = i / HEADS;
+      if (hh >= heads) continue;
       float m = -INFINITY;
 #pragma unroll
       for (int v = 0; v < kSplit; ++v) m = fmaxf(m, stat[v * HEADS + hh][row][0]);
       const float top_of = m == -INFINITY ? 0.f : m;
-      float o = 0.f, l = 0.f;
+      float o[kCols] = {}, l = 0.f;
 #pragma unroll
       for (int v = 0; v < kSplit; ++v) {
         const float f = exp2_approx(stat[v * HEADS + hh][row][0] - top_of);
-        o += f * reinterpret_cast<float*>(smem)[((v * HEADS + hh) * kRows + row) * D + col];
+        const float* from_warp = reinterpret_cast<const float*>(smem) + ((v * HEADS + hh) * kRows + row) * D + lane * kCols;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) o[c] += f * from_warp[c];
         l += f * stat[v * HEADS + hh][row][1];
       }
-      if (bad_page) l = o = __int_as_float(0x7fc00000);
+      if (bad_page) {
+        l = __int_as_float(0x7fc00000);
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) o[c] = l;
+      }
       if (whole) {
-        const int of = row0 + row, token = of / a.group;
-        const int h = (it.head + hh) * a.group + (of - token * a.group);
-        static_cast<T*>(a.out)[(q.first + token) * a.out_n + h * a.out_h + col] = from_float<T>(l == 0.f ? 0.f : o / l);
-        if (a.lse && col == 0) a.lse[(int64_t)(q.first + token) * a.heads + h] = (m + log2f(l)) * 0.6931471805599453f;
+        const int token = token_of(row), h = (it.head + hh) * a.group + (row0 + row - token * a.group);
+        T* out = static_cast<T*>(a.out) + (q.first + token) * a.out_n + h * a.out_h + lane * kCols;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) out[c] = from_float<T>(l == 0.f ? 0.f : o[c] / l);
+        if (a.lse && lane == 0) a.lse[(int64_t)(q.first + token) * a.heads + h] = (m + log2f(l)) * 0.6931471805599453f;
       } else {
         const int64_t to = (slot * HEADS + hh) * kRows + row;
-        part_out[to * D + col] = o;
-        if (col == 0) {
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) part_out[to * D + lane * kCols + c] = o[c];
+        if (lane == 0) {
           part_stat[to * 2] = m;
           part_stat[to * 2 + 1] = l;
         }
