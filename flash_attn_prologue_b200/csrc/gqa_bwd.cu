@@ -142,11 +142,10 @@ __global__ void __launch_bounds__(kThreads, 2) gqa_bwd_kernel(const GqaBwdArgs a
     [[maybe_unused]] int rows[4];
     if constexpr (AXES) pos = there && rotation_rows(a.tab, b, n, rows) ? 0 : -1;
     else pos = there ? rotation_row(a.tab, b, n) : -1;
+    if constexpr (AXES)
+      load_turned<T, D, VEC>(sn, cs, a.tab, rows, pos >= 0, j0, a.p.log2_hs, hslot, (tslot << a.p.log2_hs) * L + c_lane);
     if (pos >= 0) {
-      if constexpr (AXES) {
-        load_turned<T, D, VEC>(sn, a.tab.sin, a.tab.sin_n, a.tab.sin_j, a.tab, rows, j0);
-        load_turned<T, D, VEC>(cs, a.tab.cos, a.tab.cos_n, a.tab.cos_j, a.tab, rows, j0);
-      } else {
+      if constexpr (!AXES) {
         load_columns<T, D, VEC>(sn, a.tab.sin + pos * a.tab.sin_n + j0 * a.tab.sin_j, a.tab.sin_j);
         load_columns<T, D, VEC>(cs, a.tab.cos + pos * a.tab.cos_n + j0 * a.tab.cos_j, a.tab.cos_j);
       }

@@ -208,26 +208,60 @@ __device__ __forceinline__ void load_columns(float (&v)[kChunk], const float* ha
   }
 }
 
-// The lane's 8 values of the rows that turn its pairs, each by its axis. Four pairs of
-// one axis are read at once; mixed ones (interleaved axes) one by one, from rows that
-// the warp's other lanes read too. First column of the lane: j0.
-template <typename T, int D, bool VEC>
-__device__ __forceinline__ void load_turned(float (&v)[kChunk], const float* table, int64_t s_row, int64_t s_col,
-                                            const GqaTables& t, const int (&row)[4], int j0) {
+// The lane's 8 sin and cos values, each of the row that its pair's axis turns by. Where no lane has mixed
+// pairs (axes in blocks of whole quads) quads are read at once. Else one by one, and the lanes that hold
+// other heads of the token read other pairs and hand them over: a lane's own 16 reads, with an address
+// each, were a sixth of the forward's instructions (65,536 tokens x 40 heads x 128, three interleaved axes,
+// forward and backward: 623 us then, 564 us so). PER pairs a lane, of HS >= 8 / PER heads.
+template <typename T, int D, int PER>
+__device__ __forceinline__ void share_turned(float (&sn)[kChunk], float (&cs)[kChunk], const GqaTables& t,
+                                             const int (&row)[4], bool there, int j0, int hslot, int first_lane) {
   using C = Columns<T, D>;
+  constexpr int L = D / 16;
+  float s[PER], c[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int e = (hslot * PER + k) & (kChunk - 1), col = j0 + C::of(0, e);
+    const uint32_t axis = (uint32_t)(t.pair_axes[col >> 5] >> (2 * (col & 31))) & 3u;
+    const int64_t at = axis == 0 ? row[0] : axis == 1 ? row[1] : axis == 2 ? row[2] : row[3];
+    s[k] = there ? __ldg(t.sin + at * t.sin_n + col * t.sin_j) : 0.f;
+    c[k] = there ? __ldg(t.cos + at * t.cos_n + col * t.cos_j) : 0.f;
+  }
+#pragma unroll
+  for (int e = 0; e < kChunk; ++e) {
+    sn[e] = __shfl_sync(0xffffffffu, s[e % PER], first_lane + e / PER * L);
+    cs[e] = __shfl_sync(0xffffffffu, c[e % PER], first_lane + e / PER * L);
+  }
+}
+// first_lane: the lane of the token's first head that owns this lane's columns. All lanes call it; without
+// `there` (the token has no rows) a lane's values mean nothing.
+template <typename T, int D, bool VEC>
+__device__ __forceinline__ void load_turned(float (&sn)[kChunk], float (&cs)[kChunk], const GqaTables& t,
+                                            const int (&row)[4], bool there, int j0, int log2_hs, int hslot, int first_lane) {
+  using C = Columns<T, D>;
+  uint32_t byte[2];
+  bool mixed = !VEC;
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
     const int col = j0 + C::of(0, 4 * q);
-    const uint32_t byte = (uint32_t)(t.pair_axes[col >> 5] >> (2 * (col & 31))) & 0xffu;
-    const auto row_of = [&](uint32_t axis) {
-      return table + (int64_t)(axis == 0 ? row[0] : axis == 1 ? row[1] : axis == 2 ? row[2] : row[3]) * s_row;
-    };
-    if (VEC && byte == (byte & 3u) * 0x55u) {
-      const float4 x = __ldg(reinterpret_cast<const float4*>(row_of(byte & 3u) + col));
-      v[4 * q] = x.x; v[4 * q + 1] = x.y; v[4 * q + 2] = x.z; v[4 * q + 3] = x.w;
-    } else {
+    byte[q] = (uint32_t)(t.pair_axes[col >> 5] >> (2 * (col & 31))) & 0xffu;
+    mixed |= byte[q] != (byte[q] & 3u) * 0x55u;
+  }
+  if (__any_sync(0xffffffffu, mixed)) {
+    if (log2_hs >= 3) share_turned<T, D, 1>(sn, cs, t, row, there, j0, hslot, first_lane);
+    else if (log2_hs == 2) share_turned<T, D, 2>(sn, cs, t, row, there, j0, hslot, first_lane);
+    else if (log2_hs == 1) share_turned<T, D, 4>(sn, cs, t, row, there, j0, hslot, first_lane);
+    else share_turned<T, D, 8>(sn, cs, t, row, there, j0, hslot, first_lane);
+  } else if (there) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[4 * q + e] = __ldg(row_of(byte >> (2 * e) & 3u) + (col + e) * s_col);
+    for (int q = 0; q < 2; ++q) {
+      const int col = j0 + C::of(0, 4 * q);
+      const uint32_t axis = byte[q] & 3u;
+      const int64_t at = axis == 0 ? row[0] : axis == 1 ? row[1] : axis == 2 ? row[2] : row[3];
+      const float4 x = __ldg(reinterpret_cast<const float4*>(t.sin + at * t.sin_n + col));
+      const float4 y = __ldg(reinterpret_cast<const float4*>(t.cos + at * t.cos_n + col));
+      sn[4 * q] = x.x; sn[4 * q + 1] = x.y; sn[4 * q + 2] = x.z; sn[4 * q + 3] = x.w;
+      cs[4 * q] = y.x; cs[4 * q + 1] = y.y; cs[4 * q + 2] = y.z; cs[4 * q + 3] = y.w;
     }
   }
 }

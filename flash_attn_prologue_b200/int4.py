@@ -181,6 +181,12 @@ def paged_attention_int4(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_
     return (out, lse) if return_lse else out
 
 
+def _packed(t):
+    """t, or a copy that is contiguous and starts on 16 bytes."""
+    t = t.contiguous()
+    return t if not t.data_ptr() & 15 else t.clone()
+
+
 def _unpack(cache, scale, dtype):
     if cache.ndim < 1 or cache.dtype is not torch.uint8 or scale.dtype is not torch.bfloat16:
         raise ValueError("unpack_int4 takes uint8 codes and bfloat16 scales")
@@ -195,14 +201,17 @@ def _unpack(cache, scale, dtype):
         raise ValueError("all tensors must share a device")
     if cache.device.type != "cuda":
         raise ValueError("the kernels run on CUDA devices only")
-    cache, scale = (t.contiguous() for t in (cache, scale))
-    cache, scale = (t if not t.data_ptr() & 15 else t.clone() for t in (cache, scale))
-    out = torch.empty((*cache.shape[:-1], dim), dtype=dtype, device=cache.device)
+    cache, scale = _packed(cache), _packed(scale)
     device = cache.device
-    with _DeviceGuard(device):
-        _lib.check(_lib.load().flash_prologue_unpack_int4(
-            cache.data_ptr(), scale.data_ptr(), out.data_ptr(), out.numel() // dim, dim, _lib.DTYPE_CODES[dtype],
-            _lib.raw_stream(device.index)), "flash_prologue_unpack_int4")
+    out = cache.new_empty((*cache.shape[:-1], dim), dtype=dtype)
+    args = (cache.data_ptr(), scale.data_ptr(), out.data_ptr(), out.numel() // dim, dim, _lib.DTYPE_CODES[dtype])
+    if device.index == torch._C._cuda_getDevice():
+        status = _lib.load().flash_prologue_unpack_int4(*args, _lib.raw_stream(device.index))
+    else:
+        with _DeviceGuard(device):
+            status = _lib.load().flash_prologue_unpack_int4(*args, _lib.raw_stream(device.index))
+    if status:
+        _lib.check(status, "flash_prologue_unpack_int4")
     return out
 
 

@@ -26,23 +26,26 @@ class PagedStep(NamedTuple):
 
 
 def _plan(page_table, seq_lens, new_lens, free_pages, free_count, page_size, tokens, keep):
-    device, int32 = page_table.device, torch.int32
-    if page_table.ndim != 2 or seq_lens.shape != page_table.shape[:1] or new_lens.shape != seq_lens.shape:
+    device, int32, lens, shape = page_table.device, torch.int32, seq_lens.shape, page_table.shape
+    if len(shape) != 2 or lens != shape[:1] or new_lens.shape != lens:
         raise ValueError("page_table must be [B, max_pages], seq_lens and new_lens [B]")
     if free_pages.ndim != 1 or free_count.shape != (1,):
         raise ValueError("free_pages must be a stack [pages] and free_count [1]")
-    if keep is not None and keep.shape != seq_lens.shape:
+    if keep is not None and keep.shape != lens:
         raise ValueError("keep must be [B]")
-    given = [page_table, seq_lens, new_lens, free_pages, free_count, *([] if keep is None else [keep])]
-    if any(t.dtype is not int32 for t in given):
-        raise ValueError("tables, lengths, free_pages and free_count must be int32")
-    if any(t.device != device for t in given):
-        raise ValueError("all tensors must share a device")
-    batch, width = page_table.shape
+    batch, width = shape
     stride = page_table.stride()
-    if (width > 1 and stride[1] != 1) or not all(t.is_contiguous() for t in given[1:]):
+    right, shared = page_table.dtype is int32, True
+    packed = width <= 1 or stride[1] == 1
+    for t in (seq_lens, new_lens, free_pages, free_count) if keep is None else (seq_lens, new_lens, free_pages, free_count, keep):
+        right, shared, packed = right and t.dtype is int32, shared and t.device == device, packed and t.is_contiguous()
+    if not right:
+        raise ValueError("tables, lengths, free_pages and free_count must be int32")
+    if not shared:
+        raise ValueError("all tensors must share a device")
+    if not packed:
         raise ValueError("page_table rows, lengths and free_pages must be contiguous")
-    if batch > 1 and 0 < stride[0] < width or batch > 1 and stride[0] == 0:
+    if batch > 1 and width > 0 and stride[0] < width:
         raise ValueError("page_table rows must not share memory")
     if page_size < 8 or page_size & (page_size - 1):
         raise ValueError("page_size must be a power of two, at least 8")
@@ -52,8 +55,8 @@ def _plan(page_table, seq_lens, new_lens, free_pages, free_count, page_size, tok
         raise ValueError("tokens must not be negative")
     if device.type != "cuda":
         raise ValueError("the planning kernel runs on CUDA devices only")
-    out = PagedStep(torch.empty_like(seq_lens), seq_lens.new_empty(batch + 1), seq_lens.new_empty(tokens),
-                    seq_lens.new_empty(tokens, dtype=torch.int64), seq_lens.new_empty(tokens), torch.empty_like(free_count))
+    new = seq_lens.new_empty
+    out = PagedStep(new(batch), new(batch + 1), new(tokens), new(tokens, dtype=torch.int64), new(tokens), new(1))
     args = _lib.PLAN_ARGS.pack(
         page_table.data_ptr(), stride[0], width, seq_lens.data_ptr(), new_lens.data_ptr(),
         0 if keep is None else keep.data_ptr(), free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(),
@@ -96,7 +99,7 @@ def plan_paged_step(page_table, seq_lens, new_lens, free_pages, free_count, page
     the stack has no room for set the device error word.
     """
     args = (page_table, seq_lens, new_lens, free_pages, free_count, page_size, tokens, keep)
-    if not eager(*(t for t in args if isinstance(t, torch.Tensor))):
+    if not eager(page_table, seq_lens, new_lens, free_pages, free_count, keep):
         return PagedStep(*torch.ops.flash_prologue.plan_paged_step(*args))
     out = _plan(*args)
     increment_version((page_table, free_pages))
