@@ -52,6 +52,9 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ void sts128(uint32_t addr, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
 __device__ __forceinline__ uint2 lds64(uint32_t addr) {
   uint2 v;
   asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
@@ -173,6 +176,16 @@ __device__ __forceinline__ bool phase_wait(uint64_t* bar, uint32_t parity) {
   return false;
 }
 
+// Shared memory of a CTA: its rings, later its warps' sums; then the warps' Q (kept there, since registers are
+// what limits the warps of an SM).
+template <int D, int NT>
+constexpr size_t room_of() {
+  constexpr size_t ring = (size_t)kDecodeWarps * kRing * Step<D>::kBytes, joined = (size_t)kDecodeWarps * 8 * NT * D * 4;
+  return ring > joined ? ring : joined;
+}
+template <int D, int NT>
+constexpr uint32_t kQueryBytes = NT * (D / 32) * (512 + 64);
+
 struct Int4Args {
   AttentionArgs a;  // k, v: codes, strides in bytes
   const uint16_t* k_scale;
@@ -201,6 +214,8 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr uint32_t kStage = TMA ? kDecodeWarps * S::kBytes : S::kBytes;
   const uint32_t ring = smem_u32(smem) + (TMA ? 0 : warp * kRing * kStage), ring_end = ring + kRing * kStage;
+  // The warp's Q fragments (16 bytes a lane and group), then what their sums start at (16 bytes a pair of columns).
+  const uint32_t q_s = smem_u32(smem) + (uint32_t)room_of<D, NT>() + warp * kQueryBytes<D, NT>, start_s = q_s + NT * G * 512;
 
   if (!a.whole) start_next_kernel();
   if constexpr (TMA) {
@@ -246,8 +261,6 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
     const bool idle = HEADS > 1 && head >= a.kv_heads;
 
     // Q: row 8 n + j of the tile, this lane's channels 8 (p G + g) .. + 7 of each group, times a power of two.
-    uint32_t qf[NT][G][4];
-    float start[NT][G][2];   // -8 sum of q over a group, of this lane's two columns 2 p and 2 p + 1
     float row_scale[NT][2];  // takes their sums to base-2 scores
     int see_hi[NT][2];       // last position that they see
     const auto token_of = [&](int row) { return q.news == 1 ? 0 : (row0 + row) / a.group; };  // (a division)
@@ -274,15 +287,17 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         const T* v = reinterpret_cast<const T*>(&x[g]);
+        uint32_t qf[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c)
-          qf[n][g][c] = half2_of((float)v[2 * c] * (c & 1 ? f16 : f), (float)v[2 * c + 1] * (c & 1 ? f16 : f));
-        // As keys whose codes are all 8.
+          qf[c] = half2_of((float)v[2 * c] * (c & 1 ? f16 : f), (float)v[2 * c + 1] * (c & 1 ? f16 : f));
+        // -8 sum of q over the group, of this lane's two columns 2 p and 2 p + 1: as keys whose codes are all 8.
         float c[4];
-        mma_f16(c, 0x00080008u, 0x00080008u, 0x00800080u, 0x00800080u, qf[n][g][0], qf[n][g][1], 0.f, 0.f, 0.f, 0.f);
-        mma_f16(c, 0x00080008u, 0x00080008u, 0x00800080u, 0x00800080u, qf[n][g][2], qf[n][g][3], c[0], c[1], c[2], c[3]);
-        start[n][g][0] = -c[0];
-        start[n][g][1] = -c[1];
+        mma_f16(c, 0x00080008u, 0x00080008u, 0x00800080u, 0x00800080u, qf[0], qf[1], 0.f, 0.f, 0.f, 0.f);
+        mma_f16(c, 0x00080008u, 0x00080008u, 0x00800080u, 0x00800080u, qf[2], qf[3], c[0], c[1], c[2], c[3]);
+        sts128(q_s + (n * G + g) * 512 + lane * 16, make_uint4(qf[0], qf[1], qf[2], qf[3]));
+        const uint32_t c0 = __float_as_uint(-c[0]), c1 = __float_as_uint(-c[1]);
+        if (j == 0) sts128(start_s + (n * G + g) * 64 + p * 16, make_uint4(c0, c1, c0, c1));
       }
 #pragma unroll
       for (int x2 = 0; x2 < 2; ++x2) {
@@ -338,10 +353,11 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
           const float fa = sa.get(g), fb = sb.get(g);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
+            const uint4 qf = lds128(q_s + (n * G + g) * 512 + lane * 16), c0 = lds128(start_s + (n * G + g) * 64 + p * 16);
             float c[4];
-            mma_f16(c, wa[g] & kLow, wb[g] & kLow, wa[g] & kHigh, wb[g] & kHigh, qf[n][g][0], qf[n][g][1], start[n][g][0],
-                    start[n][g][1], start[n][g][0], start[n][g][1]);
-            mma_f16(c, ua & kLow, ub & kLow, ua & kHigh, ub & kHigh, qf[n][g][2], qf[n][g][3], c[0], c[1], c[2], c[3]);
+            mma_f16(c, wa[g] & kLow, wb[g] & kLow, wa[g] & kHigh, wb[g] & kHigh, qf.x, qf.y, __uint_as_float(c0.x),
+                    __uint_as_float(c0.y), __uint_as_float(c0.z), __uint_as_float(c0.w));
+            mma_f16(c, ua & kLow, ub & kLow, ua & kHigh, ub & kHigh, qf.z, qf.w, c[0], c[1], c[2], c[3]);
 #pragma unroll
             for (int x = 0; x < 4; ++x) s[n][x] = fmaf(c[x], x < 2 ? fa : fb, s[n][x]);
           }
@@ -673,8 +689,7 @@ cudaError_t launch(Int4Args args, const Maps& maps, cudaStream_t stream) {
   AttentionArgs& a = args.a;
   constexpr int kRows = 8 * NT;
   a.whole = a.max_keys <= kWholeKeys;
-  constexpr size_t ring = (size_t)kDecodeWarps * kRing * Step<D>::kBytes, joined = (size_t)kDecodeWarps * kRows * D * 4;
-  constexpr size_t smem = ring > joined ? ring : joined;
+  constexpr size_t smem = room_of<D, NT>() + kDecodeWarps * kQueryBytes<D, NT>;
   const void* fn = reinterpret_cast<const void*>(&paged_int4_decode_kernel<T, D, NT, HEADS, TMA>);
   cudaError_t err = allow_shared_memory(fn, smem);
   if (err != cudaSuccess) return err;
