@@ -54,7 +54,12 @@ namespace {
 constexpr int kTile = 128;             // rows of a tile
 constexpr int kKeys = 64;              // keys of a block
 constexpr int kPrefillThreads = 256;
-constexpr int kInt4Threads = kPrefillThreads + 256;  // eight more warps turn codes into values
+// Over a cache of 4 bits more warps turn codes into values: kCodeWarps make K, as many V.
+template <int D>
+constexpr int kCodeWarps = D / 32;
+template <int D>
+constexpr int kInt4Threads = kPrefillThreads + 64 * kCodeWarps<D>;
+constexpr int kMostThreads = kInt4Threads<128>;
 constexpr int kRowThreads = 128;
 constexpr int kTmemCols = 256;
 
@@ -92,7 +97,7 @@ struct Barriers {
   uint64_t s_full[2], s_read[2], p_full[2], o_done[2], clean_ask, v_clean, drain[2];
   uint64_t q_full, q_empty, work_full[2], work_empty[2], next_here;
   uint32_t tmem;
-  int sums[kInt4Threads / 32];
+  int sums[kMostThreads / 32];
   int found, found_start;  // request of the CTA's first tile (-1: none), tiles before it
   Work work[2];            // the tile that the warps are at and the next
   // Where a wait ran out: the tiles that were put into work, and one that was taken over and not put there.
@@ -329,12 +334,18 @@ template <int N>
 __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-// 512 threads at 64 registers each, split among the four warpgroups.
-constexpr int kRowRegisters = 112, kOtherRegisters = 48;
-static_assert(kRowRegisters + 3 * kOtherRegisters == 4 * 64, "registers of a CTA");
+// The registers of a CTA's threads (384 of 80, D = 128: 512 of 64), split among the three (four) warpgroups.
+template <int D>
+constexpr int kRowRegisters = D == 64 ? 120 : 112;
+template <int D>
+constexpr int kIssueRegisters = D == 64 ? 56 : 48;
+template <int D>
+constexpr int kCodeRegisters = D == 64 ? 64 : 48;
+static_assert(kRowRegisters<64> + kIssueRegisters<64> + kCodeRegisters<64> == 3 * 80, "registers of a CTA");
+static_assert(kRowRegisters<128> + kIssueRegisters<128> + 2 * kCodeRegisters<128> == 4 * 64, "registers of a CTA");
 
 template <typename T, int D, bool kSelfTest = false, bool kInt4 = false>
-__global__ void __launch_bounds__(kInt4 ? kInt4Threads : kPrefillThreads, 2)
+__global__ void __launch_bounds__(kInt4 ? kInt4Threads<D> : kPrefillThreads, 2)
     paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                          const __grid_constant__ CUtensorMap v_map, const __grid_constant__ PrefillArgs p) {
   using L = Layout<D>;
@@ -362,9 +373,9 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads : kPrefillThreads, 2)
   const int requests = requests_of(a.pages);
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::kStages; ++s) {
-      mbar_init(&bar.k_full[s], kInt4 ? 4 : 1);
+      mbar_init(&bar.k_full[s], kInt4 ? kCodeWarps<D> : 1);
       mbar_init(&bar.k_empty[s], 1);
-      mbar_init(&bar.v_full[s], kInt4 ? 4 : 1);
+      mbar_init(&bar.v_full[s], kInt4 ? kCodeWarps<D> : 1);
       mbar_init(&bar.v_empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -373,7 +384,7 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads : kPrefillThreads, 2)
       mbar_init(&bar.p_full[b], kRowThreads / 32);
       mbar_init(&bar.o_done[b], 1);
       mbar_init(&bar.work_full[b], 1);
-      mbar_init(&bar.work_empty[b], kRowThreads / 32 + (kInt4 ? 10 : 3));
+      mbar_init(&bar.work_empty[b], kRowThreads / 32 + (kInt4 ? 2 + 2 * kCodeWarps<D> : 3));
       mbar_init(&bar.drain[b], 1);
     }
     mbar_init(&bar.clean_ask, 1);
@@ -394,7 +405,7 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads : kPrefillThreads, 2)
   int all_tiles = 0;
   {
     const int tile = tile_at(blockIdx.x);
-    constexpr int kThreadsHere = kInt4 ? kInt4Threads : kPrefillThreads;
+    constexpr int kThreadsHere = kInt4 ? kInt4Threads<D> : kPrefillThreads;
     for (int r0 = 0; r0 < requests; r0 += kThreadsHere) {
       const int r = r0 + threadIdx.x;
       Request q{0, 0, 0};
@@ -443,18 +454,18 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads : kPrefillThreads, 2)
   };
 
   if (kInt4 && warp >= 8) {
-    fewer_registers<kOtherRegisters>();
+    fewer_registers<kCodeRegisters<D>>();
     // ---------------- codes to values ----------------
-    // Warps 8-11 make K, warps 12-15 V. A thread has a key of the block and half its words (at D = 128 those
-    // of one 64-column half), loads them a block ahead and writes the values as the tensor maps of a 16-bit
-    // cache would: rows of 128 bytes, 16-byte chunks swizzled by the row. (At D = 128 the two threads of a
-    // row go through their words in different orders, so that eight lanes write to eight banks.)
-    constexpr int G = D / 32, kPieces = D / 64;  // 16-byte pieces of a thread
-    const bool values = warp >= 12;
-    const int key_row = threadIdx.x % 128 / 2, part = threadIdx.x & 1, turn = D == 128 ? part : 0;
+    // Half the warps make K, half V. A thread has 32 bytes of codes (8 words) of a key of the block, a
+    // 64-column half of the row, loads them a block ahead and writes the values as the tensor maps of a
+    // 16-bit cache would: rows of 128 bytes, 16-byte chunks swizzled by the row. (At D = 128 the two threads
+    // of a row go through their words in different orders, so that eight lanes write to eight banks.)
+    constexpr int G = D / 32, kPieces = 2, kParts = D / 64;
+    const bool values = warp >= 8 + kCodeWarps<D>;
+    const int index = threadIdx.x % D, key_row = index / kParts, part = index % kParts, turn = part;
     const int in_page = (1 << a.pages.page_log2) - 1;
-    unsigned char* const to = (values ? v_s : k_s) + (D == 128 ? part * L::kHalf : 0) + key_row * 128;
-    const int swizzle = key_row & 7, chunk0 = D == 128 ? 0 : 4 * part;
+    unsigned char* const to = (values ? v_s : k_s) + part * L::kHalf + key_row * 128;
+    const int swizzle = key_row & 7;
     uint64_t* const full = values ? bar.v_full : bar.k_full;
     uint64_t* const empty = values ? bar.v_empty : bar.k_empty;
     // Strides of pages and slots take 31 bits (the host checks).
@@ -543,7 +554,7 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads : kPrefillThreads, 2)
           for (int e = 0; e < 4; ++e) {
             uint32_t v[4];
             int4_values<T>(word[e], s2[e % G], s24[e % G], v);
-            *reinterpret_cast<uint4*>(dst + ((chunk0 + 4 * (i ^ turn) + e) ^ swizzle) * 16) = make_uint4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<uint4*>(dst + ((4 * (i ^ turn) + e) ^ swizzle) * 16) = make_uint4(v[0], v[1], v[2], v[3]);
           }
         }
         fence_proxy_async_smem();
@@ -555,7 +566,7 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads : kPrefillThreads, 2)
       done_with(t);
     }
   } else if (warp >= 4) {
-    if constexpr (kInt4) fewer_registers<kOtherRegisters>();
+    if constexpr (kInt4) fewer_registers<kIssueRegisters<D>>();
     if (warp == 4) {
       // ---------------- scores ----------------
       // The issuing warps walk the blocks whole, with values the compiler knows to be the same
@@ -895,7 +906,7 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads : kPrefillThreads, 2)
       }
     }
   } else {
-    if constexpr (kInt4) more_registers<kRowRegisters>();
+    if constexpr (kInt4) more_registers<kRowRegisters<D>>();
     // ---------------- softmax and output rows ----------------
     const int row = threadIdx.x;
     const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
@@ -1162,7 +1173,7 @@ cudaError_t launch(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUt
   cudaError_t err = allow_shared_memory(fn, Layout<D>::kSmem);
   if (err != cudaSuccess) return err;
   const int64_t cut = items - p.whole_items;
-  err = launch_kernel(paged_prefill_kernel<T, D, kSelfTest, kInt4>, dim3((unsigned)(p.whole_items + cut * p.splits)), dim3(kInt4 ? kInt4Threads : kPrefillThreads),
+  err = launch_kernel(paged_prefill_kernel<T, D, kSelfTest, kInt4>, dim3((unsigned)(p.whole_items + cut * p.splits)), dim3(kInt4 ? kInt4Threads<D> : kPrefillThreads),
                       Layout<D>::kSmem, stream, q_map, k_map, v_map, p);
   if (err != cudaSuccess || p.splits == 1) return err;
   return launch_following(prefill_join_kernel<T, D>, dim3((unsigned)(cut * (kTile / 16))), dim3(512), stream, p);
