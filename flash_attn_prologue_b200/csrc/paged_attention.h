@@ -71,13 +71,14 @@ __device__ __forceinline__ Request request_at(const PagedTarget& p, int tokens, 
 size_t paged_decode_workspace(int D, int sms);
 size_t paged_prefill_workspace(int D, int sms);
 struct PrefillPlan {
-  int tile_tokens;   // whole tokens of a 128-row tile
+  int tile_rows;     // 128 or (over a cache of 4 bits, D = 128) 256
+  int tile_tokens;   // whole tokens of a tile
   int splits;        // shares of the keys of the items behind whole_items
   int64_t whole_items;
   int64_t tiles;     // tiles there can be, all requests
 };
 PrefillPlan plan_paged_prefill(int64_t tokens, int64_t batch, bool ragged, int64_t kv_heads, int64_t group, int D,
-                               int64_t max_keys, int64_t window, int sms);
+                               int64_t max_keys, int64_t window, int sms, bool int4);
 // False where the cache's layout has no tensor map (the other kernel reads it). wait_cycles: 0, or
 // (self-test, BF16) the limit of the kernel's waits, but for those for copies and products under way.
 // scales: null, or the cache is one of 4 bits (a.k, a.v: codes, strides in bytes).

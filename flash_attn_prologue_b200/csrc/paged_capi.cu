@@ -104,7 +104,7 @@ int attention(const flash_prologue_attention_args* a, const flash_prologue_scale
   g.window = a->window < g.max_keys ? (int)a->window : 0;  // as long as any request: all keys
   if (use_prefill(a, g.scale_log2)) {
     const PrefillPlan plan = plan_paged_prefill(a->tokens, c.batch, c.cu_seqlens != nullptr, a->Hk, g.group, (int)a->D,
-                                                g.max_keys, g.window, sms);
+                                                g.max_keys, g.window, sms, scales != nullptr);
     cudaError_t err = cudaSuccess;
     if (launch_paged_prefill(g, plan, scales, (int)a->dtype, (int)a->D, c.page_size,
                              wait_cycles, static_cast<cudaStream_t>(stream), &err))

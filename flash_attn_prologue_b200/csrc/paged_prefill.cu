@@ -57,17 +57,22 @@ constexpr int kPrefillThreads = 256;
 // Over a cache of 4 bits more warps turn codes into values: kCodeWarps make K, as many V.
 template <int D>
 constexpr int kCodeWarps = D / 32;
-template <int D>
-constexpr int kInt4Threads = kPrefillThreads + 64 * kCodeWarps<D>;
-constexpr int kMostThreads = kInt4Threads<128>;
-constexpr int kRowThreads = 128;
-constexpr int kTmemCols = 256;
+constexpr int kIssueThreads = 128;
+constexpr int kTmemCols = 256;         // of 128 rows
+// At D = 128 two tiles of 128 rows share the values that are made of the codes, in one CTA an SM instead of
+// two: 4,096 tokens over 16,384 keys, 32/8 heads, 897 us instead of 1,097. At D = 64 a tile more of rows costs
+// what it saves: windowed chunks 75 us instead of 71.
+template <int D, bool kInt4>
+constexpr int kPair = kInt4 && D == 128 ? 2 : 1;
+template <int D, bool kInt4>
+constexpr int kThreadsOf = kInt4 ? kPair<D, kInt4> * kTile + kIssueThreads + 64 * kCodeWarps<D> : kPrefillThreads;
+constexpr int kMostThreads = kThreadsOf<128, true>;
 
-template <int D>
+template <int D, int PAIR>
 struct Layout {
   static constexpr int kHalves = D / 64;           // 64-column (128-byte) halves of a row
-  static constexpr int kStages = D == 64 ? 4 : 2;  // K and V blocks in flight
-  static constexpr int kQ = kTile * D * 2, kQHalf = kTile * 128;      // bytes of the Q tile, of its halves
+  static constexpr int kStages = D == 64 || PAIR == 2 ? 4 : 2;  // K and V blocks in flight
+  static constexpr int kQ = PAIR * kTile * D * 2, kQHalf = PAIR * kTile * 128;  // bytes of the Q tile, of its halves
   static constexpr int kBlock = kKeys * D * 2, kHalf = kKeys * 128;   // of a K or V block
   // Tensor-memory columns: blocks of scores (two where there is room), two of probabilities, the output.
   static constexpr int kScores = D == 64 ? 2 : 1;
@@ -94,7 +99,8 @@ struct Work {
 constexpr int kMaxStages = 4;
 struct Barriers {
   uint64_t k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages];
-  uint64_t s_full[2], s_read[2], p_full[2], o_done[2], clean_ask, v_clean, drain[2];
+  uint64_t s_full[2][2], s_read[2][2], p_full[2][2], o_done[2][2];  // of each 128 rows
+  uint64_t clean_ask, v_clean, drain[2];
   uint64_t q_full, q_empty, work_full[2], work_empty[2], next_here;
   uint32_t tmem;
   int sums[kMostThreads / 32];
@@ -287,12 +293,12 @@ __device__ __forceinline__ uint32_t finite_only(uint32_t pair) {
 }
 
 // NaN for row `row` of a tile (or of this share of it) that was not computed.
-template <typename T, int D>
+template <typename T, int D, int PAIR>
 __device__ __noinline__ void void_row(const PrefillArgs& p, const Work& w, int row) {
   if (row >= w.rows) return;
   const float nan = __int_as_float(0x7fc00000);
   if (w.parts > 1) {
-    float* stat = p.part_stat + ((int64_t)w.share * kTile + row) * 2;
+    float* stat = p.part_stat + ((int64_t)w.share * (PAIR * kTile) + row) * 2;
     stat[0] = -INFINITY;
     stat[1] = nan;
     return;
@@ -334,21 +340,22 @@ template <int N>
 __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-// The registers of a CTA's threads (384 of 80, D = 128: 512 of 64), split among the three (four) warpgroups.
+// Over a cache of 4 bits the CTA has 384 threads at 80 registers each (D = 128: 640 at 96), split among its
+// three (five) warpgroups.
+constexpr int kRowRegisters = 120;
 template <int D>
-constexpr int kRowRegisters = D == 64 ? 120 : 112;
+constexpr int kIssueRegisters = D == 64 ? 56 : 80;
 template <int D>
-constexpr int kIssueRegisters = D == 64 ? 56 : 48;
-template <int D>
-constexpr int kCodeRegisters = D == 64 ? 64 : 48;
-static_assert(kRowRegisters<64> + kIssueRegisters<64> + kCodeRegisters<64> == 3 * 80, "registers of a CTA");
-static_assert(kRowRegisters<128> + kIssueRegisters<128> + 2 * kCodeRegisters<128> == 4 * 64, "registers of a CTA");
+constexpr int kCodeRegisters = D == 64 ? 64 : 80;
+static_assert(kRowRegisters + kIssueRegisters<64> + kCodeRegisters<64> == 3 * 80, "registers of a CTA");
+static_assert(2 * kRowRegisters + kIssueRegisters<128> + 2 * kCodeRegisters<128> == 5 * 96, "registers of a CTA");
 
 template <typename T, int D, bool kSelfTest = false, bool kInt4 = false>
-__global__ void __launch_bounds__(kInt4 ? kInt4Threads<D> : kPrefillThreads, 2)
+__global__ void __launch_bounds__(kThreadsOf<D, kInt4>, 2 / kPair<D, kInt4>)
     paged_prefill_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                          const __grid_constant__ CUtensorMap v_map, const __grid_constant__ PrefillArgs p) {
-  using L = Layout<D>;
+  constexpr int PAIR = kPair<D, kInt4>, kRowWarps = PAIR * kTile / 32;
+  using L = Layout<D, PAIR>;
   extern __shared__ unsigned char smem_raw[];
   __shared__ Barriers bar;
   __shared__ __align__(16) unsigned char answer[16];
@@ -379,12 +386,14 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads<D> : kPrefillThreads, 2)
       mbar_init(&bar.v_empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(&bar.s_full[b], 1);
-      mbar_init(&bar.s_read[b], kRowThreads / 32);
-      mbar_init(&bar.p_full[b], kRowThreads / 32);
-      mbar_init(&bar.o_done[b], 1);
+      for (int half = 0; half < PAIR; ++half) {
+        mbar_init(&bar.s_full[half][b], 1);
+        mbar_init(&bar.s_read[half][b], kTile / 32);
+        mbar_init(&bar.p_full[half][b], kTile / 32);
+        mbar_init(&bar.o_done[half][b], 1);
+      }
       mbar_init(&bar.work_full[b], 1);
-      mbar_init(&bar.work_empty[b], kRowThreads / 32 + (kInt4 ? 2 + 2 * kCodeWarps<D> : 3));
+      mbar_init(&bar.work_empty[b], kRowWarps + (kInt4 ? 2 + 2 * kCodeWarps<D> : 3));
       mbar_init(&bar.drain[b], 1);
     }
     mbar_init(&bar.clean_ask, 1);
@@ -405,7 +414,7 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads<D> : kPrefillThreads, 2)
   int all_tiles = 0;
   {
     const int tile = tile_at(blockIdx.x);
-    constexpr int kThreadsHere = kInt4 ? kInt4Threads<D> : kPrefillThreads;
+    constexpr int kThreadsHere = kThreadsOf<D, kInt4>;
     for (int r0 = 0; r0 < requests; r0 += kThreadsHere) {
       const int r = r0 + threadIdx.x;
       Request q{0, 0, 0};
@@ -433,8 +442,8 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads<D> : kPrefillThreads, 2)
       __syncthreads();
     }
   }
-  if (warp == 4) {
-    tmem_alloc(&bar.tmem, kTmemCols);
+  if (warp == kRowWarps) {
+    tmem_alloc(&bar.tmem, PAIR * kTmemCols);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -453,7 +462,10 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads<D> : kPrefillThreads, 2)
     if (lane == 0) mbar_arrive(&bar.work_empty[t & 1]);
   };
 
-  if (kInt4 && warp >= 8) {
+  constexpr int kCodeWarp0 = kRowWarps + kIssueThreads / 32;
+  // 128 rows each that a tile has.
+  const auto halves_of = [](const Work& w) { return PAIR == 1 ? 1 : (w.rows + kTile - 1) / kTile; };
+  if (kInt4 && warp >= kCodeWarp0) {
     fewer_registers<kCodeRegisters<D>>();
     // ---------------- codes to values ----------------
     // Half the warps make K, half V. A thread has 32 bytes of codes (8 words) of a key of the block, a
@@ -461,8 +473,8 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads<D> : kPrefillThreads, 2)
     // 16-bit cache would: rows of 128 bytes, 16-byte chunks swizzled by the row. (At D = 128 the two threads
     // of a row go through their words in different orders, so that eight lanes write to eight banks.)
     constexpr int G = D / 32, kPieces = 2, kParts = D / 64;
-    const bool values = warp >= 8 + kCodeWarps<D>;
-    const int index = threadIdx.x % D, key_row = index / kParts, part = index % kParts, turn = part;
+    const bool values = warp >= kCodeWarp0 + kCodeWarps<D>;
+    const int index = (threadIdx.x - kCodeWarp0 * 32) % D, key_row = index / kParts, part = index % kParts, turn = part;
     const int in_page = (1 << a.pages.page_log2) - 1;
     unsigned char* const to = (values ? v_s : k_s) + part * L::kHalf + key_row * 128;
     const int swizzle = key_row & 7;
@@ -565,9 +577,9 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads<D> : kPrefillThreads, 2)
       }
       done_with(t);
     }
-  } else if (warp >= 4) {
+  } else if (warp >= kRowWarps) {
     if constexpr (kInt4) fewer_registers<kIssueRegisters<D>>();
-    if (warp == 4) {
+    if (warp == kRowWarps) {
       // ---------------- scores ----------------
       // The issuing warps walk the blocks whole, with values the compiler knows to be the same
       // in all lanes, and one lane issues. Each has one product: a warp that issued both, with
@@ -576,75 +588,93 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads<D> : kPrefillThreads, 2)
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
       const uint64_t q_desc = smem_desc_k_sw128(smem_u32(q_s));
       bool ok = true;
-      uint32_t queries = 0;
+      uint32_t queries = 0, made[PAIR] = {};  // blocks of scores of each 128 rows
       for (uint32_t t = 0; ok; ++t) {
         if (!(ok = next_work(t))) break;
         const Work& w = bar.work[t & 1];
         const int n = __shfl_sync(0xffffffffu, w.blocks, 0);
         if (w.rows < 0) break;
         if (n) ok = __all_sync(0xffffffffu, wait_for(&bar.q_full, queries++ & 1));
+        const int halves = __shfl_sync(0xffffffffu, halves_of(w), 0);
         for (int j = 0; j < n && ok; ++j, ++g) {
-          const uint32_t s = g % L::kStages, b = g % L::kScores;
-          // The last scores of this buffer are in the rows' registers, K is here.
-          if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.s_read[b], ((g / L::kScores) & 1) ^ 1) &&
-                                                 wait_for(&bar.k_full[s], (g / L::kStages) & 1))))
-            break;
-          tc_fence_after();
-          const uint64_t k_desc = smem_desc_k_sw128(smem_u32(k_s) + s * L::kBlock);
-          if (elect_one()) {
+          const uint32_t s = g % L::kStages;
 #pragma unroll
-            for (int h = 0; h < L::kHalves; ++h)
+          for (int half = 0; half < PAIR; ++half) {
+            if (half >= halves) break;
+            const uint32_t b = made[half] % L::kScores;
+            // The last scores of this buffer are in the rows' registers, K is here.
+            if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.s_read[half][b], ((made[half] / L::kScores) & 1) ^ 1) &&
+                                                   (half > 0 || wait_for(&bar.k_full[s], (g / L::kStages) & 1)))))
+              break;
+            tc_fence_after();
+            ++made[half];
+            const uint64_t k_desc = smem_desc_k_sw128(smem_u32(k_s) + s * L::kBlock);
+            if (elect_one()) {
 #pragma unroll
-              for (int c = 0; c < 4; ++c)  // 16 columns (32 bytes) a step
-                umma_bf16(tm + L::kSCol + b * kKeys, q_desc + h * (L::kQHalf / 16) + 2 * c,
-                          k_desc + h * (L::kHalf / 16) + 2 * c, idesc, (h | c) != 0);
-            umma_commit(&bar.k_empty[s]);
-            umma_commit(&bar.s_full[b]);
-            if (j == n - 1) umma_commit(&bar.q_empty);
+              for (int h = 0; h < L::kHalves; ++h)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)  // 16 columns (32 bytes) a step
+                  umma_bf16(tm + half * kTmemCols + L::kSCol + b * kKeys,
+                            q_desc + half * (kTile * 128 / 16) + h * (L::kQHalf / 16) + 2 * c,
+                            k_desc + h * (L::kHalf / 16) + 2 * c, idesc, (h | c) != 0);
+              if (half == halves - 1) umma_commit(&bar.k_empty[s]);
+              umma_commit(&bar.s_full[half][b]);
+              if (half == halves - 1 && j == n - 1) umma_commit(&bar.q_empty);
+            }
+            __syncwarp();
           }
-          __syncwarp();
+          if (!ok) break;
         }
         done_with(t);
       }
       // Neither tensor memory nor the tiles are released under products still running.
       if (elect_one()) umma_commit(&bar.drain[0]);
       drain(&bar.drain[0], 0);
-    } else if (warp == 6) {
+    } else if (warp == kRowWarps + 2) {
       // ---------------- output ----------------
       constexpr uint32_t idesc = idesc_of<T>(D, true);
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
       bool ok = true;
-      uint32_t cleaned = 0;
+      uint32_t cleaned = 0, made[PAIR] = {};
       for (uint32_t t = 0; ok; ++t) {
         if (!(ok = next_work(t))) break;
         const Work& w = bar.work[t & 1];
         const int n = __shfl_sync(0xffffffffu, w.blocks, 0), full0 = __shfl_sync(0xffffffffu, w.full0, 0),
-                  full1 = __shfl_sync(0xffffffffu, w.full1, 0);
+                  full1 = __shfl_sync(0xffffffffu, w.full1, 0), halves = __shfl_sync(0xffffffffu, halves_of(w), 0);
         if (w.rows < 0) break;
         for (int j = 0; j < n; ++j, ++g) {
           const uint32_t s = g % L::kStages;
           ok = wait_for(&bar.v_full[s], (g / L::kStages) & 1);
           const bool partial = !kInt4 && (j < full0 || j >= full1);
           if (partial && lane == 0) mbar_arrive(&bar.clean_ask);  // cleaned beside the block's softmax
-          ok = ok && (!partial || wait_for(&bar.v_clean, cleaned & 1)) && wait_for(&bar.p_full[g & 1], (g >> 1) & 1);
+          ok = ok && (!partial || wait_for(&bar.v_clean, cleaned & 1));
           cleaned += partial;
-          if (!(ok = __all_sync(0xffffffffu, ok))) break;
-          tc_fence_after();
-          const uint64_t v_desc = smem_desc_mn_sw128(smem_u32(v_s) + s * L::kBlock, L::kHalf);
-          if (elect_one()) {
 #pragma unroll
-            for (int c = 0; c < kKeys / 16; ++c)  // 16 keys a step: 8 columns of P, two 8-row groups of V (2,048 bytes)
-              umma_ts(tm + L::kOCol, tm + L::kPCol + (g & 1) * (kKeys / 2) + 8 * c, v_desc + 128 * c, idesc, (j | c) != 0);
-            umma_commit(&bar.v_empty[s]);
-            umma_commit(&bar.o_done[g & 1]);
+          for (int half = 0; half < PAIR; ++half) {
+            if (half >= halves) break;
+            const uint32_t b = made[half] & 1;
+            ok = ok && wait_for(&bar.p_full[half][b], (made[half] >> 1) & 1);
+            if (!(ok = __all_sync(0xffffffffu, ok))) break;
+            tc_fence_after();
+            ++made[half];
+            const uint64_t v_desc = smem_desc_mn_sw128(smem_u32(v_s) + s * L::kBlock, L::kHalf);
+            const uint32_t cols = tm + half * kTmemCols;
+            if (elect_one()) {
+#pragma unroll
+              for (int c = 0; c < kKeys / 16; ++c)  // 16 keys a step: 8 columns of P, two 8-row groups of V (2,048 bytes)
+                umma_ts(cols + L::kOCol, cols + L::kPCol + b * (kKeys / 2) + 8 * c, v_desc + 128 * c, idesc, (j | c) != 0);
+              if (half == halves - 1) umma_commit(&bar.v_empty[s]);
+              umma_commit(&bar.o_done[half][b]);
+            }
+            __syncwarp();
           }
-          __syncwarp();
+          if (!ok) break;
         }
         done_with(t);
       }
       if (elect_one()) umma_commit(&bar.drain[1]);
       drain(&bar.drain[1], 0);
-    } else if (warp == 5) {
+    } else if (warp == kRowWarps + 1) {
       // ---------------- tiles and loads ----------------
       const int in_page = (1 << a.pages.page_log2) - 1, boxes = kKeys / p.box_rows;
       const uint32_t box_bytes = (uint32_t)p.box_rows * 128;
@@ -858,9 +888,9 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads<D> : kPrefillThreads, 2)
           if (v_loads >= back) drain(&bar.v_full[(v_loads - back) % L::kStages], ((v_loads - back) / L::kStages) & 1);
         }
       }
-    } else if (kInt4 && warp == 7) {
+    } else if (kInt4 && warp == kRowWarps + 3) {
       // (no cleaning: scales are looked at where they are turned into values)
-    } else if (warp == 7) {
+    } else if (warp == kRowWarps + 3) {
       // ---------------- cleaning ----------------
       uint32_t asked = 0;
       bool ok = true;
@@ -906,10 +936,11 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads<D> : kPrefillThreads, 2)
       }
     }
   } else {
-    if constexpr (kInt4) more_registers<kRowRegisters<D>>();
+    if constexpr (kInt4) more_registers<kRowRegisters>();
     // ---------------- softmax and output rows ----------------
     const int row = threadIdx.x;
-    const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);
+    const int half = PAIR == 1 ? 0 : row / kTile;
+    const uint32_t mine = tmem + ((uint32_t)(warp % 4 * 32) << 16) + half * kTmemCols;
     const float scale = a.scale_log2;
     bool ok = true;
     for (; ok; ++rows_done) {
@@ -917,6 +948,10 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads<D> : kPrefillThreads, 2)
       if (!(ok = next_work(t))) break;
       const Work& w = bar.work[t & 1];
       if (w.rows < 0) break;
+      if (PAIR == 2 && w.rows <= half * kTile) {  // none of these rows
+        done_with(t);
+        continue;
+      }
       // Row state; the row's keys are [see_lo, see_hi].
       const int blocks = w.blocks, first = w.first, full0 = w.full0, full1 = w.full1;
       int see_hi = -1, see_lo = 0;
@@ -927,7 +962,7 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads<D> : kPrefillThreads, 2)
       }
       for (int j = 0; j < blocks; ++j, ++g) {
         const uint32_t b = g % L::kScores;
-        if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.s_full[b], (g / L::kScores) & 1)))) break;
+        if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.s_full[half][b], (g / L::kScores) & 1)))) break;
         tc_fence_after();
         uint32_t s[2][32];
         tmem_ld32(mine + L::kSCol + b * kKeys, s[0]);
@@ -937,7 +972,7 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads<D> : kPrefillThreads, 2)
         pin(s[1]);
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.s_read[b]);
+        if (lane == 0) mbar_arrive(&bar.s_read[half][b]);
         if (j < full0 || j >= full1) {
           const int hi = see_hi - (first + j) * kKeys, lo = see_lo - (first + j) * kKeys;
 #pragma unroll
@@ -961,7 +996,7 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads<D> : kPrefillThreads, 2)
         const bool move = !fresh && (now - top) * scale > 8.f;
         if (__any_sync(0xffffffffu, move)) {
           // O has to be at rest: the last product with V done; the next one waits for this block's P.
-          if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1)))) break;
+          if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.o_done[half][(g - 1) & 1], ((g - 1) >> 1) & 1)))) break;
           tc_fence_after();
           const float f = move ? exp2_approx((top - now) * scale) : 1.f;
           sum *= f;
@@ -991,7 +1026,7 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads<D> : kPrefillThreads, 2)
           out[i] = pack2<T>(x.x, x.y);
         }
         // The buffer's last P has to be used up.
-        if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.o_done[g & 1], ((g >> 1) & 1) ^ 1)))) break;
+        if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.o_done[half][g & 1], ((g >> 1) & 1) ^ 1)))) break;
         tc_fence_after();
         tmem_st32(mine + L::kPCol + (g & 1) * (kKeys / 2), out);
         const float2 both = __fadd2_rn(__fadd2_rn(add[0], add[1]), __fadd2_rn(add[2], add[3]));
@@ -999,9 +1034,9 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads<D> : kPrefillThreads, 2)
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.p_full[g & 1]);
+        if (lane == 0) mbar_arrive(&bar.p_full[half][g & 1]);
       }
-      if (blocks && ok) ok = wait_for(&bar.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
+      if (blocks && ok) ok = wait_for(&bar.o_done[half][(g - 1) & 1], ((g - 1) >> 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) sum = __int_as_float(0x7fc00000);  // a wait ran out: no output that could pass for one
 
@@ -1070,7 +1105,7 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads<D> : kPrefillThreads, 2)
             out[i] = make_uint4(x[0], x[1], x[2], x[3]);
           }
         } else {
-          float4* out = reinterpret_cast<float4*>(p.part_out + (share * kTile + row) * D + 32 * c);
+          float4* out = reinterpret_cast<float4*>(p.part_out + (share * (PAIR * kTile) + row) * D + 32 * c);
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             out[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
@@ -1079,8 +1114,8 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads<D> : kPrefillThreads, 2)
       }
       if (valid) {
         if (!whole) {
-          p.part_stat[(share * kTile + row) * 2] = top2;
-          p.part_stat[(share * kTile + row) * 2 + 1] = sum;
+          p.part_stat[(share * (PAIR * kTile) + row) * 2] = top2;
+          p.part_stat[(share * (PAIR * kTile) + row) * 2 + 1] = sum;
         } else if (a.lse) {
           a.lse[(int64_t)token * a.heads + h] = (top2 + log2f(sum) - kProbabilityShift<T>) * 0.6931471805599453f;
         }
@@ -1092,38 +1127,38 @@ __global__ void __launch_bounds__(kInt4 ? kInt4Threads<D> : kPrefillThreads, 2)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 4) {
+  if (warp == kRowWarps) {
     tc_fence_after();
-    tmem_dealloc(tmem, kTmemCols);
+    tmem_dealloc(tmem, PAIR * kTmemCols);
   }
   // Tiles that were left where a wait ran out (at most the two that are in work, and one more).
-  if (warp < 4) {
-    for (; rows_done < bar.posted; ++rows_done) void_row<T, D>(p, bar.work[rows_done & 1], threadIdx.x);
-    if (bar.has_left) void_row<T, D>(p, bar.left, threadIdx.x);
+  if (warp < kRowWarps) {
+    for (; rows_done < bar.posted; ++rows_done) void_row<T, D, PAIR>(p, bar.work[rows_done & 1], threadIdx.x);
+    if (bar.has_left) void_row<T, D, PAIR>(p, bar.left, threadIdx.x);
   }
 }
 
 // Adds up the shares of a tile, a row a warp: 16 rows a CTA.
-template <typename T, int D>
+template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(512) prefill_join_kernel(const PrefillArgs p) {
   const AttentionArgs& a = p.a;
-  const int64_t item = blockIdx.x / (kTile / 16);  // of those that were cut
+  const int64_t item = blockIdx.x / (ROWS / 16);  // of those that were cut
   wait_for_previous_kernel();
   const Tile t = p.joins[item];
-  const int row = (int)(blockIdx.x % (kTile / 16)) * 16 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int row = (int)(blockIdx.x % (ROWS / 16)) * 16 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (t.parts <= 1 || row >= t.rows) return;
   // What no CTA wrote (a wait ran out) may be anything.
-  if (t.parts > p.splits || t.rows > kTile || t.kv_head < 0 || t.kv_head >= a.kv_heads || t.token0 < 0 ||
+  if (t.parts > p.splits || t.rows > ROWS || t.kv_head < 0 || t.kv_head >= a.kv_heads || t.token0 < 0 ||
       t.token0 >= a.tokens - (t.rows - 1) / a.group)
     return;
   const int64_t slot0 = item * p.splits;
   float m = -INFINITY;
-  for (int s = 0; s < t.parts; ++s) m = fmaxf(m, p.part_stat[((slot0 + s) * kTile + row) * 2]);
+  for (int s = 0; s < t.parts; ++s) m = fmaxf(m, p.part_stat[((slot0 + s) * ROWS + row) * 2]);
   const float from = m == -INFINITY ? 0.f : m;
   float o[D / 32] = {}, l = 0.f;
 #pragma unroll 4
   for (int s = 0; s < t.parts; ++s) {
-    const int64_t at = (slot0 + s) * kTile + row;
+    const int64_t at = (slot0 + s) * ROWS + row;
     const float f = exp2_approx(p.part_stat[at * 2] - from);
     l += f * p.part_stat[at * 2 + 1];
 #pragma unroll
@@ -1169,21 +1204,24 @@ bool encode_rows(CUtensorMap* map, const void* base, int dtype, int D, int64_t h
 template <typename T, int D, bool kSelfTest = false, bool kInt4 = false>
 cudaError_t launch(const CUtensorMap& q_map, const CUtensorMap& k_map, const CUtensorMap& v_map, const PrefillArgs& p, int64_t items,
                    cudaStream_t stream) {
+  constexpr int kRows = kPair<D, kInt4> * kTile;
+  constexpr size_t smem = Layout<D, kPair<D, kInt4>>::kSmem;
   const void* fn = reinterpret_cast<const void*>(&paged_prefill_kernel<T, D, kSelfTest, kInt4>);
-  cudaError_t err = allow_shared_memory(fn, Layout<D>::kSmem);
+  cudaError_t err = allow_shared_memory(fn, smem);
   if (err != cudaSuccess) return err;
   const int64_t cut = items - p.whole_items;
-  err = launch_kernel(paged_prefill_kernel<T, D, kSelfTest, kInt4>, dim3((unsigned)(p.whole_items + cut * p.splits)), dim3(kInt4 ? kInt4Threads<D> : kPrefillThreads),
-                      Layout<D>::kSmem, stream, q_map, k_map, v_map, p);
+  err = launch_kernel(paged_prefill_kernel<T, D, kSelfTest, kInt4>, dim3((unsigned)(p.whole_items + cut * p.splits)),
+                      dim3(kThreadsOf<D, kInt4>), smem, stream, q_map, k_map, v_map, p);
   if (err != cudaSuccess || p.splits == 1) return err;
-  return launch_following(prefill_join_kernel<T, D>, dim3((unsigned)(cut * (kTile / 16))), dim3(512), stream, p);
+  return launch_following(prefill_join_kernel<T, D, kRows>, dim3((unsigned)(cut * (kRows / 16))), dim3(512), stream, p);
 }
 
 }  // namespace
 
 constexpr int kMostShares = 3;  // for each CTA that the device holds
 
-// Tiles, and the shares that blocks are cut into. The GPU holds 2 CTAs an SM;
+// Tiles, and the shares that blocks are cut into. The GPU holds 2 CTAs an SM (one of twice
+// the rows);
 // the items that would leave its last round partly empty (all of them, where
 // there are few) are cut where the rounds of their shares are shorter together.
 // Lengths are only known on the device: the bound on the shares is the page
@@ -1191,9 +1229,11 @@ constexpr int kMostShares = 3;  // for each CTA that the device holds
 // 16,384 keys (1,024 items, 3.46 rounds) 1,075 and 1,046 us; 16 requests of 4,096
 // keys, 6 tokens each (128 items) 78 and 57 us, 64 tokens each (256) 96 and 84 us.
 PrefillPlan plan_paged_prefill(int64_t tokens, int64_t batch, bool ragged, int64_t kv_heads, int64_t group, int D,
-                               int64_t max_keys, int64_t window, int sms) {
+                               int64_t max_keys, int64_t window, int sms, bool int4) {
   PrefillPlan p{};
-  p.tile_tokens = (int)(kTile / group);
+  const int pair = !int4 ? 1 : D == 64 ? kPair<64, true> : kPair<128, true>;
+  p.tile_rows = pair * kTile;
+  p.tile_tokens = (int)(p.tile_rows / group);
   p.tiles = tokens;
   if (ragged) {
     // Every request (and the padding on either side) may leave its last tile partly empty.
@@ -1203,7 +1243,7 @@ PrefillPlan plan_paged_prefill(int64_t tokens, int64_t batch, bool ragged, int64
   // Tiles that there are likely to be (requests of the same size): those beyond them come first and end at once.
   const int64_t asked = tokens < batch ? tokens : batch, each = (tokens + asked - 1) / asked;
   const int64_t likely = asked * ((each + p.tile_tokens - 1) / p.tile_tokens);
-  const int64_t items = p.tiles * kv_heads, slots = 2 * (int64_t)sms;
+  const int64_t items = p.tiles * kv_heads, slots = 2 / pair * (int64_t)sms;
   const int64_t real = likely < p.tiles ? likely * kv_heads : items, cut = real % slots;
   // Where all may run at once, none is left whole: it would take as long as all its keys.
   const int64_t room = real < slots ? items : cut;
@@ -1241,7 +1281,7 @@ bool launch_paged_prefill(const AttentionArgs& a, const PrefillPlan& plan, const
   p.tiles = (int)plan.tiles;
   p.box_rows = page_size < kKeys ? (int)page_size : kKeys;
   const int64_t items = plan.tiles * a.kv_heads;
-  if (items * plan.splits * (kTile / 16) >= (int64_t(1) << 31)) return false;
+  if (items * plan.splits * (plan.tile_rows / 16) >= (int64_t(1) << 31)) return false;
   CUtensorMap q_map, k_map{}, v_map{};
   if (!encode_rows(&q_map, a.q, dtype, D, a.heads, a.tokens, a.q_h, a.q_n, a.group, plan.tile_tokens)) return false;
   if (scales) {
@@ -1262,8 +1302,8 @@ bool launch_paged_prefill(const AttentionArgs& a, const PrefillPlan& plan, const
   if (p.splits > 1) {
     p.part_out = static_cast<float*>(a.workspace);
     const int64_t shares = (items - p.whole_items) * p.splits;
-    p.part_stat = p.part_out + shares * kTile * D;
-    p.joins = reinterpret_cast<Tile*>(p.part_stat + shares * kTile * 2);
+    p.part_stat = p.part_out + shares * plan.tile_rows * D;
+    p.joins = reinterpret_cast<Tile*>(p.part_stat + shares * plan.tile_rows * 2);
   }
   if (scales && wait_cycles)
     *err = D == 64 ? launch<__nv_bfloat16, 64, true, true>(q_map, k_map, v_map, p, items, stream)
