@@ -133,8 +133,8 @@ struct Step {  // bytes of a head's step: K, V, scales of K, scales of V
   static constexpr int kCodes = kWarpKeys * D / 2, kScale = kWarpKeys * D / 16, kBytes = 2 * (kCodes + kScale);
 };
 
-// A cache as the copies of a CTA's four heads see it (HEADS 4, pages of 16 slots at least, scales next to each
-// other along the heads or along the slots).
+// A cache as the copies of a CTA's heads see it (pages that hold a step's keys, scales next to each other along
+// the heads or along the slots).
 struct Maps {
   CUtensorMap k, v, k_scale, v_scale;
   int scales_by_slot;  // a step's scales lie [head][slot] in memory, else [slot][head]
@@ -193,14 +193,13 @@ struct Int4Args {
   int64_t ks_page, ks_slot, ks_head, vs_page, vs_slot, vs_head;  // elements
 };
 
-// NT tiles of 8 rows; HEADS key heads a CTA, so 4 / HEADS warps share a head's keys. TMA: the four heads'
-// steps come by tensor copies into a ring of the CTA, issued by its warps in turn; else every warp loads its
-// own with cp.async.
+// NT tiles of 8 rows; HEADS key heads a CTA, so 4 / HEADS warps share a head's keys. TMA: a step of all
+// four warps comes by tensor copies into a ring of the CTA, issued by its warps in turn; else every warp loads
+// its own with cp.async.
 template <typename T, int D, int NT, int HEADS, bool TMA>
 __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
     paged_int4_decode_kernel(const Int4Args args, const __grid_constant__ Maps maps) {
   const AttentionArgs& a = args.a;
-  static_assert(!TMA || HEADS == kDecodeWarps, "a warp a head");
   constexpr int kRows = 8 * NT, kSplit = kDecodeWarps / HEADS, kStepKeys = kWarpKeys * kSplit;  // keys of a CTA's step
   constexpr int G = D / 32;  // groups of channels; words of a piece
   constexpr int kPerBlock = kBlockKeys / kStepKeys;
@@ -238,13 +237,15 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
   // half (even or odd channels) of the words, slots 2 p, 2 p + 1 and 8 more. In bytes of a stage.
   const int j = lane / 4, p = lane % 4;
   constexpr int kEight = kWarpKeys * D / 4;  // 8 keys on
-  const uint32_t codes_at = TMA ? warp * S::kCodes : 0, v_codes = (TMA ? kDecodeWarps : 1) * S::kCodes + codes_at;
+  const int split = warp / HEADS, step_row = TMA ? (warp % HEADS) * kSplit + split : 0;  // copies: [head][key]
+  const uint32_t codes_at = step_row * S::kCodes, v_codes = (TMA ? kDecodeWarps : 1) * S::kCodes + codes_at;
   const uint32_t k_at = codes_at + at<D>(key_of<D>(j), p);
   const uint32_t v_at[2] = {v_codes + at<D>(key_of<D>(2 * p), j % 4), v_codes + at<D>(key_of<D>(2 * p + 1), j % 4)};
   const uint32_t half_of = j / 4 ? 0x7632u : 0x5410u;
   const bool by_head = TMA && !maps.scales_by_slot;  // [slot][head]
-  const uint32_t scale_pitch = by_head ? kDecodeWarps * D / 16 : D / 16, scale_eight = 8 * scale_pitch;
-  const uint32_t ks_at = (TMA ? 2 * kDecodeWarps : 2) * S::kCodes + (!TMA ? 0 : by_head ? warp * (D / 16) : warp * S::kScale) +
+  const uint32_t scale_pitch = by_head ? HEADS * D / 16 : D / 16, scale_eight = 8 * scale_pitch;
+  const uint32_t ks_at = (TMA ? 2 * kDecodeWarps : 2) * S::kCodes +
+                         (by_head ? split * kWarpKeys * scale_pitch + warp % HEADS * (D / 16) : step_row * S::kScale) +
                          key_of<D>(j) * scale_pitch;
   const uint32_t vs_at = ks_at + (TMA ? kDecodeWarps : 1) * S::kScale;
   const bool wide = a.pages.page_log2 >= 4;  // a step's keys are in one page
@@ -330,7 +331,7 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
 
     // Positions relative to this warp's first key, in 32 bits (a request has fewer than 2^30 keys).
     const int steps = idle ? 0 : (b1 - b0) * kPerBlock;
-    const int warp_key = it.key0 + b0 * kBlockKeys + warp / HEADS * kWarpKeys;
+    const int warp_key = it.key0 + b0 * kBlockKeys + split * kWarpKeys;
     const int key_lo = it.lo - warp_key, key_hi = it.hi - warp_key;
     const int all_lo = a.window ? base + (row0 + rows - 1) / a.group - a.window + 1 - warp_key : kNone;
     const int all_hi = base + row0 / a.group - warp_key;  // every row sees keys all_lo .. all_hi
@@ -472,7 +473,9 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
     };
     if constexpr (TMA) {
       // Steps with keys that some row sees; warp i % 4 has the copies of step i.
-      const int step0 = max(key_lo, 0) / kWarpKeys, count = max(min(steps, (key_hi + kWarpKeys - 1) / kWarpKeys) - step0, 0);
+      const int first = warp_key - split * kWarpKeys, step0 = max(it.lo - first, 0) / kStepKeys;
+      const int count = max(min(steps, (it.hi - first + kStepKeys - 1) / kStepKeys) - step0, 0);
+      const bool was_lost = lost;
       int page_of = -1;  // page of step 4 (lane + 32 n) + warp
       uint32_t issued = loads, load = loads;  // this warp's last copies, the step that is waited for
       const auto issue = [&](int i) {
@@ -480,9 +483,9 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
         const int mine = i >> 2;
         if ((mine & 31) == 0) {
           const int step = (mine + lane) * 4 + warp;
-          page_of = step < count ? __ldg(table + ((warp_key + (step0 + step) * kWarpKeys) >> a.pages.page_log2)) : -1;
+          page_of = step < count ? __ldg(table + ((first + (step0 + step) * kStepKeys) >> a.pages.page_log2)) : -1;
         }
-        const int page = __shfl_sync(0xffffffffu, page_of, mine & 31), slot = (warp_key + (step0 + i) * kWarpKeys) & in_page;
+        const int page = __shfl_sync(0xffffffffu, page_of, mine & 31), slot = (first + (step0 + i) * kStepKeys) & in_page;
         const uint32_t load = loads + i, s = load % kRing, dst = ring + s * kStage;
         issued = load;
         if (!(lost = !__all_sync(0xffffffffu, phase_wait(&empty[s], (load / kRing & 1) ^ 1)))) {
@@ -510,7 +513,7 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
         load = loads + i;
         const uint32_t s = load % kRing;
         if (lost || (lost = !__all_sync(0xffffffffu, phase_wait(&full[s], load / kRing & 1)))) break;
-        products(ring + s * kStage, (step0 + i) * kWarpKeys);
+        products(ring + s * kStage, (step0 + i) * kStepKeys);
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[s]);
       }
@@ -518,7 +521,7 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
       if (lost) {
         bad_page = 1;  // rows without their keys are NaN
         // Copies of this warp that are under way have to arrive before the CTA goes on or ends.
-        for (; load <= issued; ++load) phase_wait(&full[load % kRing], load / kRing & 1);
+        for (; !was_lost && load <= issued; ++load) phase_wait(&full[load % kRing], load / kRing & 1);
       }
     } else {
       // Its places in the loads: a 16-byte chunk of K and of V in each pass over a step's rows, a row's scales of
@@ -707,25 +710,32 @@ cudaError_t launch(Int4Args args, const Maps& maps, cudaStream_t stream) {
                       args, maps);
   if (err != cudaSuccess || a.whole) return err;
   const unsigned rows = a.pages.cu_seqlens || a.group > kRows ? kRows : a.group;  // rows a tile can have
-  return launch_following(paged_join_kernel<T, D, kRows, false, HEADS>, dim3((unsigned)grid, rows, HEADS), dim3(kJoinWarps * 32),
-                          stream, a, grid);
+  const int64_t items = tiles * ((a.kv_heads + HEADS - 1) / HEADS);  // CTAs that can have begun one
+  // Many parts an item: wide CTAs, of which an SM holds one (2 requests of 131,071 keys, 222 parts an item:
+  // 33 us in all instead of 40 with 8 warps of 4 parts in flight); else small ones (64 requests of 8,192
+  // keys, up to 5 parts: 103 us instead of 123 with wide ones).
+  const dim3 joins((unsigned)(items < grid ? items : grid), rows, HEADS);
+  return items * 16 < grid ? launch_following(paged_join_kernel<T, D, kRows, false, HEADS, 16, 8, true>, joins, dim3(512), stream, a, grid)
+                           : launch_following(paged_join_kernel<T, D, kRows, false, HEADS, 4, 4, true>, joins, dim3(128), stream, a, grid);
 }
 
-// The maps of a cache that the copies of four heads can take: pages of 16 slots, four heads (or a multiple), scales
+// The maps of a cache that the copies of HEADS heads can take: pages of a step's keys, a multiple of the heads, scales
 // contiguous along the heads or along the slots, and what tensor maps want of strides.
+template <int HEADS>
 bool make_maps(const Int4Args& args, int D, Maps* maps) {
+  constexpr uint32_t kStepKeys = kWarpKeys * kDecodeWarps / HEADS;
   const AttentionArgs& a = args.a;
   const uint64_t slots = (uint64_t)1 << a.pages.page_log2, heads = (uint64_t)a.kv_heads, pages = (uint64_t)a.pages.num_pages;
-  if (slots < kWarpKeys || heads % kDecodeWarps || pages == 0) return false;
+  if (slots < kStepKeys || heads % HEADS || pages == 0) return false;
   const int G = D / 32;
-  const bool by_head = args.ks_head == G && args.vs_head == G, by_slot = args.ks_slot == G && args.vs_slot == G;
+  const bool by_slot = args.ks_slot == G && args.vs_slot == G, by_head = !(HEADS == 1 && by_slot) && args.ks_head == G && args.vs_head == G;
   if (!by_head && !by_slot) return false;
   maps->scales_by_slot = !by_head;
   const auto positive = [](int64_t bytes) { return bytes > 0; };
   const auto codes = [&](CUtensorMap* map, const void* base, int64_t slot, int64_t head, int64_t page) {
     const uint64_t dims[4] = {(uint64_t)D / 2, slots, heads, pages};
     const uint64_t strides[3] = {(uint64_t)slot, (uint64_t)head, pages > 1 ? (uint64_t)page : 128};
-    const uint32_t box[4] = {(uint32_t)D / 2, kWarpKeys, kDecodeWarps, 1};
+    const uint32_t box[4] = {(uint32_t)D / 2, kStepKeys, HEADS, 1};
     return positive(slot) && positive(head) && (pages == 1 || positive(page)) &&
            encode_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, base, dims, strides, box,
                              D == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B);
@@ -734,7 +744,7 @@ bool make_maps(const Int4Args& args, int D, Maps* maps) {
     const uint64_t dims[3] = {(by_head ? heads : slots) * G, by_head ? slots : heads, pages};
     const int64_t along = 2 * (by_head ? slot : head);
     const uint64_t strides[2] = {(uint64_t)along, pages > 1 ? (uint64_t)(2 * page) : 128};
-    const uint32_t box[3] = {(uint32_t)((by_head ? kDecodeWarps : kWarpKeys) * G), (uint32_t)(by_head ? kWarpKeys : kDecodeWarps), 1};
+    const uint32_t box[3] = {(by_head ? HEADS : kStepKeys) * G, by_head ? kStepKeys : HEADS, 1};
     return positive(along) && (pages == 1 || positive(page)) &&
            encode_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
   };
@@ -743,15 +753,18 @@ bool make_maps(const Int4Args& args, int D, Maps* maps) {
          scales(&maps->v_scale, args.v_scale, args.vs_slot, args.vs_head, args.vs_page);
 }
 
-// Key heads of a CTA: a cache line holds the scales of several heads' slots, and is fetched
+// Copies of four heads at a time want pages of 16 slots, those of two or one 32 and 64: a step of
+// the CTA's four warps is in one page. Key heads of a CTA: a cache line holds the scales of several heads' slots, and is fetched
 // once where one CTA reads them together. Four at a time, two, or one where most of four would idle.
 template <typename T, int D, int NT>
 cudaError_t launch_heads(const Int4Args& args, cudaStream_t stream) {
   const int heads = args.a.kv_heads;
   Maps maps{};
-  if (make_maps(args, D, &maps)) return launch<T, D, NT, 4, true>(args, maps, stream);
-  if (heads % 4 == 0 || heads % 4 == 3) return launch<T, D, NT, 4, false>(args, maps, stream);
-  return heads % 2 == 0 ? launch<T, D, NT, 2, false>(args, maps, stream) : launch<T, D, NT, 1, false>(args, maps, stream);
+  if (heads % 4 == 0 || heads % 4 == 3)
+    return make_maps<4>(args, D, &maps) ? launch<T, D, NT, 4, true>(args, maps, stream) : launch<T, D, NT, 4, false>(args, maps, stream);
+  if (heads % 2 == 0)
+    return make_maps<2>(args, D, &maps) ? launch<T, D, NT, 2, true>(args, maps, stream) : launch<T, D, NT, 2, false>(args, maps, stream);
+  return make_maps<1>(args, D, &maps) ? launch<T, D, NT, 1, true>(args, maps, stream) : launch<T, D, NT, 1, false>(args, maps, stream);
 }
 
 template <typename T, int D>

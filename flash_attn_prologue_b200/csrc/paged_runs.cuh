@@ -280,28 +280,51 @@ __device__ __forceinline__ Part part_of(const Run& run, const Item& it) {
   return p;
 }
 
-// Joins the parts of one row (and head) of the item that CTA blockIdx.x of the first kernel
-// began: every warp takes each eighth part, its columns over the lanes.
+// Joins the parts of one row (and head) of an item that CTAs of the first kernel share: every warp
+// takes each WARPS-th part, its columns over the lanes. Which item: the one that CTA blockIdx.x
+// of the first kernel began, or (PICK) the blockIdx.x-th of those that any CTA began, with a grid as large as the
+// items there can be.
 constexpr int kJoinWarps = 8;
-template <typename T, int D, int ROWS, bool SHIFTED, int HEADS = 1>
-__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const AttentionArgs a, int64_t ctas) {
+template <typename T, int D, int ROWS, bool SHIFTED, int HEADS = 1, int WARPS = kJoinWarps, int FLIGHT = 4, bool PICK = false>
+__global__ void __launch_bounds__(WARPS * 32) paged_join_kernel(const AttentionArgs a, int64_t ctas) {
   constexpr int kCols = D / 32;  // columns of a lane
-  __shared__ float joined[kJoinWarps][D], sums[kJoinWarps], tops[kJoinWarps];
+  __shared__ float joined[WARPS][D], sums[WARPS], tops[WARPS];
   const float* part_out = static_cast<const float*>(a.workspace);
   const float* part_stat = part_out + 2 * ctas * HEADS * ROWS * D;
   wait_for_previous_kernel();
-  const Part p = reinterpret_cast<const Part*>(part_stat + 2 * ctas * HEADS * ROWS * 2)[blockIdx.x];
+  const Part* all_parts = reinterpret_cast<const Part*>(part_stat + 2 * ctas * HEADS * ROWS * 2);
   const int head = HEADS == 1 ? 0 : blockIdx.z, row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (p.last < 0 || row >= p.rows || (HEADS > 1 && p.kv_head + head >= a.kv_heads)) return;
-  const int first = blockIdx.x, parts = p.last - first + 1;
-  float top = -INFINITY, sum = 0.f, o[kCols] = {};
-  constexpr int kFlight = 4;
-  for (int i0 = warp; i0 < parts; i0 += kJoinWarps * kFlight) {
-    float2 st[kFlight];
-    float x[kFlight][kCols];
+  int first = blockIdx.x;
+  if constexpr (PICK) {
+    __shared__ int counts[WARPS], found;
+    int before = 0;
+    for (int c0 = 0; c0 < ctas; c0 += WARPS * 32) {
+      const int c = c0 + threadIdx.x;
+      const unsigned begun = __ballot_sync(0xffffffffu, c < ctas && all_parts[c < ctas ? c : 0].last >= 0);
+      if (lane == 0) counts[warp] = __popc(begun);
+      __syncthreads();
+      int at = before + __popc(begun & ((1u << lane) - 1u));
 #pragma unroll
-    for (int f = 0; f < kFlight; ++f) {
-      const int i = i0 + f * kJoinWarps;
+      for (int w = 0; w < WARPS; ++w) {
+        if (w < warp) at += counts[w];
+        before += counts[w];
+      }
+      if (begun >> lane & 1 && at == (int)blockIdx.x) found = c;
+      __syncthreads();
+    }
+    if (before <= (int)blockIdx.x) return;
+    first = found;
+  }
+  const Part p = all_parts[first];
+  if (p.last < 0 || row >= p.rows || (HEADS > 1 && p.kv_head + head >= a.kv_heads)) return;
+  const int parts = p.last - first + 1;
+  float top = -INFINITY, sum = 0.f, o[kCols] = {};
+  for (int i0 = warp; i0 < parts; i0 += WARPS * FLIGHT) {
+    float2 st[FLIGHT];
+    float x[FLIGHT][kCols];
+#pragma unroll
+    for (int f = 0; f < FLIGHT; ++f) {
+      const int i = i0 + f * WARPS;
       st[f] = make_float2(-INFINITY, 0.f);
 #pragma unroll
       for (int c = 0; c < kCols; ++c) x[f][c] = 0.f;
@@ -321,14 +344,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Atten
     }
     float now = top;
 #pragma unroll
-    for (int f = 0; f < kFlight; ++f) now = fmaxf(now, st[f].x);
+    for (int f = 0; f < FLIGHT; ++f) now = fmaxf(now, st[f].x);
     const float from = now == -INFINITY ? 0.f : now, moved = exp2_approx(top - from);
     top = now;
     sum *= moved;
 #pragma unroll
     for (int c = 0; c < kCols; ++c) o[c] *= moved;
 #pragma unroll
-    for (int f = 0; f < kFlight; ++f) {
+    for (int f = 0; f < FLIGHT; ++f) {
       const float e = exp2_approx(st[f].x - from);
       sum += e * st[f].y;
 #pragma unroll
@@ -346,11 +369,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Atten
   if (col >= D) return;
   float m = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) m = fmaxf(m, tops[w]);
+  for (int w = 0; w < WARPS; ++w) m = fmaxf(m, tops[w]);
   const float from = m == -INFINITY ? 0.f : m;
   float v = 0.f, l = 0.f;
 #pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) {
+  for (int w = 0; w < WARPS; ++w) {
     const float e = exp2_approx(tops[w] - from);
     v += e * joined[w][col];
     l += e * sums[w];

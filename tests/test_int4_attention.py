@@ -492,3 +492,33 @@ def test_refused_layouts():
                       ("k_scale", torch.zeros(4, 16, 2, 3, dtype=BF16, device="cuda")[..., :2])):
         with pytest.raises(ValueError, match="align"):
             fap.paged_attention_int4(**{**args, name: bad})
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,dtype", [(64, FP16), (128, BF16)])
+@pytest.mark.parametrize("Hq,Hk,news,totals", [
+    (16, 2, [1, 1], [50001, 333]),
+    (12, 6, [2, 1, 1], [9000, 65, 64]),
+    (8, 1, [1], [30011]),
+    (9, 3, [1, 1, 0, 1], [4097, 31, 9, 20000]),
+    (5, 5, [1, 2], [70, 6001]),
+])
+@pytest.mark.parametrize("page,hnd,window", [(32, False, 0), (64, True, 0), (64, False, 1000), (128, True, 65)])
+def test_few_key_heads(Hq, Hk, news, totals, page, hnd, window, D, dtype):
+    req = Requests4(news, totals, Hq, Hk, D, page, dtype, hnd, seed=Hk)
+    _check(req, req.q.to(dtype), window=window)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Hk", [1, 2, 4])
+def test_pages_of_whole_steps_out_of_range(Hk):
+    req = Requests4([1, 1, 1], [700, 200, 900], 8, Hk, 128, 64, BF16)
+    q = req.q.to(BF16)
+    clean = _attend(req, q, decode=True)
+    _lib.device_error()
+    for wrong in (-1, 10 ** 6):
+        table = req.table.clone()
+        table[1, 1] = wrong
+        got = fap.paged_attention_int4(q, *req.cache, table, req.seq_lens)
+        assert _lib.device_error() == 2
+        assert got[1].isnan().all() and torch.equal(got[::2], clean[::2])
