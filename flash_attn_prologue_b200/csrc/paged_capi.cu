@@ -38,6 +38,10 @@ int size_checks(const flash_prologue_attention_args* a, bool int4) {
 // the maximum of the unscaled scores and multiplies masked ones (-infinity) by the
 // scale, so the FP32 scale has to be positive (and normal), and a tile holds at
 // least one whole token.
+//
+// Over a cache of 4 bits the other kernel takes tiles of 8 and 16 rows, and the rule stays. 12 rows a key head
+// (20 rows, tiled), 8 key heads x 128: 64 requests of 8,192 keys 270 (473) us, 64 of 2,048 keys 103 (130), 16 of
+// 4,096 60 (63); where there is little to read tiles would win, 32 of 1,024 45 (39), 4 of 4,096 34 (27).
 bool use_prefill(const flash_prologue_attention_args* a, float scale_log2) {
   const int64_t group = a->Hq / a->Hk;
   return a->tokens * group > 16 * a->cache.batch && group <= 128 && scale_log2 >= FLT_MIN;
@@ -61,9 +65,11 @@ int attention(const flash_prologue_attention_args* a, const flash_prologue_scale
   if (st != FLASH_PROLOGUE_OK || a->tokens == 0 || a->Hq == 0) return st;
   if (scales) {
     if ((st = check_scales(*scales, a->cache, a->D)) != FLASH_PROLOGUE_OK) return st;
-    // The kernels multiply pages and slots by strides of 31 bits.
-    for (int64_t s : {a->cache.k_page, a->cache.k_slot, a->cache.v_page, a->cache.v_slot, 2 * scales->k_page,
-                      2 * scales->k_slot, 2 * scales->v_page, 2 * scales->v_slot})
+    // The kernels multiply pages and slots by strides of 31 bits. (A single page has none.)
+    const bool pages = a->cache.num_pages > 1;
+    for (int64_t s : {a->cache.k_slot, a->cache.v_slot, 2 * scales->k_slot, 2 * scales->v_slot,
+                      pages ? a->cache.k_page : 0, pages ? a->cache.v_page : 0, pages ? 2 * scales->k_page : 0,
+                      pages ? 2 * scales->v_page : 0})
       if (s > INT32_MAX || s < INT32_MIN) return FLASH_PROLOGUE_ERR_UNSUPPORTED;
   }
   const flash_prologue_cache& c = a->cache;

@@ -631,7 +631,8 @@ typedef struct flash_prologue_scales {
 FLASH_PROLOGUE_API int flash_prologue_append_paged_int4(const flash_prologue_append_args* args,
                                                         const flash_prologue_scales* scales,
                                                         const flash_prologue_axes* axes, void* stream);
-/* flash_prologue_paged_attention over such a cache. */
+/* flash_prologue_paged_attention over such a cache. Strides of pages and slots have to fit 31 bits in bytes, of
+ * codes and of scales (FLASH_PROLOGUE_ERR_UNSUPPORTED); the strides of a single page count as none. */
 FLASH_PROLOGUE_API int flash_prologue_paged_attention_int4(const flash_prologue_attention_args* args,
                                                            const flash_prologue_scales* scales, void* stream);
 /* flash_prologue_selftest_attention_waits over such a cache. */

@@ -226,3 +226,15 @@ def test_too_many_requests_are_refused():
     i = lambda *x: torch.zeros(*x, dtype=torch.int32)  # noqa: E731
     with pytest.raises(ValueError, match="8192"):
         fap.plan_paged_step(i(n, 1), i(n), i(n), i(8), i(1), 8, 0)
+
+
+@pytest.mark.gpu
+def test_nothing_to_plan():
+    empty = torch.zeros(0, dtype=torch.int32, device="cuda")
+    count = torch.zeros(1, dtype=torch.int32, device="cuda")
+    _lib.device_error()
+    for tokens in (0, 3):
+        step = fap.plan_paged_step(empty.view(0, 4), empty, empty, empty, count, 16, tokens)
+        assert step.cu_seqlens.tolist() == [0] and step.free_count.tolist() == [0] and step.seq_lens.numel() == 0
+        assert step.requests.tolist() == step.slots.tolist() == [-1] * tokens and step.positions.tolist() == [0] * tokens
+    assert _lib.device_error() == 0

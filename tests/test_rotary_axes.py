@@ -262,3 +262,17 @@ def test_refusals(positions, axes, text):
     from flash_attn_prologue_b200.gqa import axes_of
     with pytest.raises(ValueError, match=text):
         axes_of(axes, positions, torch.zeros(5, 8, 64), 10)
+
+
+@pytest.mark.gpu
+def test_expanded_and_strided_positions():
+    q, k, w, s, sin, cos, pos, axes, up = _problem("packed", 1, 60, 8, 2, 64, BF16, 3, "interleaved")
+    same = fap.qknorm_rope_scale_gqa(q, k, w, s, sin, cos, pos[1])
+    for p in (pos[1].expand(3, -1), pos[1].long().expand(3, -1)):
+        assert all(torch.equal(x, y) for x, y in zip(fap.qknorm_rope_scale_gqa(q, k, w, s, sin, cos, p, axes=axes), same))
+    first = fap.qknorm_rope_scale_gqa(q, k, w, s, sin, cos, pos, axes=axes)
+    by_token = pos.t().contiguous().t()  # [axes, T], tokens outside
+    again = fap.qknorm_rope_scale_gqa(q, k, w, s, sin, cos, by_token, axes=list(axes))
+    assert all(torch.equal(x, y) for x, y in zip(again, first))
+    none = fap.qknorm_rope_scale_gqa(q[:0], k[:0], w, s, sin, cos, pos[:, :0], axes=axes)
+    assert [t.shape for t in none] == [q[:0].shape, k[:0].shape]
