@@ -2,10 +2,11 @@
 
 Training runs the prologue over packed documents (positions restart in each) with
 ``qknorm_rope_scale_gqa`` and its backward; serving feeds prompts in chunks and then single
-tokens through ``append_paged_kv`` and ``paged_attention``, with several requests in one step,
-and checks each request against the model run over its whole text at once.
+tokens through ``append_paged_kv`` and ``paged_attention``, with several requests in one step
+whose pages ``plan_paged_step`` hands out, and compares each request with the model run over its
+whole text at once. ``--int4`` holds the cache in 4 bits, which that comparison then shows.
 
-    python examples/serve_paged.py [--steps 30] [--requests 6] [--new 24]
+    python examples/serve_paged.py [--steps 30] [--requests 6] [--new 24] [--int4]
 """
 import argparse
 import math
@@ -66,42 +67,41 @@ class Model(nn.Module):
     def step(self, tokens, caches, table, lens, cu):
         """Logits of a serving step's new tokens, which join the caches."""
         x = self.embed(tokens)
-        for layer, (k_cache, v_cache) in zip(self.layers, caches):
+        for layer, cache in zip(self.layers, caches):
+            append, attend = ((fap.append_paged_kv, fap.paged_attention) if len(cache) == 2 else
+                              (fap.append_paged_kv_int4, fap.paged_attention_int4))
             q, k, v = layer.rows(x)
-            q = fap.append_paged_kv(q, k, v, layer.qk_weight, layer.scales, self.sin, self.cos, k_cache, v_cache, table,
-                                    lens, cu)
-            y = fap.paged_attention(q, k_cache, v_cache, table, lens, cu)
+            q = append(q, k, v, layer.qk_weight, layer.scales, self.sin, self.cos, *cache, table, lens, cu)
+            y = attend(q, *cache, table, lens, cu)
             x = x + layer.out(y.float().flatten(1))
         return self.head(x)
 
 
 class Server:
-    """Requests on a pool of pages: pages are handed out as requests grow."""
+    """Requests on a pool of pages: a table, lengths and a stack of free pages that stay on the GPU."""
 
-    def __init__(self, model, pages=256, page_size=16):
-        self.model, self.page_size = model, page_size
-        self.free = list(range(pages))
+    def __init__(self, model, requests, int4=False, pages=256, page_size=16):
+        self.model, self.requests, self.page_size = model, requests, page_size
+        self.table = torch.full((requests, MAX_LEN // page_size), -1, dtype=torch.int32, device="cuda")
+        self.lens = torch.zeros(requests, dtype=torch.int32, device="cuda")
+        self.free = torch.arange(pages, dtype=torch.int32, device="cuda")
+        self.free_count = torch.tensor([pages], dtype=torch.int32, device="cuda")
         shape = (pages, page_size, KV_HEADS, DIM)
-        self.caches = [tuple(torch.empty(shape, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        self.caches = [fap.int4_cache(*shape) if int4 else
+                       tuple(torch.empty(shape, dtype=torch.bfloat16, device="cuda") for _ in range(2))
                        for _ in model.layers]
-        self.pages, self.lens = {}, {}
 
     def step(self, new):
         """{request: its new tokens} -> {request: logits of the last of them}."""
-        names = list(new)
-        for r in names:
-            self.lens[r] = self.lens.get(r, 0) + len(new[r])
-            held = self.pages.setdefault(r, [])
-            while len(held) * self.page_size < self.lens[r]:
-                held.append(self.free.pop())
-        width = max(len(self.pages[r]) for r in names)
-        table = torch.tensor([self.pages[r] + [0] * (width - len(self.pages[r])) for r in names], dtype=torch.int32)
-        lens = torch.tensor([self.lens[r] for r in names], dtype=torch.int32)
-        ends = torch.tensor([0] + [len(new[r]) for r in names]).cumsum(0).to(torch.int32)
-        cu = None if int(ends[-1]) == len(names) else ends.cuda()
-        tokens = torch.tensor([t for r in names for t in new[r]])
-        logits = self.model.step(tokens.cuda(), self.caches, table.cuda(), lens.cuda(), cu)
-        return dict(zip(names, logits[(ends[1:] - 1).long().cuda()]))
+        news = torch.tensor([len(new.get(r, ())) for r in range(self.requests)], dtype=torch.int32)
+        tokens = torch.tensor([t for r in range(self.requests) for t in new.get(r, ())])
+        plan = fap.plan_paged_step(self.table, self.lens, news.cuda(), self.free, self.free_count, self.page_size,
+                                   len(tokens))
+        self.lens, self.free_count = plan.seq_lens, plan.free_count
+        cu = None if bool((news == 1).all()) else plan.cu_seqlens
+        logits = self.model.step(tokens.cuda(), self.caches, self.table, self.lens, cu)
+        last = news.cumsum(0) - 1
+        return {r: logits[int(last[r])] for r in new}
 
 
 def train(model, steps):
@@ -125,10 +125,10 @@ def train(model, steps):
     return float(losses[0]), float(losses[-1])
 
 
-def serve(model, requests, new):
+def serve(model, requests, new, int4=False):
     """Greedy continuations; the largest difference of a step's logits from the whole text's."""
     g = torch.Generator().manual_seed(1)
-    server = Server(model)
+    server = Server(model, requests, int4)
     texts = {r: torch.randint(0, VOCAB, (int(n),), generator=g).tolist()
              for r, n in enumerate(torch.randint(3, 120, (requests,), generator=g))}
     # prompts in chunks of up to 32 tokens, all requests together until each is read
@@ -161,12 +161,13 @@ def main(argv=None):
     ap.add_argument("--steps", type=int, default=30)
     ap.add_argument("--requests", type=int, default=6)
     ap.add_argument("--new", type=int, default=24)
+    ap.add_argument("--int4", action="store_true", help="hold the cache in 4 bits")
     args = ap.parse_args(argv)
     torch.manual_seed(0)
     model = Model().cuda()
     first, final = train(model, args.steps)
     print(f"trained {args.steps} steps: loss {first:.3f} -> {final:.3f}")
-    worst, rate = serve(model, args.requests, args.new)
+    worst, rate = serve(model, args.requests, args.new, args.int4)
     print(f"served {args.requests} requests: {rate:.0f} tokens/s, logits within {worst:.4f} of the whole text's")
     return first, final, worst
 
