@@ -33,6 +33,14 @@
 //              zeros for slots outside the tile's keys, and for infinities and
 //              NaNs, which 0 * V would carry into rows that do not see them
 //              (the epilogue adds them to the rows that do).
+// Over a cache of 4 bits, kInt4, more warps behind these eight turn codes into the values
+// they stand for, exactly, in the places where TMA would have put them (half of these
+// warps make K, half V; they do warp 7's work on the scales), and the rest stays as it is. A thread of theirs
+// has 64 values of a key, about three instructions for two of them, so at D = 128 two tiles of 128 rows,
+// each with four warps of its own, share what is made (kPair). 4,096 tokens over 16,384 keys, 32/8 heads x 128 BF16:
+// 896 us, 1,074 TFLOP/s (16-bit cache 770 to 785 us), back to back 910 to 1,010 under the power cap; tensor and
+// exponential pipes 50% busy each, issue slots 58%. A warp for each tile's scores instead of one for both: the
+// same. The windowed chunks above: 71 us (16-bit cache 61); issue slots 53%, exponentials 41%.
 // The running maximum that scales O is only moved when a row's maximum has
 // grown by more than 2^8: until then the probabilities are at most 2^8 instead
 // of 1, which neither type nor sum minds, and O stays where it is.
