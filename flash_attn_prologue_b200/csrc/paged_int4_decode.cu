@@ -29,7 +29,8 @@
 // the four warps' step and the layout is one for tensor maps, a step comes by four
 // copies into a ring of the CTA, else every warp loads its own with cp.async (64 requests:
 // 113 us instead of 120). 16 keys a step and 3 CTAs an SM at D = 128 are what 168 registers
-// hold: 32 keys 123 to 127 us, 4 CTAs 125 to 154 (spilled registers), 2 CTAs 117 instead of 103.
+// hold: 32 keys 123 to 127 us, 4 CTAs 123 (at 128 registers), 2 CTAs 117 instead of 103. One product's
+// rows for the 8 sum p s of all groups would save 12 registers, but its sums wait for one another: 106 us.
 //
 // Measured (32/8 heads x 128 BF16 unless said): 64 requests of up to 8,192 keys 103 us, 343 MB, 3.3
 // TB/s (52 us at the copy rate; the same over a 16-bit cache 199 to 209 us); issue slots 52% and ALU 49%
