@@ -29,10 +29,10 @@
 // the four warps' step and the layout is one for tensor maps, a step comes by four
 // copies into a ring of the CTA, else every warp loads its own with cp.async (64 requests:
 // 113 us instead of 120). 16 keys a step and 3 CTAs an SM at D = 128 are what 168 registers
-// hold: 32 keys 123 to 127 us, 4 CTAs 123 (at 128 registers), 2 CTAs 117 instead of 103. One product's
-// rows for the 8 sum p s of all groups would save 12 registers, but its sums wait for one another: 106 us.
+// hold: 32 keys 123 to 127 us, 4 CTAs 123 (at 128 registers), 2 CTAs 117 (3 took 102 to 103 then). One product's
+// rows for the 8 sum p s of all groups would save 12 registers, but its sums wait for one another: 106 us instead of 102.
 //
-// Measured (32/8 heads x 128 BF16 unless said): 64 requests of up to 8,192 keys 103 us, 343 MB, 3.3
+// Measured (32/8 heads x 128 BF16 unless said): 64 requests of up to 8,192 keys 98 us, 339 MB, 3.5
 // TB/s (52 us at the copy rate; the same over a 16-bit cache 199 to 209 us); issue slots 52% and ALU 49%
 // busy with three warps a scheduler: about 390 instructions a step, half of them products, masks of codes
 // and the scales' multiplications. 2 requests of 131,071 keys, 16/2 heads FP16: 33 us (16-bit cache 54). 1
@@ -722,11 +722,16 @@ cudaError_t launch(Int4Args args, const Maps& maps, cudaStream_t stream) {
   const unsigned rows = a.pages.cu_seqlens || a.group > kRows ? kRows : a.group;  // rows a tile can have
   const int64_t items = tiles * ((a.kv_heads + HEADS - 1) / HEADS);  // CTAs that can have begun one
   // Many parts an item: wide CTAs, of which an SM holds one (2 requests of 131,071 keys, 222 parts an item:
-  // 33 us in all instead of 40 with 8 warps of 4 parts in flight); else small ones (64 requests of 8,192
-  // keys, up to 5 parts: 103 us instead of 123 with wide ones).
+  // 33 us in all instead of 40 with 8 warps of 4 parts in flight). Few: a warp a row (64 requests of up to 8,192
+  // keys, up to 5 parts: 98 us; 101 with a small CTA a row, 123 with wide ones). Between them a small CTA a row (1
+  // request of 1,000 keys, 16 parts: 11.6 us; 13.0 with a warp a row).
   const dim3 joins((unsigned)(items < grid ? items : grid), rows, HEADS);
-  return items * 16 < grid ? launch_following(paged_join_kernel<T, D, kRows, false, HEADS, 16, 8, true>, joins, dim3(512), stream, a, grid)
-                           : launch_following(paged_join_kernel<T, D, kRows, false, HEADS, 4, 4, true>, joins, dim3(128), stream, a, grid);
+  if (items * 16 < grid)
+    return launch_following(paged_join_kernel<T, D, kRows, false, HEADS, 16, 8, true>, joins, dim3(512), stream, a, grid);
+  if (items * 8 < grid)
+    return launch_following(paged_join_kernel<T, D, kRows, false, HEADS, 4, 4, true>, joins, dim3(128), stream, a, grid);
+  return launch_following(paged_join_kernel<T, D, kRows, false, HEADS, 4, 8, true, 1>, dim3(joins.x, (rows + 3) / 4, HEADS),
+                          dim3(128), stream, a, grid);
 }
 
 // The maps of a cache that the copies of HEADS heads can take: pages of a step's keys, a multiple of the heads, scales

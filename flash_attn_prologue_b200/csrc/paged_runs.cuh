@@ -280,36 +280,51 @@ __device__ __forceinline__ Part part_of(const Run& run, const Item& it) {
   return p;
 }
 
-// Joins the parts of one row (and head) of an item that CTAs of the first kernel share: every warp
-// takes each WARPS-th part, its columns over the lanes. Which item: the one that CTA blockIdx.x
+// Joins the parts of one row (and head) of an item that CTAs of the first kernel share: each of TEAM warps
+// takes every TEAM-th part, its columns over the lanes; a CTA has WARPS / TEAM rows. Which item: the one that CTA blockIdx.x
 // of the first kernel began, or (PICK) the blockIdx.x-th of those that any CTA began, with a grid as large as the
 // items there can be.
 constexpr int kJoinWarps = 8;
-template <typename T, int D, int ROWS, bool SHIFTED, int HEADS = 1, int WARPS = kJoinWarps, int FLIGHT = 4, bool PICK = false>
+template <typename T, int D, int ROWS, bool SHIFTED, int HEADS = 1, int WARPS = kJoinWarps, int FLIGHT = 4, bool PICK = false,
+          int TEAM = WARPS>
 __global__ void __launch_bounds__(WARPS * 32) paged_join_kernel(const AttentionArgs a, int64_t ctas) {
   constexpr int kCols = D / 32;  // columns of a lane
-  __shared__ float joined[WARPS][D], sums[WARPS], tops[WARPS];
   const float* part_out = static_cast<const float*>(a.workspace);
   const float* part_stat = part_out + 2 * ctas * HEADS * ROWS * D;
   wait_for_previous_kernel();
   const Part* all_parts = reinterpret_cast<const Part*>(part_stat + 2 * ctas * HEADS * ROWS * 2);
-  const int head = HEADS == 1 ? 0 : blockIdx.z, row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  static_assert(TEAM == WARPS || TEAM == 1, "rows of a CTA");
+  const int head = HEADS == 1 ? 0 : blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = TEAM == 1 ? blockIdx.y * WARPS + warp : blockIdx.y, mate = TEAM == 1 ? 0 : warp;
   int first = blockIdx.x;
   if constexpr (PICK) {
-    __shared__ int counts[WARPS], found;
+    constexpr int kRounds = 16 / WARPS;  // loads in flight
+    __shared__ int counts[kRounds * WARPS], found;
     int before = 0;
-    for (int c0 = 0; c0 < ctas; c0 += WARPS * 32) {
-      const int c = c0 + threadIdx.x;
-      const unsigned begun = __ballot_sync(0xffffffffu, c < ctas && all_parts[c < ctas ? c : 0].last >= 0);
-      if (lane == 0) counts[warp] = __popc(begun);
-      __syncthreads();
-      int at = before + __popc(begun & ((1u << lane) - 1u));
+    for (int c0 = 0; c0 < ctas; c0 += kRounds * WARPS * 32) {
+      int last[kRounds];
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        if (w < warp) at += counts[w];
-        before += counts[w];
+      for (int r = 0; r < kRounds; ++r) {
+        const int c = c0 + (r * WARPS + warp) * 32 + lane;
+        last[r] = c < ctas ? all_parts[c].last : -1;
       }
-      if (begun >> lane & 1 && at == (int)blockIdx.x) found = c;
+      unsigned begun[kRounds];
+#pragma unroll
+      for (int r = 0; r < kRounds; ++r) {
+        begun[r] = __ballot_sync(0xffffffffu, last[r] >= 0);
+        if (lane == 0) counts[r * WARPS + warp] = __popc(begun[r]);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < kRounds; ++r) {
+        int at = before + __popc(begun[r] & ((1u << lane) - 1u));
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+          if (w < warp) at += counts[r * WARPS + w];
+          before += counts[r * WARPS + w];
+        }
+        if (begun[r] >> lane & 1 && at == (int)blockIdx.x) found = c0 + (r * WARPS + warp) * 32 + lane;
+      }
       __syncthreads();
     }
     if (before <= (int)blockIdx.x) return;
@@ -319,12 +334,12 @@ __global__ void __launch_bounds__(WARPS * 32) paged_join_kernel(const AttentionA
   if (p.last < 0 || row >= p.rows || (HEADS > 1 && p.kv_head + head >= a.kv_heads)) return;
   const int parts = p.last - first + 1;
   float top = -INFINITY, sum = 0.f, o[kCols] = {};
-  for (int i0 = warp; i0 < parts; i0 += WARPS * FLIGHT) {
+  for (int i0 = mate; i0 < parts; i0 += TEAM * FLIGHT) {
     float2 st[FLIGHT];
     float x[FLIGHT][kCols];
 #pragma unroll
     for (int f = 0; f < FLIGHT; ++f) {
-      const int i = i0 + f * WARPS;
+      const int i = i0 + f * TEAM;
       st[f] = make_float2(-INFINITY, 0.f);
 #pragma unroll
       for (int c = 0; c < kCols; ++c) x[f][c] = 0.f;
@@ -358,30 +373,41 @@ __global__ void __launch_bounds__(WARPS * 32) paged_join_kernel(const AttentionA
       for (int c = 0; c < kCols; ++c) o[c] += e * x[f][c];
     }
   }
-#pragma unroll
-  for (int c = 0; c < kCols; ++c) joined[warp][lane * kCols + c] = o[c];
-  if (lane == 0) {
-    sums[warp] = sum;
-    tops[warp] = top;
-  }
-  __syncthreads();
-  const int col = threadIdx.x;
-  if (col >= D) return;
-  float m = -INFINITY;
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) m = fmaxf(m, tops[w]);
-  const float from = m == -INFINITY ? 0.f : m;
-  float v = 0.f, l = 0.f;
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) {
-    const float e = exp2_approx(tops[w] - from);
-    v += e * joined[w][col];
-    l += e * sums[w];
-  }
   const int at = p.row0 + row, token = at / a.group;
   const int h = (p.kv_head + head) * a.group + (at - token * a.group);
-  static_cast<T*>(a.out)[(p.token0 + token) * a.out_n + h * a.out_h + col] = from_float<T>(l == 0.f ? 0.f : v / l);
-  if (a.lse && col == 0) a.lse[(int64_t)(p.token0 + token) * a.heads + h] = (m + log2f(l) - (SHIFTED ? kProbabilityShift<T> : 0.f)) * 0.6931471805599453f;
+  T* out = static_cast<T*>(a.out) + (p.token0 + token) * a.out_n + h * a.out_h;
+  const auto put_lse = [&](float m, float l) {
+    if (a.lse) a.lse[(int64_t)(p.token0 + token) * a.heads + h] = (m + log2f(l) - (SHIFTED ? kProbabilityShift<T> : 0.f)) * 0.6931471805599453f;
+  };
+  if constexpr (TEAM == 1) {
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) out[lane * kCols + c] = from_float<T>(sum == 0.f ? 0.f : o[c] / sum);
+    if (lane == 0) put_lse(top, sum);
+  } else {
+    __shared__ float joined[WARPS][D], sums[WARPS], tops[WARPS];
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) joined[warp][lane * kCols + c] = o[c];
+    if (lane == 0) {
+      sums[warp] = sum;
+      tops[warp] = top;
+    }
+    __syncthreads();
+    const int col = threadIdx.x;
+    if (col >= D) return;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) m = fmaxf(m, tops[w]);
+    const float from = m == -INFINITY ? 0.f : m;
+    float v = 0.f, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float e = exp2_approx(tops[w] - from);
+      v += e * joined[w][col];
+      l += e * sums[w];
+    }
+    out[col] = from_float<T>(l == 0.f ? 0.f : v / l);
+    if (col == 0) put_lse(m, l);
+  }
 }
 
 }  // namespace
