@@ -44,8 +44,10 @@
 namespace flash_prologue {
 namespace {
 
-constexpr int kRing = 4;             // steps of a ring
-constexpr int kAhead = 2;            // steps that a CTA's common ring is loaded ahead
+// Steps of a ring, and how many a CTA's common ring is loaded ahead. (6 and 4, 6 and 3, 5 and 3: 99 to 100 us
+// where 4 and 2 take 98.)
+constexpr int kRing = 4;
+constexpr int kAhead = 2;
 constexpr int kBlockKeys = kWarpKeys * kDecodeWarps;
 constexpr int kCtasPerSm = 4;
 constexpr int kLeastScale = -80;     // least exponent of sigma: sums of 2^(15 + 80) stay inside FP32
