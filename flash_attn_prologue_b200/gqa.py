@@ -93,16 +93,28 @@ def rotary_axes(sections, interleaved=False):
     return tuple(out)
 
 
+def _axis_bytes(axes):
+    """The axes' numbers, a byte each: patterns are kept by these, never by objects whose value may change."""
+    if not isinstance(axes, torch.Tensor):
+        try:
+            return bytes(axes if type(axes) is tuple else tuple(axes))
+        except TypeError:
+            pass
+        except ValueError:
+            raise ValueError(f"axes must be in 0 .. {MAX_AXES - 1}") from None
+    raise ValueError("axes must be a sequence of whole numbers")
+
+
 @functools.lru_cache(maxsize=64)
 def _packed_axes(axes, half):
     """``pairs`` of flash_prologue_axes, and one more than the last axis."""
     if len(axes) != half:
         raise ValueError("axes must name the axis of each of the D / 2 rotation pairs")
-    if min(axes) < 0 or max(axes) >= MAX_AXES:
+    if max(axes) >= MAX_AXES:
         raise ValueError(f"axes must be in 0 .. {MAX_AXES - 1}")
     words = [0] * 4
     for j, a in enumerate(axes):
-        words[j // 32] |= int(a) << 2 * (j % 32)
+        words[j // 32] |= a << 2 * (j % 32)
     return tuple(words), max(axes) + 1
 
 
@@ -120,7 +132,7 @@ def axes_of(axes, positions, q, rows):
         words, count, named = (0, 0, 0, 0), 1, 1
         shape, st = (1, *shape), (0, *st)
     else:
-        words, named = _packed_axes(tuple(axes), half)
+        words, named = _packed_axes(_axis_bytes(axes), half)
         count = shape[0] if shape else 0
     if shape[1:] != tokens and shape[1:] != tokens[1:] or not named <= count <= MAX_AXES or len(shape) < 2:
         raise ValueError("positions must be [axes,T] for packed rows, [axes,N] or [axes,B,N] for dense rows")
