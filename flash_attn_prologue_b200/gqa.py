@@ -307,7 +307,7 @@ class _GqaEager(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, rmsnorm_weight, scales, sin, cos, positions, eps, axes):
         ctx.save_for_backward(q, k, rmsnorm_weight, scales, sin, cos, positions)
-        ctx.eps, ctx.axes = eps, axes
+        ctx.eps, ctx.axes = eps, None if axes is None else tuple(_axis_bytes(axes))  # a list may change until the backward
         return _forward(q, k, rmsnorm_weight, scales, sin, cos, positions, eps, axes)
 
     @staticmethod

@@ -3,8 +3,10 @@ import numpy as np
 import pytest
 import torch
 
+import flash_attn_prologue_b200 as fap
 from flash_attn_prologue_b200 import _lib
 from flash_attn_prologue_b200.gqa import axes_of
+from tests._paged import tables
 
 ROWS, POSITIONS = torch.zeros(5, 8, 64), torch.zeros(3, 5, dtype=torch.int32)
 
@@ -47,3 +49,20 @@ def test_numbers_out_of_range():
     for wrong in (-1, 4, 255, 256, 2 ** 70):
         with pytest.raises(ValueError, match="in 0 .. 3"):
             _words([0] * 31 + [wrong])
+
+
+@pytest.mark.gpu
+def test_a_list_that_changes_before_the_backward():
+    g = torch.Generator(device="cuda").manual_seed(0)
+    q, k = (torch.randn(5, h, 64, generator=g, device="cuda").requires_grad_() for h in (4, 2))
+    w, s = torch.ones(2, 1, 64, device="cuda"), torch.zeros(4, 1, 1, device="cuda")
+    positions = torch.randint(0, 30, (3, 5), generator=g, device="cuda")
+    up = [torch.randn(t.shape, generator=g, device="cuda") for t in (q, k)]
+    axes = [j % 3 for j in range(32)]
+    grads = []
+    for change in (False, True):
+        out = fap.qknorm_rope_scale_gqa(q, k, w, s, *tables(30, 64), positions, axes=axes)
+        if change:
+            axes[:] = [0] * 32
+        grads.append(torch.autograd.grad(out, (q, k), up))
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
