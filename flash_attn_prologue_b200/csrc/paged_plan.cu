@@ -50,6 +50,9 @@ __device__ __forceinline__ Growth growth_of(const flash_prologue_plan_args& a, i
   return g;
 }
 
+// Sums end at kMostTokens, where two of them still fit 32 bits unsigned (new tokens may be 2^30 in many requests).
+__device__ __forceinline__ int sum_of(int a, int b) { return (int)min((unsigned)a + (unsigned)b, (unsigned)kMostTokens); }
+
 // The last request whose sum is at most i: sums[r] <= i < sums[r + 1].
 __device__ __forceinline__ int request_at_sum(const int* sums, int batch, int i) {
   int lo = 0, hi = batch;
@@ -86,7 +89,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const flash_pr
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, upto[s], o);
-        if (lane >= o) upto[s] = min(upto[s] + v, kMostTokens);  // saturates: sums stay inside 32 bits
+        if (lane >= o) upto[s] = sum_of(upto[s], v);
       }
       if (lane == 31) warp_sums[s][warp] = upto[s];
     }
@@ -98,12 +101,12 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const flash_pr
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int v = __shfl_up_sync(0xffffffffu, all, o);
-        if (lane >= o) all = min(all + v, kMostTokens);
+        if (lane >= o) all = sum_of(all, v);
       }
       const int in_front = warp ? __shfl_sync(0xffffffffu, all, warp - 1) : 0;
-      const int start = min(before[s] + in_front, kMostTokens);
-      if (r < batch) of[s][r + 1] = min(start + upto[s], kMostTokens);
-      before[s] = min(before[s] + __shfl_sync(0xffffffffu, all, 31), kMostTokens);
+      const int start = sum_of(before[s], in_front);
+      if (r < batch) of[s][r + 1] = sum_of(start, upto[s]);
+      before[s] = sum_of(before[s], __shfl_sync(0xffffffffu, all, 31));
     }
     __syncthreads();
   }
