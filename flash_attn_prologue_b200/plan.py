@@ -95,7 +95,9 @@ def plan_paged_step(page_table, seq_lens, new_lens, free_pages, free_count, page
 
     page_size is a power of two, at least 8; at most 8,192 requests. Nothing is read back from the
     GPU. Where free pages run out the table gets -1 (append_paged_kv then leaves such tokens out, and
-    their attention is NaN) and so do the tokens' slots; that, lengths out of range, and pages that
+    their attention is NaN) and so do the tokens' slots. Lengths count such tokens all the same, and
+    the entries stay -1 until the request ends, which returns the pages that it has and no other
+    entry (nor any that a caller set below 0). A shortage, lengths out of range, and pages that
     the stack has no room for set the device error word.
     """
     args = (page_table, seq_lens, new_lens, free_pages, free_count, page_size, tokens, keep)

@@ -649,15 +649,16 @@ FLASH_PROLOGUE_API int flash_prologue_unpack_int4(const void* codes, const void*
  * ---------------------------------------------------------------------------
  * A step's page tables, lengths, positions and slots from its requests' lengths.
  * Request r holds seq_lens[r] tokens and gets new_lens[r] more; below 0 it has
- * ended: its pages (but the first keep[r]) go on top of the stack of free pages,
- * request by request, and it is empty. Then requests take the pages that they
+ * ended: its pages (but the first keep[r]; entries below 0 are none) go on top of the
+ * stack of free pages, request by request, and it is empty. Then requests take the pages that they
  * grow by from the top of the stack, in order, into page_table. seq_lens_out are
  * the lengths after the step, cu_seqlens the running sum of the new tokens,
  * free_count_out the pages left on the stack. requests, positions, slots: of each
  * of `tokens` packed new tokens its request, its position in it and page *
  * page_size + slot; -1, 0 and -1 behind the last. Inputs other than page_table and
  * free_pages stay as they are, and these may not overlap the outputs.
- * Where pages run out the table's entries are -1 and the tokens' slots too; where
+ * Where pages run out the table's entries are -1 and the tokens' slots too, and they
+ * stay so until the request ends and returns the pages that it has; where
  * the stack has no room returned pages are lost; a length that the table has no
  * room for leaves slots of -1. All of these set bit 1 of the device error word,
  * as do lengths out of range.
