@@ -17,11 +17,14 @@
 // product where 16-row tiles of Q would leave half empty.
 //
 // Q is FP16 for the product, scaled by a power of two a row so that its largest
-// value is 2^14 to 2^15 (what falls below 2^-24 is 2^-39 of that). The weights
-// p s are rounded to FP16 once, scaled by 2^7 and the power of two sigma above the
-// largest scale that the row has seen, so that they are at most 2^15; an error of the size
-// of a 16-bit output's rounding. Scores, statistics and sums are FP32. The maximum
-// that scales a row of O moves only when the row's has grown by more than 2^8.
+// value is 2^14 to 2^15, or 2^10 to 2^11 beside codes of 16 u: values below 2^-24 of these
+// (2^-35 of the row's largest) lose bits to FP16's steps. The weights
+// p s are rounded to FP16 once, p 2^8 times as large and s less the power of two sigma above the
+// largest scales that the row has seen in this group of channels, so that they are below 2^15: an error of the size
+// of a 16-bit output's rounding, and where a weight is below 2^-14, of 2^-33 of that power (with one
+// sigma for all groups it was that of the largest group for all: 2 us of 100 less). A sigma that moves goes one
+// further than it has to (each time as far as it has to: 3 us more). Scores, statistics and sums are FP32. The
+// maximum that scales a row of O moves only when the row's has grown by more than 2^7.
 //
 // Work is shared out as in paged_decode.cu (paged_runs.cuh). A warp takes 16 keys of
 // one key head a step; a CTA's four warps take neighbouring heads of the same keys
@@ -50,7 +53,10 @@ constexpr int kRing = 4;
 constexpr int kAhead = 2;
 constexpr int kBlockKeys = kWarpKeys * kDecodeWarps;
 constexpr int kCtasPerSm = 4;
-constexpr int kLeastScale = -80;     // least exponent of sigma: sums of 2^(15 + 80) stay inside FP32
+// Exponents of the powers of two above a group's scales: with these, 2^-sigma and 2^(sigma - 8) are normal numbers.
+constexpr int kLeastScale = -110, kMostScale = 126;
+// A probability of 1 is 2^8 here, and a row's maximum moves where one would be more than 2^15.
+constexpr float kShift = 8.f, kMostWeight = 0x1p15f, kMostGrowth = 7.f;
 constexpr float kNoTop = -3e38f;      // the maximum of a row that has seen no key
 constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
 
@@ -96,6 +102,17 @@ __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
 }
 __device__ __forceinline__ float2 floats_of(uint32_t half2) { return __half22float2(*reinterpret_cast<__half2*>(&half2)); }
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }  // -126 .. 127
+// Words of two 16-bit numbers. Magnitudes of BF16 numbers compare as whole numbers do.
+__device__ __forceinline__ uint32_t finite_sizes(uint32_t x) {  // |x|, zero for infinities and NaNs
+  x &= 0x7fff7fffu;
+  return x & ~(((x + 0x00800080u) >> 15 & 0x00010001u) * 0xffffu);
+}
+__device__ __forceinline__ uint32_t bf16_power(int e) { return (uint32_t)(e + 127) << 7; }
+__device__ __forceinline__ __nv_bfloat162 bf16x2_of(uint32_t a) { return *reinterpret_cast<__nv_bfloat162*>(&a); }
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {  // (exact by powers of two)
+  const __nv_bfloat162 x = __hmul2(bf16x2_of(a), bf16x2_of(b));
+  return *reinterpret_cast<const uint32_t*>(&x);
+}
 // The two BF16 numbers of a word.
 __device__ __forceinline__ float low_bf16(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float high_bf16(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
@@ -220,6 +237,8 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ RunScratch shared;
   __shared__ float stat[kDecodeWarps][kRows][2];
+  // 2^-sigma of each group and column of a warp's tile: sigma is the power of two above the scales of V that the row has seen.
+  __shared__ __align__(8) float inv_scale[kDecodeWarps][NT][G][8];
   __shared__ int bad_page;
   __shared__ uint64_t full[kRing], empty[kRing];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -275,7 +294,7 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
 
     // Q: row 8 n + j of the tile, this lane's channels 8 (p G + g) .. + 7 of each group, times a power of two.
     float row_scale[NT][2];  // takes their sums to base-2 scores
-    int see_hi[NT][2];       // last position that they see
+    int see_hi[NT][2];       // last position that they see (behind the tile's rows: as its last row)
     const auto token_of = [&](int row) { return q.news == 1 ? 0 : (row0 + row) / a.group; };  // (a division)
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -318,13 +337,15 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
         const int up = __shfl_sync(0xffffffffu, e, (2 * p + x2) * 4) + 10;
         row_scale[n][x2] = a.scale_log2 * power_of_two(up / 2) * power_of_two(up - up / 2);
         const int at_row = 8 * n + 2 * p + x2;
-        see_hi[n][x2] = at_row < rows ? base + token_of(at_row) : -1;
+        see_hi[n][x2] = base + token_of(min(at_row, rows - 1));
       }
     }
-    // Of a column: probabilities are 2^(score - from), from = top + sigma - 7 (whole numbers: no
-    // rounding); `over` is what they reach 2^8 above top, 2^(15 - sigma); `limit` is 2^(least sigma).
-    float acc[NT][G][2][4], eights[NT][G][4], from[NT][2], over[NT][2], sum[NT][2], limit = power_of_two(kLeastScale);
-    const auto sigma_of = [](float over) { return 15 - ((int)(__float_as_uint(over) >> 23) - 127); };
+    // Of a column: probabilities are 2^(score - from), from = top - kShift (whole numbers: no rounding). inv: 2^-sigma of each group, sigma the least of this lane's columns, as BF16 numbers.
+    float acc[NT][G][2][4], eights[NT][G][4], from[NT][2], sum[NT][2];
+    uint32_t inv[G / 2];
+#pragma unroll
+    for (int i = 0; i < G / 2; ++i) inv[i] = bf16_power(-kLeastScale) * 0x10001u;
+    for (int i = lane; i < NT * G * 8; i += 32) (&inv_scale[warp][0][0][0])[i] = power_of_two(-kLeastScale);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -334,7 +355,6 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         from[n][x] = kNoTop;
-        over[n][x] = power_of_two(15 - kLeastScale);
         sum[n][x] = 0.f;
       }
     }
@@ -347,10 +367,12 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
     const int key_lo = it.lo - warp_key, key_hi = it.hi - warp_key;
     const int all_lo = a.window ? base + (row0 + rows - 1) / a.group - a.window + 1 - warp_key : kNone;
     const int all_hi = base + row0 / a.group - warp_key;  // every row sees keys all_lo .. all_hi
+    const bool one_token = token_of(0) == token_of(rows - 1);
     const int32_t* table = a.pages.page_table + (int64_t)it.r * a.pages.table_stride;
-    // A step's scores, probabilities and product; EDGE: some row does not see some key.
-    const auto compute = [&](auto edge, uint32_t here, int key) {
-      constexpr bool EDGE = decltype(edge)::value;
+    // A step's scores, probabilities and product; EDGE: some row does not see some key. ONE: all rows see the same keys, so
+    // the columns' sigmas are the same.
+    const auto compute = [&](auto edge, auto one, uint32_t here, int key) {
+      constexpr bool EDGE = decltype(edge)::value, ONE = decltype(one)::value;
       // Sums of keys key_of(j) and 8 more (x / 2), columns 2 p and 2 p + 1 (x % 2).
       float s[NT][4] = {};
       {
@@ -379,72 +401,89 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
       Scales<G> va, vb;
       va.load(here + vs_at);
       vb.load(here + vs_at + scale_eight);
-      float fa[G], fb[G], largest = 0.f;
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        fa[g] = va.get(g);
-        fb[g] = vb.get(g);
-        largest = fmaxf(largest, fmaxf(fabsf(fa[g]), fabsf(fb[g])));
-      }
       const auto sees = [&](int n, int x) {
         const int k = warp_key + key + key_of<D>(j) + (x / 2) * 8, hi = see_hi[n][x & 1];
         return k <= hi && (!a.window || k > hi - a.window);
       };
-      float w[NT][4];  // probabilities times 2^(7 - sigma)
-      bool move = EDGE || largest >= limit;
+      float w[NT][4];  // probabilities times 2^8
+      Scales<G> ua, ub;  // the scales of V times 2^-sigma: below 1, or a sigma moves
+      __nv_bfloat162 largest = bf16x2_of(0);
+#pragma unroll
+      for (int i = 0; i < G / 2; ++i) {
+        ua.w[i] = mul_bf16x2(va.w[i], inv[i]);
+        ub.w[i] = mul_bf16x2(vb.w[i], inv[i]);
+        largest = __hmax2(largest, __hmax2(__habs2(bf16x2_of(ua.w[i])), __habs2(bf16x2_of(ub.w[i]))));
+      }
+      bool move = EDGE || !__hblt2(largest, __float2bfloat162_rn(1.f));
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int x = 0; x < 4; ++x) w[n][x] = exp2_approx(fmaf(s[n][x], row_scale[n][x & 1], -from[n][x & 1]));
-        move |= fmaxf(w[n][0], w[n][2]) > over[n][0] || fmaxf(w[n][1], w[n][3]) > over[n][1];
+        move |= fmaxf(fmaxf(w[n][0], w[n][2]), fmaxf(w[n][1], w[n][3])) > kMostWeight;
       }
       if (__any_sync(0xffffffffu, move)) {
-        // A row's maximum or its largest scale may have moved: its O and sums follow. Each row goes by
+        // A row's maximum or a group's largest scale may have moved: its O and sums follow. Each row goes by
         // the keys that it sees, so what others see does not change its bits.
-        float size[2] = {0.f, 0.f};  // largest scale of this lane's keys; infinities and NaNs lose their own group only
+        uint32_t size[2][G / 2];  // scales of this lane's keys; infinities and NaNs lose their own group only
+        int least[G];
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          const float x = fabsf(fa[g]), y = fabsf(fb[g]);
-          if (x < INFINITY) size[0] = fmaxf(size[0], x);
-          if (y < INFINITY) size[1] = fmaxf(size[1], y);
+        for (int i = 0; i < G / 2; ++i) {
+          size[0][i] = finite_sizes(va.w[i]);
+          size[1][i] = finite_sizes(vb.w[i]);
+          least[2 * i] = least[2 * i + 1] = kMostScale;
         }
-        int least = 127;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            float most = kNoTop, big = 0.f;
+            float most = kNoTop;
+            uint32_t big[G / 2] = {};
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
               if (EDGE && !sees(n, x + 2 * y)) continue;
               most = fmaxf(most, s[n][x + 2 * y] * row_scale[n][x]);
-              big = fmaxf(big, size[y]);
+#pragma unroll
+              for (int i = 0; i < G / 2; ++i) big[i] = __vmaxu2(big[i], size[y][i]);
             }
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) {
               most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-              big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+#pragma unroll
+              for (int i = 0; i < G / 2; ++i) big[i] = __vmaxu2(big[i], __shfl_xor_sync(0xffffffffu, big[i], o));
             }
-            const int sigma_was = sigma_of(over[n][x]), sigma = min(max(sigma_was, (int)(__float_as_uint(big) >> 23) - 126), 127);
-            const float was = from[n][x] - (float)(sigma_was - 7), top = most > was + 8.f ? ceilf(most) : was;
-            least = min(least, sigma);
-            from[n][x] = top + (float)(sigma - 7);
-            over[n][x] = power_of_two(15 - sigma);
-            const float f = exp2_approx(fmaxf(was - top, -300.f) + (float)(sigma_was - sigma));
+            const float was = from[n][x] + kShift, top = most > was + kMostGrowth ? ceilf(most) : was;
+            from[n][x] = top - kShift;
+            const float f = exp2_approx(fmaxf(was - top, -300.f));
             sum[n][x] *= f;
 #pragma unroll
-            for (int g = 0; g < G; ++g)
+            for (int g = 0; g < G; ++g) {
+              float& inv_of = inv_scale[warp][n][g][2 * p + x];
+              const int sigma_was = 127 - (int)(__float_as_uint(inv_of) >> 23);
+              // The power of two above the largest scale; where that has grown one more, so that it seldom does again.
+              const int least_of = (int)(big[g / 2] >> (g & 1 ? 23 : 7) & 0xff) - 126;
+              const int sigma = least_of > sigma_was ? min(least_of + 1, kMostScale) : sigma_was;
+              least[g] = min(least[g], sigma);
+              const float fg = f * power_of_two(max(sigma_was - sigma, -126));
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
-                acc[n][g][0][2 * r + x] *= f;
-                acc[n][g][1][2 * r + x] *= f;
-                eights[n][g][2 * r + x] *= f;
+                acc[n][g][0][2 * r + x] *= fg;
+                acc[n][g][1][2 * r + x] *= fg;
+                eights[n][g][2 * r + x] *= fg;
               }
+              __syncwarp();  // read by the eight lanes of the column
+              if (j == 0) inv_of = power_of_two(-sigma);
+            }
 #pragma unroll
             for (int y = 0; y < 2; ++y)
               w[n][x + 2 * y] = exp2_approx(fmaf(s[n][x + 2 * y], row_scale[n][x], -from[n][x]));
           }
-        limit = power_of_two(least);
+#pragma unroll
+        for (int i = 0; i < G / 2; ++i) {
+          inv[i] = bf16_power(-least[2 * i]) | bf16_power(-least[2 * i + 1]) << 16;
+          ua.w[i] = mul_bf16x2(va.w[i], inv[i]);
+          ub.w[i] = mul_bf16x2(vb.w[i], inv[i]);
+        }
+        __syncwarp();
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -466,11 +505,21 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float z[4];
+          if constexpr (ONE) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            z[i] = w[n][i] * (i < 2 ? fa[g] : fb[g]);
-            if (EDGE && !sees(n, i)) z[i] = 0.f;  // whatever the scale is
+            for (int i = 0; i < 4; ++i) z[i] = w[n][i] * (i < 2 ? ua : ub).get(g);
+          } else {
+            const float2 by = *reinterpret_cast<const float2*>(&inv_scale[warp][n][g][2 * p]);
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const float2 x2 = __fmul2_rn(make_float2(w[n][2 * y], w[n][2 * y + 1]), __fmul2_rn(splat2((y ? vb : va).get(g)), by));
+              z[2 * y] = x2.x;
+              z[2 * y + 1] = x2.y;
+            }
           }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (EDGE && !sees(n, i)) z[i] = 0.f;  // whatever the scale is
           const uint32_t w_lo = transposed(half2_of(z[0], z[1])), w_hi = transposed(half2_of(z[2], z[3]));
           float (&o0)[4] = acc[n][g][0], (&o1)[4] = acc[n][g][1], (&e)[4] = eights[n][g];
           mma_f16(o0, x & kLow, x & kHigh, y & kLow, y & kHigh, w_lo, w_hi, o0[0], o0[1], o0[2], o0[3]);
@@ -480,8 +529,15 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
       }
     };
     const auto products = [&](uint32_t here, int key) {
-      if (key >= all_lo && key + kWarpKeys - 1 <= all_hi) compute(std::false_type{}, here, key);
-      else if (key < key_hi && key + kWarpKeys > key_lo) compute(std::true_type{}, here, key);
+      const bool inside = key >= all_lo && key + kWarpKeys - 1 <= all_hi;
+      if (!inside && (key >= key_hi || key + kWarpKeys <= key_lo)) return;
+      if (one_token) {
+        if (inside) compute(std::false_type{}, std::true_type{}, here, key);
+        else compute(std::true_type{}, std::true_type{}, here, key);
+      } else {
+        if (inside) compute(std::false_type{}, std::false_type{}, here, key);
+        else compute(std::true_type{}, std::false_type{}, here, key);
+      }
     };
     if constexpr (TMA) {
       // Steps with keys that some row sees; warp i % 4 has the copies of step i.
@@ -633,20 +689,21 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
         l += __shfl_xor_sync(0xffffffffu, l, 8);
         l += __shfl_xor_sync(0xffffffffu, l, 16);
         const int row = 8 * n + 2 * p + x;
-        const int sigma = sigma_of(over[n][x]);
-        const float down = power_of_two(sigma - 7), top = from[n][x] - (float)(sigma - 7);
+        const float top = from[n][x] + kShift;
         if (j == 0) {
           stat[warp][row][0] = top == kNoTop ? -INFINITY : top;
-          stat[warp][row][1] = l * down;
+          stat[warp][row][1] = l * 0x1p-8f;
         }
 #pragma unroll
-        for (int g = 0; g < G; ++g)
+        for (int g = 0; g < G; ++g) {
+          const float down = power_of_two(119 - (int)(__float_as_uint(inv_scale[warp][n][g][2 * p + x]) >> 23));  // 2^(sigma - 8)
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             const int channel = 8 * (j % 4 * G + g) + 4 * t + j / 4;
-            joined[row * D + channel] = (acc[n][g][t][x] - eights[n][g][x]) * down * 0x1p24f;
-            joined[row * D + channel + 2] = (acc[n][g][t][2 + x] - eights[n][g][2 + x]) * down * 0x1p20f;
+            joined[row * D + channel] = (acc[n][g][t][x] - eights[n][g][x]) * 0x1p24f * down;
+            joined[row * D + channel + 2] = (acc[n][g][t][2 + x] - eights[n][g][2 + x]) * 0x1p20f * down;
           }
+        }
       }
     __syncthreads();
     const bool whole = b0 == 0 && b1 == it.blocks;

@@ -172,7 +172,9 @@ def paged_attention_int4(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_
     """paged_attention over a cache held in 4 bits, with the exact values that it stands for.
 
     Arguments, masks, windows, rows without keys, indices out of range and derivatives as in
-    paged_attention. A scale that is NaN makes the rows that see its slot NaN, and no others.
+    paged_attention. A scale that is NaN makes the rows that see its slot NaN, and no others. Besides
+    the output's rounding there is one of each probability (or probability times scale) to 16 bits; each
+    group of channels keeps its own, however large the scales of the others.
     """
     tensors = (q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, cu_seqlens)
     no_grad("paged_attention_int4", q, k_scale, v_scale)
