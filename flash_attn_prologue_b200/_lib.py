@@ -99,6 +99,8 @@ SIGNATURES = {
     "flash_prologue_paged_attention_int4": ([ctypes.c_char_p, ctypes.c_char_p, _vp], ctypes.c_int),
     "flash_prologue_paged_attention_int4_workspace_size": ([_i64, ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
     "flash_prologue_selftest_attention_int4_waits": ([ctypes.c_char_p, ctypes.c_char_p, _i64, _vp], ctypes.c_int),
+    "flash_prologue_selftest_attention_plan": ([ctypes.c_char_p, ctypes.c_int, _i64, ctypes.POINTER(ctypes.c_size_t),
+                                                ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
     "flash_prologue_unpack_int4": ([_vp, _vp, _vp, _i64, _i64, _i64, _vp], ctypes.c_int),
     "flash_prologue_plan_paged_step": ([ctypes.c_char_p, _vp], ctypes.c_int),
 }

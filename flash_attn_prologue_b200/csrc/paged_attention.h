@@ -79,6 +79,8 @@ struct PrefillPlan {
 };
 PrefillPlan plan_paged_prefill(int64_t tokens, int64_t batch, bool ragged, int64_t kv_heads, int64_t group, int D,
                                int64_t max_keys, int64_t window, int sms, bool int4);
+// Workspace bytes that the plan's shares take: never more than paged_prefill_workspace, which a test and each call check.
+size_t paged_prefill_needs(const PrefillPlan& plan, int64_t kv_heads, int D);
 // False where the cache's layout has no tensor map (the other kernel reads it). wait_cycles: 0, or
 // (self-test, BF16) the limit of the kernel's waits, but for those for copies and products under way.
 // scales: null, or the cache is one of 4 bits (a.k, a.v: codes, strides in bytes).

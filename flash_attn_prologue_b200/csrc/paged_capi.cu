@@ -111,6 +111,8 @@ int attention(const flash_prologue_attention_args* a, const flash_prologue_scale
   if (use_prefill(a, g.scale_log2)) {
     const PrefillPlan plan = plan_paged_prefill(a->tokens, c.batch, c.cu_seqlens != nullptr, a->Hk, g.group, (int)a->D,
                                                 g.max_keys, g.window, sms, scales != nullptr);
+    if (paged_prefill_needs(plan, a->Hk, (int)a->D) > paged_prefill_workspace((int)a->D, sms))
+      return FLASH_PROLOGUE_ERR_WORKSPACE;
     cudaError_t err = cudaSuccess;
     if (launch_paged_prefill(g, plan, scales, (int)a->dtype, (int)a->D, c.page_size,
                              wait_cycles, static_cast<cudaStream_t>(stream), &err))
@@ -157,6 +159,23 @@ int flash_prologue_paged_attention_int4_workspace_size(int64_t D, size_t* bytes)
 int flash_prologue_paged_attention_int4(const flash_prologue_attention_args* a, const flash_prologue_scales* scales,
                                         void* stream) {
   return scales ? attention(a, scales, 0, stream) : FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
+}
+
+int flash_prologue_selftest_attention_plan(const flash_prologue_attention_args* a, int int4, int64_t sms, size_t* needed,
+                                           size_t* available) {
+  if (!a || !needed || !available || sms < 1 || sms > 4096) return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
+  *needed = *available = 0;
+  if (a->tokens < 1 || a->Hk < 1 || a->Hq < a->Hk || a->Hq % a->Hk || a->cache.batch < 1 || a->window < 0 ||
+      (a->D != 64 && a->D != 128))
+    return FLASH_PROLOGUE_ERR_INVALID_ARGUMENT;
+  const int64_t max_keys = a->cache.max_pages * a->cache.page_size;
+  *available = paged_prefill_workspace((int)a->D, (int)sms);
+  if (use_prefill(a, (float)scale_log2_of(a)))
+    *needed = paged_prefill_needs(
+        plan_paged_prefill(a->tokens, a->cache.batch, a->cache.cu_seqlens != nullptr, a->Hk, a->Hq / a->Hk, (int)a->D,
+                           max_keys, a->window < max_keys ? a->window : 0, (int)sms, int4 != 0),
+        a->Hk, (int)a->D);
+  return FLASH_PROLOGUE_OK;
 }
 
 static int attention_waits(const flash_prologue_attention_args* a, const flash_prologue_scales* scales, int64_t wait_cycles,

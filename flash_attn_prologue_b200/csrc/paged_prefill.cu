@@ -126,13 +126,13 @@ struct Tile {  // what the join needs to know of a tile
 
 struct PrefillArgs {
   AttentionArgs a;
-  int tile_tokens;       // whole tokens of a tile: 128 / group
+  int tile_tokens;       // whole tokens of a tile: its rows (128, of paired tiles 256) / group
   int splits;            // shares that the blocks of the last items may be cut into
   int whole_items;       // items (tile, key head) before those
   int box_rows;          // keys of a TMA box: page_size, at most 64
   int tiles;             // tiles the grid has room for, all requests
-  float* part_out;       // [cut items * splits][128][D]
-  float* part_stat;      // [...][128][2]
+  float* part_out;       // [cut items * splits][rows of a tile][D]
+  float* part_stat;      // [...][rows of a tile][2]
   Tile* joins;           // [cut items]
   long long wait_cycles; // self-test: limit of a wait
   // A cache of 4 bits (a.k, a.v: codes, strides in bytes): its scales, strides in elements.
@@ -1274,8 +1274,15 @@ PrefillPlan plan_paged_prefill(int64_t tokens, int64_t batch, bool ragged, int64
   return p;
 }
 
+// The same bytes for tiles of 256 rows, of which the plan makes shares for half the slots.
 size_t paged_prefill_workspace(int D, int sms) {
   return (size_t)(kMostShares * 2 * sms) * (kTile * (size_t)(D + 2) * sizeof(float) + sizeof(Tile));
+}
+
+size_t paged_prefill_needs(const PrefillPlan& plan, int64_t kv_heads, int D) {
+  if (plan.splits == 1) return 0;
+  const int64_t cut = plan.tiles * kv_heads - plan.whole_items;
+  return (size_t)cut * ((size_t)plan.splits * plan.tile_rows * (size_t)(D + 2) * sizeof(float) + sizeof(Tile));
 }
 
 bool launch_paged_prefill(const AttentionArgs& a, const PrefillPlan& plan, const flash_prologue_scales* scales, int dtype,

@@ -639,6 +639,10 @@ FLASH_PROLOGUE_API int flash_prologue_paged_attention_int4(const flash_prologue_
 FLASH_PROLOGUE_API int flash_prologue_selftest_attention_int4_waits(const flash_prologue_attention_args* args,
                                                                     const flash_prologue_scales* scales,
                                                                     int64_t wait_cycles, void* stream);
+/* Without a GPU: the workspace bytes that the shares of chunks' tiles take in a call with these sizes (over a 4-bit cache where
+ * int4 is not 0; pointers are not followed) on a device of `sms` SMs, and what a call has there for them. */
+FLASH_PROLOGUE_API int flash_prologue_selftest_attention_plan(const flash_prologue_attention_args* args, int int4,
+                                                              int64_t sms, size_t* needed, size_t* available);
 /* Bytes of workspace that cover every call of it with head dimension D on the current device. */
 FLASH_PROLOGUE_API int flash_prologue_paged_attention_int4_workspace_size(int64_t D, size_t* bytes);
 /* What `rows` rows of codes and scales stand for, as BF16 or FP16 rows [rows, D]; all contiguous, 16-byte aligned. */
