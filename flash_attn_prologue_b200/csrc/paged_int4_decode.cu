@@ -794,7 +794,8 @@ cudaError_t launch(Int4Args args, const Maps& maps, cudaStream_t stream) {
 }
 
 // The maps of a cache that the copies of HEADS heads can take: pages of a step's keys, a multiple of the heads, scales
-// contiguous along the heads or along the slots, and what tensor maps want of strides.
+// contiguous along the heads or along the slots, and what tensor maps want of strides. With scales [slot][head] that
+// leaves multiples of four heads, and of two at D = 128; with [head][slot] any number but 3, 7, 11, ...
 template <int HEADS>
 bool make_maps(const Int4Args& args, int D, Maps* maps) {
   constexpr uint32_t kStepKeys = kWarpKeys * kDecodeWarps / HEADS;
@@ -805,6 +806,13 @@ bool make_maps(const Int4Args& args, int D, Maps* maps) {
   const bool by_slot = args.ks_slot == G && args.vs_slot == G, by_head = !(HEADS == 1 && by_slot) && args.ks_head == G && args.vs_head == G;
   if (!by_head && !by_slot) return false;
   maps->scales_by_slot = !by_head;
+  // Copies are of whole 16 bytes, and so are the steps from one to the next.
+  const auto whole16 = [](int64_t elements) { return (2 * elements & 15) == 0; };
+  const auto along = [&](int64_t slot, int64_t head) { return by_head ? slot : heads > 1 ? head : 64; };  // (one head: no step)
+  if (!whole16((by_head ? HEADS : kStepKeys) * G) || !whole16(along(args.ks_slot, args.ks_head)) ||
+      !whole16(along(args.vs_slot, args.vs_head)) || (pages > 1 && (!whole16(args.ks_page) || !whole16(args.vs_page))) ||
+      ((reinterpret_cast<uintptr_t>(args.k_scale) | reinterpret_cast<uintptr_t>(args.v_scale)) & 15))
+    return false;
   const auto positive = [](int64_t bytes) { return bytes > 0; };
   const auto codes = [&](CUtensorMap* map, const void* base, int64_t slot, int64_t head, int64_t page) {
     const uint64_t dims[4] = {(uint64_t)D / 2, slots, heads, pages};
@@ -816,10 +824,9 @@ bool make_maps(const Int4Args& args, int D, Maps* maps) {
   };
   const auto scales = [&](CUtensorMap* map, const void* base, int64_t slot, int64_t head, int64_t page) {
     const uint64_t dims[3] = {(by_head ? heads : slots) * G, by_head ? slots : heads, pages};
-    const int64_t along = 2 * (by_head ? slot : head);
-    const uint64_t strides[2] = {(uint64_t)along, pages > 1 ? (uint64_t)(2 * page) : 128};
+    const uint64_t strides[2] = {(uint64_t)(2 * along(slot, head)), pages > 1 ? (uint64_t)(2 * page) : 128};
     const uint32_t box[3] = {(by_head ? HEADS : kStepKeys) * G, by_head ? kStepKeys : HEADS, 1};
-    return positive(along) && (pages == 1 || positive(page)) &&
+    return positive(along(slot, head)) && (pages == 1 || positive(page)) &&
            encode_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
   };
   return codes(&maps->k, a.k, a.k_slot, a.k_head, a.k_page) && codes(&maps->v, a.v, a.v_slot, a.v_head, a.v_page) &&
