@@ -780,10 +780,11 @@ cudaError_t launch(Int4Args args, const Maps& maps, cudaStream_t stream) {
   if (err != cudaSuccess || a.whole) return err;
   const unsigned rows = a.pages.cu_seqlens || a.group > kRows ? kRows : a.group;  // rows a tile can have
   const int64_t items = tiles * ((a.kv_heads + HEADS - 1) / HEADS);  // CTAs that can have begun one
-  // Many parts an item: wide CTAs, of which an SM holds one (2 requests of 131,071 keys, 222 parts an item:
-  // 33 us in all instead of 40 with 8 warps of 4 parts in flight). Few: a warp a row (64 requests of up to 8,192
-  // keys, up to 5 parts: 98 us; 101 with a small CTA a row, 123 with wide ones). Between them a small CTA a row (1
-  // request of 1,000 keys, 16 parts: 11.6 us; 13.0 with a warp a row).
+  // By how many CTAs there are to an item, which is how many parts it may have (lengths are not known here, and with few items
+  // the grid goes by the page table's width). Wide CTAs, of which an SM holds one; a small CTA a row; a warp a row, in us
+  // with each form, 32/8 heads x 128, tables of 131,072 keys: 1 request of 1,000 keys 12.6, 12.6, 12.9; of 16,000 20.8, 25.6, 29.8;
+  // of 131,071 54, 64, 72; 8 of 1,000 19.1, 17.1, 17.3; 8 of 8,000 34.4, 33.9, 33.6; 12 of 1,000 21.3, 18.4, 18.1; 16 of 8,000
+  // 58.5, 53.9, 54.5; 32 of 4,000 67.8, 57.4, 56.8; 64 of 1,000 58.4, 37.6, 35.6.
   const dim3 joins((unsigned)(items < grid ? items : grid), rows, HEADS);
   if (items * 16 < grid)
     return launch_following(paged_join_kernel<T, D, kRows, false, HEADS, 16, 8, true>, joins, dim3(512), stream, a, grid);
