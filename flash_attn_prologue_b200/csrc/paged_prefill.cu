@@ -172,6 +172,7 @@ __device__ __forceinline__ int next_cta(const void* answer) {
       : "=r"(got), "=r"(x) : "r"(smem_u32(answer)) : "memory");
   return got ? (int)x : -1;
 }
+constexpr long long kMostCycles = 8000000000ll;  // of a wait: about 4 s
 // mbar_wait without the suspend hint, whose try takes twice as long where the
 // phase is complete (102 cycles instead of 51) and wakes later where it is not
 // (a round trip of two warps: 434 cycles instead of 289); bounded by the clock.
@@ -183,21 +184,25 @@ __device__ __forceinline__ bool phase_done(uint32_t bar, uint32_t parity) {
       : "=r"(done) : "r"(bar), "r"(parity) : "memory");
   return done != 0;
 }
-__device__ __forceinline__ bool phase_wait(uint64_t* bar, uint32_t parity) {
-  constexpr long long kMostCycles = 8000000000ll;  // about 4 s
+__device__ __forceinline__ bool phase_wait(uint64_t* bar, uint32_t parity, long long most_cycles = kMostCycles) {
   const uint32_t a = smem_u32(bar);
   if (phase_done(a, parity)) return true;
   const long long start = clock64();
   do {
     if (phase_done(a, parity)) return true;
-  } while (clock64() - start < kMostCycles);
+  } while (clock64() - start < most_cycles);
   atomicOr(&g_device_error, kDeviceErrorTimeout);
   return false;
 }
-// A wait whose end nobody is in a hurry for, in suspended tries (mbar_wait's limit) that leave the issue slots to others.
+// The limit of a wait for a whole tile goes by the keys that one can have: four times the 2,000 cycles that a block takes.
+__device__ __forceinline__ long long tile_cycles(int max_keys) { return kMostCycles + (long long)(max_keys / kKeys) * 8192; }
+// A wait for a tile whose end nobody is in a hurry for, in suspended tries that leave the issue slots to others: twice as many
+// as a tile of 2^30 keys needs (21 s; half of them ran out there). With a limit that goes by the keys 4,096 tokens over 16,384
+// keys took 908 us instead of 895.
+constexpr uint32_t kIdleTries = 2 * kMaxWaitTries;
 __device__ __forceinline__ bool idle_wait(uint64_t* bar, uint32_t parity) {
   const uint32_t a = smem_u32(bar);
-  for (uint32_t i = 0; i < kMaxWaitTries; ++i) {
+  for (uint32_t i = 0; i < kIdleTries; ++i) {
     uint32_t done;
     asm volatile(
         "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2, %3;\n"
@@ -375,6 +380,11 @@ __global__ void __launch_bounds__(kThreadsOf<D, kInt4>, 2 / kPair<D, kInt4>)
   // Where K and V are values made here, warps that only hand out tiles wait for a whole tile's time.
   const auto wait_idle = [&](uint64_t* b, uint32_t parity) {
     if constexpr (kInt4 && !kSelfTest) return idle_wait(b, parity);
+    else return wait_for(b, parity);
+  };
+  // A CTA's last waits (the next CTA waits for its place, so not idle).
+  const auto wait_last = [&](uint64_t* b, uint32_t parity) {
+    if constexpr (kInt4 && !kSelfTest) return phase_wait(b, parity, tile_cycles(a.max_keys));
     else return wait_for(b, parity);
   };
   // For copies and products under way, which end by themselves: never cut short.
@@ -869,7 +879,7 @@ __global__ void __launch_bounds__(kThreadsOf<D, kInt4>, 2 / kPair<D, kInt4>)
       }
       if (lane == 0) bar.posted = t;
       if (ok) {
-        ok = __all_sync(0xffffffffu, wait_for(&bar.work_empty[t & 1], ((t >> 1) & 1) ^ 1));
+        ok = __all_sync(0xffffffffu, wait_last(&bar.work_empty[t & 1], ((t >> 1) & 1) ^ 1));
         if (ok && lane == 0) {
           bar.work[t & 1].rows = -1;
           bar.work[t & 1].blocks = 0;
@@ -879,9 +889,9 @@ __global__ void __launch_bounds__(kThreadsOf<D, kInt4>, 2 / kPair<D, kInt4>)
         // No product's arrival on an empty barrier lands after the CTA has gone.
         for (uint32_t e = g; e < g + L::kStages && ok; ++e) {
           const uint32_t s = e % L::kStages, parity = ((e / L::kStages) & 1) ^ 1;
-          ok = __all_sync(0xffffffffu, wait_for(&bar.k_empty[s], parity) && wait_for(&bar.v_empty[s], parity));
+          ok = __all_sync(0xffffffffu, wait_last(&bar.k_empty[s], parity) && wait_last(&bar.v_empty[s], parity));
         }
-        if (ok) ok = __all_sync(0xffffffffu, wait_for(&bar.q_empty, (queries & 1) ^ 1));
+        if (ok) ok = __all_sync(0xffffffffu, wait_last(&bar.q_empty, (queries & 1) ^ 1));
       }
       if (!ok) {
         // A wait ran out: what is still on its way to shared memory has to arrive. A tile that does is not computed.

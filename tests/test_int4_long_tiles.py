@@ -1,0 +1,26 @@
+"""Tiles of rows that take longer than a wait for one block may."""
+import pytest
+import torch
+
+import flash_attn_prologue_b200 as fap
+from flash_attn_prologue_b200 import _lib
+
+
+@pytest.mark.gpu
+def test_a_tile_of_seconds_sets_no_error():
+    """As many tiles as the GPU holds at once, of 335 million keys each (a table that names the same pages again)."""
+    g = torch.Generator(device="cuda").manual_seed(0)
+    tokens = 2 * torch.cuda.get_device_properties(0).multi_processor_count  # of 128 rows, whole tiles
+    cache = fap.int4_cache(4, 1024, 1, 64)
+    for codes, scale in zip(cache[:2], cache[2:]):
+        codes.random_(0, 256, generator=g)
+        scale.fill_(0.25)
+    width = 327680
+    table = torch.randint(0, 4, (1, width), generator=g, device="cuda", dtype=torch.int32)
+    lens = torch.tensor([1024 * width], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, tokens], dtype=torch.int32, device="cuda")
+    q = (0.1 * torch.randn(tokens, 128, 64, generator=g, device="cuda")).to(torch.bfloat16)
+    _lib.device_error()
+    out = fap.paged_attention_int4(q, *cache, table, lens, cu)
+    assert _lib.device_error() == 0
+    assert out.isfinite().all()
