@@ -382,9 +382,14 @@ __global__ void __launch_bounds__(kThreadsOf<D, kInt4>, 2 / kPair<D, kInt4>)
     if constexpr (kInt4 && !kSelfTest) return idle_wait(b, parity);
     else return wait_for(b, parity);
   };
-  // A CTA's last waits (the next CTA waits for its place, so not idle).
+  // For a whole tile's blocks, where somebody waits behind it.
+  const auto wait_tile = [&](uint64_t* b, uint32_t parity) {
+    if constexpr (kSelfTest) return wait_for(b, parity);
+    else return phase_wait(b, parity, tile_cycles(a.max_keys));
+  };
+  // A CTA's last waits (the next CTA waits for its place). Where K and V are copied here, their waits came before.
   const auto wait_last = [&](uint64_t* b, uint32_t parity) {
-    if constexpr (kInt4 && !kSelfTest) return phase_wait(b, parity, tile_cycles(a.max_keys));
+    if constexpr (kInt4) return wait_tile(b, parity);
     else return wait_for(b, parity);
   };
   // For copies and products under way, which end by themselves: never cut short.
@@ -913,15 +918,15 @@ __global__ void __launch_bounds__(kThreadsOf<D, kInt4>, 2 / kPair<D, kInt4>)
       uint32_t asked = 0;
       bool ok = true;
       for (uint32_t t = 0; ok; ++t) {
-        if (!(ok = next_work(t))) break;
+        if (!(ok = __all_sync(0xffffffffu, wait_tile(&bar.work_full[t & 1], (t >> 1) & 1)))) break;
         Work& w = bar.work[t & 1];
         if (w.rows < 0) break;
         const int n = w.blocks, full0 = w.full0, full1 = w.full1;
         for (int j = 0; j < n; ++j, ++g) {
           if (j >= full0 && j < full1) continue;
           const uint32_t s = g % L::kStages;
-          // Asked by the warp that has seen the block arrive.
-          if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.clean_ask, asked++ & 1) &&
+          // Asked by the warp that has seen the block arrive, after all blocks between two that are cleaned.
+          if (!(ok = __all_sync(0xffffffffu, wait_tile(&bar.clean_ask, asked++ & 1) &&
                                                  wait_for(&bar.v_full[s], (g / L::kStages) & 1))))
             break;
           const int kb = (w.first + j) * kKeys, lo = w.lo - kb, hi = w.hi - kb;

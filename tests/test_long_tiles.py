@@ -24,3 +24,19 @@ def test_a_tile_of_seconds_sets_no_error():
     out = fap.paged_attention_int4(q, *cache, table, lens, cu)
     assert _lib.device_error() == 0
     assert out.isfinite().all()
+
+
+@pytest.mark.gpu
+def test_a_tile_of_seconds_over_a_16_bit_cache():
+    g = torch.Generator(device="cuda").manual_seed(0)
+    tokens = 2 * torch.cuda.get_device_properties(0).multi_processor_count
+    k, v = (torch.randn(4, 1024, 1, 64, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    width = 360448
+    table = torch.randint(0, 4, (1, width), generator=g, device="cuda", dtype=torch.int32)
+    lens = torch.tensor([1024 * width], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, tokens], dtype=torch.int32, device="cuda")
+    q = (0.1 * torch.randn(tokens, 128, 64, generator=g, device="cuda")).to(torch.bfloat16)
+    _lib.device_error()
+    out = fap.paged_attention(q, k, v, table, lens, cu)
+    assert _lib.device_error() == 0
+    assert out.isfinite().all()
