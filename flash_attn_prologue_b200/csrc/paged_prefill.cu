@@ -968,7 +968,8 @@ __global__ void __launch_bounds__(kThreadsOf<D, kInt4>, 2 / kPair<D, kInt4>)
     bool ok = true;
     for (; ok; ++rows_done) {
       const uint32_t t = rows_done;
-      if (!(ok = next_work(t))) break;
+      // A paired tile's second half may have no rows: its warps wait for another tile to end, for the next one or its scores.
+      if (!(ok = PAIR == 2 ? __all_sync(0xffffffffu, wait_tile(&bar.work_full[t & 1], (t >> 1) & 1)) : next_work(t))) break;
       const Work& w = bar.work[t & 1];
       if (w.rows < 0) break;
       if (PAIR == 2 && w.rows <= half * kTile) {  // none of these rows
@@ -985,7 +986,9 @@ __global__ void __launch_bounds__(kThreadsOf<D, kInt4>, 2 / kPair<D, kInt4>)
       }
       for (int j = 0; j < blocks; ++j, ++g) {
         const uint32_t b = g % L::kScores;
-        if (!(ok = __all_sync(0xffffffffu, wait_for(&bar.s_full[half][b], (g / L::kScores) & 1)))) break;
+        if (!(ok = __all_sync(0xffffffffu, PAIR == 2 && j == 0 ? wait_tile(&bar.s_full[half][b], (g / L::kScores) & 1)
+                                                               : wait_for(&bar.s_full[half][b], (g / L::kScores) & 1))))
+          break;
         tc_fence_after();
         uint32_t s[2][32];
         tmem_ld32(mine + L::kSCol + b * kKeys, s[0]);
