@@ -22,7 +22,7 @@
 // p s are rounded to FP16 once, p 2^8 times as large and s less the power of two sigma above the
 // largest scales that the row has seen in this group of channels, so that they are below 2^15: an error of the size
 // of a 16-bit output's rounding, and where a weight is below 2^-14, of 2^-33 of that power (with one
-// sigma for all groups it was that of the largest group for all: 2 us of 100 less). A sigma that moves goes one
+// sigma for all groups it was that of the largest group for all; 64 requests 98 us instead of 99). A sigma that moves goes one
 // further than it has to (each time as far as it has to: 3 us more). Scores, statistics and sums are FP32. The
 // maximum that scales a row of O moves only when the row's has grown by more than 2^7.
 //
@@ -367,12 +367,15 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
     const int key_lo = it.lo - warp_key, key_hi = it.hi - warp_key;
     const int all_lo = a.window ? base + (row0 + rows - 1) / a.group - a.window + 1 - warp_key : kNone;
     const int all_hi = base + row0 / a.group - warp_key;  // every row sees keys all_lo .. all_hi
-    const bool one_token = token_of(0) == token_of(rows - 1);
     const int32_t* table = a.pages.page_table + (int64_t)it.r * a.pages.table_stride;
-    // A step's scores, probabilities and product; EDGE: some row does not see some key. ONE: all rows see the same keys, so
-    // the columns' sigmas are the same.
+    // Where a group's sigmas are the same in all columns the products take scales that have them already. With one tile of 8
+    // rows that goes by the rows (one token: all see the same keys), in code of its own; with two by the sigmas. (64 requests, up to
+    // 20 rows: 175 us; by the rows 185. 64 single tokens: 99 us, by the sigmas 101.)
+    const bool one_token = token_of(0) == token_of(rows - 1);
+    [[maybe_unused]] bool same = true;
+    // A step's scores, probabilities and product; EDGE: some row does not see some key.
     const auto compute = [&](auto edge, auto one, uint32_t here, int key) {
-      constexpr bool EDGE = decltype(edge)::value, ONE = decltype(one)::value;
+      constexpr bool EDGE = decltype(edge)::value;
       // Sums of keys key_of(j) and 8 more (x / 2), columns 2 p and 2 p + 1 (x % 2).
       float s[NT][4] = {};
       {
@@ -406,6 +409,13 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
         return k <= hi && (!a.window || k > hi - a.window);
       };
       float w[NT][4];  // probabilities times 2^8
+      const auto weights = [&] {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            w[n][x] = EDGE && !sees(n, x) ? 0.f : exp2_approx(fmaf(s[n][x], row_scale[n][x & 1], -from[n][x & 1]));
+      };
       Scales<G> ua, ub;  // the scales of V times 2^-sigma: below 1, or a sigma moves
       __nv_bfloat162 largest = bf16x2_of(0);
 #pragma unroll
@@ -414,124 +424,138 @@ __global__ void __launch_bounds__(kDecodeThreads, NT == 1 ? D == 64 ? 4 : 3 : 2)
         ub.w[i] = mul_bf16x2(vb.w[i], inv[i]);
         largest = __hmax2(largest, __hmax2(__habs2(bf16x2_of(ua.w[i])), __habs2(bf16x2_of(ub.w[i]))));
       }
-      bool move = EDGE || !__hblt2(largest, __float2bfloat162_rn(1.f));
+      weights();
+      const bool grown = !__hblt2(largest, __float2bfloat162_rn(1.f));
+      bool move = grown;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) w[n][x] = exp2_approx(fmaf(s[n][x], row_scale[n][x & 1], -from[n][x & 1]));
-        move |= fmaxf(fmaxf(w[n][0], w[n][2]), fmaxf(w[n][1], w[n][3])) > kMostWeight;
-      }
+      for (int n = 0; n < NT; ++n) move |= fmaxf(fmaxf(w[n][0], w[n][2]), fmaxf(w[n][1], w[n][3])) > kMostWeight;
       if (__any_sync(0xffffffffu, move)) {
         // A row's maximum or a group's largest scale may have moved: its O and sums follow. Each row goes by
         // the keys that it sees, so what others see does not change its bits.
-        uint32_t size[2][G / 2];  // scales of this lane's keys; infinities and NaNs lose their own group only
-        int least[G];
-#pragma unroll
-        for (int i = 0; i < G / 2; ++i) {
-          size[0][i] = finite_sizes(va.w[i]);
-          size[1][i] = finite_sizes(vb.w[i]);
-          least[2 * i] = least[2 * i + 1] = kMostScale;
-        }
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             float most = kNoTop;
-            uint32_t big[G / 2] = {};
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              if (EDGE && !sees(n, x + 2 * y)) continue;
-              most = fmaxf(most, s[n][x + 2 * y] * row_scale[n][x]);
+            for (int y = 0; y < 2; ++y)
+              if (!EDGE || sees(n, x + 2 * y)) most = fmaxf(most, s[n][x + 2 * y] * row_scale[n][x]);
 #pragma unroll
-              for (int i = 0; i < G / 2; ++i) big[i] = __vmaxu2(big[i], size[y][i]);
-            }
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) {
-              most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-#pragma unroll
-              for (int i = 0; i < G / 2; ++i) big[i] = __vmaxu2(big[i], __shfl_xor_sync(0xffffffffu, big[i], o));
-            }
+            for (int o = 4; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
             const float was = from[n][x] + kShift, top = most > was + kMostGrowth ? ceilf(most) : was;
             from[n][x] = top - kShift;
             const float f = exp2_approx(fmaxf(was - top, -300.f));
             sum[n][x] *= f;
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-              float& inv_of = inv_scale[warp][n][g][2 * p + x];
-              const int sigma_was = 127 - (int)(__float_as_uint(inv_of) >> 23);
-              // The power of two above the largest scale; where that has grown one more, so that it seldom does again.
-              const int least_of = (int)(big[g / 2] >> (g & 1 ? 23 : 7) & 0xff) - 126;
-              const int sigma = least_of > sigma_was ? min(least_of + 1, kMostScale) : sigma_was;
-              least[g] = min(least[g], sigma);
-              const float fg = f * power_of_two(max(sigma_was - sigma, -126));
+            for (int g = 0; g < G; ++g)
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
-                acc[n][g][0][2 * r + x] *= fg;
-                acc[n][g][1][2 * r + x] *= fg;
-                eights[n][g][2 * r + x] *= fg;
+                acc[n][g][0][2 * r + x] *= f;
+                acc[n][g][1][2 * r + x] *= f;
+                eights[n][g][2 * r + x] *= f;
               }
-              __syncwarp();  // read by the eight lanes of the column
-              if (j == 0) inv_of = power_of_two(-sigma);
-            }
+          }
+        weights();
+        if (__any_sync(0xffffffffu, grown)) {
+          int least[G], largest_of[G];
 #pragma unroll
-            for (int y = 0; y < 2; ++y)
-              w[n][x + 2 * y] = exp2_approx(fmaf(s[n][x + 2 * y], row_scale[n][x], -from[n][x]));
+          for (int g = 0; g < G; ++g) {
+            least[g] = kMostScale;
+            largest_of[g] = kLeastScale;
           }
 #pragma unroll
-        for (int i = 0; i < G / 2; ++i) {
-          inv[i] = bf16_power(-least[2 * i]) | bf16_power(-least[2 * i + 1]) << 16;
-          ua.w[i] = mul_bf16x2(va.w[i], inv[i]);
-          ub.w[i] = mul_bf16x2(vb.w[i], inv[i]);
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              uint32_t big[G / 2];  // infinities and NaNs lose their own group only
+#pragma unroll
+              for (int i = 0; i < G / 2; ++i) {
+                big[i] = __vmaxu2(!EDGE || sees(n, x) ? finite_sizes(va.w[i]) : 0, !EDGE || sees(n, x + 2) ? finite_sizes(vb.w[i]) : 0);
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) big[i] = __vmaxu2(big[i], __shfl_xor_sync(0xffffffffu, big[i], o));
+              }
+#pragma unroll
+              for (int g = 0; g < G; ++g) {
+                float& inv_of = inv_scale[warp][n][g][2 * p + x];
+                const int sigma_was = 127 - (int)(__float_as_uint(inv_of) >> 23);
+                // The power of two above the largest scale; where that has grown one more, so that it seldom does again.
+                const int least_of = (int)(big[g / 2] >> (g & 1 ? 23 : 7) & 0xff) - 126;
+                const int sigma = least_of > sigma_was ? min(least_of + 1, kMostScale) : sigma_was;
+                least[g] = min(least[g], sigma);
+                largest_of[g] = max(largest_of[g], sigma);
+                const float f = power_of_two(max(sigma_was - sigma, -126));
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                  acc[n][g][0][2 * r + x] *= f;
+                  acc[n][g][1][2 * r + x] *= f;
+                  eights[n][g][2 * r + x] *= f;
+                }
+                __syncwarp();  // read by the eight lanes of the column
+                if (j == 0) inv_of = power_of_two(-sigma);
+              }
+            }
+          bool equal = true;
+#pragma unroll
+          for (int i = 0; i < G / 2; ++i) {
+            inv[i] = bf16_power(-least[2 * i]) | bf16_power(-least[2 * i + 1]) << 16;
+            ua.w[i] = mul_bf16x2(va.w[i], inv[i]);
+            ub.w[i] = mul_bf16x2(vb.w[i], inv[i]);
+            const uint32_t first = __shfl_sync(0xffffffffu, inv[i], 0);
+            equal &= (first == inv[i]) & (least[2 * i] == largest_of[2 * i]) & (least[2 * i + 1] == largest_of[2 * i + 1]);
+          }
+          if constexpr (NT > 1) same = __all_sync(0xffffffffu, equal);
+          __syncwarp();
         }
-        __syncwarp();
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          if (EDGE && !sees(n, x)) w[n][x] = 0.f;
-          sum[n][x & 1] += w[n][x];
-        }
+        for (int x = 0; x < 4; ++x) sum[n][x & 1] += w[n][x];
       // Channels of this lane: words j % 4 of the four keys, even or odd ones.
       uint32_t w0[G], w1[G], w8[G], w9[G];
       load_words<G>(w0, here + v_at[0]);
       load_words<G>(w1, here + v_at[1]);
       load_words<G>(w8, here + v_at[0] + kEight);
       load_words<G>(w9, here + v_at[1] + kEight);
+      const auto add_up = [&](auto alike) {
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const uint32_t x = __byte_perm(w0[g], w1[g], half_of), y = __byte_perm(w8[g], w9[g], half_of);
-        const uint32_t x8 = x >> 8, y8 = y >> 8;
+        for (int g = 0; g < G; ++g) {
+          const uint32_t x = __byte_perm(w0[g], w1[g], half_of), y = __byte_perm(w8[g], w9[g], half_of);
+          const uint32_t x8 = x >> 8, y8 = y >> 8;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float z[4];
-          if constexpr (ONE) {
+          for (int n = 0; n < NT; ++n) {
+            float z[4];
+            if constexpr (decltype(alike)::value) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) z[i] = w[n][i] * (i < 2 ? ua : ub).get(g);
-          } else {
-            const float2 by = *reinterpret_cast<const float2*>(&inv_scale[warp][n][g][2 * p]);
+              for (int i = 0; i < 4; ++i) z[i] = w[n][i] * (i < 2 ? ua : ub).get(g);
+            } else {
+              const float2 by = *reinterpret_cast<const float2*>(&inv_scale[warp][n][g][2 * p]);
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              const float2 x2 = __fmul2_rn(make_float2(w[n][2 * y], w[n][2 * y + 1]), __fmul2_rn(splat2((y ? vb : va).get(g)), by));
-              z[2 * y] = x2.x;
-              z[2 * y + 1] = x2.y;
+              for (int i = 0; i < 2; ++i) {
+                const float2 x2 = __fmul2_rn(make_float2(w[n][2 * i], w[n][2 * i + 1]), __fmul2_rn(splat2((i ? vb : va).get(g)), by));
+                z[2 * i] = x2.x;
+                z[2 * i + 1] = x2.y;
+              }
             }
-          }
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (EDGE && !sees(n, i)) z[i] = 0.f;  // whatever the scale is
-          const uint32_t w_lo = transposed(half2_of(z[0], z[1])), w_hi = transposed(half2_of(z[2], z[3]));
-          float (&o0)[4] = acc[n][g][0], (&o1)[4] = acc[n][g][1], (&e)[4] = eights[n][g];
-          mma_f16(o0, x & kLow, x & kHigh, y & kLow, y & kHigh, w_lo, w_hi, o0[0], o0[1], o0[2], o0[3]);
-          mma_f16(o1, x8 & kLow, x8 & kHigh, y8 & kLow, y8 & kHigh, w_lo, w_hi, o1[0], o1[1], o1[2], o1[3]);
-          mma_f16(e, 0x00080008u, 0x00800080u, 0x00080008u, 0x00800080u, w_lo, w_hi, e[0], e[1], e[2], e[3]);
+            for (int i = 0; i < 4; ++i)
+              if (EDGE && !sees(n, i)) z[i] = 0.f;  // whatever the scale is
+            const uint32_t w_lo = transposed(half2_of(z[0], z[1])), w_hi = transposed(half2_of(z[2], z[3]));
+            float (&o0)[4] = acc[n][g][0], (&o1)[4] = acc[n][g][1], (&e)[4] = eights[n][g];
+            mma_f16(o0, x & kLow, x & kHigh, y & kLow, y & kHigh, w_lo, w_hi, o0[0], o0[1], o0[2], o0[3]);
+            mma_f16(o1, x8 & kLow, x8 & kHigh, y8 & kLow, y8 & kHigh, w_lo, w_hi, o1[0], o1[1], o1[2], o1[3]);
+            mma_f16(e, 0x00080008u, 0x00800080u, 0x00080008u, 0x00800080u, w_lo, w_hi, e[0], e[1], e[2], e[3]);
+          }
         }
-      }
+      };
+      if constexpr (NT == 1) add_up(one);
+      else if (same) add_up(std::true_type{});
+      else add_up(std::false_type{});
     };
     const auto products = [&](uint32_t here, int key) {
       const bool inside = key >= all_lo && key + kWarpKeys - 1 <= all_hi;
       if (!inside && (key >= key_hi || key + kWarpKeys <= key_lo)) return;
-      if (one_token) {
+      if (NT == 1 && one_token) {
         if (inside) compute(std::false_type{}, std::true_type{}, here, key);
         else compute(std::true_type{}, std::true_type{}, here, key);
       } else {
