@@ -40,8 +40,8 @@ int size_checks(const flash_prologue_attention_args* a, bool int4) {
 // least one whole token.
 //
 // Over a cache of 4 bits the other kernel takes tiles of 8 and 16 rows, and the rule stays. 12 rows a key head
-// (20 rows, tiled), 8 key heads x 128: 64 requests of 8,192 keys 270 (473) us, 64 of 2,048 keys 103 (130), 16 of
-// 4,096 54 (64); where there is little to read tiles would win a little, 32 of 1,024 41 (38), 4 of 4,096 32 (27).
+// (20 rows, tiled), 8 key heads x 128: 64 requests of 8,192 keys 250 (465) us, 64 of 2,048 keys 88 (128), 16 of
+// 4,096 50 (64), 32 of 1,024 34 (38); where there is little to read tiles would win a little, 4 of 4,096 32 (27).
 bool use_prefill(const flash_prologue_attention_args* a, float scale_log2) {
   const int64_t group = a->Hq / a->Hk;
   return a->tokens * group > 16 * a->cache.batch && group <= 128 && scale_log2 >= FLT_MIN;

@@ -35,11 +35,11 @@
 // hold: 32 keys 123 to 127 us, 4 CTAs 123 (at 128 registers), 2 CTAs 117 (3 took 102 to 103 then). One product's
 // rows for the 8 sum p s of all groups would save 12 registers, but its sums wait for one another: 106 us instead of 102.
 //
-// Measured (32/8 heads x 128 BF16 unless said): 64 requests of up to 8,192 keys 98 us, 339 MB, 3.5
-// TB/s (52 us at the copy rate; the same over a 16-bit cache 199 to 209 us); issue slots 52% and ALU 49%
-// busy with three warps a scheduler: about 390 instructions a step, half of them products, masks of codes
-// and the scales' multiplications. 2 requests of 131,071 keys, 16/2 heads FP16: 33 us (16-bit cache 54). 1
-// request of 1,000 keys: 11.6 us, latency.
+// Measured (32/8 heads x 128 BF16 unless said): 64 requests of up to 8,192 keys 99 us, 339 MB, 3.4
+// TB/s (52 us at the copy rate; the same over a 16-bit cache 201 us); issue slots 51% and ALU 46%
+// busy with three warps a scheduler: about 350 instructions a step, half of them products, masks of codes
+// and the scales' multiplications. 2 requests of 131,071 keys, 16/2 heads FP16: 31.5 us (16-bit cache 48). 1
+// request of 1,000 keys: 12.0 us, latency.
 #include "paged_runs.cuh"
 #include "tensor_map.h"
 #include "umma_util.cuh"
@@ -48,7 +48,7 @@ namespace flash_prologue {
 namespace {
 
 // Steps of a ring, and how many a CTA's common ring is loaded ahead. (6 and 4, 6 and 3, 5 and 3: 99 to 100 us
-// where 4 and 2 take 98.)
+// where 4 and 2 took 98.)
 constexpr int kRing = 4;
 constexpr int kAhead = 2;
 constexpr int kBlockKeys = kWarpKeys * kDecodeWarps;

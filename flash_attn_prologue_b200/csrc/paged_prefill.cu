@@ -870,7 +870,8 @@ __global__ void __launch_bounds__(kThreadsOf<D, kInt4>, 2 / kPair<D, kInt4>)
           }
           if (!ok) break;
         }
-        // Asked for late, while the last blocks are computed, so that an idle CTA is not left without.
+        // Asked for late, while the last blocks are computed, so that an idle CTA is not left without. (Over a cache of 4 bits,
+        // where this warp has no blocks to load, once Q is under way: a CTA may have two tiles where another has none.)
         if (lane == 0) {
           fence_proxy_async_smem();  // the last answer has been read
           mbar_arrive_expect_tx(&bar.next_here, 16);
