@@ -172,7 +172,8 @@ def paged_attention_int4(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_
     """paged_attention over a cache held in 4 bits, with the exact values that it stands for.
 
     Arguments, masks, windows, rows without keys, indices out of range and derivatives as in
-    paged_attention. A scale that is NaN makes the rows that see its slot NaN, and no others. q has the
+    paged_attention. A scale that is NaN makes the rows that see its slot NaN (of V: their
+    channels of its group), and no others. q has the
     type of the rows that were appended: a cache does not know it, and FP16 rows over one of BF16 rows
     want scales of 2^-20 to 7,936 (chunks are multiplied in FP16, where larger ones overflow). Besides
     the output's rounding there is one of each probability (or probability times scale) to 16 bits; each

@@ -11,12 +11,17 @@ BF16 = torch.bfloat16
 def _by_copies(call):
     """Whether the kernel that `call` runs is the one with tensor copies."""
     call()
-    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as p:
-        call()
-        torch.cuda.synchronize()
-    names = [e.name for e in p.events() if "paged_int4_decode_kernel" in e.name]
-    assert len(names) == 1 and names[0].count("<") == 1, names
-    last = names[0][names[0].index("<") + 1:names[0].index(">")].split(",")[-1]
+    names = set()
+    for _ in range(3):  # a profile may come back without its events
+        with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as p:
+            call()
+            torch.cuda.synchronize()
+        names |= {e.name for e in p.events() if "paged_int4_decode_kernel<" in e.name}
+        if names:
+            break
+    assert len(names) == 1, names
+    name = names.pop()
+    last = name[name.index("<") + 1:name.index(">")].split(",")[-1]
     return "true" in last or last.strip().endswith("1")
 
 
